@@ -197,6 +197,117 @@ int qwen_sample_scratch(const uint16_t* logits, uint32_t n_seq, uint32_t row_str
                         float temperature, float top_p, const uint32_t* u24, int32_t* out_ids,
                         void* scratch, void* stream);
 
+/* ---- paged key/value cache ------------------------------------------------
+ * The reference keeps one contiguous cache row per layer
+ * (InferenceManager.swift:63-65) and has no paged form; these operators are
+ * the rotation, cache write and attention chain of InferenceEngine.swift:130-182
+ * over a cache of fixed-size pages, for fp16 or bf16, head_dim 64 or 128 and any
+ * head counts. */
+#define QWEN_DTYPE_F16 0
+#define QWEN_DTYPE_BF16 1
+
+/* A layer's cache: position p of sequence s lives in slot p % page_size of pool
+ * page t = page_table[s * table_stride + p / page_size]; element d of its kv
+ * head h is at t * page_stride + slot * pos_stride + h * head_stride + d of k and
+ * of v (strides in elements, so [page][slot][head][d], [page][head][slot][d] and
+ * pools that hold k beside v are all described).  k, v and bounds are 16-byte
+ * aligned, strides positive multiples of 8.  page_size is a power of two,
+ * 16 .. 256.  bounds (NULL: none kept) is [n_pages][2][n_kv_heads][head_dim],
+ * contiguous: per page the least and the largest stored key, element by element.
+ * A sequence holds at most max_pages * page_size positions. */
+typedef struct qwen_paged_kv {
+  uint16_t* k;
+  uint16_t* v;
+  uint16_t* bounds;
+  const int32_t* page_table; /* [n_seq][table_stride], device */
+  int64_t page_stride, pos_stride, head_stride;
+  uint32_t n_pages, page_size, n_kv_heads, head_dim;
+  uint32_t n_seq, max_pages, table_stride;
+  int32_t dtype; /* QWEN_DTYPE_* of q, k, v, bounds and outputs */
+} qwen_paged_kv;
+
+/* What all operators below share.  seq_len[n_seq] (device) counts a sequence's
+ * positions in the cache.  A length beyond max_pages * page_size is reported by
+ * qwen_ops_status and that sequence's outputs are left as they were; a page
+ * number outside the pool is reported, and its positions are left out (no key is
+ * read or written there).  Rows of q, k, v and outputs are head-contiguous
+ * ([heads][head_dim]) with the given row strides (elements, multiples of 8) and
+ * 16-byte aligned.  workspace: device memory of at least the *_workspace bytes
+ * for the same arguments, 256-byte aligned, with any contents; calls that may
+ * overlap on the GPU need one each.  n_heads is a multiple of n_kv_heads, at
+ * most 64 query heads share a kv head. */
+
+/* apply_rope_q4 and write_kv_cache (rope.metal:12-39, attention.metal:67-84) for
+ * a batch of new tokens over a paged cache, in one launch: rotates q into q_out
+ * (which may be q), writes rotated k, and v, to the cache, and keeps bounds.
+ * seq_len counts the new tokens too.  cu_tokens (device, [n_seq + 1]): sequence
+ * s owns rows cu_tokens[s] .. cu_tokens[s+1]-1, its last positions, in order; rows
+ * from cu_tokens[n_seq] on are not touched.  cu_tokens NULL: row s is sequence
+ * s's newest token (n_tokens = n_seq; seq_len 0: the row is not touched).
+ * Rotation of pair i < rot_dim / 2 by the angle position * inv_freq[i] (the
+ * product formed exactly): elements (i, i + rot_dim/2), or (2i, 2i+1) if
+ * interleaved; fp32 arithmetic, one rounding.  rot_dim: a multiple of 16, at most
+ * head_dim; the rest of a head passes through.  A page's bounds start anew with
+ * its slot 0, and otherwise take the new keys in.  Two sequences of a call must
+ * not append to the same page. */
+int qwen_rope_append_paged(const qwen_paged_kv* kv, const uint16_t* q, int64_t q_stride,
+                           const uint16_t* k, int64_t k_stride, const uint16_t* v,
+                           int64_t v_stride, uint16_t* q_out, int64_t q_out_stride,
+                           uint32_t n_heads, uint32_t n_tokens, const uint32_t* seq_len,
+                           const int32_t* cu_tokens, const float* inv_freq, uint32_t rot_dim,
+                           int interleaved, void* stream);
+
+/* qwen_attention_decode_batched over a paged cache: one query row per sequence
+ * against its seq_len positions, out = softmax(scale * q K^T) V.  lse (NULL or
+ * [n_seq][n_heads] fp32): natural log of the sum of exp(scale * q K^T).  A
+ * sequence without positions gives zeros and -inf. */
+size_t qwen_attention_paged_workspace(const qwen_paged_kv* kv, uint32_t n_heads);
+int qwen_attention_paged(const qwen_paged_kv* kv, const uint16_t* q, int64_t q_stride,
+                         uint16_t* out, int64_t out_stride, float* lse, uint32_t n_heads,
+                         const uint32_t* seq_len, float scale, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/* The same where every sequence begins with the same prefix_len positions, held
+ * once in the pool pages prefix_pages[] (device, ceil(prefix_len / page_size)
+ * numbers); seq_len and page_table describe what follows the prefix (a sequence
+ * may hold none).  The prefix is read once for the whole batch. */
+size_t qwen_attention_prefix_paged_workspace(const qwen_paged_kv* kv, uint32_t n_heads,
+                                             uint32_t prefix_len);
+int qwen_attention_prefix_paged(const qwen_paged_kv* kv, const uint16_t* q, int64_t q_stride,
+                                uint16_t* out, int64_t out_stride, float* lse, uint32_t n_heads,
+                                const uint32_t* seq_len, const int32_t* prefix_pages,
+                                uint32_t prefix_len, float scale, void* workspace,
+                                size_t workspace_bytes, void* stream);
+
+/* The n_select pages per sequence and kv head that a bound on their scores puts
+ * first: score(page) = sum over the kv head's query heads and over d of
+ * max(q_d lo_d, q_d hi_d) with the page's bounds lo, hi (kv->bounds must be set), at
+ * least the sum of q . k for every key of the page; 64-bit sums, and an element
+ * that no query head multiplies (all zero) adds nothing.  The first
+ * n_first and last n_last pages of a sequence are always on its list (n_first +
+ * n_last <= n_select); ties go to the lower page, NaN scores come first.  pages
+ * [n_seq][n_kv_heads][n_select] (int32, device) receives page_table columns in
+ * ascending order, -1 behind the last (all pages of a sequence with no more than
+ * n_select). */
+size_t qwen_select_pages_workspace(const qwen_paged_kv* kv);
+int qwen_select_pages(const qwen_paged_kv* kv, const uint16_t* q, int64_t q_stride,
+                      uint32_t n_heads, const uint32_t* seq_len, uint32_t n_select,
+                      uint32_t n_first, uint32_t n_last, int32_t* pages, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* qwen_attention_paged over the listed pages alone: pages
+ * [n_seq][n_kv_heads][n_select] are page_table columns, -1 for none, in any
+ * order (a column listed twice counts twice); only positions below seq_len
+ * count.  A column outside 0 .. max_pages - 1 other than -1 is reported and left
+ * out. */
+size_t qwen_attention_sparse_paged_workspace(const qwen_paged_kv* kv, uint32_t n_heads,
+                                             uint32_t n_select);
+int qwen_attention_sparse_paged(const qwen_paged_kv* kv, const int32_t* pages, uint32_t n_select,
+                                const uint16_t* q, int64_t q_stride, uint16_t* out,
+                                int64_t out_stride, float* lse, uint32_t n_heads,
+                                const uint32_t* seq_len, float scale, void* workspace,
+                                size_t workspace_bytes, void* stream);
+
 /* 24-bit uniform for (seed, sequence, step), SplitMix64 based; host helper. */
 uint32_t qwen_uniform24(uint64_t seed, uint64_t sequence, uint64_t step);
 

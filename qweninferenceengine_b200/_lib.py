@@ -31,9 +31,9 @@ QWEN_CTX_ERROR = 1
 QWEN_PREFILL_CHUNKED = 0
 QWEN_PREFILL_STEPS = 1
 
-c_void_p, c_int, c_uint32, c_int32, c_uint64, c_size_t, c_float = (
+c_void_p, c_int, c_uint32, c_int32, c_uint64, c_size_t, c_float, c_int64 = (
     ctypes.c_void_p, ctypes.c_int, ctypes.c_uint32, ctypes.c_int32, ctypes.c_uint64,
-    ctypes.c_size_t, ctypes.c_float)
+    ctypes.c_size_t, ctypes.c_float, ctypes.c_int64)
 _i32p = ctypes.POINTER(ctypes.c_int32)
 _u16p = ctypes.POINTER(ctypes.c_uint16)
 
@@ -46,6 +46,22 @@ class EngineConfig(ctypes.Structure):
                 ("seed", c_uint64), ("stop_on_eos", c_int), ("ctx_overflow", c_int),
                 ("prefill_mode", c_int)]
 
+
+QWEN_DTYPE_F16 = 0
+QWEN_DTYPE_BF16 = 1
+
+
+class PagedKVStruct(ctypes.Structure):
+    """qwen_paged_kv."""
+
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("bounds", c_void_p), ("page_table", c_void_p),
+                ("page_stride", c_int64), ("pos_stride", c_int64), ("head_stride", c_int64),
+                ("n_pages", c_uint32), ("page_size", c_uint32), ("n_kv_heads", c_uint32),
+                ("head_dim", c_uint32), ("n_seq", c_uint32), ("max_pages", c_uint32),
+                ("table_stride", c_uint32), ("dtype", c_int32)]
+
+
+_kvp = ctypes.POINTER(PagedKVStruct)
 
 # name -> (restype, argtypes)
 SIGNATURES = {
@@ -80,6 +96,23 @@ SIGNATURES = {
     "qwen_sample_scratch_bytes": (c_size_t, [c_uint32]),
     "qwen_sample_scratch": (c_int, [c_void_p, c_uint32, c_uint32, c_uint32, c_float, c_float,
                                     c_void_p, c_void_p, c_void_p, c_void_p]),
+    "qwen_rope_append_paged": (c_int, [_kvp, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                                       c_int64, c_void_p, c_int64, c_uint32, c_uint32, c_void_p,
+                                       c_void_p, c_void_p, c_uint32, c_int, c_void_p]),
+    "qwen_attention_paged_workspace": (c_size_t, [_kvp, c_uint32]),
+    "qwen_attention_paged": (c_int, [_kvp, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                                     c_uint32, c_void_p, c_float, c_void_p, c_size_t, c_void_p]),
+    "qwen_attention_prefix_paged_workspace": (c_size_t, [_kvp, c_uint32, c_uint32]),
+    "qwen_attention_prefix_paged": (c_int, [_kvp, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                                            c_uint32, c_void_p, c_void_p, c_uint32, c_float,
+                                            c_void_p, c_size_t, c_void_p]),
+    "qwen_select_pages_workspace": (c_size_t, [_kvp]),
+    "qwen_select_pages": (c_int, [_kvp, c_void_p, c_int64, c_uint32, c_void_p, c_uint32, c_uint32,
+                                  c_uint32, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "qwen_attention_sparse_paged_workspace": (c_size_t, [_kvp, c_uint32, c_uint32]),
+    "qwen_attention_sparse_paged": (c_int, [_kvp, c_void_p, c_uint32, c_void_p, c_int64, c_void_p,
+                                            c_int64, c_void_p, c_uint32, c_void_p, c_float,
+                                            c_void_p, c_size_t, c_void_p]),
     "qwen_uniform24": (c_uint32, [c_uint64, c_uint64, c_uint64]),
     "qwen_engine_config_default": (None, [ctypes.POINTER(EngineConfig)]),
     "qwen_engine_create": (c_int, [ctypes.POINTER(EngineConfig), ctypes.POINTER(c_void_p)]),

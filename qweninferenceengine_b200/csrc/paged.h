@@ -1,0 +1,67 @@
+// paged.h -- operators over a paged key/value cache (qwen_paged_kv of
+// include/qwen_b200.h): parameters the entry points hand to the launchers.
+#pragma once
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "../../include/qwen_b200.h"
+
+namespace qwen {
+
+constexpr int kMaxGroup = 64;   // query heads per kv head
+
+// What an attention launch reads and writes.  Rows are [heads][head_dim].
+struct PagedAttnArgs {
+  qwen_paged_kv kv;
+  int page_shift;               // page_size = 1 << page_shift
+  const uint16_t* q;
+  long long q_stride;
+  uint16_t* out;
+  long long out_stride;
+  float* lse;                   // may be null
+  int n_heads;
+  const uint32_t* seq_len;
+  float scale;
+  const int32_t* list;          // sparse: [n_seq][n_kv_heads][n_list] page_table columns
+  int n_list;
+  const int32_t* prefix_pages;  // shared prefix: pool pages, null without one
+  uint32_t prefix_len;
+  void* workspace;
+  int* err;                     // operator status word
+};
+int launch_paged_attention(const PagedAttnArgs& a, cudaStream_t st);
+
+struct PagedAppendArgs {
+  qwen_paged_kv kv;
+  int page_shift;
+  const uint16_t *q, *k, *v;
+  long long q_stride, k_stride, v_stride;
+  uint16_t* q_out;
+  long long q_out_stride;
+  int n_heads;
+  int n_tokens;
+  const uint32_t* seq_len;
+  const int32_t* cu_tokens;     // null: one token per sequence
+  const float* inv_freq;
+  int rot_dim;
+  int interleaved;
+  int* err;
+};
+int launch_rope_append(const PagedAppendArgs& a, cudaStream_t st);
+
+struct PagedSelectArgs {
+  qwen_paged_kv kv;
+  int page_shift;
+  const uint16_t* q;
+  long long q_stride;
+  int n_heads;
+  const uint32_t* seq_len;
+  int n_select, n_first, n_last;
+  int32_t* pages;               // [n_seq][n_kv_heads][n_select]
+  double* scores;               // workspace: [n_seq][n_kv_heads][max_pages]
+  int* err;
+};
+int launch_select_pages(const PagedSelectArgs& a, cudaStream_t st);
+
+}  // namespace qwen

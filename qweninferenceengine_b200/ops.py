@@ -5,9 +5,11 @@ torch stream.
 """
 from __future__ import annotations
 
+from ctypes import byref
+
 import torch
 
-from ._lib import check, lib
+from ._lib import QWEN_DTYPE_BF16, QWEN_DTYPE_F16, PagedKVStruct, check, lib
 
 HIDDEN, INTER, HEADS, KV_DIM, HEAD_DIM = 1536, 8960, 12, 256, 128
 VOCAB, ACTUAL_VOCAB = 151936, 151666
@@ -175,3 +177,201 @@ def sample_scratch(n_seq: int, device) -> torch.Tensor | None:
 
 def uniform24(seed: int, sequence: int, step: int) -> int:
     return lib().qwen_uniform24(seed, sequence, step)
+
+
+# ---------------------------------------------------------- paged cache -----
+_DTYPES = {torch.float16: QWEN_DTYPE_F16, torch.bfloat16: QWEN_DTYPE_BF16}
+
+
+class PagedKV:
+    """One layer's paged key/value cache (qwen_paged_kv) over the caller's tensors.
+
+    k_pages, v_pages: [n_pages, page_size, n_kv_heads, head_dim], fp16 or bf16, any
+    (equal) strides with the head's elements adjacent: head-major pages are
+    `pool.transpose(1, 2)`.  page_table: int32 [n_seq, max_pages], the pool page of
+    each sequence's page.  bounds: [n_pages, 2, n_kv_heads, head_dim], the least and
+    largest stored key of each page (kept by rope_append_paged, read by
+    select_pages); None keeps none.  The object holds references to the tensors and
+    reads nothing of their contents; their shapes and addresses must not change."""
+
+    __slots__ = ("k_pages", "v_pages", "page_table", "bounds", "dtype", "device", "n_seq",
+                 "n_kv_heads", "head_dim", "struct", "ref")
+
+    def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                 bounds: torch.Tensor | None = None):
+        dtype, device = k_pages.dtype, k_pages.device
+        if dtype not in _DTYPES:
+            raise ValueError(f"k_pages must be float16 or bfloat16, not {dtype}")
+        if not k_pages.is_cuda:
+            raise ValueError("expected a CUDA tensor")
+        if k_pages.dim() != 4:
+            raise ValueError("k_pages must be [n_pages, page_size, n_kv_heads, head_dim]")
+        n_pages, page_size, n_kv, dim = k_pages.shape
+        st = k_pages.stride()
+        if v_pages.shape != k_pages.shape or v_pages.stride() != st or v_pages.dtype != dtype:
+            raise ValueError("k_pages and v_pages must have the same shape, strides and dtype")
+        if st[3] != 1:
+            raise ValueError("the elements of a head must be adjacent")
+        if page_table.dim() != 2 or page_table.dtype != torch.int32 or \
+                (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+            raise ValueError("page_table must be int32 [n_seq, max_pages] with adjacent columns")
+        if v_pages.device != device or page_table.device != device:
+            raise ValueError("the cache's tensors must be on one device")
+        if bounds is not None and (bounds.shape != (n_pages, 2, n_kv, dim) or bounds.dtype != dtype
+                                   or not bounds.is_contiguous() or bounds.device != device):
+            raise ValueError("bounds must be a contiguous [n_pages, 2, n_kv_heads, head_dim] tensor "
+                             "of the cache's dtype and device")
+        n_seq, max_pages = page_table.shape
+        self.k_pages, self.v_pages, self.page_table, self.bounds = k_pages, v_pages, page_table, bounds
+        self.dtype, self.device, self.n_seq = dtype, device, n_seq
+        self.n_kv_heads, self.head_dim = n_kv, dim
+        # the stride of an axis of one element is never used: any valid value
+        self.struct = PagedKVStruct(
+            k_pages.data_ptr(), v_pages.data_ptr(), None if bounds is None else bounds.data_ptr(),
+            page_table.data_ptr(), st[0] if n_pages > 1 else page_size * n_kv * dim, st[1],
+            st[2] if n_kv > 1 else dim, n_pages, page_size, n_kv, dim, n_seq, max_pages,
+            page_table.stride(0) if n_seq > 1 else max_pages, _DTYPES[dtype])
+        self.ref = byref(self.struct)
+
+
+def _rows(name: str, x: torch.Tensor, kv: PagedKV, n_rows: int | None, n_heads: int | None = None):
+    """(address, row stride) of a [rows, heads, head_dim] tensor whose rows are head-contiguous."""
+    if x.dtype != kv.dtype or x.device != kv.device:
+        raise ValueError(f"{name} must be {kv.dtype} on {kv.device}")
+    if x.dim() != 3 or x.shape[2] != kv.head_dim or (n_rows is not None and x.shape[0] != n_rows) or \
+            (n_heads is not None and x.shape[1] != n_heads):
+        raise ValueError(f"{name} has shape {tuple(x.shape)}: expected [{n_rows or 'rows'}, "
+                         f"{n_heads or 'heads'}, {kv.head_dim}]")
+    row, head, el = x.stride()
+    if el != 1 or (x.shape[1] > 1 and head != kv.head_dim):
+        raise ValueError(f"{name}: the heads of a row must be adjacent")
+    return x.data_ptr(), row if x.shape[0] > 1 else x.shape[1] * kv.head_dim
+
+
+def _ints(name: str, x: torch.Tensor, kv: PagedKV, n: int | None) -> int:
+    """Address of a contiguous int32 (or uint32) vector of n values."""
+    if x.dtype not in (torch.int32, torch.uint32) or x.device != kv.device or x.dim() != 1 or \
+            (n is not None and x.shape[0] != n) or not x.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor"
+                         f"{'' if n is None else f' of {n} values'} on {kv.device}")
+    return x.data_ptr()
+
+
+def _on(kv: PagedKV, fn, *args) -> None:
+    """Calls a library entry on the cache's device and its current stream."""
+    index = kv.device.index
+    if index == torch.cuda.current_device():
+        check(fn(kv.ref, *args, torch.cuda.current_stream().cuda_stream))
+    else:
+        with torch.cuda.device(index):
+            check(fn(kv.ref, *args, torch.cuda.current_stream().cuda_stream))
+
+
+def rope_append_paged(kv: PagedKV, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                      seq_len: torch.Tensor, inv_freq: torch.Tensor,
+                      cu_tokens: torch.Tensor | None = None, interleaved: bool = False,
+                      out: torch.Tensor | None = None) -> torch.Tensor:
+    """apply_rope_q4 and write_kv_cache (rope.metal:12-39, attention.metal:67-84)
+    of a batch of new tokens over a paged cache (qwen_rope_append_paged): rotates
+    q [n, heads, d] into `out` (which may be q; new memory by default), writes
+    rotated k and v [n, kv_heads, d] to the cache and keeps its bounds.
+
+    seq_len [n_seq] counts the new tokens.  cu_tokens int32 [n_seq + 1]: sequence s
+    owns rows cu_tokens[s]:cu_tokens[s + 1], its last positions; rows behind the last
+    sequence are not touched.  None: row s is sequence s's newest token, and a
+    sequence of length 0 is passed over.  inv_freq: fp32 [rot_dim / 2]."""
+    n, heads = q.shape[0], q.shape[1]
+    qp, qs = _rows("q", q, kv, None)
+    kp, ks = _rows("k", k, kv, n, kv.n_kv_heads)
+    vp, vs = _rows("v", v, kv, n, kv.n_kv_heads)
+    if out is None:
+        out = torch.empty((n, heads, kv.head_dim), dtype=kv.dtype, device=kv.device)
+    op, os_ = _rows("out", out, kv, n, heads)
+    if inv_freq.dtype != torch.float32 or inv_freq.device != kv.device or inv_freq.dim() != 1 or \
+            not inv_freq.is_contiguous():
+        raise ValueError(f"inv_freq must be a contiguous float32 vector on {kv.device}")
+    _on(kv, lib().qwen_rope_append_paged, qp, qs, kp, ks, vp, vs, op, os_, heads, n,
+        _ints("seq_len", seq_len, kv, kv.n_seq),
+        None if cu_tokens is None else _ints("cu_tokens", cu_tokens, kv, kv.n_seq + 1),
+        inv_freq.data_ptr(), 2 * inv_freq.shape[0], 1 if interleaved else 0)
+    return out
+
+
+def _attend(kv, fn, need: int, lead, q, seq_len, extra, scale, out, return_lse):
+    heads = q.shape[1]
+    qp, qs = _rows("q", q, kv, kv.n_seq)
+    if out is None:
+        out = torch.empty((kv.n_seq, heads, kv.head_dim), dtype=kv.dtype, device=kv.device)
+    op, os_ = _rows("out", out, kv, kv.n_seq, heads)
+    lse = torch.empty((kv.n_seq, heads), dtype=torch.float32, device=kv.device) if return_lse else None
+    ws = torch.empty(need, dtype=torch.uint8, device=kv.device) if need else None
+    _on(kv, fn, *lead, qp, qs, op, os_, None if lse is None else lse.data_ptr(), heads,
+        _ints("seq_len", seq_len, kv, kv.n_seq), *extra,
+        kv.head_dim ** -0.5 if scale is None else scale,
+        None if ws is None else ws.data_ptr(), need)
+    return (out, lse) if return_lse else out
+
+
+def attention_paged(kv: PagedKV, q: torch.Tensor, seq_len: torch.Tensor, scale: float | None = None,
+                    out: torch.Tensor | None = None, return_lse: bool = False):
+    """attention_decode_batched over a paged cache (qwen_attention_paged): q
+    [n_seq, heads, d] against each sequence's seq_len positions.  scale defaults to
+    d ** -0.5; lse is the natural log of the sum of exp(scale q K^T), [n_seq, heads]
+    fp32.  A sequence of length 0 gives zeros and -inf."""
+    return _attend(kv, lib().qwen_attention_paged,
+                   lib().qwen_attention_paged_workspace(kv.ref, q.shape[1]), (), q, seq_len, (), scale,
+                   out, return_lse)
+
+
+def attention_prefix_paged(kv: PagedKV, q: torch.Tensor, seq_len: torch.Tensor,
+                           prefix_pages: torch.Tensor, prefix_len: int, scale: float | None = None,
+                           out: torch.Tensor | None = None, return_lse: bool = False):
+    """attention_paged where every sequence begins with the same prefix_len
+    positions, held once in pool pages prefix_pages (int32), read once for the batch
+    (qwen_attention_prefix_paged).  seq_len and the page table describe what follows
+    the prefix."""
+    pages = _ints("prefix_pages", prefix_pages, kv, None)
+    if prefix_len < 0 or prefix_pages.shape[0] * kv.struct.page_size < prefix_len:
+        raise ValueError(f"prefix_len={prefix_len} in {prefix_pages.shape[0]} pages")
+    return _attend(kv, lib().qwen_attention_prefix_paged,
+                   lib().qwen_attention_prefix_paged_workspace(kv.ref, q.shape[1], prefix_len), (), q,
+                   seq_len, (pages, prefix_len), scale, out, return_lse)
+
+
+def select_pages(kv: PagedKV, q: torch.Tensor, seq_len: torch.Tensor, n_select: int, n_first: int = 1,
+                 n_last: int = 1, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The n_select pages of each sequence and kv head whose bounds promise the
+    highest scores for q [n_seq, heads, d] (qwen_select_pages): int32
+    [n_seq, kv_heads, n_select] page-table columns, ascending, -1 behind the last.
+    The first n_first and last n_last pages are always among them; ties go to the
+    lower page."""
+    if n_first < 0 or n_last < 0 or n_select < 1:
+        raise ValueError(f"n_select={n_select} n_first={n_first} n_last={n_last}")
+    qp, qs = _rows("q", q, kv, kv.n_seq)
+    shape = (kv.n_seq, kv.n_kv_heads, n_select)
+    if out is None:
+        out = torch.empty(shape, dtype=torch.int32, device=kv.device)
+    elif out.shape != shape or out.dtype != torch.int32 or out.device != kv.device or \
+            not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous int32 tensor {shape} on {kv.device}")
+    need = lib().qwen_select_pages_workspace(kv.ref)
+    ws = torch.empty(need, dtype=torch.uint8, device=kv.device)
+    _on(kv, lib().qwen_select_pages, qp, qs, q.shape[1], _ints("seq_len", seq_len, kv, kv.n_seq),
+        n_select, n_first, n_last, out.data_ptr(), ws.data_ptr(), need)
+    return out
+
+
+def attention_sparse_paged(kv: PagedKV, q: torch.Tensor, seq_len: torch.Tensor, pages: torch.Tensor,
+                           scale: float | None = None, out: torch.Tensor | None = None,
+                           return_lse: bool = False):
+    """attention_paged over the listed pages alone (qwen_attention_sparse_paged):
+    pages int32 [n_seq, kv_heads, n], page-table columns, -1 for none (a
+    select_pages result); only positions below seq_len count."""
+    if pages.dim() != 3 or pages.shape[:2] != (kv.n_seq, kv.n_kv_heads) or \
+            pages.dtype != torch.int32 or pages.device != kv.device or not pages.is_contiguous():
+        raise ValueError(f"pages must be a contiguous int32 [{kv.n_seq}, {kv.n_kv_heads}, n] tensor "
+                         f"on {kv.device}")
+    n = pages.shape[2]
+    return _attend(kv, lib().qwen_attention_sparse_paged,
+                   lib().qwen_attention_sparse_paged_workspace(kv.ref, q.shape[1], n),
+                   (pages.data_ptr(), n), q, seq_len, (), scale, out, return_lse)
