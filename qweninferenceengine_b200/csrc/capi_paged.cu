@@ -89,8 +89,10 @@ int attention(const char* op, PagedAttnArgs& a, const qwen_paged_kv* kv, const u
   a.scale = scale;
   a.workspace = workspace;
   QWEN_TRY(ops_status_word(&a.err));
-  if (launch_paged_attention(a, static_cast<cudaStream_t>(stream)) != 0) return launch_status(op);
-  return launch_status(op);
+  const int rc = a.prefix_pages ? launch_paged_attention(a, static_cast<cudaStream_t>(stream))
+                                : launch_paged_decode(a, static_cast<cudaStream_t>(stream));
+  QWEN_TRY(launch_status(op));
+  return rc == 0 ? QWEN_OK : set_error(QWEN_ERR_CUDA, "%s: launch failed", op);
 }
 
 }  // namespace
@@ -141,7 +143,9 @@ int qwen_rope_append_paged(const qwen_paged_kv* kv, const uint16_t* q, int64_t q
   return launch_status(op);
 }
 
-size_t qwen_attention_paged_workspace(const qwen_paged_kv*, uint32_t) { return 0; }
+size_t qwen_attention_paged_workspace(const qwen_paged_kv* kv, uint32_t) {
+  return kv ? paged_decode_workspace(*kv) : 0;
+}
 
 int qwen_attention_paged(const qwen_paged_kv* kv, const uint16_t* q, int64_t q_stride,
                          uint16_t* out, int64_t out_stride, float* lse, uint32_t n_heads,
@@ -152,7 +156,9 @@ int qwen_attention_paged(const qwen_paged_kv* kv, const uint16_t* q, int64_t q_s
                    workspace, workspace_bytes, qwen_attention_paged_workspace(kv, n_heads), stream);
 }
 
-size_t qwen_attention_prefix_paged_workspace(const qwen_paged_kv*, uint32_t, uint32_t) { return 0; }
+size_t qwen_attention_prefix_paged_workspace(const qwen_paged_kv* kv, uint32_t, uint32_t) {
+  return kv ? paged_decode_workspace(*kv) : 0;
+}
 
 int qwen_attention_prefix_paged(const qwen_paged_kv* kv, const uint16_t* q, int64_t q_stride,
                                 uint16_t* out, int64_t out_stride, float* lse, uint32_t n_heads,
@@ -205,7 +211,9 @@ int qwen_select_pages(const qwen_paged_kv* kv, const uint16_t* q, int64_t q_stri
   return launch_status(op);
 }
 
-size_t qwen_attention_sparse_paged_workspace(const qwen_paged_kv*, uint32_t, uint32_t) { return 0; }
+size_t qwen_attention_sparse_paged_workspace(const qwen_paged_kv* kv, uint32_t, uint32_t) {
+  return kv ? paged_decode_workspace(*kv) : 0;
+}
 
 int qwen_attention_sparse_paged(const qwen_paged_kv* kv, const int32_t* pages, uint32_t n_select,
                                 const uint16_t* q, int64_t q_stride, uint16_t* out,

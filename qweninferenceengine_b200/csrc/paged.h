@@ -31,6 +31,10 @@ struct PagedAttnArgs {
   int* err;                     // operator status word
 };
 int launch_paged_attention(const PagedAttnArgs& a, cudaStream_t st);
+// Decode attention over own or listed pages (paged_decode.cu); 0, or -1 for a
+// launch failure.
+int launch_paged_decode(const PagedAttnArgs& a, cudaStream_t st);
+size_t paged_decode_workspace(const qwen_paged_kv& kv);
 
 struct PagedAppendArgs {
   qwen_paged_kv kv;

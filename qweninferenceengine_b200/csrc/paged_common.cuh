@@ -1,5 +1,6 @@
 // paged_common.cuh -- device helpers shared by the paged-cache kernels.
 #pragma once
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -9,17 +10,6 @@
 namespace qwen {
 
 // fp16 / bf16 value types behind the 16-bit patterns of the C ABI.
-template <typename T>
-struct Half2Of;
-template <>
-struct Half2Of<__half> {
-  using type = __half2;
-};
-template <>
-struct Half2Of<__nv_bfloat16> {
-  using type = __nv_bfloat162;
-};
-
 __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
 template <typename T>
@@ -28,6 +18,75 @@ template <>
 __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+__device__ __forceinline__ uint32_t pack2(__half, float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(__nv_bfloat16, float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// D = A(16x16, row) * B(16x8, col) + D, fp32 accumulation.
+__device__ __forceinline__ void mma_16816_t(__half, float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                            uint32_t b1) {
+  mma_16816(d, a, b0, b1, d);
+}
+__device__ __forceinline__ void mma_16816_t(__nv_bfloat16, float (&d)[4], const uint32_t (&a)[4],
+                                            uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float exp2_fast(float x) {   // ex2.approx: 2 steps of fp32; -inf gives 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ unsigned long long global_ns() {
+  unsigned long long t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+constexpr unsigned long long kPagedWaitNs = 2000000000ull;
+// Bounded parity wait: false once it ran out (2 s; recorded, *abort set) or,
+// where `heed`, once another role of the CTA gave up.
+static __device__ __noinline__ bool paged_wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort,
+                                             int* err, bool heed) {
+  const unsigned long long t0 = global_ns();
+  for (uint32_t i = 1;; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 63) == 0) {
+      if (heed && *abort) return false;
+      if (global_ns() - t0 > kPagedWaitNs) {
+        *abort = 1;
+        raise_error(err, kDevWaitTimeout);
+        return false;
+      }
+    }
+  }
+}
+__device__ __forceinline__ bool paged_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* err,
+                                           bool heed = true) {
+  return mbar_try_wait(bar, parity) || paged_wait_slow(bar, parity, abort, err, heed);
+}
+
+// 5-D tile load (element, slot, half, head, page) of a cache's tensor map; the
+// box is (64, rows, head_dim / 64, 1, 1), so it lands as [half][rows][128 B].
+__device__ __forceinline__ void tma_load_pages(void* dst, const CUtensorMap* map, int slot, int head,
+                                               int page, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
+      "[%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(slot), "r"(0), "r"(head), "r"(page),
+      "r"(smem_u32(bar))
+      : "memory");
+}
 
 // Positions of sequence s, or 0 with the status word set when the length does
 // not fit its row of the page table (*ok false).

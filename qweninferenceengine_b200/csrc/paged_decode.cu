@@ -1,0 +1,721 @@
+// paged_decode.cu -- decode attention over a paged cache, one query token per
+// sequence, over all of a sequence's pages or over listed ones:
+//   out = sum_t softmax(scale q . K_t) V_t
+//
+// Bound: HBM, each key and value read once (512 B a position and kv head of 128;
+// 4 group flops a byte).  So the kernel is a stream of pages through shared
+// memory with just enough arithmetic beside it.
+//
+// Work: a unit is one (sequence, kv head, up to 16 query heads), a tile 64
+// positions of a unit.  All tiles of all units stand in one row, and CTA c of G
+// (two per SM) takes an equal run of them, start(c) = c T / G, wherever units begin
+// and end: a ragged batch, one long sequence and a batch of short ones all divide
+// evenly.  A unit within one CTA is finished there; a unit cut by a run's end
+// leaves fp32 partials (max, sum, unnormalised output), which k_paged_combine
+// joins in CTA order -- results do not depend on timing, and nothing has to be
+// zero beforehand.
+//
+// CTA: 4 consumer warps and a producer warp.  Per tile the producer's lanes read
+// list and page table (32 entries at a time), issue one TMA load per box of 16 or
+// 32 positions for K and for V (a 5-D map over the pool, so any stride order; the
+// 128-byte swizzle keeps fragment loads free of bank conflicts), and write how many
+// of each warp's 16 positions count.  Positions past a sequence's end and pages
+// outside the pool are never loaded or, inside a box, masked in registers.
+// Consumer warp w takes positions 16w..16w+15 of a tile on its own:
+//   S^T[16 pos x 8 heads] = K q^T, the softmax, o^T[d x 8] += V^T P^T
+// with m16n8k16 MMAs (8 = the heads that share the kv head; tcgen05's smallest
+// M of 64 would be nine tenths padding), P^T turned by movmatrix.
+// The running maximum moves only when a score passes it by 2^15 (a vote, no
+// shuffles, in most tiles): weights are formed as 2^(s - r), r = max - 7 when last
+// moved, which keeps them within fp16's normal range from 2^15 down to 2^-21 of
+// the largest.  P is rounded once to the cache's type for the MMA (relative 2^-11 or
+// 2^-8, averaged over positions); sums, maxima and outputs are fp32.
+#include <cudaTypedefs.h>
+
+#include <mutex>
+
+#include "paged_common.cuh"
+#include "qwen_internal.h"
+
+namespace qwen {
+namespace {
+
+constexpr int kTile = 64;                     // positions of a tile
+constexpr int kWarps = kTile / 16;            // consumer warps
+constexpr int kThreads = (kWarps + 1) * 32;
+constexpr int kCtasPerSm = 2;
+constexpr int kMaxSlotHeads = 16;             // query heads of a unit
+
+enum StageFlags { kFirst = 1, kLast = 2, kEnd = 4 };
+
+struct StageMeta {
+  int valid[kWarps];   // positions of each warp's 16 that count
+  int flags;
+  int seq, head, heads;   // the unit: sequence, first query head, query heads
+  int dest;            // partial slot, or -1: the whole unit, or -2: nothing is written
+};
+
+template <int D>
+constexpr int stages() {
+  return D == 128 ? 3 : 6;
+}
+
+template <int D>
+struct __align__(1024) DecodeSmem {
+  uint8_t kv[stages<D>()][2][kTile * D * 2];
+  float o[kWarps][4][D + 8];
+  uint16_t q[kMaxSlotHeads * D];
+  float m[kWarps][kMaxSlotHeads], l[kWarps][kMaxSlotHeads];
+  StageMeta meta[stages<D>()];
+  uint64_t full[stages<D>()], empty[stages<D>()], qfull, qempty, joined;
+  unsigned long long scan[kWarps + 1];
+  unsigned long long found_cum;
+  int found_seq;
+  int abort;
+};
+
+struct DecodeArgs {
+  PagedAttnArgs a;
+  int units_per_seq;        // kv heads x chunks of at most 16 query heads
+  int chunks;               // chunks per kv head
+  int list_tiles;           // tiles of a listed unit
+  float scale_log2;
+  float* part_o;            // [2 G][16][D]
+  float* part_ml;           // [2 G][16][2]
+};
+
+__device__ __forceinline__ uint32_t seq_tiles(const DecodeArgs& p, uint32_t L) {
+  if (p.a.list) return p.list_tiles;
+  if (L > p.a.kv.max_pages * p.a.kv.page_size) return 0;
+  return L ? (L + kTile - 1) / kTile : 1;   // an empty sequence still has its zeros written
+}
+
+// Total number of tiles, and the sequence that holds tile `at(total)` with the
+// number of tiles per unit before it.  Called by all n threads of a block.
+template <typename At>
+__device__ unsigned long long find_tile(const DecodeArgs& p, unsigned long long* scan,
+                                        unsigned long long* found_cum, int* found_seq, bool report, At at) {
+  const int n = blockDim.x, tid = threadIdx.x, n_seq = p.a.kv.n_seq;
+  if (p.a.list) {
+    const unsigned long long total = (unsigned long long)p.list_tiles * n_seq;
+    if (tid == 0) {
+      *found_seq = (int)(at(total * p.units_per_seq) / ((unsigned long long)p.list_tiles * p.units_per_seq));
+      *found_cum = (unsigned long long)*found_seq * p.list_tiles;
+    }
+    __syncthreads();
+    return total * p.units_per_seq;
+  }
+  const int per = (n_seq + n - 1) / n, s0 = min(n_seq, tid * per), s1 = min(n_seq, s0 + per);
+  unsigned long long sum = 0;
+  for (int s = s0; s < s1; ++s) {
+    const uint32_t t = seq_tiles(p, p.a.seq_len[s]);
+    if (t == 0 && report) raise_error(p.a.err, kDevBadArgument);
+    sum += t;
+  }
+  unsigned long long inc = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned long long v = __shfl_up_sync(0xffffffffu, inc, o);
+    if ((tid & 31) >= o) inc += v;
+  }
+  if ((tid & 31) == 31) scan[tid >> 5] = inc;
+  if (tid == 0) *found_seq = n_seq;
+  __syncthreads();
+  unsigned long long before = inc - sum, total = 0;
+  for (int w = 0; w < n / 32; ++w) {
+    if (w < (tid >> 5)) before += scan[w];
+    total += scan[w];
+  }
+  total *= p.units_per_seq;
+  const unsigned long long target = at(total), u = p.units_per_seq;
+  if (target >= u * before && target < u * (before + sum)) {
+    int s = s0;
+    for (uint32_t t; target >= u * (before + (t = seq_tiles(p, p.a.seq_len[s]))); ++s) before += t;
+    *found_seq = s;
+    *found_cum = before;
+  }
+  __syncthreads();
+  return total;
+}
+
+__device__ __forceinline__ unsigned long long run_start(unsigned long long total, int c, int G) {
+  return total * (unsigned)c / (unsigned)G;
+}
+// The run that holds tile x: the largest c with run_start(c) <= x.
+__device__ __forceinline__ int run_of(unsigned long long total, unsigned long long x, int G) {
+  return (int)(((x + 1) * G - 1) / total);
+}
+
+template <typename T>
+__device__ __forceinline__ void store_vec(T* dst, const float* v, int n) {
+  if (n == 4) {
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(T{}, v[0], v[1]), pack2(T{}, v[2], v[3]));
+  } else {
+    *reinterpret_cast<uint32_t*>(dst) = pack2(T{}, v[0], v[1]);
+  }
+}
+
+__device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ void ldmatrix_x4_t(uint32_t (&r)[4], const void* p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(smem_u32(p))
+               : "memory");
+}
+
+// NT: 8-head MMA columns of a unit (1 or 2).
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm)
+    k_paged_decode(const __grid_constant__ DecodeArgs p, int box_rows,
+                   const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv) {
+  constexpr int ST = stages<D>();
+  extern __shared__ uint8_t smem_raw[];
+  DecodeSmem<D>& s = *reinterpret_cast<DecodeSmem<D>*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
+  const PagedAttnArgs& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(&s.full[i], 1);
+      mbar_init(&s.empty[i], kWarps);
+    }
+    mbar_init(&s.qfull, 1);
+    mbar_init(&s.qempty, kWarps);
+    mbar_init(&s.joined, kWarps);
+    s.abort = 0;
+    fence_mbar_init();
+    pdl_launch_dependents();
+  }
+  pdl_wait();
+  const int c = blockIdx.x, G = gridDim.x;
+  const unsigned long long total = find_tile(p, s.scan, &s.found_cum, &s.found_seq, c == 0,
+                                             [&](unsigned long long n) { return run_start(n, c, G); });
+  const unsigned long long t1 = run_start(total, c + 1, G);
+  unsigned long long t = run_start(total, c, G);
+  if (t >= t1) return;
+
+  if (warp == kWarps) {
+    // ------------------------------------------------------------ producer --
+    const int P = a.kv.page_size;
+    const int boxes = kTile / box_rows;                  // of K, and as many of V
+    const uint32_t box_bytes = (uint32_t)box_rows * D * 2;
+    const uint32_t capacity = a.kv.max_pages * a.kv.page_size;
+    uint32_t it = 0, pieces = 0;
+    int seq = s.found_seq;
+    unsigned long long cum = s.found_cum;
+    uint32_t L = a.seq_len[seq], ts = seq_tiles(p, L);
+    int cached_unit = -1, cached_base = 0, col = -1, page = -1;   // lane i: list / table entry cached_base + i
+    bool alive = true;
+    while (t < t1 && alive) {
+      while (ts == 0 || t >= p.units_per_seq * (cum + ts)) {
+        cum += ts;
+        L = a.seq_len[++seq];
+        ts = seq_tiles(p, L);
+      }
+      const unsigned long long rel = t - p.units_per_seq * cum;
+      const uint32_t unit = (uint32_t)(rel / ts), tile0 = (uint32_t)(rel % ts);
+      const uint32_t tile1 = (uint32_t)min((unsigned long long)ts, tile0 + (t1 - t));
+      t += tile1 - tile0;
+      const int h = (int)unit / p.chunks, chunk = (int)unit % p.chunks;
+      const int group = a.n_heads / (int)a.kv.n_kv_heads;
+      const int head = h * group + chunk * kMaxSlotHeads, heads = min(kMaxSlotHeads, group - chunk * kMaxSlotHeads);
+      const bool fits = L <= capacity;
+      if (!fits && lane == 0) raise_error(a.err, kDevBadArgument);
+      const int dest = !fits ? -2 : tile0 == 0 && tile1 == ts ? -1 : 2 * c + (tile0 == 0 ? 1 : 0);
+      // the unit's queries
+      if (pieces && !__all_sync(0xffffffffu, paged_wait(&s.qempty, (pieces - 1) & 1, &s.abort, a.err))) break;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&s.qfull, (uint32_t)heads * D * 2);
+        bulk_g2s(s.q, a.q + (long long)seq * a.q_stride + (long long)head * D, (uint32_t)heads * D * 2, &s.qfull);
+      }
+      ++pieces;
+      const int32_t* table = a.kv.page_table + (long long)seq * a.kv.table_stride;
+      const int32_t* list = a.list ? a.list + ((long long)seq * a.kv.n_kv_heads + h) * a.n_list : nullptr;
+      const int n_entries = a.list ? a.n_list : (int)((L + P - 1) >> a.page_shift);
+      const int unit_id = a.list ? seq * (int)a.kv.n_kv_heads + h : seq;   // one table row serves all heads
+      bool first = true;
+      for (uint32_t tile = tile0; tile < tile1; ++tile) {
+        // this lane's box: positions box_pos .. + box_rows - 1 of the unit
+        const int b = lane % boxes;
+        const int box_pos = (int)tile * kTile + b * box_rows;
+        const int entry = box_pos >> a.page_shift, off = box_pos & (P - 1);
+        const int last_entry = ((int)tile * kTile + kTile - 1) >> a.page_shift;
+        const int first_entry = ((int)tile * kTile) >> a.page_shift;
+        if (cached_unit != unit_id || first_entry < cached_base || last_entry >= cached_base + 32) {
+          cached_unit = unit_id;
+          cached_base = first_entry;
+          const int e = cached_base + lane;
+          col = e < n_entries ? (list ? list[e] : e) : -1;
+          page = -1;
+          if (fits && col != -1) {
+            const bool in_table = col >= 0 && col < (int)a.kv.max_pages;
+            if (in_table && (uint32_t)col * P < L) page = table[col];
+            const bool bad = !in_table || ((uint32_t)col * P < L && (page < 0 || (uint32_t)page >= a.kv.n_pages));
+            if (bad) {
+              raise_error(a.err, kDevBadArgument);
+              page = -1;
+            }
+          }
+        }
+        const int my_col = __shfl_sync(0xffffffffu, col, entry - cached_base);
+        const int my_page = __shfl_sync(0xffffffffu, page, entry - cached_base);
+        int rows = 0;   // positions of the box that count
+        if (my_page >= 0) rows = min(max((int)L - (my_col * P + off), 0), box_rows);
+        const uint32_t any = __ballot_sync(0xffffffffu, lane < boxes && rows > 0);
+        const bool last = tile + 1 == tile1;
+        if (!any && !last) continue;   // nothing of the tile is listed
+        const int st = it % ST;
+        if (it >= ST &&
+            !__all_sync(0xffffffffu, paged_wait(&s.empty[st], ((it / ST) - 1) & 1, &s.abort, a.err))) {
+          alive = false;
+          break;
+        }
+        // how many of each warp's 16 positions count
+        const int slice_rows = __shfl_sync(0xffffffffu, rows, (lane & (kWarps - 1)) * 16 / box_rows);
+        StageMeta& meta = s.meta[st];
+        if (lane < kWarps) meta.valid[lane] = min(max(slice_rows - lane * 16 % box_rows, 0), 16);
+        if (lane == 0) {
+          meta.flags = (first ? kFirst : 0) | (last ? kLast : 0);
+          meta.seq = seq;
+          meta.head = head;
+          meta.heads = heads;
+          meta.dest = dest;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive_expect_tx(&s.full[st], 2 * box_bytes * __popc(any));
+        __syncwarp();
+        if (lane < 2 * boxes && rows > 0)
+          tma_load_pages(s.kv[st][lane / boxes] + b * box_bytes, lane < boxes ? &tmk : &tmv, off, h, my_page,
+                         &s.full[st]);
+        first = false;
+        ++it;
+      }
+    }
+    uint32_t drained = it >= (uint32_t)ST ? it - ST : 0;
+    if (alive) {   // the end of the run, in a stage whose last copy was consumed
+      const int st = it % ST;
+      alive = it < ST || __all_sync(0xffffffffu, paged_wait(&s.empty[st], ((it / ST) - 1) & 1, &s.abort, a.err));
+      if (alive) {
+        if (it >= ST) ++drained;
+        if (lane == 0) {
+          s.meta[st].flags = kEnd;
+          mbar_arrive(&s.full[st]);
+        }
+      }
+    }
+    __syncwarp();
+    // Every issued copy lands before the CTA may exit.
+    for (uint32_t j = drained; j < it; ++j)
+      paged_wait(&s.full[j % ST], (j / ST) & 1, &s.abort, a.err, false);
+    if (pieces) paged_wait(&s.qfull, (pieces - 1) & 1, &s.abort, a.err, false);
+    return;
+  }
+
+  // -------------------------------------------------------------- consumers --
+  const int g = lane >> 2, t4 = lane & 3;
+  const int box = 16 * warp / box_rows, row0 = 16 * warp % box_rows;
+  const uint32_t box_off = (uint32_t)box * box_rows * D * 2;
+  const uint32_t half_bytes = (uint32_t)box_rows * 128;   // [half][rows][128 B] of a box
+  uint32_t qf[NT][D / 8];
+  float o[NT][D / 16][4], m[NT][2], l[NT][2];
+  uint32_t pieces = 0, joins = 0;
+  auto join = [&]() {   // the consumer warps' barrier
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&s.joined);
+    return __all_sync(0xffffffffu, paged_wait(&s.joined, joins++ & 1, &s.abort, a.err));
+  };
+  for (uint32_t it = 0;; ++it) {
+    const int st = it % ST;
+    if (!__all_sync(0xffffffffu, paged_wait(&s.full[st], (it / ST) & 1, &s.abort, a.err))) return;
+    const StageMeta meta = s.meta[st];
+    if (meta.flags & kEnd) return;
+    if (meta.flags & kFirst) {
+      if (!__all_sync(0xffffffffu, paged_wait(&s.qfull, pieces & 1, &s.abort, a.err))) return;
+      ++pieces;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {
+          const uint4 v = 8 * n + g < meta.heads
+                              ? *reinterpret_cast<const uint4*>(s.q + (8 * n + g) * D + (j >> 1) * 64 +
+                                                                (2 * t4 + (j & 1)) * 8)
+                              : make_uint4(0, 0, 0, 0);
+          qf[n][4 * j] = v.x;
+          qf[n][4 * j + 1] = v.y;
+          qf[n][4 * j + 2] = v.z;
+          qf[n][4 * j + 3] = v.w;
+        }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.qempty);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        m[n][0] = m[n][1] = -INFINITY;
+        l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+      }
+    }
+    const int valid = warp == 0 ? meta.valid[0] : warp == 1 ? meta.valid[1] : warp == 2 ? meta.valid[2] : meta.valid[3];
+    if (valid > 0) {
+      const uint8_t* kb = s.kv[st][0] + box_off;
+      const uint8_t* vb = s.kv[st][1] + box_off;
+      // ---- S^T = K q^T.  Lane (g, t) holds 16-byte chunks 2t, 2t+1 of each half of
+      // rows g and g+8 (with the swizzle, eight lanes touch eight bank groups); the
+      // MMA's k order is the lanes' order, the same for q.
+      float sv[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) sv[n][0] = sv[n][1] = sv[n][2] = sv[n][3] = 0.f;
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) {
+        const uint8_t* p0 = kb + (j >> 1) * half_bytes + (row0 + g) * 128 + (((2 * t4 + (j & 1)) ^ g) << 4);
+        const uint4 x = *reinterpret_cast<const uint4*>(p0), y = *reinterpret_cast<const uint4*>(p0 + 8 * 128);
+        const uint32_t a0[4] = {x.x, y.x, x.y, y.y}, a1[4] = {x.z, y.z, x.w, y.w};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          mma_16816_t(T{}, sv[n], a0, qf[n][4 * j], qf[n][4 * j + 1]);
+          mma_16816_t(T{}, sv[n], a1, qf[n][4 * j + 2], qf[n][4 * j + 3]);
+        }
+      }
+      // sv: (pos g, heads 2t, 2t+1), (pos g+8, heads 2t, 2t+1)
+      bool grown = false;
+      float mx[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sv[n][e] *= p.scale_log2;
+        if (g >= valid) sv[n][0] = sv[n][1] = -INFINITY;
+        if (g + 8 >= valid) sv[n][2] = sv[n][3] = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          mx[n][e] = fmaxf(sv[n][e], sv[n][2 + e]);
+          grown |= mx[n][e] > m[n][e] + 15.f;
+        }
+      }
+      if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float x = mx[n][e];
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            const float r = fmaxf(m[n][e], x - 7.f);
+            const float f = r == -INFINITY ? 1.f : exp2_fast(m[n][e] - r);
+            m[n][e] = r;
+            l[n][e] *= f;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+              o[n][i][e] *= f;
+              o[n][i][2 + e] *= f;
+            }
+          }
+      }
+      uint32_t b0[NT], b1[NT];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float r = m[n][e] == -INFINITY ? 0.f : m[n][e];
+          sv[n][e] = exp2_fast(sv[n][e] - r);
+          sv[n][2 + e] = exp2_fast(sv[n][2 + e] - r);
+          l[n][e] += sv[n][e] + sv[n][2 + e];
+        }
+        b0[n] = movmatrix(pack2(T{}, sv[n][0], sv[n][1]));   // (head g; pos 2t, 2t+1)
+        b1[n] = movmatrix(pack2(T{}, sv[n][2], sv[n][3]));   // (head g; pos 2t+8, 2t+9)
+      }
+      // ---- o^T += V^T P^T: A = V^T[16 d x 16 pos] by ldmatrix.trans.
+      const int vrow = row0 + (lane & 7) + ((lane >> 4) << 3);
+      const uint8_t* vp = vb + vrow * 128;
+      const int vchunk = (lane >> 3) & 1;
+      if (valid == 16) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          uint32_t av[4];
+          ldmatrix_x4_t(av, vp + (i >> 2) * half_bytes + (((2 * (i & 3) + vchunk) ^ (lane & 7)) << 4));
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_16816_t(T{}, o[n][i], av, b0[n], b1[n]);
+        }
+      } else {   // what lies past the end may be anything: 0 weight times NaN would be NaN
+        const uint32_t k0 = (2 * t4 < valid ? 0xffffu : 0u) | (2 * t4 + 1 < valid ? 0xffff0000u : 0u);
+        const uint32_t k1 = (2 * t4 + 8 < valid ? 0xffffu : 0u) | (2 * t4 + 9 < valid ? 0xffff0000u : 0u);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          uint32_t av[4];
+          ldmatrix_x4_t(av, vp + (i >> 2) * half_bytes + (((2 * (i & 3) + vchunk) ^ (lane & 7)) << 4));
+          av[0] &= k0;
+          av[1] &= k0;
+          av[2] &= k1;
+          av[3] &= k1;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_16816_t(T{}, o[n][i], av, b0[n], b1[n]);
+        }
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&s.empty[st]);
+    if (!(meta.flags & kLast)) continue;
+
+    // ---- join the warps: o[n][i][e]: (d 16i+g, head 8n+2t+e), [2+e]: (d 16i+g+8, ..)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float x = l[n][e];
+        x += __shfl_xor_sync(0xffffffffu, x, 4);
+        x += __shfl_xor_sync(0xffffffffu, x, 8);
+        x += __shfl_xor_sync(0xffffffffu, x, 16);
+        if (g == 0) {
+          s.m[warp][8 * n + 2 * t4 + e] = m[n][e];
+          s.l[warp][8 * n + 2 * t4 + e] = x;
+        }
+      }
+    if (!join()) return;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        // a pass: heads 8n + 2t + e, t = 0..3; lane's share of the output: head t = warp
+        const int mine = 8 * n + 2 * t4 + e;
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s.m[w][mine]);
+        const float f = m[n][e] == -INFINITY ? 0.f : exp2_fast(m[n][e] - M);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          s.o[warp][t4][16 * i + g] = o[n][i][e] * f;
+          s.o[warp][t4][16 * i + g + 8] = o[n][i][2 + e] * f;
+        }
+        if (!join()) return;
+        const int hh = 8 * n + 2 * warp + e;
+        if (hh < meta.heads && meta.dest != -2) {
+          float Mh = -INFINITY, Lh = 0.f;
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) Mh = fmaxf(Mh, s.m[w][hh]);
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w)
+            Lh += s.m[w][hh] == -INFINITY ? 0.f : s.l[w][hh] * exp2_fast(s.m[w][hh] - Mh);
+          constexpr int V = D / 32;   // elements of this lane
+          float v[V];
+#pragma unroll
+          for (int k = 0; k < V; ++k) v[k] = 0.f;
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w)
+#pragma unroll
+            for (int k = 0; k < V; ++k) v[k] += s.o[w][warp][V * lane + k];
+          if (meta.dest == -1) {
+            const float inv = Lh == 0.f ? 0.f : 1.f / Lh;
+#pragma unroll
+            for (int k = 0; k < V; ++k) v[k] *= inv;
+            store_vec(reinterpret_cast<T*>(a.out) + (long long)meta.seq * a.out_stride +
+                          (long long)(meta.head + hh) * D + V * lane, v, V);
+            if (a.lse && lane == 0)
+              a.lse[(long long)meta.seq * a.n_heads + meta.head + hh] =
+                  Lh == 0.f ? -INFINITY : (Mh + log2f(Lh)) * kLn2;
+          } else {
+            const long long slot = (long long)meta.dest * kMaxSlotHeads + hh;
+#pragma unroll
+            for (int k = 0; k < V; ++k) p.part_o[slot * D + V * lane + k] = v[k];
+            if (lane == 0) {
+              p.part_ml[2 * slot] = Mh;
+              p.part_ml[2 * slot + 1] = Lh;
+            }
+          }
+        }
+        if (!join()) return;   // s.o, s.m and s.l are written again
+      }
+  }
+}
+
+// Joins the partials of the units that run ends cut: CTA c - 1 takes the unit cut
+// at the end of run c - 1 if that is the unit's first cut.  Warps take the unit's
+// heads (and, with heads_split, blockIdx.y one head each, its warps the partials).
+template <typename T, int D>
+__global__ void __launch_bounds__(256) k_paged_combine(const __grid_constant__ DecodeArgs p, int G,
+                                                       int heads_split) {
+  __shared__ unsigned long long scan[8], found_cum;
+  __shared__ int found_seq;
+  __shared__ float sm[8], sl[8];
+  __shared__ float so[8][D];
+  constexpr int V = D / 32;
+  pdl_wait();
+  const PagedAttnArgs& a = p.a;
+  const int c = blockIdx.x + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const unsigned long long total = find_tile(p, scan, &found_cum, &found_seq, false,
+                                             [&](unsigned long long n) { return run_start(n, c, G); });
+  const unsigned long long cut = run_start(total, c, G);
+  if (cut >= total) return;
+  const int seq = found_seq;
+  const uint32_t L = a.seq_len[seq], ts = seq_tiles(p, L);
+  const unsigned long long rel = cut - p.units_per_seq * found_cum;
+  const uint32_t tile = (uint32_t)(rel % ts);
+  const unsigned long long begin = cut - tile, end = begin + ts;
+  if (tile == 0 || run_start(total, c - 1, G) > begin) return;
+  if (L > a.kv.max_pages * a.kv.page_size) return;
+  const int c0 = run_of(total, begin, G), c1 = run_of(total, end - 1, G);
+  const int unit = (int)(rel / ts), h = unit / p.chunks, chunk = unit % p.chunks;
+  const int group = a.n_heads / (int)a.kv.n_kv_heads;
+  const int head = h * group + chunk * kMaxSlotHeads, heads = min(kMaxSlotHeads, group - chunk * kMaxSlotHeads);
+  // the unit's partials: slot 1 of run c0, slot 0 of the non-empty runs after it
+  auto slot_of = [&](int r, int hh) { return (long long)(2 * r + (r == c0 ? 1 : 0)) * kMaxSlotHeads + hh; };
+  const int step = heads_split ? 8 : 1;
+  for (int hh = heads_split ? (int)blockIdx.y : warp; hh < heads; hh += heads_split ? heads : 8) {
+    float M = -INFINITY, Lsum = 0.f, v[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = 0.f;
+#pragma unroll 4
+    for (int r = c0 + (heads_split ? warp : 0); r <= c1; r += step) {
+      if (run_start(total, r, G) == run_start(total, r + 1, G)) continue;
+      const long long slot = slot_of(r, hh);
+      const float m = __ldcg(p.part_ml + 2 * slot), l = __ldcg(p.part_ml + 2 * slot + 1);
+      float x[V];
+#pragma unroll
+      for (int k = 0; k < V; ++k) x[k] = __ldcg(p.part_o + slot * D + V * lane + k);
+      const float M1 = fmaxf(M, m);
+      const float f0 = M1 == -INFINITY ? 0.f : exp2_fast(M - M1), f1 = M1 == -INFINITY ? 0.f : exp2_fast(m - M1);
+      M = M1;
+      Lsum = Lsum * f0 + l * f1;
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[k] = v[k] * f0 + x[k] * f1;
+    }
+    if (heads_split) {
+      if (lane == 0) {
+        sm[warp] = M;
+        sl[warp] = Lsum;
+      }
+#pragma unroll
+      for (int k = 0; k < V; ++k) so[warp][V * lane + k] = v[k];
+      __syncthreads();
+      if (warp) return;
+      M = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) M = fmaxf(M, sm[w]);
+      Lsum = 0.f;
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[k] = 0.f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        const float f = sm[w] == -INFINITY ? 0.f : exp2_fast(sm[w] - M);
+        Lsum += sl[w] * f;
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] += so[w][V * lane + k] * f;
+      }
+    }
+    const float inv = Lsum == 0.f ? 0.f : 1.f / Lsum;
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] *= inv;
+    store_vec(reinterpret_cast<T*>(a.out) + (long long)seq * a.out_stride + (long long)(head + hh) * D + V * lane, v, V);
+    if (a.lse && lane == 0)
+      a.lse[(long long)seq * a.n_heads + head + hh] = Lsum == 0.f ? -INFINITY : (M + log2f(Lsum)) * kLn2;
+  }
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
+  static std::once_flag once;
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  std::call_once(once, [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  });
+  return fn;
+}
+
+int sm_count() {
+  static std::mutex mu;
+  static int counts[DeviceSymbolCache::kMaxDevices] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= DeviceSymbolCache::kMaxDevices) return 148;
+  std::lock_guard<std::mutex> lk(mu);
+  if (!counts[dev] && cudaDeviceGetAttribute(&counts[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return 148;
+  return counts[dev];
+}
+
+template <typename T, int D, int NT>
+int launch(const DecodeArgs& p, int G, const CUtensorMap& tmk, const CUtensorMap& tmv, int box_rows,
+           cudaStream_t st) {
+  auto kern = k_paged_decode<T, D, NT>;
+  const int smem = (int)sizeof(DecodeSmem<D>) + 1024;
+  static_assert((sizeof(DecodeSmem<D>) + 2048) * kCtasPerSm <= 228 * 1024, "CTAs per SM");
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -1;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(G);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kern, p, box_rows, tmk, tmv) != cudaSuccess) return -1;
+  // With many partials to a unit (few units), one CTA per head joins them, else one per cut.
+  const long long units = (long long)p.a.kv.n_seq * p.units_per_seq;
+  const int split = G / units > 8 ? 1 : 0;
+  const int group = p.a.n_heads / (int)p.a.kv.n_kv_heads;
+  cfg.gridDim = dim3(G - 1, split ? (group < kMaxSlotHeads ? group : kMaxSlotHeads) : 1);
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = 0;
+  return cudaLaunchKernelEx(&cfg, k_paged_combine<T, D>, p, G, split) == cudaSuccess ? 0 : -1;
+}
+
+int units_per_head(const qwen_paged_kv& kv, int n_heads) {
+  return (n_heads / (int)kv.n_kv_heads + kMaxSlotHeads - 1) / kMaxSlotHeads;
+}
+
+}  // namespace
+
+// Rows = positions of the pool, innermost 64 elements: (element, slot, half, head, page).
+int encode_pages_map(CUtensorMap* map, const qwen_paged_kv& kv, const uint16_t* base, int box_rows) {
+  auto enc = tensor_map_encoder();
+  if (!enc) return -1;
+  const int halves = (int)kv.head_dim / 64;
+  const cuuint64_t dims[5] = {64, kv.page_size, (cuuint64_t)halves, kv.n_kv_heads, kv.n_pages};
+  const cuuint64_t strides[4] = {(cuuint64_t)kv.pos_stride * 2, 128, (cuuint64_t)kv.head_stride * 2,
+                                 (cuuint64_t)kv.page_stride * 2};
+  const cuuint32_t box[5] = {64, (cuuint32_t)box_rows, (cuuint32_t)halves, 1, 1};
+  const cuuint32_t elem[5] = {1, 1, 1, 1, 1};
+  return enc(map, kv.dtype == QWEN_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
+             const_cast<uint16_t*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? 0
+             : -1;
+}
+
+size_t paged_decode_workspace(const qwen_paged_kv& kv) {
+  const size_t slots = (size_t)2 * kCtasPerSm * sm_count() * kMaxSlotHeads;
+  return slots * (kv.head_dim + 2) * sizeof(float);
+}
+
+int launch_paged_decode(const PagedAttnArgs& a, cudaStream_t st) {
+  DecodeArgs p{};
+  p.a = a;
+  p.chunks = units_per_head(a.kv, a.n_heads);
+  p.units_per_seq = (int)a.kv.n_kv_heads * p.chunks;
+  p.list_tiles = (int)(((long long)a.n_list * a.kv.page_size + kTile - 1) / kTile);
+  p.scale_log2 = a.scale * kLog2e;
+  const int G = kCtasPerSm * sm_count();
+  p.part_o = static_cast<float*>(a.workspace);
+  p.part_ml = p.part_o + (size_t)2 * G * kMaxSlotHeads * a.kv.head_dim;
+  // Boxes of 32 positions, or 16 where a page holds no more: a sequence's last
+  // page costs at most 31 positions of traffic that do not count.
+  const int box_rows = a.kv.page_size < 32 ? 16 : 32;
+  CUtensorMap tmk, tmv;
+  if (encode_pages_map(&tmk, a.kv, a.kv.k, box_rows) || encode_pages_map(&tmv, a.kv, a.kv.v, box_rows)) return -1;
+  const bool f16 = a.kv.dtype == QWEN_DTYPE_F16, d64 = a.kv.head_dim == 64;
+  const bool wide = a.n_heads / (int)a.kv.n_kv_heads > 8;
+  if (f16)
+    return d64 ? (wide ? launch<__half, 64, 2> : launch<__half, 64, 1>)(p, G, tmk, tmv, box_rows, st)
+               : (wide ? launch<__half, 128, 2> : launch<__half, 128, 1>)(p, G, tmk, tmv, box_rows, st);
+  return d64 ? (wide ? launch<__nv_bfloat16, 64, 2> : launch<__nv_bfloat16, 64, 1>)(p, G, tmk, tmv, box_rows, st)
+             : (wide ? launch<__nv_bfloat16, 128, 2> : launch<__nv_bfloat16, 128, 1>)(p, G, tmk, tmv, box_rows, st);
+}
+
+}  // namespace qwen
