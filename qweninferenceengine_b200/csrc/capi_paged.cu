@@ -143,8 +143,8 @@ int qwen_rope_append_paged(const qwen_paged_kv* kv, const uint16_t* q, int64_t q
   return launch_status(op);
 }
 
-size_t qwen_attention_paged_workspace(const qwen_paged_kv* kv, uint32_t) {
-  return kv ? paged_decode_workspace(*kv) : 0;
+size_t qwen_attention_paged_workspace(const qwen_paged_kv* kv, uint32_t n_heads) {
+  return kv ? paged_decode_workspace(*kv, (int)n_heads) : 0;
 }
 
 int qwen_attention_paged(const qwen_paged_kv* kv, const uint16_t* q, int64_t q_stride,
@@ -156,8 +156,8 @@ int qwen_attention_paged(const qwen_paged_kv* kv, const uint16_t* q, int64_t q_s
                    workspace, workspace_bytes, qwen_attention_paged_workspace(kv, n_heads), stream);
 }
 
-size_t qwen_attention_prefix_paged_workspace(const qwen_paged_kv* kv, uint32_t, uint32_t) {
-  return kv ? paged_decode_workspace(*kv) : 0;
+size_t qwen_attention_prefix_paged_workspace(const qwen_paged_kv* kv, uint32_t n_heads, uint32_t) {
+  return kv ? paged_decode_workspace(*kv, (int)n_heads) : 0;
 }
 
 int qwen_attention_prefix_paged(const qwen_paged_kv* kv, const uint16_t* q, int64_t q_stride,
@@ -211,8 +211,8 @@ int qwen_select_pages(const qwen_paged_kv* kv, const uint16_t* q, int64_t q_stri
   return launch_status(op);
 }
 
-size_t qwen_attention_sparse_paged_workspace(const qwen_paged_kv* kv, uint32_t, uint32_t) {
-  return kv ? paged_decode_workspace(*kv) : 0;
+size_t qwen_attention_sparse_paged_workspace(const qwen_paged_kv* kv, uint32_t n_heads, uint32_t) {
+  return kv ? paged_decode_workspace(*kv, (int)n_heads) : 0;
 }
 
 int qwen_attention_sparse_paged(const qwen_paged_kv* kv, const int32_t* pages, uint32_t n_select,

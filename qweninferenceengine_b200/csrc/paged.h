@@ -5,6 +5,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/qwen_b200.h"
 
 namespace qwen {
@@ -34,7 +36,27 @@ int launch_paged_attention(const PagedAttnArgs& a, cudaStream_t st);
 // Decode attention over own or listed pages (paged_decode.cu); 0, or -1 for a
 // launch failure.
 int launch_paged_decode(const PagedAttnArgs& a, cudaStream_t st);
-size_t paged_decode_workspace(const qwen_paged_kv& kv);
+size_t paged_decode_workspace(const qwen_paged_kv& kv, int n_heads);
+
+// Host set-up that a kernel needs once per device (dynamic shared memory limits).
+class OncePerDevice {
+ public:
+  bool done() {
+    const int d = device();
+    return d >= 0 && (mask_.load(std::memory_order_acquire) >> d & 1);
+  }
+  void set() {
+    const int d = device();
+    if (d >= 0) mask_.fetch_or(1ull << d, std::memory_order_release);
+  }
+
+ private:
+  static int device() {
+    int d = 0;
+    return cudaGetDevice(&d) == cudaSuccess && d >= 0 && d < 64 ? d : -1;
+  }
+  std::atomic<unsigned long long> mask_{0};
+};
 
 struct PagedAppendArgs {
   qwen_paged_kv kv;

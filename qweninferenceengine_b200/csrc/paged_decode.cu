@@ -11,9 +11,12 @@
 // (two per SM) takes an equal run of them, start(c) = c T / G, wherever units begin
 // and end: a ragged batch, one long sequence and a batch of short ones all divide
 // evenly.  A unit within one CTA is finished there; a unit cut by a run's end
-// leaves fp32 partials (max, sum, unnormalised output), which k_paged_combine
-// joins in CTA order -- results do not depend on timing, and nothing has to be
-// zero beforehand.
+// leaves fp32 partials (max, sum, unnormalised output), which are joined in run
+// order whoever joins them, so results do not depend on timing: the CTA whose piece
+// arrives last joins up to 16 of them; of more, the last of each 16 joins those,
+// and the last of the joined ones the rest (one CTA reading 148 partials of six
+// heads would take as long as streaming 128K positions).  Nothing waits, and a
+// call's arrival counts carry its own tag, so the workspace needs no zeroing.
 //
 // CTA: 4 consumer warps and a producer warp.  Per tile the producer's lanes read
 // list and page table (32 entries at a time), issue one TMA load per box of 16 or
@@ -32,6 +35,8 @@
 // 2^-8, averaged over positions); sums, maxima and outputs are fp32.
 #include <cudaTypedefs.h>
 
+#include <atomic>
+#include <chrono>
 #include <mutex>
 
 #include "paged_common.cuh"
@@ -45,6 +50,7 @@ constexpr int kWarps = kTile / 16;            // consumer warps
 constexpr int kThreads = (kWarps + 1) * 32;
 constexpr int kCtasPerSm = 2;
 constexpr int kMaxSlotHeads = 16;             // query heads of a unit
+constexpr int kJoin = 16;                     // partials joined at once
 
 enum StageFlags { kFirst = 1, kLast = 2, kEnd = 4 };
 
@@ -53,6 +59,10 @@ struct StageMeta {
   int flags;
   int seq, head, heads;   // the unit: sequence, first query head, query heads
   int dest;            // partial slot, or -1: the whole unit, or -2: nothing is written
+  int unit;            // of the launch
+  uint32_t tiles;      // of the unit
+  uint32_t tile;       // first of this piece
+  unsigned long long begin;   // its first tile
 };
 
 template <int D>
@@ -71,6 +81,7 @@ struct __align__(1024) DecodeSmem {
   unsigned long long scan[kWarps + 1];
   unsigned long long found_cum;
   int found_seq;
+  int last;
   int abort;
 };
 
@@ -82,60 +93,14 @@ struct DecodeArgs {
   float scale_log2;
   float* part_o;            // [2 G][16][D]
   float* part_ml;           // [2 G][16][2]
+  unsigned long long* arrived;   // [2 G] by partial slot, then [units]: tag << 16 | arrivals
+  unsigned long long tag;
 };
 
 __device__ __forceinline__ uint32_t seq_tiles(const DecodeArgs& p, uint32_t L) {
   if (p.a.list) return p.list_tiles;
   if (L > p.a.kv.max_pages * p.a.kv.page_size) return 0;
   return L ? (L + kTile - 1) / kTile : 1;   // an empty sequence still has its zeros written
-}
-
-// Total number of tiles, and the sequence that holds tile `at(total)` with the
-// number of tiles per unit before it.  Called by all n threads of a block.
-template <typename At>
-__device__ unsigned long long find_tile(const DecodeArgs& p, unsigned long long* scan,
-                                        unsigned long long* found_cum, int* found_seq, bool report, At at) {
-  const int n = blockDim.x, tid = threadIdx.x, n_seq = p.a.kv.n_seq;
-  if (p.a.list) {
-    const unsigned long long total = (unsigned long long)p.list_tiles * n_seq;
-    if (tid == 0) {
-      *found_seq = (int)(at(total * p.units_per_seq) / ((unsigned long long)p.list_tiles * p.units_per_seq));
-      *found_cum = (unsigned long long)*found_seq * p.list_tiles;
-    }
-    __syncthreads();
-    return total * p.units_per_seq;
-  }
-  const int per = (n_seq + n - 1) / n, s0 = min(n_seq, tid * per), s1 = min(n_seq, s0 + per);
-  unsigned long long sum = 0;
-  for (int s = s0; s < s1; ++s) {
-    const uint32_t t = seq_tiles(p, p.a.seq_len[s]);
-    if (t == 0 && report) raise_error(p.a.err, kDevBadArgument);
-    sum += t;
-  }
-  unsigned long long inc = sum;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const unsigned long long v = __shfl_up_sync(0xffffffffu, inc, o);
-    if ((tid & 31) >= o) inc += v;
-  }
-  if ((tid & 31) == 31) scan[tid >> 5] = inc;
-  if (tid == 0) *found_seq = n_seq;
-  __syncthreads();
-  unsigned long long before = inc - sum, total = 0;
-  for (int w = 0; w < n / 32; ++w) {
-    if (w < (tid >> 5)) before += scan[w];
-    total += scan[w];
-  }
-  total *= p.units_per_seq;
-  const unsigned long long target = at(total), u = p.units_per_seq;
-  if (target >= u * before && target < u * (before + sum)) {
-    int s = s0;
-    for (uint32_t t; target >= u * (before + (t = seq_tiles(p, p.a.seq_len[s]))); ++s) before += t;
-    *found_seq = s;
-    *found_cum = before;
-  }
-  __syncthreads();
-  return total;
 }
 
 __device__ __forceinline__ unsigned long long run_start(unsigned long long total, int c, int G) {
@@ -146,13 +111,137 @@ __device__ __forceinline__ int run_of(unsigned long long total, unsigned long lo
   return (int)(((x + 1) * G - 1) / total);
 }
 
-template <typename T>
-__device__ __forceinline__ void store_vec(T* dst, const float* v, int n) {
-  if (n == 4) {
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(T{}, v[0], v[1]), pack2(T{}, v[2], v[3]));
-  } else {
-    *reinterpret_cast<uint32_t*>(dst) = pack2(T{}, v[0], v[1]);
+// The pieces of a unit of `tiles` tiles from `begin` on: how many runs share it, and
+// the partial slot of piece i.  With fewer tiles than runs each run has one tile
+// or none.
+__device__ __forceinline__ int pieces_of(unsigned long long total, unsigned long long begin, uint32_t tiles, int G) {
+  return total < (unsigned)G ? (int)tiles : run_of(total, begin + tiles - 1, G) - run_of(total, begin, G) + 1;
+}
+__device__ __forceinline__ int piece_slot(unsigned long long total, unsigned long long begin, int i, int G) {
+  const int r = total < (unsigned)G ? run_of(total, begin + i, G) : run_of(total, begin, G) + i;
+  return 2 * r + (i == 0 ? 1 : 0);
+}
+
+// Total number of tiles, and the sequence that holds tile run_start(total, c) with
+// the number of tiles per unit before it.  Called by all threads of a CTA.
+template <int D>
+__device__ unsigned long long find_run(const DecodeArgs& p, DecodeSmem<D>& sm, int c, int G) {
+  const int tid = threadIdx.x, n_seq = p.a.kv.n_seq;
+  const unsigned long long u = p.units_per_seq;
+  if (p.a.list) {
+    const unsigned long long total = u * p.list_tiles * n_seq;
+    if (tid == 0) {
+      sm.found_seq = (int)(run_start(total, c, G) / (u * p.list_tiles));
+      sm.found_cum = (unsigned long long)sm.found_seq * p.list_tiles;
+    }
+    __syncthreads();
+    return total;
   }
+  const int per = (n_seq + kThreads - 1) / kThreads, s0 = min(n_seq, tid * per), s1 = min(n_seq, s0 + per);
+  unsigned long long sum = 0;
+  for (int s = s0; s < s1; ++s) {
+    const uint32_t t = seq_tiles(p, p.a.seq_len[s]);
+    if (t == 0 && c == 0) raise_error(p.a.err, kDevBadArgument);
+    sum += t;
+  }
+  unsigned long long inc = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned long long v = __shfl_up_sync(0xffffffffu, inc, o);
+    if ((tid & 31) >= o) inc += v;
+  }
+  if ((tid & 31) == 31) sm.scan[tid >> 5] = inc;
+  __syncthreads();
+  unsigned long long before = inc - sum, total = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < (tid >> 5)) before += sm.scan[w];
+    total += sm.scan[w];
+  }
+  total *= u;
+  const unsigned long long target = run_start(total, c, G);
+  if (target >= u * before && target < u * (before + sum)) {
+    int s = s0;
+    for (uint32_t t; target >= u * (before + (t = seq_tiles(p, p.a.seq_len[s]))); ++s) before += t;
+    sm.found_seq = s;
+    sm.found_cum = before;
+  }
+  __syncthreads();
+  return total;
+}
+
+// 128 or 64 fp32 values of a row, D / 32 to a lane.
+__device__ __forceinline__ void load_vec(float (&v)[4], const float* p) {
+  const float4 x = __ldcg(reinterpret_cast<const float4*>(p));
+  v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+}
+__device__ __forceinline__ void load_vec(float (&v)[2], const float* p) {
+  const float2 x = __ldcg(reinterpret_cast<const float2*>(p));
+  v[0] = x.x, v[1] = x.y;
+}
+// Output row and log-sum-exp from the unnormalised row v, its maximum and sum.
+template <typename T, int D>
+__device__ __forceinline__ void write_row(const PagedAttnArgs& a, int seq, int head, const float (&v)[D / 32],
+                                          float M, float sum, int lane) {
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  T* dst = reinterpret_cast<T*>(a.out) + (long long)seq * a.out_stride + (long long)head * D + D / 32 * lane;
+  if constexpr (D == 128)
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(T{}, v[0] * inv, v[1] * inv), pack2(T{}, v[2] * inv, v[3] * inv));
+  else
+    *reinterpret_cast<uint32_t*>(dst) = pack2(T{}, v[0] * inv, v[1] * inv);
+  if (a.lse && lane == 0)
+    a.lse[(long long)seq * a.n_heads + head] = sum == 0.f ? -INFINITY : (M + log2f(sum)) * kLn2;
+}
+// Joins n <= 32 partials of head hh of a unit, pieces first, first + step, .. (one
+// warp): into the output row, or into the first one's slot.
+template <typename T, int D>
+__device__ void join_pieces(const DecodeArgs& p, unsigned long long total, const StageMeta& u, int G, int first,
+                            int step, int n, bool final, int hh, int lane) {
+  constexpr int V = D / 32;
+  float m = -INFINITY, l = 0.f;
+  long long slot = 0;
+  if (lane < n) {
+    slot = (long long)piece_slot(total, u.begin, first + lane * step, G) * kMaxSlotHeads + hh;
+    const float2 x = __ldcg(reinterpret_cast<const float2*>(p.part_ml + 2 * slot));
+    m = x.x;
+    l = x.y;
+  }
+  const float M = warp_max(m), f = m == -INFINITY ? 0.f : exp2_fast(m - M);
+  l *= f;
+  float v[V], sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < V; ++k) v[k] = 0.f;
+#pragma unroll 8
+  for (int i = 0; i < n; ++i) {
+    float x[V];
+    load_vec(x, p.part_o + __shfl_sync(0xffffffffu, slot, i) * D + V * lane);
+    const float fi = __shfl_sync(0xffffffffu, f, i);
+    sum += __shfl_sync(0xffffffffu, l, i);
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] += x[k] * fi;
+  }
+  if (final) {
+    write_row<T, D>(p.a, u.seq, u.head + hh, v, M, sum, lane);
+  } else {
+    slot = __shfl_sync(0xffffffffu, slot, 0);
+#pragma unroll
+    for (int k = 0; k < V; ++k) p.part_o[slot * D + V * lane + k] = v[k];
+    if (lane == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * slot) = make_float2(M, sum);
+  }
+}
+// Counts an arrival; true for the last of `expected`, which leaves the count at 0.
+__device__ __forceinline__ bool arrive_last(unsigned long long* count, unsigned long long tag, int expected) {
+  unsigned long long old = *(volatile unsigned long long*)count, now;
+  for (;;) {   // another call's count reads as none
+    now = (old >> 16 == tag ? old : tag << 16) + 1;
+    const unsigned long long seen = atomicCAS(count, old, now);
+    if (seen == old) break;
+    old = seen;
+  }
+  const bool last = (int)(now & 0xffff) == expected;
+  if (last) *(volatile unsigned long long*)count = 0;
+  __threadfence();
+  return last;
 }
 
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
@@ -191,8 +280,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   }
   pdl_wait();
   const int c = blockIdx.x, G = gridDim.x;
-  const unsigned long long total = find_tile(p, s.scan, &s.found_cum, &s.found_seq, c == 0,
-                                             [&](unsigned long long n) { return run_start(n, c, G); });
+  const unsigned long long total = find_run(p, s, c, G);
   const unsigned long long t1 = run_start(total, c + 1, G);
   unsigned long long t = run_start(total, c, G);
   if (t >= t1) return;
@@ -283,6 +371,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
           meta.head = head;
           meta.heads = heads;
           meta.dest = dest;
+          meta.unit = seq * p.units_per_seq + (int)unit;
+          meta.tiles = ts;
+          meta.tile = tile0;
+          meta.begin = p.units_per_seq * cum + (unsigned long long)unit * ts;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive_expect_tx(&s.full[st], 2 * box_bytes * __popc(any));
@@ -507,14 +599,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
 #pragma unroll
             for (int k = 0; k < V; ++k) v[k] += s.o[w][warp][V * lane + k];
           if (meta.dest == -1) {
-            const float inv = Lh == 0.f ? 0.f : 1.f / Lh;
-#pragma unroll
-            for (int k = 0; k < V; ++k) v[k] *= inv;
-            store_vec(reinterpret_cast<T*>(a.out) + (long long)meta.seq * a.out_stride +
-                          (long long)(meta.head + hh) * D + V * lane, v, V);
-            if (a.lse && lane == 0)
-              a.lse[(long long)meta.seq * a.n_heads + meta.head + hh] =
-                  Lh == 0.f ? -INFINITY : (Mh + log2f(Lh)) * kLn2;
+            write_row<T, D>(a, meta.seq, meta.head + hh, v, Mh, Lh, lane);
           } else {
             const long long slot = (long long)meta.dest * kMaxSlotHeads + hh;
 #pragma unroll
@@ -525,91 +610,33 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
             }
           }
         }
+        if (meta.dest >= 0) __threadfence();
         if (!join()) return;   // s.o, s.m and s.l are written again
       }
-  }
-}
+    if (meta.dest < 0) continue;
 
-// Joins the partials of the units that run ends cut: CTA c - 1 takes the unit cut
-// at the end of run c - 1 if that is the unit's first cut.  Warps take the unit's
-// heads (and, with heads_split, blockIdx.y one head each, its warps the partials).
-template <typename T, int D>
-__global__ void __launch_bounds__(256) k_paged_combine(const __grid_constant__ DecodeArgs p, int G,
-                                                       int heads_split) {
-  __shared__ unsigned long long scan[8], found_cum;
-  __shared__ int found_seq;
-  __shared__ float sm[8], sl[8];
-  __shared__ float so[8][D];
-  constexpr int V = D / 32;
-  pdl_wait();
-  const PagedAttnArgs& a = p.a;
-  const int c = blockIdx.x + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const unsigned long long total = find_tile(p, scan, &found_cum, &found_seq, false,
-                                             [&](unsigned long long n) { return run_start(n, c, G); });
-  const unsigned long long cut = run_start(total, c, G);
-  if (cut >= total) return;
-  const int seq = found_seq;
-  const uint32_t L = a.seq_len[seq], ts = seq_tiles(p, L);
-  const unsigned long long rel = cut - p.units_per_seq * found_cum;
-  const uint32_t tile = (uint32_t)(rel % ts);
-  const unsigned long long begin = cut - tile, end = begin + ts;
-  if (tile == 0 || run_start(total, c - 1, G) > begin) return;
-  if (L > a.kv.max_pages * a.kv.page_size) return;
-  const int c0 = run_of(total, begin, G), c1 = run_of(total, end - 1, G);
-  const int unit = (int)(rel / ts), h = unit / p.chunks, chunk = unit % p.chunks;
-  const int group = a.n_heads / (int)a.kv.n_kv_heads;
-  const int head = h * group + chunk * kMaxSlotHeads, heads = min(kMaxSlotHeads, group - chunk * kMaxSlotHeads);
-  // the unit's partials: slot 1 of run c0, slot 0 of the non-empty runs after it
-  auto slot_of = [&](int r, int hh) { return (long long)(2 * r + (r == c0 ? 1 : 0)) * kMaxSlotHeads + hh; };
-  const int step = heads_split ? 8 : 1;
-  for (int hh = heads_split ? (int)blockIdx.y : warp; hh < heads; hh += heads_split ? heads : 8) {
-    float M = -INFINITY, Lsum = 0.f, v[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) v[k] = 0.f;
-#pragma unroll 4
-    for (int r = c0 + (heads_split ? warp : 0); r <= c1; r += step) {
-      if (run_start(total, r, G) == run_start(total, r + 1, G)) continue;
-      const long long slot = slot_of(r, hh);
-      const float m = __ldcg(p.part_ml + 2 * slot), l = __ldcg(p.part_ml + 2 * slot + 1);
-      float x[V];
-#pragma unroll
-      for (int k = 0; k < V; ++k) x[k] = __ldcg(p.part_o + slot * D + V * lane + k);
-      const float M1 = fmaxf(M, m);
-      const float f0 = M1 == -INFINITY ? 0.f : exp2_fast(M - M1), f1 = M1 == -INFINITY ? 0.f : exp2_fast(m - M1);
-      M = M1;
-      Lsum = Lsum * f0 + l * f1;
-#pragma unroll
-      for (int k = 0; k < V; ++k) v[k] = v[k] * f0 + x[k] * f1;
-    }
-    if (heads_split) {
-      if (lane == 0) {
-        sm[warp] = M;
-        sl[warp] = Lsum;
-      }
-#pragma unroll
-      for (int k = 0; k < V; ++k) so[warp][V * lane + k] = v[k];
-      __syncthreads();
-      if (warp) return;
-      M = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < 8; ++w) M = fmaxf(M, sm[w]);
-      Lsum = 0.f;
-#pragma unroll
-      for (int k = 0; k < V; ++k) v[k] = 0.f;
-#pragma unroll
-      for (int w = 0; w < 8; ++w) {
-        const float f = sm[w] == -INFINITY ? 0.f : exp2_fast(sm[w] - M);
-        Lsum += sl[w] * f;
-#pragma unroll
-        for (int k = 0; k < V; ++k) v[k] += so[w][V * lane + k] * f;
+    // ---- the last pieces to arrive join the others'
+    const int n = pieces_of(total, meta.begin, meta.tiles, G);
+    const int mine = total < (unsigned)G ? (int)meta.tile : c - run_of(total, meta.begin, G);
+    const int groups = (n + kJoin - 1) / kJoin, first = mine / kJoin * kJoin, size = min(kJoin, n - first);
+    unsigned long long* unit_count = p.arrived + 2 * G + meta.unit;
+    if (threadIdx.x == 0)
+      s.last = arrive_last(groups == 1 ? unit_count : p.arrived + piece_slot(total, meta.begin, first, G), p.tag, size);
+    if (!join()) return;
+    if (s.last) {
+      for (int hh = warp; hh < meta.heads; hh += kWarps)
+        join_pieces<T, D>(p, total, meta, G, first, 1, size, groups == 1, hh, lane);
+      if (groups > 1) {
+        __threadfence();
+        if (!join()) return;
+        if (threadIdx.x == 0) s.last = arrive_last(unit_count, p.tag, groups);
+        if (!join()) return;
+        if (s.last)
+          for (int hh = warp; hh < meta.heads; hh += kWarps)
+            join_pieces<T, D>(p, total, meta, G, 0, kJoin, groups, true, hh, lane);
       }
     }
-    const float inv = Lsum == 0.f ? 0.f : 1.f / Lsum;
-#pragma unroll
-    for (int k = 0; k < V; ++k) v[k] *= inv;
-    store_vec(reinterpret_cast<T*>(a.out) + (long long)seq * a.out_stride + (long long)(head + hh) * D + V * lane, v, V);
-    if (a.lse && lane == 0)
-      a.lse[(long long)seq * a.n_heads + head + hh] = Lsum == 0.f ? -INFINITY : (M + log2f(Lsum)) * kLn2;
+    if (!join()) return;   // s.last is written again
   }
 }
 
@@ -637,13 +664,24 @@ int sm_count() {
   return counts[dev];
 }
 
+// A tag no other call of this process has, 48 bits, spread so that stale memory
+// does not hold it by chance.
+unsigned long long next_tag() {
+  static std::atomic<uint64_t> calls{splitmix64((uint64_t)std::chrono::steady_clock::now().time_since_epoch().count())};
+  return (splitmix64(calls.fetch_add(1, std::memory_order_relaxed)) >> 16) | 1;
+}
+
 template <typename T, int D, int NT>
 int launch(const DecodeArgs& p, int G, const CUtensorMap& tmk, const CUtensorMap& tmv, int box_rows,
            cudaStream_t st) {
   auto kern = k_paged_decode<T, D, NT>;
   const int smem = (int)sizeof(DecodeSmem<D>) + 1024;
   static_assert((sizeof(DecodeSmem<D>) + 2048) * kCtasPerSm <= 228 * 1024, "CTAs per SM");
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -1;
+  static OncePerDevice once;
+  if (!once.done() &&
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return -1;
+  once.set();
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -654,15 +692,7 @@ int launch(const DecodeArgs& p, int G, const CUtensorMap& tmk, const CUtensorMap
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kern, p, box_rows, tmk, tmv) != cudaSuccess) return -1;
-  // With many partials to a unit (few units), one CTA per head joins them, else one per cut.
-  const long long units = (long long)p.a.kv.n_seq * p.units_per_seq;
-  const int split = G / units > 8 ? 1 : 0;
-  const int group = p.a.n_heads / (int)p.a.kv.n_kv_heads;
-  cfg.gridDim = dim3(G - 1, split ? (group < kMaxSlotHeads ? group : kMaxSlotHeads) : 1);
-  cfg.blockDim = dim3(256);
-  cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, k_paged_combine<T, D>, p, G, split) == cudaSuccess ? 0 : -1;
+  return cudaLaunchKernelEx(&cfg, kern, p, box_rows, tmk, tmv) == cudaSuccess ? 0 : -1;
 }
 
 int units_per_head(const qwen_paged_kv& kv, int n_heads) {
@@ -689,9 +719,10 @@ int encode_pages_map(CUtensorMap* map, const qwen_paged_kv& kv, const uint16_t* 
              : -1;
 }
 
-size_t paged_decode_workspace(const qwen_paged_kv& kv) {
-  const size_t slots = (size_t)2 * kCtasPerSm * sm_count() * kMaxSlotHeads;
-  return slots * (kv.head_dim + 2) * sizeof(float);
+size_t paged_decode_workspace(const qwen_paged_kv& kv, int n_heads) {
+  if (kv.n_kv_heads == 0 || n_heads < (int)kv.n_kv_heads) return 0;   // refused later
+  const size_t G = kCtasPerSm * sm_count(), units = (size_t)kv.n_seq * kv.n_kv_heads * units_per_head(kv, n_heads);
+  return 2 * G * kMaxSlotHeads * (kv.head_dim + 2) * sizeof(float) + (2 * G + units) * sizeof(unsigned long long);
 }
 
 int launch_paged_decode(const PagedAttnArgs& a, cudaStream_t st) {
@@ -704,6 +735,8 @@ int launch_paged_decode(const PagedAttnArgs& a, cudaStream_t st) {
   const int G = kCtasPerSm * sm_count();
   p.part_o = static_cast<float*>(a.workspace);
   p.part_ml = p.part_o + (size_t)2 * G * kMaxSlotHeads * a.kv.head_dim;
+  p.arrived = reinterpret_cast<unsigned long long*>(p.part_ml + (size_t)2 * G * kMaxSlotHeads * 2);
+  p.tag = next_tag();
   // Boxes of 32 positions, or 16 where a page holds no more: a sequence's last
   // page costs at most 31 positions of traffic that do not count.
   const int box_rows = a.kv.page_size < 32 ? 16 : 32;

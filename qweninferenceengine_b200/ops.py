@@ -260,11 +260,12 @@ def _ints(name: str, x: torch.Tensor, kv: PagedKV, n: int | None) -> int:
 def _on(kv: PagedKV, fn, *args) -> None:
     """Calls a library entry on the cache's device and its current stream."""
     index = kv.device.index
+    stream = torch._C._cuda_getCurrentRawStream(index)   # current_stream(index).cuda_stream, 3 us less
     if index == torch.cuda.current_device():
-        check(fn(kv.ref, *args, torch.cuda.current_stream().cuda_stream))
+        check(fn(kv.ref, *args, stream))
     else:
         with torch.cuda.device(index):
-            check(fn(kv.ref, *args, torch.cuda.current_stream().cuda_stream))
+            check(fn(kv.ref, *args, stream))
 
 
 def rope_append_paged(kv: PagedKV, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
