@@ -12,11 +12,12 @@
 // and end: a ragged batch, one long sequence and a batch of short ones all divide
 // evenly.  A unit within one CTA is finished there; a unit cut by a run's end
 // leaves fp32 partials (max, sum, unnormalised output), which are joined in run
-// order whoever joins them, so results do not depend on timing: the CTA whose piece
-// arrives last joins up to 16 of them; of more, the last of each 16 joins those,
-// and the last of the joined ones the rest (one CTA reading 148 partials of six
-// heads would take as long as streaming 128K positions).  Nothing waits, and a
-// call's arrival counts carry its own tag, so the workspace needs no zeroing.
+// order whoever joins them, so results do not depend on timing.  At the end of its
+// run a CTA counts in its pieces (two at most); the last to arrive at a unit joins up
+// to 16 of them; of more, the last of each 16 joins those, and the last of the
+// joined ones the rest (one CTA reading 148 partials of six heads would take as
+// long as streaming 128K positions).  Nothing waits for another CTA, and a call's
+// counts carry its own tag, so the workspace needs no zeroing.
 //
 // CTA: 4 consumer warps and a producer warp.  Per tile the producer's lanes read
 // list and page table (32 entries at a time), issue one TMA load per box of 16 or
@@ -59,10 +60,13 @@ struct StageMeta {
   int flags;
   int seq, head, heads;   // the unit: sequence, first query head, query heads
   int dest;            // partial slot, or -1: the whole unit, or -2: nothing is written
-  int unit;            // of the launch
-  uint32_t tiles;      // of the unit
-  uint32_t tile;       // first of this piece
-  unsigned long long begin;   // its first tile
+};
+
+// A piece that a run leaves of a unit it shares with others.
+struct CutPiece {
+  int seq, head, heads;
+  int unit, pieces, piece, run0;   // number in the launch, pieces, this one, run of the first
+  uint32_t total, begin;           // fewer tiles than runs: their number, the unit's first
 };
 
 template <int D>
@@ -73,15 +77,13 @@ constexpr int stages() {
 template <int D>
 struct __align__(1024) DecodeSmem {
   uint8_t kv[stages<D>()][2][kTile * D * 2];
-  float o[kWarps][4][D + 8];
   uint16_t q[kMaxSlotHeads * D];
-  float m[kWarps][kMaxSlotHeads], l[kWarps][kMaxSlotHeads];
+  float2 ml[2][kWarps][kMaxSlotHeads];   // by piece parity: maximum and sum of each warp
   StageMeta meta[stages<D>()];
   uint64_t full[stages<D>()], empty[stages<D>()], qfull, qempty, joined;
-  unsigned long long scan[kWarps + 1];
-  unsigned long long found_cum;
-  int found_seq;
-  int last;
+  CutPiece cut[2];
+  int n_cut;
+  int last[2];
   int abort;
 };
 
@@ -103,42 +105,39 @@ __device__ __forceinline__ uint32_t seq_tiles(const DecodeArgs& p, uint32_t L) {
   return L ? (L + kTile - 1) / kTile : 1;   // an empty sequence still has its zeros written
 }
 
+// x / d; the 32-bit division where it suffices (a 64-bit one takes ~0.1 us here).
+__device__ __forceinline__ unsigned long long divide(unsigned long long x, unsigned long long d) {
+  return (x | d) >> 32 ? x / d : (uint32_t)x / (uint32_t)d;
+}
 __device__ __forceinline__ unsigned long long run_start(unsigned long long total, int c, int G) {
-  return total * (unsigned)c / (unsigned)G;
+  return divide(total * (unsigned)c, (unsigned)G);
 }
 // The run that holds tile x: the largest c with run_start(c) <= x.
 __device__ __forceinline__ int run_of(unsigned long long total, unsigned long long x, int G) {
-  return (int)(((x + 1) * G - 1) / total);
+  return (int)divide((x + 1) * G - 1, total);
 }
-
-// The pieces of a unit of `tiles` tiles from `begin` on: how many runs share it, and
-// the partial slot of piece i.  With fewer tiles than runs each run has one tile
-// or none.
-__device__ __forceinline__ int pieces_of(unsigned long long total, unsigned long long begin, uint32_t tiles, int G) {
-  return total < (unsigned)G ? (int)tiles : run_of(total, begin + tiles - 1, G) - run_of(total, begin, G) + 1;
-}
-__device__ __forceinline__ int piece_slot(unsigned long long total, unsigned long long begin, int i, int G) {
-  const int r = total < (unsigned)G ? run_of(total, begin + i, G) : run_of(total, begin, G) + i;
+// The partial slot of piece i: runs follow one another, or (fewer tiles than runs)
+// each has one tile or none.
+__device__ __forceinline__ int piece_slot(const CutPiece& u, int i, int G) {
+  const int r = u.total < (unsigned)G ? run_of(u.total, u.begin + i, G) : u.run0 + i;
   return 2 * r + (i == 0 ? 1 : 0);
 }
 
 // Total number of tiles, and the sequence that holds tile run_start(total, c) with
-// the number of tiles per unit before it.  Called by all threads of a CTA.
-template <int D>
-__device__ unsigned long long find_run(const DecodeArgs& p, DecodeSmem<D>& sm, int c, int G) {
-  const int tid = threadIdx.x, n_seq = p.a.kv.n_seq;
+// the number of tiles per unit before it and its length (one warp).
+__device__ unsigned long long find_run(const DecodeArgs& p, int c, int G, int lane, int* seq,
+                                       unsigned long long* cum) {
+  const int n_seq = p.a.kv.n_seq;
   const unsigned long long u = p.units_per_seq;
   if (p.a.list) {
     const unsigned long long total = u * p.list_tiles * n_seq;
-    if (tid == 0) {
-      sm.found_seq = (int)(run_start(total, c, G) / (u * p.list_tiles));
-      sm.found_cum = (unsigned long long)sm.found_seq * p.list_tiles;
-    }
-    __syncthreads();
+    *seq = (int)divide(run_start(total, c, G), u * p.list_tiles);
+    *cum = (unsigned long long)*seq * p.list_tiles;
     return total;
   }
-  const int per = (n_seq + kThreads - 1) / kThreads, s0 = min(n_seq, tid * per), s1 = min(n_seq, s0 + per);
+  const int per = (n_seq + 31) / 32, s0 = min(n_seq, lane * per), s1 = min(n_seq, s0 + per);
   unsigned long long sum = 0;
+#pragma unroll 8
   for (int s = s0; s < s1; ++s) {
     const uint32_t t = seq_tiles(p, p.a.seq_len[s]);
     if (t == 0 && c == 0) raise_error(p.a.err, kDevBadArgument);
@@ -148,25 +147,18 @@ __device__ unsigned long long find_run(const DecodeArgs& p, DecodeSmem<D>& sm, i
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const unsigned long long v = __shfl_up_sync(0xffffffffu, inc, o);
-    if ((tid & 31) >= o) inc += v;
+    if (lane >= o) inc += v;
   }
-  if ((tid & 31) == 31) sm.scan[tid >> 5] = inc;
-  __syncthreads();
-  unsigned long long before = inc - sum, total = 0;
-#pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < (tid >> 5)) before += sm.scan[w];
-    total += sm.scan[w];
-  }
-  total *= u;
+  unsigned long long before = inc - sum;
+  const unsigned long long total = u * __shfl_sync(0xffffffffu, inc, 31);
   const unsigned long long target = run_start(total, c, G);
-  if (target >= u * before && target < u * (before + sum)) {
-    int s = s0;
+  const uint32_t mine = __ballot_sync(0xffffffffu, target >= u * before && target < u * (before + sum));
+  int s = s0;
+  if (mine >> lane & 1)
     for (uint32_t t; target >= u * (before + (t = seq_tiles(p, p.a.seq_len[s]))); ++s) before += t;
-    sm.found_seq = s;
-    sm.found_cum = before;
-  }
-  __syncthreads();
+  const int from = mine ? __ffs(mine) - 1 : 0;   // none: the run is empty
+  *seq = __shfl_sync(0xffffffffu, s, from);
+  *cum = __shfl_sync(0xffffffffu, before, from);
   return total;
 }
 
@@ -192,58 +184,91 @@ __device__ __forceinline__ void write_row(const PagedAttnArgs& a, int seq, int h
   if (a.lse && lane == 0)
     a.lse[(long long)seq * a.n_heads + head] = sum == 0.f ? -INFINITY : (M + log2f(sum)) * kLn2;
 }
-// Joins n <= 32 partials of head hh of a unit, pieces first, first + step, .. (one
-// warp): into the output row, or into the first one's slot.
+// Joins n <= 32 partials of every head of a unit, pieces first, first + step, .. (four
+// warps, two heads of each at a time so that their loads are one round trip): into
+// the output rows, or into the first piece's slot.
 template <typename T, int D>
-__device__ void join_pieces(const DecodeArgs& p, unsigned long long total, const StageMeta& u, int G, int first,
-                            int step, int n, bool final, int hh, int lane) {
-  constexpr int V = D / 32;
-  float m = -INFINITY, l = 0.f;
-  long long slot = 0;
-  if (lane < n) {
-    slot = (long long)piece_slot(total, u.begin, first + lane * step, G) * kMaxSlotHeads + hh;
-    const float2 x = __ldcg(reinterpret_cast<const float2*>(p.part_ml + 2 * slot));
-    m = x.x;
-    l = x.y;
-  }
-  const float M = warp_max(m), f = m == -INFINITY ? 0.f : exp2_fast(m - M);
-  l *= f;
-  float v[V], sum = 0.f;
+__device__ void join_pieces(const DecodeArgs& p, const CutPiece& u, int G, int first, int step, int n, bool final,
+                            int warp, int lane) {
+  constexpr int V = D / 32, HB = 2;
+  const int slot = lane < n ? piece_slot(u, first + lane * step, G) * kMaxSlotHeads : 0;
+  for (int h0 = warp; h0 < u.heads; h0 += HB * kWarps) {
+    float2 ml[HB];
+    float v[HB][V], f[HB], M[HB], sum[HB];
 #pragma unroll
-  for (int k = 0; k < V; ++k) v[k] = 0.f;
-#pragma unroll 8
-  for (int i = 0; i < n; ++i) {
-    float x[V];
-    load_vec(x, p.part_o + __shfl_sync(0xffffffffu, slot, i) * D + V * lane);
-    const float fi = __shfl_sync(0xffffffffu, f, i);
-    sum += __shfl_sync(0xffffffffu, l, i);
+    for (int b = 0; b < HB; ++b) {
+      const int hh = min(h0 + b * kWarps, u.heads - 1);
+      ml[b] = make_float2(-INFINITY, 0.f);
+      if (lane < n) ml[b] = __ldcg(reinterpret_cast<const float2*>(p.part_ml) + slot + hh);
 #pragma unroll
-    for (int k = 0; k < V; ++k) v[k] += x[k] * fi;
-  }
-  if (final) {
-    write_row<T, D>(p.a, u.seq, u.head + hh, v, M, sum, lane);
-  } else {
-    slot = __shfl_sync(0xffffffffu, slot, 0);
+      for (int k = 0; k < V; ++k) v[b][k] = 0.f;
+    }
+    for (int i0 = 0; i0 < n; i0 += 4) {
+      float x[4][HB][V];
 #pragma unroll
-    for (int k = 0; k < V; ++k) p.part_o[slot * D + V * lane + k] = v[k];
-    if (lane == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * slot) = make_float2(M, sum);
+      for (int i = 0; i < 4; ++i) {
+        const long long at = __shfl_sync(0xffffffffu, slot, min(i0 + i, n - 1));
+#pragma unroll
+        for (int b = 0; b < HB; ++b)
+          load_vec(x[i][b], p.part_o + (at + min(h0 + b * kWarps, u.heads - 1)) * D + V * lane);
+      }
+      if (i0 == 0) {
+#pragma unroll
+        for (int b = 0; b < HB; ++b) {
+          M[b] = warp_max(ml[b].x);
+          f[b] = ml[b].x == -INFINITY ? 0.f : exp2_fast(ml[b].x - M[b]);
+          sum[b] = warp_sum(ml[b].y * f[b]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int b = 0; b < HB; ++b) {
+          const float fi = __shfl_sync(0xffffffffu, f[b], (i0 + i) & 31);
+          if (i0 + i < n) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) v[b][k] += x[i][b][k] * fi;
+          }
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < HB; ++b) {
+      const int hh = h0 + b * kWarps;
+      if (hh >= u.heads) continue;
+      if (final) {
+        write_row<T, D>(p.a, u.seq, u.head + hh, v[b], M[b], sum[b], lane);
+      } else {
+        const long long at = __shfl_sync(0xffffffffu, slot, 0) + hh;
+#pragma unroll
+        for (int k = 0; k < V; ++k) p.part_o[at * D + V * lane + k] = v[b][k];
+        if (lane == 0) reinterpret_cast<float2*>(p.part_ml)[at] = make_float2(M[b], sum[b]);
+      }
+    }
   }
+}
+// Makes a count this call's, at 0, unless another CTA did.
+__device__ __forceinline__ void open_count(unsigned long long* count, unsigned long long tag) {
+  const unsigned long long old = *(volatile unsigned long long*)count;
+  if (old >> 16 != tag) atomicCAS(count, old, tag << 16);
 }
 // Counts an arrival; true for the last of `expected`, which leaves the count at 0.
 __device__ __forceinline__ bool arrive_last(unsigned long long* count, unsigned long long tag, int expected) {
-  unsigned long long old = *(volatile unsigned long long*)count, now;
-  for (;;) {   // another call's count reads as none
-    now = (old >> 16 == tag ? old : tag << 16) + 1;
-    const unsigned long long seen = atomicCAS(count, old, now);
-    if (seen == old) break;
-    old = seen;
+  __threadfence();
+  unsigned long long now = atomicAdd(count, 1ull) + 1;
+  while (now >> 16 != tag) {   // not opened yet: what was there is another call's
+    const unsigned long long seen = atomicCAS(count, now, tag << 16 | 1);
+    if (seen == now) now = tag << 16 | 1;
+    else now = seen >> 16 == tag ? atomicAdd(count, 1ull) + 1 : seen;
   }
   const bool last = (int)(now & 0xffff) == expected;
-  if (last) *(volatile unsigned long long*)count = 0;
+  if (last) *(volatile unsigned long long*)count = tag << 16;
   __threadfence();
   return last;
 }
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
   uint32_t y;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -276,14 +301,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     mbar_init(&s.joined, kWarps);
     s.abort = 0;
     fence_mbar_init();
+    prefetch_map(&tmk);
+    prefetch_map(&tmv);
     pdl_launch_dependents();
   }
+  __syncthreads();
   pdl_wait();
   const int c = blockIdx.x, G = gridDim.x;
-  const unsigned long long total = find_run(p, s, c, G);
-  const unsigned long long t1 = run_start(total, c + 1, G);
-  unsigned long long t = run_start(total, c, G);
-  if (t >= t1) return;
 
   if (warp == kWarps) {
     // ------------------------------------------------------------ producer --
@@ -292,9 +316,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     const uint32_t box_bytes = (uint32_t)box_rows * D * 2;
     const uint32_t capacity = a.kv.max_pages * a.kv.page_size;
     uint32_t it = 0, pieces = 0;
-    int seq = s.found_seq;
-    unsigned long long cum = s.found_cum;
-    uint32_t L = a.seq_len[seq], ts = seq_tiles(p, L);
+    int seq, n_cut = 0;
+    unsigned long long cum;
+    const unsigned long long total = find_run(p, c, G, lane, &seq, &cum);
+    const unsigned long long t1 = run_start(total, c + 1, G);
+    unsigned long long t = run_start(total, c, G);
+    uint32_t L = t < t1 ? a.seq_len[seq] : 0, ts = t < t1 ? seq_tiles(p, L) : 0;
     int cached_unit = -1, cached_base = 0, col = -1, page = -1;   // lane i: list / table entry cached_base + i
     bool alive = true;
     while (t < t1 && alive) {
@@ -304,7 +331,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         ts = seq_tiles(p, L);
       }
       const unsigned long long rel = t - p.units_per_seq * cum;
-      const uint32_t unit = (uint32_t)(rel / ts), tile0 = (uint32_t)(rel % ts);
+      const uint32_t unit = (uint32_t)divide(rel, ts), tile0 = (uint32_t)(rel - (unsigned long long)unit * ts);
+      const unsigned long long begin = t - tile0;
       const uint32_t tile1 = (uint32_t)min((unsigned long long)ts, tile0 + (t1 - t));
       t += tile1 - tile0;
       const int h = (int)unit / p.chunks, chunk = (int)unit % p.chunks;
@@ -320,6 +348,21 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         bulk_g2s(s.q, a.q + (long long)seq * a.q_stride + (long long)head * D, (uint32_t)heads * D * 2, &s.qfull);
       }
       ++pieces;
+      if (dest >= 0) {
+        const int run0 = run_of(total, begin, G), unit_no = seq * p.units_per_seq + (int)unit;
+        CutPiece u;
+        u.seq = seq;
+        u.head = head;
+        u.heads = heads;
+        u.unit = unit_no;
+        u.pieces = total < (unsigned)G ? (int)ts : run_of(total, begin + ts - 1, G) - run0 + 1;
+        u.piece = total < (unsigned)G ? (int)tile0 : c - run0;
+        u.run0 = run0;
+        u.total = (uint32_t)min(total, (unsigned long long)G);
+        u.begin = (uint32_t)begin;
+        if (lane == 0) s.cut[n_cut] = u;
+        ++n_cut;
+      }
       const int32_t* table = a.kv.page_table + (long long)seq * a.kv.table_stride;
       const int32_t* list = a.list ? a.list + ((long long)seq * a.kv.n_kv_heads + h) * a.n_list : nullptr;
       const int n_entries = a.list ? a.n_list : (int)((L + P - 1) >> a.page_shift);
@@ -371,10 +414,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
           meta.head = head;
           meta.heads = heads;
           meta.dest = dest;
-          meta.unit = seq * p.units_per_seq + (int)unit;
-          meta.tiles = ts;
-          meta.tile = tile0;
-          meta.begin = p.units_per_seq * cum + (unsigned long long)unit * ts;
         }
         __syncwarp();
         if (lane == 0) mbar_arrive_expect_tx(&s.full[st], 2 * box_bytes * __popc(any));
@@ -386,6 +425,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         ++it;
       }
     }
+    if (lane < n_cut) {   // counts of the units it shares, opened while the last tiles are on their way
+      const CutPiece& u = s.cut[lane];
+      open_count(p.arrived + 2 * G + u.unit, p.tag);
+      if (u.pieces > kJoin) open_count(p.arrived + piece_slot(u, u.piece / kJoin * kJoin, G), p.tag);
+    }
     uint32_t drained = it >= (uint32_t)ST ? it - ST : 0;
     if (alive) {   // the end of the run, in a stage whose last copy was consumed
       const int st = it % ST;
@@ -393,6 +437,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       if (alive) {
         if (it >= ST) ++drained;
         if (lane == 0) {
+          s.n_cut = n_cut;
           s.meta[st].flags = kEnd;
           mbar_arrive(&s.full[st]);
         }
@@ -422,9 +467,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   for (uint32_t it = 0;; ++it) {
     const int st = it % ST;
     if (!__all_sync(0xffffffffu, paged_wait(&s.full[st], (it / ST) & 1, &s.abort, a.err))) return;
-    const StageMeta meta = s.meta[st];
-    if (meta.flags & kEnd) return;
-    if (meta.flags & kFirst) {
+    const StageMeta& meta = s.meta[st];
+    const int flags = meta.flags, valid = meta.valid[warp];
+    if (flags & kEnd) break;
+    if (flags & kFirst) {
       if (!__all_sync(0xffffffffu, paged_wait(&s.qfull, pieces & 1, &s.abort, a.err))) return;
       ++pieces;
 #pragma unroll
@@ -450,7 +496,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         for (int i = 0; i < D / 16; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
       }
     }
-    const int valid = warp == 0 ? meta.valid[0] : warp == 1 ? meta.valid[1] : warp == 2 ? meta.valid[2] : meta.valid[3];
     if (valid > 0) {
       const uint8_t* kb = s.kv[st][0] + box_off;
       const uint8_t* vb = s.kv[st][1] + box_off;
@@ -547,11 +592,17 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         }
       }
     }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&s.empty[st]);
-    if (!(meta.flags & kLast)) continue;
+    if (!(flags & kLast)) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.empty[st]);
+      continue;
+    }
 
-    // ---- join the warps: o[n][i][e]: (d 16i+g, head 8n+2t+e), [2+e]: (d 16i+g+8, ..)
+    // ---- the end of a piece.  Join the warps: o[n][i][e]: (d 16i+g, head 8n+2t+e),
+    // [2+e]: (d 16i+g+8, ..).  The piece's last stage, which every warp is done with
+    // after the first join, holds their rows: [warp][head][d ^ 8 (head / 2 % 4)].
+    const StageMeta u = meta;
+    float2(*ml)[kMaxSlotHeads] = s.ml[(pieces - 1) & 1];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -560,83 +611,78 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         x += __shfl_xor_sync(0xffffffffu, x, 4);
         x += __shfl_xor_sync(0xffffffffu, x, 8);
         x += __shfl_xor_sync(0xffffffffu, x, 16);
-        if (g == 0) {
-          s.m[warp][8 * n + 2 * t4 + e] = m[n][e];
-          s.l[warp][8 * n + 2 * t4 + e] = x;
-        }
+        if (g == 0) ml[warp][8 * n + 2 * t4 + e] = make_float2(m[n][e], x);
       }
     if (!join()) return;
+    float* rows = reinterpret_cast<float*>(s.kv[st][0]);
+    static_assert(kWarps * 8 * NT * D * 4 <= 2 * kTile * D * 2, "the warps' rows exceed a stage");
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        // a pass: heads 8n + 2t + e, t = 0..3; lane's share of the output: head t = warp
-        const int mine = 8 * n + 2 * t4 + e;
+        const int head = 8 * n + 2 * t4 + e;
         float M = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s.m[w][mine]);
+        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, ml[w][head].x);
         const float f = m[n][e] == -INFINITY ? 0.f : exp2_fast(m[n][e] - M);
+        float* row = rows + (warp * 8 * NT + head) * D;
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
-          s.o[warp][t4][16 * i + g] = o[n][i][e] * f;
-          s.o[warp][t4][16 * i + g + 8] = o[n][i][2 + e] * f;
+          row[(16 * i + g) ^ (8 * t4)] = o[n][i][e] * f;
+          row[(16 * i + g + 8) ^ (8 * t4)] = o[n][i][2 + e] * f;
         }
-        if (!join()) return;
-        const int hh = 8 * n + 2 * warp + e;
-        if (hh < meta.heads && meta.dest != -2) {
-          float Mh = -INFINITY, Lh = 0.f;
-#pragma unroll
-          for (int w = 0; w < kWarps; ++w) Mh = fmaxf(Mh, s.m[w][hh]);
-#pragma unroll
-          for (int w = 0; w < kWarps; ++w)
-            Lh += s.m[w][hh] == -INFINITY ? 0.f : s.l[w][hh] * exp2_fast(s.m[w][hh] - Mh);
-          constexpr int V = D / 32;   // elements of this lane
-          float v[V];
-#pragma unroll
-          for (int k = 0; k < V; ++k) v[k] = 0.f;
-#pragma unroll
-          for (int w = 0; w < kWarps; ++w)
-#pragma unroll
-            for (int k = 0; k < V; ++k) v[k] += s.o[w][warp][V * lane + k];
-          if (meta.dest == -1) {
-            write_row<T, D>(a, meta.seq, meta.head + hh, v, Mh, Lh, lane);
-          } else {
-            const long long slot = (long long)meta.dest * kMaxSlotHeads + hh;
-#pragma unroll
-            for (int k = 0; k < V; ++k) p.part_o[slot * D + V * lane + k] = v[k];
-            if (lane == 0) {
-              p.part_ml[2 * slot] = Mh;
-              p.part_ml[2 * slot + 1] = Lh;
-            }
-          }
-        }
-        if (meta.dest >= 0) __threadfence();
-        if (!join()) return;   // s.o, s.m and s.l are written again
       }
-    if (meta.dest < 0) continue;
-
-    // ---- the last pieces to arrive join the others'
-    const int n = pieces_of(total, meta.begin, meta.tiles, G);
-    const int mine = total < (unsigned)G ? (int)meta.tile : c - run_of(total, meta.begin, G);
-    const int groups = (n + kJoin - 1) / kJoin, first = mine / kJoin * kJoin, size = min(kJoin, n - first);
-    unsigned long long* unit_count = p.arrived + 2 * G + meta.unit;
-    if (threadIdx.x == 0)
-      s.last = arrive_last(groups == 1 ? unit_count : p.arrived + piece_slot(total, meta.begin, first, G), p.tag, size);
     if (!join()) return;
-    if (s.last) {
-      for (int hh = warp; hh < meta.heads; hh += kWarps)
-        join_pieces<T, D>(p, total, meta, G, first, 1, size, groups == 1, hh, lane);
-      if (groups > 1) {
-        __threadfence();
-        if (!join()) return;
-        if (threadIdx.x == 0) s.last = arrive_last(unit_count, p.tag, groups);
-        if (!join()) return;
-        if (s.last)
-          for (int hh = warp; hh < meta.heads; hh += kWarps)
-            join_pieces<T, D>(p, total, meta, G, 0, kJoin, groups, true, hh, lane);
+    for (int head = warp; head < u.heads && u.dest != -2; head += kWarps) {
+      constexpr int V = D / 32;   // elements of this lane
+      float M = -INFINITY, sum = 0.f, v[V];
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) M = fmaxf(M, ml[w][head].x);
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[k] = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        sum += ml[w][head].x == -INFINITY ? 0.f : ml[w][head].y * exp2_fast(ml[w][head].x - M);
+        const float* row = rows + (w * 8 * NT + head) * D + ((V * lane) ^ (8 * (head / 2 % 4)));
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] += row[k];
+      }
+      if (u.dest == -1) {
+        write_row<T, D>(a, u.seq, u.head + head, v, M, sum, lane);
+      } else {
+        const long long slot = (long long)u.dest * kMaxSlotHeads + head;
+#pragma unroll
+        for (int k = 0; k < V; ++k) p.part_o[slot * D + V * lane + k] = v[k];
+        if (lane == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * slot) = make_float2(M, sum);
       }
     }
-    if (!join()) return;   // s.last is written again
+    fence_proxy_async();   // the rows before the next TMA write
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&s.empty[st]);
+  }
+
+  // ---- the last pieces to arrive join the others'
+  const int n_cut = s.n_cut;
+  if (n_cut == 0) return;
+  if (!join()) return;   // every warp's partials are written
+  if (threadIdx.x < n_cut) {
+    const CutPiece& u = s.cut[threadIdx.x];
+    const int first = u.piece / kJoin * kJoin;
+    s.last[threadIdx.x] = arrive_last(
+        u.pieces <= kJoin ? p.arrived + 2 * G + u.unit : p.arrived + piece_slot(u, first, G), p.tag,
+        min(kJoin, u.pieces - first));
+  }
+  if (!join()) return;
+  for (int k = 0; k < n_cut; ++k) {
+    if (!s.last[k]) continue;
+    const CutPiece& u = s.cut[k];
+    const int groups = (u.pieces + kJoin - 1) / kJoin, first = u.piece / kJoin * kJoin;
+    join_pieces<T, D>(p, u, G, first, 1, min(kJoin, u.pieces - first), groups == 1, warp, lane);
+    if (groups == 1) continue;
+    if (!join()) return;
+    if (threadIdx.x == 0) s.last[k] = arrive_last(p.arrived + 2 * G + u.unit, p.tag, groups);
+    if (!join()) return;
+    if (s.last[k]) join_pieces<T, D>(p, u, G, 0, kJoin, groups, true, warp, lane);
   }
 }
 
