@@ -89,8 +89,8 @@ int attention(const char* op, PagedAttnArgs& a, const qwen_paged_kv* kv, const u
   a.scale = scale;
   a.workspace = workspace;
   QWEN_TRY(ops_status_word(&a.err));
-  const int rc = a.prefix_pages ? launch_paged_attention(a, static_cast<cudaStream_t>(stream))
-                                : launch_paged_decode(a, static_cast<cudaStream_t>(stream));
+  const int rc = a.prefix_len ? launch_paged_prefix(a, static_cast<cudaStream_t>(stream))
+                              : launch_paged_decode(a, static_cast<cudaStream_t>(stream));
   QWEN_TRY(launch_status(op));
   return rc == 0 ? QWEN_OK : set_error(QWEN_ERR_CUDA, "%s: launch failed", op);
 }
@@ -156,8 +156,8 @@ int qwen_attention_paged(const qwen_paged_kv* kv, const uint16_t* q, int64_t q_s
                    workspace, workspace_bytes, qwen_attention_paged_workspace(kv, n_heads), stream);
 }
 
-size_t qwen_attention_prefix_paged_workspace(const qwen_paged_kv* kv, uint32_t n_heads, uint32_t) {
-  return kv ? paged_decode_workspace(*kv, (int)n_heads) : 0;
+size_t qwen_attention_prefix_paged_workspace(const qwen_paged_kv* kv, uint32_t n_heads, uint32_t prefix_len) {
+  return kv ? paged_prefix_workspace(*kv, (int)n_heads, prefix_len) : 0;
 }
 
 int qwen_attention_prefix_paged(const qwen_paged_kv* kv, const uint16_t* q, int64_t q_stride,

@@ -1,6 +1,7 @@
 // paged.h -- operators over a paged key/value cache (qwen_paged_kv of
 // include/qwen_b200.h): parameters the entry points hand to the launchers.
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stddef.h>
 #include <stdint.h>
@@ -32,11 +33,18 @@ struct PagedAttnArgs {
   void* workspace;
   int* err;                     // operator status word
 };
-int launch_paged_attention(const PagedAttnArgs& a, cudaStream_t st);
 // Decode attention over own or listed pages (paged_decode.cu); 0, or -1 for a
-// launch failure.
-int launch_paged_decode(const PagedAttnArgs& a, cudaStream_t st);
+// launch failure.  own_o, own_ml: where set, unnormalised rows and (max, sum) per
+// query head go there instead of outputs.
+int launch_paged_decode(const PagedAttnArgs& a, cudaStream_t st, float* own_o = nullptr, float2* own_ml = nullptr);
 size_t paged_decode_workspace(const qwen_paged_kv& kv, int n_heads);
+// The same over a shared prefix (prefix_len > 0) and own pages (paged_prefix.cu).
+int launch_paged_prefix(const PagedAttnArgs& a, cudaStream_t st);
+size_t paged_prefix_workspace(const qwen_paged_kv& kv, int n_heads, uint32_t prefix_len);
+int paged_sm_count();
+// Tensor map of a pool, (element of 64, slot, half, head, page), boxes of box_rows
+// slots and box_halves halves; 0 or -1.
+int encode_pages_map(CUtensorMap* map, const qwen_paged_kv& kv, const uint16_t* base, int box_rows, int box_halves);
 
 // Host set-up that a kernel needs once per device (dynamic shared memory limits).
 class OncePerDevice {

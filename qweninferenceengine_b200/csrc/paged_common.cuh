@@ -88,6 +88,39 @@ __device__ __forceinline__ void tma_load_pages(void* dst, const CUtensorMap* map
       : "memory");
 }
 
+// One half (64 elements) of the same, box (64, rows, 1, 1, 1).
+__device__ __forceinline__ void tma_load_half(void* dst, const CUtensorMap* map, int slot, int half, int head,
+                                              int page, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
+      "[%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(slot), "r"(half), "r"(head), "r"(page),
+      "r"(smem_u32(bar))
+      : "memory");
+}
+
+// 128 or 64 fp32 values of a row, D / 32 to a lane.
+__device__ __forceinline__ void load_vec(float (&v)[4], const float* p) {
+  const float4 x = __ldcg(reinterpret_cast<const float4*>(p));
+  v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+}
+__device__ __forceinline__ void load_vec(float (&v)[2], const float* p) {
+  const float2 x = __ldcg(reinterpret_cast<const float2*>(p));
+  v[0] = x.x, v[1] = x.y;
+}
+// Output row and log-sum-exp from the unnormalised row v, its maximum and sum.
+template <typename T, int D>
+__device__ __forceinline__ void write_row(const PagedAttnArgs& a, int seq, int head, const float (&v)[D / 32],
+                                          float M, float sum, int lane) {
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  T* dst = reinterpret_cast<T*>(a.out) + (long long)seq * a.out_stride + (long long)head * D + D / 32 * lane;
+  if constexpr (D == 128)
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(T{}, v[0] * inv, v[1] * inv), pack2(T{}, v[2] * inv, v[3] * inv));
+  else
+    *reinterpret_cast<uint32_t*>(dst) = pack2(T{}, v[0] * inv, v[1] * inv);
+  if (a.lse && lane == 0)
+    a.lse[(long long)seq * a.n_heads + head] = sum == 0.f ? -INFINITY : (M + log2f(sum)) * kLn2;
+}
 // Positions of sequence s, or 0 with the status word set when the length does
 // not fit its row of the page table (*ok false).
 __device__ __forceinline__ uint32_t checked_len(const qwen_paged_kv& kv, const uint32_t* seq_len,

@@ -97,6 +97,8 @@ struct DecodeArgs {
   float* part_ml;           // [2 G][16][2]
   unsigned long long* arrived;   // [2 G] by partial slot, then [units]: tag << 16 | arrivals
   unsigned long long tag;
+  float* own_o;             // if set: unnormalised rows [n_seq][n_heads][D] and their (max,
+  float2* own_ml;           //   sum) go here instead of outputs, for the shared-prefix join
 };
 
 __device__ __forceinline__ uint32_t seq_tiles(const DecodeArgs& p, uint32_t L) {
@@ -162,27 +164,19 @@ __device__ unsigned long long find_run(const DecodeArgs& p, int c, int G, int la
   return total;
 }
 
-// 128 or 64 fp32 values of a row, D / 32 to a lane.
-__device__ __forceinline__ void load_vec(float (&v)[4], const float* p) {
-  const float4 x = __ldcg(reinterpret_cast<const float4*>(p));
-  v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
-}
-__device__ __forceinline__ void load_vec(float (&v)[2], const float* p) {
-  const float2 x = __ldcg(reinterpret_cast<const float2*>(p));
-  v[0] = x.x, v[1] = x.y;
-}
-// Output row and log-sum-exp from the unnormalised row v, its maximum and sum.
+// A finished row: output and log-sum-exp, or for the shared-prefix join what they
+// are made of.
 template <typename T, int D>
-__device__ __forceinline__ void write_row(const PagedAttnArgs& a, int seq, int head, const float (&v)[D / 32],
-                                          float M, float sum, int lane) {
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  T* dst = reinterpret_cast<T*>(a.out) + (long long)seq * a.out_stride + (long long)head * D + D / 32 * lane;
-  if constexpr (D == 128)
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(T{}, v[0] * inv, v[1] * inv), pack2(T{}, v[2] * inv, v[3] * inv));
-  else
-    *reinterpret_cast<uint32_t*>(dst) = pack2(T{}, v[0] * inv, v[1] * inv);
-  if (a.lse && lane == 0)
-    a.lse[(long long)seq * a.n_heads + head] = sum == 0.f ? -INFINITY : (M + log2f(sum)) * kLn2;
+__device__ __forceinline__ void finish_row(const DecodeArgs& p, int seq, int head, const float (&v)[D / 32], float M,
+                                           float sum, int lane) {
+  if (!p.own_o) {
+    write_row<T, D>(p.a, seq, head, v, M, sum, lane);
+    return;
+  }
+  const long long row = (long long)seq * p.a.n_heads + head;
+#pragma unroll
+  for (int k = 0; k < D / 32; ++k) p.own_o[row * D + D / 32 * lane + k] = v[k];
+  if (lane == 0) p.own_ml[row] = make_float2(M, sum);
 }
 // Joins n <= 32 partials of every head of a unit, pieces first, first + step, .. (four
 // warps, two heads of each at a time so that their loads are one round trip): into
@@ -236,7 +230,7 @@ __device__ void join_pieces(const DecodeArgs& p, const CutPiece& u, int G, int f
       const int hh = h0 + b * kWarps;
       if (hh >= u.heads) continue;
       if (final) {
-        write_row<T, D>(p.a, u.seq, u.head + hh, v[b], M[b], sum[b], lane);
+        finish_row<T, D>(p, u.seq, u.head + hh, v[b], M[b], sum[b], lane);
       } else {
         const long long at = __shfl_sync(0xffffffffu, slot, 0) + hh;
 #pragma unroll
@@ -303,10 +297,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     fence_mbar_init();
     prefetch_map(&tmk);
     prefetch_map(&tmv);
-    pdl_launch_dependents();
   }
   __syncthreads();
   pdl_wait();
+  // After the wait: a dependent that starts before this kernel ends (k_prefix, which
+  // reads nothing of it) finds everything that came before.
+  if (threadIdx.x == 0) pdl_launch_dependents();
   const int c = blockIdx.x, G = gridDim.x;
 
   if (warp == kWarps) {
@@ -648,7 +644,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         for (int k = 0; k < V; ++k) v[k] += row[k];
       }
       if (u.dest == -1) {
-        write_row<T, D>(a, u.seq, u.head + head, v, M, sum, lane);
+        finish_row<T, D>(p, u.seq, u.head + head, v, M, sum, lane);
       } else {
         const long long slot = (long long)u.dest * kMaxSlotHeads + head;
 #pragma unroll
@@ -699,17 +695,6 @@ PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
   return fn;
 }
 
-int sm_count() {
-  static std::mutex mu;
-  static int counts[DeviceSymbolCache::kMaxDevices] = {};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= DeviceSymbolCache::kMaxDevices) return 148;
-  std::lock_guard<std::mutex> lk(mu);
-  if (!counts[dev] && cudaDeviceGetAttribute(&counts[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return 148;
-  return counts[dev];
-}
-
 // A tag no other call of this process has, 48 bits, spread so that stale memory
 // does not hold it by chance.
 unsigned long long next_tag() {
@@ -747,15 +732,26 @@ int units_per_head(const qwen_paged_kv& kv, int n_heads) {
 
 }  // namespace
 
+int paged_sm_count() {
+  static std::mutex mu;
+  static int counts[DeviceSymbolCache::kMaxDevices] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= DeviceSymbolCache::kMaxDevices) return 148;
+  std::lock_guard<std::mutex> lk(mu);
+  if (!counts[dev] && cudaDeviceGetAttribute(&counts[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return 148;
+  return counts[dev];
+}
+
 // Rows = positions of the pool, innermost 64 elements: (element, slot, half, head, page).
-int encode_pages_map(CUtensorMap* map, const qwen_paged_kv& kv, const uint16_t* base, int box_rows) {
+int encode_pages_map(CUtensorMap* map, const qwen_paged_kv& kv, const uint16_t* base, int box_rows, int box_halves) {
   auto enc = tensor_map_encoder();
   if (!enc) return -1;
   const int halves = (int)kv.head_dim / 64;
   const cuuint64_t dims[5] = {64, kv.page_size, (cuuint64_t)halves, kv.n_kv_heads, kv.n_pages};
   const cuuint64_t strides[4] = {(cuuint64_t)kv.pos_stride * 2, 128, (cuuint64_t)kv.head_stride * 2,
                                  (cuuint64_t)kv.page_stride * 2};
-  const cuuint32_t box[5] = {64, (cuuint32_t)box_rows, (cuuint32_t)halves, 1, 1};
+  const cuuint32_t box[5] = {64, (cuuint32_t)box_rows, (cuuint32_t)box_halves, 1, 1};
   const cuuint32_t elem[5] = {1, 1, 1, 1, 1};
   return enc(map, kv.dtype == QWEN_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
              const_cast<uint16_t*>(base), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -767,27 +763,31 @@ int encode_pages_map(CUtensorMap* map, const qwen_paged_kv& kv, const uint16_t* 
 
 size_t paged_decode_workspace(const qwen_paged_kv& kv, int n_heads) {
   if (kv.n_kv_heads == 0 || n_heads < (int)kv.n_kv_heads) return 0;   // refused later
-  const size_t G = kCtasPerSm * sm_count(), units = (size_t)kv.n_seq * kv.n_kv_heads * units_per_head(kv, n_heads);
+  const size_t G = kCtasPerSm * paged_sm_count(), units = (size_t)kv.n_seq * kv.n_kv_heads * units_per_head(kv, n_heads);
   return 2 * G * kMaxSlotHeads * (kv.head_dim + 2) * sizeof(float) + (2 * G + units) * sizeof(unsigned long long);
 }
 
-int launch_paged_decode(const PagedAttnArgs& a, cudaStream_t st) {
+int launch_paged_decode(const PagedAttnArgs& a, cudaStream_t st, float* own_o, float2* own_ml) {
   DecodeArgs p{};
   p.a = a;
   p.chunks = units_per_head(a.kv, a.n_heads);
   p.units_per_seq = (int)a.kv.n_kv_heads * p.chunks;
   p.list_tiles = (int)(((long long)a.n_list * a.kv.page_size + kTile - 1) / kTile);
   p.scale_log2 = a.scale * kLog2e;
-  const int G = kCtasPerSm * sm_count();
+  const int G = kCtasPerSm * paged_sm_count();
   p.part_o = static_cast<float*>(a.workspace);
   p.part_ml = p.part_o + (size_t)2 * G * kMaxSlotHeads * a.kv.head_dim;
   p.arrived = reinterpret_cast<unsigned long long*>(p.part_ml + (size_t)2 * G * kMaxSlotHeads * 2);
   p.tag = next_tag();
+  p.own_o = own_o;
+  p.own_ml = own_ml;
   // Boxes of 32 positions, or 16 where a page holds no more: a sequence's last
   // page costs at most 31 positions of traffic that do not count.
   const int box_rows = a.kv.page_size < 32 ? 16 : 32;
   CUtensorMap tmk, tmv;
-  if (encode_pages_map(&tmk, a.kv, a.kv.k, box_rows) || encode_pages_map(&tmv, a.kv, a.kv.v, box_rows)) return -1;
+  const int halves = (int)a.kv.head_dim / 64;
+  if (encode_pages_map(&tmk, a.kv, a.kv.k, box_rows, halves) || encode_pages_map(&tmv, a.kv, a.kv.v, box_rows, halves))
+    return -1;
   const bool f16 = a.kv.dtype == QWEN_DTYPE_F16, d64 = a.kv.head_dim == 64;
   const bool wide = a.n_heads / (int)a.kv.n_kv_heads > 8;
   if (f16)

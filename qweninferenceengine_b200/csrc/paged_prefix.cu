@@ -1,0 +1,633 @@
+// paged_prefix.cu -- decode attention of a batch over a prefix that all its
+// sequences share, held once in the pool, and the join with their own positions.
+//
+// For one kv head the batch's queries are a matrix of n_seq x group rows against
+// the same keys, so the prefix is read once and its products fill the tensor
+// cores: 4 rows D L flops against 4 D L bytes -- from ~250 rows on it is bound by
+// tcgen05 (and by the exponentials: 128 x 128 of them take the SFUs as long as the
+// two MMAs of a tile take), below that by HBM.
+//
+// Three launches, each a programmatic dependent of the one before:
+//   k_paged_decode (paged_decode.cu)  every sequence's own positions; it leaves
+//       (max, sum, unnormalised row) per query head instead of outputs
+//   k_prefix        below; starts while the former's last CTAs still run
+//   k_prefix_join   per query head: own part and the prefix's partials, in a fixed
+//       order, into out and lse
+//
+// k_prefix: a unit is a kv head and 256 rows (two tiles of M = 128; an odd last
+// tile stands alone), its steps the prefix's 128-position tiles.  All units'
+// steps stand in one row weighted by their MMAs, and one CTA per SM takes an equal
+// run of it.  Warps of a CTA:
+//   0-3, 4-7  softmax of stream 0 and 1 (thread = row): S from tensor memory, the
+//       weights back over it as fp16 / bf16 (P)
+//   8  producer: page table, TMA loads of K and V tiles into a 5-slot ring
+//   9  MMA issue: S = Q K^T (smem x smem), O += P V (tensor memory x smem, V read
+//       N-major as it lies in the pool)
+// The two streams are the unit's two row tiles over the same K / V slots; a lone
+// row tile runs alternate position tiles in each stream instead.  While one
+// stream's softmax runs, the tensor core works for the other.  O stays in tensor
+// memory; it is rescaled by its row's thread only when a score passes the row's
+// reference by 2^15 (weights are 2^(s - r) with r = max - 7 when last moved, see
+// paged_decode.cu).
+#include <cudaTypedefs.h>
+
+#include "paged_common.cuh"
+#include "qwen_internal.h"
+
+namespace qwen {
+namespace {
+
+constexpr int kRows = 128;                 // rows of a stream (M)
+constexpr int kPos = 128;                  // positions of a tile
+constexpr int kSlots = 5;
+constexpr int kPrefixThreads = 320;
+constexpr int kProducer = 8, kIssuer = 9;
+constexpr int kColS = 0, kColO = 256;      // tensor-memory columns: S0 S1 (P over S), O0 O1
+
+struct PrefixArgs {
+  PagedAttnArgs a;
+  int group, rows, tiles, pairs;   // query heads and rows per kv head, row tiles, units
+  int steps;                       // position tiles
+  unsigned long long total;        // weighted steps of all units
+  float scale_log2;
+  float* part_o;                   // [units + runs][2][128][D]
+  float2* part_ml;                 // [units + runs][2][128]
+  const float* own_o;              // [n_seq][n_heads][D]
+  const float2* own_ml;
+};
+
+// Units of a kv head come pair by pair, an odd tile's last; a step weighs its MMAs.
+__host__ __device__ __forceinline__ int unit_weight(const PrefixArgs& p, int pair) {
+  return 2 * pair + 1 < p.tiles ? 2 : 1;
+}
+__device__ __forceinline__ unsigned long long unit_begin(const PrefixArgs& p, int unit) {
+  const int h = unit / p.pairs, pair = unit % p.pairs;
+  return (unsigned long long)p.steps * ((unsigned long long)h * p.tiles + 2 * pair);
+}
+__device__ __forceinline__ unsigned long long prefix_run_start(const PrefixArgs& p, int c, int G) {
+  return p.total * (unsigned)c / (unsigned)G;
+}
+// Steps i of a unit that run c takes: those that begin (at begin + w i) in it.
+__device__ __forceinline__ void steps_of(const PrefixArgs& p, unsigned long long begin, int w, int c, int G, int* i0,
+                                         int* i1) {
+  const unsigned long long x0 = prefix_run_start(p, c, G), x1 = prefix_run_start(p, c + 1, G);
+  *i0 = x0 <= begin ? 0 : (int)min((unsigned long long)p.steps, (x0 - begin + w - 1) / w);
+  *i1 = x1 <= begin ? 0 : (int)min((unsigned long long)p.steps, (x1 - begin + w - 1) / w);
+}
+
+template <int D>
+struct __align__(1024) PrefixSmem {
+  uint8_t q[2][kRows * D * 2];             // [half][row][128 B], swizzled
+  uint8_t kv[kSlots][kPos * D * 2];
+  uint64_t full[kSlots], empty[kSlots], qfull[2], sfull[2], pfull[2], ofull[2], done;
+  uint32_t groups[kSlots];                 // of a K slot: 16-position groups that are there
+  uint32_t tmem;
+  int abort;
+};
+
+// ------------------------------------------------------------ tcgen05 PTX --
+__device__ __forceinline__ void t5_alloc(uint32_t* slot) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(slot)) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void t5_free(uint32_t t) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(t) : "memory");
+}
+__device__ __forceinline__ void t5_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void t5_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void t5_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void t5_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+      : "memory");
+}
+__device__ __forceinline__ void t5_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+      : "memory");
+}
+#define T5_R32(v) \
+  "=r"((v)[0]), "=r"((v)[1]), "=r"((v)[2]), "=r"((v)[3]), "=r"((v)[4]), "=r"((v)[5]), "=r"((v)[6]), "=r"((v)[7]), \
+  "=r"((v)[8]), "=r"((v)[9]), "=r"((v)[10]), "=r"((v)[11]), "=r"((v)[12]), "=r"((v)[13]), "=r"((v)[14]), \
+  "=r"((v)[15]), "=r"((v)[16]), "=r"((v)[17]), "=r"((v)[18]), "=r"((v)[19]), "=r"((v)[20]), "=r"((v)[21]), \
+  "=r"((v)[22]), "=r"((v)[23]), "=r"((v)[24]), "=r"((v)[25]), "=r"((v)[26]), "=r"((v)[27]), "=r"((v)[28]), \
+  "=r"((v)[29]), "=r"((v)[30]), "=r"((v)[31])
+#define T5_RW32(v) \
+  "+r"((v)[0]), "+r"((v)[1]), "+r"((v)[2]), "+r"((v)[3]), "+r"((v)[4]), "+r"((v)[5]), "+r"((v)[6]), "+r"((v)[7]), \
+  "+r"((v)[8]), "+r"((v)[9]), "+r"((v)[10]), "+r"((v)[11]), "+r"((v)[12]), "+r"((v)[13]), "+r"((v)[14]), \
+  "+r"((v)[15]), "+r"((v)[16]), "+r"((v)[17]), "+r"((v)[18]), "+r"((v)[19]), "+r"((v)[20]), "+r"((v)[21]), \
+  "+r"((v)[22]), "+r"((v)[23]), "+r"((v)[24]), "+r"((v)[25]), "+r"((v)[26]), "+r"((v)[27]), "+r"((v)[28]), \
+  "+r"((v)[29]), "+r"((v)[30]), "+r"((v)[31])
+#define T5_IN32(v) \
+  "r"((v)[0]), "r"((v)[1]), "r"((v)[2]), "r"((v)[3]), "r"((v)[4]), "r"((v)[5]), "r"((v)[6]), "r"((v)[7]), \
+  "r"((v)[8]), "r"((v)[9]), "r"((v)[10]), "r"((v)[11]), "r"((v)[12]), "r"((v)[13]), "r"((v)[14]), "r"((v)[15]), \
+  "r"((v)[16]), "r"((v)[17]), "r"((v)[18]), "r"((v)[19]), "r"((v)[20]), "r"((v)[21]), "r"((v)[22]), "r"((v)[23]), \
+  "r"((v)[24]), "r"((v)[25]), "r"((v)[26]), "r"((v)[27]), "r"((v)[28]), "r"((v)[29]), "r"((v)[30]), "r"((v)[31])
+// 32 columns of this thread's lane; the values are there after t5_landed on them.
+__device__ __forceinline__ void t5_ld32(uint32_t addr, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : T5_R32(v)
+      : "r"(addr));
+}
+__device__ __forceinline__ void t5_landed(uint32_t* v) {   // names the registers: no use of them moves before it
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : T5_RW32(v)::"memory");
+}
+__device__ __forceinline__ void t5_st32(uint32_t addr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::T5_IN32(v),
+      "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void t5_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Shared-memory matrix descriptors, 128-byte swizzle, version 1.  K-major: 8-row
+// groups 1024 B apart.  N-major (V as [position][64 elements]): 8-position groups
+// 1024 B apart (SBO), the next 64 elements kPos * 128 B on (LBO).
+__device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ uint64_t desc_n(uint32_t addr) {
+  return desc_k(addr) | ((uint64_t)((kPos * 128) >> 4) << 16);
+}
+// kind::f16: fp32 accumulator; A and B both fp16 or both bf16; B N-major if nmajor.
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t idesc_of(int n, bool nmajor) {
+  const uint32_t bf = sizeof(T) == 2 && __is_same(T, __nv_bfloat16) ? 1u : 0u;
+  return (1u << 4) | (bf << 7) | (bf << 10) | ((nmajor ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(kRows >> 4) << 24);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kPrefixThreads, 1)
+    k_prefix(const __grid_constant__ PrefixArgs p, int box_rows, const __grid_constant__ CUtensorMap tmk,
+             const __grid_constant__ CUtensorMap tmv) {
+  extern __shared__ uint8_t smem_raw[];
+  PrefixSmem<D>& s = *reinterpret_cast<PrefixSmem<D>*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
+  const PagedAttnArgs& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int c = blockIdx.x, G = gridDim.x;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kSlots; ++i) {
+      mbar_init(&s.full[i], 1);
+      mbar_init(&s.empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.qfull[i], 4);
+      mbar_init(&s.sfull[i], 1);
+      mbar_init(&s.pfull[i], 4);
+      mbar_init(&s.ofull[i], 1);
+    }
+    mbar_init(&s.done, 1);
+    s.abort = 0;
+    fence_mbar_init();
+    pdl_launch_dependents();
+  }
+  if (warp == kIssuer) t5_alloc(&s.tmem);
+  t5_before();
+  __syncthreads();
+  t5_after();
+  const uint32_t tmem = s.tmem;
+  const unsigned long long x0 = prefix_run_start(p, c, G), x1 = prefix_run_start(p, c + 1, G);
+  const int units = (int)a.kv.n_kv_heads * p.pairs;
+  // first unit with a step in this run: the one that holds x0, or the next
+  int unit0 = 0;
+  if (x0 < x1) {
+    const unsigned long long per_head = (unsigned long long)p.steps * p.tiles;
+    const int h = (int)(x0 / per_head);
+    unit0 = h * p.pairs + (int)((x0 - h * per_head) / (2ull * p.steps));
+  } else {
+    unit0 = units;
+  }
+  // The queries, pages and page numbers that this kernel reads come from before
+  // the own-positions kernel, which lets this one start only once those are there.
+
+  if (warp == kProducer) {
+    // ------------------------------------------------------------ producer --
+    const int P = a.kv.page_size, boxes = kPos / box_rows, halves = D / 64;
+    uint32_t it = 0;   // loads so far: K, V, K, V, ..
+    bool alive = true;
+    for (int unit = unit0; unit < units && alive; ++unit) {
+      const unsigned long long begin = unit_begin(p, unit);
+      if (begin >= x1) break;
+      int i0, i1;
+      steps_of(p, begin, unit_weight(p, unit % p.pairs), c, G, &i0, &i1);
+      const int h = unit / p.pairs;
+      for (int step = i0; step < i1 && alive; ++step) {
+        // lane: box lane / halves of a tile, half lane % halves
+        const int box = lane / halves, half = lane % halves;
+        const int pos = step * kPos + box * box_rows;
+        int page = (int)a.kv.n_pages;   // outside the pool: the box is filled with zeros
+        bool there = false;
+        if (box < boxes && pos < (int)a.prefix_len) {
+          const int x = a.prefix_pages[pos >> a.page_shift];
+          there = x >= 0 && (uint32_t)x < a.kv.n_pages;
+          if (there) page = x;
+          else raise_error(a.err, kDevBadArgument);
+        }
+        const uint32_t have = __ballot_sync(0xffffffffu, there && half == 0);
+        for (int kv = 0; kv < 2; ++kv, ++it) {
+          const int slot = it % kSlots;
+          if (it >= kSlots &&
+              !__all_sync(0xffffffffu, paged_wait(&s.empty[slot], ((it / kSlots) - 1) & 1, &s.abort, a.err))) {
+            alive = false;
+            break;
+          }
+          if (lane == 0) {
+            if (kv == 0) {
+              uint32_t groups = 0;
+              for (int b = 0; b < boxes; ++b)
+                if (have >> (b * halves) & 1) groups |= ((1u << (box_rows / 16)) - 1) << (b * box_rows / 16);
+              s.groups[slot] = groups;
+            }
+            mbar_arrive_expect_tx(&s.full[slot], kPos * D * 2);
+          }
+          __syncwarp();
+          if (box < boxes)
+            tma_load_half(s.kv[slot] + half * kPos * 128 + box * box_rows * 128, kv ? &tmv : &tmk, pos & (P - 1), half, h,
+                          page, &s.full[slot]);
+        }
+      }
+    }
+    __syncwarp();
+    // Every issued copy lands before the CTA may exit.
+    for (uint32_t j = it > kSlots ? it - kSlots : 0; j < it; ++j)
+      paged_wait(&s.full[j % kSlots], (j / kSlots) & 1, &s.abort, a.err, false);
+  } else if (warp == kIssuer) {
+    // ----------------------------------------------------------------- MMA --
+    constexpr uint32_t id_s = idesc_of<T>(kPos, false), id_o = idesc_of<T>(D, true);
+    uint32_t base = 0, qcount[2] = {0, 0}, pcount[2] = {0, 0};
+    bool alive = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      return __all_sync(0xffffffffu, paged_wait(bar, parity, &s.abort, a.err));
+    };
+    for (int unit = unit0; unit < units && alive; ++unit) {
+      const unsigned long long begin = unit_begin(p, unit);
+      if (begin >= x1) break;
+      int i0, i1;
+      const int w = unit_weight(p, unit % p.pairs);
+      steps_of(p, begin, w, c, G, &i0, &i1);
+      const int n = i1 - i0;
+      if (n <= 0) continue;
+      // stream i's k-th step: k, or (a lone row tile) 2 k + i
+      const int cnt[2] = {w == 2 ? n : (n + 1) / 2, w == 2 ? n : n / 2};
+      auto step_of = [&](int i, int k) { return w == 2 ? k : 2 * k + i; };
+      auto qk = [&](int i, int k) -> bool {
+        const uint32_t ld = base + 2 * step_of(i, k);
+        const int slot = ld % kSlots;
+        if (!wait(&s.full[slot], (ld / kSlots) & 1)) return false;
+        t5_after();
+        if (lane == 0) {
+          const uint32_t qa = smem_u32(s.q[i]), ka = smem_u32(s.kv[slot]);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+            t5_mma_ss(tmem + kColS + 128 * i, desc_k(qa + (kk >> 2) * kRows * 128 + (kk & 3) * 32),
+                      desc_k(ka + (kk >> 2) * kPos * 128 + (kk & 3) * 32), id_s, kk > 0);
+          t5_commit(&s.sfull[i]);
+          if (w == 1 || i == 1) t5_commit(&s.empty[slot]);
+        }
+        __syncwarp();
+        return true;
+      };
+      auto pv = [&](int i, int k) -> bool {
+        const uint32_t ld = base + 2 * step_of(i, k) + 1;
+        const int slot = ld % kSlots;
+        if (!wait(&s.pfull[i], pcount[i]++ & 1) || !wait(&s.full[slot], (ld / kSlots) & 1)) return false;
+        t5_after();
+        const int valid = (int)a.prefix_len - (i0 + step_of(i, k)) * kPos;   // positions of the tile
+        if (valid < kPos && (w == 1 || i == 0)) {
+          // past the prefix's end a page holds anything, and 0 weight times NaN is NaN
+          for (int x = valid * 8 + lane; x < kPos * 8; x += 32)
+#pragma unroll
+            for (int half = 0; half < D / 64; ++half)
+              *reinterpret_cast<uint4*>(s.kv[slot] + half * kPos * 128 + x * 16) = make_uint4(0, 0, 0, 0);
+          fence_proxy_async();
+          __syncwarp();
+        }
+        if (lane == 0) {
+          const uint32_t va = smem_u32(s.kv[slot]);
+#pragma unroll
+          for (int kk = 0; kk < kPos / 16; ++kk)
+            t5_mma_ts(tmem + kColO + 128 * i, tmem + kColS + 128 * i + 8 * kk, desc_n(va + kk * 2048), id_o,
+                      k > 0 || kk > 0);
+          t5_commit(&s.ofull[i]);
+          if (w == 1 || i == 1) t5_commit(&s.empty[slot]);
+        }
+        __syncwarp();
+        return true;
+      };
+      for (int i = 0; i < 2 && alive; ++i)
+        if (cnt[i] > 0) alive = wait(&s.qfull[i], qcount[i]++ & 1);
+      t5_after();
+      for (int i = 0; i < 2 && alive; ++i)
+        if (cnt[i] > 0) alive = qk(i, 0);
+      for (int k = 0; k < cnt[0] && alive; ++k)
+        for (int i = 0; i < 2 && alive; ++i) {
+          if (k < cnt[i]) alive = pv(i, k);
+          if (alive && k + 1 < cnt[i]) alive = qk(i, k + 1);
+        }
+      base += 2 * n;
+    }
+    // All MMAs have completed before tensor memory is freed.
+    if (lane == 0) t5_commit(&s.done);
+    __syncwarp();
+    paged_wait(&s.done, 0, &s.abort, a.err, false);
+  } else {
+    // ------------------------------------------------------------- softmax --
+    const int i = warp >> 2, row = threadIdx.x & (kRows - 1);
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + lanes + kColS + 128 * i, to = tmem + lanes + kColO + 128 * i;
+    uint32_t base = 0, scount = 0, ocount = 0;
+    bool alive = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      return __all_sync(0xffffffffu, paged_wait(bar, parity, &s.abort, a.err));
+    };
+    for (int unit = unit0; unit < units && alive; ++unit) {
+      const unsigned long long begin = unit_begin(p, unit);
+      if (begin >= x1) break;
+      int i0, i1;
+      const int pair = unit % p.pairs, h = unit / p.pairs, w = unit_weight(p, pair);
+      steps_of(p, begin, w, c, G, &i0, &i1);
+      const int n = i1 - i0;
+      if (n <= 0) continue;
+      const int cnt = w == 2 ? n : i == 0 ? (n + 1) / 2 : n / 2;
+      // this thread's row of Q into shared memory
+      const int r = (2 * pair + (w == 2 ? i : 0)) * kRows + row;   // of the kv head's rows
+      if (cnt > 0) {
+        const int seq = r / p.group, j = r % p.group;
+        const uint4* src = reinterpret_cast<const uint4*>(a.q + (long long)seq * a.q_stride + (long long)(h * p.group + j) * D);
+#pragma unroll
+        for (int x = 0; x < D / 8; ++x) {
+          const uint4 v = r < p.rows ? src[x] : make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(s.q[i] + (x >> 3) * kRows * 128 + row * 128 + (((x & 7) ^ (row & 7)) << 4)) = v;
+        }
+        fence_proxy_async();
+        t5_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.qfull[i]);
+      }
+      float ref = -INFINITY, sum = 0.f;
+      for (int k = 0; k < cnt && alive; ++k) {
+        const int step = w == 2 ? k : 2 * k + i;
+        alive = wait(&s.sfull[i], scount++ & 1);
+        if (!alive) break;
+        t5_after();
+        uint32_t v[128];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) t5_ld32(ts + 32 * q, v + 32 * q);
+        const uint32_t groups = s.groups[(base + 2 * step) % kSlots];
+        const int valid = (int)a.prefix_len - (i0 + step) * kPos;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) t5_landed(v + 32 * q);
+        if (groups != 0xffu || valid < kPos) {
+          const uint32_t none = __float_as_uint(p.scale_log2 < 0.f ? INFINITY : -INFINITY);
+#pragma unroll
+          for (int x = 0; x < 128; ++x)
+            if (x >= valid || !(groups >> (x / 16) & 1)) v[x] = none;
+        }
+        float mx[4];
+        if (p.scale_log2 >= 0.f) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) mx[q] = __uint_as_float(v[q]);
+#pragma unroll
+          for (int x = 4; x < 128; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(v[x]));
+          mx[0] = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) mx[q] = __uint_as_float(v[q]);
+#pragma unroll
+          for (int x = 4; x < 128; ++x) mx[x & 3] = fminf(mx[x & 3], __uint_as_float(v[x]));
+          mx[0] = fminf(fminf(mx[0], mx[1]), fminf(mx[2], mx[3]));
+        }
+        const float top = mx[0] * p.scale_log2;
+        const bool grown = top > ref + 15.f;
+        if (__any_sync(0xffffffffu, grown)) {
+          const float now = grown ? top - 7.f : ref;
+          const float f = ref == now ? 1.f : exp2_fast(ref - now);
+          ref = now;
+          sum *= f;
+          if (k > 0) {
+            alive = wait(&s.ofull[i], (ocount - 1) & 1);   // the last O += P V has completed
+            if (!alive) break;
+            t5_after();
+#pragma unroll
+            for (int q = 0; q < D / 32; ++q) {
+              uint32_t o[32];
+              t5_ld32(to + 32 * q, o);
+              t5_landed(o);
+#pragma unroll
+              for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+              t5_st32(to + 32 * q, o);
+            }
+          }
+        }
+        const float off = ref == -INFINITY ? 0.f : ref;
+        float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < 128; ++x) {
+          const float e = exp2_fast(fmaf(__uint_as_float(v[x]), p.scale_log2, -off));
+          part[x & 3] += e;
+          v[x] = __float_as_uint(e);
+        }
+        sum += (part[0] + part[1]) + (part[2] + part[3]);
+#pragma unroll
+        for (int x = 0; x < 64; ++x)
+          v[x] = pack2(T{}, __uint_as_float(v[2 * x]), __uint_as_float(v[2 * x + 1]));
+        t5_st32(ts, v);
+        t5_st32(ts + 32, v + 32);
+        t5_stored();
+        t5_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.pfull[i]);
+        ++ocount;
+      }
+      if (!alive) break;
+      // the stream's partial
+      const long long slot = ((long long)(unit + c) * 2 + i) * kRows + row;
+      if (cnt > 0) {
+        alive = wait(&s.ofull[i], (ocount - 1) & 1);
+        if (!alive) break;
+        t5_after();
+      }
+      if (r < p.rows) p.part_ml[slot] = make_float2(ref, sum);
+#pragma unroll
+      for (int q = 0; q < D / 32 && cnt > 0; ++q) {
+        uint32_t o[32];
+        t5_ld32(to + 32 * q, o);
+        t5_landed(o);
+        if (r < p.rows) {
+          uint4* dst = reinterpret_cast<uint4*>(p.part_o + slot * D + 32 * q);
+#pragma unroll
+          for (int x = 0; x < 8; ++x) dst[x] = make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+        }
+      }
+      t5_before();
+      base += 2 * n;
+    }
+  }
+  pdl_wait();   // so that the join, which waits for this kernel, also finds the own parts
+  t5_before();
+  __syncthreads();
+  if (warp == kIssuer) t5_free(tmem);
+}
+
+// One warp per query row: its own part and the prefix's partials, run by run.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) k_prefix_join(const __grid_constant__ PrefixArgs p, int G) {
+  constexpr int V = D / 32;
+  const PagedAttnArgs& a = p.a;
+  const int lane = threadIdx.x & 31;
+  const long long id = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  pdl_wait();
+  if (id >= (long long)a.kv.n_seq * a.n_heads) return;
+  const int seq = (int)(id / a.n_heads), head = (int)(id % a.n_heads);
+  if (a.seq_len[seq] > a.kv.max_pages * a.kv.page_size) return;   // reported by the own-positions kernel
+  const int h = head / p.group, r = seq * p.group + head % p.group;
+  const int tile = r / kRows, pair = tile / 2, w = unit_weight(p, pair), unit = h * p.pairs + pair;
+  const unsigned long long begin = unit_begin(p, unit), last = begin + (unsigned long long)w * (p.steps - 1);
+  const int c0 = (int)(((begin + 1) * G - 1) / p.total), c1 = (int)(((last + 1) * G - 1) / p.total);
+  const int n = (c1 - c0 + 1) * (w == 2 ? 1 : 2);   // partials: run c0 + i, or (lone tile) run c0 + i / 2, stream i % 2
+  const float2 own = p.own_ml[id];
+  float M = own.x, sum = own.y, v[V];
+  load_vec(v, p.own_o + id * D + V * lane);
+  if (sum == 0.f)
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = 0.f;
+  for (int b = 0; b < n; b += 32) {
+    float2 ml = make_float2(-INFINITY, 0.f);
+    int slot = 0;
+    if (b + lane < n) {
+      const int c = c0 + (w == 2 ? b + lane : (b + lane) / 2);
+      int i0, i1;
+      steps_of(p, begin, w, c, G, &i0, &i1);
+      slot = ((unit + c) * 2 + (w == 2 ? tile & 1 : lane & 1)) * kRows + r % kRows;
+      if (i1 > i0) ml = __ldcg(p.part_ml + slot);
+    }
+    const bool some = ml.y != 0.f;   // NaN counts as some
+    const float m1 = fmaxf(M, warp_max(some ? ml.x : -INFINITY));
+    const float f0 = sum == 0.f ? 0.f : exp2_fast(M - m1), f = some ? exp2_fast(ml.x - m1) : 0.f;
+    M = m1;
+    sum = sum * f0 + warp_sum(ml.y * f);
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] *= f0;
+    uint32_t mask = __ballot_sync(0xffffffffu, some);
+    while (mask) {   // four rows at a time
+      float x[4][V], fx[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int src = mask ? __ffs(mask) - 1 : 0;
+        fx[q] = __shfl_sync(0xffffffffu, f, src);
+        const int at = __shfl_sync(0xffffffffu, slot, src);
+        if (mask) {
+          load_vec(x[q], p.part_o + (long long)at * D + V * lane);
+        } else {
+          fx[q] = 0.f;
+#pragma unroll
+          for (int k = 0; k < V; ++k) x[q][k] = 0.f;
+        }
+        mask &= mask - 1;
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] += x[q][k] * fx[q];
+    }
+  }
+  write_row<T, D>(a, seq, head, v, M, sum, lane);
+}
+
+template <typename T, int D>
+int launch(const PrefixArgs& p, int G, const CUtensorMap& tmk, const CUtensorMap& tmv, int box_rows, cudaStream_t st) {
+  auto kern = k_prefix<T, D>;
+  const int smem = (int)sizeof(PrefixSmem<D>) + 1024;
+  static_assert(sizeof(PrefixSmem<D>) + 1024 <= 227 * 1024, "shared memory");
+  static OncePerDevice once;
+  if (!once.done() &&
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return -1;
+  once.set();
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(G);
+  cfg.blockDim = dim3(kPrefixThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kern, p, box_rows, tmk, tmv) != cudaSuccess) return -1;
+  const long long rows = (long long)p.a.kv.n_seq * p.a.n_heads;
+  cfg.gridDim = dim3((unsigned)((rows + 7) / 8));
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = 0;
+  return cudaLaunchKernelEx(&cfg, k_prefix_join<T, D>, p, G) == cudaSuccess ? 0 : -1;
+}
+
+void plan(PrefixArgs& p, const qwen_paged_kv& kv, int n_heads, uint32_t prefix_len) {
+  p.group = n_heads / (int)kv.n_kv_heads;
+  p.rows = (int)kv.n_seq * p.group;
+  p.tiles = (p.rows + kRows - 1) / kRows;
+  p.pairs = (p.tiles + 1) / 2;
+  p.steps = (int)((prefix_len + kPos - 1) / kPos);
+  p.total = (unsigned long long)kv.n_kv_heads * p.tiles * p.steps;
+}
+
+struct Layout {
+  size_t own_o, own_ml, part_o, part_ml, bytes;   // offsets after the decode kernel's part
+};
+Layout layout(const PrefixArgs& p, const qwen_paged_kv& kv, int n_heads, int G) {
+  const size_t heads = (size_t)kv.n_seq * n_heads, D = kv.head_dim;
+  const size_t slots = ((size_t)kv.n_kv_heads * p.pairs + G) * 2 * kRows;
+  Layout l;
+  l.own_o = (paged_decode_workspace(kv, n_heads) + 255) / 256 * 256;
+  l.own_ml = l.own_o + heads * D * 4;
+  l.part_o = (l.own_ml + heads * 8 + 255) / 256 * 256;
+  l.part_ml = l.part_o + slots * D * 4;
+  l.bytes = l.part_ml + slots * 8;
+  return l;
+}
+
+}  // namespace
+
+size_t paged_prefix_workspace(const qwen_paged_kv& kv, int n_heads, uint32_t prefix_len) {
+  if (prefix_len == 0 || kv.n_kv_heads == 0 || n_heads < (int)kv.n_kv_heads) return paged_decode_workspace(kv, n_heads);
+  PrefixArgs p{};
+  plan(p, kv, n_heads, prefix_len);
+  return layout(p, kv, n_heads, paged_sm_count()).bytes;
+}
+
+int launch_paged_prefix(const PagedAttnArgs& a, cudaStream_t st) {
+  PrefixArgs p{};
+  p.a = a;
+  plan(p, a.kv, a.n_heads, a.prefix_len);
+  const int G = paged_sm_count();
+  const Layout l = layout(p, a.kv, a.n_heads, G);
+  uint8_t* ws = static_cast<uint8_t*>(a.workspace);
+  p.own_o = reinterpret_cast<float*>(ws + l.own_o);
+  p.own_ml = reinterpret_cast<float2*>(ws + l.own_ml);
+  p.part_o = reinterpret_cast<float*>(ws + l.part_o);
+  p.part_ml = reinterpret_cast<float2*>(ws + l.part_ml);
+  p.scale_log2 = a.scale * kLog2e;
+  if (launch_paged_decode(a, st, reinterpret_cast<float*>(ws + l.own_o), reinterpret_cast<float2*>(ws + l.own_ml)) != 0)
+    return -1;
+  const int box_rows = a.kv.page_size < (uint32_t)kPos ? (int)a.kv.page_size : kPos;
+  CUtensorMap tmk, tmv;
+  if (encode_pages_map(&tmk, a.kv, a.kv.k, box_rows, 1) || encode_pages_map(&tmv, a.kv, a.kv.v, box_rows, 1)) return -1;
+  const bool d64 = a.kv.head_dim == 64;
+  if (a.kv.dtype == QWEN_DTYPE_F16)
+    return d64 ? launch<__half, 64>(p, G, tmk, tmv, box_rows, st) : launch<__half, 128>(p, G, tmk, tmv, box_rows, st);
+  return d64 ? launch<__nv_bfloat16, 64>(p, G, tmk, tmv, box_rows, st)
+             : launch<__nv_bfloat16, 128>(p, G, tmk, tmv, box_rows, st);
+}
+
+}  // namespace qwen

@@ -299,17 +299,20 @@ def rope_append_paged(kv: PagedKV, q: torch.Tensor, k: torch.Tensor, v: torch.Te
 
 
 def _attend(kv, fn, need: int, lead, q, seq_len, extra, scale, out, return_lse):
-    heads = q.shape[1]
+    n, heads, dim = q.shape
     qp, qs = _rows("q", q, kv, kv.n_seq)
     if out is None:
-        out = torch.empty((kv.n_seq, heads, kv.head_dim), dtype=kv.dtype, device=kv.device)
-    op, os_ = _rows("out", out, kv, kv.n_seq, heads)
-    lse = torch.empty((kv.n_seq, heads), dtype=torch.float32, device=kv.device) if return_lse else None
-    ws = torch.empty(need, dtype=torch.uint8, device=kv.device) if need else None
-    _on(kv, fn, *lead, qp, qs, op, os_, None if lse is None else lse.data_ptr(), heads,
-        _ints("seq_len", seq_len, kv, kv.n_seq), *extra,
-        kv.head_dim ** -0.5 if scale is None else scale,
-        None if ws is None else ws.data_ptr(), need)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        op, os_ = out.data_ptr(), heads * dim
+    else:
+        op, os_ = _rows("out", out, kv, n, heads)
+    lse = lp = None
+    if return_lse:
+        lse = torch.empty_strided((n, heads), (heads, 1), dtype=torch.float32, device=kv.device)
+        lp = lse.data_ptr()
+    ws = torch.empty(need, dtype=torch.uint8, device=kv.device)
+    _on(kv, fn, *lead, qp, qs, op, os_, lp, heads, _ints("seq_len", seq_len, kv, kv.n_seq), *extra,
+        dim ** -0.5 if scale is None else scale, ws.data_ptr(), need)
     return (out, lse) if return_lse else out
 
 
