@@ -8,109 +8,342 @@
 // of the page.  Sums are held in 64 bits: the list is whole numbers, and in
 // 32 bits two pages closer than ~1e-6 would change places with the order of a
 // sum.
+//
+// k_page_scores streams the bounds (HBM: 512 B a page and kv head of 128) into one
+// 64-bit key a page whose order is the scores'; the conversions to 64 bits, 16 a
+// clock and SM, take nearly as long as the stream and run beside it.
+// k_page_list picks, a CTA per kv head and sequence: bins the keys linearly between
+// their least and greatest (2048 bins), finds the bin that the last place falls
+// in, and goes on inside it -- one round where scores are spread, and a round per 11
+// bits at worst -- until the bin is taken whole, small enough to rank directly, or
+// one value.
 #include "paged_common.cuh"
 #include "qwen_internal.h"
 
 namespace qwen {
 namespace {
 
-constexpr int kSelectThreads = 256;
+constexpr int kScoreWarps = 8;
+constexpr int kBatch = 8;             // pages a warp has in flight
+constexpr int kListThreads = 512;
+constexpr int kBins = 2048;
+constexpr int kRank = 128;            // keys ranked directly
+constexpr int kCached = 8192;         // keys held in shared memory
+
+typedef unsigned long long u64;
 
 // Ascending order of keys = ascending order of scores; NaN above everything.
-__device__ __forceinline__ unsigned long long score_key(double x) {
+__device__ __forceinline__ u64 score_key(double x) {
   if (x != x) return ~0ull;
-  const unsigned long long b = (unsigned long long)__double_as_longlong(x + 0.0);
+  const u64 b = (u64)__double_as_longlong(x + 0.0);
   return b >> 63 ? ~b : b | 0x8000000000000000ull;
 }
 
-// One CTA per (kv head, sequence): scores, then each page's rank by counting.
+__device__ __forceinline__ float2 unpack2(__half, uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+__device__ __forceinline__ float2 unpack2(__nv_bfloat16, uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
+// CTA: pages [pages_per_cta * blockIdx.x, ..) of sequence blockIdx.y, all kv heads.  A
+// warp keeps one kv head's Q+- in registers; a group of D / 4 lanes reads a page's
+// bounds, lower half lo and upper half hi, 8 elements a lane.
 template <typename T, int D>
-__global__ void __launch_bounds__(kSelectThreads) k_select_pages(PagedSelectArgs a) {
-  const int h = blockIdx.x, s = blockIdx.y, K = a.kv.n_kv_heads, G = a.n_heads / K;
-  const int tid = threadIdx.x;
-  __shared__ double qp[D], qn[D];
-  __shared__ int count;
+__global__ void __launch_bounds__(kScoreWarps * 32) k_page_scores(const __grid_constant__ PagedSelectArgs a,
+                                                                  int pages_per_cta) {
+  constexpr int kLanes = D / 4, kAtOnce = 32 / kLanes;   // lanes of a page, pages of a load
+  pdl_wait();
+  if (threadIdx.x == 0) pdl_launch_dependents();
+  const int s = blockIdx.y, K = a.kv.n_kv_heads, G = a.n_heads / K;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   bool ok;
   const int L = (int)checked_len(a.kv, a.seq_len, s, &ok);
   if (!ok) {
-    if (tid == 0) raise_error(a.err, kDevBadArgument);
+    if (threadIdx.x == 0 && blockIdx.x == 0) raise_error(a.err, kDevBadArgument);
     return;
   }
   const int n = (L + a.kv.page_size - 1) >> a.page_shift;
+  const int begin = blockIdx.x * pages_per_cta, end = min(n, begin + pages_per_cta);
+  if (n <= a.n_select || begin >= end) return;
+  const int32_t* table = a.kv.page_table + (long long)s * a.kv.table_stride;
+  // warps per head, where there are fewer heads than warps
+  const int share = K >= kScoreWarps ? 1 : kScoreWarps / K;
+  const int part = lane & (kLanes - 1), sub = lane / kLanes;
+  const bool upper = part >= kLanes / 2;
+  const int d0 = 8 * (part & (kLanes / 2 - 1));
+  for (int h = warp / share; h < K; h += kScoreWarps / share) {
+    double w[8];
+    uint32_t used[4];   // bounds that no query multiplies read as 0 (they may be infinite)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = 0;
+    for (int g = 0; g < G; ++g) {
+      const uint4 x = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + s * a.q_stride +
+                                                      (long long)(h * G + g) * D + d0);
+      const uint32_t b[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 v = unpack2(T{}, b[i]);
+        w[2 * i] += (v.x > 0.f) == upper ? v.x : 0.f;   // NaN goes to the lower half
+        w[2 * i + 1] += (v.y > 0.f) == upper ? v.y : 0.f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) used[i] = (w[2 * i] != 0 ? 0xffffu : 0u) | (w[2 * i + 1] != 0 ? 0xffff0000u : 0u);
+    u64* keys = reinterpret_cast<u64*>(a.scores) + ((long long)s * K + h) * a.kv.max_pages;
+    const T* bounds = reinterpret_cast<const T*>(a.kv.bounds) + (upper ? (long long)K * D : 0) + (long long)h * D + d0;
+    constexpr int kPages = kBatch * kAtOnce;
+    for (int p0 = begin + (warp % share) * kPages; p0 < end; p0 += share * kPages) {
+      int page = lane < kPages && p0 + lane < end ? table[p0 + lane] : 0;
+      const bool bad = page < 0 || (uint32_t)page >= a.kv.n_pages;
+      if (bad) {
+        raise_error(a.err, kDevBadArgument);
+        page = 0;
+      }
+      const uint32_t bads = __ballot_sync(0xffffffffu, bad);
+      uint4 x[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const long long at = __shfl_sync(0xffffffffu, page, i * kAtOnce + sub);
+        x[i] = __ldg(reinterpret_cast<const uint4*>(bounds + at * 2 * K * D));
+      }
+      double sum[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const uint32_t b[4] = {x[i].x & used[0], x[i].y & used[1], x[i].z & used[2], x[i].w & used[3]};
+        sum[i] = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 v = unpack2(T{}, b[j]);
+          sum[i] = fma(w[2 * j], (double)v.x, sum[i]);
+          sum[i] = fma(w[2 * j + 1], (double)v.y, sum[i]);
+        }
+      }
+      // Eight sums over kLanes lanes: halve the sums while exchanging, so that lane
+      // part = 4 x (its page in reading order, bits swapped) holds one.
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) {
+        const int keep = kBatch / (2 * o);
+#pragma unroll
+        for (int i = 0; i < keep; ++i) {
+          const bool odd = lane & o;
+          const double mine = odd ? sum[keep + i] : sum[i], other = odd ? sum[i] : sum[keep + i];
+          sum[i] = mine + __shfl_xor_sync(0xffffffffu, other, o);
+        }
+      }
+#pragma unroll
+      for (int o = 8; o < kLanes; o <<= 1) sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], o);
+      const int i = ((lane & 1) << 2) | (lane & 2) | ((lane & 4) >> 2);   // of the batch
+      const int at = i * kAtOnce + sub;
+      if (part < 8 && p0 + at < end) keys[p0 + at] = bads >> at & 1 ? 0 : score_key(sum[0]);
+    }
+  }
+}
+
+struct ListSmem {
+  uint32_t bins[kBins];
+  u64 rank_key[kRank];
+  int rank_at[kRank];
+  u64 red[2][kListThreads / 32];
+  uint32_t warp_sum[kListThreads / 32];
+  u64 warp_pair[kListThreads / 32];
+  uint32_t count, found_bin, found_above;
+  u64 key;
+  int at;
+};
+
+// Exclusive sum over the CTA's threads of v (and the total), packed or not.
+template <typename V>
+__device__ __forceinline__ V exclusive_sum(V v, V* warp_sums, V* total) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  V inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const V x = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += x;
+  }
+  if (lane == 31) warp_sums[warp] = inc;
+  __syncthreads();
+  V before = inc - v, all = 0;
+#pragma unroll
+  for (int w = 0; w < kListThreads / 32; ++w) {
+    if (w < warp) before += warp_sums[w];
+    all += warp_sums[w];
+  }
+  *total = all;
+  __syncthreads();
+  return before;
+}
+
+__global__ void __launch_bounds__(kListThreads) k_page_list(const __grid_constant__ PagedSelectArgs a) {
+  extern __shared__ u64 cached[];
+  __shared__ ListSmem sm;
+  pdl_wait();
+  if (threadIdx.x == 0) pdl_launch_dependents();
+  const int h = blockIdx.x, s = blockIdx.y, K = a.kv.n_kv_heads, tid = threadIdx.x;
+  bool ok;
+  const int L = (int)checked_len(a.kv, a.seq_len, s, &ok);
+  if (!ok) return;   // reported by k_page_scores
+  const int n = (L + a.kv.page_size - 1) >> a.page_shift;
   int32_t* list = a.pages + ((long long)s * K + h) * a.n_select;
   if (n <= a.n_select) {
-    for (int i = tid; i < a.n_select; i += kSelectThreads) list[i] = i < n ? i : -1;
+    for (int i = tid; i < a.n_select; i += kListThreads) list[i] = i < n ? i : -1;
     return;
   }
-  for (int d = tid; d < D; d += kSelectThreads) {
-    double p = 0, m = 0;
-    for (int g = 0; g < G; ++g) {
-      const double x = to_f32(reinterpret_cast<const T*>(a.q)[s * a.q_stride + (h * G + g) * D + d]);
-      p += x > 0 ? x : 0;
-      m += x > 0 ? 0 : x;
-    }
-    qp[d] = p;
-    qn[d] = m;
+  // The pages that compete: [first, end); `wanted` of them are taken.
+  const int first = a.n_first, end = n - a.n_last, m = end - first;
+  uint32_t wanted = a.n_select - a.n_first - a.n_last;
+  const u64* global = reinterpret_cast<const u64*>(a.scores) + ((long long)s * K + h) * a.kv.max_pages + first;
+  const u64* keys = global;
+  u64 lo = ~0ull, hi = 0;
+  for (int i = tid; i < m; i += kListThreads) {
+    const u64 x = __ldcg(global + i);
+    if (m <= kCached) cached[i] = x;
+    lo = min(lo, x);
+    hi = max(hi, x);
   }
-  if (tid == 0) count = 0;
+  if (m <= kCached) keys = cached;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+  }
+  if ((tid & 31) == 0) {
+    sm.red[0][tid >> 5] = lo;
+    sm.red[1][tid >> 5] = hi;
+  }
   __syncthreads();
-  unsigned long long* keys =
-      reinterpret_cast<unsigned long long*>(a.scores) + ((long long)s * K + h) * a.kv.max_pages;
-  const int32_t* table = a.kv.page_table + (long long)s * a.kv.table_stride;
-  for (int i = tid; i < n; i += kSelectThreads) {
-    const int page = table[i];
-    unsigned long long key = 0;
-    if (page < 0 || (uint32_t)page >= a.kv.n_pages) {
-      raise_error(a.err, kDevBadArgument);
-    } else {
-      const T* lo = reinterpret_cast<const T*>(a.kv.bounds) + ((long long)page * 2 * K + h) * D;
-      const T* hi = lo + (long long)K * D;
-      double x = 0;
-      for (int d = 0; d < D; ++d)
-        x += qp[d] * (double)to_f32(hi[d]) + qn[d] * (double)to_f32(lo[d]);
-      if (x != x) {   // 0 times an infinite bound that no query reads adds nothing
-        x = 0;
-        for (int d = 0; d < D; ++d)
-          x += (qp[d] != 0 ? qp[d] * (double)to_f32(hi[d]) : 0) + (qn[d] != 0 ? qn[d] * (double)to_f32(lo[d]) : 0);
+#pragma unroll
+  for (int w = 0; w < kListThreads / 32; ++w) {
+    lo = min(lo, sm.red[0][w]);
+    hi = max(hi, sm.red[1][w]);
+  }
+  // Taken: keys above `cut`, and of those equal to it the first `ties`.
+  u64 cut = ~0ull;
+  uint32_t ties = 0;
+  if (wanted == 0) {
+    cut = ~0ull;
+  } else {
+    for (;;) {
+      if (lo == hi) {
+        cut = lo;
+        ties = wanted;
+        break;
       }
-      key = score_key(x);
+      const int shift = max(0, 64 - __clzll(hi - lo) - 11);
+      for (int i = tid; i < kBins; i += kListThreads) sm.bins[i] = 0;
+      if (tid == 0) sm.count = 0;
+      __syncthreads();
+      for (int i = tid; i < m; i += kListThreads) {
+        const u64 x = keys[i];
+        if (x >= lo && x <= hi) atomicAdd(&sm.bins[(x - lo) >> shift], 1u);
+      }
+      __syncthreads();
+      // From the top: the bin where the count reaches `wanted`.
+      constexpr int kPer = kBins / kListThreads;
+      uint32_t c[kPer], sum = 0, total;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) sum += c[j] = sm.bins[kBins - 1 - (tid * kPer + j)];
+      uint32_t above = exclusive_sum(sum, sm.warp_sum, &total);
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        if (above < wanted && above + c[j] >= wanted) {
+          sm.found_bin = kBins - 1 - (tid * kPer + j);
+          sm.found_above = above;
+        }
+        above += c[j];
+      }
+      __syncthreads();
+      const uint32_t bin = sm.found_bin, held = sm.bins[bin];
+      wanted -= sm.found_above;
+      lo += (u64)bin << shift;
+      hi = lo + min(hi - lo, ((u64)1 << shift) - 1);
+      if (held == wanted) {   // the whole bin
+        cut = lo - 1;         // lo > 0: a bin below the top one, or lo == hi above
+        if (lo == 0) {
+          cut = 0;
+          ties = 0xffffffffu;
+        }
+        break;
+      }
+      if (held <= kRank) {    // rank them: higher key first, then lower page
+        for (int i = tid; i < m; i += kListThreads) {
+          const u64 x = keys[i];
+          if (x >= lo && x <= hi) {
+            const uint32_t at = atomicAdd(&sm.count, 1u);
+            sm.rank_key[at] = x;
+            sm.rank_at[at] = i;
+          }
+        }
+        __syncthreads();
+        if (tid < (int)held) {
+          const u64 x = sm.rank_key[tid];
+          const int at = sm.rank_at[tid];
+          uint32_t rank = 0, same = 0;
+          for (uint32_t j = 0; j < held; ++j) {
+            rank += sm.rank_key[j] > x || (sm.rank_key[j] == x && sm.rank_at[j] < at);
+            same += sm.rank_key[j] == x && sm.rank_at[j] <= at;
+          }
+          if (rank == wanted - 1) {
+            sm.key = x;
+            sm.count = same;
+          }
+        }
+        __syncthreads();
+        cut = sm.key;
+        ties = sm.count;
+        break;
+      }
+      __syncthreads();
     }
-    keys[i] = key;
   }
-  __syncthreads();
-  const int wanted = a.n_select - a.n_first - a.n_last, end = n - a.n_last;
-  for (int i = tid; i < n; i += kSelectThreads) {
-    bool take = i < a.n_first || i >= end;
-    if (!take) {
-      int better = 0;
-      for (int j = a.n_first; j < end; ++j)
-        better += keys[j] > keys[i] || (keys[j] == keys[i] && j < i);
-      take = better < wanted;
-    }
-    if (take) list[atomicAdd(&count, 1)] = i;
+  // Ascending list: each thread a run of pages; places from one sum over the CTA of
+  // (keys above the cut, keys equal to it).
+  const int per = (m + kListThreads - 1) / kListThreads, i0 = min(m, tid * per), i1 = min(m, i0 + per);
+  u64 mine = 0, total;
+  for (int i = i0; i < i1; ++i) mine += keys[i] > cut ? 1ull << 32 : keys[i] == cut ? 1ull : 0ull;
+  const u64 before = exclusive_sum(mine, sm.warp_pair, &total);
+  uint32_t equal = (uint32_t)before;
+  int at = a.n_first + (int)(before >> 32) + (int)min(equal, ties);
+  for (int i = i0; i < i1; ++i) {
+    const bool take = keys[i] > cut || (keys[i] == cut && equal++ < ties);
+    if (take) list[at++] = first + i;
   }
-  __syncthreads();
-  if (tid == 0)   // ascending
-    for (int i = 1; i < a.n_select; ++i) {
-      const int x = list[i];
-      int j = i;
-      for (; j > 0 && list[j - 1] > x; --j) list[j] = list[j - 1];
-      list[j] = x;
-    }
+  for (int i = tid; i < a.n_first; i += kListThreads) list[i] = i;
+  for (int i = tid; i < a.n_last; i += kListThreads) list[a.n_select - a.n_last + i] = end + i;
+}
+
+template <typename T, int D>
+int launch(const PagedSelectArgs& a, cudaStream_t st) {
+  static OncePerDevice once;
+  const int smem = kCached * (int)sizeof(u64);
+  if (!once.done() &&
+      cudaFuncSetAttribute(k_page_list, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return -1;
+  once.set();
+  // Pages of a CTA: fewer where the whole batch would not fill the SMs twice.
+  int per = 256;
+  while (per > 32 && (long long)((a.kv.max_pages + per - 1) / per) * a.kv.n_seq < 2 * paged_sm_count()) per /= 2;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((a.kv.max_pages + per - 1) / per, a.kv.n_seq);
+  cfg.blockDim = dim3(kScoreWarps * 32);
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, k_page_scores<T, D>, a, per) != cudaSuccess) return -1;
+  cfg.gridDim = dim3(a.kv.n_kv_heads, a.kv.n_seq);
+  cfg.blockDim = dim3(kListThreads);
+  cfg.dynamicSmemBytes = (size_t)(a.kv.max_pages < (uint32_t)kCached ? a.kv.max_pages : kCached) * sizeof(u64);
+  return cudaLaunchKernelEx(&cfg, k_page_list, a) == cudaSuccess ? 0 : -1;
 }
 
 }  // namespace
 
 int launch_select_pages(const PagedSelectArgs& a, cudaStream_t st) {
-  const dim3 grid(a.kv.n_kv_heads, a.kv.n_seq);
   const bool d64 = a.kv.head_dim == 64;
-  if (a.kv.dtype == QWEN_DTYPE_F16)
-    d64 ? k_select_pages<__half, 64><<<grid, kSelectThreads, 0, st>>>(a)
-        : k_select_pages<__half, 128><<<grid, kSelectThreads, 0, st>>>(a);
-  else
-    d64 ? k_select_pages<__nv_bfloat16, 64><<<grid, kSelectThreads, 0, st>>>(a)
-        : k_select_pages<__nv_bfloat16, 128><<<grid, kSelectThreads, 0, st>>>(a);
-  return 0;
+  if (a.kv.dtype == QWEN_DTYPE_F16) return d64 ? launch<__half, 64>(a, st) : launch<__half, 128>(a, st);
+  return d64 ? launch<__nv_bfloat16, 64>(a, st) : launch<__nv_bfloat16, 128>(a, st);
 }
 
 }  // namespace qwen
