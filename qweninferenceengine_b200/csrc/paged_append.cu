@@ -1,141 +1,390 @@
 // paged_append.cu -- rotation of new queries and keys, and the keys' and values'
-// way into a paged cache.
+// way into a paged cache, in one launch.
 //
 //   y1 = x1 cos a - x2 sin a,  y2 = x1 sin a + x2 cos a,  a = position * inv_freq[i]
 //
-// One CTA per (sequence, page that its new tokens touch): it rotates those
-// tokens' rows, writes them, and takes the keys into the page's bounds -- no
-// other CTA touches that page, so the bounds need no atomics.  With ragged
-// tokens the CTAs are numbered so that sequence s begins at
-// cu_tokens[s] / page_size + 2 s: n tokens touch at most n / page_size + 2 pages.
+// Bound: HBM for prompts (each row read and written once), latency for a decode
+// step.  A thread moves 16 elements of a head as two 16-byte loads and stores:
+// chunk c is elements 8c.. and R/2 + 8c.. (the two sides of 8 pairs), or with
+// interleaved pairs, and behind the rotated part of a head, elements 16c .. 16c+15.
 //
 // The angle is formed exactly (24 + 24 bits fit a double) and reduced to turns
-// in 64 bits: an fp32 product at position 100,000 is off by up to 0.004 rad.
+// in 64 bits: an fp32 product at position 100,000 is off by up to 0.004 rad.  Its
+// sine and cosine cost as much as rotating six heads by it, so prompts compute each
+// once: k_append_rows' query CTAs keep eight of a thread's angles in registers for
+// all query heads, its key CTAs a page's in shared memory for all kv heads.
+//
+// Bounds: a key CTA owns two chunks of one page's new keys (all kv heads), so the
+// least and greatest are reduced inside it: no atomics, and a page begun anew
+// starts from its own keys.  The new rows of a sequence touch at most
+// n / page_size + 2 pages; the key CTAs of sequence s are numbered from
+// cu_tokens[s] / page_size + 2 s on.
 #include "paged_common.cuh"
 #include "qwen_internal.h"
 
 namespace qwen {
 namespace {
 
-constexpr int kAppendThreads = 256;
+constexpr int kTokenThreads = 128;    // decode: a CTA per token
+constexpr int kRowThreads = 128;      // prompts
+constexpr int kHeadsAtOnce = 4;       // heads of a query CTA in flight
+constexpr int kReduceHeads = 8;       // kv heads between a key CTA's barriers
 
 __device__ __forceinline__ void sincos_of(float pos, float inv_freq, float* sn, float* cs) {
   const double turns = (double)pos * (double)inv_freq * 0.15915494309189533577;
   sincospif(2.0f * (float)(turns - rint(turns)), sn, cs);
 }
 
-// First sequence s with base(s + 1) > slot, base(s) = cu[s] / P + 2 s.
-__device__ __forceinline__ int seq_of_slot(const int32_t* cu, int n_seq, int shift, int slot) {
+__device__ __forceinline__ float2 to_f32x2(__half, uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+__device__ __forceinline__ float2 to_f32x2(__nv_bfloat16, uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
+// 16 elements: the words of two 16-byte halves.
+struct Chunk {
+  uint32_t w[8];
+};
+__device__ __forceinline__ Chunk load_chunk(const void* a, const void* b) {
+  const uint4 x = *reinterpret_cast<const uint4*>(a), y = *reinterpret_cast<const uint4*>(b);
+  return {{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w}};
+}
+__device__ __forceinline__ void store_chunk(void* a, void* b, const Chunk& c) {
+  *reinterpret_cast<uint4*>(a) = make_uint4(c.w[0], c.w[1], c.w[2], c.w[3]);
+  *reinterpret_cast<uint4*>(b) = make_uint4(c.w[4], c.w[5], c.w[6], c.w[7]);
+}
+// Where chunk c's halves lie in a head.
+template <bool kInterleaved>
+__device__ __forceinline__ void places(int c, int R, int* a, int* b) {
+  const bool split = !kInterleaved && 16 * c < R;
+  *a = split ? 8 * c : 16 * c;
+  *b = split ? R / 2 + 8 * c : 16 * c + 8;
+}
+// rot: (cos, sin) of the chunk's eight pairs.
+template <typename T, bool kInterleaved>
+__device__ __forceinline__ void rotate_chunk(Chunk& x, const float2 (&rot)[8]) {
+  if constexpr (kInterleaved) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 v = to_f32x2(T{}, x.w[i]);
+      x.w[i] = pack2(T{}, v.x * rot[i].x - v.y * rot[i].y, v.x * rot[i].y + v.y * rot[i].x);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 a = to_f32x2(T{}, x.w[i]), b = to_f32x2(T{}, x.w[4 + i]);
+      const float2 r0 = rot[2 * i], r1 = rot[2 * i + 1];
+      x.w[i] = pack2(T{}, a.x * r0.x - b.x * r0.y, a.y * r1.x - b.y * r1.y);
+      x.w[4 + i] = pack2(T{}, a.x * r0.y + b.x * r0.x, a.y * r1.y + b.y * r1.x);
+    }
+  }
+}
+__device__ __forceinline__ void rotation_of(const PagedAppendArgs& a, int pos, int c, float2 (&rot)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float sn, cs;
+    sincos_of((float)pos, a.inv_freq[8 * c + i], &sn, &cs);
+    rot[i] = make_float2(cs, sn);
+  }
+}
+
+__device__ __forceinline__ uint32_t min2(__half, uint32_t a, uint32_t b) {
+  const __half2 r = __hmin2_nan(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t max2(__half, uint32_t a, uint32_t b) {
+  const __half2 r = __hmax2_nan(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t min2(__nv_bfloat16, uint32_t a, uint32_t b) {
+  const __nv_bfloat162 r = __hmin2_nan(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t max2(__nv_bfloat16, uint32_t a, uint32_t b) {
+  const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t inf2(__half) { return 0x7c007c00u; }
+__device__ __forceinline__ uint32_t inf2(__nv_bfloat16) { return 0x7f807f80u; }
+
+// The pool page of a table entry, or -1 with the status word set.
+__device__ __forceinline__ int pool_page(const PagedAppendArgs& a, int s, int col) {
+  const int page = a.kv.page_table[(long long)s * a.kv.table_stride + col];
+  if (page >= 0 && (uint32_t)page < a.kv.n_pages) return page;
+  raise_error(a.err, kDevBadArgument);
+  return -1;
+}
+
+// One token per sequence: a CTA per token, a thread per (head, chunk).
+template <typename T, int D, bool kInterleaved>
+__global__ void __launch_bounds__(kTokenThreads) k_append_token(const __grid_constant__ PagedAppendArgs a) {
+  constexpr int NC = D / 16;
+  pdl_wait();
+  if (threadIdx.x == 0) pdl_launch_dependents();
+  const int s = blockIdx.x, H = a.n_heads, K = a.kv.n_kv_heads, R = a.rot_dim;
+  bool ok;
+  const int L = (int)checked_len(a.kv, a.seq_len, s, &ok);
+  if (L == 0) {
+    if (!ok && threadIdx.x == 0) raise_error(a.err, kDevBadArgument);
+    return;
+  }
+  const int pos = L - 1, slot = pos & (a.kv.page_size - 1);
+  const int c = threadIdx.x % NC;   // the same for all of a thread's heads
+  int pa, pb;
+  places<kInterleaved>(c, R, &pa, &pb);
+  float2 rot[8];
+  const bool turns = 16 * c < R;
+  if (turns) rotation_of(a, pos, c, rot);
+  const int page = pool_page(a, s, pos >> a.page_shift);
+  for (int head = threadIdx.x / NC; head < H + 2 * K; head += kTokenThreads / NC) {
+    const T* src = head < H ? reinterpret_cast<const T*>(a.q) + s * a.q_stride + head * D
+                   : head < H + K ? reinterpret_cast<const T*>(a.k) + s * a.k_stride + (head - H) * D
+                                  : reinterpret_cast<const T*>(a.v) + s * a.v_stride + (head - H - K) * D;
+    Chunk x = load_chunk(src + pa, src + pb);
+    if (turns && head < H + K) rotate_chunk<T, kInterleaved>(x, rot);
+    if (head < H) {
+      T* dst = reinterpret_cast<T*>(a.q_out) + s * a.q_out_stride + head * D;
+      store_chunk(dst + pa, dst + pb, x);
+      continue;
+    }
+    if (page < 0) continue;
+    const int h = head < H + K ? head - H : head - H - K;
+    T* dst = reinterpret_cast<T*>(head < H + K ? a.kv.k : a.kv.v) + page * a.kv.page_stride + slot * a.kv.pos_stride +
+             h * a.kv.head_stride;
+    store_chunk(dst + pa, dst + pb, x);
+    if (a.kv.bounds && head < H + K) {
+      T* lo = reinterpret_cast<T*>(a.kv.bounds) + ((long long)page * 2 * K + h) * D;
+      T* hi = lo + (long long)K * D;
+      Chunk least = x, most = x;
+      if (slot != 0) {
+        const Chunk l0 = load_chunk(lo + pa, lo + pb), m0 = load_chunk(hi + pa, hi + pb);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          least.w[i] = min2(T{}, l0.w[i], x.w[i]);
+          most.w[i] = max2(T{}, m0.w[i], x.w[i]);
+        }
+      }
+      store_chunk(lo + pa, lo + pb, least);
+      store_chunk(hi + pa, hi + pb, most);
+    }
+  }
+}
+
+// First sequence s with base(s + 1) > x, base(s) = (cu[s] >> shift) + per_seq * s.
+__device__ __forceinline__ int seq_of(const int32_t* cu, int n_seq, int shift, int per_seq, int x) {
   int lo = 0, hi = n_seq - 1;
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
-    if ((cu[mid + 1] >> shift) + 2 * (mid + 1) > slot) hi = mid;
+    if ((cu[mid + 1] >> shift) + per_seq * (mid + 1) > x) hi = mid;
     else lo = mid + 1;
   }
   return lo;
 }
-
-template <typename T, int D>
-__global__ void __launch_bounds__(kAppendThreads) k_rope_append(PagedAppendArgs a) {
-  const int P = a.kv.page_size, H = a.n_heads, K = a.kv.n_kv_heads, R = a.rot_dim;
-  int s, row0, n_new, index;
-  if (a.cu_tokens) {
-    s = seq_of_slot(a.cu_tokens, a.kv.n_seq, a.page_shift, blockIdx.x);
-    row0 = a.cu_tokens[s];
-    const int row1 = a.cu_tokens[s + 1];
-    if (row0 < 0 || row1 < row0 || row1 > a.n_tokens) {
-      if (threadIdx.x == 0) raise_error(a.err, kDevBadArgument);
-      return;
-    }
-    n_new = row1 - row0;
-    index = blockIdx.x - ((row0 >> a.page_shift) + 2 * s);
-  } else {
-    s = blockIdx.x;
-    row0 = s;
-    n_new = a.seq_len[s] > 0 ? 1 : 0;
-    index = 0;
+// Rows of sequence s and its length; false (reported if `report`) where they do not fit.
+__device__ __forceinline__ bool rows_of(const PagedAppendArgs& a, int s, bool report, int* row0, int* row1, int* L) {
+  *row0 = a.cu_tokens[s];
+  *row1 = a.cu_tokens[s + 1];
+  bool ok = *row0 >= 0 && *row1 >= *row0 && *row1 <= a.n_tokens;
+  if (ok && *row1 > *row0) {
+    bool fits;
+    *L = (int)checked_len(a.kv, a.seq_len, s, &fits);
+    ok = fits && *L >= *row1 - *row0;
   }
-  if (n_new == 0 || index < 0) return;
-  bool ok;
-  const int L = (int)checked_len(a.kv, a.seq_len, s, &ok);
-  if (!ok || L < n_new) {
-    if (threadIdx.x == 0) raise_error(a.err, kDevBadArgument);
+  if (!ok && report) raise_error(a.err, kDevBadArgument);
+  return ok;
+}
+
+// Ragged tokens.  CTAs 0 .. key_ctas - 1: chunks 2j, 2j+1 of the new keys of one page
+// (slot blockIdx.x / (D / 32)); the rest: q and v of
+// kRowThreads / (D / 16) tokens.
+template <typename T, int D, bool kInterleaved>
+__global__ void __launch_bounds__(kRowThreads) k_append_rows(const __grid_constant__ PagedAppendArgs a, int key_ctas) {
+  constexpr int NC = D / 16;
+  extern __shared__ float2 page_rot[];   // key CTA: [page_size][16]
+  __shared__ uint32_t part[kReduceHeads][kRowThreads / 32][32];
+  const int H = a.n_heads, K = a.kv.n_kv_heads, R = a.rot_dim, P = a.kv.page_size, tid = threadIdx.x;
+  const int n_seq = a.kv.n_seq;
+  pdl_wait();
+  if (tid == 0) pdl_launch_dependents();
+
+  if ((int)blockIdx.x >= key_ctas) {
+    // ------------------------------------------------------------- q and v --
+    const int row = ((int)blockIdx.x - key_ctas) * (kRowThreads / NC) + tid / NC, c = tid % NC;
+    if (row >= a.n_tokens || row >= a.cu_tokens[n_seq]) return;
+    const int s = seq_of(a.cu_tokens, n_seq, 0, 0, row);
+    int row0, row1, L;
+    if (!rows_of(a, s, false, &row0, &row1, &L) || row < row0 || row >= row1) return;
+    const int pos = L - (row1 - row);
+    int pa, pb;
+    places<kInterleaved>(c, R, &pa, &pb);
+    const bool turns = 16 * c < R;
+    const int page = pool_page(a, s, pos >> a.page_shift);
+    const T* q = reinterpret_cast<const T*>(a.q) + row * a.q_stride;
+    T* q_out = reinterpret_cast<T*>(a.q_out) + row * a.q_out_stride;
+    float2 rot[8];
+    if (turns) rotation_of(a, pos, c, rot);
+    for (int h0 = 0; h0 < H; h0 += kHeadsAtOnce) {
+      Chunk x[kHeadsAtOnce];
+#pragma unroll
+      for (int j = 0; j < kHeadsAtOnce; ++j)
+        if (h0 + j < H) x[j] = load_chunk(q + (h0 + j) * D + pa, q + (h0 + j) * D + pb);
+#pragma unroll
+      for (int j = 0; j < kHeadsAtOnce; ++j)
+        if (h0 + j < H) {
+          if (turns) rotate_chunk<T, kInterleaved>(x[j], rot);
+          store_chunk(q_out + (h0 + j) * D + pa, q_out + (h0 + j) * D + pb, x[j]);
+        }
+    }
+    if (page < 0) return;
+    const T* v = reinterpret_cast<const T*>(a.v) + row * a.v_stride + 16 * c;
+    T* v_out = reinterpret_cast<T*>(a.kv.v) + page * a.kv.page_stride + (pos & (P - 1)) * a.kv.pos_stride + 16 * c;
+    for (int h0 = 0; h0 < K; h0 += kHeadsAtOnce) {
+      Chunk x[kHeadsAtOnce];
+#pragma unroll
+      for (int j = 0; j < kHeadsAtOnce; ++j)
+        if (h0 + j < K) x[j] = load_chunk(v + (h0 + j) * D, v + (h0 + j) * D + 8);
+#pragma unroll
+      for (int j = 0; j < kHeadsAtOnce; ++j)
+        if (h0 + j < K) store_chunk(v_out + (h0 + j) * a.kv.head_stride, v_out + (h0 + j) * a.kv.head_stride + 8, x[j]);
+    }
     return;
   }
-  const int start = L - n_new;
+
+  // ------------------------------------------------------------------ keys --
+  const int page_slot = blockIdx.x / (D / 32), pair = blockIdx.x % (D / 32);
+  const int s = seq_of(a.cu_tokens, n_seq, a.page_shift, 2, page_slot);
+  int row0, row1, L;
+  if (!rows_of(a, s, tid == 0, &row0, &row1, &L) || row1 == row0) return;
+  const int index = page_slot - ((row0 >> a.page_shift) + 2 * s), start = L - (row1 - row0);
+  if (index < 0) return;
   const int col = (start >> a.page_shift) + index;
-  const int p0 = max(start, col * P), p1 = min(L, (col + 1) * P);   // positions of this CTA
-  if (p0 >= p1) return;
-  const int page = a.kv.page_table[(long long)s * a.kv.table_stride + col];
-  const bool in_pool = page >= 0 && (uint32_t)page < a.kv.n_pages;
-  if (!in_pool && threadIdx.x == 0) raise_error(a.err, kDevBadArgument);
-  const int n = p1 - p0;
-  const long long row = row0 + (p0 - start);
-  T* kc = reinterpret_cast<T*>(a.kv.k) + (long long)page * a.kv.page_stride;
-  T* vc = reinterpret_cast<T*>(a.kv.v) + (long long)page * a.kv.page_stride;
-  // rotated pairs, then what passes through, then the values
-  for (int i = threadIdx.x; i < n * (H + K) * (R / 2); i += kAppendThreads) {
-    const int pair = i % (R / 2), head = i / (R / 2) % (H + K), r = i / (R / 2) / (H + K);
-    const int d1 = a.interleaved ? 2 * pair : pair, d2 = a.interleaved ? d1 + 1 : d1 + R / 2;
-    float sn, cs;
-    sincos_of((float)(p0 + r), a.inv_freq[pair], &sn, &cs);
-    const T* x;
-    T* y;
-    if (head < H) {
-      x = reinterpret_cast<const T*>(a.q) + (row + r) * a.q_stride + head * D;
-      y = reinterpret_cast<T*>(a.q_out) + (row + r) * a.q_out_stride + head * D;
-    } else {
-      if (!in_pool) continue;
-      x = reinterpret_cast<const T*>(a.k) + (row + r) * a.k_stride + (head - H) * D;
-      y = kc + ((p0 + r) & (P - 1)) * a.kv.pos_stride + (head - H) * a.kv.head_stride;
+  const int p0 = max(start, col * P), n = min(L, (col + 1) * P) - p0;   // positions p0 .. p0 + n - 1
+  if (n <= 0) return;
+  const int page = pool_page(a, s, col);
+  if (page < 0) return;
+  const int c = 2 * pair + (tid & 1), r0 = tid >> 1, warp = tid >> 5, lane = tid & 31;
+  int pa, pb;
+  places<kInterleaved>(c, R, &pa, &pb);
+  const bool turns = 16 * c < R;
+  // the angles of this CTA's chunks: 16 a row
+  for (int i = tid; i < n * 16; i += kRowThreads) {
+    const int f = 16 * pair + (i & 15);
+    if (f < R / 2) {
+      float sn, cs;
+      sincos_of((float)(p0 + (i >> 4)), a.inv_freq[f], &sn, &cs);
+      page_rot[i] = make_float2(cs, sn);
     }
-    const float x1 = to_f32(x[d1]), x2 = to_f32(x[d2]);
-    y[d1] = from_f32<T>(x1 * cs - x2 * sn);
-    y[d2] = from_f32<T>(x1 * sn + x2 * cs);
   }
-  for (int i = threadIdx.x; i < n * (H + K) * (D - R); i += kAppendThreads) {
-    const int d = R + i % (D - R), head = i / (D - R) % (H + K), r = i / (D - R) / (H + K);
-    if (head < H)
-      reinterpret_cast<T*>(a.q_out)[(row + r) * a.q_out_stride + head * D + d] =
-          reinterpret_cast<const T*>(a.q)[(row + r) * a.q_stride + head * D + d];
-    else if (in_pool)
-      kc[((p0 + r) & (P - 1)) * a.kv.pos_stride + (head - H) * a.kv.head_stride + d] =
-          reinterpret_cast<const T*>(a.k)[(row + r) * a.k_stride + (head - H) * D + d];
-  }
-  if (!in_pool) return;
-  for (int i = threadIdx.x; i < n * K * D; i += kAppendThreads) {
-    const int d = i % D, h = i / D % K, r = i / D / K;
-    vc[((p0 + r) & (P - 1)) * a.kv.pos_stride + h * a.kv.head_stride + d] =
-        reinterpret_cast<const T*>(a.v)[(row + r) * a.v_stride + h * D + d];
-  }
-  if (!a.kv.bounds) return;
-  __syncthreads();   // the keys just written are read back below
+  __syncthreads();
   const bool anew = (p0 & (P - 1)) == 0;
-  T* bounds = reinterpret_cast<T*>(a.kv.bounds) + (long long)page * 2 * K * D;
-  for (int i = threadIdx.x; i < K * D; i += kAppendThreads) {
-    const T* x = kc + (p0 & (P - 1)) * a.kv.pos_stride + (i / D) * a.kv.head_stride + i % D;
-    T lo = anew ? x[0] : bounds[i], hi = anew ? x[0] : bounds[K * D + i];
-    for (int r = 0; r < n; ++r) {
-      lo = __hmin_nan(lo, x[r * a.kv.pos_stride]);
-      hi = __hmax_nan(hi, x[r * a.kv.pos_stride]);
+  const T* k = reinterpret_cast<const T*>(a.k) + (long long)(row0 + (p0 - start)) * a.k_stride;
+  T* dst = reinterpret_cast<T*>(a.kv.k) + page * a.kv.page_stride + (p0 & (P - 1)) * a.kv.pos_stride;
+  for (int hb = 0; hb < K; hb += kReduceHeads) {
+    for (int h = hb; h < min(K, hb + kReduceHeads); ++h) {
+      uint32_t least[8], most[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        least[i] = inf2(T{});
+        most[i] = inf2(T{}) | 0x80008000u;
+      }
+#pragma unroll 2
+      for (int r = r0; r < n; r += kRowThreads / 2) {
+        const T* src = k + r * a.k_stride + h * D;
+        Chunk x = load_chunk(src + pa, src + pb);
+        if (turns) {
+          float2 rot[8];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float4 v = reinterpret_cast<const float4*>(page_rot + 16 * r + 8 * (c & 1))[i];
+            rot[2 * i] = make_float2(v.x, v.y);
+            rot[2 * i + 1] = make_float2(v.z, v.w);
+          }
+          rotate_chunk<T, kInterleaved>(x, rot);
+        }
+        T* y = dst + r * a.kv.pos_stride + h * a.kv.head_stride;
+        store_chunk(y + pa, y + pb, x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          least[i] = min2(T{}, least[i], x.w[i]);
+          most[i] = max2(T{}, most[i], x.w[i]);
+        }
+      }
+      if (!a.kv.bounds) continue;
+      // Over the warp's 16 rows, halving what a lane keeps at each exchange: in the end
+      // bit 4 of the lane says least or most, bits 3, 2, 1 which word, bit 0 the chunk.
+      uint32_t v[8];
+      const bool up = lane & 16;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, up ? least[i] : most[i], 16);
+        v[i] = up ? max2(T{}, most[i], other) : min2(T{}, least[i], other);
+      }
+#pragma unroll
+      for (int o = 8; o >= 2; o >>= 1) {
+        const int keep = o / 2;
+#pragma unroll
+        for (int i = 0; i < keep; ++i) {
+          const bool odd = lane & o;
+          const uint32_t mine = odd ? v[keep + i] : v[i];
+          const uint32_t other = __shfl_xor_sync(0xffffffffu, odd ? v[i] : v[keep + i], o);
+          v[i] = up ? max2(T{}, mine, other) : min2(T{}, mine, other);
+        }
+      }
+      part[h - hb][warp][lane] = v[0];
     }
-    bounds[i] = lo;
-    bounds[K * D + i] = hi;
+    if (!a.kv.bounds) continue;
+    __syncthreads();
+    for (int h = hb + warp; h < min(K, hb + kReduceHeads); h += kRowThreads / 32) {
+      const bool up = lane & 16;
+      const int word = (lane >> 1) & 7;   // of the chunk's eight
+      uint32_t v = part[h - hb][0][lane];
+#pragma unroll
+      for (int w = 1; w < kRowThreads / 32; ++w)
+        v = up ? max2(T{}, v, part[h - hb][w][lane]) : min2(T{}, v, part[h - hb][w][lane]);
+      T* at = reinterpret_cast<T*>(a.kv.bounds) + (((long long)page * 2 + (up ? 1 : 0)) * K + h) * D +
+              (word < 4 ? pa + 2 * word : pb + 2 * (word - 4));
+      if (!anew) {
+        const uint32_t old = *reinterpret_cast<const uint32_t*>(at);
+        v = up ? max2(T{}, v, old) : min2(T{}, v, old);
+      }
+      *reinterpret_cast<uint32_t*>(at) = v;
+    }
+    __syncthreads();
   }
+}
+
+template <typename T, int D, bool kInterleaved>
+int launch(const PagedAppendArgs& a, cudaStream_t st) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (!a.cu_tokens) {
+    cfg.gridDim = dim3(a.kv.n_seq);
+    cfg.blockDim = dim3(kTokenThreads);
+    return cudaLaunchKernelEx(&cfg, k_append_token<T, D, kInterleaved>, a) == cudaSuccess ? 0 : -1;
+  }
+  const int key_ctas = ((a.n_tokens >> a.page_shift) + 2 * (int)a.kv.n_seq) * (D / 32);
+  constexpr int kTileRows = kRowThreads / (D / 16);
+  cfg.gridDim = dim3(key_ctas + (a.n_tokens + kTileRows - 1) / kTileRows);
+  cfg.blockDim = dim3(kRowThreads);
+  cfg.dynamicSmemBytes = (size_t)a.kv.page_size * 16 * sizeof(float2);
+  return cudaLaunchKernelEx(&cfg, k_append_rows<T, D, kInterleaved>, a, key_ctas) == cudaSuccess ? 0 : -1;
+}
+
+template <typename T, int D>
+int launch(const PagedAppendArgs& a, cudaStream_t st) {
+  return a.interleaved ? launch<T, D, true>(a, st) : launch<T, D, false>(a, st);
 }
 
 }  // namespace
 
 int launch_rope_append(const PagedAppendArgs& a, cudaStream_t st) {
-  const int grid = a.cu_tokens ? (a.n_tokens >> a.page_shift) + 2 * (int)a.kv.n_seq : (int)a.kv.n_seq;
   const bool d64 = a.kv.head_dim == 64;
-  if (a.kv.dtype == QWEN_DTYPE_F16)
-    d64 ? k_rope_append<__half, 64><<<grid, kAppendThreads, 0, st>>>(a)
-        : k_rope_append<__half, 128><<<grid, kAppendThreads, 0, st>>>(a);
-  else
-    d64 ? k_rope_append<__nv_bfloat16, 64><<<grid, kAppendThreads, 0, st>>>(a)
-        : k_rope_append<__nv_bfloat16, 128><<<grid, kAppendThreads, 0, st>>>(a);
-  return 0;
+  if (a.kv.dtype == QWEN_DTYPE_F16) return d64 ? launch<__half, 64>(a, st) : launch<__half, 128>(a, st);
+  return d64 ? launch<__nv_bfloat16, 64>(a, st) : launch<__nv_bfloat16, 128>(a, st);
 }
 
 }  // namespace qwen
