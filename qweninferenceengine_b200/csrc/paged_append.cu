@@ -27,7 +27,8 @@ namespace {
 
 constexpr int kTokenThreads = 128;    // decode: a CTA per token
 constexpr int kRowThreads = 128;      // prompts
-constexpr int kHeadsAtOnce = 4;       // heads of a query CTA in flight
+constexpr int kHeadsAtOnce = 8;       // heads of a query CTA in flight
+constexpr int kHeadsPerCta = 16;      // its query heads
 constexpr int kReduceHeads = 8;       // kv heads between a key CTA's barriers
 
 __device__ __forceinline__ void sincos_of(float pos, float inv_freq, float* sn, float* cs) {
@@ -194,8 +195,8 @@ __device__ __forceinline__ bool rows_of(const PagedAppendArgs& a, int s, bool re
 }
 
 // Ragged tokens.  CTAs 0 .. key_ctas - 1: chunks 2j, 2j+1 of the new keys of one page
-// (slot blockIdx.x / (D / 32)); the rest: q and v of
-// kRowThreads / (D / 16) tokens.
+// (slot blockIdx.x / (D / 32)); the rest: 16 query heads and
+// v of kRowThreads / (D / 16) tokens.
 template <typename T, int D, bool kInterleaved>
 __global__ void __launch_bounds__(kRowThreads) k_append_rows(const __grid_constant__ PagedAppendArgs a, int key_ctas) {
   constexpr int NC = D / 16;
@@ -208,7 +209,9 @@ __global__ void __launch_bounds__(kRowThreads) k_append_rows(const __grid_consta
 
   if ((int)blockIdx.x >= key_ctas) {
     // ------------------------------------------------------------- q and v --
-    const int row = ((int)blockIdx.x - key_ctas) * (kRowThreads / NC) + tid / NC, c = tid % NC;
+    const int parts = (H + kHeadsPerCta - 1) / kHeadsPerCta;   // and v goes with the first
+    const int x0 = ((int)blockIdx.x - key_ctas) / parts, first = ((int)blockIdx.x - key_ctas) % parts * kHeadsPerCta;
+    const int row = x0 * (kRowThreads / NC) + tid / NC, c = tid % NC, last = min(H, first + kHeadsPerCta);
     if (row >= a.n_tokens || row >= a.cu_tokens[n_seq]) return;
     const int s = seq_of(a.cu_tokens, n_seq, 0, 0, row);
     int row0, row1, L;
@@ -222,19 +225,19 @@ __global__ void __launch_bounds__(kRowThreads) k_append_rows(const __grid_consta
     T* q_out = reinterpret_cast<T*>(a.q_out) + row * a.q_out_stride;
     float2 rot[8];
     if (turns) rotation_of(a, pos, c, rot);
-    for (int h0 = 0; h0 < H; h0 += kHeadsAtOnce) {
+    for (int h0 = first; h0 < last; h0 += kHeadsAtOnce) {
       Chunk x[kHeadsAtOnce];
 #pragma unroll
       for (int j = 0; j < kHeadsAtOnce; ++j)
-        if (h0 + j < H) x[j] = load_chunk(q + (h0 + j) * D + pa, q + (h0 + j) * D + pb);
+        if (h0 + j < last) x[j] = load_chunk(q + (h0 + j) * D + pa, q + (h0 + j) * D + pb);
 #pragma unroll
       for (int j = 0; j < kHeadsAtOnce; ++j)
-        if (h0 + j < H) {
+        if (h0 + j < last) {
           if (turns) rotate_chunk<T, kInterleaved>(x[j], rot);
           store_chunk(q_out + (h0 + j) * D + pa, q_out + (h0 + j) * D + pb, x[j]);
         }
     }
-    if (page < 0) return;
+    if (page < 0 || first > 0) return;
     const T* v = reinterpret_cast<const T*>(a.v) + row * a.v_stride + 16 * c;
     T* v_out = reinterpret_cast<T*>(a.kv.v) + page * a.kv.page_stride + (pos & (P - 1)) * a.kv.pos_stride + 16 * c;
     for (int h0 = 0; h0 < K; h0 += kHeadsAtOnce) {
@@ -368,7 +371,8 @@ int launch(const PagedAppendArgs& a, cudaStream_t st) {
   }
   const int key_ctas = ((a.n_tokens >> a.page_shift) + 2 * (int)a.kv.n_seq) * (D / 32);
   constexpr int kTileRows = kRowThreads / (D / 16);
-  cfg.gridDim = dim3(key_ctas + (a.n_tokens + kTileRows - 1) / kTileRows);
+  const int parts = (a.n_heads + kHeadsPerCta - 1) / kHeadsPerCta;
+  cfg.gridDim = dim3(key_ctas + (a.n_tokens + kTileRows - 1) / kTileRows * parts);
   cfg.blockDim = dim3(kRowThreads);
   cfg.dynamicSmemBytes = (size_t)a.kv.page_size * 16 * sizeof(float2);
   return cudaLaunchKernelEx(&cfg, k_append_rows<T, D, kInterleaved>, a, key_ctas) == cudaSuccess ? 0 : -1;

@@ -58,6 +58,7 @@ constexpr unsigned long long kPagedWaitNs = 2000000000ull;
 // where `heed`, once another role of the CTA gave up.
 static __device__ __noinline__ bool paged_wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort,
                                              int* err, bool heed) {
+  if (heed && *abort) return false;
   const unsigned long long t0 = global_ns();
   for (uint32_t i = 1;; ++i) {
     if (mbar_try_wait(bar, parity)) return true;
@@ -74,6 +75,22 @@ static __device__ __noinline__ bool paged_wait_slow(uint64_t* bar, uint32_t pari
 __device__ __forceinline__ bool paged_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* err,
                                            bool heed = true) {
   return mbar_try_wait(bar, parity) || paged_wait_slow(bar, parity, abort, err, heed);
+}
+// The same where the wait is short and on the critical path: polls that do not
+// suspend the warp come first.
+__device__ __forceinline__ bool paged_spin(uint64_t* bar, uint32_t parity, volatile int* abort, int* err) {
+  for (int i = 0; i < 256; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    if (ok) return true;
+  }
+  return paged_wait_slow(bar, parity, abort, err, true);
 }
 
 // 5-D tile load (element, slot, half, head, page) of a cache's tensor map; the
@@ -120,6 +137,10 @@ __device__ __forceinline__ void write_row(const PagedAttnArgs& a, int seq, int h
     *reinterpret_cast<uint32_t*>(dst) = pack2(T{}, v[0] * inv, v[1] * inv);
   if (a.lse && lane == 0)
     a.lse[(long long)seq * a.n_heads + head] = sum == 0.f ? -INFINITY : (M + log2f(sum)) * kLn2;
+}
+// x / d; the 32-bit division where it suffices (a 64-bit one takes ~0.1 us here).
+__device__ __forceinline__ unsigned long long divide(unsigned long long x, unsigned long long d) {
+  return (x | d) >> 32 ? x / d : (uint32_t)x / (uint32_t)d;
 }
 // Positions of sequence s, or 0 with the status word set when the length does
 // not fit its row of the page table (*ok false).

@@ -107,10 +107,6 @@ __device__ __forceinline__ uint32_t seq_tiles(const DecodeArgs& p, uint32_t L) {
   return L ? (L + kTile - 1) / kTile : 1;   // an empty sequence still has its zeros written
 }
 
-// x / d; the 32-bit division where it suffices (a 64-bit one takes ~0.1 us here).
-__device__ __forceinline__ unsigned long long divide(unsigned long long x, unsigned long long d) {
-  return (x | d) >> 32 ? x / d : (uint32_t)x / (uint32_t)d;
-}
 __device__ __forceinline__ unsigned long long run_start(unsigned long long total, int c, int G) {
   return divide(total * (unsigned)c, (unsigned)G);
 }

@@ -18,10 +18,11 @@
 // tile stands alone), its steps the prefix's 128-position tiles.  All units'
 // steps stand in one row weighted by their MMAs, and one CTA per SM takes an equal
 // run of it.  Warps of a CTA:
-//   0-3, 4-7  softmax of stream 0 and 1 (thread = row): S from tensor memory, the
-//       weights back over it as fp16 / bf16 (P)
-//   8  producer: page table, TMA loads of K and V tiles into a 5-slot ring
-//   9  MMA issue: S = Q K^T (smem x smem), O += P V (tensor memory x smem, V read
+//   0-7, 8-15  softmax of stream 0 and 1: a thread has half a row (64 scores) of S
+//       from tensor memory, and puts the weights back over it as fp16 / bf16 (P);
+//       the two halves of a row agree on its maximum through shared memory
+//   16 producer: page table, TMA loads of K and V tiles into a 5-slot ring
+//   17 MMA issue: S = Q K^T (smem x smem), O += P V (tensor memory x smem, V read
 //       N-major as it lies in the pool)
 // The two streams are the unit's two row tiles over the same K / V slots; a lone
 // row tile runs alternate position tiles in each stream instead.  While one
@@ -40,8 +41,9 @@ namespace {
 constexpr int kRows = 128;                 // rows of a stream (M)
 constexpr int kPos = 128;                  // positions of a tile
 constexpr int kSlots = 5;
-constexpr int kPrefixThreads = 320;
-constexpr int kProducer = 8, kIssuer = 9;
+constexpr uint32_t kSmemBytes = 227 * 1024;
+constexpr int kPrefixThreads = 576;
+constexpr int kProducer = 16, kIssuer = 17;
 constexpr int kColS = 0, kColO = 256;      // tensor-memory columns: S0 S1 (P over S), O0 O1
 
 struct PrefixArgs {
@@ -65,22 +67,23 @@ __device__ __forceinline__ unsigned long long unit_begin(const PrefixArgs& p, in
   return (unsigned long long)p.steps * ((unsigned long long)h * p.tiles + 2 * pair);
 }
 __device__ __forceinline__ unsigned long long prefix_run_start(const PrefixArgs& p, int c, int G) {
-  return p.total * (unsigned)c / (unsigned)G;
+  return divide(p.total * (unsigned)c, (unsigned)G);
 }
 // Steps i of a unit that run c takes: those that begin (at begin + w i) in it.
 __device__ __forceinline__ void steps_of(const PrefixArgs& p, unsigned long long begin, int w, int c, int G, int* i0,
                                          int* i1) {
   const unsigned long long x0 = prefix_run_start(p, c, G), x1 = prefix_run_start(p, c + 1, G);
-  *i0 = x0 <= begin ? 0 : (int)min((unsigned long long)p.steps, (x0 - begin + w - 1) / w);
-  *i1 = x1 <= begin ? 0 : (int)min((unsigned long long)p.steps, (x1 - begin + w - 1) / w);
+  *i0 = x0 <= begin ? 0 : (int)min((unsigned long long)p.steps, (x0 - begin + w - 1) >> (w - 1));
+  *i1 = x1 <= begin ? 0 : (int)min((unsigned long long)p.steps, (x1 - begin + w - 1) >> (w - 1));
 }
 
 template <int D>
-struct __align__(1024) PrefixSmem {
+struct PrefixSmem {   // on a 1024-byte boundary
   uint8_t q[2][kRows * D * 2];             // [half][row][128 B], swizzled
   uint8_t kv[kSlots][kPos * D * 2];
   uint64_t full[kSlots], empty[kSlots], qfull[2], sfull[2], pfull[2], ofull[2], done;
   uint32_t groups[kSlots];                 // of a K slot: 16-position groups that are there
+  float top[2][2][kRows];                  // [stream][half][row]
   uint32_t tmem;
   int abort;
 };
@@ -148,8 +151,29 @@ __device__ __forceinline__ void t5_st32(uint32_t addr, const uint32_t* v) {
       "r"(addr)
       : "memory");
 }
+// Eight columns times f, in place (few registers: the caller holds 64 scores).
+__device__ __forceinline__ void t5_scale8(uint32_t addr, float f) {
+  uint32_t v[8];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+               : "r"(addr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7])::"memory");
+#pragma unroll
+  for (int x = 0; x < 8; ++x) v[x] = __float_as_uint(__uint_as_float(v[x]) * f);
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(v[0]), "r"(v[1]),
+               "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(addr)
+               : "memory");
+}
 __device__ __forceinline__ void t5_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// One lane of the warp; the branch on it is warp-uniform to the compiler, which
+// keeps descriptors in uniform registers.
+__device__ __forceinline__ bool t5_elect() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
 // Shared-memory matrix descriptors, 128-byte swizzle, version 1.  K-major: 8-row
 // groups 1024 B apart.  N-major (V as [position][64 elements]): 8-position groups
 // 1024 B apart (SBO), the next 64 elements kPos * 128 B on (LBO).
@@ -172,8 +196,13 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     k_prefix(const __grid_constant__ PrefixArgs p, int box_rows, const __grid_constant__ CUtensorMap tmk,
              const __grid_constant__ CUtensorMap tmv) {
   extern __shared__ uint8_t smem_raw[];
-  PrefixSmem<D>& s = *reinterpret_cast<PrefixSmem<D>*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
+  const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;   // 0: nothing lies before it
   const PagedAttnArgs& a = p.a;
+  if (pad + sizeof(PrefixSmem<D>) > kSmemBytes) {
+    if (threadIdx.x == 0) raise_error(a.err, kDevBadArgument);
+    return;
+  }
+  PrefixSmem<D>& s = *reinterpret_cast<PrefixSmem<D>*>(smem_raw + pad);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int c = blockIdx.x, G = gridDim.x;
   if (threadIdx.x == 0) {
@@ -182,9 +211,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       mbar_init(&s.empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&s.qfull[i], 4);
+      mbar_init(&s.qfull[i], 8);
       mbar_init(&s.sfull[i], 1);
-      mbar_init(&s.pfull[i], 4);
+      mbar_init(&s.pfull[i], 8);
       mbar_init(&s.ofull[i], 1);
     }
     mbar_init(&s.done, 1);
@@ -203,8 +232,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
   int unit0 = 0;
   if (x0 < x1) {
     const unsigned long long per_head = (unsigned long long)p.steps * p.tiles;
-    const int h = (int)(x0 / per_head);
-    unit0 = h * p.pairs + (int)((x0 - h * per_head) / (2ull * p.steps));
+    const int h = (int)divide(x0, per_head);
+    unit0 = h * p.pairs + (int)divide(x0 - h * per_head, 2ull * p.steps);
   } else {
     unit0 = units;
   }
@@ -281,27 +310,27 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       // stream i's k-th step: k, or (a lone row tile) 2 k + i
       const int cnt[2] = {w == 2 ? n : (n + 1) / 2, w == 2 ? n : n / 2};
       auto step_of = [&](int i, int k) { return w == 2 ? k : 2 * k + i; };
-      auto qk = [&](int i, int k) -> bool {
+      auto qk = [&](int i, int k) {   // the K tile has landed
         const uint32_t ld = base + 2 * step_of(i, k);
         const int slot = ld % kSlots;
-        if (!wait(&s.full[slot], (ld / kSlots) & 1)) return false;
-        t5_after();
-        if (lane == 0) {
-          const uint32_t qa = smem_u32(s.q[i]), ka = smem_u32(s.kv[slot]);
+        if (t5_elect()) {
+          // +32 B of d an MMA inside the 128-byte rows, then the other half
+          const uint64_t qd = desc_k(smem_u32(s.q[i])), kd = desc_k(smem_u32(s.kv[slot]));
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk)
-            t5_mma_ss(tmem + kColS + 128 * i, desc_k(qa + (kk >> 2) * kRows * 128 + (kk & 3) * 32),
-                      desc_k(ka + (kk >> 2) * kPos * 128 + (kk & 3) * 32), id_s, kk > 0);
+            t5_mma_ss(tmem + kColS + 128 * i, qd + (kk >> 2) * (kRows * 128 >> 4) + (kk & 3) * 2,
+                      kd + (kk >> 2) * (kPos * 128 >> 4) + (kk & 3) * 2, id_s, kk > 0);
           t5_commit(&s.sfull[i]);
           if (w == 1 || i == 1) t5_commit(&s.empty[slot]);
         }
         __syncwarp();
-        return true;
       };
       auto pv = [&](int i, int k) -> bool {
         const uint32_t ld = base + 2 * step_of(i, k) + 1;
         const int slot = ld % kSlots;
-        if (!wait(&s.pfull[i], pcount[i]++ & 1) || !wait(&s.full[slot], (ld / kSlots) & 1)) return false;
+        // One wait for P, its V tile and the stream's next K tile: a wait on a completed
+        // barrier takes ~150 cycles while MMAs run, so a softmax warp makes the other two.
+        if (!wait(&s.pfull[i], pcount[i]++ & 1)) return false;
         t5_after();
         const int valid = (int)a.prefix_len - (i0 + step_of(i, k)) * kPos;   // positions of the tile
         if (valid < kPos && (w == 1 || i == 0)) {
@@ -313,11 +342,11 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
           fence_proxy_async();
           __syncwarp();
         }
-        if (lane == 0) {
-          const uint32_t va = smem_u32(s.kv[slot]);
+        if (t5_elect()) {
+          const uint64_t vd = desc_n(smem_u32(s.kv[slot]));   // +16 positions of 128 B an MMA
 #pragma unroll
           for (int kk = 0; kk < kPos / 16; ++kk)
-            t5_mma_ts(tmem + kColO + 128 * i, tmem + kColS + 128 * i + 8 * kk, desc_n(va + kk * 2048), id_o,
+            t5_mma_ts(tmem + kColO + 128 * i, tmem + kColS + 128 * i + 8 * kk, vd + kk * (2048 >> 4), id_o,
                       k > 0 || kk > 0);
           t5_commit(&s.ofull[i]);
           if (w == 1 || i == 1) t5_commit(&s.empty[slot]);
@@ -329,11 +358,16 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         if (cnt[i] > 0) alive = wait(&s.qfull[i], qcount[i]++ & 1);
       t5_after();
       for (int i = 0; i < 2 && alive; ++i)
-        if (cnt[i] > 0) alive = qk(i, 0);
+        if (cnt[i] > 0) {
+          const uint32_t ld = base + 2 * step_of(i, 0);
+          alive = wait(&s.full[ld % kSlots], (ld / kSlots) & 1);
+          t5_after();
+          if (alive) qk(i, 0);
+        }
       for (int k = 0; k < cnt[0] && alive; ++k)
         for (int i = 0; i < 2 && alive; ++i) {
           if (k < cnt[i]) alive = pv(i, k);
-          if (alive && k + 1 < cnt[i]) alive = qk(i, k + 1);
+          if (alive && k + 1 < cnt[i]) qk(i, k + 1);
         }
       base += 2 * n;
     }
@@ -343,15 +377,16 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     paged_wait(&s.done, 0, &s.abort, a.err, false);
   } else {
     // ------------------------------------------------------------- softmax --
-    const int i = warp >> 2, row = threadIdx.x & (kRows - 1);
+    // On a wait that ran out the loop goes on (every later wait gives up at once), so
+    // that the two warps of a row block keep meeting at their barrier.
+    const int i = warp >> 3, half = (warp >> 2) & 1, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t ts = tmem + lanes + kColS + 128 * i, to = tmem + lanes + kColO + 128 * i;
+    const uint32_t ts = tmem + lanes + kColS + 128 * i + 64 * half, tp = tmem + lanes + kColS + 128 * i + 32 * half;
+    const uint32_t to = tmem + lanes + kColO + 128 * i + D / 2 * half;
+    const int pair_bar = 1 + i * 4 + (warp & 3);
     uint32_t base = 0, scount = 0, ocount = 0;
-    bool alive = true;
-    auto wait = [&](uint64_t* bar, uint32_t parity) {
-      return __all_sync(0xffffffffu, paged_wait(bar, parity, &s.abort, a.err));
-    };
-    for (int unit = unit0; unit < units && alive; ++unit) {
+    auto wait = [&](uint64_t* bar, uint32_t parity) { paged_wait(bar, parity, &s.abort, a.err); __syncwarp(); };
+    for (int unit = unit0; unit < units; ++unit) {
       const unsigned long long begin = unit_begin(p, unit);
       if (begin >= x1) break;
       int i0, i1;
@@ -360,13 +395,14 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       const int n = i1 - i0;
       if (n <= 0) continue;
       const int cnt = w == 2 ? n : i == 0 ? (n + 1) / 2 : n / 2;
-      // this thread's row of Q into shared memory
+      // this thread's half row of Q into shared memory
       const int r = (2 * pair + (w == 2 ? i : 0)) * kRows + row;   // of the kv head's rows
       if (cnt > 0) {
         const int seq = r / p.group, j = r % p.group;
         const uint4* src = reinterpret_cast<const uint4*>(a.q + (long long)seq * a.q_stride + (long long)(h * p.group + j) * D);
 #pragma unroll
-        for (int x = 0; x < D / 8; ++x) {
+        for (int x0 = 0; x0 < D / 16; ++x0) {
+          const int x = x0 + D / 16 * half;
           const uint4 v = r < p.rows ? src[x] : make_uint4(0, 0, 0, 0);
           *reinterpret_cast<uint4*>(s.q[i] + (x >> 3) * kRows * 128 + row * 128 + (((x & 7) ^ (row & 7)) << 4)) = v;
         }
@@ -376,96 +412,102 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         if (lane == 0) mbar_arrive(&s.qfull[i]);
       }
       float ref = -INFINITY, sum = 0.f;
-      for (int k = 0; k < cnt && alive; ++k) {
+      for (int k = 0; k < cnt; ++k) {
         const int step = w == 2 ? k : 2 * k + i;
-        alive = wait(&s.sfull[i], scount++ & 1);
-        if (!alive) break;
+        if ((warp & 7) == 0) {   // for the issuer: this step's V tile, the stream's next K tile
+          const uint32_t ld = base + 2 * step + 1, next = base + 2 * (w == 2 ? k + 1 : 2 * k + 2 + i);
+          wait(&s.full[ld % kSlots], (ld / kSlots) & 1);
+          if (k + 1 < cnt) wait(&s.full[next % kSlots], (next / kSlots) & 1);
+        }
+        wait(&s.sfull[i], scount++ & 1);
         t5_after();
-        uint32_t v[128];
+        const uint32_t groups = s.groups[(base + 2 * step) % kSlots] >> (4 * half);
+        const int valid = (int)a.prefix_len - (i0 + step) * kPos - 64 * half;
+        const bool whole = (groups & 15u) == 15u && valid >= 64;
+        uint32_t w2[32];
+        float add;
+        // Weights against reference `off`, their sum, and the greatest score.
+        auto weigh = [&](float off) -> float {
+          uint32_t v[64];
+          t5_ld32(ts, v);
+          t5_ld32(ts + 32, v + 32);
+          float mx[4], part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int q = 0; q < 4; ++q) t5_ld32(ts + 32 * q, v + 32 * q);
-        const uint32_t groups = s.groups[(base + 2 * step) % kSlots];
-        const int valid = (int)a.prefix_len - (i0 + step) * kPos;
+          for (int q = 0; q < 4; ++q) mx[q] = -INFINITY;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) t5_landed(v + 32 * q);
-        if (groups != 0xffu || valid < kPos) {
-          const uint32_t none = __float_as_uint(p.scale_log2 < 0.f ? INFINITY : -INFINITY);
+          for (int b = 0; b < 2; ++b) {
+            t5_landed(v + 32 * b);
+            if (!whole) {
+              const uint32_t none = __float_as_uint(p.scale_log2 < 0.f ? INFINITY : -INFINITY);
 #pragma unroll
-          for (int x = 0; x < 128; ++x)
-            if (x >= valid || !(groups >> (x / 16) & 1)) v[x] = none;
-        }
-        float mx[4];
-        if (p.scale_log2 >= 0.f) {
+              for (int x = 32 * b; x < 32 * b + 32; ++x)
+                if (x >= valid || !(groups >> (x / 16) & 1)) v[x] = none;
+            }
 #pragma unroll
-          for (int q = 0; q < 4; ++q) mx[q] = __uint_as_float(v[q]);
-#pragma unroll
-          for (int x = 4; x < 128; ++x) mx[x & 3] = fmaxf(mx[x & 3], __uint_as_float(v[x]));
-          mx[0] = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        } else {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) mx[q] = __uint_as_float(v[q]);
-#pragma unroll
-          for (int x = 4; x < 128; ++x) mx[x & 3] = fminf(mx[x & 3], __uint_as_float(v[x]));
-          mx[0] = fminf(fminf(mx[0], mx[1]), fminf(mx[2], mx[3]));
-        }
-        const float top = mx[0] * p.scale_log2;
+            for (int x = 32 * b; x < 32 * b + 32; x += 2) {
+              const float s0 = __uint_as_float(v[x]) * p.scale_log2, s1 = __uint_as_float(v[x + 1]) * p.scale_log2;
+              mx[x / 2 & 3] = fmaxf(mx[x / 2 & 3], fmaxf(s0, s1));
+              const float e0 = exp2_fast(s0 - off), e1 = exp2_fast(s1 - off);
+              part[2 * (x / 2 & 1)] += e0;
+              part[2 * (x / 2 & 1) + 1] += e1;
+              w2[x / 2] = pack2(T{}, e0, e1);
+            }
+          }
+          add = (part[0] + part[1]) + (part[2] + part[3]);
+          return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        };
+        // The reference holds for nearly every tile, so the weights are formed with it
+        // while the maximum is still being found, and again where it had to move.
+        const float mine = weigh(ref == -INFINITY ? 0.f : ref);
+        // The row's other half; also: both halves have read S before either writes P.
+        // (They have read the last step's maxima: the next S takes both their P.)
+        float* tops = &s.top[i][0][row];
+        tops[kRows * half] = mine;
+        asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
+        const float top = fmaxf(tops[0], tops[kRows]);
         const bool grown = top > ref + 15.f;
-        if (__any_sync(0xffffffffu, grown)) {
+        if (__any_sync(0xffffffffu, grown)) {   // the same in both halves
           const float now = grown ? top - 7.f : ref;
           const float f = ref == now ? 1.f : exp2_fast(ref - now);
           ref = now;
           sum *= f;
           if (k > 0) {
-            alive = wait(&s.ofull[i], (ocount - 1) & 1);   // the last O += P V has completed
-            if (!alive) break;
+            wait(&s.ofull[i], (ocount - 1) & 1);   // the last O += P V has completed
             t5_after();
-#pragma unroll
-            for (int q = 0; q < D / 32; ++q) {
-              uint32_t o[32];
-              t5_ld32(to + 32 * q, o);
-              t5_landed(o);
-#pragma unroll
-              for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
-              t5_st32(to + 32 * q, o);
-            }
+#pragma unroll 1
+            for (int q = 0; q < D / 2; q += 8) t5_scale8(to + q, f);
           }
+          weigh(ref == -INFINITY ? 0.f : ref);
+          asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");   // S is read again before P
         }
-        const float off = ref == -INFINITY ? 0.f : ref;
-        float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int x = 0; x < 128; ++x) {
-          const float e = exp2_fast(fmaf(__uint_as_float(v[x]), p.scale_log2, -off));
-          part[x & 3] += e;
-          v[x] = __float_as_uint(e);
-        }
-        sum += (part[0] + part[1]) + (part[2] + part[3]);
-#pragma unroll
-        for (int x = 0; x < 64; ++x)
-          v[x] = pack2(T{}, __uint_as_float(v[2 * x]), __uint_as_float(v[2 * x + 1]));
-        t5_st32(ts, v);
-        t5_st32(ts + 32, v + 32);
+        t5_st32(tp, w2);
+        sum += add;
         t5_stored();
         t5_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&s.pfull[i]);
         ++ocount;
       }
-      if (!alive) break;
-      // the stream's partial
+      // the stream's partial: the first half adds up the sums
       const long long slot = ((long long)(unit + c) * 2 + i) * kRows + row;
       if (cnt > 0) {
-        alive = wait(&s.ofull[i], (ocount - 1) & 1);
-        if (!alive) break;
+        wait(&s.ofull[i], (ocount - 1) & 1);
         t5_after();
       }
-      if (r < p.rows) p.part_ml[slot] = make_float2(ref, sum);
+      if (cnt > 0) {
+        float* sums = &s.top[i][0][row];
+        if (half == 1) sums[0] = sum;
+        asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
+        if (half == 0) sum += sums[0];
+      }
+      if (half == 0 && r < p.rows) p.part_ml[slot] = make_float2(ref, sum);
 #pragma unroll
-      for (int q = 0; q < D / 32 && cnt > 0; ++q) {
+      for (int q = 0; q < D / 64 && cnt > 0; ++q) {
         uint32_t o[32];
         t5_ld32(to + 32 * q, o);
         t5_landed(o);
         if (r < p.rows) {
-          uint4* dst = reinterpret_cast<uint4*>(p.part_o + slot * D + 32 * q);
+          uint4* dst = reinterpret_cast<uint4*>(p.part_o + slot * D + D / 2 * half + 32 * q);
 #pragma unroll
           for (int x = 0; x < 8; ++x) dst[x] = make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
         }
@@ -494,7 +536,7 @@ __global__ void __launch_bounds__(256) k_prefix_join(const __grid_constant__ Pre
   const int h = head / p.group, r = seq * p.group + head % p.group;
   const int tile = r / kRows, pair = tile / 2, w = unit_weight(p, pair), unit = h * p.pairs + pair;
   const unsigned long long begin = unit_begin(p, unit), last = begin + (unsigned long long)w * (p.steps - 1);
-  const int c0 = (int)(((begin + 1) * G - 1) / p.total), c1 = (int)(((last + 1) * G - 1) / p.total);
+  const int c0 = (int)divide((begin + 1) * G - 1, p.total), c1 = (int)divide((last + 1) * G - 1, p.total);
   const int n = (c1 - c0 + 1) * (w == 2 ? 1 : 2);   // partials: run c0 + i, or (lone tile) run c0 + i / 2, stream i % 2
   const float2 own = p.own_ml[id];
   float M = own.x, sum = own.y, v[V];
@@ -548,8 +590,8 @@ __global__ void __launch_bounds__(256) k_prefix_join(const __grid_constant__ Pre
 template <typename T, int D>
 int launch(const PrefixArgs& p, int G, const CUtensorMap& tmk, const CUtensorMap& tmv, int box_rows, cudaStream_t st) {
   auto kern = k_prefix<T, D>;
-  const int smem = (int)sizeof(PrefixSmem<D>) + 1024;
-  static_assert(sizeof(PrefixSmem<D>) + 1024 <= 227 * 1024, "shared memory");
+  const int smem = (int)kSmemBytes;
+  static_assert(sizeof(PrefixSmem<D>) <= kSmemBytes - 768, "shared memory");
   static OncePerDevice once;
   if (!once.done() &&
       cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
