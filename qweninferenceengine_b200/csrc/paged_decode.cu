@@ -74,13 +74,19 @@ constexpr int stages() {
   return D == 128 ? 3 : 6;
 }
 
-template <int D>
+// Queries in flight: of 16 heads two units', of 8 four.
+template <int NT>
+constexpr int query_slots() {
+  return 4 / NT;
+}
+
+template <int D, int NT>
 struct __align__(1024) DecodeSmem {
   uint8_t kv[stages<D>()][2][kTile * D * 2];
-  uint16_t q[kMaxSlotHeads * D];
+  uint16_t q[query_slots<NT>()][8 * NT * D];
   float2 ml[2][kWarps][kMaxSlotHeads];   // by piece parity: maximum and sum of each warp
   StageMeta meta[stages<D>()];
-  uint64_t full[stages<D>()], empty[stages<D>()], qfull, qempty, joined;
+  uint64_t full[stages<D>()], empty[stages<D>()], qfull[query_slots<NT>()], qempty[query_slots<NT>()], joined;
   CutPiece cut[2];
   int n_cut;
   int last[2];
@@ -276,9 +282,9 @@ template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     k_paged_decode(const __grid_constant__ DecodeArgs p, int box_rows,
                    const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv) {
-  constexpr int ST = stages<D>();
+  constexpr int ST = stages<D>(), QS = query_slots<NT>();
   extern __shared__ uint8_t smem_raw[];
-  DecodeSmem<D>& s = *reinterpret_cast<DecodeSmem<D>*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
+  DecodeSmem<D, NT>& s = *reinterpret_cast<DecodeSmem<D, NT>*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
   const PagedAttnArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -286,8 +292,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       mbar_init(&s.full[i], 1);
       mbar_init(&s.empty[i], kWarps);
     }
-    mbar_init(&s.qfull, 1);
-    mbar_init(&s.qempty, kWarps);
+    for (int i = 0; i < QS; ++i) {
+      mbar_init(&s.qfull[i], 1);
+      mbar_init(&s.qempty[i], kWarps);
+    }
     mbar_init(&s.joined, kWarps);
     s.abort = 0;
     fence_mbar_init();
@@ -334,10 +342,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       if (!fits && lane == 0) raise_error(a.err, kDevBadArgument);
       const int dest = !fits ? -2 : tile0 == 0 && tile1 == ts ? -1 : 2 * c + (tile0 == 0 ? 1 : 0);
       // the unit's queries
-      if (pieces && !__all_sync(0xffffffffu, paged_wait(&s.qempty, (pieces - 1) & 1, &s.abort, a.err))) break;
+      const int qs = pieces % QS;
+      if (pieces >= QS &&
+          !__all_sync(0xffffffffu, paged_wait(&s.qempty[qs], (pieces / QS - 1) & 1, &s.abort, a.err)))
+        break;
       if (lane == 0) {
-        mbar_arrive_expect_tx(&s.qfull, (uint32_t)heads * D * 2);
-        bulk_g2s(s.q, a.q + (long long)seq * a.q_stride + (long long)head * D, (uint32_t)heads * D * 2, &s.qfull);
+        mbar_arrive_expect_tx(&s.qfull[qs], (uint32_t)heads * D * 2);
+        bulk_g2s(s.q[qs], a.q + (long long)seq * a.q_stride + (long long)head * D, (uint32_t)heads * D * 2, &s.qfull[qs]);
       }
       ++pieces;
       if (dest >= 0) {
@@ -439,7 +450,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     // Every issued copy lands before the CTA may exit.
     for (uint32_t j = drained; j < it; ++j)
       paged_wait(&s.full[j % ST], (j / ST) & 1, &s.abort, a.err, false);
-    if (pieces) paged_wait(&s.qfull, (pieces - 1) & 1, &s.abort, a.err, false);
+    for (uint32_t j = pieces > (uint32_t)QS ? pieces - QS : 0; j < pieces; ++j)
+      paged_wait(&s.qfull[j % QS], (j / QS) & 1, &s.abort, a.err, false);
     return;
   }
 
@@ -463,14 +475,15 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     const int flags = meta.flags, valid = meta.valid[warp];
     if (flags & kEnd) break;
     if (flags & kFirst) {
-      if (!__all_sync(0xffffffffu, paged_wait(&s.qfull, pieces & 1, &s.abort, a.err))) return;
+      const int qs = pieces % QS;
+      if (!__all_sync(0xffffffffu, paged_wait(&s.qfull[qs], (pieces / QS) & 1, &s.abort, a.err))) return;
       ++pieces;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int j = 0; j < D / 32; ++j) {
           const uint4 v = 8 * n + g < meta.heads
-                              ? *reinterpret_cast<const uint4*>(s.q + (8 * n + g) * D + (j >> 1) * 64 +
+                              ? *reinterpret_cast<const uint4*>(s.q[qs] + (8 * n + g) * D + (j >> 1) * 64 +
                                                                 (2 * t4 + (j & 1)) * 8)
                               : make_uint4(0, 0, 0, 0);
           qf[n][4 * j] = v.x;
@@ -479,7 +492,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
           qf[n][4 * j + 3] = v.w;
         }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&s.qempty);
+      if (lane == 0) mbar_arrive(&s.qempty[qs]);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         m[n][0] = m[n][1] = -INFINITY;
@@ -702,8 +715,8 @@ template <typename T, int D, int NT>
 int launch(const DecodeArgs& p, int G, const CUtensorMap& tmk, const CUtensorMap& tmv, int box_rows,
            cudaStream_t st) {
   auto kern = k_paged_decode<T, D, NT>;
-  const int smem = (int)sizeof(DecodeSmem<D>) + 1024;
-  static_assert((sizeof(DecodeSmem<D>) + 2048) * kCtasPerSm <= 228 * 1024, "CTAs per SM");
+  const int smem = (int)sizeof(DecodeSmem<D, NT>) + 1024;
+  static_assert((sizeof(DecodeSmem<D, NT>) + 2048) * kCtasPerSm <= 228 * 1024, "CTAs per SM");
   static OncePerDevice once;
   if (!once.done() &&
       cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)

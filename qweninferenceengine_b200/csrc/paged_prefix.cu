@@ -15,9 +15,12 @@
 //       order, into out and lse
 //
 // k_prefix: a unit is a kv head and 256 rows (two tiles of M = 128; an odd last
-// tile stands alone), its steps the prefix's 128-position tiles.  All units'
-// steps stand in one row weighted by their MMAs, and one CTA per SM takes an equal
-// run of it.  Warps of a CTA:
+// tile stands alone), its steps the prefix's 128-position tiles.  With fewer units
+// than SMs each gets a whole number of CTAs, by its MMAs, which share its steps:
+// a CTA that went on from one unit to the next would load queries and store
+// partials twice (~5 us; 8 units of 68 steps took 57 us so, 44 us for the CTAs
+// with one unit).  With more, all steps stand in one row, weighted by their MMAs,
+// and one CTA per SM takes an equal run of it.  Warps of a CTA:
 //   0-7, 8-15  softmax of stream 0 and 1: a thread has half a row (64 scores) of S
 //       from tensor memory, and puts the weights back over it as fp16 / bf16 (P);
 //       the two halves of a row agree on its maximum through shared memory
@@ -31,6 +34,8 @@
 // reference by 2^15 (weights are 2^(s - r) with r = max - 7 when last moved, see
 // paged_decode.cu).
 #include <cudaTypedefs.h>
+
+#include <algorithm>
 
 #include "paged_common.cuh"
 #include "qwen_internal.h"
@@ -51,6 +56,7 @@ struct PrefixArgs {
   int group, rows, tiles, pairs;   // query heads and rows per kv head, row tiles, units
   int steps;                       // position tiles
   unsigned long long total;        // weighted steps of all units
+  int share2, share1;              // CTAs of a unit of two tiles, of one; 0: runs over all units
   float scale_log2;
   float* part_o;                   // [units + runs][2][128][D]
   float2* part_ml;                 // [units + runs][2][128]
@@ -76,6 +82,55 @@ __device__ __forceinline__ void steps_of(const PrefixArgs& p, unsigned long long
   *i0 = x0 <= begin ? 0 : (int)min((unsigned long long)p.steps, (x0 - begin + w - 1) >> (w - 1));
   *i1 = x1 <= begin ? 0 : (int)min((unsigned long long)p.steps, (x1 - begin + w - 1) >> (w - 1));
 }
+// First CTA of a unit with CTAs of its own.
+__device__ __forceinline__ int first_cta(const PrefixArgs& p, int h, int pair) {
+  const int per_head = p.tiles / 2 * p.share2 + (p.tiles & 1) * p.share1;
+  return h * per_head + pair * p.share2;
+}
+
+// The pieces of CTA c, one after another: steps [i0, i1) of a unit, partials in
+// slots 2 id, 2 id + 1.
+struct Pieces {
+  const PrefixArgs& p;
+  int c, G, unit, w, h, pair, i0, i1, id;
+  __device__ __forceinline__ Pieces(const PrefixArgs& p, int c, int G) : p(p), c(c), G(G), unit(-1) {}
+  __device__ __forceinline__ bool next() {
+    if (p.share2) {
+      if (unit >= 0) return false;
+      const int per_head = p.tiles / 2 * p.share2 + (p.tiles & 1) * p.share1;
+      h = c / per_head;
+      const int rest = c - h * per_head;
+      if (h >= (int)p.a.kv.n_kv_heads) return false;
+      pair = min(rest / p.share2, p.pairs - 1);
+      w = unit_weight(p, pair);
+      const int part = rest - pair * p.share2, parts = w == 2 ? p.share2 : p.share1;
+      unit = h * p.pairs + pair;
+      i0 = (int)divide((unsigned long long)p.steps * part, parts);
+      i1 = (int)divide((unsigned long long)p.steps * (part + 1), parts);
+      id = c;
+      return i1 > i0;
+    }
+    const int units = (int)p.a.kv.n_kv_heads * p.pairs;
+    const unsigned long long x0 = prefix_run_start(p, c, G), x1 = prefix_run_start(p, c + 1, G);
+    if (unit < 0) {
+      if (x0 >= x1) return false;
+      const unsigned long long per_head = (unsigned long long)p.steps * p.tiles;
+      const int hh = (int)divide(x0, per_head);
+      unit = hh * p.pairs + (int)divide(x0 - hh * per_head, 2ull * p.steps) - 1;
+    }
+    for (;;) {
+      if (++unit >= units) return false;
+      const unsigned long long begin = unit_begin(p, unit);
+      if (begin >= x1) return false;
+      h = unit / p.pairs;
+      pair = unit - h * p.pairs;
+      w = unit_weight(p, pair);
+      id = unit + c;
+      steps_of(p, begin, w, c, G, &i0, &i1);
+      if (i1 > i0) return true;
+    }
+  }
+};
 
 template <int D>
 struct PrefixSmem {   // on a 1024-byte boundary
@@ -226,17 +281,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
   __syncthreads();
   t5_after();
   const uint32_t tmem = s.tmem;
-  const unsigned long long x0 = prefix_run_start(p, c, G), x1 = prefix_run_start(p, c + 1, G);
-  const int units = (int)a.kv.n_kv_heads * p.pairs;
-  // first unit with a step in this run: the one that holds x0, or the next
-  int unit0 = 0;
-  if (x0 < x1) {
-    const unsigned long long per_head = (unsigned long long)p.steps * p.tiles;
-    const int h = (int)divide(x0, per_head);
-    unit0 = h * p.pairs + (int)divide(x0 - h * per_head, 2ull * p.steps);
-  } else {
-    unit0 = units;
-  }
+  Pieces piece(p, c, G);
   // The queries, pages and page numbers that this kernel reads come from before
   // the own-positions kernel, which lets this one start only once those are there.
 
@@ -245,12 +290,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     const int P = a.kv.page_size, boxes = kPos / box_rows, halves = D / 64;
     uint32_t it = 0;   // loads so far: K, V, K, V, ..
     bool alive = true;
-    for (int unit = unit0; unit < units && alive; ++unit) {
-      const unsigned long long begin = unit_begin(p, unit);
-      if (begin >= x1) break;
-      int i0, i1;
-      steps_of(p, begin, unit_weight(p, unit % p.pairs), c, G, &i0, &i1);
-      const int h = unit / p.pairs;
+    while (alive && piece.next()) {
+      const int h = piece.h, i0 = piece.i0, i1 = piece.i1;
       for (int step = i0; step < i1 && alive; ++step) {
         // lane: box lane / halves of a tile, half lane % halves
         const int box = lane / halves, half = lane % halves;
@@ -299,14 +340,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     auto wait = [&](uint64_t* bar, uint32_t parity) {
       return __all_sync(0xffffffffu, paged_wait(bar, parity, &s.abort, a.err));
     };
-    for (int unit = unit0; unit < units && alive; ++unit) {
-      const unsigned long long begin = unit_begin(p, unit);
-      if (begin >= x1) break;
-      int i0, i1;
-      const int w = unit_weight(p, unit % p.pairs);
-      steps_of(p, begin, w, c, G, &i0, &i1);
-      const int n = i1 - i0;
-      if (n <= 0) continue;
+    while (alive && piece.next()) {
+      const int i0 = piece.i0, n = piece.i1 - i0, w = piece.w;
       // stream i's k-th step: k, or (a lone row tile) 2 k + i
       const int cnt[2] = {w == 2 ? n : (n + 1) / 2, w == 2 ? n : n / 2};
       auto step_of = [&](int i, int k) { return w == 2 ? k : 2 * k + i; };
@@ -386,14 +421,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     const int pair_bar = 1 + i * 4 + (warp & 3);
     uint32_t base = 0, scount = 0, ocount = 0;
     auto wait = [&](uint64_t* bar, uint32_t parity) { paged_wait(bar, parity, &s.abort, a.err); __syncwarp(); };
-    for (int unit = unit0; unit < units; ++unit) {
-      const unsigned long long begin = unit_begin(p, unit);
-      if (begin >= x1) break;
-      int i0, i1;
-      const int pair = unit % p.pairs, h = unit / p.pairs, w = unit_weight(p, pair);
-      steps_of(p, begin, w, c, G, &i0, &i1);
-      const int n = i1 - i0;
-      if (n <= 0) continue;
+    while (piece.next()) {
+      const int i0 = piece.i0, n = piece.i1 - i0, w = piece.w, pair = piece.pair, h = piece.h;
       const int cnt = w == 2 ? n : i == 0 ? (n + 1) / 2 : n / 2;
       // this thread's half row of Q into shared memory
       const int r = (2 * pair + (w == 2 ? i : 0)) * kRows + row;   // of the kv head's rows
@@ -489,7 +518,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         ++ocount;
       }
       // the stream's partial: the first half adds up the sums
-      const long long slot = ((long long)(unit + c) * 2 + i) * kRows + row;
+      const long long slot = ((long long)piece.id * 2 + i) * kRows + row;
       if (cnt > 0) {
         wait(&s.ofull[i], (ocount - 1) & 1);
         t5_after();
@@ -522,68 +551,75 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
   if (warp == kIssuer) t5_free(tmem);
 }
 
-// One warp per query row: its own part and the prefix's partials, run by run.
+// One warp per query row: its own part and the prefix's partials, in order.  What it
+// reads it asks for at once, eight partials at a time: the kernel is one round
+// trip or two to L2.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) k_prefix_join(const __grid_constant__ PrefixArgs p, int G) {
-  constexpr int V = D / 32;
+  constexpr int V = D / 32, kAtOnce = 8;
   const PagedAttnArgs& a = p.a;
   const int lane = threadIdx.x & 31;
   const long long id = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  pdl_wait();
-  if (id >= (long long)a.kv.n_seq * a.n_heads) return;
-  const int seq = (int)(id / a.n_heads), head = (int)(id % a.n_heads);
-  if (a.seq_len[seq] > a.kv.max_pages * a.kv.page_size) return;   // reported by the own-positions kernel
-  const int h = head / p.group, r = seq * p.group + head % p.group;
+  const bool mine = id < (long long)a.kv.n_seq * a.n_heads;
+  const int seq = mine ? (int)(id / a.n_heads) : 0, head = mine ? (int)(id - (long long)seq * a.n_heads) : 0;
+  const int h = head / p.group, r = seq * p.group + head - h * p.group;
   const int tile = r / kRows, pair = tile / 2, w = unit_weight(p, pair), unit = h * p.pairs + pair;
-  const unsigned long long begin = unit_begin(p, unit), last = begin + (unsigned long long)w * (p.steps - 1);
-  const int c0 = (int)divide((begin + 1) * G - 1, p.total), c1 = (int)divide((last + 1) * G - 1, p.total);
-  const int n = (c1 - c0 + 1) * (w == 2 ? 1 : 2);   // partials: run c0 + i, or (lone tile) run c0 + i / 2, stream i % 2
+  // Partial k of the row: piece first + k, or (a lone tile) first + k / 2, stream k % 2.
+  const unsigned long long begin = unit_begin(p, unit);
+  int c0, n;
+  if (p.share2) {
+    c0 = first_cta(p, h, pair);
+    n = w == 2 ? p.share2 : 2 * p.share1;
+  } else {
+    c0 = (int)divide((begin + 1) * G - 1, p.total);
+    n = ((int)divide((begin + (unsigned long long)w * (p.steps - 1) + 1) * G - 1, p.total) - c0 + 1) * (w == 2 ? 1 : 2);
+  }
+  const int first = c0 + (p.share2 ? 0 : unit);
+  auto slot_of = [&](int k) { return ((first + (w == 2 ? k : k / 2)) * 2 + (w == 2 ? tile & 1 : k & 1)) * kRows + r % kRows; };
+  pdl_wait();
+  if (!mine) return;
+  const uint32_t L = a.seq_len[seq];
   const float2 own = p.own_ml[id];
   float M = own.x, sum = own.y, v[V];
   load_vec(v, p.own_o + id * D + V * lane);
-  if (sum == 0.f)
-#pragma unroll
-    for (int k = 0; k < V; ++k) v[k] = 0.f;
   for (int b = 0; b < n; b += 32) {
+    const int m = min(32, n - b);
     float2 ml = make_float2(-INFINITY, 0.f);
-    int slot = 0;
-    if (b + lane < n) {
-      const int c = c0 + (w == 2 ? b + lane : (b + lane) / 2);
-      int i0, i1;
-      steps_of(p, begin, w, c, G, &i0, &i1);
-      slot = ((unit + c) * 2 + (w == 2 ? tile & 1 : lane & 1)) * kRows + r % kRows;
-      if (i1 > i0) ml = __ldcg(p.part_ml + slot);
+    if (lane < m) {
+      ml = __ldcg(p.part_ml + slot_of(b + lane));
+      if (!p.share2) {   // a run may have none of the unit's steps
+        int i0, i1;
+        steps_of(p, begin, w, c0 + (w == 2 ? b + lane : (b + lane) / 2), G, &i0, &i1);
+        if (i1 <= i0) ml = make_float2(-INFINITY, 0.f);
+      }
     }
-    const bool some = ml.y != 0.f;   // NaN counts as some
-    const float m1 = fmaxf(M, warp_max(some ? ml.x : -INFINITY));
-    const float f0 = sum == 0.f ? 0.f : exp2_fast(M - m1), f = some ? exp2_fast(ml.x - m1) : 0.f;
-    M = m1;
-    sum = sum * f0 + warp_sum(ml.y * f);
+    float f = 0.f;
+    for (int k0 = 0; k0 < m; k0 += kAtOnce) {
+      float x[kAtOnce][V];
 #pragma unroll
-    for (int k = 0; k < V; ++k) v[k] *= f0;
-    uint32_t mask = __ballot_sync(0xffffffffu, some);
-    while (mask) {   // four rows at a time
-      float x[4][V], fx[4];
+      for (int q = 0; q < kAtOnce; ++q)
+        load_vec(x[q], p.part_o + (long long)slot_of(b + min(k0 + q, m - 1)) * D + V * lane);
+      if (k0 == 0) {
+        const bool some = ml.y != 0.f;   // NaN counts as some
+        const float m1 = fmaxf(sum == 0.f ? -INFINITY : M, warp_max(some ? ml.x : -INFINITY));
+        const float f0 = sum == 0.f ? 0.f : exp2_fast(M - m1);
+        f = some ? exp2_fast(ml.x - m1) : 0.f;
+        M = m1;
+        sum = sum * f0 + warp_sum(ml.y * f);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int src = mask ? __ffs(mask) - 1 : 0;
-        fx[q] = __shfl_sync(0xffffffffu, f, src);
-        const int at = __shfl_sync(0xffffffffu, slot, src);
-        if (mask) {
-          load_vec(x[q], p.part_o + (long long)at * D + V * lane);
-        } else {
-          fx[q] = 0.f;
-#pragma unroll
-          for (int k = 0; k < V; ++k) x[q][k] = 0.f;
-        }
-        mask &= mask - 1;
+        for (int k = 0; k < V; ++k) v[k] = f0 == 0.f ? 0.f : v[k] * f0;
       }
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
+      for (int q = 0; q < kAtOnce; ++q) {
+        const float fq = __shfl_sync(0xffffffffu, f, (k0 + q) & 31);
+        if (k0 + q < m && fq != 0.f) {   // what no piece has written is not read into the sum
 #pragma unroll
-        for (int k = 0; k < V; ++k) v[k] += x[q][k] * fx[q];
+          for (int k = 0; k < V; ++k) v[k] += x[q][k] * fq;
+        }
+      }
     }
   }
+  if (L > a.kv.max_pages * a.kv.page_size) return;   // reported by the own-positions kernel
   write_row<T, D>(a, seq, head, v, M, sum, lane);
 }
 
@@ -615,13 +651,16 @@ int launch(const PrefixArgs& p, int G, const CUtensorMap& tmk, const CUtensorMap
   return cudaLaunchKernelEx(&cfg, k_prefix_join<T, D>, p, G) == cudaSuccess ? 0 : -1;
 }
 
-void plan(PrefixArgs& p, const qwen_paged_kv& kv, int n_heads, uint32_t prefix_len) {
+void plan(PrefixArgs& p, const qwen_paged_kv& kv, int n_heads, uint32_t prefix_len, int G) {
   p.group = n_heads / (int)kv.n_kv_heads;
   p.rows = (int)kv.n_seq * p.group;
   p.tiles = (p.rows + kRows - 1) / kRows;
   p.pairs = (p.tiles + 1) / 2;
   p.steps = (int)((prefix_len + kPos - 1) / kPos);
   p.total = (unsigned long long)kv.n_kv_heads * p.tiles * p.steps;
+  const int weight = (int)kv.n_kv_heads * p.tiles;   // one row tile: 1
+  p.share1 = std::min(G / weight, p.steps);
+  p.share2 = p.share1 ? std::min(2 * G / weight, p.steps) : 0;
 }
 
 struct Layout {
@@ -644,15 +683,15 @@ Layout layout(const PrefixArgs& p, const qwen_paged_kv& kv, int n_heads, int G) 
 size_t paged_prefix_workspace(const qwen_paged_kv& kv, int n_heads, uint32_t prefix_len) {
   if (prefix_len == 0 || kv.n_kv_heads == 0 || n_heads < (int)kv.n_kv_heads) return paged_decode_workspace(kv, n_heads);
   PrefixArgs p{};
-  plan(p, kv, n_heads, prefix_len);
+  plan(p, kv, n_heads, prefix_len, paged_sm_count());
   return layout(p, kv, n_heads, paged_sm_count()).bytes;
 }
 
 int launch_paged_prefix(const PagedAttnArgs& a, cudaStream_t st) {
   PrefixArgs p{};
   p.a = a;
-  plan(p, a.kv, a.n_heads, a.prefix_len);
   const int G = paged_sm_count();
+  plan(p, a.kv, a.n_heads, a.prefix_len, G);
   const Layout l = layout(p, a.kv, a.n_heads, G);
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
   p.own_o = reinterpret_cast<float*>(ws + l.own_o);
