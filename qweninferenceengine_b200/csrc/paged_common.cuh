@@ -125,23 +125,29 @@ __device__ __forceinline__ void load_vec(float (&v)[2], const float* p) {
   const float2 x = __ldcg(reinterpret_cast<const float2*>(p));
   v[0] = x.x, v[1] = x.y;
 }
-// Output row and log-sum-exp from the unnormalised row v, its maximum and sum.
+// Output row and log-sum-exp from the unnormalised row v (this lane's D / 32 values
+// of it), its maximum and sum.  rcp and lg2 approximate to 2 steps of fp32.
 template <typename T, int D>
-__device__ __forceinline__ void write_row(const PagedAttnArgs& a, int seq, int head, const float (&v)[D / 32],
-                                          float M, float sum, int lane) {
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+__device__ __forceinline__ void write_row(const PagedAttnArgs& a, int seq, int head, float4 v, float M, float sum,
+                                          int lane) {
+  const float inv = sum == 0.f ? 0.f : __fdividef(1.f, sum);
   T* dst = reinterpret_cast<T*>(a.out) + (long long)seq * a.out_stride + (long long)head * D + D / 32 * lane;
-  if constexpr (D == 128)
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(T{}, v[0] * inv, v[1] * inv), pack2(T{}, v[2] * inv, v[3] * inv));
-  else
-    *reinterpret_cast<uint32_t*>(dst) = pack2(T{}, v[0] * inv, v[1] * inv);
+  const uint32_t lo = pack2(T{}, v.x * inv, v.y * inv);
+  if constexpr (D == 128) *reinterpret_cast<uint2*>(dst) = make_uint2(lo, pack2(T{}, v.z * inv, v.w * inv));
+  else *reinterpret_cast<uint32_t*>(dst) = lo;
   if (a.lse && lane == 0)
-    a.lse[(long long)seq * a.n_heads + head] = sum == 0.f ? -INFINITY : (M + log2f(sum)) * kLn2;
+    a.lse[(long long)seq * a.n_heads + head] = sum == 0.f ? -INFINITY : (M + __log2f(sum)) * kLn2;
 }
-// x / d; the 32-bit division where it suffices (a 64-bit one takes ~0.1 us here).
-__device__ __forceinline__ unsigned long long divide(unsigned long long x, unsigned long long d) {
+__device__ __forceinline__ float4 as_float4(const float (&v)[4]) { return make_float4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ float4 as_float4(const float (&v)[2]) { return make_float4(v[0], v[1], 0.f, 0.f); }
+
+// x / d.  Out of line, as all that runs once a call or rarely: these kernels start
+// with a cold instruction cache, and each further KB of straight-line code is a miss
+// of ~0.5 us on the way to the first load.
+static __device__ __noinline__ unsigned long long divide(unsigned long long x, unsigned long long d) {
   return (x | d) >> 32 ? x / d : (uint32_t)x / (uint32_t)d;
 }
+
 // Positions of sequence s, or 0 with the status word set when the length does
 // not fit its row of the page table (*ok false).
 __device__ __forceinline__ uint32_t checked_len(const qwen_paged_kv& kv, const uint32_t* seq_len,

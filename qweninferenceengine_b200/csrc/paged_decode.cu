@@ -129,7 +129,7 @@ __device__ __forceinline__ int piece_slot(const CutPiece& u, int i, int G) {
 
 // Total number of tiles, and the sequence that holds tile run_start(total, c) with
 // the number of tiles per unit before it and its length (one warp).
-__device__ unsigned long long find_run(const DecodeArgs& p, int c, int G, int lane, int* seq,
+__device__ __forceinline__ unsigned long long find_run(const DecodeArgs& p, int c, int G, int lane, int* seq,
                                        unsigned long long* cum) {
   const int n_seq = p.a.kv.n_seq;
   const unsigned long long u = p.units_per_seq;
@@ -141,7 +141,7 @@ __device__ unsigned long long find_run(const DecodeArgs& p, int c, int G, int la
   }
   const int per = (n_seq + 31) / 32, s0 = min(n_seq, lane * per), s1 = min(n_seq, s0 + per);
   unsigned long long sum = 0;
-#pragma unroll 8
+#pragma unroll 4
   for (int s = s0; s < s1; ++s) {
     const uint32_t t = seq_tiles(p, p.a.seq_len[s]);
     if (t == 0 && c == 0) raise_error(p.a.err, kDevBadArgument);
@@ -159,6 +159,7 @@ __device__ unsigned long long find_run(const DecodeArgs& p, int c, int G, int la
   const uint32_t mine = __ballot_sync(0xffffffffu, target >= u * before && target < u * (before + sum));
   int s = s0;
   if (mine >> lane & 1)
+#pragma unroll 1
     for (uint32_t t; target >= u * (before + (t = seq_tiles(p, p.a.seq_len[s]))); ++s) before += t;
   const int from = mine ? __ffs(mine) - 1 : 0;   // none: the run is empty
   *seq = __shfl_sync(0xffffffffu, s, from);
@@ -169,25 +170,32 @@ __device__ unsigned long long find_run(const DecodeArgs& p, int c, int G, int la
 // A finished row: output and log-sum-exp, or for the shared-prefix join what they
 // are made of.
 template <typename T, int D>
-__device__ __forceinline__ void finish_row(const DecodeArgs& p, int seq, int head, const float (&v)[D / 32], float M,
-                                           float sum, int lane) {
+__device__ __noinline__ void finish_row(const DecodeArgs& p, int seq, int head, float4 v, float M, float sum, int lane) {
   if (!p.own_o) {
     write_row<T, D>(p.a, seq, head, v, M, sum, lane);
     return;
   }
   const long long row = (long long)seq * p.a.n_heads + head;
-#pragma unroll
-  for (int k = 0; k < D / 32; ++k) p.own_o[row * D + D / 32 * lane + k] = v[k];
+  if constexpr (D == 128) reinterpret_cast<float4*>(p.own_o)[row * 32 + lane] = v;
+  else reinterpret_cast<float2*>(p.own_o)[row * 32 + lane] = make_float2(v.x, v.y);
   if (lane == 0) p.own_ml[row] = make_float2(M, sum);
+}
+// The same into a partial slot (in units of heads).
+template <int D>
+__device__ __forceinline__ void store_partial(const DecodeArgs& p, int at, float4 v, float M, float sum, int lane) {
+  if constexpr (D == 128) reinterpret_cast<float4*>(p.part_o)[(long long)at * 32 + lane] = v;
+  else reinterpret_cast<float2*>(p.part_o)[(long long)at * 32 + lane] = make_float2(v.x, v.y);
+  if (lane == 0) reinterpret_cast<float2*>(p.part_ml)[at] = make_float2(M, sum);
 }
 // Joins n <= 32 partials of every head of a unit, pieces first, first + step, .. (four
 // warps, two heads of each at a time so that their loads are one round trip): into
 // the output rows, or into the first piece's slot.
 template <typename T, int D>
-__device__ void join_pieces(const DecodeArgs& p, const CutPiece& u, int G, int first, int step, int n, bool final,
+__device__ __noinline__ void join_pieces(const DecodeArgs& p, const CutPiece& u, int G, int first, int step, int n, bool final,
                             int warp, int lane) {
   constexpr int V = D / 32, HB = 2;
   const int slot = lane < n ? piece_slot(u, first + lane * step, G) * kMaxSlotHeads : 0;
+#pragma unroll 1
   for (int h0 = warp; h0 < u.heads; h0 += HB * kWarps) {
     float2 ml[HB];
     float v[HB][V], f[HB], M[HB], sum[HB];
@@ -199,6 +207,7 @@ __device__ void join_pieces(const DecodeArgs& p, const CutPiece& u, int G, int f
 #pragma unroll
       for (int k = 0; k < V; ++k) v[b][k] = 0.f;
     }
+#pragma unroll 1
     for (int i0 = 0; i0 < n; i0 += 4) {
       float x[4][HB][V];
 #pragma unroll
@@ -231,24 +240,18 @@ __device__ void join_pieces(const DecodeArgs& p, const CutPiece& u, int G, int f
     for (int b = 0; b < HB; ++b) {
       const int hh = h0 + b * kWarps;
       if (hh >= u.heads) continue;
-      if (final) {
-        finish_row<T, D>(p, u.seq, u.head + hh, v[b], M[b], sum[b], lane);
-      } else {
-        const long long at = __shfl_sync(0xffffffffu, slot, 0) + hh;
-#pragma unroll
-        for (int k = 0; k < V; ++k) p.part_o[at * D + V * lane + k] = v[b][k];
-        if (lane == 0) reinterpret_cast<float2*>(p.part_ml)[at] = make_float2(M[b], sum[b]);
-      }
+      if (final) finish_row<T, D>(p, u.seq, u.head + hh, as_float4(v[b]), M[b], sum[b], lane);
+      else store_partial<D>(p, __shfl_sync(0xffffffffu, slot, 0) + hh, as_float4(v[b]), M[b], sum[b], lane);
     }
   }
 }
 // Makes a count this call's, at 0, unless another CTA did.
-__device__ __forceinline__ void open_count(unsigned long long* count, unsigned long long tag) {
+__device__ __noinline__ void open_count(unsigned long long* count, unsigned long long tag) {
   const unsigned long long old = *(volatile unsigned long long*)count;
   if (old >> 16 != tag) atomicCAS(count, old, tag << 16);
 }
 // Counts an arrival; true for the last of `expected`, which leaves the count at 0.
-__device__ __forceinline__ bool arrive_last(unsigned long long* count, unsigned long long tag, int expected) {
+__device__ __noinline__ bool arrive_last(unsigned long long* count, unsigned long long tag, int expected) {
   __threadfence();
   unsigned long long now = atomicAdd(count, 1ull) + 1;
   while (now >> 16 != tag) {   // not opened yet: what was there is another call's
@@ -324,7 +327,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     uint32_t L = t < t1 ? a.seq_len[seq] : 0, ts = t < t1 ? seq_tiles(p, L) : 0;
     int cached_unit = -1, cached_base = 0, col = -1, page = -1;   // lane i: list / table entry cached_base + i
     bool alive = true;
+#pragma unroll 1
     while (t < t1 && alive) {
+#pragma unroll 1
       while (ts == 0 || t >= p.units_per_seq * (cum + ts)) {
         cum += ts;
         L = a.seq_len[++seq];
@@ -371,6 +376,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       const int n_entries = a.list ? a.n_list : (int)((L + P - 1) >> a.page_shift);
       const int unit_id = a.list ? seq * (int)a.kv.n_kv_heads + h : seq;   // one table row serves all heads
       bool first = true;
+#pragma unroll 1
       for (uint32_t tile = tile0; tile < tile1; ++tile) {
         // this lane's box: positions box_pos .. + box_rows - 1 of the unit
         const int b = lane % boxes;
@@ -448,8 +454,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     }
     __syncwarp();
     // Every issued copy lands before the CTA may exit.
+#pragma unroll 1
     for (uint32_t j = drained; j < it; ++j)
       paged_wait(&s.full[j % ST], (j / ST) & 1, &s.abort, a.err, false);
+#pragma unroll 1
     for (uint32_t j = pieces > (uint32_t)QS ? pieces - QS : 0; j < pieces; ++j)
       paged_wait(&s.qfull[j % QS], (j / QS) & 1, &s.abort, a.err, false);
     return;
@@ -468,6 +476,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     if (lane == 0) mbar_arrive(&s.joined);
     return __all_sync(0xffffffffu, paged_wait(&s.joined, joins++ & 1, &s.abort, a.err));
   };
+#pragma unroll 1
   for (uint32_t it = 0;; ++it) {
     const int st = it % ST;
     if (!__all_sync(0xffffffffu, paged_wait(&s.full[st], (it / ST) & 1, &s.abort, a.err))) return;
@@ -638,6 +647,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         }
       }
     if (!join()) return;
+#pragma unroll 1
     for (int head = warp; head < u.heads && u.dest != -2; head += kWarps) {
       constexpr int V = D / 32;   // elements of this lane
       float M = -INFINITY, sum = 0.f, v[V];
@@ -652,14 +662,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
 #pragma unroll
         for (int k = 0; k < V; ++k) v[k] += row[k];
       }
-      if (u.dest == -1) {
-        finish_row<T, D>(p, u.seq, u.head + head, v, M, sum, lane);
-      } else {
-        const long long slot = (long long)u.dest * kMaxSlotHeads + head;
-#pragma unroll
-        for (int k = 0; k < V; ++k) p.part_o[slot * D + V * lane + k] = v[k];
-        if (lane == 0) *reinterpret_cast<float2*>(p.part_ml + 2 * slot) = make_float2(M, sum);
-      }
+      if (u.dest == -1) finish_row<T, D>(p, u.seq, u.head + head, as_float4(v), M, sum, lane);
+      else store_partial<D>(p, u.dest * kMaxSlotHeads + head, as_float4(v), M, sum, lane);
     }
     fence_proxy_async();   // the rows before the next TMA write
     __syncwarp();
@@ -678,6 +682,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         min(kJoin, u.pieces - first));
   }
   if (!join()) return;
+#pragma unroll 1
   for (int k = 0; k < n_cut; ++k) {
     if (!s.last[k]) continue;
     const CutPiece& u = s.cut[k];

@@ -94,7 +94,7 @@ struct Pieces {
   const PrefixArgs& p;
   int c, G, unit, w, h, pair, i0, i1, id;
   __device__ __forceinline__ Pieces(const PrefixArgs& p, int c, int G) : p(p), c(c), G(G), unit(-1) {}
-  __device__ __forceinline__ bool next() {
+  __device__ __noinline__ bool next() {
     if (p.share2) {
       if (unit >= 0) return false;
       const int per_head = p.tiles / 2 * p.share2 + (p.tiles & 1) * p.share1;
@@ -105,8 +105,8 @@ struct Pieces {
       w = unit_weight(p, pair);
       const int part = rest - pair * p.share2, parts = w == 2 ? p.share2 : p.share1;
       unit = h * p.pairs + pair;
-      i0 = (int)divide((unsigned long long)p.steps * part, parts);
-      i1 = (int)divide((unsigned long long)p.steps * (part + 1), parts);
+      i0 = (int)((uint32_t)p.steps * (uint32_t)part / (uint32_t)parts);   // 2^17 steps, 2^8 parts at most
+      i1 = (int)((uint32_t)p.steps * (uint32_t)(part + 1) / (uint32_t)parts);
       id = c;
       return i1 > i0;
     }
@@ -196,6 +196,14 @@ __device__ __forceinline__ void t5_ld32(uint32_t addr, uint32_t* v) {
       : T5_R32(v)
       : "r"(addr));
 }
+__device__ __forceinline__ void t5_ld16(uint32_t addr, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(addr));
+  for (int x = 16; x < 32; ++x) v[x] = 0;
+}
 __device__ __forceinline__ void t5_landed(uint32_t* v) {   // names the registers: no use of them moves before it
   asm volatile("tcgen05.wait::ld.sync.aligned;" : T5_RW32(v)::"memory");
 }
@@ -219,6 +227,12 @@ __device__ __forceinline__ void t5_scale8(uint32_t addr, float f) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(v[0]), "r"(v[1]),
                "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(addr)
                : "memory");
+}
+// Sixteen columns, those from `valid` on overwritten with `none`.
+__device__ __forceinline__ void t5_mask16(uint32_t addr, int valid, uint32_t none) {
+#pragma unroll 1
+  for (int x = max(valid, 0); x < 16; ++x)
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(addr + x), "r"(none) : "memory");
 }
 __device__ __forceinline__ void t5_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -426,14 +440,23 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       const int cnt = w == 2 ? n : i == 0 ? (n + 1) / 2 : n / 2;
       // this thread's half row of Q into shared memory
       const int r = (2 * pair + (w == 2 ? i : 0)) * kRows + row;   // of the kv head's rows
+      // (a warp takes 16 whole rows of the stream's 128, lanes side by side)
       if (cnt > 0) {
-        const int seq = r / p.group, j = r % p.group;
-        const uint4* src = reinterpret_cast<const uint4*>(a.q + (long long)seq * a.q_stride + (long long)(h * p.group + j) * D);
+        constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes, kLoads = 16 / kAtOnce;   // lanes of a row, rows of a load
+        const int row0 = ((warp >> 2 & 1) * 4 + (warp & 3)) * 16, x = lane % kLanes;
+        // lane l < 16 finds row l's place
+        const int r_of = r - row + row0 + (lane & 15);
+        const long long at = r_of < p.rows ? (long long)(r_of / p.group) * a.q_stride + (long long)(h * p.group + r_of % p.group) * D : -1;
+        uint4 v[kLoads];
 #pragma unroll
-        for (int x0 = 0; x0 < D / 16; ++x0) {
-          const int x = x0 + D / 16 * half;
-          const uint4 v = r < p.rows ? src[x] : make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<uint4*>(s.q[i] + (x >> 3) * kRows * 128 + row * 128 + (((x & 7) ^ (row & 7)) << 4)) = v;
+        for (int q = 0; q < kLoads; ++q) {
+          const long long src = __shfl_sync(0xffffffffu, at, q * kAtOnce + lane / kLanes);
+          v[q] = src >= 0 ? *reinterpret_cast<const uint4*>(a.q + src + 8 * x) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int q = 0; q < kLoads; ++q) {
+          const int rr = row0 + q * kAtOnce + lane / kLanes;
+          *reinterpret_cast<uint4*>(s.q[i] + (x >> 3) * kRows * 128 + rr * 128 + (((x & 7) ^ (rr & 7)) << 4)) = v[q];
         }
         fence_proxy_async();
         t5_before();
@@ -453,6 +476,12 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         const uint32_t groups = s.groups[(base + 2 * step) % kSlots] >> (4 * half);
         const int valid = (int)a.prefix_len - (i0 + step) * kPos - 64 * half;
         const bool whole = (groups & 15u) == 15u && valid >= 64;
+        if (!whole) {   // scores of what is not there never win: written back over S
+          const uint32_t none = __float_as_uint(p.scale_log2 < 0.f ? INFINITY : -INFINITY);
+#pragma unroll 1
+          for (int x = 0; x < 64; x += 16) t5_mask16(ts + x, groups >> (x / 16) & 1 ? valid - x : 0, none);
+          t5_stored();
+        }
         uint32_t w2[32];
         float add;
         // Weights against reference `off`, their sum, and the greatest score.
@@ -466,12 +495,6 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
             t5_landed(v + 32 * b);
-            if (!whole) {
-              const uint32_t none = __float_as_uint(p.scale_log2 < 0.f ? INFINITY : -INFINITY);
-#pragma unroll
-              for (int x = 32 * b; x < 32 * b + 32; ++x)
-                if (x >= valid || !(groups >> (x / 16) & 1)) v[x] = none;
-            }
 #pragma unroll
             for (int x = 32 * b; x < 32 * b + 32; x += 2) {
               const float s0 = __uint_as_float(v[x]) * p.scale_log2, s1 = __uint_as_float(v[x + 1]) * p.scale_log2;
@@ -530,15 +553,33 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         if (half == 0) sum += sums[0];
       }
       if (half == 0 && r < p.rows) p.part_ml[slot] = make_float2(ref, sum);
+      // O through this warp's 4 KB of the query tile, whose MMAs are done, so that rows
+      // go out in whole 128-byte lines.
+      if (cnt > 0) {
+        uint8_t* mine = s.q[i] + ((warp >> 2 & 1) * 4 + (warp & 3)) * (kRows * D * 2 / 8);
+        constexpr int kCols = D / 4;   // fp32 columns a round: 4 KB (2 KB) of 32 rows
+        static_assert(32 * kCols * 4 == kRows * D * 2 / 8, "a warp's share of the query tile");
+#pragma unroll 1
+        for (int q = 0; q < 2; ++q) {
+          uint32_t o[32];
+          if constexpr (kCols == 32) t5_ld32(to + kCols * q, o);
+          else t5_ld16(to + kCols * q, o);
+          t5_landed(o);
+          constexpr int kChunks = kCols / 4;
 #pragma unroll
-      for (int q = 0; q < D / 64 && cnt > 0; ++q) {
-        uint32_t o[32];
-        t5_ld32(to + 32 * q, o);
-        t5_landed(o);
-        if (r < p.rows) {
-          uint4* dst = reinterpret_cast<uint4*>(p.part_o + slot * D + D / 2 * half + 32 * q);
+          for (int x = 0; x < kChunks; ++x)
+            *reinterpret_cast<uint4*>(mine + lane * kCols * 4 + ((x ^ (lane & (kChunks - 1))) << 4)) =
+                make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+          __syncwarp();
+          const int rows_here = p.rows - (r - lane);   // of this warp's 32
 #pragma unroll
-          for (int x = 0; x < 8; ++x) dst[x] = make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+          for (int x = 0; x < kChunks; ++x) {
+            const int rr = x * (32 / kChunks) + lane / kChunks, ch = lane % kChunks;
+            const uint4 v = *reinterpret_cast<const uint4*>(mine + rr * kCols * 4 + ((ch ^ (rr & (kChunks - 1))) << 4));
+            if (rr < rows_here)
+              *reinterpret_cast<uint4*>(p.part_o + (slot - lane + rr) * D + D / 2 * half + kCols * q + 4 * ch) = v;
+          }
+          __syncwarp();
         }
       }
       t5_before();
@@ -620,7 +661,7 @@ __global__ void __launch_bounds__(256) k_prefix_join(const __grid_constant__ Pre
     }
   }
   if (L > a.kv.max_pages * a.kv.page_size) return;   // reported by the own-positions kernel
-  write_row<T, D>(a, seq, head, v, M, sum, lane);
+  write_row<T, D>(a, seq, head, as_float4(v), M, sum, lane);
 }
 
 template <typename T, int D>

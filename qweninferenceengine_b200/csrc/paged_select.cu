@@ -152,7 +152,7 @@ struct ListSmem {
 
 // Exclusive sum over the CTA's threads of v (and the total), packed or not.
 template <typename V>
-__device__ __forceinline__ V exclusive_sum(V v, V* warp_sums, V* total) {
+__device__ __noinline__ V exclusive_sum(V v, V* warp_sums, V* total) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   V inc = v;
 #pragma unroll
@@ -232,6 +232,7 @@ __global__ void __launch_bounds__(kListThreads) k_page_list(const __grid_constan
       for (int i = tid; i < kBins; i += kListThreads) sm.bins[i] = 0;
       if (tid == 0) sm.count = 0;
       __syncthreads();
+#pragma unroll 4
       for (int i = tid; i < m; i += kListThreads) {
         const u64 x = keys[i];
         if (x >= lo && x <= hi) atomicAdd(&sm.bins[(x - lo) >> shift], 1u);
@@ -265,6 +266,7 @@ __global__ void __launch_bounds__(kListThreads) k_page_list(const __grid_constan
         break;
       }
       if (held <= kRank) {    // rank them: higher key first, then lower page
+#pragma unroll 1
         for (int i = tid; i < m; i += kListThreads) {
           const u64 x = keys[i];
           if (x >= lo && x <= hi) {
@@ -278,6 +280,7 @@ __global__ void __launch_bounds__(kListThreads) k_page_list(const __grid_constan
           const u64 x = sm.rank_key[tid];
           const int at = sm.rank_at[tid];
           uint32_t rank = 0, same = 0;
+#pragma unroll 1
           for (uint32_t j = 0; j < held; ++j) {
             rank += sm.rank_key[j] > x || (sm.rank_key[j] == x && sm.rank_at[j] < at);
             same += sm.rank_key[j] == x && sm.rank_at[j] <= at;
@@ -299,15 +302,19 @@ __global__ void __launch_bounds__(kListThreads) k_page_list(const __grid_constan
   // (keys above the cut, keys equal to it).
   const int per = (m + kListThreads - 1) / kListThreads, i0 = min(m, tid * per), i1 = min(m, i0 + per);
   u64 mine = 0, total;
+#pragma unroll 1
   for (int i = i0; i < i1; ++i) mine += keys[i] > cut ? 1ull << 32 : keys[i] == cut ? 1ull : 0ull;
   const u64 before = exclusive_sum(mine, sm.warp_pair, &total);
   uint32_t equal = (uint32_t)before;
   int at = a.n_first + (int)(before >> 32) + (int)min(equal, ties);
+#pragma unroll 1
   for (int i = i0; i < i1; ++i) {
     const bool take = keys[i] > cut || (keys[i] == cut && equal++ < ties);
     if (take) list[at++] = first + i;
   }
+#pragma unroll 1
   for (int i = tid; i < a.n_first; i += kListThreads) list[i] = i;
+#pragma unroll 1
   for (int i = tid; i < a.n_last; i += kListThreads) list[a.n_select - a.n_last + i] = end + i;
 }
 
