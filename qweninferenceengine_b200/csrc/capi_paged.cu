@@ -78,6 +78,11 @@ int attention(const char* op, PagedAttnArgs& a, const qwen_paged_kv* kv, const u
   QWEN_TRY(check_rows(op, "out", out, out_stride, n_heads * kv->head_dim));
   if (!seq_len) return set_error(QWEN_ERR_INVALID_ARGUMENT, "%s: null seq_len", op);
   QWEN_TRY(check_workspace(op, workspace, workspace_bytes, need));
+  if (!paged_decode_fits(*kv, (int)n_heads, a.n_list))
+    return set_error(QWEN_ERR_INVALID_ARGUMENT,
+                     "%s: %u sequences of %u kv heads and up to %llu positions are more than one call takes", op,
+                     kv->n_seq, kv->n_kv_heads,
+                     (unsigned long long)(a.n_list ? a.n_list : kv->max_pages) * kv->page_size);
   a.kv = *kv;
   a.q = q;
   a.q_stride = q_stride;

@@ -37,6 +37,8 @@ struct PagedAttnArgs {
 // launch failure.  own_o, own_ml: where set, unnormalised rows and (max, sum) per
 // query head go there instead of outputs.
 int launch_paged_decode(const PagedAttnArgs& a, cudaStream_t st, float* own_o = nullptr, float2* own_ml = nullptr);
+// Whether its tiles can be counted in 31 bits; n_list: listed pages, 0 without a list.
+bool paged_decode_fits(const qwen_paged_kv& kv, int n_heads, int n_list);
 size_t paged_decode_workspace(const qwen_paged_kv& kv, int n_heads);
 // The same over a shared prefix (prefix_len > 0) and own pages (paged_prefix.cu).
 int launch_paged_prefix(const PagedAttnArgs& a, cudaStream_t st);

@@ -36,8 +36,10 @@
 // 2^-8, averaged over positions); sums, maxima and outputs are fp32.
 #include <cudaTypedefs.h>
 
+#include <algorithm>
 #include <atomic>
 #include <chrono>
+#include <cmath>
 #include <mutex>
 
 #include "paged_common.cuh"
@@ -97,6 +99,7 @@ struct DecodeArgs {
   PagedAttnArgs a;
   int units_per_seq;        // kv heads x chunks of at most 16 query heads
   int chunks;               // chunks per kv head
+  int group;                // query heads per kv head
   int list_tiles;           // tiles of a listed unit
   float scale_log2;
   float* part_o;            // [2 G][16][D]
@@ -113,57 +116,67 @@ __device__ __forceinline__ uint32_t seq_tiles(const DecodeArgs& p, uint32_t L) {
   return L ? (L + kTile - 1) / kTile : 1;   // an empty sequence still has its zeros written
 }
 
-__device__ __forceinline__ unsigned long long run_start(unsigned long long total, int c, int G) {
-  return divide(total * (unsigned)c, (unsigned)G);
+// total < 2^31 (the entry points refuse more).
+__device__ __forceinline__ uint32_t run_start(uint32_t total, uint32_t c, uint32_t G) {
+  const uint32_t q = total / G;
+  return q * c + (total - q * G) * c / G;   // = total c / G, in 32 bits
 }
 // The run that holds tile x: the largest c with run_start(c) <= x.
-__device__ __forceinline__ int run_of(unsigned long long total, unsigned long long x, int G) {
-  return (int)divide((x + 1) * G - 1, total);
+__device__ __forceinline__ int run_of(uint32_t total, uint32_t x, uint32_t G) {
+  return (int)divide((unsigned long long)(x + 1) * G - 1, total);
 }
 // The partial slot of piece i: runs follow one another, or (fewer tiles than runs)
 // each has one tile or none.
-__device__ __forceinline__ int piece_slot(const CutPiece& u, int i, int G) {
+__device__ __noinline__ int piece_slot(const CutPiece& u, int i, int G) {
   const int r = u.total < (unsigned)G ? run_of(u.total, u.begin + i, G) : u.run0 + i;
   return 2 * r + (i == 0 ? 1 : 0);
 }
 
 // Total number of tiles, and the sequence that holds tile run_start(total, c) with
-// the number of tiles per unit before it and its length (one warp).
-__device__ __forceinline__ unsigned long long find_run(const DecodeArgs& p, int c, int G, int lane, int* seq,
-                                       unsigned long long* cum) {
+// its length and the number of tiles before it (one warp).
+__device__ __forceinline__ uint32_t find_run(const DecodeArgs& p, uint32_t c, uint32_t G, int lane, int* seq,
+                                             uint32_t* before, uint32_t* length) {
   const int n_seq = p.a.kv.n_seq;
-  const unsigned long long u = p.units_per_seq;
+  const uint32_t u = p.units_per_seq;
   if (p.a.list) {
-    const unsigned long long total = u * p.list_tiles * n_seq;
-    *seq = (int)divide(run_start(total, c, G), u * p.list_tiles);
-    *cum = (unsigned long long)*seq * p.list_tiles;
+    const uint32_t total = u * p.list_tiles * n_seq;
+    *seq = min((int)(run_start(total, c, G) / (u * p.list_tiles)), n_seq - 1);
+    *before = (uint32_t)*seq * u * p.list_tiles;
+    *length = p.a.seq_len[*seq];
     return total;
   }
   const int per = (n_seq + 31) / 32, s0 = min(n_seq, lane * per), s1 = min(n_seq, s0 + per);
-  unsigned long long sum = 0;
+  uint32_t sum = 0, L = 0;
 #pragma unroll 4
   for (int s = s0; s < s1; ++s) {
-    const uint32_t t = seq_tiles(p, p.a.seq_len[s]);
+    L = p.a.seq_len[s];
+    const uint32_t t = seq_tiles(p, L);
     if (t == 0 && c == 0) raise_error(p.a.err, kDevBadArgument);
     sum += t;
   }
-  unsigned long long inc = sum;
+  uint32_t inc = sum * u;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const unsigned long long v = __shfl_up_sync(0xffffffffu, inc, o);
+    const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
     if (lane >= o) inc += v;
   }
-  unsigned long long before = inc - sum;
-  const unsigned long long total = u * __shfl_sync(0xffffffffu, inc, 31);
-  const unsigned long long target = run_start(total, c, G);
-  const uint32_t mine = __ballot_sync(0xffffffffu, target >= u * before && target < u * (before + sum));
+  const uint32_t total = __shfl_sync(0xffffffffu, inc, 31), target = run_start(total, c, G);
+  uint32_t at = inc - sum * u;
+  const uint32_t mine = __ballot_sync(0xffffffffu, target >= at && target < inc);
   int s = s0;
-  if (mine >> lane & 1)
+  if (per > 1 && mine >> lane & 1) {
 #pragma unroll 1
-    for (uint32_t t; target >= u * (before + (t = seq_tiles(p, p.a.seq_len[s]))); ++s) before += t;
+    for (;; ++s) {
+      L = p.a.seq_len[s];
+      const uint32_t t = seq_tiles(p, L) * u;
+      if (target < at + t) break;
+      at += t;
+    }
+  }
   const int from = mine ? __ffs(mine) - 1 : 0;   // none: the run is empty
   *seq = __shfl_sync(0xffffffffu, s, from);
-  *cum = __shfl_sync(0xffffffffu, before, from);
+  *before = __shfl_sync(0xffffffffu, at, from);
+  *length = __shfl_sync(0xffffffffu, L, from);
   return total;
 }
 
@@ -314,63 +327,39 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
 
   if (warp == kWarps) {
     // ------------------------------------------------------------ producer --
+    // What a CTA does before its first load is on the path of every call: 32-bit
+    // arithmetic, lengths handed on by shuffles, pieces described only after their loads.
     const int P = a.kv.page_size;
-    const int boxes = kTile / box_rows;                  // of K, and as many of V
-    const uint32_t box_bytes = (uint32_t)box_rows * D * 2;
-    const uint32_t capacity = a.kv.max_pages * a.kv.page_size;
+    const uint32_t box_bytes = (uint32_t)box_rows * D * 2, capacity = a.kv.max_pages * a.kv.page_size;
+    // lane l < 8: 16-position slice l % 4 of a tile, of K (l < 4) or of V; it loads the
+    // box that begins with its slice
+    const int slice = lane & (kWarps - 1), per_box = box_rows / 16;
+    const bool loads = lane < 2 * kWarps && slice % per_box == 0;
+    const uint32_t box_at = (uint32_t)slice / per_box * box_bytes;
     uint32_t it = 0, pieces = 0;
     int seq, n_cut = 0;
-    unsigned long long cum;
-    const unsigned long long total = find_run(p, c, G, lane, &seq, &cum);
-    const unsigned long long t1 = run_start(total, c + 1, G);
-    unsigned long long t = run_start(total, c, G);
-    uint32_t L = t < t1 ? a.seq_len[seq] : 0, ts = t < t1 ? seq_tiles(p, L) : 0;
-    int cached_unit = -1, cached_base = 0, col = -1, page = -1;   // lane i: list / table entry cached_base + i
+    uint32_t before, L;
+    const uint32_t total = find_run(p, c, G, lane, &seq, &before, &L);
+    const uint32_t t1 = run_start(total, c + 1, G);
+    uint32_t t = run_start(total, c, G), ts = seq_tiles(p, L);
+    int cached_unit = -1, cached_base = 0, page = -1, left = 0;   // lane i: entry cached_base + i
     bool alive = true;
 #pragma unroll 1
     while (t < t1 && alive) {
 #pragma unroll 1
-      while (ts == 0 || t >= p.units_per_seq * (cum + ts)) {
-        cum += ts;
+      while (t >= before + ts * p.units_per_seq) {
+        before += ts * p.units_per_seq;
         L = a.seq_len[++seq];
         ts = seq_tiles(p, L);
       }
-      const unsigned long long rel = t - p.units_per_seq * cum;
-      const uint32_t unit = (uint32_t)divide(rel, ts), tile0 = (uint32_t)(rel - (unsigned long long)unit * ts);
-      const unsigned long long begin = t - tile0;
-      const uint32_t tile1 = (uint32_t)min((unsigned long long)ts, tile0 + (t1 - t));
+      const uint32_t unit = (t - before) / ts, begin = before + unit * ts, tile0 = t - begin;
+      const uint32_t tile1 = min(ts, tile0 + (t1 - t));
       t += tile1 - tile0;
-      const int h = (int)unit / p.chunks, chunk = (int)unit % p.chunks;
-      const int group = a.n_heads / (int)a.kv.n_kv_heads;
-      const int head = h * group + chunk * kMaxSlotHeads, heads = min(kMaxSlotHeads, group - chunk * kMaxSlotHeads);
+      const int h = p.chunks == 1 ? (int)unit : (int)unit / p.chunks, chunk = (int)unit - h * p.chunks;
+      const int head = h * p.group + chunk * kMaxSlotHeads, heads = min(kMaxSlotHeads, p.group - chunk * kMaxSlotHeads);
       const bool fits = L <= capacity;
       if (!fits && lane == 0) raise_error(a.err, kDevBadArgument);
       const int dest = !fits ? -2 : tile0 == 0 && tile1 == ts ? -1 : 2 * c + (tile0 == 0 ? 1 : 0);
-      // the unit's queries
-      const int qs = pieces % QS;
-      if (pieces >= QS &&
-          !__all_sync(0xffffffffu, paged_wait(&s.qempty[qs], (pieces / QS - 1) & 1, &s.abort, a.err)))
-        break;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&s.qfull[qs], (uint32_t)heads * D * 2);
-        bulk_g2s(s.q[qs], a.q + (long long)seq * a.q_stride + (long long)head * D, (uint32_t)heads * D * 2, &s.qfull[qs]);
-      }
-      ++pieces;
-      if (dest >= 0) {
-        const int run0 = run_of(total, begin, G), unit_no = seq * p.units_per_seq + (int)unit;
-        CutPiece u;
-        u.seq = seq;
-        u.head = head;
-        u.heads = heads;
-        u.unit = unit_no;
-        u.pieces = total < (unsigned)G ? (int)ts : run_of(total, begin + ts - 1, G) - run0 + 1;
-        u.piece = total < (unsigned)G ? (int)tile0 : c - run0;
-        u.run0 = run0;
-        u.total = (uint32_t)min(total, (unsigned long long)G);
-        u.begin = (uint32_t)begin;
-        if (lane == 0) s.cut[n_cut] = u;
-        ++n_cut;
-      }
       const int32_t* table = a.kv.page_table + (long long)seq * a.kv.table_stride;
       const int32_t* list = a.list ? a.list + ((long long)seq * a.kv.n_kv_heads + h) * a.n_list : nullptr;
       const int n_entries = a.list ? a.n_list : (int)((L + P - 1) >> a.page_shift);
@@ -378,33 +367,31 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       bool first = true;
 #pragma unroll 1
       for (uint32_t tile = tile0; tile < tile1; ++tile) {
-        // this lane's box: positions box_pos .. + box_rows - 1 of the unit
-        const int b = lane % boxes;
-        const int box_pos = (int)tile * kTile + b * box_rows;
-        const int entry = box_pos >> a.page_shift, off = box_pos & (P - 1);
-        const int last_entry = ((int)tile * kTile + kTile - 1) >> a.page_shift;
         const int first_entry = ((int)tile * kTile) >> a.page_shift;
-        if (cached_unit != unit_id || first_entry < cached_base || last_entry >= cached_base + 32) {
+        if (cached_unit != unit_id || first_entry < cached_base ||
+            ((int)tile * kTile + kTile - 1) >> a.page_shift >= cached_base + 32) {
           cached_unit = unit_id;
           cached_base = first_entry;
+          // page of the pool, and how many of the sequence's positions begin with it
           const int e = cached_base + lane;
-          col = e < n_entries ? (list ? list[e] : e) : -1;
+          const int col = e < n_entries ? (list ? list[e] : e) : -1;
           page = -1;
+          left = 0;
           if (fits && col != -1) {
-            const bool in_table = col >= 0 && col < (int)a.kv.max_pages;
-            if (in_table && (uint32_t)col * P < L) page = table[col];
-            const bool bad = !in_table || ((uint32_t)col * P < L && (page < 0 || (uint32_t)page >= a.kv.n_pages));
-            if (bad) {
-              raise_error(a.err, kDevBadArgument);
-              page = -1;
+            bool bad = col < 0 || col >= (int)a.kv.max_pages;
+            if (!bad && (uint32_t)col * P < L) {
+              page = table[col];
+              bad = page < 0 || (uint32_t)page >= a.kv.n_pages;
+              if (!bad) left = (int)(L - (uint32_t)col * P);
             }
+            if (bad) raise_error(a.err, kDevBadArgument);
           }
         }
-        const int my_col = __shfl_sync(0xffffffffu, col, entry - cached_base);
-        const int my_page = __shfl_sync(0xffffffffu, page, entry - cached_base);
-        int rows = 0;   // positions of the box that count
-        if (my_page >= 0) rows = min(max((int)L - (my_col * P + off), 0), box_rows);
-        const uint32_t any = __ballot_sync(0xffffffffu, lane < boxes && rows > 0);
+        const int pos = (int)tile * kTile + 16 * slice, from = (pos >> a.page_shift) - cached_base;
+        const int off = pos & (P - 1);
+        const int valid = min(max(__shfl_sync(0xffffffffu, left, from) - off, 0), 16);   // of this slice's positions
+        const int my_page = __shfl_sync(0xffffffffu, page, from);
+        const uint32_t any = __ballot_sync(0xffffffffu, loads && valid > 0);
         const bool last = tile + 1 == tile1;
         if (!any && !last) continue;   // nothing of the tile is listed
         const int st = it % ST;
@@ -413,27 +400,56 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
           alive = false;
           break;
         }
-        // how many of each warp's 16 positions count
-        const int slice_rows = __shfl_sync(0xffffffffu, rows, (lane & (kWarps - 1)) * 16 / box_rows);
         StageMeta& meta = s.meta[st];
-        if (lane < kWarps) meta.valid[lane] = min(max(slice_rows - lane * 16 % box_rows, 0), 16);
+        if (lane < kWarps) meta.valid[lane] = valid;
         if (lane == 0) {
           meta.flags = (first ? kFirst : 0) | (last ? kLast : 0);
-          meta.seq = seq;
-          meta.head = head;
           meta.heads = heads;
-          meta.dest = dest;
+          if (last) {
+            meta.seq = seq;
+            meta.head = head;
+            meta.dest = dest;
+          }
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive_expect_tx(&s.full[st], 2 * box_bytes * __popc(any));
+        if (lane == 0) mbar_arrive_expect_tx(&s.full[st], box_bytes * __popc(any));
         __syncwarp();
-        if (lane < 2 * boxes && rows > 0)
-          tma_load_pages(s.kv[st][lane / boxes] + b * box_bytes, lane < boxes ? &tmk : &tmv, off, h, my_page,
-                         &s.full[st]);
-        first = false;
+        if (any >> lane & 1)
+          tma_load_pages(s.kv[st][lane / kWarps] + box_at, lane < kWarps ? &tmk : &tmv, off, h, my_page, &s.full[st]);
         ++it;
+        if (first) {   // the unit's queries, behind its first tile
+          first = false;
+          const int qs = pieces % QS;
+          if (pieces >= QS &&
+              !__all_sync(0xffffffffu, paged_wait(&s.qempty[qs], (pieces / QS - 1) & 1, &s.abort, a.err))) {
+            alive = false;
+            break;
+          }
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&s.qfull[qs], (uint32_t)heads * D * 2);
+            bulk_g2s(s.q[qs], a.q + (long long)seq * a.q_stride + (long long)head * D, (uint32_t)heads * D * 2,
+                     &s.qfull[qs]);
+          }
+          ++pieces;
+        }
+      }
+      if (dest >= 0) {
+        const int run0 = run_of(total, begin, G);
+        CutPiece u;
+        u.seq = seq;
+        u.head = head;
+        u.heads = heads;
+        u.unit = seq * p.units_per_seq + (int)unit;
+        u.pieces = total < (unsigned)G ? (int)ts : run_of(total, begin + ts - 1, G) - run0 + 1;
+        u.piece = total < (unsigned)G ? (int)tile0 : c - run0;
+        u.run0 = run0;
+        u.total = min(total, (uint32_t)G);
+        u.begin = begin;
+        if (lane == 0) s.cut[n_cut] = u;
+        ++n_cut;
       }
     }
+    __syncwarp();
     if (lane < n_cut) {   // counts of the units it shares, opened while the last tiles are on their way
       const CutPiece& u = s.cut[lane];
       open_count(p.arrived + 2 * G + u.unit, p.tag);
@@ -775,6 +791,12 @@ int encode_pages_map(CUtensorMap* map, const qwen_paged_kv& kv, const uint16_t* 
              : -1;
 }
 
+bool paged_decode_fits(const qwen_paged_kv& kv, int n_heads, int n_list) {
+  const double units = (double)kv.n_seq * kv.n_kv_heads * units_per_head(kv, n_heads);
+  const double tiles = std::ceil((n_list ? n_list : (double)kv.max_pages) * kv.page_size / kTile);
+  return units * std::max(tiles, 1.0) < 2147483648.0;
+}
+
 size_t paged_decode_workspace(const qwen_paged_kv& kv, int n_heads) {
   if (kv.n_kv_heads == 0 || n_heads < (int)kv.n_kv_heads) return 0;   // refused later
   const size_t G = kCtasPerSm * paged_sm_count(), units = (size_t)kv.n_seq * kv.n_kv_heads * units_per_head(kv, n_heads);
@@ -785,6 +807,7 @@ int launch_paged_decode(const PagedAttnArgs& a, cudaStream_t st, float* own_o, f
   DecodeArgs p{};
   p.a = a;
   p.chunks = units_per_head(a.kv, a.n_heads);
+  p.group = a.n_heads / (int)a.kv.n_kv_heads;
   p.units_per_seq = (int)a.kv.n_kv_heads * p.chunks;
   p.list_tiles = (int)(((long long)a.n_list * a.kv.page_size + kTile - 1) / kTile);
   p.scale_log2 = a.scale * kLog2e;

@@ -95,6 +95,11 @@ def test_outputs_and_workspace(call):
     refused(call, kv(), "out must", os=-1536)
 
 
+def test_more_tiles_than_a_call_takes():
+    refused(paged, kv(n_seq=65535, n_kv_heads=1024, head_stride=128, max_pages=1 << 16, table_stride=1 << 16),
+            "more than one call", heads=1024, qs=131072, os=131072)
+
+
 def test_workspace_too_small_or_misaligned():
     s = kv()
     need = lib().qwen_select_pages_workspace(ctypes.byref(s))
