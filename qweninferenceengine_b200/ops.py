@@ -180,7 +180,12 @@ def uniform24(seed: int, sequence: int, step: int) -> int:
 
 
 # ---------------------------------------------------------- paged cache -----
+# A decode step's kernels take 2 to 25 us, and torch's and ctypes' share of a call as
+# much: these wrappers read each property of a tensor once and pass plain numbers on.
 _DTYPES = {torch.float16: QWEN_DTYPE_F16, torch.bfloat16: QWEN_DTYPE_BF16}
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") \
+    else lambda index: torch.cuda.current_stream(index).cuda_stream
+_workspace_bytes: dict = {}   # by sizes: the library's answers are functions of nothing else
 
 
 class PagedKV:
@@ -194,78 +199,96 @@ class PagedKV:
     select_pages); None keeps none.  The object holds references to the tensors and
     reads nothing of their contents; their shapes and addresses must not change."""
 
-    __slots__ = ("k_pages", "v_pages", "page_table", "bounds", "dtype", "device", "n_seq",
-                 "n_kv_heads", "head_dim", "struct", "ref")
+    __slots__ = ("k_pages", "v_pages", "page_table", "bounds", "dtype", "device", "index", "n_seq",
+                 "n_kv_heads", "head_dim", "page_size", "ref", "_struct")
 
     def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
                  bounds: torch.Tensor | None = None):
-        dtype, device = k_pages.dtype, k_pages.device
+        dtype, index = k_pages.dtype, k_pages.get_device()
         if dtype not in _DTYPES:
             raise ValueError(f"k_pages must be float16 or bfloat16, not {dtype}")
-        if not k_pages.is_cuda:
+        if index < 0:
             raise ValueError("expected a CUDA tensor")
-        if k_pages.dim() != 4:
+        shape, st = k_pages.shape, k_pages.stride()
+        if len(shape) != 4:
             raise ValueError("k_pages must be [n_pages, page_size, n_kv_heads, head_dim]")
-        n_pages, page_size, n_kv, dim = k_pages.shape
-        st = k_pages.stride()
-        if v_pages.shape != k_pages.shape or v_pages.stride() != st or v_pages.dtype != dtype:
+        if v_pages.shape != shape or v_pages.stride() != st or v_pages.dtype is not dtype:
             raise ValueError("k_pages and v_pages must have the same shape, strides and dtype")
+        n_pages, page_size, n_kv, dim = shape
         if st[3] != 1:
             raise ValueError("the elements of a head must be adjacent")
-        if page_table.dim() != 2 or page_table.dtype != torch.int32 or \
-                (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        table_shape, table_st = page_table.shape, page_table.stride()
+        if len(table_shape) != 2 or page_table.dtype is not torch.int32 or \
+                (table_shape[1] > 1 and table_st[1] != 1):
             raise ValueError("page_table must be int32 [n_seq, max_pages] with adjacent columns")
-        if v_pages.device != device or page_table.device != device:
+        if v_pages.get_device() != index or page_table.get_device() != index:
             raise ValueError("the cache's tensors must be on one device")
-        if bounds is not None and (bounds.shape != (n_pages, 2, n_kv, dim) or bounds.dtype != dtype
-                                   or not bounds.is_contiguous() or bounds.device != device):
+        if bounds is not None and (bounds.shape != (n_pages, 2, n_kv, dim) or bounds.dtype is not dtype
+                                   or not bounds.is_contiguous() or bounds.get_device() != index):
             raise ValueError("bounds must be a contiguous [n_pages, 2, n_kv_heads, head_dim] tensor "
                              "of the cache's dtype and device")
-        n_seq, max_pages = page_table.shape
+        n_seq, max_pages = table_shape
         self.k_pages, self.v_pages, self.page_table, self.bounds = k_pages, v_pages, page_table, bounds
-        self.dtype, self.device, self.n_seq = dtype, device, n_seq
-        self.n_kv_heads, self.head_dim = n_kv, dim
+        self.dtype, self.device, self.index, self.n_seq = dtype, k_pages.device, index, n_seq
+        self.n_kv_heads, self.head_dim, self.page_size = n_kv, dim, page_size
         # the stride of an axis of one element is never used: any valid value
-        self.struct = PagedKVStruct(
+        self._struct = PagedKVStruct(
             k_pages.data_ptr(), v_pages.data_ptr(), None if bounds is None else bounds.data_ptr(),
             page_table.data_ptr(), st[0] if n_pages > 1 else page_size * n_kv * dim, st[1],
             st[2] if n_kv > 1 else dim, n_pages, page_size, n_kv, dim, n_seq, max_pages,
-            page_table.stride(0) if n_seq > 1 else max_pages, _DTYPES[dtype])
-        self.ref = byref(self.struct)
+            table_st[0] if n_seq > 1 else max_pages, _DTYPES[dtype])
+        self.ref = byref(self._struct)
 
 
-def _rows(name: str, x: torch.Tensor, kv: PagedKV, n_rows: int | None, n_heads: int | None = None):
-    """(address, row stride) of a [rows, heads, head_dim] tensor whose rows are head-contiguous."""
-    if x.dtype != kv.dtype or x.device != kv.device:
+def _rows(name: str, x: torch.Tensor, kv: PagedKV, n_rows: int, n_heads: int) -> int:
+    """Row stride of a [n_rows, n_heads, head_dim] tensor whose rows are head-contiguous."""
+    shape, (row, head, el) = x.shape, x.stride() if x.dim() == 3 else (0, 0, 0)
+    dim = kv.head_dim
+    if shape != (n_rows, n_heads, dim):
+        raise ValueError(f"{name} has shape {tuple(shape)}: expected [{n_rows}, {n_heads}, {dim}]")
+    if x.dtype is not kv.dtype or x.get_device() != kv.index:
         raise ValueError(f"{name} must be {kv.dtype} on {kv.device}")
-    if x.dim() != 3 or x.shape[2] != kv.head_dim or (n_rows is not None and x.shape[0] != n_rows) or \
-            (n_heads is not None and x.shape[1] != n_heads):
-        raise ValueError(f"{name} has shape {tuple(x.shape)}: expected [{n_rows or 'rows'}, "
-                         f"{n_heads or 'heads'}, {kv.head_dim}]")
-    row, head, el = x.stride()
-    if el != 1 or (x.shape[1] > 1 and head != kv.head_dim):
+    if el != 1 or (head != dim and n_heads > 1):
         raise ValueError(f"{name}: the heads of a row must be adjacent")
-    return x.data_ptr(), row if x.shape[0] > 1 else x.shape[1] * kv.head_dim
+    return row if n_rows > 1 else n_heads * dim
 
 
-def _ints(name: str, x: torch.Tensor, kv: PagedKV, n: int | None) -> int:
+def _ints(name: str, x: torch.Tensor, kv: PagedKV, n: int) -> int:
     """Address of a contiguous int32 (or uint32) vector of n values."""
-    if x.dtype not in (torch.int32, torch.uint32) or x.device != kv.device or x.dim() != 1 or \
-            (n is not None and x.shape[0] != n) or not x.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int32 tensor"
-                         f"{'' if n is None else f' of {n} values'} on {kv.device}")
+    if (x.dtype is not torch.int32 and x.dtype is not torch.uint32) or x.get_device() != kv.index or \
+            x.shape != (n,) or not x.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of {n} values on {kv.device}")
     return x.data_ptr()
 
 
-def _on(kv: PagedKV, fn, *args) -> None:
-    """Calls a library entry on the cache's device and its current stream."""
-    index = kv.device.index
-    stream = torch._C._cuda_getCurrentRawStream(index)   # current_stream(index).cuda_stream, 3 us less
-    if index == torch.cuda.current_device():
-        check(fn(kv.ref, *args, stream))
+def _heads(q: torch.Tensor) -> int:
+    if q.dim() != 3:
+        raise ValueError(f"q has shape {tuple(q.shape)}: expected [rows, heads, head_dim]")
+    return q.shape[1]
+
+
+def _call(kv: PagedKV, fn, *args) -> None:
+    """A library entry on the cache's device and its current stream (appended)."""
+    index = kv.index
+    if index == torch._C._cuda_getDevice():
+        rc = fn(kv.ref, *args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            check(fn(kv.ref, *args, stream))
+            rc = fn(kv.ref, *args, _raw_stream(index))
+    if rc:
+        check(rc)
+
+
+def _workspace(kv: PagedKV, query: str, *sizes) -> tuple:
+    """(memory, bytes) that the library function `query` asks for."""
+    st = kv._struct
+    key = (query, kv.index, kv.n_seq, kv.n_kv_heads, kv.head_dim, st.max_pages, sizes)
+    need = _workspace_bytes.get(key)
+    if need is None:
+        if len(_workspace_bytes) > 4096:
+            _workspace_bytes.clear()
+        need = _workspace_bytes[key] = getattr(lib(), query)(kv.ref, *sizes)
+    return torch.empty(need, dtype=torch.uint8, device=kv.device), need
 
 
 def rope_append_paged(kv: PagedKV, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -281,38 +304,38 @@ def rope_append_paged(kv: PagedKV, q: torch.Tensor, k: torch.Tensor, v: torch.Te
     owns rows cu_tokens[s]:cu_tokens[s + 1], its last positions; rows behind the last
     sequence are not touched.  None: row s is sequence s's newest token, and a
     sequence of length 0 is passed over.  inv_freq: fp32 [rot_dim / 2]."""
-    n, heads = q.shape[0], q.shape[1]
-    qp, qs = _rows("q", q, kv, None)
-    kp, ks = _rows("k", k, kv, n, kv.n_kv_heads)
-    vp, vs = _rows("v", v, kv, n, kv.n_kv_heads)
+    heads, n = _heads(q), q.shape[0]
+    qs = _rows("q", q, kv, n, heads)
+    ks = _rows("k", k, kv, n, kv.n_kv_heads)
+    vs = _rows("v", v, kv, n, kv.n_kv_heads)
     if out is None:
         out = torch.empty((n, heads, kv.head_dim), dtype=kv.dtype, device=kv.device)
-    op, os_ = _rows("out", out, kv, n, heads)
-    if inv_freq.dtype != torch.float32 or inv_freq.device != kv.device or inv_freq.dim() != 1 or \
-            not inv_freq.is_contiguous():
+    os_ = _rows("out", out, kv, n, heads)
+    if inv_freq.dtype is not torch.float32 or inv_freq.get_device() != kv.index or \
+            inv_freq.dim() != 1 or not inv_freq.is_contiguous():
         raise ValueError(f"inv_freq must be a contiguous float32 vector on {kv.device}")
-    _on(kv, lib().qwen_rope_append_paged, qp, qs, kp, ks, vp, vs, op, os_, heads, n,
-        _ints("seq_len", seq_len, kv, kv.n_seq),
-        None if cu_tokens is None else _ints("cu_tokens", cu_tokens, kv, kv.n_seq + 1),
-        inv_freq.data_ptr(), 2 * inv_freq.shape[0], 1 if interleaved else 0)
+    _call(kv, lib().qwen_rope_append_paged, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
+          out.data_ptr(), os_, heads, n, _ints("seq_len", seq_len, kv, kv.n_seq),
+          None if cu_tokens is None else _ints("cu_tokens", cu_tokens, kv, kv.n_seq + 1),
+          inv_freq.data_ptr(), 2 * inv_freq.shape[0], 1 if interleaved else 0)
     return out
 
 
-def _attend(kv, fn, need: int, lead, q, seq_len, extra, scale, out, return_lse):
-    n, heads, dim = q.shape
-    qp, qs = _rows("q", q, kv, kv.n_seq)
+def _attend(kv, fn, query, sizes, lead, q, seq_len, extra, scale, out, return_lse):
+    n, heads = kv.n_seq, _heads(q)
+    qs = _rows("q", q, kv, n, heads)
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        op, os_ = out.data_ptr(), heads * dim
+        out, os_ = torch.empty_like(q, memory_format=torch.contiguous_format), heads * kv.head_dim
     else:
-        op, os_ = _rows("out", out, kv, n, heads)
+        os_ = _rows("out", out, kv, n, heads)
     lse = lp = None
     if return_lse:
         lse = torch.empty_strided((n, heads), (heads, 1), dtype=torch.float32, device=kv.device)
         lp = lse.data_ptr()
-    ws = torch.empty(need, dtype=torch.uint8, device=kv.device)
-    _on(kv, fn, *lead, qp, qs, op, os_, lp, heads, _ints("seq_len", seq_len, kv, kv.n_seq), *extra,
-        dim ** -0.5 if scale is None else scale, ws.data_ptr(), need)
+    ws, need = _workspace(kv, query, heads, *sizes)
+    _call(kv, fn, *lead, q.data_ptr(), qs, out.data_ptr(), os_, lp, heads,
+          _ints("seq_len", seq_len, kv, n), *extra,
+          kv.head_dim ** -0.5 if scale is None else scale, ws.data_ptr(), need)
     return (out, lse) if return_lse else out
 
 
@@ -322,9 +345,8 @@ def attention_paged(kv: PagedKV, q: torch.Tensor, seq_len: torch.Tensor, scale: 
     [n_seq, heads, d] against each sequence's seq_len positions.  scale defaults to
     d ** -0.5; lse is the natural log of the sum of exp(scale q K^T), [n_seq, heads]
     fp32.  A sequence of length 0 gives zeros and -inf."""
-    return _attend(kv, lib().qwen_attention_paged,
-                   lib().qwen_attention_paged_workspace(kv.ref, q.shape[1]), (), q, seq_len, (), scale,
-                   out, return_lse)
+    return _attend(kv, lib().qwen_attention_paged, "qwen_attention_paged_workspace", (), (), q, seq_len, (),
+                   scale, out, return_lse)
 
 
 def attention_prefix_paged(kv: PagedKV, q: torch.Tensor, seq_len: torch.Tensor,
@@ -334,12 +356,11 @@ def attention_prefix_paged(kv: PagedKV, q: torch.Tensor, seq_len: torch.Tensor,
     positions, held once in pool pages prefix_pages (int32), read once for the batch
     (qwen_attention_prefix_paged).  seq_len and the page table describe what follows
     the prefix."""
-    pages = _ints("prefix_pages", prefix_pages, kv, None)
-    if prefix_len < 0 or prefix_pages.shape[0] * kv.struct.page_size < prefix_len:
-        raise ValueError(f"prefix_len={prefix_len} in {prefix_pages.shape[0]} pages")
-    return _attend(kv, lib().qwen_attention_prefix_paged,
-                   lib().qwen_attention_prefix_paged_workspace(kv.ref, q.shape[1], prefix_len), (), q,
-                   seq_len, (pages, prefix_len), scale, out, return_lse)
+    pages = _ints("prefix_pages", prefix_pages, kv, prefix_pages.numel())
+    if prefix_len < 0 or prefix_pages.numel() * kv.page_size < prefix_len:
+        raise ValueError(f"prefix_len={prefix_len} in {prefix_pages.numel()} pages")
+    return _attend(kv, lib().qwen_attention_prefix_paged, "qwen_attention_prefix_paged_workspace",
+                   (prefix_len,), (), q, seq_len, (pages, prefix_len), scale, out, return_lse)
 
 
 def select_pages(kv: PagedKV, q: torch.Tensor, seq_len: torch.Tensor, n_select: int, n_first: int = 1,
@@ -351,17 +372,17 @@ def select_pages(kv: PagedKV, q: torch.Tensor, seq_len: torch.Tensor, n_select: 
     lower page."""
     if n_first < 0 or n_last < 0 or n_select < 1:
         raise ValueError(f"n_select={n_select} n_first={n_first} n_last={n_last}")
-    qp, qs = _rows("q", q, kv, kv.n_seq)
-    shape = (kv.n_seq, kv.n_kv_heads, n_select)
+    heads, n = _heads(q), kv.n_seq
+    qs = _rows("q", q, kv, n, heads)
+    shape = (n, kv.n_kv_heads, n_select)
     if out is None:
         out = torch.empty(shape, dtype=torch.int32, device=kv.device)
-    elif out.shape != shape or out.dtype != torch.int32 or out.device != kv.device or \
+    elif out.shape != shape or out.dtype is not torch.int32 or out.get_device() != kv.index or \
             not out.is_contiguous():
         raise ValueError(f"out must be a contiguous int32 tensor {shape} on {kv.device}")
-    need = lib().qwen_select_pages_workspace(kv.ref)
-    ws = torch.empty(need, dtype=torch.uint8, device=kv.device)
-    _on(kv, lib().qwen_select_pages, qp, qs, q.shape[1], _ints("seq_len", seq_len, kv, kv.n_seq),
-        n_select, n_first, n_last, out.data_ptr(), ws.data_ptr(), need)
+    ws, need = _workspace(kv, "qwen_select_pages_workspace")
+    _call(kv, lib().qwen_select_pages, q.data_ptr(), qs, heads, _ints("seq_len", seq_len, kv, n), n_select,
+          n_first, n_last, out.data_ptr(), ws.data_ptr(), need)
     return out
 
 
@@ -371,11 +392,10 @@ def attention_sparse_paged(kv: PagedKV, q: torch.Tensor, seq_len: torch.Tensor, 
     """attention_paged over the listed pages alone (qwen_attention_sparse_paged):
     pages int32 [n_seq, kv_heads, n], page-table columns, -1 for none (a
     select_pages result); only positions below seq_len count."""
-    if pages.dim() != 3 or pages.shape[:2] != (kv.n_seq, kv.n_kv_heads) or \
-            pages.dtype != torch.int32 or pages.device != kv.device or not pages.is_contiguous():
+    n = pages.shape[-1] if pages.dim() == 3 else 0
+    if pages.shape != (kv.n_seq, kv.n_kv_heads, n) or pages.dtype is not torch.int32 or \
+            pages.get_device() != kv.index or not pages.is_contiguous():
         raise ValueError(f"pages must be a contiguous int32 [{kv.n_seq}, {kv.n_kv_heads}, n] tensor "
                          f"on {kv.device}")
-    n = pages.shape[2]
-    return _attend(kv, lib().qwen_attention_sparse_paged,
-                   lib().qwen_attention_sparse_paged_workspace(kv.ref, q.shape[1], n),
+    return _attend(kv, lib().qwen_attention_sparse_paged, "qwen_attention_sparse_paged_workspace", (n,),
                    (pages.data_ptr(), n), q, seq_len, (), scale, out, return_lse)
