@@ -48,7 +48,7 @@ __device__ __forceinline__ float2 unpack2(__nv_bfloat16, uint32_t w) {
 // warp keeps one kv head's Q+- in registers; a group of D / 4 lanes reads a page's
 // bounds, lower half lo and upper half hi, 8 elements a lane.
 template <typename T, int D>
-__global__ void __launch_bounds__(kScoreWarps * 32) k_page_scores(const __grid_constant__ PagedSelectArgs a,
+__global__ void __launch_bounds__(kScoreWarps * 32, 2) k_page_scores(const __grid_constant__ PagedSelectArgs a,
                                                                   int pages_per_cta) {
   constexpr int kLanes = D / 4, kAtOnce = 32 / kLanes;   // lanes of a page, pages of a load
   pdl_wait();
@@ -70,6 +70,7 @@ __global__ void __launch_bounds__(kScoreWarps * 32) k_page_scores(const __grid_c
   const int part = lane & (kLanes - 1), sub = lane / kLanes;
   const bool upper = part >= kLanes / 2;
   const int d0 = 8 * (part & (kLanes / 2 - 1));
+#pragma unroll 1
   for (int h = warp / share; h < K; h += kScoreWarps / share) {
     double w[8];
     uint32_t used[4];   // bounds that no query multiplies read as 0 (they may be infinite)
@@ -91,20 +92,29 @@ __global__ void __launch_bounds__(kScoreWarps * 32) k_page_scores(const __grid_c
     u64* keys = reinterpret_cast<u64*>(a.scores) + ((long long)s * K + h) * a.kv.max_pages;
     const T* bounds = reinterpret_cast<const T*>(a.kv.bounds) + (upper ? (long long)K * D : 0) + (long long)h * D + d0;
     constexpr int kPages = kBatch * kAtOnce;
-    for (int p0 = begin + (warp % share) * kPages; p0 < end; p0 += share * kPages) {
-      int page = lane < kPages && p0 + lane < end ? table[p0 + lane] : 0;
-      const bool bad = page < 0 || (uint32_t)page >= a.kv.n_pages;
-      if (bad) {
-        raise_error(a.err, kDevBadArgument);
-        page = 0;
+    // One batch's bounds are on their way while the one before is summed, and the page
+    // numbers of the one after.
+    const int step = share * kPages, p_first = begin + (warp % share) * kPages;
+    auto page_of = [&](int p0) {   // lane i: page p0 + i of the sequence, or -1
+      int page = 0;
+      if (lane < kPages && p0 + lane < end) {
+        page = table[p0 + lane];
+        if (page < 0 || (uint32_t)page >= a.kv.n_pages) {
+          raise_error(a.err, kDevBadArgument);
+          page = -1;
+        }
       }
-      const uint32_t bads = __ballot_sync(0xffffffffu, bad);
-      uint4 x[kBatch];
+      return page;
+    };
+    auto fetch = [&](int page, uint4 (&x)[kBatch]) {
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
-        const long long at = __shfl_sync(0xffffffffu, page, i * kAtOnce + sub);
+        const long long at = max(__shfl_sync(0xffffffffu, page, i * kAtOnce + sub), 0);
         x[i] = __ldg(reinterpret_cast<const uint4*>(bounds + at * 2 * K * D));
       }
+    };
+    auto score = [&](int p0, int page, const uint4 (&x)[kBatch]) {
+      const uint32_t bads = __ballot_sync(0xffffffffu, page < 0);
       double sum[kBatch];
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
@@ -134,6 +144,21 @@ __global__ void __launch_bounds__(kScoreWarps * 32) k_page_scores(const __grid_c
       const int i = ((lane & 1) << 2) | (lane & 2) | ((lane & 4) >> 2);   // of the batch
       const int at = i * kAtOnce + sub;
       if (part < 8 && p0 + at < end) keys[p0 + at] = bads >> at & 1 ? 0 : score_key(sum[0]);
+    };
+    uint4 x0[kBatch], x1[kBatch];
+    int page0 = page_of(p_first), page1 = page_of(p_first + step);
+    fetch(page0, x0);
+#pragma unroll 1
+    for (int p0 = p_first; p0 < end; p0 += 2 * step) {
+      fetch(page1, x1);
+      const int next0 = page_of(p0 + 2 * step);
+      score(p0, page0, x0);
+      page0 = next0;
+      if (p0 + step >= end) break;
+      fetch(page0, x0);
+      const int next1 = page_of(p0 + 3 * step);
+      score(p0 + step, page1, x1);
+      page1 = next1;
     }
   }
 }
