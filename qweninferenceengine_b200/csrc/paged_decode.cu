@@ -19,11 +19,12 @@
 // long as streaming 128K positions).  Nothing waits for another CTA, and a call's
 // counts carry its own tag, so the workspace needs no zeroing.
 //
-// CTA: 4 consumer warps and a producer warp.  Per tile the producer's lanes read
-// list and page table (32 entries at a time), issue one TMA load per box of 16 or
-// 32 positions for K and for V (a 5-D map over the pool, so any stride order; the
-// 128-byte swizzle keeps fragment loads free of bank conflicts), and write how many
-// of each warp's 16 positions count.  Positions past a sequence's end and pages
+// CTA: 4 consumer warps and two producer warps, one for K and one for V (a lane's TMA
+// issue takes ~75 cycles and lanes take turns, so one warp with pages of 16 could not
+// keep up).  Per tile a producer's lanes read list and page table (32 entries at a
+// time) and issue one TMA load per box of 16 or 32 positions (a 5-D map over the
+// pool, so any stride order; the 128-byte swizzle keeps fragment loads free of bank
+// conflicts); K's also writes how many of each warp's 16 positions count.  Positions past a sequence's end and pages
 // outside the pool are never loaded or, inside a box, masked in registers.
 // Consumer warp w takes positions 16w..16w+15 of a tile on its own:
 //   S^T[16 pos x 8 heads] = K q^T, the softmax, o^T[d x 8] += V^T P^T
@@ -50,7 +51,7 @@ namespace {
 
 constexpr int kTile = 64;                     // positions of a tile
 constexpr int kWarps = kTile / 16;            // consumer warps
-constexpr int kThreads = (kWarps + 1) * 32;
+constexpr int kThreads = (kWarps + 2) * 32;
 constexpr int kCtasPerSm = 2;
 constexpr int kMaxSlotHeads = 16;             // query heads of a unit
 constexpr int kJoin = 16;                     // partials joined at once
@@ -151,7 +152,7 @@ __device__ __forceinline__ uint32_t find_run(const DecodeArgs& p, uint32_t c, ui
   for (int s = s0; s < s1; ++s) {
     L = p.a.seq_len[s];
     const uint32_t t = seq_tiles(p, L);
-    if (t == 0 && c == 0) raise_error(p.a.err, kDevBadArgument);
+    if (t == 0 && c == 0) raise_error(p.a.err, kDevBadArgument);   // (by both producers)
     sum += t;
   }
   uint32_t inc = sum * u;
@@ -305,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < ST; ++i) {
-      mbar_init(&s.full[i], 1);
+      mbar_init(&s.full[i], 2);   // both producers
       mbar_init(&s.empty[i], kWarps);
     }
     for (int i = 0; i < QS; ++i) {
@@ -325,16 +326,16 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   if (threadIdx.x == 0) pdl_launch_dependents();
   const int c = blockIdx.x, G = gridDim.x;
 
-  if (warp == kWarps) {
+  if (warp >= kWarps) {
     // ------------------------------------------------------------ producer --
     // What a CTA does before its first load is on the path of every call: 32-bit
     // arithmetic, lengths handed on by shuffles, pieces described only after their loads.
     const int P = a.kv.page_size;
     const uint32_t box_bytes = (uint32_t)box_rows * D * 2, capacity = a.kv.max_pages * a.kv.page_size;
-    // lane l < 8: 16-position slice l % 4 of a tile, of K (l < 4) or of V; it loads the
-    // box that begins with its slice
+    // lane l < 4: 16-position slice l of a tile; it loads the box that begins with it
+    const bool is_k = warp == kWarps;   // also writes what the consumers and the join read
     const int slice = lane & (kWarps - 1), per_box = box_rows / 16;
-    const bool loads = lane < 2 * kWarps && slice % per_box == 0;
+    const bool loads = lane < kWarps && slice % per_box == 0;
     const uint32_t box_at = (uint32_t)slice / per_box * box_bytes;
     uint32_t it = 0, pieces = 0;
     int seq, n_cut = 0;
@@ -401,8 +402,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
           break;
         }
         StageMeta& meta = s.meta[st];
-        if (lane < kWarps) meta.valid[lane] = valid;
-        if (lane == 0) {
+        if (is_k && lane < kWarps) meta.valid[lane] = valid;
+        if (is_k && lane == 0) {
           meta.flags = (first ? kFirst : 0) | (last ? kLast : 0);
           meta.heads = heads;
           if (last) {
@@ -415,10 +416,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         if (lane == 0) mbar_arrive_expect_tx(&s.full[st], box_bytes * __popc(any));
         __syncwarp();
         if (any >> lane & 1)
-          tma_load_pages(s.kv[st][lane / kWarps] + box_at, lane < kWarps ? &tmk : &tmv, off, h, my_page, &s.full[st]);
+          tma_load_pages(s.kv[st][is_k ? 0 : 1] + box_at, is_k ? &tmk : &tmv, off, h, my_page, &s.full[st]);
         ++it;
-        if (first) {   // the unit's queries, behind its first tile
-          first = false;
+        if (first && !is_k) {   // the unit's queries, behind its first tile
           const int qs = pieces % QS;
           if (pieces >= QS &&
               !__all_sync(0xffffffffu, paged_wait(&s.qempty[qs], (pieces / QS - 1) & 1, &s.abort, a.err))) {
@@ -432,8 +432,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
           }
           ++pieces;
         }
+        first = false;
       }
-      if (dest >= 0) {
+      if (dest >= 0 && is_k) {
         const int run0 = run_of(total, begin, G);
         CutPiece u;
         u.seq = seq;
@@ -462,8 +463,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       if (alive) {
         if (it >= ST) ++drained;
         if (lane == 0) {
-          s.n_cut = n_cut;
-          s.meta[st].flags = kEnd;
+          if (is_k) {
+            s.n_cut = n_cut;
+            s.meta[st].flags = kEnd;
+          }
           mbar_arrive(&s.full[st]);
         }
       }
