@@ -12,8 +12,9 @@
 // and end: a ragged batch, one long sequence and a batch of short ones all divide
 // evenly.  A unit within one CTA is finished there; a unit cut by a run's end
 // leaves fp32 partials (max, sum, unnormalised output), which are joined in run
-// order whoever joins them, so results do not depend on timing.  At the end of its
-// run a CTA counts in its pieces (two at most); the last to arrive at a unit joins up
+// order whoever joins them, so results do not depend on timing.  A CTA counts in its
+// pieces (two at most): the one its run began with while its last tiles are on their
+// way, the one its run ends with at the end; the last to arrive at a unit joins up
 // to 16 of them; of more, the last of each 16 joins those, and the last of the
 // joined ones the rest (one CTA reading 148 partials of six heads would take as
 // long as streaming 128K positions).  Nothing waits for another CTA, and a call's
@@ -89,9 +90,9 @@ struct __align__(1024) DecodeSmem {
   uint16_t q[query_slots<NT>()][8 * NT * D];
   float2 ml[2][kWarps][kMaxSlotHeads];   // by piece parity: maximum and sum of each warp
   StageMeta meta[stages<D>()];
-  uint64_t full[stages<D>()], empty[stages<D>()], qfull[query_slots<NT>()], qempty[query_slots<NT>()], joined;
+  uint64_t full[stages<D>()], empty[stages<D>()], qfull[query_slots<NT>()], qempty[query_slots<NT>()], joined, early;
   CutPiece cut[2];
-  int n_cut;
+  int n_cut, n_early;   // cut pieces; of those counted in before the end
   int last[2];
   int abort;
 };
@@ -279,6 +280,13 @@ __device__ __noinline__ bool arrive_last(unsigned long long* count, unsigned lon
   return last;
 }
 
+// Arrival of a piece at the first level of its join.
+__device__ __forceinline__ int arrive_first(const DecodeArgs& p, const CutPiece& u, int G) {
+  const int first = u.piece / kJoin * kJoin;
+  return arrive_last(u.pieces <= kJoin ? p.arrived + 2 * G + u.unit : p.arrived + piece_slot(u, first, G), p.tag,
+                     min(kJoin, u.pieces - first));
+}
+
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
@@ -314,6 +322,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       mbar_init(&s.qempty[i], kWarps);
     }
     mbar_init(&s.joined, kWarps);
+    mbar_init(&s.early, kWarps);
     s.abort = 0;
     fence_mbar_init();
     prefetch_map(&tmk);
@@ -333,7 +342,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     const int P = a.kv.page_size;
     const uint32_t box_bytes = (uint32_t)box_rows * D * 2, capacity = a.kv.max_pages * a.kv.page_size;
     // lane l < 4: 16-position slice l of a tile; it loads the box that begins with it
-    const bool is_k = warp == kWarps;   // also writes what the consumers and the join read
+    const bool is_k = warp == kWarps;   // K's also writes what the consumers read, V's what the join reads
     const int slice = lane & (kWarps - 1), per_box = box_rows / 16;
     const bool loads = lane < kWarps && slice % per_box == 0;
     const uint32_t box_at = (uint32_t)slice / per_box * box_bytes;
@@ -344,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     const uint32_t t1 = run_start(total, c + 1, G);
     uint32_t t = run_start(total, c, G), ts = seq_tiles(p, L);
     int cached_unit = -1, cached_base = 0, page = -1, left = 0;   // lane i: entry cached_base + i
-    bool alive = true;
+    bool alive = true, cut_first = false;
 #pragma unroll 1
     while (t < t1 && alive) {
 #pragma unroll 1
@@ -434,7 +443,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         }
         first = false;
       }
-      if (dest >= 0 && is_k) {
+      if (dest >= 0 && !is_k) {
         const int run0 = run_of(total, begin, G);
         CutPiece u;
         u.seq = seq;
@@ -447,14 +456,29 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         u.total = min(total, (uint32_t)G);
         u.begin = begin;
         if (lane == 0) s.cut[n_cut] = u;
+        if (pieces == 1) cut_first = true;
         ++n_cut;
       }
     }
     __syncwarp();
-    if (lane < n_cut) {   // counts of the units it shares, opened while the last tiles are on their way
-      const CutPiece& u = s.cut[lane];
-      open_count(p.arrived + 2 * G + u.unit, p.tag);
-      if (u.pieces > kJoin) open_count(p.arrived + piece_slot(u, u.piece / kJoin * kJoin, G), p.tag);
+    if (!is_k) {
+      // While the last tiles are on their way: the counts of the units it shares, and
+      // the arrival of a piece that is not the run's last.
+      if (lane < n_cut) {
+        const CutPiece& u = s.cut[lane];
+        open_count(p.arrived + 2 * G + u.unit, p.tag);
+        if (u.pieces > kJoin) open_count(p.arrived + piece_slot(u, u.piece / kJoin * kJoin, G), p.tag);
+      }
+      const int n_early = alive && n_cut > 0 && pieces > 1 && cut_first ? 1 : 0;
+      if (n_early) {
+        alive = __all_sync(0xffffffffu, paged_wait(&s.early, 0, &s.abort, a.err));
+        if (alive && lane == 0) s.last[0] = arrive_first(p, s.cut[0], G);
+      }
+      if (lane == 0) {
+        s.n_cut = n_cut;
+        s.n_early = n_early;
+      }
+      __syncwarp();
     }
     uint32_t drained = it >= (uint32_t)ST ? it - ST : 0;
     if (alive) {   // the end of the run, in a stage whose last copy was consumed
@@ -463,10 +487,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       if (alive) {
         if (it >= ST) ++drained;
         if (lane == 0) {
-          if (is_k) {
-            s.n_cut = n_cut;
-            s.meta[st].flags = kEnd;
-          }
+          if (is_k) s.meta[st].flags = kEnd;
           mbar_arrive(&s.full[st]);
         }
       }
@@ -686,20 +707,17 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     }
     fence_proxy_async();   // the rows before the next TMA write
     __syncwarp();
-    if (lane == 0) mbar_arrive(&s.empty[st]);
+    if (lane == 0) {
+      mbar_arrive(&s.empty[st]);
+      if (pieces == 1) mbar_arrive(&s.early);   // the run's first piece is written
+    }
   }
 
   // ---- the last pieces to arrive join the others'
-  const int n_cut = s.n_cut;
+  const int n_cut = s.n_cut, n_early = s.n_early;
   if (n_cut == 0) return;
   if (!join()) return;   // every warp's partials are written
-  if (threadIdx.x < n_cut) {
-    const CutPiece& u = s.cut[threadIdx.x];
-    const int first = u.piece / kJoin * kJoin;
-    s.last[threadIdx.x] = arrive_last(
-        u.pieces <= kJoin ? p.arrived + 2 * G + u.unit : p.arrived + piece_slot(u, first, G), p.tag,
-        min(kJoin, u.pieces - first));
-  }
+  if (threadIdx.x == 0 && n_early < n_cut) s.last[n_early] = arrive_first(p, s.cut[n_early], G);
   if (!join()) return;
 #pragma unroll 1
   for (int k = 0; k < n_cut; ++k) {
