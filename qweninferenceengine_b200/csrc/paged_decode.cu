@@ -6,8 +6,8 @@
 // 4 group flops a byte).  So the kernel is a stream of pages through shared
 // memory with just enough arithmetic beside it.
 //
-// Work: a unit is one (sequence, kv head, up to 16 query heads), a tile 64
-// positions of a unit.  All tiles of all units stand in one row, and CTA c of G
+// Work: a unit is one (sequence, kv head, up to 16 query heads), a tile 64 positions
+// of a unit (128 with head_dim 64).  All tiles of all units stand in one row, and CTA c of G
 // (two per SM) takes an equal run of them, start(c) = c T / G, wherever units begin
 // and end: a ragged batch, one long sequence and a batch of short ones all divide
 // evenly.  A unit within one CTA is finished there; a unit cut by a run's end
@@ -27,7 +27,7 @@
 // pool, so any stride order; the 128-byte swizzle keeps fragment loads free of bank
 // conflicts); K's also writes how many of each warp's 16 positions count.  Positions past a sequence's end and pages
 // outside the pool are never loaded or, inside a box, masked in registers.
-// Consumer warp w takes positions 16w..16w+15 of a tile on its own:
+// Consumer warp w takes positions 16w..16w+15 (and 64 behind) of a tile on its own:
 //   S^T[16 pos x 8 heads] = K q^T, the softmax, o^T[d x 8] += V^T P^T
 // with m16n8k16 MMAs (8 = the heads that share the kv head; tcgen05's smallest
 // M of 64 would be nine tenths padding), P^T turned by movmatrix.
@@ -50,8 +50,11 @@
 namespace qwen {
 namespace {
 
-constexpr int kTile = 64;                     // positions of a tile
-constexpr int kWarps = kTile / 16;            // consumer warps
+constexpr int kWarps = 4;                      // consumer warps
+// 16-position slices of a tile that a warp takes, and positions of a tile: 32 KB of K
+// and V either way (a tile costs the producers ~500 cycles whatever its size).
+constexpr int slices_of(int D) { return D == 64 ? 2 : 1; }
+constexpr int tile_of(int D) { return 16 * kWarps * slices_of(D); }
 constexpr int kThreads = (kWarps + 2) * 32;
 constexpr int kCtasPerSm = 2;
 constexpr int kMaxSlotHeads = 16;             // query heads of a unit
@@ -60,7 +63,7 @@ constexpr int kJoin = 16;                     // partials joined at once
 enum StageFlags { kFirst = 1, kLast = 2, kEnd = 4 };
 
 struct StageMeta {
-  int valid[kWarps];   // positions of each warp's 16 that count
+  int valid[8];        // positions of each 16 that count
   int flags;
   int seq, head, heads;   // the unit: sequence, first query head, query heads
   int dest;            // partial slot, or -1: the whole unit, or -2: nothing is written
@@ -73,10 +76,7 @@ struct CutPiece {
   uint32_t total, begin;           // fewer tiles than runs: their number, the unit's first
 };
 
-template <int D>
-constexpr int stages() {
-  return D == 128 ? 3 : 6;
-}
+constexpr int kStages = 3;
 
 // Queries in flight: of 16 heads two units', of 8 four.
 template <int NT>
@@ -86,11 +86,11 @@ constexpr int query_slots() {
 
 template <int D, int NT>
 struct __align__(1024) DecodeSmem {
-  uint8_t kv[stages<D>()][2][kTile * D * 2];
+  uint8_t kv[kStages][2][tile_of(D) * D * 2];
   uint16_t q[query_slots<NT>()][8 * NT * D];
   float2 ml[2][kWarps][kMaxSlotHeads];   // by piece parity: maximum and sum of each warp
-  StageMeta meta[stages<D>()];
-  uint64_t full[stages<D>()], empty[stages<D>()], qfull[query_slots<NT>()], qempty[query_slots<NT>()], joined, early;
+  StageMeta meta[kStages];
+  uint64_t full[kStages], empty[kStages], qfull[query_slots<NT>()], qempty[query_slots<NT>()], joined, early;
   CutPiece cut[2];
   int n_cut, n_early;   // cut pieces; of those counted in before the end
   int last[2];
@@ -103,6 +103,7 @@ struct DecodeArgs {
   int chunks;               // chunks per kv head
   int group;                // query heads per kv head
   int list_tiles;           // tiles of a listed unit
+  int tile_shift;           // positions of a tile: 1 << tile_shift
   float scale_log2;
   float* part_o;            // [2 G][16][D]
   float* part_ml;           // [2 G][16][2]
@@ -115,7 +116,7 @@ struct DecodeArgs {
 __device__ __forceinline__ uint32_t seq_tiles(const DecodeArgs& p, uint32_t L) {
   if (p.a.list) return p.list_tiles;
   if (L > p.a.kv.max_pages * p.a.kv.page_size) return 0;
-  return L ? (L + kTile - 1) / kTile : 1;   // an empty sequence still has its zeros written
+  return L ? ((L - 1) >> p.tile_shift) + 1 : 1;   // an empty sequence still has its zeros written
 }
 
 // total < 2^31 (the entry points refuse more).
@@ -307,7 +308,7 @@ template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     k_paged_decode(const __grid_constant__ DecodeArgs p, int box_rows,
                    const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv) {
-  constexpr int ST = stages<D>(), QS = query_slots<NT>();
+  constexpr int ST = kStages, SL = slices_of(D), kTile = tile_of(D), QS = query_slots<NT>();
   extern __shared__ uint8_t smem_raw[];
   DecodeSmem<D, NT>& s = *reinterpret_cast<DecodeSmem<D, NT>*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
   const PagedAttnArgs& a = p.a;
@@ -341,10 +342,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     // arithmetic, lengths handed on by shuffles, pieces described only after their loads.
     const int P = a.kv.page_size;
     const uint32_t box_bytes = (uint32_t)box_rows * D * 2, capacity = a.kv.max_pages * a.kv.page_size;
-    // lane l < 4: 16-position slice l of a tile; it loads the box that begins with it
+    // lane l < 4 (8): 16-position slice l of a tile; it loads the box that begins with it
     const bool is_k = warp == kWarps;   // K's also writes what the consumers read, V's what the join reads
-    const int slice = lane & (kWarps - 1), per_box = box_rows / 16;
-    const bool loads = lane < kWarps && slice % per_box == 0;
+    const int slice = lane & (kWarps * SL - 1), per_box = box_rows / 16;
+    const bool loads = lane < kWarps * SL && slice % per_box == 0;
     const uint32_t box_at = (uint32_t)slice / per_box * box_bytes;
     uint32_t it = 0, pieces = 0;
     int seq, n_cut = 0;
@@ -352,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     const uint32_t total = find_run(p, c, G, lane, &seq, &before, &L);
     const uint32_t t1 = run_start(total, c + 1, G);
     uint32_t t = run_start(total, c, G), ts = seq_tiles(p, L);
-    int cached_unit = -1, cached_base = 0, page = -1, left = 0;   // lane i: entry cached_base + i
+    int cached_unit = -1, cached_base = 0, page = -1, left = 0, next_page = -1;   // lane i: entry cached_base + i
     bool alive = true, cut_first = false;
 #pragma unroll 1
     while (t < t1 && alive) {
@@ -380,22 +381,25 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         const int first_entry = ((int)tile * kTile) >> a.page_shift;
         if (cached_unit != unit_id || first_entry < cached_base ||
             ((int)tile * kTile + kTile - 1) >> a.page_shift >= cached_base + 32) {
-          cached_unit = unit_id;
-          cached_base = first_entry;
           // page of the pool, and how many of the sequence's positions begin with it
-          const int e = cached_base + lane;
+          const int e = first_entry + lane;
+          const bool ahead = cached_unit == unit_id && !list && first_entry == cached_base + 32;
           const int col = e < n_entries ? (list ? list[e] : e) : -1;
           page = -1;
           left = 0;
           if (fits && col != -1) {
             bool bad = col < 0 || col >= (int)a.kv.max_pages;
             if (!bad && (uint32_t)col * P < L) {
-              page = table[col];
+              page = ahead ? next_page : table[col];
               bad = page < 0 || (uint32_t)page >= a.kv.n_pages;
               if (!bad) left = (int)(L - (uint32_t)col * P);
             }
             if (bad) raise_error(a.err, kDevBadArgument);
           }
+          cached_unit = unit_id;
+          cached_base = first_entry;
+          // the next 32 of the table row, asked for now
+          if (!list && e + 32 < n_entries) next_page = table[e + 32];
         }
         const int pos = (int)tile * kTile + 16 * slice, from = (pos >> a.page_shift) - cached_base;
         const int off = pos & (P - 1);
@@ -411,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
           break;
         }
         StageMeta& meta = s.meta[st];
-        if (is_k && lane < kWarps) meta.valid[lane] = valid;
+        if (is_k && lane < kWarps * SL) meta.valid[lane] = valid;
         if (is_k && lane == 0) {
           meta.flags = (first ? kFirst : 0) | (last ? kLast : 0);
           meta.heads = heads;
@@ -505,8 +509,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
 
   // -------------------------------------------------------------- consumers --
   const int g = lane >> 2, t4 = lane & 3;
-  const int box = 16 * warp / box_rows, row0 = 16 * warp % box_rows;
-  const uint32_t box_off = (uint32_t)box * box_rows * D * 2;
   const uint32_t half_bytes = (uint32_t)box_rows * 128;   // [half][rows][128 B] of a box
   uint32_t qf[NT][D / 8];
   float o[NT][D / 16][4], m[NT][2], l[NT][2];
@@ -521,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     const int st = it % ST;
     if (!__all_sync(0xffffffffu, paged_wait(&s.full[st], (it / ST) & 1, &s.abort, a.err))) return;
     const StageMeta& meta = s.meta[st];
-    const int flags = meta.flags, valid = meta.valid[warp];
+    const int flags = meta.flags;
     if (flags & kEnd) break;
     if (flags & kFirst) {
       const int qs = pieces % QS;
@@ -550,7 +552,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         for (int i = 0; i < D / 16; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
       }
     }
-    if (valid > 0) {
+#pragma unroll
+    for (int sl = 0; sl < SL; ++sl) {
+      const int valid = meta.valid[warp + kWarps * sl];
+      if (valid <= 0) continue;
+      const int first_row = 16 * (warp + kWarps * sl), row0 = first_row % box_rows;
+      const uint32_t box_off = (uint32_t)(first_row / box_rows) * box_rows * D * 2;
       const uint8_t* kb = s.kv[st][0] + box_off;
       const uint8_t* vb = s.kv[st][1] + box_off;
       // ---- S^T = K q^T.  Lane (g, t) holds 16-byte chunks 2t, 2t+1 of each half of
@@ -669,7 +676,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       }
     if (!join()) return;
     float* rows = reinterpret_cast<float*>(s.kv[st][0]);
-    static_assert(kWarps * 8 * NT * D * 4 <= 2 * kTile * D * 2, "the warps' rows exceed a stage");
+    static_assert(kWarps * 8 * NT * D * 4 <= 2 * tile_of(D) * D * 2, "the warps' rows exceed a stage");
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -814,7 +821,7 @@ int encode_pages_map(CUtensorMap* map, const qwen_paged_kv& kv, const uint16_t* 
 
 bool paged_decode_fits(const qwen_paged_kv& kv, int n_heads, int n_list) {
   const double units = (double)kv.n_seq * kv.n_kv_heads * units_per_head(kv, n_heads);
-  const double tiles = std::ceil((n_list ? n_list : (double)kv.max_pages) * kv.page_size / kTile);
+  const double tiles = std::ceil((n_list ? n_list : (double)kv.max_pages) * kv.page_size / tile_of((int)kv.head_dim));
   return units * std::max(tiles, 1.0) < 2147483648.0;
 }
 
@@ -830,7 +837,9 @@ int launch_paged_decode(const PagedAttnArgs& a, cudaStream_t st, float* own_o, f
   p.chunks = units_per_head(a.kv, a.n_heads);
   p.group = a.n_heads / (int)a.kv.n_kv_heads;
   p.units_per_seq = (int)a.kv.n_kv_heads * p.chunks;
-  p.list_tiles = (int)(((long long)a.n_list * a.kv.page_size + kTile - 1) / kTile);
+  p.tile_shift = a.kv.head_dim == 64 ? 7 : 6;
+  static_assert(tile_of(64) == 128 && tile_of(128) == 64, "tile_shift");
+  p.list_tiles = (int)(((long long)a.n_list * a.kv.page_size + (1 << p.tile_shift) - 1) >> p.tile_shift);
   p.scale_log2 = a.scale * kLog2e;
   const int G = kCtasPerSm * paged_sm_count();
   p.part_o = static_cast<float*>(a.workspace);

@@ -36,6 +36,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "paged_common.cuh"
 #include "qwen_internal.h"
@@ -57,7 +58,8 @@ struct PrefixArgs {
   int steps;                       // position tiles
   unsigned long long total;        // weighted steps of all units
   int share2, share1;              // CTAs of a unit of two tiles, of one; 0: runs over all units
-  float scale_log2;
+  float scale_log2;                // above 0: a negative scale's sign is put on the queries
+  uint32_t negate;                 // 0x80008000 then, else 0
   float* part_o;                   // [units + runs][2][128][D]
   float2* part_ml;                 // [units + runs][2][128]
   const float* own_o;              // [n_seq][n_heads][D]
@@ -213,6 +215,23 @@ __device__ __forceinline__ void t5_st32(uint32_t addr, const uint32_t* v) {
       "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::T5_IN32(v),
       "r"(addr)
       : "memory");
+}
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
 }
 // Eight columns times f, in place (few registers: the caller holds 64 scores).
 __device__ __forceinline__ void t5_scale8(uint32_t addr, float f) {
@@ -456,7 +475,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
 #pragma unroll
         for (int q = 0; q < kLoads; ++q) {
           const int rr = row0 + q * kAtOnce + lane / kLanes;
-          *reinterpret_cast<uint4*>(s.q[i] + (x >> 3) * kRows * 128 + rr * 128 + (((x & 7) ^ (rr & 7)) << 4)) = v[q];
+          const uint32_t m = p.negate;
+          *reinterpret_cast<uint4*>(s.q[i] + (x >> 3) * kRows * 128 + rr * 128 + (((x & 7) ^ (rr & 7)) << 4)) =
+              make_uint4(v[q].x ^ m, v[q].y ^ m, v[q].z ^ m, v[q].w ^ m);
         }
         fence_proxy_async();
         t5_before();
@@ -477,7 +498,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         const int valid = (int)a.prefix_len - (i0 + step) * kPos - 64 * half;
         const bool whole = (groups & 15u) == 15u && valid >= 64;
         if (!whole) {   // scores of what is not there never win: written back over S
-          const uint32_t none = __float_as_uint(p.scale_log2 < 0.f ? INFINITY : -INFINITY);
+          const uint32_t none = __float_as_uint(-INFINITY);
 #pragma unroll 1
           for (int x = 0; x < 64; x += 16) t5_mask16(ts + x, groups >> (x / 16) & 1 ? valid - x : 0, none);
           t5_stored();
@@ -489,7 +510,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
           uint32_t v[64];
           t5_ld32(ts, v);
           t5_ld32(ts + 32, v + 32);
-          float mx[4], part[4] = {0.f, 0.f, 0.f, 0.f};
+          float mx[4];
+          float2 part[2] = {};
 #pragma unroll
           for (int q = 0; q < 4; ++q) mx[q] = -INFINITY;
 #pragma unroll
@@ -497,16 +519,17 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
             t5_landed(v + 32 * b);
 #pragma unroll
             for (int x = 32 * b; x < 32 * b + 32; x += 2) {
-              const float s0 = __uint_as_float(v[x]) * p.scale_log2, s1 = __uint_as_float(v[x + 1]) * p.scale_log2;
-              mx[x / 2 & 3] = fmaxf(mx[x / 2 & 3], fmaxf(s0, s1));
-              const float e0 = exp2_fast(s0 - off), e1 = exp2_fast(s1 - off);
-              part[2 * (x / 2 & 1)] += e0;
-              part[2 * (x / 2 & 1) + 1] += e1;
-              w2[x / 2] = pack2(T{}, e0, e1);
+              const float2 s = make_float2(__uint_as_float(v[x]), __uint_as_float(v[x + 1]));
+              mx[x / 2 & 3] = fmaxf(mx[x / 2 & 3], fmaxf(s.x, s.y));
+              float2 e = fma2(s, make_float2(p.scale_log2, p.scale_log2), make_float2(-off, -off));
+              e.x = exp2_fast(e.x);
+              e.y = exp2_fast(e.y);
+              part[x / 2 & 1] = add2(part[x / 2 & 1], e);
+              w2[x / 2] = pack2(T{}, e.x, e.y);
             }
           }
-          add = (part[0] + part[1]) + (part[2] + part[3]);
-          return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          add = (part[0].x + part[0].y) + (part[1].x + part[1].y);
+          return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
         };
         // The reference holds for nearly every tile, so the weights are formed with it
         // while the maximum is still being found, and again where it had to move.
@@ -739,7 +762,9 @@ int launch_paged_prefix(const PagedAttnArgs& a, cudaStream_t st) {
   p.own_ml = reinterpret_cast<float2*>(ws + l.own_ml);
   p.part_o = reinterpret_cast<float*>(ws + l.part_o);
   p.part_ml = reinterpret_cast<float2*>(ws + l.part_ml);
-  p.scale_log2 = a.scale * kLog2e;
+  // (above 0, so that a masked score, -inf, stays one: products scaled so weigh alike)
+  p.scale_log2 = std::max(std::fabs(a.scale) * kLog2e, 1e-37f);
+  p.negate = a.scale < 0.f ? 0x80008000u : 0u;
   if (launch_paged_decode(a, st, reinterpret_cast<float*>(ws + l.own_o), reinterpret_cast<float2*>(ws + l.own_ml)) != 0)
     return -1;
   const int box_rows = a.kv.page_size < (uint32_t)kPos ? (int)a.kv.page_size : kPos;

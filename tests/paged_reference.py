@@ -108,7 +108,7 @@ def attention(cache, scale, lists=None, q=None):
             rows = slice(h * G, (h + 1) * G)
             x = q[i, rows].double()
             s = x @ k.T * scale
-            d = 2.0 ** -23 * (D * (x.abs() @ k.abs().T * scale).amax(-1) + 16 + 2 * s.abs().amax(-1))
+            d = 2.0 ** -23 * (D * (x.abs() @ k.abs().T * abs(scale)).amax(-1) + 16 + 2 * s.abs().amax(-1))
             w = torch.softmax(s, -1)
             out[i, rows] = w @ v
             L = k.shape[0]

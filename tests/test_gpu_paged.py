@@ -258,6 +258,18 @@ def test_attention_prefix_large_and_tiny_scores():
     ref.assert_attention(got, ref.attention(c, 0.5))
 
 
+@pytest.mark.parametrize("scale", [-0.1, 0.0])
+def test_attention_any_scale(scale):
+    """A negative scale prefers the least products, a zero scale none."""
+    c = ref.Cache(23, [100, 7, 0], 12, 2, 128, 32, BF16, prefix=300)
+    kv = c.handle()
+    got = ops.attention_prefix_paged(kv, c.q, c.seq_len, c.prefix_pages, 300, scale=scale, return_lse=True)
+    ref.assert_attention(got, ref.attention(c, scale))
+    c.prefix = 0
+    got = ops.attention_paged(kv, c.q, c.seq_len, scale=scale, return_lse=True)
+    ref.assert_attention(got, ref.attention(c, scale))
+
+
 def test_attention_prefix_is_paged_attention_of_the_whole():
     """The same positions through one table: prefix pages, then a sequence's own."""
     c = ref.Cache(22, [50, 64, 1, 0], 12, 2, 128, 64, BF16, prefix=640)

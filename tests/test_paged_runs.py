@@ -5,7 +5,7 @@ import random
 
 import pytest
 
-TILE, JOIN = 64, 16
+TILE, JOIN = 64, 16   # (the tile is 128 with head_dim 64; the rule is the same)
 
 
 def run_start(total, c, g):
