@@ -130,7 +130,7 @@ __device__ __forceinline__ int run_of(uint32_t total, uint32_t x, uint32_t G) {
 }
 // The partial slot of piece i: runs follow one another, or (fewer tiles than runs)
 // each has one tile or none.
-__device__ __noinline__ int piece_slot(const CutPiece& u, int i, int G) {
+__device__ __forceinline__ int piece_slot(const CutPiece& u, int i, int G) {
   const int r = u.total < (unsigned)G ? run_of(u.total, u.begin + i, G) : u.run0 + i;
   return 2 * r + (i == 0 ? 1 : 0);
 }
@@ -186,7 +186,7 @@ __device__ __forceinline__ uint32_t find_run(const DecodeArgs& p, uint32_t c, ui
 // A finished row: output and log-sum-exp, or for the shared-prefix join what they
 // are made of.
 template <typename T, int D>
-__device__ __noinline__ void finish_row(const DecodeArgs& p, int seq, int head, float4 v, float M, float sum, int lane) {
+__device__ __forceinline__ void finish_row(const DecodeArgs& p, int seq, int head, float4 v, float M, float sum, int lane) {
   if (!p.own_o) {
     write_row<T, D>(p.a, seq, head, v, M, sum, lane);
     return;
@@ -207,7 +207,7 @@ __device__ __forceinline__ void store_partial(const DecodeArgs& p, int at, float
 // warps, two heads of each at a time so that their loads are one round trip): into
 // the output rows, or into the first piece's slot.
 template <typename T, int D>
-__device__ __noinline__ void join_pieces(const DecodeArgs& p, const CutPiece& u, int G, int first, int step, int n, bool final,
+__device__ __forceinline__ void join_pieces(const DecodeArgs& p, const CutPiece& u, int G, int first, int step, int n, bool final,
                             int warp, int lane) {
   constexpr int V = D / 32, HB = 2;
   const int slot = lane < n ? piece_slot(u, first + lane * step, G) * kMaxSlotHeads : 0;
@@ -731,12 +731,21 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     if (!s.last[k]) continue;
     const CutPiece& u = s.cut[k];
     const int groups = (u.pieces + kJoin - 1) / kJoin, first = u.piece / kJoin * kJoin;
-    join_pieces<T, D>(p, u, G, first, 1, min(kJoin, u.pieces - first), groups == 1, warp, lane);
-    if (groups == 1) continue;
-    if (!join()) return;
-    if (threadIdx.x == 0) s.last[k] = arrive_last(p.arrived + 2 * G + u.unit, p.tag, groups);
-    if (!join()) return;
-    if (s.last[k]) join_pieces<T, D>(p, u, G, 0, kJoin, groups, true, warp, lane);
+    int from = first, step = 1, n = min(kJoin, u.pieces - first);
+    bool final = groups == 1;
+#pragma unroll 1
+    for (;;) {   // its sixteen, then the unit's sixteens
+      join_pieces<T, D>(p, u, G, from, step, n, final, warp, lane);
+      if (final) break;
+      if (!join()) return;
+      if (threadIdx.x == 0) s.last[k] = arrive_last(p.arrived + 2 * G + u.unit, p.tag, groups);
+      if (!join()) return;
+      if (!s.last[k]) break;
+      from = 0;
+      step = kJoin;
+      n = groups;
+      final = true;
+    }
   }
 }
 

@@ -96,7 +96,7 @@ struct Pieces {
   const PrefixArgs& p;
   int c, G, unit, w, h, pair, i0, i1, id;
   __device__ __forceinline__ Pieces(const PrefixArgs& p, int c, int G) : p(p), c(c), G(G), unit(-1) {}
-  __device__ __noinline__ bool next() {
+  __device__ __forceinline__ bool next() {
     if (p.share2) {
       if (unit >= 0) return false;
       const int per_head = p.tiles / 2 * p.share2 + (p.tiles & 1) * p.share1;
