@@ -48,23 +48,28 @@ int paged_sm_count();
 // slots and box_halves halves; 0 or -1.
 int encode_pages_map(CUtensorMap* map, const qwen_paged_kv& kv, const uint16_t* base, int box_rows, int box_halves);
 
-// Host set-up that a kernel needs once per device (dynamic shared memory limits).
+// A kernel's dynamic shared memory limit, raised before its first launch on each
+// device, and again where a launch fails (a device that was reset forgets it).
 class OncePerDevice {
  public:
-  bool done() {
-    const int d = device();
-    return d >= 0 && (mask_.load(std::memory_order_acquire) >> d & 1);
-  }
-  void set() {
-    const int d = device();
-    if (d >= 0) mask_.fetch_or(1ull << d, std::memory_order_release);
+  template <typename Launch>
+  cudaError_t launch(const void* kernel, int smem, Launch&& go) {
+    int d = 0;
+    cudaError_t e = cudaGetDevice(&d);
+    if (e != cudaSuccess) return e;
+    const unsigned long long bit = 1ull << (d & 63);
+    if (d < 64 && mask_.load(std::memory_order_acquire) & bit) {
+      e = go();
+      if (e != cudaErrorInvalidValue) return e;
+      cudaGetLastError();
+    }
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    mask_.fetch_or(bit, std::memory_order_release);
+    return go();
   }
 
  private:
-  static int device() {
-    int d = 0;
-    return cudaGetDevice(&d) == cudaSuccess && d >= 0 && d < 64 ? d : -1;
-  }
   std::atomic<unsigned long long> mask_{0};
 };
 

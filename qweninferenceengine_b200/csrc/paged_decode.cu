@@ -775,11 +775,6 @@ int launch(const DecodeArgs& p, int G, const CUtensorMap& tmk, const CUtensorMap
   auto kern = k_paged_decode<T, D, NT>;
   const int smem = (int)sizeof(DecodeSmem<D, NT>) + 1024;
   static_assert((sizeof(DecodeSmem<D, NT>) + 2048) * kCtasPerSm <= 228 * 1024, "CTAs per SM");
-  static OncePerDevice once;
-  if (!once.done() &&
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return -1;
-  once.set();
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -790,7 +785,12 @@ int launch(const DecodeArgs& p, int G, const CUtensorMap& tmk, const CUtensorMap
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, p, box_rows, tmk, tmv) == cudaSuccess ? 0 : -1;
+  static OncePerDevice once;
+  return once.launch(reinterpret_cast<const void*>(kern), smem, [&] {
+           return cudaLaunchKernelEx(&cfg, kern, p, box_rows, tmk, tmv);
+         }) == cudaSuccess
+             ? 0
+             : -1;
 }
 
 int units_per_head(const qwen_paged_kv& kv, int n_heads) {

@@ -288,6 +288,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
   const PagedAttnArgs& a = p.a;
   if (pad + sizeof(PrefixSmem<D>) > kSmemBytes) {
     if (threadIdx.x == 0) raise_error(a.err, kDevBadArgument);
+    pdl_wait();
     return;
   }
   PrefixSmem<D>& s = *reinterpret_cast<PrefixSmem<D>*>(smem_raw + pad);
@@ -692,11 +693,6 @@ int launch(const PrefixArgs& p, int G, const CUtensorMap& tmk, const CUtensorMap
   auto kern = k_prefix<T, D>;
   const int smem = (int)kSmemBytes;
   static_assert(sizeof(PrefixSmem<D>) <= kSmemBytes - 768, "shared memory");
-  static OncePerDevice once;
-  if (!once.done() &&
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return -1;
-  once.set();
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -707,7 +703,11 @@ int launch(const PrefixArgs& p, int G, const CUtensorMap& tmk, const CUtensorMap
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kern, p, box_rows, tmk, tmv) != cudaSuccess) return -1;
+  static OncePerDevice once;
+  if (once.launch(reinterpret_cast<const void*>(kern), smem, [&] {
+        return cudaLaunchKernelEx(&cfg, kern, p, box_rows, tmk, tmv);
+      }) != cudaSuccess)
+    return -1;
   const long long rows = (long long)p.a.kv.n_seq * p.a.n_heads;
   cfg.gridDim = dim3((unsigned)((rows + 7) / 8));
   cfg.blockDim = dim3(256);

@@ -345,12 +345,6 @@ __global__ void __launch_bounds__(kListThreads) k_page_list(const __grid_constan
 
 template <typename T, int D>
 int launch(const PagedSelectArgs& a, cudaStream_t st) {
-  static OncePerDevice once;
-  const int smem = kCached * (int)sizeof(u64);
-  if (!once.done() &&
-      cudaFuncSetAttribute(k_page_list, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return -1;
-  once.set();
   // Pages of a CTA: fewer where the whole batch would not fill the SMs twice.
   int per = 256;
   while (per > 32 && (long long)((a.kv.max_pages + per - 1) / per) * a.kv.n_seq < 2 * paged_sm_count()) per /= 2;
@@ -367,7 +361,12 @@ int launch(const PagedSelectArgs& a, cudaStream_t st) {
   cfg.gridDim = dim3(a.kv.n_kv_heads, a.kv.n_seq);
   cfg.blockDim = dim3(kListThreads);
   cfg.dynamicSmemBytes = (size_t)(a.kv.max_pages < (uint32_t)kCached ? a.kv.max_pages : kCached) * sizeof(u64);
-  return cudaLaunchKernelEx(&cfg, k_page_list, a) == cudaSuccess ? 0 : -1;
+  static OncePerDevice once;
+  return once.launch(reinterpret_cast<const void*>(k_page_list), kCached * (int)sizeof(u64), [&] {
+           return cudaLaunchKernelEx(&cfg, k_page_list, a);
+         }) == cudaSuccess
+             ? 0
+             : -1;
 }
 
 }  // namespace

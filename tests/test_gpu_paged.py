@@ -379,9 +379,15 @@ def test_attention_reports_what_only_the_device_sees():
     columns[2, 1, 0] = 4
     ops.attention_sparse_paged(kv, c.q, c.seq_len, columns)
     assert status() == QWEN_ERR_INVALID_ARGUMENT
-    pages = torch.tensor([c.n_pages, int(c.table[0, 0])], dtype=torch.int32, device="cuda")
-    ops.attention_prefix_paged(kv, c.q, c.seq_len, pages, 20)
+    # ... in a shared prefix, for every row
+    shared = ref.Cache(42, [40, 0, 33], 12, 2, 128, 16, F16, prefix=300)
+    pages = shared.prefix_pages.clone()
+    pages[3], pages[18] = c.n_pages + 100, -1
+    got = ops.attention_prefix_paged(shared.handle(), shared.q, shared.seq_len, pages, 300, return_lse=True)
     assert status() == QWEN_ERR_INVALID_ARGUMENT
+    keep = [i for i in range(19) if i not in (3, 18)]
+    shared.prefix_pages, shared.prefix = shared.prefix_pages[keep], 17 * 16
+    ref.assert_attention(got, ref.attention(shared, 128 ** -0.5))
     ref.assert_attention(ops.attention_paged(kv, c.q, c.seq_len, return_lse=True), whole)
 
 
