@@ -185,6 +185,7 @@ def uniform24(seed: int, sequence: int, step: int) -> int:
 _DTYPES = {torch.float16: QWEN_DTYPE_F16, torch.bfloat16: QWEN_DTYPE_BF16}
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") \
     else lambda index: torch.cuda.current_stream(index).cuda_stream
+_current_device = torch._C._cuda_getDevice
 _workspace_bytes: dict = {}   # by sizes: the library's answers are functions of nothing else
 
 
@@ -200,7 +201,7 @@ class PagedKV:
     reads nothing of their contents; their shapes and addresses must not change."""
 
     __slots__ = ("k_pages", "v_pages", "page_table", "bounds", "dtype", "device", "index", "n_seq",
-                 "n_kv_heads", "head_dim", "page_size", "ref", "_struct")
+                 "n_kv_heads", "head_dim", "page_size", "sizes", "ref", "_struct")
 
     def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
                  bounds: torch.Tensor | None = None):
@@ -231,6 +232,7 @@ class PagedKV:
         self.k_pages, self.v_pages, self.page_table, self.bounds = k_pages, v_pages, page_table, bounds
         self.dtype, self.device, self.index, self.n_seq = dtype, k_pages.device, index, n_seq
         self.n_kv_heads, self.head_dim, self.page_size = n_kv, dim, page_size
+        self.sizes = (index, n_seq, n_kv, dim, max_pages)
         # the stride of an axis of one element is never used: any valid value
         self._struct = PagedKVStruct(
             k_pages.data_ptr(), v_pages.data_ptr(), None if bounds is None else bounds.data_ptr(),
@@ -270,7 +272,7 @@ def _heads(q: torch.Tensor) -> int:
 def _call(kv: PagedKV, fn, *args) -> None:
     """A library entry on the cache's device and its current stream (appended)."""
     index = kv.index
-    if index == torch._C._cuda_getDevice():
+    if index == _current_device():
         rc = fn(kv.ref, *args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -281,8 +283,7 @@ def _call(kv: PagedKV, fn, *args) -> None:
 
 def _workspace(kv: PagedKV, query: str, *sizes) -> tuple:
     """(memory, bytes) that the library function `query` asks for."""
-    st = kv._struct
-    key = (query, kv.index, kv.n_seq, kv.n_kv_heads, kv.head_dim, st.max_pages, sizes)
+    key = (query, sizes, kv.sizes)
     need = _workspace_bytes.get(key)
     if need is None:
         if len(_workspace_bytes) > 4096:
@@ -322,20 +323,23 @@ def rope_append_paged(kv: PagedKV, q: torch.Tensor, k: torch.Tensor, v: torch.Te
 
 
 def _attend(kv, fn, query, sizes, lead, q, seq_len, extra, scale, out, return_lse):
-    n, heads = kv.n_seq, _heads(q)
+    n, dim, device = kv.n_seq, kv.head_dim, kv.device
+    heads = _heads(q)
     qs = _rows("q", q, kv, n, heads)
     if out is None:
-        out, os_ = torch.empty_like(q, memory_format=torch.contiguous_format), heads * kv.head_dim
+        out = torch.empty_like(q) if q.is_contiguous() else \
+            torch.empty((n, heads, dim), dtype=kv.dtype, device=device)
+        os_ = heads * dim
     else:
         os_ = _rows("out", out, kv, n, heads)
     lse = lp = None
     if return_lse:
-        lse = torch.empty_strided((n, heads), (heads, 1), dtype=torch.float32, device=kv.device)
+        lse = torch.empty_strided((n, heads), (heads, 1), dtype=torch.float32, device=device)
         lp = lse.data_ptr()
     ws, need = _workspace(kv, query, heads, *sizes)
     _call(kv, fn, *lead, q.data_ptr(), qs, out.data_ptr(), os_, lp, heads,
-          _ints("seq_len", seq_len, kv, n), *extra,
-          kv.head_dim ** -0.5 if scale is None else scale, ws.data_ptr(), need)
+          _ints("seq_len", seq_len, kv, n), *extra, dim ** -0.5 if scale is None else scale,
+          ws.data_ptr(), need)
     return (out, lse) if return_lse else out
 
 
@@ -376,7 +380,8 @@ def select_pages(kv: PagedKV, q: torch.Tensor, seq_len: torch.Tensor, n_select: 
     qs = _rows("q", q, kv, n, heads)
     shape = (n, kv.n_kv_heads, n_select)
     if out is None:
-        out = torch.empty(shape, dtype=torch.int32, device=kv.device)
+        out = torch.empty_strided(shape, (kv.n_kv_heads * n_select, n_select, 1), dtype=torch.int32,
+                                  device=kv.device)
     elif out.shape != shape or out.dtype is not torch.int32 or out.get_device() != kv.index or \
             not out.is_contiguous():
         raise ValueError(f"out must be a contiguous int32 tensor {shape} on {kv.device}")
