@@ -289,26 +289,37 @@ __global__ void __launch_bounds__(kRowThreads) k_append_rows(const __grid_consta
         least[i] = inf2(T{});
         most[i] = inf2(T{}) | 0x80008000u;
       }
-#pragma unroll 2
-      for (int r = r0; r < n; r += kRowThreads / 2) {
-        const T* src = k + r * a.k_stride + h * D;
-        Chunk x = load_chunk(src + pa, src + pb);
-        if (turns) {
-          float2 rot[8];
+      constexpr int kAtOnce = 4, kStep = kRowThreads / 2;   // rows of a thread in flight, and between them
+#pragma unroll 1
+      for (int r = r0; r < n; r += kAtOnce * kStep) {
+        Chunk x[kAtOnce];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float4 v = reinterpret_cast<const float4*>(page_rot + 16 * r + 8 * (c & 1))[i];
-            rot[2 * i] = make_float2(v.x, v.y);
-            rot[2 * i + 1] = make_float2(v.z, v.w);
+        for (int j = 0; j < kAtOnce; ++j)
+          if (r + j * kStep < n) {
+            const T* src = k + (r + j * kStep) * a.k_stride + h * D;
+            x[j] = load_chunk(src + pa, src + pb);
           }
-          rotate_chunk<T, kInterleaved>(x, rot);
-        }
-        T* y = dst + r * a.kv.pos_stride + h * a.kv.head_stride;
-        store_chunk(y + pa, y + pb, x);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          least[i] = min2(T{}, least[i], x.w[i]);
-          most[i] = max2(T{}, most[i], x.w[i]);
+        for (int j = 0; j < kAtOnce; ++j) {
+          const int row = r + j * kStep;
+          if (row >= n) break;
+          if (turns) {
+            float2 rot[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float4 v = reinterpret_cast<const float4*>(page_rot + 16 * row + 8 * (c & 1))[i];
+              rot[2 * i] = make_float2(v.x, v.y);
+              rot[2 * i + 1] = make_float2(v.z, v.w);
+            }
+            rotate_chunk<T, kInterleaved>(x[j], rot);
+          }
+          T* y = dst + row * a.kv.pos_stride + h * a.kv.head_stride;
+          store_chunk(y + pa, y + pb, x[j]);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            least[i] = min2(T{}, least[i], x[j].w[i]);
+            most[i] = max2(T{}, most[i], x[j].w[i]);
+          }
         }
       }
       if (!a.kv.bounds) continue;
