@@ -11,8 +11,9 @@
 // The angle is formed exactly (24 + 24 bits fit a double) and reduced to turns
 // in 64 bits: an fp32 product at position 100,000 is off by up to 0.004 rad.  Its
 // sine and cosine cost as much as rotating six heads by it, so prompts compute each
-// once: k_append_rows' query CTAs keep eight of a thread's angles in registers for
-// all query heads, its key CTAs a page's in shared memory for all kv heads.
+// once or a few times: k_append_rows' query CTAs keep eight of a thread's angles in
+// registers for eight heads (sixteen took 18 us where eight took 15: it is the number of
+// CTAs that hides the memory's latency), its key CTAs a page's in shared memory for four.
 //
 // Bounds: a key CTA owns two chunks of one page's new keys (all kv heads), so the
 // least and greatest are reduced inside it: no atomics, and a page begun anew
@@ -27,9 +28,8 @@ namespace {
 
 constexpr int kTokenThreads = 128;    // decode: a CTA per token
 constexpr int kRowThreads = 128;      // prompts
-constexpr int kHeadsAtOnce = 8;       // heads of a query CTA in flight
-constexpr int kHeadsPerCta = 16;      // its query heads
-constexpr int kReduceHeads = 8;       // kv heads between a key CTA's barriers
+constexpr int kHeads = 8;             // query or value heads of a CTA, in flight together
+constexpr int kKeyHeads = 4;          // kv heads of a key CTA
 
 __device__ __forceinline__ void sincos_of(float pos, float inv_freq, float* sn, float* cs) {
   const double turns = (double)pos * (double)inv_freq * 0.15915494309189533577;
@@ -171,7 +171,22 @@ __global__ void __launch_bounds__(kTokenThreads) k_append_token(const __grid_con
 }
 
 // First sequence s with base(s + 1) > x, base(s) = (cu[s] >> shift) + per_seq * s.
-__device__ __forceinline__ int seq_of(const int32_t* cu, int n_seq, int shift, int per_seq, int x) {
+// A warp: x is the same for the lanes of each group of kLanes.
+template <int kLanes>
+__device__ __forceinline__ int seq_of(const int32_t* cu, int n_seq, int shift, int per_seq, int x, int lane) {
+  if (n_seq <= 256) {   // the lanes read all starts at once and count those up to x
+    int s = 0;
+#pragma unroll 1
+    for (int b = 0; b < n_seq; b += 32) {
+      const int start = b + lane < n_seq ? (cu[b + lane + 1] >> shift) + per_seq * (b + lane + 1) : 0x7fffffff;
+#pragma unroll
+      for (int g = 0; g < 32; g += kLanes) {
+        const int count = __popc(__ballot_sync(0xffffffffu, start <= __shfl_sync(0xffffffffu, x, g)));
+        if (lane / kLanes == g / kLanes) s += count;
+      }
+    }
+    return min(s, n_seq - 1);
+  }
   int lo = 0, hi = n_seq - 1;
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
@@ -194,95 +209,100 @@ __device__ __forceinline__ bool rows_of(const PagedAppendArgs& a, int s, bool re
   return ok;
 }
 
-// Ragged tokens.  CTAs 0 .. key_ctas - 1: chunks 2j, 2j+1 of the new keys of one page
-// (slot blockIdx.x / (D / 32)); the rest: 16 query heads and
-// v of kRowThreads / (D / 16) tokens.
+// Ragged tokens.  CTAs 0 .. key_ctas - 1: chunks 2j, 2j+1 of the new keys of one page,
+// or of the two or four whose rows make up 64; the rest: 8 query or value heads of
+// kRowThreads / (D / 16) tokens.
 template <typename T, int D, bool kInterleaved>
-__global__ void __launch_bounds__(kRowThreads) k_append_rows(const __grid_constant__ PagedAppendArgs a, int key_ctas) {
-  constexpr int NC = D / 16;
-  extern __shared__ float2 page_rot[];   // key CTA: [page_size][16]
-  __shared__ uint32_t part[kReduceHeads][kRowThreads / 32][32];
+__global__ void __launch_bounds__(kRowThreads, 4) k_append_rows(const __grid_constant__ PagedAppendArgs a, int key_ctas) {
+  constexpr int NC = D / 16, kWarps = kRowThreads / 32;
+  extern __shared__ float2 page_rot[];   // key CTA: [max(page_size, 64)][16]
+  __shared__ uint32_t part[kKeyHeads][kWarps][32];
   const int H = a.n_heads, K = a.kv.n_kv_heads, R = a.rot_dim, P = a.kv.page_size, tid = threadIdx.x;
-  const int n_seq = a.kv.n_seq;
+  const int n_seq = a.kv.n_seq, warp = tid >> 5, lane = tid & 31;
   pdl_wait();
   if (tid == 0) pdl_launch_dependents();
 
   if ((int)blockIdx.x >= key_ctas) {
     // ------------------------------------------------------------- q and v --
-    const int parts = (H + kHeadsPerCta - 1) / kHeadsPerCta;   // and v goes with the first
-    const int x0 = ((int)blockIdx.x - key_ctas) / parts, first = ((int)blockIdx.x - key_ctas) % parts * kHeadsPerCta;
-    const int row = x0 * (kRowThreads / NC) + tid / NC, c = tid % NC, last = min(H, first + kHeadsPerCta);
-    if (row >= a.n_tokens || row >= a.cu_tokens[n_seq]) return;
-    const int s = seq_of(a.cu_tokens, n_seq, 0, 0, row);
+    // The rows' elements are on their way while their sequence is looked up.
+    const int q_parts = (H + kHeads - 1) / kHeads, parts = q_parts + (K + kHeads - 1) / kHeads;
+    const int tile = ((int)blockIdx.x - key_ctas) / parts, part_no = (int)blockIdx.x - key_ctas - tile * parts;
+    const bool is_q = part_no < q_parts;
+    const int first = (is_q ? part_no : part_no - q_parts) * kHeads, count = min(kHeads, (is_q ? H : K) - first);
+    const int row = tile * (kRowThreads / NC) + tid / NC, c = tid % NC;
+    const bool there = row < a.n_tokens, turns = is_q && 16 * c < R;
+    int pa = 16 * c, pb = 16 * c + 8;
+    if (is_q) places<kInterleaved>(c, R, &pa, &pb);
+    const T* src = (is_q ? reinterpret_cast<const T*>(a.q) + row * a.q_stride : reinterpret_cast<const T*>(a.v) + row * a.v_stride) + first * D;
+    Chunk x[kHeads];
+#pragma unroll
+    for (int j = 0; j < kHeads; ++j)
+      if (there && j < count) x[j] = load_chunk(src + j * D + pa, src + j * D + pb);
+    const int s = seq_of<NC>(a.cu_tokens, n_seq, 0, 0, row, lane);
     int row0, row1, L;
-    if (!rows_of(a, s, false, &row0, &row1, &L) || row < row0 || row >= row1) return;
+    if (!there || !rows_of(a, s, false, &row0, &row1, &L) || row < row0 || row >= row1) return;
     const int pos = L - (row1 - row);
-    int pa, pb;
-    places<kInterleaved>(c, R, &pa, &pb);
-    const bool turns = 16 * c < R;
-    const int page = pool_page(a, s, pos >> a.page_shift);
-    const T* q = reinterpret_cast<const T*>(a.q) + row * a.q_stride;
-    T* q_out = reinterpret_cast<T*>(a.q_out) + row * a.q_out_stride;
+    T* dst;
+    long long stride = D;
+    if (is_q) {
+      dst = reinterpret_cast<T*>(a.q_out) + row * a.q_out_stride + first * D;
+    } else {
+      const int page = pool_page(a, s, pos >> a.page_shift);
+      if (page < 0) return;
+      stride = a.kv.head_stride;
+      dst = reinterpret_cast<T*>(a.kv.v) + page * a.kv.page_stride + (pos & (P - 1)) * a.kv.pos_stride + first * stride;
+    }
     float2 rot[8];
     if (turns) rotation_of(a, pos, c, rot);
-    for (int h0 = first; h0 < last; h0 += kHeadsAtOnce) {
-      Chunk x[kHeadsAtOnce];
 #pragma unroll
-      for (int j = 0; j < kHeadsAtOnce; ++j)
-        if (h0 + j < last) x[j] = load_chunk(q + (h0 + j) * D + pa, q + (h0 + j) * D + pb);
-#pragma unroll
-      for (int j = 0; j < kHeadsAtOnce; ++j)
-        if (h0 + j < last) {
-          if (turns) rotate_chunk<T, kInterleaved>(x[j], rot);
-          store_chunk(q_out + (h0 + j) * D + pa, q_out + (h0 + j) * D + pb, x[j]);
-        }
-    }
-    if (page < 0 || first > 0) return;
-    const T* v = reinterpret_cast<const T*>(a.v) + row * a.v_stride + 16 * c;
-    T* v_out = reinterpret_cast<T*>(a.kv.v) + page * a.kv.page_stride + (pos & (P - 1)) * a.kv.pos_stride + 16 * c;
-    for (int h0 = 0; h0 < K; h0 += kHeadsAtOnce) {
-      Chunk x[kHeadsAtOnce];
-#pragma unroll
-      for (int j = 0; j < kHeadsAtOnce; ++j)
-        if (h0 + j < K) x[j] = load_chunk(v + (h0 + j) * D, v + (h0 + j) * D + 8);
-#pragma unroll
-      for (int j = 0; j < kHeadsAtOnce; ++j)
-        if (h0 + j < K) store_chunk(v_out + (h0 + j) * a.kv.head_stride, v_out + (h0 + j) * a.kv.head_stride + 8, x[j]);
-    }
+    for (int j = 0; j < kHeads; ++j)
+      if (j < count) {
+        if (turns) rotate_chunk<T, kInterleaved>(x[j], rot);
+        store_chunk(dst + j * stride + pa, dst + j * stride + pb, x[j]);
+      }
     return;
   }
 
   // ------------------------------------------------------------------ keys --
-  const int page_slot = blockIdx.x / (D / 32), pair = blockIdx.x % (D / 32);
-  const int s = seq_of(a.cu_tokens, n_seq, a.page_shift, 2, page_slot);
-  int row0, row1, L;
-  if (!rows_of(a, s, tid == 0, &row0, &row1, &L) || row1 == row0) return;
-  const int index = page_slot - ((row0 >> a.page_shift) + 2 * s), start = L - (row1 - row0);
-  if (index < 0) return;
-  const int col = (start >> a.page_shift) + index;
-  const int p0 = max(start, col * P), n = min(L, (col + 1) * P) - p0;   // positions p0 .. p0 + n - 1
-  if (n <= 0) return;
-  const int page = pool_page(a, s, col);
-  if (page < 0) return;
-  const int c = 2 * pair + (tid & 1), r0 = tid >> 1, warp = tid >> 5, lane = tid & 31;
+  // A warp has 16 rows of one page; page_warps warps share a page of up to 64 rows, and
+  // go on in steps of 64 through a larger one.
+  const int page_warps = min(P / 16, kWarps), sub = warp / page_warps;
+  const int splits = (K + kKeyHeads - 1) / kKeyHeads;   // CTAs by kv heads
+  const int pair = blockIdx.x % (D / 32), rest = blockIdx.x / (D / 32);
+  const int slot = rest / splits * (kWarps / page_warps) + sub;
+  const int hb = rest % splits * kKeyHeads, he = min(K, hb + kKeyHeads);
+  const int s = seq_of<32>(a.cu_tokens, n_seq, a.page_shift, 2, slot, lane);
+  int row0 = 0, row1 = 0, L = 0, n = 0, p0 = 0, start = 0, page = -1;   // positions p0 .. p0 + n - 1
+  if (rows_of(a, s, lane == 0, &row0, &row1, &L) && row1 > row0) {
+    const int index = slot - ((row0 >> a.page_shift) + 2 * s);
+    start = L - (row1 - row0);
+    const int col = (start >> a.page_shift) + index;
+    p0 = max(start, col * P);
+    if (index >= 0) n = max(0, min(L, (col + 1) * P) - p0);
+    if (n > 0) page = pool_page(a, s, col);
+    if (page < 0) n = 0;
+  }
+  const int c = 2 * pair + (lane & 1), group_tid = tid - sub * page_warps * 32, r0 = group_tid >> 1;
   int pa, pb;
   places<kInterleaved>(c, R, &pa, &pb);
   const bool turns = 16 * c < R;
-  // the angles of this CTA's chunks: 16 a row
-  for (int i = tid; i < n * 16; i += kRowThreads) {
+  float2* my_rot = page_rot + sub * P * 16;   // the angles of the page's chunks: 16 a row
+#pragma unroll 4
+  for (int i = group_tid; i < n * 16; i += page_warps * 32) {
     const int f = 16 * pair + (i & 15);
     if (f < R / 2) {
       float sn, cs;
       sincos_of((float)(p0 + (i >> 4)), a.inv_freq[f], &sn, &cs);
-      page_rot[i] = make_float2(cs, sn);
+      my_rot[i] = make_float2(cs, sn);
     }
   }
   __syncthreads();
   const bool anew = (p0 & (P - 1)) == 0;
   const T* k = reinterpret_cast<const T*>(a.k) + (long long)(row0 + (p0 - start)) * a.k_stride;
-  T* dst = reinterpret_cast<T*>(a.kv.k) + page * a.kv.page_stride + (p0 & (P - 1)) * a.kv.pos_stride;
-  for (int hb = 0; hb < K; hb += kReduceHeads) {
-    for (int h = hb; h < min(K, hb + kReduceHeads); ++h) {
+  T* dst = reinterpret_cast<T*>(a.kv.k) + (long long)max(page, 0) * a.kv.page_stride + (p0 & (P - 1)) * a.kv.pos_stride;
+  {
+#pragma unroll 1
+    for (int h = hb; h < he; ++h) {
       uint32_t least[8], most[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -307,7 +327,7 @@ __global__ void __launch_bounds__(kRowThreads) k_append_rows(const __grid_consta
             float2 rot[8];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const float4 v = reinterpret_cast<const float4*>(page_rot + 16 * row + 8 * (c & 1))[i];
+              const float4 v = reinterpret_cast<const float4*>(my_rot + 16 * row + 8 * (c & 1))[i];
               rot[2 * i] = make_float2(v.x, v.y);
               rot[2 * i + 1] = make_float2(v.z, v.w);
             }
@@ -345,15 +365,18 @@ __global__ void __launch_bounds__(kRowThreads) k_append_rows(const __grid_consta
       }
       part[h - hb][warp][lane] = v[0];
     }
-    if (!a.kv.bounds) continue;
+    if (!a.kv.bounds) return;
     __syncthreads();
-    for (int h = hb + warp; h < min(K, hb + kReduceHeads); h += kRowThreads / 32) {
+    // A page's warps take its heads in turn.
+    for (int h = hb + warp % page_warps; h < he && n > 0; h += page_warps) {
       const bool up = lane & 16;
       const int word = (lane >> 1) & 7;   // of the chunk's eight
-      uint32_t v = part[h - hb][0][lane];
-#pragma unroll
-      for (int w = 1; w < kRowThreads / 32; ++w)
-        v = up ? max2(T{}, v, part[h - hb][w][lane]) : min2(T{}, v, part[h - hb][w][lane]);
+      uint32_t v = part[h - hb][sub * page_warps][lane];
+#pragma unroll 1
+      for (int w = 1; w < page_warps; ++w) {
+        const uint32_t other = part[h - hb][sub * page_warps + w][lane];
+        v = up ? max2(T{}, v, other) : min2(T{}, v, other);
+      }
       T* at = reinterpret_cast<T*>(a.kv.bounds) + (((long long)page * 2 + (up ? 1 : 0)) * K + h) * D +
               (word < 4 ? pa + 2 * word : pb + 2 * (word - 4));
       if (!anew) {
@@ -362,7 +385,6 @@ __global__ void __launch_bounds__(kRowThreads) k_append_rows(const __grid_consta
       }
       *reinterpret_cast<uint32_t*>(at) = v;
     }
-    __syncthreads();
   }
 }
 
@@ -380,12 +402,14 @@ int launch(const PagedAppendArgs& a, cudaStream_t st) {
     cfg.blockDim = dim3(kTokenThreads);
     return cudaLaunchKernelEx(&cfg, k_append_token<T, D, kInterleaved>, a) == cudaSuccess ? 0 : -1;
   }
-  const int key_ctas = ((a.n_tokens >> a.page_shift) + 2 * (int)a.kv.n_seq) * (D / 32);
+  const int per_cta = a.kv.page_size >= 64 ? 1 : 64 / (int)a.kv.page_size;   // pages
+  const int slots = (a.n_tokens >> a.page_shift) + 2 * (int)a.kv.n_seq;
+  const int key_ctas = (slots + per_cta - 1) / per_cta * (D / 32) * (((int)a.kv.n_kv_heads + kKeyHeads - 1) / kKeyHeads);
   constexpr int kTileRows = kRowThreads / (D / 16);
-  const int parts = (a.n_heads + kHeadsPerCta - 1) / kHeadsPerCta;
+  const int parts = (a.n_heads + kHeads - 1) / kHeads + ((int)a.kv.n_kv_heads + kHeads - 1) / kHeads;
   cfg.gridDim = dim3(key_ctas + (a.n_tokens + kTileRows - 1) / kTileRows * parts);
   cfg.blockDim = dim3(kRowThreads);
-  cfg.dynamicSmemBytes = (size_t)a.kv.page_size * 16 * sizeof(float2);
+  cfg.dynamicSmemBytes = (size_t)(a.kv.page_size < 64 ? 64 : a.kv.page_size) * 16 * sizeof(float2);
   return cudaLaunchKernelEx(&cfg, k_append_rows<T, D, kInterleaved>, a, key_ctas) == cudaSuccess ? 0 : -1;
 }
 
