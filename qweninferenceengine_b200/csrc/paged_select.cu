@@ -175,10 +175,12 @@ struct ListSmem {
   int at;
 };
 
-// Exclusive sum over the CTA's threads of v (and the total), packed or not.
+// Exclusive sum over the CTA's threads of v (and the total), packed or not.  Small
+// code throughout this kernel: it runs once, from a cold instruction cache.
 template <typename V>
-__device__ __noinline__ V exclusive_sum(V v, V* warp_sums, V* total) {
+__device__ __forceinline__ V exclusive_sum(V v, V* warp_sums, V* total) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kW = kListThreads / 32;
   V inc = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -187,15 +189,15 @@ __device__ __noinline__ V exclusive_sum(V v, V* warp_sums, V* total) {
   }
   if (lane == 31) warp_sums[warp] = inc;
   __syncthreads();
-  V before = inc - v, all = 0;
+  V ws = lane < kW ? warp_sums[lane] : 0;   // every warp adds up the warps' sums
 #pragma unroll
-  for (int w = 0; w < kListThreads / 32; ++w) {
-    if (w < warp) before += warp_sums[w];
-    all += warp_sums[w];
+  for (int o = 1; o < kW; o <<= 1) {
+    const V x = __shfl_up_sync(0xffffffffu, ws, o);
+    if (lane >= o) ws += x;
   }
-  *total = all;
-  __syncthreads();
-  return before;
+  *total = __shfl_sync(0xffffffffu, ws, kW - 1);
+  const V before = __shfl_sync(0xffffffffu, ws, (warp - 1) & 31);
+  return inc - v + (warp ? before : 0);
 }
 
 __global__ void __launch_bounds__(kListThreads) k_page_list(const __grid_constant__ PagedSelectArgs a) {
@@ -219,6 +221,7 @@ __global__ void __launch_bounds__(kListThreads) k_page_list(const __grid_constan
   const u64* global = reinterpret_cast<const u64*>(a.scores) + ((long long)s * K + h) * a.kv.max_pages + first;
   const u64* keys = global;
   u64 lo = ~0ull, hi = 0;
+#pragma unroll 4
   for (int i = tid; i < m; i += kListThreads) {
     const u64 x = __ldcg(global + i);
     if (m <= kCached) cached[i] = x;
@@ -226,21 +229,22 @@ __global__ void __launch_bounds__(kListThreads) k_page_list(const __grid_constan
     hi = max(hi, x);
   }
   if (m <= kCached) keys = cached;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-  }
+  auto extremes = [&]() {
+#pragma unroll 1
+    for (int o = 16; o > 0; o >>= 1) {
+      lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+  };
+  extremes();
   if ((tid & 31) == 0) {
     sm.red[0][tid >> 5] = lo;
     sm.red[1][tid >> 5] = hi;
   }
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kListThreads / 32; ++w) {
-    lo = min(lo, sm.red[0][w]);
-    hi = max(hi, sm.red[1][w]);
-  }
+  lo = sm.red[0][tid & (kListThreads / 32 - 1)];
+  hi = sm.red[1][tid & (kListThreads / 32 - 1)];
+  extremes();
   // Taken: keys above `cut`, and of those equal to it the first `ties`.
   u64 cut = ~0ull;
   uint32_t ties = 0;
