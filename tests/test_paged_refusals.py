@@ -144,6 +144,14 @@ def test_no_sequences_is_nothing_to_do():
     assert append(kv(), n=0, cu=A, q=None, k=None, v=None, out=None) == _lib.QWEN_OK
 
 
+def test_python_handle_is_packed_as_the_struct_is_laid_out():
+    from qweninferenceengine_b200 import ops
+
+    values = list(range(1, 16))
+    packed = PagedKVStruct.from_buffer_copy(ops._PAGED_KV.pack(*values))
+    assert [getattr(packed, f) for f, _ in PagedKVStruct._fields_] == values
+
+
 def test_python_handle_wants_device_tensors():
     import torch
 
