@@ -233,9 +233,15 @@ typedef struct qwen_paged_kv {
  * read or written there).  Rows of q, k, v and outputs are head-contiguous
  * ([heads][head_dim]) with the given row strides (elements, multiples of 8) and
  * 16-byte aligned.  workspace: device memory of at least the *_workspace bytes
- * for the same arguments, 256-byte aligned, with any contents; calls that may
- * overlap on the GPU need one each.  n_heads is a multiple of n_kv_heads, at
- * most 64 query heads share a kv head. */
+ * for the same arguments (0 for arguments that will be refused), 256-byte aligned,
+ * with any contents; calls that may overlap on the GPU need one each, calls one
+ * after another, captured ones too, can share one.  (After a
+ * QWEN_ERR_DEVICE_TIMEOUT clear it before a captured call is replayed.)
+ * n_heads is a multiple of n_kv_heads, at most 64 query heads share a kv head.
+ * A sequence has at most 2^24 positions, a call at most 65535 sequences, and an
+ * attention call fewer than 2^31 tiles of 64 positions (128 with head_dim 64) per
+ * 16 query heads of a kv head, counted with every sequence at full capacity (sparse:
+ * at n_select pages); a larger one is refused.  An attention's out may be its q. */
 
 /* apply_rope_q4 and write_kv_cache (rope.metal:12-39, attention.metal:67-84) for
  * a batch of new tokens over a paged cache, in one launch: rotates q into q_out

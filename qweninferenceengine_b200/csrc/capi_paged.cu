@@ -13,6 +13,19 @@ namespace {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+constexpr uint32_t kMaxPositions = 1u << 24;   // of a sequence: positions are exact in fp32
+constexpr uint32_t kMaxSeqs = 65535;           // of a call: grid rows
+
+bool heads_fit(const qwen_paged_kv& kv, uint32_t n_heads) {
+  return kv.n_kv_heads != 0 && kv.n_kv_heads <= 1024 && n_heads != 0 && n_heads % kv.n_kv_heads == 0 &&
+         n_heads / kv.n_kv_heads <= (uint32_t)kMaxGroup;
+}
+// Whether a workspace can be sized for these arguments; none for a call without
+// sequences, or one that will be refused.
+bool workspace_for(const qwen_paged_kv* kv, uint32_t n_heads) {
+  return kv && kv->n_seq != 0 && kv->n_seq <= kMaxSeqs && heads_fit(*kv, n_heads) && kv->max_pages <= kMaxPositions;
+}
+
 int check_kv(const char* op, const qwen_paged_kv* kv, uint32_t n_heads, int* page_shift) {
   if (!kv) return set_error(QWEN_ERR_INVALID_ARGUMENT, "%s: null kv", op);
   if (!kv->k || !kv->v || (!kv->page_table && kv->n_seq))
@@ -29,14 +42,13 @@ int check_kv(const char* op, const qwen_paged_kv* kv, uint32_t n_heads, int* pag
   *page_shift = shift;
   if (kv->n_pages == 0 || kv->n_pages > (1u << 30))
     return set_error(QWEN_ERR_INVALID_ARGUMENT, "%s: n_pages=%u", op, kv->n_pages);
-  if (kv->n_seq > 65535) return set_error(QWEN_ERR_INVALID_ARGUMENT, "%s: n_seq=%u", op, kv->n_seq);
-  if (kv->max_pages == 0 || (uint64_t)kv->max_pages * kv->page_size > (1u << 24) ||
+  if (kv->n_seq > kMaxSeqs) return set_error(QWEN_ERR_INVALID_ARGUMENT, "%s: n_seq=%u", op, kv->n_seq);
+  if (kv->max_pages == 0 || (uint64_t)kv->max_pages * kv->page_size > kMaxPositions ||
       kv->table_stride < kv->max_pages)
     return set_error(QWEN_ERR_INVALID_ARGUMENT,
                      "%s: max_pages=%u (at most 2^24 positions) table_stride=%u", op, kv->max_pages,
                      kv->table_stride);
-  if (kv->n_kv_heads == 0 || kv->n_kv_heads > 1024 || n_heads == 0 || n_heads % kv->n_kv_heads != 0 ||
-      n_heads / kv->n_kv_heads > (uint32_t)kMaxGroup)
+  if (!heads_fit(*kv, n_heads))
     return set_error(QWEN_ERR_INVALID_ARGUMENT,
                      "%s: n_heads=%u must be a multiple of n_kv_heads=%u, at most %d times it", op,
                      n_heads, kv->n_kv_heads, kMaxGroup);
@@ -68,6 +80,11 @@ int check_workspace(const char* op, const void* p, size_t bytes, size_t need) {
   return QWEN_OK;
 }
 
+int finish(const char* op, int launched) {
+  QWEN_TRY(launch_status(op));
+  return launched == 0 ? QWEN_OK : set_error(QWEN_ERR_CUDA, "%s: launch failed", op);
+}
+
 int attention(const char* op, PagedAttnArgs& a, const qwen_paged_kv* kv, const uint16_t* q,
               int64_t q_stride, uint16_t* out, int64_t out_stride, float* lse, uint32_t n_heads,
               const uint32_t* seq_len, float scale, void* workspace, size_t workspace_bytes,
@@ -94,10 +111,8 @@ int attention(const char* op, PagedAttnArgs& a, const qwen_paged_kv* kv, const u
   a.scale = scale;
   a.workspace = workspace;
   QWEN_TRY(ops_status_word(&a.err));
-  const int rc = a.prefix_len ? launch_paged_prefix(a, static_cast<cudaStream_t>(stream))
-                              : launch_paged_decode(a, static_cast<cudaStream_t>(stream));
-  QWEN_TRY(launch_status(op));
-  return rc == 0 ? QWEN_OK : set_error(QWEN_ERR_CUDA, "%s: launch failed", op);
+  return finish(op, a.prefix_len ? launch_paged_prefix(a, static_cast<cudaStream_t>(stream))
+                                 : launch_paged_decode(a, static_cast<cudaStream_t>(stream)));
 }
 
 }  // namespace
@@ -144,12 +159,11 @@ int qwen_rope_append_paged(const qwen_paged_kv* kv, const uint16_t* q, int64_t q
   a.rot_dim = (int)rot_dim;
   a.interleaved = interleaved ? 1 : 0;
   QWEN_TRY(ops_status_word(&a.err));
-  if (launch_rope_append(a, static_cast<cudaStream_t>(stream)) != 0) return launch_status(op);
-  return launch_status(op);
+  return finish(op, launch_rope_append(a, static_cast<cudaStream_t>(stream)));
 }
 
 size_t qwen_attention_paged_workspace(const qwen_paged_kv* kv, uint32_t n_heads) {
-  return kv ? paged_decode_workspace(*kv, (int)n_heads) : 0;
+  return workspace_for(kv, n_heads) ? paged_decode_workspace(*kv, (int)n_heads) : 0;
 }
 
 int qwen_attention_paged(const qwen_paged_kv* kv, const uint16_t* q, int64_t q_stride,
@@ -162,7 +176,9 @@ int qwen_attention_paged(const qwen_paged_kv* kv, const uint16_t* q, int64_t q_s
 }
 
 size_t qwen_attention_prefix_paged_workspace(const qwen_paged_kv* kv, uint32_t n_heads, uint32_t prefix_len) {
-  return kv ? paged_prefix_workspace(*kv, (int)n_heads, prefix_len) : 0;
+  return workspace_for(kv, n_heads) && prefix_len <= kMaxPositions
+             ? paged_prefix_workspace(*kv, (int)n_heads, prefix_len)
+             : 0;
 }
 
 int qwen_attention_prefix_paged(const qwen_paged_kv* kv, const uint16_t* q, int64_t q_stride,
@@ -171,7 +187,7 @@ int qwen_attention_prefix_paged(const qwen_paged_kv* kv, const uint16_t* q, int6
                                 uint32_t prefix_len, float scale, void* workspace,
                                 size_t workspace_bytes, void* stream) {
   const char* op = "attention_prefix_paged";
-  if (prefix_len > (1u << 24))
+  if (prefix_len > kMaxPositions)
     return set_error(QWEN_ERR_INVALID_ARGUMENT, "%s: prefix_len=%u", op, prefix_len);
   if (prefix_len && !prefix_pages)
     return set_error(QWEN_ERR_INVALID_ARGUMENT, "%s: null prefix_pages", op);
@@ -183,7 +199,9 @@ int qwen_attention_prefix_paged(const qwen_paged_kv* kv, const uint16_t* q, int6
 }
 
 size_t qwen_select_pages_workspace(const qwen_paged_kv* kv) {
-  return kv ? (size_t)kv->n_seq * kv->n_kv_heads * kv->max_pages * sizeof(double) : 0;
+  return workspace_for(kv, kv ? kv->n_kv_heads : 0)
+             ? (size_t)kv->n_seq * kv->n_kv_heads * kv->max_pages * sizeof(double)
+             : 0;
 }
 
 int qwen_select_pages(const qwen_paged_kv* kv, const uint16_t* q, int64_t q_stride,
@@ -212,12 +230,11 @@ int qwen_select_pages(const qwen_paged_kv* kv, const uint16_t* q, int64_t q_stri
   a.pages = pages;
   a.scores = static_cast<double*>(workspace);
   QWEN_TRY(ops_status_word(&a.err));
-  if (launch_select_pages(a, static_cast<cudaStream_t>(stream)) != 0) return launch_status(op);
-  return launch_status(op);
+  return finish(op, launch_select_pages(a, static_cast<cudaStream_t>(stream)));
 }
 
 size_t qwen_attention_sparse_paged_workspace(const qwen_paged_kv* kv, uint32_t n_heads, uint32_t) {
-  return kv ? paged_decode_workspace(*kv, (int)n_heads) : 0;
+  return qwen_attention_paged_workspace(kv, n_heads);
 }
 
 int qwen_attention_sparse_paged(const qwen_paged_kv* kv, const int32_t* pages, uint32_t n_select,

@@ -36,11 +36,6 @@ __device__ __forceinline__ void sincos_of(float pos, float inv_freq, float* sn, 
   sincospif(2.0f * (float)(turns - rint(turns)), sn, cs);
 }
 
-__device__ __forceinline__ float2 to_f32x2(__half, uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
-__device__ __forceinline__ float2 to_f32x2(__nv_bfloat16, uint32_t w) {
-  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-}
-
 // 16 elements: the words of two 16-byte halves.
 struct Chunk {
   uint32_t w[8];
@@ -66,13 +61,13 @@ __device__ __forceinline__ void rotate_chunk(Chunk& x, const float2 (&rot)[8]) {
   if constexpr (kInterleaved) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float2 v = to_f32x2(T{}, x.w[i]);
+      const float2 v = unpack2(T{}, x.w[i]);
       x.w[i] = pack2(T{}, v.x * rot[i].x - v.y * rot[i].y, v.x * rot[i].y + v.y * rot[i].x);
     }
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 a = to_f32x2(T{}, x.w[i]), b = to_f32x2(T{}, x.w[4 + i]);
+      const float2 a = unpack2(T{}, x.w[i]), b = unpack2(T{}, x.w[4 + i]);
       const float2 r0 = rot[2 * i], r1 = rot[2 * i + 1];
       x.w[i] = pack2(T{}, a.x * r0.x - b.x * r0.y, a.y * r1.x - b.y * r1.y);
       x.w[4 + i] = pack2(T{}, a.x * r0.y + b.x * r0.x, a.y * r1.y + b.y * r1.x);

@@ -9,16 +9,13 @@
 
 namespace qwen {
 
-// fp16 / bf16 value types behind the 16-bit patterns of the C ABI.
-__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <typename T>
-__device__ __forceinline__ T from_f32(float x);
-template <>
-__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
-
+// Two 16-bit values of either type in a word, and their fp32 values.
+__device__ __forceinline__ float2 unpack2(__half, uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+__device__ __forceinline__ float2 unpack2(__nv_bfloat16, uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
 __device__ __forceinline__ uint32_t pack2(__half, float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -76,23 +73,6 @@ __device__ __forceinline__ bool paged_wait(uint64_t* bar, uint32_t parity, volat
                                            bool heed = true) {
   return mbar_try_wait(bar, parity) || paged_wait_slow(bar, parity, abort, err, heed);
 }
-// The same where the wait is short and on the critical path: polls that do not
-// suspend the warp come first.
-__device__ __forceinline__ bool paged_spin(uint64_t* bar, uint32_t parity, volatile int* abort, int* err) {
-  for (int i = 0; i < 256; ++i) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.test_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    if (ok) return true;
-  }
-  return paged_wait_slow(bar, parity, abort, err, true);
-}
-
 // 5-D tile load (element, slot, half, head, page) of a cache's tensor map; the
 // box is (64, rows, head_dim / 64, 1, 1), so it lands as [half][rows][128 B].
 __device__ __forceinline__ void tma_load_pages(void* dst, const CUtensorMap* map, int slot, int head,

@@ -704,7 +704,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       for (int k = 0; k < V; ++k) v[k] = 0.f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        sum += ml[w][head].x == -INFINITY ? 0.f : ml[w][head].y * exp2_fast(ml[w][head].x - M);
+        // (a warp without a maximum has the sum 0, or NaN, which stays)
+        sum += ml[w][head].y * (ml[w][head].x == -INFINITY ? 0.f : exp2_fast(ml[w][head].x - M));
         const float* row = rows + (w * 8 * NT + head) * D + ((V * lane) ^ (8 * (head / 2 % 4)));
 #pragma unroll
         for (int k = 0; k < V; ++k) v[k] += row[k];
@@ -835,7 +836,6 @@ bool paged_decode_fits(const qwen_paged_kv& kv, int n_heads, int n_list) {
 }
 
 size_t paged_decode_workspace(const qwen_paged_kv& kv, int n_heads) {
-  if (kv.n_kv_heads == 0 || n_heads < (int)kv.n_kv_heads) return 0;   // refused later
   const size_t G = kCtasPerSm * paged_sm_count(), units = (size_t)kv.n_seq * kv.n_kv_heads * units_per_head(kv, n_heads);
   return 2 * G * kMaxSlotHeads * (kv.head_dim + 2) * sizeof(float) + (2 * G + units) * sizeof(unsigned long long);
 }

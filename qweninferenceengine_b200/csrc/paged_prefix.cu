@@ -745,7 +745,7 @@ Layout layout(const PrefixArgs& p, const qwen_paged_kv& kv, int n_heads, int G) 
 }  // namespace
 
 size_t paged_prefix_workspace(const qwen_paged_kv& kv, int n_heads, uint32_t prefix_len) {
-  if (prefix_len == 0 || kv.n_kv_heads == 0 || n_heads < (int)kv.n_kv_heads) return paged_decode_workspace(kv, n_heads);
+  if (prefix_len == 0) return paged_decode_workspace(kv, n_heads);
   PrefixArgs p{};
   plan(p, kv, n_heads, prefix_len, paged_sm_count());
   return layout(p, kv, n_heads, paged_sm_count()).bytes;

@@ -39,11 +39,6 @@ __device__ __forceinline__ u64 score_key(double x) {
   return b >> 63 ? ~b : b | 0x8000000000000000ull;
 }
 
-__device__ __forceinline__ float2 unpack2(__half, uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
-__device__ __forceinline__ float2 unpack2(__nv_bfloat16, uint32_t w) {
-  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-}
-
 // CTA: pages [pages_per_cta * blockIdx.x, ..) of sequence blockIdx.y, all kv heads.  A
 // warp keeps one kv head's Q+- in registers; a group of D / 4 lanes reads a page's
 // bounds, lower half lo and upper half hi, 8 elements a lane.

@@ -290,7 +290,8 @@ def _workspace(kv: PagedKV, query: str, *sizes) -> tuple:
     if need is None:
         if len(_workspace_bytes) > 4096:
             _workspace_bytes.clear()
-        need = _workspace_bytes[key] = getattr(lib(), query)(kv.ref, *sizes)
+        with torch.cuda.device(kv.index):
+            need = _workspace_bytes[key] = getattr(lib(), query)(kv.ref, *sizes)
     return torch.empty(need, dtype=torch.uint8, device=kv.device), need
 
 

@@ -163,7 +163,7 @@ def test_append_reports_what_only_the_device_sees():
         assert status() == QWEN_ERR_INVALID_ARGUMENT
         assert torch.equal(torch.nan_to_num(c.k[page]), torch.nan_to_num(before[page]))
         c.table[1, 1] = page
-    for cu in ([0, 1, 9, 3], [0, 2, 1, 3], [-1, 1, 2, 3], [0, 3, 3, 3]):   # last: 3 new of ... lens are 20: fine
+    for cu in ([0, 1, 9, 3], [0, 2, 1, 3], [-1, 1, 2, 3], [0, 3, 3, 3]):   # the last is in order: (3, 0, 0) new
         t = torch.tensor(cu, dtype=torch.int32, device="cuda")
         ops.rope_append_paged(kv, x[:, :4], x[:, 4:6], x[:, 6:], c.seq_len, freqs(64), cu_tokens=t, out=out)
         assert status() == (QWEN_OK if cu == [0, 3, 3, 3] else QWEN_ERR_INVALID_ARGUMENT)
@@ -344,6 +344,40 @@ def test_sparse_lists_of_any_form():
     ref.assert_attention(got, ref.attention(c, 128 ** -0.5, lists=pages))
 
 
+def test_nan_keys_show_in_their_rows_alone():
+    """A NaN among the positions that count gives NaN for the heads that read it, also
+    where it is all a sequence or a prefix has."""
+    for prefix in (0, 1, 130):
+        c = ref.Cache(34, [1, 400, 0, 33], 12, 2, 128, 32, F16, prefix=prefix)
+        kv = c.handle()
+        c.k[int(c.table[0, 0]), 0, 1] = math.nan
+        c.k[int(c.table[1, 7]), 3, 0] = math.nan
+        bad = torch.zeros((4, 12), dtype=torch.bool, device="cuda")
+        bad[0, 6:] = bad[1, :6] = True
+        for shared in (False, True):
+            if shared and prefix:
+                c.k[int(c.prefix_pages[0]), 0, 1] = math.nan
+                bad[:, 6:] = True
+            out, lse = ops.attention_prefix_paged(kv, c.q, c.seq_len, c.prefix_pages, prefix, return_lse=True)
+            assert torch.isnan(out[bad]).all() and torch.isnan(lse[bad]).all()
+            want, want_lse, tol, lse_tol = ref.attention(c, 128 ** -0.5)
+            ref.assert_attention((out[~bad], lse[~bad]), (want[~bad], want_lse[~bad], tol[~bad], lse_tol[~bad]))
+
+
+def test_attention_in_place():
+    c = ref.Cache(35, [5000, 1, 0, 300], 12, 2, 128, 32, BF16, prefix=500)
+    kv, q = c.handle(), c.q.clone()
+    c.prefix, want = 0, {}
+    want[0] = ref.attention(c, 128 ** -0.5)
+    c.prefix = 500
+    want[500] = ref.attention(c, 128 ** -0.5)
+    for prefix in (0, 500):
+        x = q.clone()
+        got = ops.attention_prefix_paged(kv, x, c.seq_len, c.prefix_pages, prefix, out=x, return_lse=True)
+        assert got[0] is x
+        ref.assert_attention(got, want[prefix])
+
+
 # ------------------------------------------------- reports, streams, graphs --
 def test_attention_reports_what_only_the_device_sees():
     c = ref.Cache(41, [40, 60, 33], 12, 2, 128, 16, F16, width=4)
@@ -457,6 +491,38 @@ def test_captured_and_replayed():
         for (c, kv), g, qkv, out in zip(caches, graphs, ins, outs):
             c.seq_len += 1
             qkv.copy_(c.randn(4, 16, 128))
+            g.replay()
+            check_step(c, out)
+
+
+@pytest.mark.parametrize("fill", [0, 0xFF, None])
+def test_workspace_of_any_contents(fill, monkeypatch):
+    """One workspace for all calls, whatever it holds; then shared by two captured graphs."""
+    sized = ops._workspace
+    memory = torch.randint(0, 256, (1 << 26,), dtype=torch.uint8, device="cuda")
+    if fill is not None:
+        memory.fill_(fill)
+
+    def given(kv, query, *sizes):
+        need = sized(kv, query, *sizes)[1]
+        assert need <= memory.numel()
+        return memory, need
+
+    monkeypatch.setattr(ops, "_workspace", given)
+    inv = freqs(128)
+    work = []
+    for seed in (63, 64):
+        c = serving_cache(seed, BF16)
+        c.seq_len += 1
+        kv, qkv = c.handle(), c.randn(4, 16, 128)
+        check_step(c, one_step(c, kv, qkv, inv))
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = one_step(c, kv, qkv, inv)
+        work.append((c, g, out, qkv))   # the graph reads qkv's memory
+    for _ in range(3):
+        for c, g, out, _ in work:
             g.replay()
             check_step(c, out)
 

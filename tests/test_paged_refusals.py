@@ -144,6 +144,30 @@ def test_no_sequences_is_nothing_to_do():
     assert append(kv(), n=0, cu=A, q=None, k=None, v=None, out=None) == _lib.QWEN_OK
 
 
+@pytest.mark.parametrize("fields,heads,length", [
+    (dict(n_seq=0), 12, 100), (dict(n_seq=0xFFFFFFFF), 12, 100), (dict(n_kv_heads=0), 12, 100), (dict(), 0, 100),
+    (dict(), 13, 100), (dict(), 0xFFFFFFFE, 100), (dict(n_kv_heads=0xFFFFFFFF), 0xFFFFFFFF, 100),
+    (dict(max_pages=0xFFFFFFFF), 12, 100)])
+def test_no_workspace_for_what_is_refused(fields, heads, length):
+    s = ctypes.byref(kv(**fields))
+    assert lib().qwen_attention_paged_workspace(s, heads) == 0
+    assert lib().qwen_attention_prefix_paged_workspace(s, heads, length) == 0
+    assert lib().qwen_attention_sparse_paged_workspace(s, heads, 4) == 0
+
+
+def test_workspace_queries():
+    s = ctypes.byref(kv())
+    assert lib().qwen_attention_prefix_paged_workspace(s, 12, 0xFFFFFFFF) == 0
+    own = lib().qwen_attention_paged_workspace(s, 12)
+    assert 0 < own == lib().qwen_attention_prefix_paged_workspace(s, 12, 0)
+    assert own < lib().qwen_attention_prefix_paged_workspace(s, 12, 1 << 24)
+    assert lib().qwen_select_pages_workspace(s) == 3 * 2 * 8 * 8
+    for q in (lib().qwen_attention_paged_workspace, lib().qwen_attention_sparse_paged_workspace,
+              lib().qwen_attention_prefix_paged_workspace, lib().qwen_select_pages_workspace):
+        assert q(None, *[12, 4][:len(q.argtypes) - 1]) == 0
+    assert lib().qwen_select_pages_workspace(ctypes.byref(kv(n_kv_heads=0))) == 0
+
+
 def test_python_handle_is_packed_as_the_struct_is_laid_out():
     from qweninferenceengine_b200 import ops
 
