@@ -10,20 +10,22 @@
 // sum.
 //
 // k_page_scores streams the bounds (HBM: 512 B a page and kv head of 128) into one
-// 64-bit key a page whose order is the scores'; the conversions to 64 bits, 16 a
-// clock and SM, take nearly as long as the stream and run beside it.
+// 64-bit key a page whose order is the scores'.  16 x 2048 pages of 8 heads, 134 MB:
+// 34 us, 4.0 TB/s; 29 us without the conversions to 64 bits (16 a clock and SM).
 // k_page_list picks, a CTA per kv head and sequence: bins the keys linearly between
 // their least and greatest (2048 bins), finds the bin that the last place falls
 // in, and goes on inside it -- one round where scores are spread, and a round per 11
 // bits at worst -- until the bin is taken whole, small enough to rank directly, or
-// one value.
+// one value.  Bound by latency: 10 us for 2048 pages, a dozen barriers and round trips.
+#include <algorithm>
+
 #include "paged_common.cuh"
 #include "qwen_internal.h"
 
 namespace qwen {
 namespace {
 
-constexpr int kScoreWarps = 8;
+constexpr int kScoreWarps = 8, kScoreCtas = 2;   // of an SM
 constexpr int kBatch = 8;             // pages a warp has in flight
 constexpr int kListThreads = 512;
 constexpr int kBins = 2048;
@@ -39,51 +41,34 @@ __device__ __forceinline__ u64 score_key(double x) {
   return b >> 63 ? ~b : b | 0x8000000000000000ull;
 }
 
-// CTA: pages [pages_per_cta * blockIdx.x, ..) of sequence blockIdx.y, all kv heads.  A
-// warp keeps one kv head's Q+- in registers; a group of D / 4 lanes reads a page's
-// bounds, lower half lo and upper half hi, 8 elements a lane.
+__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+
+// Pages of a sequence of length L that compete for a place on its list (0: all are
+// on it, or the length is refused).
+__device__ __forceinline__ uint32_t scored_pages(const PagedSelectArgs& a, uint32_t L) {
+  if (L > a.kv.max_pages * a.kv.page_size) return 0;
+  const uint32_t n = (L + a.kv.page_size - 1) >> a.page_shift;
+  return n > (uint32_t)a.n_select ? n : 0;
+}
+
+// Pages [begin, end) of sequence s, all kv heads, by the CTA's warps.  A warp keeps one
+// kv head's Q+- in registers; a group of D / 4 lanes reads a page's bounds, lower half
+// lo and upper half hi, 8 elements a lane.
 template <typename T, int D>
-__global__ void __launch_bounds__(kScoreWarps * 32, 2) k_page_scores(const __grid_constant__ PagedSelectArgs a,
-                                                                  int pages_per_cta) {
+__device__ __forceinline__ void score_pages(const PagedSelectArgs& a, int s, int begin, int end, int warp, int lane,
+                                            uint4 (&held)[2][kBatch][32]) {
   constexpr int kLanes = D / 4, kAtOnce = 32 / kLanes;   // lanes of a page, pages of a load
-  pdl_wait();
-  if (threadIdx.x == 0) pdl_launch_dependents();
-  const int s = blockIdx.y, K = a.kv.n_kv_heads, G = a.n_heads / K;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  bool ok;
-  const int L = (int)checked_len(a.kv, a.seq_len, s, &ok);
-  if (!ok) {
-    if (threadIdx.x == 0 && blockIdx.x == 0) raise_error(a.err, kDevBadArgument);
-    return;
-  }
-  const int n = (L + a.kv.page_size - 1) >> a.page_shift;
-  const int begin = blockIdx.x * pages_per_cta, end = min(n, begin + pages_per_cta);
-  if (n <= a.n_select || begin >= end) return;
-  const int32_t* table = a.kv.page_table + (long long)s * a.kv.table_stride;
+  const int K = a.kv.n_kv_heads, G = a.n_heads / K;
   // warps per head, where there are fewer heads than warps
   const int share = K >= kScoreWarps ? 1 : kScoreWarps / K;
   const int part = lane & (kLanes - 1), sub = lane / kLanes;
   const bool upper = part >= kLanes / 2;
   const int d0 = 8 * (part & (kLanes / 2 - 1));
+  const int32_t* table = a.kv.page_table + (long long)s * a.kv.table_stride;
 #pragma unroll 1
   for (int h = warp / share; h < K; h += kScoreWarps / share) {
-    double w[8];
-    uint32_t used[4];   // bounds that no query multiplies read as 0 (they may be infinite)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = 0;
-    for (int g = 0; g < G; ++g) {
-      const uint4 x = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + s * a.q_stride +
-                                                      (long long)(h * G + g) * D + d0);
-      const uint32_t b[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 v = unpack2(T{}, b[i]);
-        w[2 * i] += (v.x > 0.f) == upper ? v.x : 0.f;   // NaN goes to the lower half
-        w[2 * i + 1] += (v.y > 0.f) == upper ? v.y : 0.f;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) used[i] = (w[2 * i] != 0 ? 0xffffu : 0u) | (w[2 * i + 1] != 0 ? 0xffff0000u : 0u);
     u64* keys = reinterpret_cast<u64*>(a.scores) + ((long long)s * K + h) * a.kv.max_pages;
     const T* bounds = reinterpret_cast<const T*>(a.kv.bounds) + (upper ? (long long)K * D : 0) + (long long)h * D + d0;
     constexpr int kPages = kBatch * kAtOnce;
@@ -101,19 +86,41 @@ __global__ void __launch_bounds__(kScoreWarps * 32, 2) k_page_scores(const __gri
       }
       return page;
     };
-    auto fetch = [&](int page, uint4 (&x)[kBatch]) {
+    // A lane copies what it reads itself, so that no one else waits for it.
+    auto fetch = [&](int page, int stage) {
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
         const long long at = max(__shfl_sync(0xffffffffu, page, i * kAtOnce + sub), 0);
-        x[i] = __ldg(reinterpret_cast<const uint4*>(bounds + at * 2 * K * D));
+        cp_async16(&held[stage][i][lane], bounds + at * 2 * K * D);
       }
+      asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    auto score = [&](int p0, int page, const uint4 (&x)[kBatch]) {
+    int page0 = page_of(p_first), page1 = page_of(p_first + step), stage = 0;
+    fetch(page0, 0);
+    double w[8];
+    uint32_t used[4];   // bounds that no query multiplies read as 0 (they may be infinite)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = 0;
+    for (int g = 0; g < G; ++g) {
+      const uint4 x = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + s * a.q_stride +
+                                                      (long long)(h * G + g) * D + d0);
+      const uint32_t b[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 v = unpack2(T{}, b[i]);
+        w[2 * i] += (v.x > 0.f) == upper ? v.x : 0.f;   // NaN goes to the lower half
+        w[2 * i + 1] += (v.y > 0.f) == upper ? v.y : 0.f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) used[i] = (w[2 * i] != 0 ? 0xffffu : 0u) | (w[2 * i + 1] != 0 ? 0xffff0000u : 0u);
+    auto score = [&](int p0, int page, const uint4 (&x)[kBatch][32]) {
       const uint32_t bads = __ballot_sync(0xffffffffu, page < 0);
       double sum[kBatch];
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
-        const uint32_t b[4] = {x[i].x & used[0], x[i].y & used[1], x[i].z & used[2], x[i].w & used[3]};
+        const uint4 y = x[i][lane];
+        const uint32_t b[4] = {y.x & used[0], y.y & used[1], y.z & used[2], y.w & used[3]};
         sum[i] = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -140,21 +147,61 @@ __global__ void __launch_bounds__(kScoreWarps * 32, 2) k_page_scores(const __gri
       const int at = i * kAtOnce + sub;
       if (part < 8 && p0 + at < end) keys[p0 + at] = bads >> at & 1 ? 0 : score_key(sum[0]);
     };
-    uint4 x0[kBatch], x1[kBatch];
-    int page0 = page_of(p_first), page1 = page_of(p_first + step);
-    fetch(page0, x0);
 #pragma unroll 1
-    for (int p0 = p_first; p0 < end; p0 += 2 * step) {
-      fetch(page1, x1);
-      const int next0 = page_of(p0 + 2 * step);
-      score(p0, page0, x0);
-      page0 = next0;
-      if (p0 + step >= end) break;
-      fetch(page0, x0);
-      const int next1 = page_of(p0 + 3 * step);
-      score(p0 + step, page1, x1);
-      page1 = next1;
+    for (int p0 = p_first; p0 < end; p0 += step) {
+      fetch(page1, stage ^ 1);
+      const int next = page_of(p0 + 2 * step);
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      score(p0, page0, held[stage]);
+      page0 = page1;
+      page1 = next;
+      stage ^= 1;
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+  }
+}
+
+// The scored pages of all sequences stand in one row, and each CTA takes an equal run
+// of it.  (A CTA for 64 pages of a sequence, with the batches on their way in registers:
+// 51 us for both kernels at the size above, 44.5 us so.)
+template <typename T, int D>
+__global__ void __launch_bounds__(kScoreWarps * 32, kScoreCtas) k_page_scores(const __grid_constant__ PagedSelectArgs a) {
+  extern __shared__ uint4 smem[];   // [warp][stage][load][lane]
+  auto held = reinterpret_cast<uint4(*)[2][kBatch][32]>(smem);
+  pdl_wait();
+  if (threadIdx.x == 0) pdl_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n_seq = a.kv.n_seq;
+  // The run [x, x1), the sequence that holds x and the pages before it: each warp scans
+  // the lengths.
+  const int per_lane = (n_seq + 31) / 32, s0 = min(n_seq, lane * per_lane), s1 = min(n_seq, s0 + per_lane);
+  u64 sum = 0;
+#pragma unroll 4
+  for (int i = s0; i < s1; ++i) {
+    const uint32_t L = a.seq_len[i];
+    if (L > a.kv.max_pages * a.kv.page_size && blockIdx.x == 0) raise_error(a.err, kDevBadArgument);
+    sum += scored_pages(a, L);
+  }
+  u64 inc = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 v = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += v;
+  }
+  const u64 total = __shfl_sync(0xffffffffu, inc, 31), per = divide(total + gridDim.x - 1, gridDim.x);
+  u64 x = blockIdx.x * per;
+  const u64 x1 = min(total, x + per);
+  if (x >= x1) return;
+  const int from = __ffs(__ballot_sync(0xffffffffu, x < inc)) - 1;   // the lane whose sequences hold x
+  u64 before = __shfl_sync(0xffffffffu, inc - sum, from);
+#pragma unroll 1
+  for (int s = __shfl_sync(0xffffffffu, s0, from); x < x1; ++s) {
+    const uint32_t n = scored_pages(a, a.seq_len[s]);
+    if (x < before + n) {
+      const u64 end = min((u64)n, x1 - before);
+      score_pages<T, D>(a, s, (int)(x - before), (int)end, warp, lane, held[warp]);
+      x = before + end;
+    }
+    before += n;
   }
 }
 
@@ -344,19 +391,24 @@ __global__ void __launch_bounds__(kListThreads) k_page_list(const __grid_constan
 
 template <typename T, int D>
 int launch(const PagedSelectArgs& a, cudaStream_t st) {
-  // Pages of a CTA: fewer where the whole batch would not fill the SMs twice.
-  int per = 256;
-  while (per > 32 && (long long)((a.kv.max_pages + per - 1) / per) * a.kv.n_seq < 2 * paged_sm_count()) per /= 2;
+  // As many CTAs as run at once, fewer where that would leave a warp less than a batch of pages.
+  const int share = std::max(1, kScoreWarps / (int)a.kv.n_kv_heads), least = share * kBatch * 32 / (D / 4);
+  const long long pages = (long long)a.kv.max_pages * a.kv.n_seq;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((a.kv.max_pages + per - 1) / per, a.kv.n_seq);
+  cfg.gridDim = dim3((unsigned)std::min((long long)kScoreCtas * paged_sm_count(), (pages + least - 1) / least));
   cfg.blockDim = dim3(kScoreWarps * 32);
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, k_page_scores<T, D>, a, per) != cudaSuccess) return -1;
+  constexpr int kSmem = kScoreWarps * 2 * kBatch * 32 * (int)sizeof(uint4);
+  cfg.dynamicSmemBytes = kSmem;
+  static OncePerDevice scores;
+  if (scores.launch(reinterpret_cast<const void*>(k_page_scores<T, D>), kSmem,
+                    [&] { return cudaLaunchKernelEx(&cfg, k_page_scores<T, D>, a); }) != cudaSuccess)
+    return -1;
   cfg.gridDim = dim3(a.kv.n_kv_heads, a.kv.n_seq);
   cfg.blockDim = dim3(kListThreads);
   cfg.dynamicSmemBytes = (size_t)(a.kv.max_pages < (uint32_t)kCached ? a.kv.max_pages : kCached) * sizeof(u64);
