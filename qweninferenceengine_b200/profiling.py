@@ -104,7 +104,7 @@ def run_paged(batch: int, ctx: int, page: int, prefix: int, select: int, reps: i
     for name, call in calls.items():
         times = []
         for _ in range(reps):
-            flush.zero_()   # caches larger than L2 between the timed calls
+            flush.zero_()   # nothing of the cache is left in L2
             a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
             a.record()
             call()
