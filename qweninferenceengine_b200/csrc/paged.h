@@ -34,9 +34,17 @@ struct PagedAttnArgs {
   int* err;                     // operator status word
 };
 // Decode attention over own or listed pages (paged_decode.cu); 0, or -1 for a
-// launch failure.  own_o, own_ml: where set, unnormalised rows and (max, sum) per
-// query head go there instead of outputs.
-int launch_paged_decode(const PagedAttnArgs& a, cudaStream_t st, float* own_o = nullptr, float2* own_ml = nullptr);
+// launch failure.  Beside a kernel that reads a shared prefix (the launch before it, which
+// it does not wait for, though its end does): o, ml get unnormalised rows and (max,
+// sum) per query head instead of outputs, and up to few_tiles tiles are divided among
+// the `few` CTAs that find room at once.
+struct PagedOwn {
+  float* o = nullptr;
+  float2* ml = nullptr;
+  int few = 1;
+  uint32_t few_tiles = 0;
+};
+int launch_paged_decode(const PagedAttnArgs& a, cudaStream_t st, const PagedOwn& own = {});
 // Whether its tiles can be counted in 31 bits; n_list: listed pages, 0 without a list.
 bool paged_decode_fits(const qwen_paged_kv& kv, int n_heads, int n_list);
 size_t paged_decode_workspace(const qwen_paged_kv& kv, int n_heads);

@@ -98,6 +98,7 @@ struct __align__(1024) DecodeSmem {
   uint64_t full[kStages], empty[kStages], qfull[query_slots<NT>()], qempty[query_slots<NT>()], joined, early;
   CutPiece cut[2];
   int n_cut, n_early;   // cut pieces; of those counted in before the end
+  int runs;
   int last[2];
   int abort;
 };
@@ -116,6 +117,8 @@ struct DecodeArgs {
   unsigned long long tag;
   float* own_o;             // if set: unnormalised rows [n_seq][n_heads][D] and their (max,
   float2* own_ml;           //   sum) go here instead of outputs, for the shared-prefix join
+  uint32_t few_tiles;       // up to so many tiles are divided among `few` CTAs only
+  int few;
 };
 
 __device__ __forceinline__ uint32_t seq_tiles(const DecodeArgs& p, uint32_t L) {
@@ -140,9 +143,9 @@ __device__ __forceinline__ int piece_slot(const CutPiece& u, int i, int G) {
   return 2 * r + (i == 0 ? 1 : 0);
 }
 
-// Total number of tiles, and the sequence that holds tile run_start(total, c) with
-// its length and the number of tiles before it (one warp).
-__device__ __forceinline__ uint32_t find_run(const DecodeArgs& p, uint32_t c, uint32_t G, int lane, int* seq,
+// Total number of tiles, the number G of runs, and the sequence that holds tile
+// run_start(total, c) with its length and the number of tiles before it (one warp).
+__device__ __forceinline__ uint32_t find_run(const DecodeArgs& p, uint32_t c, uint32_t& G, int lane, int* seq,
                                              uint32_t* before, uint32_t* length) {
   const int n_seq = p.a.kv.n_seq;
   const uint32_t u = p.units_per_seq;
@@ -168,7 +171,9 @@ __device__ __forceinline__ uint32_t find_run(const DecodeArgs& p, uint32_t c, ui
     const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
     if (lane >= o) inc += v;
   }
-  const uint32_t total = __shfl_sync(0xffffffffu, inc, 31), target = run_start(total, c, G);
+  const uint32_t total = __shfl_sync(0xffffffffu, inc, 31);
+  if (total <= p.few_tiles) G = p.few;
+  const uint32_t target = run_start(total, c, G);
   uint32_t at = inc - sum * u;
   const uint32_t mine = __ballot_sync(0xffffffffu, target >= at && target < inc);
   int s = s0;
@@ -335,11 +340,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     prefetch_map(&tmv);
   }
   __syncthreads();
-  pdl_wait();
-  // After the wait: a dependent that starts before this kernel ends (k_prefix, which
-  // reads nothing of it) finds everything that came before.
+  // (Behind a shared prefix the kernel before is k_prefix, which this one runs beside: it
+  // lets this one start only once all that came before is there.)
+  if (!p.own_o) pdl_wait();
   if (threadIdx.x == 0) pdl_launch_dependents();
-  const int c = blockIdx.x, G = gridDim.x;
+  const int c = blockIdx.x;
 
   if (warp >= kWarps) {
     // ------------------------------------------------------------ producer --
@@ -354,10 +359,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     const uint32_t box_at = (uint32_t)slice / per_box * box_bytes;
     uint32_t it = 0, pieces = 0;
     int seq, n_cut = 0;
-    uint32_t before, L;
+    uint32_t before, L, G = gridDim.x;
     const uint32_t total = find_run(p, c, G, lane, &seq, &before, &L);
-    const uint32_t t1 = run_start(total, c + 1, G);
-    uint32_t t = run_start(total, c, G), ts = seq_tiles(p, L);
+    const uint32_t t1 = c < (int)G ? run_start(total, c + 1, G) : 0;
+    uint32_t t = run_start(total, c, G), ts = seq_tiles(p, L);   // (c >= G: no run)
     int cached_unit = -1, cached_base = 0, page = -1, left = 0, next_page = -1;   // lane i: entry cached_base + i
     bool alive = true, cut_first = false;
 #pragma unroll 1
@@ -459,10 +464,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         u.head = head;
         u.heads = heads;
         u.unit = seq * p.units_per_seq + (int)unit;
-        u.pieces = total < (unsigned)G ? (int)ts : run_of(total, begin + ts - 1, G) - run0 + 1;
-        u.piece = total < (unsigned)G ? (int)tile0 : c - run0;
+        u.pieces = total < G ? (int)ts : run_of(total, begin + ts - 1, G) - run0 + 1;
+        u.piece = total < G ? (int)tile0 : c - run0;
         u.run0 = run0;
-        u.total = min(total, (uint32_t)G);
+        u.total = min(total, G);
         u.begin = begin;
         if (lane == 0) s.cut[n_cut] = u;
         if (pieces == 1) cut_first = true;
@@ -485,6 +490,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       }
       if (lane == 0) {
         s.n_cut = n_cut;
+        s.runs = (int)G;
         s.n_early = n_early;
       }
       __syncwarp();
@@ -509,6 +515,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
 #pragma unroll 1
     for (uint32_t j = pieces > (uint32_t)QS ? pieces - QS : 0; j < pieces; ++j)
       paged_wait(&s.qfull[j % QS], (j / QS) & 1, &s.abort, a.err, false);
+    if (p.own_o && is_k && c == (int)gridDim.x - 1) pdl_wait();   // so that whoever waits for this kernel finds k_prefix done too
     return;
   }
 
@@ -727,7 +734,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   }
 
   // ---- the last pieces to arrive join the others'
-  const int n_cut = s.n_cut, n_early = s.n_early;
+  const int n_cut = s.n_cut, n_early = s.n_early, G = s.runs;
   if (n_cut == 0) return;
   if (!join()) return;   // every warp's partials are written
   if (threadIdx.x == 0 && n_early < n_cut) s.last[n_early] = arrive_first(p, s.cut[n_early], G);
@@ -848,7 +855,7 @@ size_t paged_decode_workspace(const qwen_paged_kv& kv, int n_heads) {
   return 2 * G * kMaxSlotHeads * (kv.head_dim + 2) * sizeof(float) + (2 * G + units) * sizeof(unsigned long long);
 }
 
-int launch_paged_decode(const PagedAttnArgs& a, cudaStream_t st, float* own_o, float2* own_ml) {
+int launch_paged_decode(const PagedAttnArgs& a, cudaStream_t st, const PagedOwn& own) {
   DecodeArgs p{};
   p.a = a;
   p.chunks = units_per_head(a.kv, a.n_heads);
@@ -863,8 +870,10 @@ int launch_paged_decode(const PagedAttnArgs& a, cudaStream_t st, float* own_o, f
   p.part_ml = p.part_o + (size_t)2 * G * kMaxSlotHeads * a.kv.head_dim;
   p.arrived = reinterpret_cast<unsigned long long*>(p.part_ml + (size_t)2 * G * kMaxSlotHeads * 2);
   p.tag = next_tag();
-  p.own_o = own_o;
-  p.own_ml = own_ml;
+  p.own_o = own.o;
+  p.own_ml = own.ml;
+  p.few = own.few;
+  p.few_tiles = own.few_tiles;
   // Boxes of 32 positions, or 16 where a page holds no more: a sequence's last
   // page costs at most 31 positions of traffic that do not count.
   const int box_rows = a.kv.page_size < 32 ? 16 : 32;

@@ -12,25 +12,30 @@
 // kernel is 1% faster.
 //
 // Three launches, each a programmatic dependent of the one before:
-//   k_paged_decode (paged_decode.cu)  every sequence's own positions; it leaves
-//       (max, sum, unnormalised row) per query head instead of outputs
-//   k_prefix        below; starts while the former's last CTAs still run
+//   k_prefix        below, on part of the SMs
+//   k_paged_decode (paged_decode.cu)  every sequence's own positions, beside it: on the
+//       other SMs, or, where those would take longer, on all of them in the end; it
+//       leaves (max, sum, unnormalised row) per query head instead of outputs
 //   k_prefix_join   per query head: own part and the prefix's partials, in a fixed
 //       order, into out and lse
-// Of 256 sequences behind 32768 positions, 12 query and 2 kv heads, with 65 .. 257 own
-// ones (73 us) they take about 18, 45 and 5 us.
+// One is arithmetic, the other a stream, and each spends 5 to 8 us on its beginning and
+// end.  One after the other / side by side: 64 sequences behind 8704 positions with 75
+// to 300 own ones, 32 query and 8 kv heads 43.4 / 34.9 us; 256 behind 32768 with 65 to
+// 257, 12 and 2 heads 73.1 / 61.5 us (55 us of it k_prefix, 5 us the join).
 //
 // k_prefix: a unit is a kv head and 256 rows (two tiles of M = 128; an odd last
 // tile stands alone), its steps the prefix's 128-position tiles.  With fewer units
 // than SMs each gets a whole number of CTAs, by its MMAs, which share its steps:
 // a CTA that went on from one unit to the next would load queries and store
-// partials twice (~5 us; 8 units of 68 steps took 57 us so, 44 us for the CTAs
-// with one unit).  With more, all steps stand in one row, weighted by their MMAs,
+// partials twice (~5 us; a call with 8 units of 68 steps took 57 us so, 44 us with
+// one unit a CTA).  With more, all steps stand in one row, weighted by their MMAs,
 // and one CTA per SM takes an equal run of it.  Warps of a CTA:
 //   0-7, 8-15  softmax of stream 0 and 1: a thread has half a row (64 scores) of S
 //       from tensor memory, and puts the weights back over it as fp16 / bf16 (P);
 //       the two halves of a row agree on its maximum through shared memory
-//   16 producer: page table, TMA loads of K and V tiles into a 5-slot ring
+//   16 producer: page table, TMA loads of tiles, three of K and two of V held, K's a
+//       step ahead (in one ring of five, K of the second next step waited for V of
+//       this one: 128 rows behind 32768 positions took 36 us, 24 us so)
 //   17 MMA issue: S = Q K^T (smem x smem), O += P V (tensor memory x smem, V read
 //       N-major as it lies in the pool)
 // The two streams are the unit's two row tiles over the same K / V slots; a lone
@@ -52,7 +57,7 @@ namespace {
 
 constexpr int kRows = 128;                 // rows of a stream (M)
 constexpr int kPos = 128;                  // positions of a tile
-constexpr int kSlots = 5;
+constexpr int kKSlots = 3, kVSlots = 2;    // tiles of K and of V held
 constexpr uint32_t kSmemBytes = 227 * 1024;
 constexpr int kPrefixThreads = 576;
 constexpr int kProducer = 16, kIssuer = 17;
@@ -143,9 +148,9 @@ struct Pieces {
 template <int D>
 struct PrefixSmem {   // on a 1024-byte boundary
   uint8_t q[2][kRows * D * 2];             // [half][row][128 B], swizzled
-  uint8_t kv[kSlots][kPos * D * 2];
-  uint64_t full[kSlots], empty[kSlots], qfull[2], sfull[2], pfull[2], ofull[2], done;
-  uint32_t groups[kSlots];                 // of a K slot: 16-position groups that are there
+  uint8_t k[kKSlots][kPos * D * 2], v[kVSlots][kPos * D * 2];
+  uint64_t kfull[kKSlots], kempty[kKSlots], vfull[kVSlots], vempty[kVSlots], qfull[2], sfull[2], pfull[2], ofull[2], done;
+  uint32_t groups[8];                      // of a step: 16-position groups that are there (read after K's slot is free)
   float top[2][2][kRows];                  // [stream][half][row]
   uint32_t tmem;
   int abort;
@@ -294,16 +299,19 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
   const PagedAttnArgs& a = p.a;
   if (pad + sizeof(PrefixSmem<D>) > kSmemBytes) {
     if (threadIdx.x == 0) raise_error(a.err, kDevBadArgument);
-    pdl_wait();
     return;
   }
   PrefixSmem<D>& s = *reinterpret_cast<PrefixSmem<D>*>(smem_raw + pad);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int c = blockIdx.x, G = gridDim.x;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kSlots; ++i) {
-      mbar_init(&s.full[i], 1);
-      mbar_init(&s.empty[i], 1);
+    for (int i = 0; i < kKSlots; ++i) {
+      mbar_init(&s.kfull[i], 1);
+      mbar_init(&s.kempty[i], 1);
+    }
+    for (int i = 0; i < kVSlots; ++i) {
+      mbar_init(&s.vfull[i], 1);
+      mbar_init(&s.vempty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.qfull[i], 8);
@@ -314,7 +322,6 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
     mbar_init(&s.done, 1);
     s.abort = 0;
     fence_mbar_init();
-    pdl_launch_dependents();
   }
   if (warp == kIssuer) t5_alloc(&s.tmem);
   t5_before();
@@ -322,56 +329,75 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
   t5_after();
   const uint32_t tmem = s.tmem;
   Pieces piece(p, c, G);
-  // The queries, pages and page numbers that this kernel reads come from before
-  // the own-positions kernel, which lets this one start only once those are there.
+  pdl_wait();
+  if (threadIdx.x == 0) pdl_launch_dependents();
 
   if (warp == kProducer) {
     // ------------------------------------------------------------ producer --
     const int P = a.kv.page_size, boxes = kPos / box_rows, halves = D / 64;
-    uint32_t it = 0;   // loads so far: K, V, K, V, ..
+    uint32_t nk = 0, nv = 0;   // tiles loaded so far
     bool alive = true;
+    // lane: box lane / halves of a tile, half lane % halves
+    const int box = lane / halves, half = lane % halves;
+    const bool loads = box < boxes;
+    const int at = half * kPos * 128 + box * box_rows * 128;   // in a slot
     while (alive && piece.next()) {
       const int h = piece.h, i0 = piece.i0, i1 = piece.i1;
-      for (int step = i0; step < i1 && alive; ++step) {
-        // lane: box lane / halves of a tile, half lane % halves
-        const int box = lane / halves, half = lane % halves;
-        const int pos = step * kPos + box * box_rows;
-        int page = (int)a.kv.n_pages;   // outside the pool: the box is filled with zeros
-        bool there = false;
-        if (box < boxes && pos < (int)a.prefix_len) {
-          const int x = a.prefix_pages[pos >> a.page_shift];
-          there = x >= 0 && (uint32_t)x < a.kv.n_pages;
-          if (there) page = x;
-          else raise_error(a.err, kDevBadArgument);
-        }
-        const uint32_t have = __ballot_sync(0xffffffffu, there && half == 0);
-        for (int kv = 0; kv < 2; ++kv, ++it) {
-          const int slot = it % kSlots;
-          if (it >= kSlots &&
-              !__all_sync(0xffffffffu, paged_wait(&s.empty[slot], ((it / kSlots) - 1) & 1, &s.abort, a.err))) {
+      int page = 0, next_page = 0;
+      // K of a step goes before V of the one before: a K slot is free as soon as its
+      // products are formed, and the stream that waits for it is not to wait for the
+      // weights that free a V slot.
+      for (int step = i0; step <= i1 && alive; ++step) {
+        if (step < i1) {
+          const int pos = step * kPos + box * box_rows;
+          next_page = (int)a.kv.n_pages;   // outside the pool: the box is filled with zeros
+          bool there = false;
+          if (loads && pos < (int)a.prefix_len) {
+            const int x = a.prefix_pages[pos >> a.page_shift];
+            there = x >= 0 && (uint32_t)x < a.kv.n_pages;
+            if (there) next_page = x;
+            else raise_error(a.err, kDevBadArgument);
+          }
+          const uint32_t have = __ballot_sync(0xffffffffu, there && half == 0);
+          const int slot = nk % kKSlots;
+          if (nk >= kKSlots &&
+              !__all_sync(0xffffffffu, paged_wait(&s.kempty[slot], (nk / kKSlots - 1) & 1, &s.abort, a.err))) {
             alive = false;
             break;
           }
           if (lane == 0) {
-            if (kv == 0) {
-              uint32_t groups = 0;
-              for (int b = 0; b < boxes; ++b)
-                if (have >> (b * halves) & 1) groups |= ((1u << (box_rows / 16)) - 1) << (b * box_rows / 16);
-              s.groups[slot] = groups;
-            }
-            mbar_arrive_expect_tx(&s.full[slot], kPos * D * 2);
+            uint32_t groups = 0;
+            for (int b = 0; b < boxes; ++b)
+              if (have >> (b * halves) & 1) groups |= ((1u << (box_rows / 16)) - 1) << (b * box_rows / 16);
+            s.groups[nk % 8] = groups;
+            mbar_arrive_expect_tx(&s.kfull[slot], kPos * D * 2);
           }
           __syncwarp();
-          if (box < boxes)
-            tma_load_half(s.kv[slot] + half * kPos * 128 + box * box_rows * 128, kv ? &tmv : &tmk, pos & (P - 1), half, h,
-                          page, &s.full[slot]);
+          if (loads) tma_load_half(s.k[slot] + at, &tmk, pos & (P - 1), half, h, next_page, &s.kfull[slot]);
+          ++nk;
         }
+        if (step > i0) {
+          const int slot = nv % kVSlots;
+          if (nv >= kVSlots &&
+              !__all_sync(0xffffffffu, paged_wait(&s.vempty[slot], (nv / kVSlots - 1) & 1, &s.abort, a.err))) {
+            alive = false;
+            break;
+          }
+          if (lane == 0) mbar_arrive_expect_tx(&s.vfull[slot], kPos * D * 2);
+          __syncwarp();
+          const int pos = (step - 1) * kPos + box * box_rows;
+          if (loads) tma_load_half(s.v[slot] + at, &tmv, pos & (P - 1), half, h, page, &s.vfull[slot]);
+          ++nv;
+        }
+        page = next_page;
       }
     }
     __syncwarp();
     // Every issued copy lands before the CTA may exit.
-    for (uint32_t j = it > kSlots ? it - kSlots : 0; j < it; ++j)
-      paged_wait(&s.full[j % kSlots], (j / kSlots) & 1, &s.abort, a.err, false);
+    for (uint32_t j = nk > kKSlots ? nk - kKSlots : 0; j < nk; ++j)
+      paged_wait(&s.kfull[j % kKSlots], (j / kKSlots) & 1, &s.abort, a.err, false);
+    for (uint32_t j = nv > kVSlots ? nv - kVSlots : 0; j < nv; ++j)
+      paged_wait(&s.vfull[j % kVSlots], (j / kVSlots) & 1, &s.abort, a.err, false);
   } else if (warp == kIssuer) {
     // ----------------------------------------------------------------- MMA --
     constexpr uint32_t id_s = idesc_of<T>(kPos, false), id_o = idesc_of<T>(D, true);
@@ -386,23 +412,21 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       const int cnt[2] = {w == 2 ? n : (n + 1) / 2, w == 2 ? n : n / 2};
       auto step_of = [&](int i, int k) { return w == 2 ? k : 2 * k + i; };
       auto qk = [&](int i, int k) {   // the K tile has landed
-        const uint32_t ld = base + 2 * step_of(i, k);
-        const int slot = ld % kSlots;
+        const uint32_t slot = (base + step_of(i, k)) % kKSlots;
         if (t5_elect()) {
           // +32 B of d an MMA inside the 128-byte rows, then the other half
-          const uint64_t qd = desc_k(smem_u32(s.q[i])), kd = desc_k(smem_u32(s.kv[slot]));
+          const uint64_t qd = desc_k(smem_u32(s.q[i])), kd = desc_k(smem_u32(s.k[slot]));
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk)
             t5_mma_ss(tmem + kColS + 128 * i, qd + (kk >> 2) * (kRows * 128 >> 4) + (kk & 3) * 2,
                       kd + (kk >> 2) * (kPos * 128 >> 4) + (kk & 3) * 2, id_s, kk > 0);
           t5_commit(&s.sfull[i]);
-          if (w == 1 || i == 1) t5_commit(&s.empty[slot]);
+          if (w == 1 || i == 1) t5_commit(&s.kempty[slot]);
         }
         __syncwarp();
       };
       auto pv = [&](int i, int k) -> bool {
-        const uint32_t ld = base + 2 * step_of(i, k) + 1;
-        const int slot = ld % kSlots;
+        const uint32_t slot = (base + step_of(i, k)) % kVSlots;
         // One wait for P, its V tile and the stream's next K tile: a wait on a completed
         // barrier takes ~150 cycles while MMAs run, so a softmax warp makes the other two.
         if (!wait(&s.pfull[i], pcount[i]++ & 1)) return false;
@@ -413,18 +437,18 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
           for (int x = valid * 8 + lane; x < kPos * 8; x += 32)
 #pragma unroll
             for (int half = 0; half < D / 64; ++half)
-              *reinterpret_cast<uint4*>(s.kv[slot] + half * kPos * 128 + x * 16) = make_uint4(0, 0, 0, 0);
+              *reinterpret_cast<uint4*>(s.v[slot] + half * kPos * 128 + x * 16) = make_uint4(0, 0, 0, 0);
           fence_proxy_async();
           __syncwarp();
         }
         if (t5_elect()) {
-          const uint64_t vd = desc_n(smem_u32(s.kv[slot]));   // +16 positions of 128 B an MMA
+          const uint64_t vd = desc_n(smem_u32(s.v[slot]));   // +16 positions of 128 B an MMA
 #pragma unroll
           for (int kk = 0; kk < kPos / 16; ++kk)
             t5_mma_ts(tmem + kColO + 128 * i, tmem + kColS + 128 * i + 8 * kk, vd + kk * (2048 >> 4), id_o,
                       k > 0 || kk > 0);
           t5_commit(&s.ofull[i]);
-          if (w == 1 || i == 1) t5_commit(&s.empty[slot]);
+          if (w == 1 || i == 1) t5_commit(&s.vempty[slot]);
         }
         __syncwarp();
         return true;
@@ -434,8 +458,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       t5_after();
       for (int i = 0; i < 2 && alive; ++i)
         if (cnt[i] > 0) {
-          const uint32_t ld = base + 2 * step_of(i, 0);
-          alive = wait(&s.full[ld % kSlots], (ld / kSlots) & 1);
+          const uint32_t ld = base + step_of(i, 0);
+          alive = wait(&s.kfull[ld % kKSlots], (ld / kKSlots) & 1);
           t5_after();
           if (alive) qk(i, 0);
         }
@@ -444,7 +468,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
           if (k < cnt[i]) alive = pv(i, k);
           if (alive && k + 1 < cnt[i]) qk(i, k + 1);
         }
-      base += 2 * n;
+      base += n;
     }
     // All MMAs have completed before tensor memory is freed.
     if (lane == 0) t5_commit(&s.done);
@@ -495,13 +519,13 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       for (int k = 0; k < cnt; ++k) {
         const int step = w == 2 ? k : 2 * k + i;
         if ((warp & 7) == 0) {   // for the issuer: this step's V tile, the stream's next K tile
-          const uint32_t ld = base + 2 * step + 1, next = base + 2 * (w == 2 ? k + 1 : 2 * k + 2 + i);
-          wait(&s.full[ld % kSlots], (ld / kSlots) & 1);
-          if (k + 1 < cnt) wait(&s.full[next % kSlots], (next / kSlots) & 1);
+          const uint32_t ld = base + step, next = base + (w == 2 ? k + 1 : 2 * k + 2 + i);
+          wait(&s.vfull[ld % kVSlots], (ld / kVSlots) & 1);
+          if (k + 1 < cnt) wait(&s.kfull[next % kKSlots], (next / kKSlots) & 1);
         }
         wait(&s.sfull[i], scount++ & 1);
         t5_after();
-        const uint32_t groups = s.groups[(base + 2 * step) % kSlots] >> (4 * half);
+        const uint32_t groups = s.groups[(base + step) % 8] >> (4 * half);
         const int valid = (int)a.prefix_len - (i0 + step) * kPos - 64 * half;
         const bool whole = (groups & 15u) == 15u && valid >= 64;
         if (!whole) {   // scores of what is not there never win: written back over S
@@ -613,10 +637,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         }
       }
       t5_before();
-      base += 2 * n;
+      base += n;
     }
   }
-  pdl_wait();   // so that the join, which waits for this kernel, also finds the own parts
   t5_before();
   __syncthreads();
   if (warp == kIssuer) t5_free(tmem);
@@ -695,7 +718,8 @@ __global__ void __launch_bounds__(256) k_prefix_join(const __grid_constant__ Pre
 }
 
 template <typename T, int D>
-int launch(const PrefixArgs& p, int G, const CUtensorMap& tmk, const CUtensorMap& tmv, int box_rows, cudaStream_t st) {
+int launch(const PrefixArgs& p, const PagedOwn& own, int G, const CUtensorMap& tmk, const CUtensorMap& tmv, int box_rows,
+           cudaStream_t st) {
   auto kern = k_prefix<T, D>;
   const int smem = (int)kSmemBytes;
   static_assert(sizeof(PrefixSmem<D>) <= kSmemBytes - 768, "shared memory");
@@ -714,6 +738,7 @@ int launch(const PrefixArgs& p, int G, const CUtensorMap& tmk, const CUtensorMap
         return cudaLaunchKernelEx(&cfg, kern, p, box_rows, tmk, tmv);
       }) != cudaSuccess)
     return -1;
+  if (launch_paged_decode(p.a, st, own) != 0) return -1;
   const long long rows = (long long)p.a.kv.n_seq * p.a.n_heads;
   cfg.gridDim = dim3((unsigned)((rows + 7) / 8));
   cfg.blockDim = dim3(256);
@@ -721,16 +746,39 @@ int launch(const PrefixArgs& p, int G, const CUtensorMap& tmk, const CUtensorMap
   return cudaLaunchKernelEx(&cfg, k_prefix_join<T, D>, p, G) == cudaSuccess ? 0 : -1;
 }
 
-void plan(PrefixArgs& p, const qwen_paged_kv& kv, int n_heads, uint32_t prefix_len, int G) {
+// What the steps take one SM: 1.92 us for two row tiles, their chain; 1.5 us for a lone
+// one, its loads.
+double prefix_us(const PrefixArgs& p, const qwen_paged_kv& kv) {
+  return (double)kv.n_kv_heads * p.steps * (p.tiles / 2 * 1.92 + (p.tiles & 1) * 1.5);
+}
+// Fills in the division of the prefix; returns the number of CTAs.  Up to two fifths of
+// the SMs, as many as cost the prefix 8 us, are left to the own positions.
+int plan(PrefixArgs& p, const qwen_paged_kv& kv, int n_heads, uint32_t prefix_len) {
   p.group = n_heads / (int)kv.n_kv_heads;
   p.rows = (int)kv.n_seq * p.group;
   p.tiles = (p.rows + kRows - 1) / kRows;
   p.pairs = (p.tiles + 1) / 2;
   p.steps = (int)((prefix_len + kPos - 1) / kPos);
   p.total = (unsigned long long)kv.n_kv_heads * p.tiles * p.steps;
+  const int sms = paged_sm_count();
+  const int G = sms - (int)std::min(0.4 * sms, 8.0 * sms * sms / prefix_us(p, kv));
   const int weight = (int)kv.n_kv_heads * p.tiles;   // one row tile: 1
-  p.share1 = std::min(G / weight, p.steps);
-  p.share2 = p.share1 ? std::min(2 * G / weight, p.steps) : 0;
+  if (weight > G) {
+    p.share1 = p.share2 = 0;
+    return G;
+  }
+  // whole CTAs for each unit, the number that comes nearest to G
+  const int share = std::min(2 * sms / weight, (4 * G + weight) / (2 * weight));
+  p.share2 = std::min(p.steps, share);
+  p.share1 = std::min(p.steps, std::max(1, share / 2));
+  return (int)kv.n_kv_heads * (p.tiles / 2 * p.share2 + (p.tiles & 1) * p.share1);
+}
+
+// How many tiles of own positions `few` CTAs finish by the time that the prefix is done
+// and all CTAs would be: a CTA takes 0.75 us a tile and 0.85 us a unit.
+uint32_t own_tiles(const PrefixArgs& p, const qwen_paged_kv& kv, int few, double us) {
+  const double units = (double)kv.n_seq * kv.n_kv_heads * ((p.group + 15) / 16);
+  return (uint32_t)std::max(0.0, std::min(2e9, (few * (us + 8) - 0.85 * units) / 0.75));
 }
 
 struct Layout {
@@ -753,34 +801,34 @@ Layout layout(const PrefixArgs& p, const qwen_paged_kv& kv, int n_heads, int G) 
 size_t paged_prefix_workspace(const qwen_paged_kv& kv, int n_heads, uint32_t prefix_len) {
   if (prefix_len == 0) return paged_decode_workspace(kv, n_heads);
   PrefixArgs p{};
-  plan(p, kv, n_heads, prefix_len, paged_sm_count());
-  return layout(p, kv, n_heads, paged_sm_count()).bytes;
+  const int G = plan(p, kv, n_heads, prefix_len);
+  return layout(p, kv, n_heads, G).bytes;
 }
 
 int launch_paged_prefix(const PagedAttnArgs& a, cudaStream_t st) {
   PrefixArgs p{};
   p.a = a;
-  const int G = paged_sm_count();
-  plan(p, a.kv, a.n_heads, a.prefix_len, G);
+  const int G = plan(p, a.kv, a.n_heads, a.prefix_len);
   const Layout l = layout(p, a.kv, a.n_heads, G);
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
-  p.own_o = reinterpret_cast<float*>(ws + l.own_o);
-  p.own_ml = reinterpret_cast<float2*>(ws + l.own_ml);
+  PagedOwn own;
+  p.own_o = own.o = reinterpret_cast<float*>(ws + l.own_o);
+  p.own_ml = own.ml = reinterpret_cast<float2*>(ws + l.own_ml);
+  own.few = std::max(1, 2 * (paged_sm_count() - G));   // two of its CTAs share an SM
+  own.few_tiles = G < paged_sm_count() ? own_tiles(p, a.kv, own.few, prefix_us(p, a.kv) / G) : 0;
   p.part_o = reinterpret_cast<float*>(ws + l.part_o);
   p.part_ml = reinterpret_cast<float2*>(ws + l.part_ml);
   // (above 0, so that a masked score, -inf, stays one: products scaled so weigh alike)
   p.scale_log2 = std::max(std::fabs(a.scale) * kLog2e, 1e-37f);
   p.negate = a.scale < 0.f ? 0x80008000u : 0u;
-  if (launch_paged_decode(a, st, reinterpret_cast<float*>(ws + l.own_o), reinterpret_cast<float2*>(ws + l.own_ml)) != 0)
-    return -1;
   const int box_rows = a.kv.page_size < (uint32_t)kPos ? (int)a.kv.page_size : kPos;
   CUtensorMap tmk, tmv;
   if (encode_pages_map(&tmk, a.kv, a.kv.k, box_rows, 1) || encode_pages_map(&tmv, a.kv, a.kv.v, box_rows, 1)) return -1;
   const bool d64 = a.kv.head_dim == 64;
   if (a.kv.dtype == QWEN_DTYPE_F16)
-    return d64 ? launch<__half, 64>(p, G, tmk, tmv, box_rows, st) : launch<__half, 128>(p, G, tmk, tmv, box_rows, st);
-  return d64 ? launch<__nv_bfloat16, 64>(p, G, tmk, tmv, box_rows, st)
-             : launch<__nv_bfloat16, 128>(p, G, tmk, tmv, box_rows, st);
+    return d64 ? launch<__half, 64>(p, own, G, tmk, tmv, box_rows, st) : launch<__half, 128>(p, own, G, tmk, tmv, box_rows, st);
+  return d64 ? launch<__nv_bfloat16, 64>(p, own, G, tmk, tmv, box_rows, st)
+             : launch<__nv_bfloat16, 128>(p, own, G, tmk, tmv, box_rows, st);
 }
 
 }  // namespace qwen
