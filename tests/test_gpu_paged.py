@@ -279,6 +279,29 @@ def test_attention_prefix_is_paged_attention_of_the_whole():
     assert (got.double() - whole.double()).abs().max().item() <= 4 * ref.U[BF16] * whole.abs().max().item()
 
 
+def test_one_table_for_appending_and_for_the_prefix():
+    """Rows that begin with the prefix's pages: new tokens are rotated at their positions in
+    the whole, and the prefix call reads the columns behind."""
+    n_prefix, P = 5, 32
+    c = ref.Cache(23, [50, 64, 1, 200], 12, 2, 128, P, F16, prefix=n_prefix * P)
+    table = torch.cat((c.prefix_pages[None].expand(4, -1), c.table), dim=1).contiguous()
+    x, whole, inv = c.randn(4, 16, 128), c.seq_len + n_prefix * P, freqs(128)
+    c.q = ops.rope_append_paged(ops.PagedKV(c.k, c.v, table), x[:, :12], x[:, 12:14], x[:, 14:], whole, inv)
+    yq, eq = ref.rotate(x[:, :12], whole.double() - 1, inv, False)
+    assert ((c.q.double() - yq).abs() - (ref.U[F16] * yq.abs() + 2 * eq + 1e-7)).max().item() <= 0
+    own = ops.PagedKV(c.k, c.v, table[:, n_prefix:])
+    got = ops.attention_prefix_paged(own, c.q, c.seq_len, table[0, :n_prefix], n_prefix * P, return_lse=True)
+    ref.assert_attention(got, ref.attention(c, 128 ** -0.5))
+
+
+def test_prefix_beside_many_own_positions():
+    """Own positions for which the SMs left beside the prefix are too few, and enough."""
+    for lens, prefix in (([2000] * 60, 3000), ([20] * 200, 9000), ([3000] + [0] * 199, 9000), ([64] * 3, 100000)):
+        c = ref.Cache(24, lens, 12, 2, 128, 128, BF16, prefix=prefix)
+        got = ops.attention_prefix_paged(c.handle(), c.q, c.seq_len, c.prefix_pages, prefix, return_lse=True)
+        ref.assert_attention(got, ref.attention(c, 128 ** -0.5))
+
+
 # ----------------------------------------------------------- page selection --
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("H,K,D", [(12, 2, 128), (32, 8, 128), (14, 2, 64), (8, 8, 64), (16, 1, 128), (64, 1, 64)])
