@@ -158,13 +158,28 @@ __device__ __forceinline__ uint32_t find_run(const DecodeArgs& p, uint32_t c, ui
   }
   const int per = (n_seq + 31) / 32, s0 = min(n_seq, lane * per), s1 = min(n_seq, s0 + per);
   uint32_t sum = 0, L = 0;
-#pragma unroll 4
-  for (int s = s0; s < s1; ++s) {
-    L = p.a.seq_len[s];
-    const uint32_t t = seq_tiles(p, L);
-    if (t == 0 && c == 0) raise_error(p.a.err, kDevBadArgument);   // (by both producers)
-    sum += t;
+  bool bad = false;
+  if (per == 1) {
+    if (lane < n_seq) {
+      L = p.a.seq_len[lane];
+      sum = seq_tiles(p, L);
+      bad = sum == 0;
+    }
+  } else {
+#pragma unroll 1
+    for (int s = s0; s < s1; s += 4) {   // four lengths a round trip
+      uint32_t x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = p.a.seq_len[min(s + j, s1 - 1)];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t t = seq_tiles(p, x[j]);
+        if (s + j < s1) sum += t;
+        bad |= t == 0;
+      }
+    }
   }
+  if (bad && c == 0) raise_error(p.a.err, kDevBadArgument);   // (by both producers)
   uint32_t inc = sum * u;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {

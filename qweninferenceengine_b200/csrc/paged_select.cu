@@ -175,12 +175,14 @@ __global__ void __launch_bounds__(kScoreWarps * 32, kScoreCtas) k_page_scores(co
   // the lengths.
   const int per_lane = (n_seq + 31) / 32, s0 = min(n_seq, lane * per_lane), s1 = min(n_seq, s0 + per_lane);
   u64 sum = 0;
+  bool bad = false;
 #pragma unroll 4
   for (int i = s0; i < s1; ++i) {
     const uint32_t L = a.seq_len[i];
-    if (L > a.kv.max_pages * a.kv.page_size && blockIdx.x == 0) raise_error(a.err, kDevBadArgument);
+    bad |= L > a.kv.max_pages * a.kv.page_size;
     sum += scored_pages(a, L);
   }
+  if (bad && blockIdx.x == 0) raise_error(a.err, kDevBadArgument);
   u64 inc = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
