@@ -216,7 +216,6 @@ struct ListSmem {
   u64 warp_pair[kListThreads / 32];
   uint32_t count, found_bin, found_above;
   u64 key;
-  int at;
 };
 
 // Exclusive sum over the CTA's threads of v (and the total), packed or not.  Small
@@ -349,16 +348,21 @@ __global__ void __launch_bounds__(kListThreads) k_page_list(const __grid_constan
           }
         }
         __syncthreads();
-        if (tid < (int)held) {
-          const u64 x = sm.rank_key[tid];
-          const int at = sm.rank_at[tid];
+        // (a warp for each of them: a thread for each took 10 us for 128)
+        for (uint32_t k = tid / 32; k < held; k += kListThreads / 32) {
+          const u64 x = sm.rank_key[k];
+          const int at = sm.rank_at[k];
           uint32_t rank = 0, same = 0;
 #pragma unroll 1
-          for (uint32_t j = 0; j < held; ++j) {
-            rank += sm.rank_key[j] > x || (sm.rank_key[j] == x && sm.rank_at[j] < at);
-            same += sm.rank_key[j] == x && sm.rank_at[j] <= at;
+          for (uint32_t j = tid & 31; j < held; j += 32) {
+            const u64 y = sm.rank_key[j];
+            const int there = sm.rank_at[j];
+            rank += y > x || (y == x && there < at);
+            same += y == x && there <= at;
           }
-          if (rank == wanted - 1) {
+          rank = __reduce_add_sync(0xffffffffu, rank);
+          same = __reduce_add_sync(0xffffffffu, same);
+          if (rank == wanted - 1 && (tid & 31) == 0) {
             sm.key = x;
             sm.count = same;
           }
