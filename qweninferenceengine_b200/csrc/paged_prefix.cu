@@ -50,12 +50,12 @@
 #include <cmath>
 
 #include "paged_common.cuh"
+#include "paged_split.h"
 #include "qwen_internal.h"
 
 namespace qwen {
 namespace {
 
-constexpr int kRows = 128;                 // rows of a stream (M)
 constexpr int kPos = 128;                  // positions of a tile
 constexpr int kKSlots = 3, kVSlots = 2;    // tiles of K and of V held
 constexpr uint32_t kSmemBytes = 227 * 1024;
@@ -493,7 +493,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
       // (a warp takes 16 whole rows of the stream's 128, lanes side by side)
       if (cnt > 0) {
         constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes, kLoads = 16 / kAtOnce;   // lanes of a row, rows of a load
-        const int row0 = ((warp >> 2 & 1) * 4 + (warp & 3)) * 16, x = lane % kLanes;
+        const int row0 = (warp & 7) * kWarpRows, x = lane % kLanes;
         // lane l < 16 finds row l's place
         const int r_of = r - row + row0 + (lane & 15);
         const long long at = r_of < p.rows ? (long long)(r_of / p.group) * a.q_stride + (long long)(h * p.group + r_of % p.group) * D : -1;
@@ -507,7 +507,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         for (int q = 0; q < kLoads; ++q) {
           const int rr = row0 + q * kAtOnce + lane / kLanes;
           const uint32_t m = p.negate;
-          *reinterpret_cast<uint4*>(s.q[i] + (x >> 3) * kRows * 128 + rr * 128 + (((x & 7) ^ (rr & 7)) << 4)) =
+          *reinterpret_cast<uint4*>(s.q[i] + query_byte(rr, x)) =
               make_uint4(v[q].x ^ m, v[q].y ^ m, v[q].z ^ m, v[q].w ^ m);
         }
         fence_proxy_async();
@@ -607,10 +607,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
         if (half == 0) sum += sums[0];
       }
       if (half == 0 && r < p.rows) p.part_ml[slot] = make_float2(ref, sum);
-      // O through this warp's 4 KB of the query tile, whose MMAs are done, so that rows
-      // go out in whole 128-byte lines.
+      // O through this warp's bytes of the query tile (stage_byte), whose MMAs are done,
+      // so that rows go out in whole 128-byte lines.
       if (cnt > 0) {
-        uint8_t* mine = s.q[i] + ((warp >> 2 & 1) * 4 + (warp & 3)) * (kRows * D * 2 / 8);
         constexpr int kCols = D / 4;   // fp32 columns a round: 4 KB (2 KB) of 32 rows
         static_assert(32 * kCols * 4 == kRows * D * 2 / 8, "a warp's share of the query tile");
 #pragma unroll 1
@@ -622,14 +621,14 @@ __global__ void __launch_bounds__(kPrefixThreads, 1)
           constexpr int kChunks = kCols / 4;
 #pragma unroll
           for (int x = 0; x < kChunks; ++x)
-            *reinterpret_cast<uint4*>(mine + lane * kCols * 4 + ((x ^ (lane & (kChunks - 1))) << 4)) =
+            *reinterpret_cast<uint4*>(s.q[i] + stage_byte(D, warp & 7, lane, x)) =
                 make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
           __syncwarp();
           const int rows_here = p.rows - (r - lane);   // of this warp's 32
 #pragma unroll
           for (int x = 0; x < kChunks; ++x) {
             const int rr = x * (32 / kChunks) + lane / kChunks, ch = lane % kChunks;
-            const uint4 v = *reinterpret_cast<const uint4*>(mine + rr * kCols * 4 + ((ch ^ (rr & (kChunks - 1))) << 4));
+            const uint4 v = *reinterpret_cast<const uint4*>(s.q[i] + stage_byte(D, warp & 7, rr, ch));
             if (rr < rows_here)
               *reinterpret_cast<uint4*>(p.part_o + (slot - lane + rr) * D + D / 2 * half + kCols * q + 4 * ch) = v;
           }
