@@ -264,7 +264,8 @@ int qwen_rope_append_paged(const qwen_paged_kv* kv, const uint16_t* q, int64_t q
                            int interleaved, void* stream);
 
 /* qwen_attention_decode_batched over a paged cache: one query row per sequence
- * against its seq_len positions, out = softmax(scale * q K^T) V.  lse (NULL or
+ * against its seq_len positions, out = softmax(scale * q K^T) V; fp32 arithmetic, the
+ * weights multiplied with V to twice the digits of the cache's type.  lse (NULL or
  * [n_seq][n_heads] fp32): natural log of the sum of exp(scale * q K^T).  A
  * sequence without positions gives zeros and -inf. */
 size_t qwen_attention_paged_workspace(const qwen_paged_kv* kv, uint32_t n_heads);
@@ -276,7 +277,10 @@ int qwen_attention_paged(const qwen_paged_kv* kv, const uint16_t* q, int64_t q_s
 /* The same where every sequence begins with the same prefix_len positions, held
  * once in the pool pages prefix_pages[] (device, ceil(prefix_len / page_size)
  * numbers); seq_len and page_table describe what follows the prefix (a sequence
- * may hold none).  The prefix is read once for the whole batch. */
+ * may hold none).  The prefix is read once for the whole batch; the weights of its
+ * positions are rounded once to the cache's type before they are multiplied with V (their
+ * sum is not): an output can be off by 2^-11 (fp16) or 2^-8 (bf16) of the weighted mean
+ * of |V|, besides its own rounding. */
 size_t qwen_attention_prefix_paged_workspace(const qwen_paged_kv* kv, uint32_t n_heads,
                                              uint32_t prefix_len);
 int qwen_attention_prefix_paged(const qwen_paged_kv* kv, const uint16_t* q, int64_t q_stride,

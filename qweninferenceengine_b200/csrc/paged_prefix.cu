@@ -43,7 +43,10 @@
 // stream's softmax runs, the tensor core works for the other.  O stays in tensor
 // memory; it is rescaled by its row's thread only when a score passes the row's
 // reference by 2^15 (weights are 2^(s - r) with r = max - 7 when last moved, see
-// paged_decode.cu).
+// paged_decode.cu).  A weight is rounded once to the cache's type (relative 2^-11 or 2^-8,
+// averaged over positions): what that leaves would take half as many MMAs again and twice
+// the writes to tensor memory in a step whose chain is the bound.  Sums and outputs are
+// fp32.
 #include <cudaTypedefs.h>
 
 #include <algorithm>
