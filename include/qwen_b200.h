@@ -233,7 +233,8 @@ typedef struct qwen_paged_kv {
  * read or written there).  Rows of q, k, v and outputs are head-contiguous
  * ([heads][head_dim]) with the given row strides (elements, multiples of 8) and
  * 16-byte aligned.  workspace: device memory of at least the *_workspace bytes
- * for the same arguments (0 for arguments that will be refused), 256-byte aligned,
+ * for the same arguments (0 for a type or sizes that will be refused, with the reason in
+ * qwen_last_error; addresses and strides are not looked at), 256-byte aligned,
  * with any contents; calls that may overlap on the GPU need one each, calls one
  * after another, captured ones too, can share one.  (After a
  * QWEN_ERR_DEVICE_TIMEOUT clear it before a captured call is replayed.)

@@ -20,16 +20,8 @@ bool heads_fit(const qwen_paged_kv& kv, uint32_t n_heads) {
   return kv.n_kv_heads != 0 && kv.n_kv_heads <= 1024 && n_heads != 0 && n_heads % kv.n_kv_heads == 0 &&
          n_heads / kv.n_kv_heads <= (uint32_t)kMaxGroup;
 }
-// Whether a workspace can be sized for these arguments; none for a call without
-// sequences, or one that will be refused.
-bool workspace_for(const qwen_paged_kv* kv, uint32_t n_heads) {
-  return kv && kv->n_seq != 0 && kv->n_seq <= kMaxSeqs && heads_fit(*kv, n_heads) && kv->max_pages <= kMaxPositions;
-}
-
-int check_kv(const char* op, const qwen_paged_kv* kv, uint32_t n_heads, int* page_shift) {
-  if (!kv) return set_error(QWEN_ERR_INVALID_ARGUMENT, "%s: null kv", op);
-  if (!kv->k || !kv->v || (!kv->page_table && kv->n_seq))
-    return set_error(QWEN_ERR_INVALID_ARGUMENT, "%s: null cache buffer", op);
+// What a call and its workspace query both look at: type and sizes.
+int check_sizes(const char* op, const qwen_paged_kv* kv, uint32_t n_heads, int* page_shift) {
   if (kv->dtype != QWEN_DTYPE_F16 && kv->dtype != QWEN_DTYPE_BF16)
     return set_error(QWEN_ERR_INVALID_ARGUMENT, "%s: dtype=%d", op, kv->dtype);
   if (kv->head_dim != 64 && kv->head_dim != 128)
@@ -52,6 +44,36 @@ int check_kv(const char* op, const qwen_paged_kv* kv, uint32_t n_heads, int* pag
     return set_error(QWEN_ERR_INVALID_ARGUMENT,
                      "%s: n_heads=%u must be a multiple of n_kv_heads=%u, at most %d times it", op,
                      n_heads, kv->n_kv_heads, kMaxGroup);
+  return QWEN_OK;
+}
+int check_tiles(const char* op, const qwen_paged_kv* kv, uint32_t n_heads, uint32_t n_list) {
+  if (paged_decode_fits(*kv, (int)n_heads, (int)n_list)) return QWEN_OK;
+  return set_error(QWEN_ERR_INVALID_ARGUMENT,
+                   "%s: %u sequences of %u kv heads and up to %llu positions are more than one call takes", op,
+                   kv->n_seq, kv->n_kv_heads,
+                   (unsigned long long)(n_list ? n_list : kv->max_pages) * kv->page_size);
+}
+int check_prefix_len(const char* op, uint32_t prefix_len) {
+  if (prefix_len <= kMaxPositions) return QWEN_OK;
+  return set_error(QWEN_ERR_INVALID_ARGUMENT, "%s: prefix_len=%u", op, prefix_len);
+}
+int check_n_select(const char* op, uint32_t n_select) {
+  if (n_select != 0 && n_select <= (1u << 20)) return QWEN_OK;
+  return set_error(QWEN_ERR_INVALID_ARGUMENT, "%s: n_select=%u", op, n_select);
+}
+// Whether an attention call (n_list listed pages, 0 without a list) can need a workspace:
+// not without sequences, nor where its sizes will be refused.
+bool attention_runs(const char* op, const qwen_paged_kv* kv, uint32_t n_heads, uint32_t n_list) {
+  int shift;
+  return kv && kv->n_seq != 0 && check_sizes(op, kv, n_heads, &shift) == QWEN_OK &&
+         check_tiles(op, kv, n_heads, n_list) == QWEN_OK;
+}
+
+int check_kv(const char* op, const qwen_paged_kv* kv, uint32_t n_heads, int* page_shift) {
+  if (!kv) return set_error(QWEN_ERR_INVALID_ARGUMENT, "%s: null kv", op);
+  if (!kv->k || !kv->v || (!kv->page_table && kv->n_seq))
+    return set_error(QWEN_ERR_INVALID_ARGUMENT, "%s: null cache buffer", op);
+  QWEN_TRY(check_sizes(op, kv, n_heads, page_shift));
   const int64_t strides[3] = {kv->page_stride, kv->pos_stride, kv->head_stride};
   for (int64_t x : strides)
     if (x <= 0 || x % 8 != 0 || x >= (1ll << 38))
@@ -95,11 +117,7 @@ int attention(const char* op, PagedAttnArgs& a, const qwen_paged_kv* kv, const u
   QWEN_TRY(check_rows(op, "out", out, out_stride, n_heads * kv->head_dim));
   if (!seq_len) return set_error(QWEN_ERR_INVALID_ARGUMENT, "%s: null seq_len", op);
   QWEN_TRY(check_workspace(op, workspace, workspace_bytes, need));
-  if (!paged_decode_fits(*kv, (int)n_heads, a.n_list))
-    return set_error(QWEN_ERR_INVALID_ARGUMENT,
-                     "%s: %u sequences of %u kv heads and up to %llu positions are more than one call takes", op,
-                     kv->n_seq, kv->n_kv_heads,
-                     (unsigned long long)(a.n_list ? a.n_list : kv->max_pages) * kv->page_size);
+  QWEN_TRY(check_tiles(op, kv, n_heads, (uint32_t)a.n_list));
   a.kv = *kv;
   a.q = q;
   a.q_stride = q_stride;
@@ -163,7 +181,7 @@ int qwen_rope_append_paged(const qwen_paged_kv* kv, const uint16_t* q, int64_t q
 }
 
 size_t qwen_attention_paged_workspace(const qwen_paged_kv* kv, uint32_t n_heads) {
-  return workspace_for(kv, n_heads) ? paged_decode_workspace(*kv, (int)n_heads) : 0;
+  return attention_runs("attention_paged", kv, n_heads, 0) ? paged_decode_workspace(*kv, (int)n_heads) : 0;
 }
 
 int qwen_attention_paged(const qwen_paged_kv* kv, const uint16_t* q, int64_t q_stride,
@@ -176,7 +194,8 @@ int qwen_attention_paged(const qwen_paged_kv* kv, const uint16_t* q, int64_t q_s
 }
 
 size_t qwen_attention_prefix_paged_workspace(const qwen_paged_kv* kv, uint32_t n_heads, uint32_t prefix_len) {
-  return workspace_for(kv, n_heads) && prefix_len <= kMaxPositions
+  const char* op = "attention_prefix_paged";
+  return attention_runs(op, kv, n_heads, 0) && check_prefix_len(op, prefix_len) == QWEN_OK
              ? paged_prefix_workspace(*kv, (int)n_heads, prefix_len)
              : 0;
 }
@@ -187,8 +206,7 @@ int qwen_attention_prefix_paged(const qwen_paged_kv* kv, const uint16_t* q, int6
                                 uint32_t prefix_len, float scale, void* workspace,
                                 size_t workspace_bytes, void* stream) {
   const char* op = "attention_prefix_paged";
-  if (prefix_len > kMaxPositions)
-    return set_error(QWEN_ERR_INVALID_ARGUMENT, "%s: prefix_len=%u", op, prefix_len);
+  QWEN_TRY(check_prefix_len(op, prefix_len));
   if (prefix_len && !prefix_pages)
     return set_error(QWEN_ERR_INVALID_ARGUMENT, "%s: null prefix_pages", op);
   PagedAttnArgs a{};
@@ -199,7 +217,8 @@ int qwen_attention_prefix_paged(const qwen_paged_kv* kv, const uint16_t* q, int6
 }
 
 size_t qwen_select_pages_workspace(const qwen_paged_kv* kv) {
-  return workspace_for(kv, kv ? kv->n_kv_heads : 0)
+  int shift;   // (query heads: not known here, any that pass)
+  return kv && kv->n_seq != 0 && check_sizes("select_pages", kv, kv->n_kv_heads, &shift) == QWEN_OK
              ? (size_t)kv->n_seq * kv->n_kv_heads * kv->max_pages * sizeof(double)
              : 0;
 }
@@ -215,7 +234,8 @@ int qwen_select_pages(const qwen_paged_kv* kv, const uint16_t* q, int64_t q_stri
   QWEN_TRY(check_rows(op, "q", q, q_stride, n_heads * kv->head_dim));
   if (!kv->bounds) return set_error(QWEN_ERR_INVALID_ARGUMENT, "%s: the cache keeps no bounds", op);
   if (!seq_len || !pages) return set_error(QWEN_ERR_INVALID_ARGUMENT, "%s: null seq_len or pages", op);
-  if (n_select == 0 || n_select > (1u << 20) || (uint64_t)n_first + n_last > n_select)
+  QWEN_TRY(check_n_select(op, n_select));
+  if ((uint64_t)n_first + n_last > n_select)
     return set_error(QWEN_ERR_INVALID_ARGUMENT, "%s: n_select=%u n_first=%u n_last=%u", op, n_select,
                      n_first, n_last);
   QWEN_TRY(check_workspace(op, workspace, workspace_bytes, qwen_select_pages_workspace(kv)));
@@ -233,8 +253,11 @@ int qwen_select_pages(const qwen_paged_kv* kv, const uint16_t* q, int64_t q_stri
   return finish(op, launch_select_pages(a, static_cast<cudaStream_t>(stream)));
 }
 
-size_t qwen_attention_sparse_paged_workspace(const qwen_paged_kv* kv, uint32_t n_heads, uint32_t) {
-  return qwen_attention_paged_workspace(kv, n_heads);
+size_t qwen_attention_sparse_paged_workspace(const qwen_paged_kv* kv, uint32_t n_heads, uint32_t n_select) {
+  const char* op = "attention_sparse_paged";
+  return check_n_select(op, n_select) == QWEN_OK && attention_runs(op, kv, n_heads, n_select)
+             ? paged_decode_workspace(*kv, (int)n_heads)
+             : 0;
 }
 
 int qwen_attention_sparse_paged(const qwen_paged_kv* kv, const int32_t* pages, uint32_t n_select,
@@ -243,8 +266,8 @@ int qwen_attention_sparse_paged(const qwen_paged_kv* kv, const int32_t* pages, u
                                 const uint32_t* seq_len, float scale, void* workspace,
                                 size_t workspace_bytes, void* stream) {
   const char* op = "attention_sparse_paged";
-  if (!pages || n_select == 0 || n_select > (1u << 20))
-    return set_error(QWEN_ERR_INVALID_ARGUMENT, "%s: pages=%p n_select=%u", op, (const void*)pages, n_select);
+  if (!pages) return set_error(QWEN_ERR_INVALID_ARGUMENT, "%s: null pages", op);
+  QWEN_TRY(check_n_select(op, n_select));
   PagedAttnArgs a{};
   a.list = pages;
   a.n_list = (int)n_select;

@@ -284,15 +284,23 @@ def _call(kv: PagedKV, fn, *args) -> None:
         check(rc)
 
 
-def _workspace(kv: PagedKV, query: str, *sizes) -> tuple:
-    """(memory, bytes) that the library function `query` asks for."""
-    key = (query, sizes, kv.sizes)
-    need = _workspace_bytes.get(key)
-    if need is None:
+def _workspace_need(kv: PagedKV, query: str, *sizes) -> int:
+    """Bytes that the library function `query` asks for on the current device, remembered.
+    (Not an answer of 0: other calls of the same key may differ in what was refused.)"""
+    need = getattr(lib(), query)(kv.ref, *sizes)
+    if need:
         if len(_workspace_bytes) > 4096:
             _workspace_bytes.clear()
+        _workspace_bytes[query, sizes, kv.sizes] = need
+    return need
+
+
+def _workspace(kv: PagedKV, query: str, *sizes) -> tuple:
+    """(memory, bytes) that the library function `query` asks for."""
+    need = _workspace_bytes.get((query, sizes, kv.sizes))
+    if need is None:
         with torch.cuda.device(kv.index):
-            need = _workspace_bytes[key] = getattr(lib(), query)(kv.ref, *sizes)
+            need = _workspace_need(kv, query, *sizes)
     return kv.k_pages.new_empty((need + 1) >> 1), need   # of 16-bit elements
 
 
