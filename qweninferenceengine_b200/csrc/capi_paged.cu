@@ -266,7 +266,7 @@ int qwen_attention_sparse_paged(const qwen_paged_kv* kv, const int32_t* pages, u
                                 const uint32_t* seq_len, float scale, void* workspace,
                                 size_t workspace_bytes, void* stream) {
   const char* op = "attention_sparse_paged";
-  if (!pages) return set_error(QWEN_ERR_INVALID_ARGUMENT, "%s: null pages", op);
+  if (!pages && kv && kv->n_seq) return set_error(QWEN_ERR_INVALID_ARGUMENT, "%s: null pages", op);
   QWEN_TRY(check_n_select(op, n_select));
   PagedAttnArgs a{};
   a.list = pages;
