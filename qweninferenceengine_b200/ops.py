@@ -189,6 +189,7 @@ _DTYPES = {torch.float16: QWEN_DTYPE_F16, torch.bfloat16: QWEN_DTYPE_BF16}
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") \
     else lambda index: torch.cuda.current_stream(index).cuda_stream
 _current_device = torch._C._cuda_getDevice
+_UINT32 = 0xFFFFFFFF   # ctypes would cut a larger number to its low 32 bits
 _workspace_bytes: dict = {}   # by sizes: the library's answers are functions of nothing else
 
 
@@ -327,7 +328,7 @@ def rope_append_paged(kv: PagedKV, q: torch.Tensor, k: torch.Tensor, v: torch.Te
     else:
         os_ = _rows("out", out, kv, n, heads)
     if inv_freq.dtype is not torch.float32 or inv_freq.get_device() != kv.index or \
-            inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+            inv_freq.dim() != 1 or not inv_freq.is_contiguous() or 2 * inv_freq.shape[0] > _UINT32:
         raise ValueError(f"inv_freq must be a contiguous float32 vector on {kv.device}")
     _call(kv, lib().qwen_rope_append_paged, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
           out.data_ptr(), os_, heads, n, _ints("seq_len", seq_len, kv, kv.n_seq),
@@ -375,7 +376,7 @@ def attention_prefix_paged(kv: PagedKV, q: torch.Tensor, seq_len: torch.Tensor,
     the prefix.  The weights of the prefix's positions are rounded once to the cache's
     type, attention_paged's to twice its digits."""
     pages = _ints("prefix_pages", prefix_pages, kv, prefix_pages.numel())
-    if prefix_len < 0 or prefix_pages.numel() * kv.page_size < prefix_len:
+    if not 0 <= prefix_len <= _UINT32 or prefix_pages.numel() * kv.page_size < prefix_len:
         raise ValueError(f"prefix_len={prefix_len} in {prefix_pages.numel()} pages")
     return _attend(kv, lib().qwen_attention_prefix_paged, "qwen_attention_prefix_paged_workspace",
                    (prefix_len,), (), q, seq_len, (pages, prefix_len), scale, out, return_lse)
@@ -388,7 +389,7 @@ def select_pages(kv: PagedKV, q: torch.Tensor, seq_len: torch.Tensor, n_select: 
     [n_seq, kv_heads, n_select] page-table columns, ascending, -1 behind the last.
     The first n_first and last n_last pages are always among them; ties go to the
     lower page."""
-    if n_first < 0 or n_last < 0 or n_select < 1:
+    if not (1 <= n_select <= _UINT32 and 0 <= n_first <= _UINT32 and 0 <= n_last <= _UINT32):
         raise ValueError(f"n_select={n_select} n_first={n_first} n_last={n_last}")
     heads, n = _heads(q), kv.n_seq
     qs = _rows("q", q, kv, n, heads)
@@ -411,7 +412,7 @@ def attention_sparse_paged(kv: PagedKV, q: torch.Tensor, seq_len: torch.Tensor, 
     pages int32 [n_seq, kv_heads, n], page-table columns, -1 for none (a
     select_pages result); only positions below seq_len count."""
     n = pages.shape[-1] if pages.dim() == 3 else 0
-    if pages.shape != (kv.n_seq, kv.n_kv_heads, n) or pages.dtype is not torch.int32 or \
+    if pages.shape != (kv.n_seq, kv.n_kv_heads, n) or n > _UINT32 or pages.dtype is not torch.int32 or \
             pages.get_device() != kv.index or not pages.is_contiguous():
         raise ValueError(f"pages must be a contiguous int32 [{kv.n_seq}, {kv.n_kv_heads}, n] tensor "
                          f"on {kv.device}")
