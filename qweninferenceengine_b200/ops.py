@@ -188,7 +188,8 @@ _PAGED_KV = struct.Struct("=4Q3q7Ii")   # qwen_paged_kv, half a microsecond fast
 _DTYPES = {torch.float16: QWEN_DTYPE_F16, torch.bfloat16: QWEN_DTYPE_BF16}
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") \
     else lambda index: torch.cuda.current_stream(index).cuda_stream
-_current_device = torch._C._cuda_getDevice
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") \
+    else torch.cuda.current_device
 _UINT32 = 0xFFFFFFFF   # ctypes would cut a larger number to its low 32 bits
 _workspace_bytes: dict = {}   # by sizes: the library's answers are functions of nothing else
 
