@@ -815,8 +815,9 @@ PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
   return fn;
 }
 
-// A tag no other call of this process has, 48 bits, spread so that stale memory
-// does not hold it by chance.
+// A call's tag: an odd number of 48 bits, spread so that stale memory does not hold it
+// but by a chance of 2^-47 a word.  Two calls may get the same one, as replays of one
+// captured call do: a call leaves its counts at 0, which is what opening them would do.
 unsigned long long next_tag() {
   static std::atomic<uint64_t> calls{splitmix64((uint64_t)std::chrono::steady_clock::now().time_since_epoch().count())};
   return (splitmix64(calls.fetch_add(1, std::memory_order_relaxed)) >> 16) | 1;
