@@ -5,6 +5,7 @@
 #include <cuda_fp16.h>
 
 #include "paged.h"
+#include "paged_split.h"
 #include "qwen_common.cuh"
 
 namespace qwen {
@@ -120,13 +121,6 @@ __device__ __forceinline__ void write_row(const PagedAttnArgs& a, int seq, int h
 }
 __device__ __forceinline__ float4 as_float4(const float (&v)[4]) { return make_float4(v[0], v[1], v[2], v[3]); }
 __device__ __forceinline__ float4 as_float4(const float (&v)[2]) { return make_float4(v[0], v[1], 0.f, 0.f); }
-
-// x / d.  Out of line, with its operands in registers.  (What takes kernel parameters
-// by reference is inlined: through a reference each is a load from memory, ~0.4 us
-// after another.)
-static __device__ __noinline__ unsigned long long divide(unsigned long long x, unsigned long long d) {
-  return (x | d) >> 32 ? x / d : (uint32_t)x / (uint32_t)d;
-}
 
 // Positions of sequence s, or 0 with the status word set when the length does
 // not fit its row of the page table (*ok false).

@@ -77,10 +77,9 @@ struct StageMeta {
 };
 
 // A piece that a run leaves of a unit it shares with others.
-struct CutPiece {
+struct CutUnit : CutPiece {
   int seq, head, heads;
-  int unit, pieces, piece, run0;   // number in the launch, pieces, this one, run of the first
-  uint32_t total, begin;           // fewer tiles than runs: their number, the unit's first
+  int unit;   // number in the launch
 };
 
 constexpr int kStages = 3;
@@ -98,7 +97,7 @@ struct __align__(1024) DecodeSmem {
   float2 ml[2][kWarps][kMaxSlotHeads];   // by piece parity: maximum and sum of each warp
   StageMeta meta[kStages];
   uint64_t full[kStages], empty[kStages], qfull[query_slots<NT>()], qempty[query_slots<NT>()], joined, early;
-  CutPiece cut[2];
+  CutUnit cut[2];
   int n_cut, n_early;   // cut pieces; of those counted in before the end
   int runs;
   int last[2];
@@ -127,22 +126,6 @@ __device__ __forceinline__ uint32_t seq_tiles(const DecodeArgs& p, uint32_t L) {
   if (p.a.list) return p.list_tiles;
   if (L > p.a.kv.max_pages * p.a.kv.page_size) return 0;
   return L ? ((L - 1) >> p.tile_shift) + 1 : 1;   // an empty sequence still has its zeros written
-}
-
-// total < 2^31 (the entry points refuse more).
-__device__ __forceinline__ uint32_t run_start(uint32_t total, uint32_t c, uint32_t G) {
-  const uint32_t q = total / G;
-  return q * c + (total - q * G) * c / G;   // = total c / G, in 32 bits
-}
-// The run that holds tile x: the largest c with run_start(c) <= x.
-__device__ __forceinline__ int run_of(uint32_t total, uint32_t x, uint32_t G) {
-  return (int)divide((unsigned long long)(x + 1) * G - 1, total);
-}
-// The partial slot of piece i: runs follow one another, or (fewer tiles than runs)
-// each has one tile or none.
-__device__ __forceinline__ int piece_slot(const CutPiece& u, int i, int G) {
-  const int r = u.total < (unsigned)G ? run_of(u.total, u.begin + i, G) : u.run0 + i;
-  return 2 * r + (i == 0 ? 1 : 0);
 }
 
 // Total number of tiles, the number G of runs, and the sequence that holds tile
@@ -235,7 +218,7 @@ __device__ __forceinline__ void store_partial(const DecodeArgs& p, int at, float
 // pieces at a time instead of four: single sequences -0.2 us, batches +0.6): into the
 // output rows, or into the first piece's slot.
 template <typename T, int D>
-__device__ __forceinline__ void join_pieces(const DecodeArgs& p, const CutPiece& u, int G, int first, int step, int n, bool final,
+__device__ __forceinline__ void join_pieces(const DecodeArgs& p, const CutUnit& u, int G, int first, int step, int n, bool final,
                             int warp, int lane) {
   constexpr int V = D / 32, HB = 2;
   const int slot = lane < n ? piece_slot(u, first + lane * step, G) * kMaxSlotHeads : 0;
@@ -322,7 +305,7 @@ __device__ __noinline__ bool arrive_last(unsigned long long* count, unsigned lon
 }
 
 // Arrival of a piece at the first level of its join.
-__device__ __forceinline__ int arrive_first(const DecodeArgs& p, const CutPiece& u, int G) {
+__device__ __forceinline__ int arrive_first(const DecodeArgs& p, const CutUnit& u, int G) {
   const int first = u.piece / kJoin * kJoin;
   return arrive_last(u.pieces <= kJoin ? p.arrived + 2 * G + u.unit : p.arrived + piece_slot(u, first, G), p.tag,
                      min(kJoin, u.pieces - first));
@@ -488,17 +471,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
         first = false;
       }
       if (dest >= 0 && !is_k) {
-        const int run0 = run_of(total, begin, G);
-        CutPiece u;
+        CutUnit u;
+        static_cast<CutPiece&>(u) = cut_piece(total, begin, ts, tile0, c, G);
         u.seq = seq;
         u.head = head;
         u.heads = heads;
         u.unit = seq * p.units_per_seq + (int)unit;
-        u.pieces = total < G ? (int)ts : run_of(total, begin + ts - 1, G) - run0 + 1;
-        u.piece = total < G ? (int)tile0 : c - run0;
-        u.run0 = run0;
-        u.total = min(total, G);
-        u.begin = begin;
         if (lane == 0) s.cut[n_cut] = u;
         if (pieces == 1) cut_first = true;
         ++n_cut;
@@ -509,7 +487,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
       // While the last tiles are on their way: the counts of the units it shares, and
       // the arrival of a piece that is not the run's last.
       if (lane < n_cut) {
-        const CutPiece& u = s.cut[lane];
+        const CutUnit& u = s.cut[lane];
         open_count(p.arrived + 2 * G + u.unit, p.tag);
         if (u.pieces > kJoin) open_count(p.arrived + piece_slot(u, u.piece / kJoin * kJoin, G), p.tag);
       }
@@ -782,7 +760,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
 #pragma unroll 1
   for (int k = 0; k < n_cut; ++k) {
     if (!s.last[k]) continue;
-    const CutPiece& u = s.cut[k];
+    const CutUnit& u = s.cut[k];
     const int groups = (u.pieces + kJoin - 1) / kJoin, first = u.piece / kJoin * kJoin;
     int from = first, step = 1, n = min(kJoin, u.pieces - first);
     bool final = groups == 1;

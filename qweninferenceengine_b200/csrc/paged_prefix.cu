@@ -53,99 +53,25 @@
 #include <cmath>
 
 #include "paged_common.cuh"
-#include "paged_split.h"
 #include "qwen_internal.h"
 
 namespace qwen {
 namespace {
 
-constexpr int kPos = 128;                  // positions of a tile
 constexpr int kKSlots = 3, kVSlots = 2;    // tiles of K and of V held
 constexpr uint32_t kSmemBytes = 227 * 1024;
 constexpr int kPrefixThreads = 576;
 constexpr int kProducer = 16, kIssuer = 17;
 constexpr int kColS = 0, kColO = 256;      // tensor-memory columns: S0 S1 (P over S), O0 O1
 
-struct PrefixArgs {
+struct PrefixArgs : PrefixSplit {
   PagedAttnArgs a;
-  int group, rows, tiles, pairs;   // query heads and rows per kv head, row tiles, units
-  int steps;                       // position tiles
-  unsigned long long total;        // weighted steps of all units
-  int share2, share1;              // CTAs of a unit of two tiles, of one; 0: runs over all units
   float scale_log2;                // above 0: a negative scale's sign is put on the queries
   uint32_t negate;                 // 0x80008000 then, else 0
   float* part_o;                   // [units + runs][2][128][D]
   float2* part_ml;                 // [units + runs][2][128]
   const float* own_o;              // [n_seq][n_heads][D]
   const float2* own_ml;
-};
-
-// Units of a kv head come pair by pair, an odd tile's last; a step weighs its MMAs.
-__host__ __device__ __forceinline__ int unit_weight(const PrefixArgs& p, int pair) {
-  return 2 * pair + 1 < p.tiles ? 2 : 1;
-}
-__device__ __forceinline__ unsigned long long unit_begin(const PrefixArgs& p, int unit) {
-  const int h = unit / p.pairs, pair = unit % p.pairs;
-  return (unsigned long long)p.steps * ((unsigned long long)h * p.tiles + 2 * pair);
-}
-__device__ __forceinline__ unsigned long long prefix_run_start(const PrefixArgs& p, int c, int G) {
-  return divide(p.total * (unsigned)c, (unsigned)G);
-}
-// Steps i of a unit that run c takes: those that begin (at begin + w i) in it.
-__device__ __forceinline__ void steps_of(const PrefixArgs& p, unsigned long long begin, int w, int c, int G, int* i0,
-                                         int* i1) {
-  const unsigned long long x0 = prefix_run_start(p, c, G), x1 = prefix_run_start(p, c + 1, G);
-  *i0 = x0 <= begin ? 0 : (int)min((unsigned long long)p.steps, (x0 - begin + w - 1) >> (w - 1));
-  *i1 = x1 <= begin ? 0 : (int)min((unsigned long long)p.steps, (x1 - begin + w - 1) >> (w - 1));
-}
-// First CTA of a unit with CTAs of its own.
-__device__ __forceinline__ int first_cta(const PrefixArgs& p, int h, int pair) {
-  const int per_head = p.tiles / 2 * p.share2 + (p.tiles & 1) * p.share1;
-  return h * per_head + pair * p.share2;
-}
-
-// The pieces of CTA c, one after another: steps [i0, i1) of a unit, partials in
-// slots 2 id, 2 id + 1.
-struct Pieces {
-  const PrefixArgs& p;
-  int c, G, unit, w, h, pair, i0, i1, id;
-  __device__ __forceinline__ Pieces(const PrefixArgs& p, int c, int G) : p(p), c(c), G(G), unit(-1) {}
-  __device__ __forceinline__ bool next() {
-    if (p.share2) {
-      if (unit >= 0) return false;
-      const int per_head = p.tiles / 2 * p.share2 + (p.tiles & 1) * p.share1;
-      h = c / per_head;
-      const int rest = c - h * per_head;
-      if (h >= (int)p.a.kv.n_kv_heads) return false;
-      pair = min(rest / p.share2, p.pairs - 1);
-      w = unit_weight(p, pair);
-      const int part = rest - pair * p.share2, parts = w == 2 ? p.share2 : p.share1;
-      unit = h * p.pairs + pair;
-      i0 = (int)((uint32_t)p.steps * (uint32_t)part / (uint32_t)parts);   // 2^17 steps, 2^8 parts at most
-      i1 = (int)((uint32_t)p.steps * (uint32_t)(part + 1) / (uint32_t)parts);
-      id = c;
-      return i1 > i0;
-    }
-    const int units = (int)p.a.kv.n_kv_heads * p.pairs;
-    const unsigned long long x0 = prefix_run_start(p, c, G), x1 = prefix_run_start(p, c + 1, G);
-    if (unit < 0) {
-      if (x0 >= x1) return false;
-      const unsigned long long per_head = (unsigned long long)p.steps * p.tiles;
-      const int hh = (int)divide(x0, per_head);
-      unit = hh * p.pairs + (int)divide(x0 - hh * per_head, 2ull * p.steps) - 1;
-    }
-    for (;;) {
-      if (++unit >= units) return false;
-      const unsigned long long begin = unit_begin(p, unit);
-      if (begin >= x1) return false;
-      h = unit / p.pairs;
-      pair = unit - h * p.pairs;
-      w = unit_weight(p, pair);
-      id = unit + c;
-      steps_of(p, begin, w, c, G, &i0, &i1);
-      if (i1 > i0) return true;
-    }
-  }
 };
 
 template <int D>
@@ -659,19 +585,9 @@ __global__ void __launch_bounds__(256) k_prefix_join(const __grid_constant__ Pre
   const bool mine = id < (long long)a.kv.n_seq * a.n_heads;
   const int seq = mine ? (int)(id / a.n_heads) : 0, head = mine ? (int)(id - (long long)seq * a.n_heads) : 0;
   const int h = head / p.group, r = seq * p.group + head - h * p.group;
-  const int tile = r / kRows, pair = tile / 2, w = unit_weight(p, pair), unit = h * p.pairs + pair;
-  // Partial k of the row: piece first + k, or (a lone tile) first + k / 2, stream k % 2.
-  const unsigned long long begin = unit_begin(p, unit);
-  int c0, n;
-  if (p.share2) {
-    c0 = first_cta(p, h, pair);
-    n = w == 2 ? p.share2 : 2 * p.share1;
-  } else {
-    c0 = (int)divide((begin + 1) * G - 1, p.total);
-    n = ((int)divide((begin + (unsigned long long)w * (p.steps - 1) + 1) * G - 1, p.total) - c0 + 1) * (w == 2 ? 1 : 2);
-  }
-  const int first = c0 + (p.share2 ? 0 : unit);
-  auto slot_of = [&](int k) { return ((first + (w == 2 ? k : k / 2)) * 2 + (w == 2 ? tile & 1 : k & 1)) * kRows + r % kRows; };
+  const Partials part(p, h, r / kRows, G);
+  const int n = part.n;
+  auto slot_of = [&](int k) { return part.slot(k) * kRows + r % kRows; };
   pdl_wait();
   if (!mine) return;
   const uint32_t L = a.seq_len[seq];
@@ -683,11 +599,7 @@ __global__ void __launch_bounds__(256) k_prefix_join(const __grid_constant__ Pre
     float2 ml = make_float2(-INFINITY, 0.f);
     if (lane < m) {
       ml = __ldcg(p.part_ml + slot_of(b + lane));
-      if (!p.share2) {   // a run may have none of the unit's steps
-        int i0, i1;
-        steps_of(p, begin, w, c0 + (w == 2 ? b + lane : (b + lane) / 2), G, &i0, &i1);
-        if (i1 <= i0) ml = make_float2(-INFINITY, 0.f);
-      }
+      if (!part.there(p, b + lane, G)) ml = make_float2(-INFINITY, 0.f);
     }
     float f = 0.f;
     for (int k0 = 0; k0 < m; k0 += kAtOnce) {
@@ -748,42 +660,11 @@ int launch(const PrefixArgs& p, const PagedOwn& own, int G, const CUtensorMap& t
   return cudaLaunchKernelEx(&cfg, k_prefix_join<T, D>, p, G) == cudaSuccess ? 0 : -1;
 }
 
-// What the steps take one SM: 1.92 us for two row tiles, their chain; 1.5 us for a lone
-// one, its loads.
-double prefix_us(const PrefixArgs& p, const qwen_paged_kv& kv) {
-  return (double)kv.n_kv_heads * p.steps * (p.tiles / 2 * 1.92 + (p.tiles & 1) * 1.5);
-}
-// Fills in the division of the prefix; returns the number of CTAs.  Up to two fifths of
-// the SMs, as many as cost the prefix 8 us, are left to the own positions, whose lengths
-// the host does not know.  (A half at most: 16 sequences behind 20000 positions 42 us
-// against 37.5; a third: 64 behind 8704 39.6 against 34.9; 5 us instead of 8: 256 behind
-// 32768 74.7 against 61.8.)
-int plan(PrefixArgs& p, const qwen_paged_kv& kv, int n_heads, uint32_t prefix_len) {
-  p.group = n_heads / (int)kv.n_kv_heads;
-  p.rows = (int)kv.n_seq * p.group;
-  p.tiles = (p.rows + kRows - 1) / kRows;
-  p.pairs = (p.tiles + 1) / 2;
-  p.steps = (int)((prefix_len + kPos - 1) / kPos);
-  p.total = (unsigned long long)kv.n_kv_heads * p.tiles * p.steps;
-  const int sms = paged_sm_count();
-  const int G = sms - (int)std::min(0.4 * sms, 8.0 * sms * sms / prefix_us(p, kv));
-  const int weight = (int)kv.n_kv_heads * p.tiles;   // one row tile: 1
-  if (weight > G) {
-    p.share1 = p.share2 = 0;
-    return G;
-  }
-  // whole CTAs for each unit, the number that comes nearest to G
-  const int share = std::min(2 * sms / weight, (4 * G + weight) / (2 * weight));
-  p.share2 = std::min(p.steps, share);
-  p.share1 = std::min(p.steps, std::max(1, share / 2));
-  return (int)kv.n_kv_heads * (p.tiles / 2 * p.share2 + (p.tiles & 1) * p.share1);
-}
-
 // How many tiles of own positions `few` CTAs finish by the time that the prefix is done
 // and all CTAs would be: a CTA takes 0.75 us a tile and 0.85 us a unit.  (Own positions
 // divided among all CTAs whatever their number: 256 behind 32768 74.5 us against 61.5,
 // since those that find room at first have only their equal shares.)
-uint32_t own_tiles(const PrefixArgs& p, const qwen_paged_kv& kv, int few, double us) {
+uint32_t own_tiles(const PrefixSplit& p, const qwen_paged_kv& kv, int few, double us) {
   const double units = (double)kv.n_seq * kv.n_kv_heads * ((p.group + 15) / 16);
   return (uint32_t)std::max(0.0, std::min(2e9, (few * (us + 8) - 0.85 * units) / 0.75));
 }
@@ -791,7 +672,7 @@ uint32_t own_tiles(const PrefixArgs& p, const qwen_paged_kv& kv, int few, double
 struct Layout {
   size_t own_o, own_ml, part_o, part_ml, bytes;   // offsets after the decode kernel's part
 };
-Layout layout(const PrefixArgs& p, const qwen_paged_kv& kv, int n_heads, int G) {
+Layout layout(const PrefixSplit& p, const qwen_paged_kv& kv, int n_heads, int G) {
   const size_t heads = (size_t)kv.n_seq * n_heads, D = kv.head_dim;
   const size_t slots = ((size_t)kv.n_kv_heads * p.pairs + G) * 2 * kRows;
   Layout l;
@@ -807,22 +688,22 @@ Layout layout(const PrefixArgs& p, const qwen_paged_kv& kv, int n_heads, int G) 
 
 size_t paged_prefix_workspace(const qwen_paged_kv& kv, int n_heads, uint32_t prefix_len) {
   if (prefix_len == 0) return paged_decode_workspace(kv, n_heads);
-  PrefixArgs p{};
-  const int G = plan(p, kv, n_heads, prefix_len);
+  PrefixSplit p{};
+  const int G = plan_prefix(p, (int)kv.n_kv_heads, (int)kv.n_seq, n_heads, prefix_len, paged_sm_count());
   return layout(p, kv, n_heads, G).bytes;
 }
 
 int launch_paged_prefix(const PagedAttnArgs& a, cudaStream_t st) {
   PrefixArgs p{};
   p.a = a;
-  const int G = plan(p, a.kv, a.n_heads, a.prefix_len);
+  const int G = plan_prefix(p, (int)a.kv.n_kv_heads, (int)a.kv.n_seq, a.n_heads, a.prefix_len, paged_sm_count());
   const Layout l = layout(p, a.kv, a.n_heads, G);
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
   PagedOwn own;
   p.own_o = own.o = reinterpret_cast<float*>(ws + l.own_o);
   p.own_ml = own.ml = reinterpret_cast<float2*>(ws + l.own_ml);
   own.few = std::max(1, 2 * (paged_sm_count() - G));   // two of its CTAs share an SM
-  own.few_tiles = G < paged_sm_count() ? own_tiles(p, a.kv, own.few, prefix_us(p, a.kv) / G) : 0;
+  own.few_tiles = G < paged_sm_count() ? own_tiles(p, a.kv, own.few, prefix_us(p) / G) : 0;
   p.part_o = reinterpret_cast<float*>(ws + l.part_o);
   p.part_ml = reinterpret_cast<float2*>(ws + l.part_ml);
   // (above 0, so that a masked score, -inf, stays one: products scaled so weigh alike)
