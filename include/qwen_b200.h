@@ -278,8 +278,8 @@ int qwen_attention_paged(const qwen_paged_kv* kv, const uint16_t* q, int64_t q_s
 /* The same where every sequence begins with the same prefix_len positions, held
  * once in the pool pages prefix_pages[] (device, ceil(prefix_len / page_size)
  * numbers); seq_len and page_table describe what follows the prefix (a sequence
- * may hold none).  The prefix is read once for the whole batch; the weights of its
- * positions are rounded once to the cache's type before they are multiplied with V (their
+ * may hold none).  The prefix is read once for the whole batch.  With prefix_len > 0 the
+ * weights are rounded once to the cache's type before they are multiplied with V (their
  * sum is not): an output can be off by 2^-11 (fp16) or 2^-8 (bf16) of the weighted mean
  * of |V|, besides its own rounding. */
 size_t qwen_attention_prefix_paged_workspace(const qwen_paged_kv* kv, uint32_t n_heads,

@@ -25,6 +25,18 @@ __device__ __forceinline__ uint32_t pack2(__nv_bfloat16, float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+// The same two values with infinities and NaN replaced by finite ones: +-65504, or +-2^96
+// (and bf16 beyond that), whose products with up to 2^24 weights of up to 2^7 are finite.
+__device__ __forceinline__ uint32_t finite2(__half, uint32_t w) {
+  uint32_t r;   // the lesser magnitude, w's sign
+  asm("min.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(0x7bff7bffu));
+  return r;
+}
+__device__ __forceinline__ uint32_t finite2(__nv_bfloat16, uint32_t w) {
+  uint32_t r;
+  asm("min.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(0x6f806f80u));
+  return r;
+}
 // D = A(16x16, row) * B(16x8, col) + D, fp32 accumulation.
 __device__ __forceinline__ void mma_16816_t(__half, float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
                                             uint32_t b1) {

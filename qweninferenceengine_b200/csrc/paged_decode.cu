@@ -40,9 +40,12 @@
 // shuffles, in most tiles): weights are formed as 2^(s - r), r = max - 7 when last
 // moved, which keeps them within fp16's normal range from 2^15 down to 2^-21 of
 // the largest.  For the MMA a weight is two values of the cache's type, itself rounded
-// and what that left (relative 2^-22 or 2^-16, as k_attention_decode's fp16 pair); sums,
-// maxima and outputs are fp32.  One value alone: 64 x 2048 22.7 us against 22.7, 64 x 4096
-// with 32 query heads of 64 a kv head, where the MMAs count most, 47.3 against 50.9.
+// and what that left (relative 2^-22 or 2^-16, as k_attention_decode's fp16 pair; the
+// second product takes V without infinities, which the first has: 0 times one would be
+// NaN); sums, maxima and outputs are fp32.  One value alone: 64 x 2048 22.6 us against
+// 22.7, 64 x 4096 with 32 query heads of 64 a kv head, where the MMAs count most, 47.4
+// against 51.9.  Beside a shared prefix, whose weights are one value, own positions' are too
+// (64 x 8704: 34.5 us against 35.9).
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -195,9 +198,9 @@ __device__ __forceinline__ uint32_t find_run(const DecodeArgs& p, uint32_t c, ui
 
 // A finished row: output and log-sum-exp, or for the shared-prefix join what they
 // are made of.
-template <typename T, int D>
+template <typename T, int D, bool kOwn>
 __device__ __forceinline__ void finish_row(const DecodeArgs& p, int seq, int head, float4 v, float M, float sum, int lane) {
-  if (!p.own_o) {
+  if constexpr (!kOwn) {
     write_row<T, D>(p.a, seq, head, v, M, sum, lane);
     return;
   }
@@ -217,7 +220,7 @@ __device__ __forceinline__ void store_partial(const DecodeArgs& p, int at, float
 // warps, two heads of each at a time so that their loads are one round trip; eight
 // pieces at a time instead of four: single sequences -0.2 us, batches +0.6): into the
 // output rows, or into the first piece's slot.
-template <typename T, int D>
+template <typename T, int D, bool kOwn>
 __device__ __forceinline__ void join_pieces(const DecodeArgs& p, const CutUnit& u, int G, int first, int step, int n, bool final,
                             int warp, int lane) {
   constexpr int V = D / 32, HB = 2;
@@ -267,7 +270,7 @@ __device__ __forceinline__ void join_pieces(const DecodeArgs& p, const CutUnit& 
     for (int b = 0; b < HB; ++b) {
       const int hh = h0 + b * kWarps;
       if (hh >= u.heads) continue;
-      if (final) finish_row<T, D>(p, u.seq, u.head + hh, as_float4(v[b]), M[b], sum[b], lane);
+      if (final) finish_row<T, D, kOwn>(p, u.seq, u.head + hh, as_float4(v[b]), M[b], sum[b], lane);
       else store_partial<D>(p, __shfl_sync(0xffffffffu, slot, 0) + hh, as_float4(v[b]), M[b], sum[b], lane);
     }
   }
@@ -326,8 +329,9 @@ __device__ __forceinline__ void ldmatrix_x4_t(uint32_t (&r)[4], const void* p) {
                : "memory");
 }
 
-// NT: 8-head MMA columns of a unit (1 or 2).
-template <typename T, int D, int NT>
+// NT: 8-head MMA columns of a unit (1 or 2).  kOwn: beside a kernel that reads a shared
+// prefix (PagedOwn), and like it with weights rounded once.
+template <typename T, int D, int NT, bool kOwn>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     k_paged_decode(const __grid_constant__ DecodeArgs p, int box_rows,
                    const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv) {
@@ -355,7 +359,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   __syncthreads();
   // (Behind a shared prefix the kernel before is k_prefix, which this one runs beside: it
   // lets this one start only once all that came before is there.)
-  if (!p.own_o) pdl_wait();
+  if (!kOwn) pdl_wait();
   if (threadIdx.x == 0) pdl_launch_dependents();
   const int c = blockIdx.x;
 
@@ -523,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
 #pragma unroll 1
     for (uint32_t j = pieces > (uint32_t)QS ? pieces - QS : 0; j < pieces; ++j)
       paged_wait(&s.qfull[j % QS], (j / QS) & 1, &s.abort, a.err, false);
-    if (p.own_o && is_k && c == (int)gridDim.x - 1) pdl_wait();   // so that whoever waits for this kernel finds k_prefix done too
+    if (kOwn && is_k && c == (int)gridDim.x - 1) pdl_wait();   // so that whoever waits for this kernel finds k_prefix done too
     return;
   }
 
@@ -659,9 +663,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
           uint32_t av[4];
           ldmatrix_x4_t(av, vp + (i >> 2) * half_bytes + (((2 * (i & 3) + vchunk) ^ (lane & 7)) << 4));
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            mma_16816_t(T{}, o[n][i], av, b0[n], b1[n]);
-            mma_16816_t(T{}, o[n][i], av, c0[n], c1[n]);
+          for (int n = 0; n < NT; ++n) mma_16816_t(T{}, o[n][i], av, b0[n], b1[n]);
+          if constexpr (!kOwn) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) av[k] = finite2(T{}, av[k]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_16816_t(T{}, o[n][i], av, c0[n], c1[n]);
           }
         }
       } else {   // what lies past the end may be anything: 0 weight times NaN would be NaN
@@ -676,9 +683,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
           av[2] &= k1;
           av[3] &= k1;
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            mma_16816_t(T{}, o[n][i], av, b0[n], b1[n]);
-            mma_16816_t(T{}, o[n][i], av, c0[n], c1[n]);
+          for (int n = 0; n < NT; ++n) mma_16816_t(T{}, o[n][i], av, b0[n], b1[n]);
+          if constexpr (!kOwn) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) av[k] = finite2(T{}, av[k]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_16816_t(T{}, o[n][i], av, c0[n], c1[n]);
           }
         }
       }
@@ -740,7 +750,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
 #pragma unroll
         for (int k = 0; k < V; ++k) v[k] += row[k];
       }
-      if (u.dest == -1) finish_row<T, D>(p, u.seq, u.head + head, as_float4(v), M, sum, lane);
+      if (u.dest == -1) finish_row<T, D, kOwn>(p, u.seq, u.head + head, as_float4(v), M, sum, lane);
       else store_partial<D>(p, u.dest * kMaxSlotHeads + head, as_float4(v), M, sum, lane);
     }
     fence_proxy_async();   // the rows before the next TMA write
@@ -766,7 +776,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     bool final = groups == 1;
 #pragma unroll 1
     for (;;) {   // its sixteen, then the unit's sixteens
-      join_pieces<T, D>(p, u, G, from, step, n, final, warp, lane);
+      join_pieces<T, D, kOwn>(p, u, G, from, step, n, final, warp, lane);
       if (final) break;
       if (!join()) return;
       if (threadIdx.x == 0) s.last[k] = arrive_last(p.arrived + 2 * G + u.unit, p.tag, groups);
@@ -801,10 +811,10 @@ unsigned long long next_tag() {
   return (splitmix64(calls.fetch_add(1, std::memory_order_relaxed)) >> 16) | 1;
 }
 
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, bool kOwn>
 int launch(const DecodeArgs& p, int G, const CUtensorMap& tmk, const CUtensorMap& tmv, int box_rows,
            cudaStream_t st) {
-  auto kern = k_paged_decode<T, D, NT>;
+  auto kern = k_paged_decode<T, D, NT, kOwn>;
   const int smem = (int)sizeof(DecodeSmem<D, NT>) + 1024;
   static_assert((sizeof(DecodeSmem<D, NT>) + 2048) * kCtasPerSm <= 228 * 1024, "CTAs per SM");
   cudaLaunchAttribute attr[1];
@@ -823,6 +833,15 @@ int launch(const DecodeArgs& p, int G, const CUtensorMap& tmk, const CUtensorMap
          }) == cudaSuccess
              ? 0
              : -1;
+}
+
+template <typename T, int D>
+int launch(const DecodeArgs& p, int G, const CUtensorMap& tmk, const CUtensorMap& tmv, int box_rows, cudaStream_t st) {
+  if (p.group > 8)
+    return p.own_o ? launch<T, D, 2, true>(p, G, tmk, tmv, box_rows, st)
+                   : launch<T, D, 2, false>(p, G, tmk, tmv, box_rows, st);
+  return p.own_o ? launch<T, D, 1, true>(p, G, tmk, tmv, box_rows, st)
+                 : launch<T, D, 1, false>(p, G, tmk, tmv, box_rows, st);
 }
 
 int units_per_head(const qwen_paged_kv& kv, int n_heads) {
@@ -900,13 +919,11 @@ int launch_paged_decode(const PagedAttnArgs& a, cudaStream_t st, const PagedOwn&
   const int halves = (int)a.kv.head_dim / 64;
   if (encode_pages_map(&tmk, a.kv, a.kv.k, box_rows, halves) || encode_pages_map(&tmv, a.kv, a.kv.v, box_rows, halves))
     return -1;
-  const bool f16 = a.kv.dtype == QWEN_DTYPE_F16, d64 = a.kv.head_dim == 64;
-  const bool wide = a.n_heads / (int)a.kv.n_kv_heads > 8;
-  if (f16)
-    return d64 ? (wide ? launch<__half, 64, 2> : launch<__half, 64, 1>)(p, G, tmk, tmv, box_rows, st)
-               : (wide ? launch<__half, 128, 2> : launch<__half, 128, 1>)(p, G, tmk, tmv, box_rows, st);
-  return d64 ? (wide ? launch<__nv_bfloat16, 64, 2> : launch<__nv_bfloat16, 64, 1>)(p, G, tmk, tmv, box_rows, st)
-             : (wide ? launch<__nv_bfloat16, 128, 2> : launch<__nv_bfloat16, 128, 1>)(p, G, tmk, tmv, box_rows, st);
+  const bool d64 = a.kv.head_dim == 64;
+  if (a.kv.dtype == QWEN_DTYPE_F16)
+    return d64 ? launch<__half, 64>(p, G, tmk, tmv, box_rows, st) : launch<__half, 128>(p, G, tmk, tmv, box_rows, st);
+  return d64 ? launch<__nv_bfloat16, 64>(p, G, tmk, tmv, box_rows, st)
+             : launch<__nv_bfloat16, 128>(p, G, tmk, tmv, box_rows, st);
 }
 
 }  // namespace qwen

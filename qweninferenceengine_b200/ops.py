@@ -374,8 +374,8 @@ def attention_prefix_paged(kv: PagedKV, q: torch.Tensor, seq_len: torch.Tensor,
     """attention_paged where every sequence begins with the same prefix_len
     positions, held once in pool pages prefix_pages (int32), read once for the batch
     (qwen_attention_prefix_paged).  seq_len and the page table describe what follows
-    the prefix.  The weights of the prefix's positions are rounded once to the cache's
-    type, attention_paged's to twice its digits."""
+    the prefix.  Weights are rounded once to the cache's type before the product with V
+    (prefix_len > 0), attention_paged's to twice its digits."""
     pages = _ints("prefix_pages", prefix_pages, kv, prefix_pages.numel())
     if not 0 <= prefix_len <= _UINT32 or prefix_pages.numel() * kv.page_size < prefix_len:
         raise ValueError(f"prefix_len={prefix_len} in {prefix_pages.numel()} pages")
