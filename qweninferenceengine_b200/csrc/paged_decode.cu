@@ -5,7 +5,7 @@
 // Bound: HBM, each key and value read once (512 B a position and kv head of 128;
 // group flops a byte).  So the kernel is a stream of pages through shared
 // memory with just enough arithmetic beside it.  32 sequences of 16384 positions, 32
-// query and 8 kv heads of 128: 322 us, 6.66 TB/s; of 64 sequences of 512 .. 2048
+// query and 8 kv heads of 128: 325 us, 6.6 TB/s; of 64 sequences of 512 .. 2048
 // positions and 2 kv heads the 79 MB take 12 us and the rest of its 22.6 us is latency:
 // launch, lengths, page numbers, first tile, join, one after another (9 us in a call
 // of 512 positions).
@@ -864,7 +864,7 @@ int paged_sm_count() {
 // Rows = positions of the pool, innermost 64 elements: (element, slot, half, head, page).
 // L2 fetches no more than a head's row at once, 128 or 256 B: with 64-element heads side
 // by side, 256 B would bring the next head's along (64 x 16384 positions of 8 heads:
-// 4400 GB/s so, 5550 GB/s with 128; in head-major pages 6500 GB/s either way).
+// 4400 GB/s so, 5550 GB/s with 128; in head-major pages 6550 GB/s either way).
 int encode_pages_map(CUtensorMap* map, const qwen_paged_kv& kv, const uint16_t* base, int box_rows, int box_halves) {
   auto enc = tensor_map_encoder();
   if (!enc) return -1;

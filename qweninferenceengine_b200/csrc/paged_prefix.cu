@@ -6,7 +6,7 @@
 // cores: 4 rows D L flops against 4 D L bytes -- from ~250 rows on it is bound by
 // tcgen05 (and by the exponentials: 128 x 128 of them take the SFUs as long as the
 // two MMAs of a tile take), below that by HBM.  64 sequences behind 131072 positions, 32
-// query and 8 kv heads of 128: 140 us, 985 TFLOP/s.  What it has there is the chain of a
+// query and 8 kv heads of 128: 143 us, 960 TFLOP/s.  What it has there is the chain of a
 // stream's step, S -> weights -> O and the next S, with its four hand-overs: ~3650
 // clocks a step of both streams where the MMAs take 2048; without any exponential the
 // kernel is 1% faster.
@@ -20,8 +20,8 @@
 //       order, into out and lse
 // One is arithmetic, the other a stream, and each spends 5 to 8 us on its beginning and
 // end.  One after the other / side by side: 64 sequences behind 8704 positions with 75
-// to 300 own ones, 32 query and 8 kv heads 43.4 / 34.9 us; 256 behind 32768 with 65 to
-// 257, 12 and 2 heads 73.1 / 61.5 us (55 us of it k_prefix, 5 us the join).
+// to 300 own ones, 32 query and 8 kv heads 43.4 / 34.0 us; 256 behind 32768 with 65 to
+// 257, 12 and 2 heads 73.1 / 62.9 us (55 us of it k_prefix, 5 us the join).
 //
 // k_prefix: a unit is a kv head and 256 rows (two tiles of M = 128; an odd last
 // tile stands alone), its steps the prefix's 128-position tiles.  With fewer units
@@ -29,13 +29,15 @@
 // a CTA that went on from one unit to the next would load queries and store
 // partials twice (~5 us; a call with 8 units of 68 steps took 57 us so, 44 us with
 // one unit a CTA).  With more, all steps stand in one row, weighted by their MMAs,
-// and one CTA per SM takes an equal run of it.  Warps of a CTA:
+// and one CTA per SM takes an equal run of it (256 sequences behind 1000 positions, 64
+// and 8 heads: 62 us; 1024 behind 32768, 32 and 8 heads: 571 us, 960 TFLOP/s).  Warps of a
+// CTA:
 //   0-7, 8-15  softmax of stream 0 and 1: a thread has half a row (64 scores) of S
 //       from tensor memory, and puts the weights back over it as fp16 / bf16 (P);
 //       the two halves of a row agree on its maximum through shared memory
 //   16 producer: page table, TMA loads of tiles, three of K and two of V held, K's a
-//       step ahead (in one ring of five, K of the second next step waited for V of
-//       this one: 128 rows behind 32768 positions took 36 us, 24 us so)
+//       step ahead (in one ring of five, K of the second next step would wait for V of
+//       this one)
 //   17 MMA issue: S = Q K^T (smem x smem), O += P V (tensor memory x smem, V read
 //       N-major as it lies in the pool)
 // The two streams are the unit's two row tiles over the same K / V slots; a lone
@@ -662,7 +664,7 @@ int launch(const PrefixArgs& p, const PagedOwn& own, int G, const CUtensorMap& t
 
 // How many tiles of own positions `few` CTAs finish by the time that the prefix is done
 // and all CTAs would be: a CTA takes 0.75 us a tile and 0.85 us a unit.  (Own positions
-// divided among all CTAs whatever their number: 256 behind 32768 74.5 us against 61.5,
+// divided among all CTAs whatever their number: 256 behind 32768 75 us against 64,
 // since those that find room at first have only their equal shares.)
 uint32_t own_tiles(const PrefixSplit& p, const qwen_paged_kv& kv, int few, double us) {
   const double units = (double)kv.n_seq * kv.n_kv_heads * ((p.group + 15) / 16);

@@ -11,7 +11,9 @@
 //
 // k_page_scores streams the bounds (HBM: 512 B a page and kv head of 128) into one
 // 64-bit key a page whose order is the scores'.  16 x 2048 pages of 8 heads, 134 MB:
-// 34 us, 4.0 TB/s; 29 us without the conversions to 64 bits (16 a clock and SM).
+// 34 us, 4.0 TB/s; 29 us without the conversions to 64 bits (16 a clock and SM).  Its SMs
+// are busy for four fifths of it: launch, lengths, first bounds and the last run's end are
+// the rest.
 // k_page_list picks, a CTA per kv head and sequence: bins the keys linearly between
 // their least and greatest (2048 bins), finds the bin that the last place falls
 // in, and goes on inside it -- one round where scores are spread, and a round per 11

@@ -160,15 +160,17 @@ struct Partials {
 };
 
 // What the steps take one SM: 1.92 us for two row tiles, their chain; 1.5 us for a lone
-// one, its loads.
+// one, its loads.  With head_dim 64 MMAs and loads halve and the chain does not: with half
+// of these figures 256 sequences behind 32768 positions, 14 and 2 heads, take 68 us
+// against 58, 64 behind 8704 and 256 behind 8704 what they take now.
 inline double prefix_us(const PrefixSplit& p) {
   return (double)p.kv_heads * p.steps * (p.tiles / 2 * 1.92 + (p.tiles & 1) * 1.5);
 }
 // Fills in the division of the prefix; returns the number of CTAs.  Up to two fifths of
 // the SMs, as many as cost the prefix 8 us, are left to the own positions, whose lengths
-// the host does not know.  (A half at most: 16 sequences behind 20000 positions 42 us
-// against 37.5; a third: 64 behind 8704 39.6 against 34.9; 5 us instead of 8: 256 behind
-// 32768 74.7 against 61.8.)
+// the host does not know.  (A half at most: 16 sequences behind 20000 positions 43 us
+// against 39; a third: 64 behind 8704 37.6 against 34.2; 5 us instead of 8: 256 behind
+// 32768 73 against 64, though 64 behind 32768 with 16 and 8 heads of 64 39 against 46.)
 inline int plan_prefix(PrefixSplit& p, int kv_heads, int n_seq, int n_heads, uint32_t prefix_len, int sms) {
   p.kv_heads = kv_heads;
   p.group = n_heads / kv_heads;
