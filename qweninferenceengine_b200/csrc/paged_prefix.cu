@@ -46,9 +46,10 @@
 // memory; it is rescaled by its row's thread only when a score passes the row's
 // reference by 2^15 (weights are 2^(s - r) with r = max - 7 when last moved, see
 // paged_decode.cu).  A weight is rounded once to the cache's type (relative 2^-11 or 2^-8,
-// averaged over positions): what that leaves would take half as many MMAs again and twice
-// the writes to tensor memory in a step whose chain is the bound.  Sums and outputs are
-// fp32.
+// averaged over positions).  With a second product of what that leaves, half as many MMAs
+// again and twice the writes to tensor memory in a step whose chain is the bound, 64 x 8704
+// take 42.5 us against 34.1, 256 x 32768 89.4 against 62.1, and V would have to be cleared of
+// infinities.  Sums and outputs are fp32.
 #include <cudaTypedefs.h>
 
 #include <algorithm>
