@@ -319,6 +319,91 @@ int qwen_attention_sparse_paged(const qwen_paged_kv* kv, const int32_t* pages, u
                                 const uint32_t* seq_len, float scale, void* workspace,
                                 size_t workspace_bytes, void* stream);
 
+/* ---- paged cache held in 4 bits -------------------------------------------
+ * The same operators over pages of 4-bit keys and values (3.2 times less memory
+ * than 16 bits), with rotary positions given by the caller and, where they are
+ * kept, the attention weight and the position of every cached slot, by which a
+ * sequence's cache is cut to a budget.  The reference has no such cache; its
+ * weights are held in blocks of 32 as well (matmul.metal:37-42).
+ *
+ * A group is 32 consecutive elements x of a head's row: low = min x, step =
+ * (max x - min x) / 15 (formed in 64 bits, rounded to fp32 and to the cache's type),
+ * code = min(15, (x - low) / step rounded to the nearest, ties to even), 0 where step
+ * is 0; it stands for low + code step.  A group with an infinity or NaN has step and
+ * low NaN.  Slots are stored in blocks of 16, 20 head_dim bytes each:
+ *   key codes    [head_dim / 32][16 slots][16]  byte j: element 2j (low four bits), 2j+1
+ *   value codes  [head_dim / 32][16 slots][16]
+ *   keys'        [head_dim / 32][16 slots][2]   step, low (16-bit)
+ *   values'      [head_dim / 32][16 slots][2]
+ * A head of a page is page_size / 16 blocks, one behind the other. */
+typedef struct qwen_paged_kv_q4 {
+  uint8_t* pool;               /* head h of page t begins at t * page_stride + h * head_stride */
+  float* weights;              /* [n_seq][n_kv_heads][max_pages * page_size] or NULL: the softmax
+                                  weights that each slot has been given, added up */
+  int32_t* positions;          /* the same shape or NULL: each slot's rotary position (of axis 0) */
+  const int32_t* page_table;   /* [n_seq][table_stride], device */
+  int64_t page_stride, head_stride; /* bytes, positive multiples of 16 */
+  uint32_t n_pages, page_size, n_kv_heads, head_dim;
+  uint32_t n_seq, max_pages, table_stride;
+  int32_t dtype;               /* QWEN_DTYPE_* of q, k, v, outputs, and of steps and lows */
+} qwen_paged_kv_q4;
+
+/* What the paged operators above share holds for these too: limits of sizes, lengths
+ * and page numbers that only the device sees, rows, workspaces.  pool, weights and
+ * positions are 16-byte aligned.  Slot j of sequence s lies in pool page
+ * page_table[s * table_stride + j / page_size]; two sequences of a call that writes
+ * must not share a page. */
+
+/* qwen_rope_append_paged into a 4-bit cache: rotates q into q_out, writes rotated k,
+ * and v, to the slots seq_len and cu_tokens name.  A token's angles come from
+ * positions[axis * position_stride + row] (device, any int32; NULL: its slot, one axis)
+ * times inv_freq[i], the axis of pair i being pair_axis[i] (device, [rot_dim / 2], below
+ * n_axes; NULL: axis 0; n_axes <= 4): time, height and width of images and video, or
+ * positions that run ahead of the slots once some were evicted.  Keys are rotated in
+ * 64-bit arithmetic and rounded to the cache's type before they are quantised.  The
+ * tokens' slots get weight 0 in kv->weights and the position of axis 0 in
+ * kv->positions.  An axis outside 0 .. n_axes - 1 is reported and counts as 0. */
+int qwen_rope_append_paged_q4(const qwen_paged_kv_q4* kv, const uint16_t* q, int64_t q_stride,
+                              const uint16_t* k, int64_t k_stride, const uint16_t* v,
+                              int64_t v_stride, uint16_t* q_out, int64_t q_out_stride,
+                              uint32_t n_heads, uint32_t n_tokens, const uint32_t* seq_len,
+                              const int32_t* cu_tokens, const int32_t* positions,
+                              int64_t position_stride, uint32_t n_axes, const uint8_t* pair_axis,
+                              const float* inv_freq, uint32_t rot_dim, int interleaved,
+                              void* stream);
+
+/* qwen_attention_paged over a 4-bit cache.  Where kv->weights is set, each slot's is
+ * increased by the sum over the query heads of its kv head of exp(scale q k - lse),
+ * the weight that they give it. */
+size_t qwen_attention_paged_q4_workspace(const qwen_paged_kv_q4* kv, uint32_t n_heads);
+int qwen_attention_paged_q4(const qwen_paged_kv_q4* kv, const uint16_t* q, int64_t q_stride,
+                            uint16_t* out, int64_t out_stride, float* lse, uint32_t n_heads,
+                            const uint32_t* seq_len, float scale, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
+/* Keys and values of cached slots in the cache's type, what a further chunk of a
+ * prompt attends: rows cu_rows[s] .. cu_rows[s+1]-1 of k and v ([n_rows][n_kv_heads *
+ * head_dim], device) get the last slots of sequence s, in order; rows from
+ * cu_rows[n_seq] on are not touched.  cu_rows NULL: row s is sequence s's last slot
+ * (n_rows = n_seq; seq_len 0: the row is not touched). */
+int qwen_expand_paged_q4(const qwen_paged_kv_q4* kv, const uint32_t* seq_len,
+                         const int32_t* cu_rows, uint32_t n_rows, uint16_t* k, int64_t k_stride,
+                         uint16_t* v, int64_t v_stride, void* stream);
+
+/* Cuts every sequence to n_keep slots, for each kv head those that come first by
+ * (guarded, greater weight, lower slot): guarded are positions below n_first and, of the
+ * newest (greatest) position of the sequence and head, those above newest - n_recent;
+ * a NaN weight counts as the greatest.  Slots below n_keep that stay are left where they
+ * are; the i-th that goes is taken by the i-th that stays of those behind: its key,
+ * value, weight and position.  What lies behind n_keep is left as it was and may be
+ * overwritten.  A sequence of at most n_keep slots stays as it is.  new_len[n_seq]
+ * (device; may be seq_len) gets min(seq_len, n_keep).  kv->weights and kv->positions must
+ * be set; 1 <= n_keep <= 2^24. */
+size_t qwen_evict_paged_q4_workspace(const qwen_paged_kv_q4* kv, uint32_t n_keep);
+int qwen_evict_paged_q4(const qwen_paged_kv_q4* kv, const uint32_t* seq_len, uint32_t n_keep,
+                        uint32_t n_first, uint32_t n_recent, uint32_t* new_len, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
 /* 24-bit uniform for (seed, sequence, step), SplitMix64 based; host helper. */
 uint32_t qwen_uniform24(uint64_t seed, uint64_t sequence, uint64_t step);
 

@@ -61,7 +61,18 @@ class PagedKVStruct(ctypes.Structure):
                 ("table_stride", c_uint32), ("dtype", c_int32)]
 
 
+class PagedKVQ4Struct(ctypes.Structure):
+    """qwen_paged_kv_q4."""
+
+    _fields_ = [("pool", c_void_p), ("weights", c_void_p), ("positions", c_void_p),
+                ("page_table", c_void_p), ("page_stride", c_int64), ("head_stride", c_int64),
+                ("n_pages", c_uint32), ("page_size", c_uint32), ("n_kv_heads", c_uint32),
+                ("head_dim", c_uint32), ("n_seq", c_uint32), ("max_pages", c_uint32),
+                ("table_stride", c_uint32), ("dtype", c_int32)]
+
+
 _kvp = ctypes.POINTER(PagedKVStruct)
+_q4p = ctypes.POINTER(PagedKVQ4Struct)
 
 # name -> (restype, argtypes)
 SIGNATURES = {
@@ -113,6 +124,18 @@ SIGNATURES = {
     "qwen_attention_sparse_paged": (c_int, [_kvp, c_void_p, c_uint32, c_void_p, c_int64, c_void_p,
                                             c_int64, c_void_p, c_uint32, c_void_p, c_float,
                                             c_void_p, c_size_t, c_void_p]),
+    "qwen_rope_append_paged_q4": (c_int, [_q4p, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                                          c_int64, c_void_p, c_int64, c_uint32, c_uint32, c_void_p,
+                                          c_void_p, c_void_p, c_int64, c_uint32, c_void_p, c_void_p,
+                                          c_uint32, c_int, c_void_p]),
+    "qwen_attention_paged_q4_workspace": (c_size_t, [_q4p, c_uint32]),
+    "qwen_attention_paged_q4": (c_int, [_q4p, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                                        c_uint32, c_void_p, c_float, c_void_p, c_size_t, c_void_p]),
+    "qwen_expand_paged_q4": (c_int, [_q4p, c_void_p, c_void_p, c_uint32, c_void_p, c_int64,
+                                     c_void_p, c_int64, c_void_p]),
+    "qwen_evict_paged_q4_workspace": (c_size_t, [_q4p, c_uint32]),
+    "qwen_evict_paged_q4": (c_int, [_q4p, c_void_p, c_uint32, c_uint32, c_uint32, c_void_p,
+                                    c_void_p, c_size_t, c_void_p]),
     "qwen_uniform24": (c_uint32, [c_uint64, c_uint64, c_uint64]),
     "qwen_engine_config_default": (None, [ctypes.POINTER(EngineConfig)]),
     "qwen_engine_create": (c_int, [ctypes.POINTER(EngineConfig), ctypes.POINTER(c_void_p)]),

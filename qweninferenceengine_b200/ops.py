@@ -10,7 +10,8 @@ from ctypes import byref
 
 import torch
 
-from ._lib import QWEN_DTYPE_BF16, QWEN_DTYPE_F16, PagedKVStruct, check, lib
+from ._lib import (QWEN_DTYPE_BF16, QWEN_DTYPE_F16, PagedKVQ4Struct, PagedKVStruct, check,
+                   lib)
 
 HIDDEN, INTER, HEADS, KV_DIM, HEAD_DIM = 1536, 8960, 12, 256, 128
 VOCAB, ACTUAL_VOCAB = 151936, 151666
@@ -303,7 +304,7 @@ def _workspace(kv: PagedKV, query: str, *sizes) -> tuple:
     if need is None:
         with torch.cuda.device(kv.index):
             need = _workspace_need(kv, query, *sizes)
-    return kv.k_pages.new_empty((need + 1) >> 1), need   # of 16-bit elements
+    return kv.page_table.new_empty((need + 3) >> 2), need   # of 32-bit elements
 
 
 def rope_append_paged(kv: PagedKV, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -419,3 +420,180 @@ def attention_sparse_paged(kv: PagedKV, q: torch.Tensor, seq_len: torch.Tensor, 
                          f"on {kv.device}")
     return _attend(kv, lib().qwen_attention_sparse_paged, "qwen_attention_sparse_paged_workspace", (n,),
                    (pages.data_ptr(), n), q, seq_len, (), scale, out, return_lse)
+
+
+# ------------------------------------------------- paged cache in 4 bits -----
+_PAGED_KV_Q4 = struct.Struct("=4Q2q7Ii")   # qwen_paged_kv_q4
+
+
+class PagedKVQ4:
+    """One layer's paged cache of 4-bit keys and values (qwen_paged_kv_q4) over the
+    caller's tensors.
+
+    pool: uint8 of pool_shape(n_pages, n_kv_heads, page_size, head_dim), the blocks of
+    a head of a page adjacent (pages and heads may have any strides that are multiples
+    of 16).  page_table: int32 [n_seq, max_pages].  dtype: float16 or bfloat16, of q, k,
+    v, outputs and of the groups' parameters.  weights (fp32) and positions (int32),
+    contiguous [n_seq, n_kv_heads, max_pages * page_size]: the attention weight that each
+    slot has been given and its rotary position, set by rope_append_paged_q4, added to by
+    attention_paged_q4 (weights) and read by evict_paged_q4; None keeps none.  The object
+    holds references to the tensors and reads nothing of their contents; their shapes and
+    addresses must not change."""
+
+    __slots__ = ("pool", "page_table", "weights", "positions", "dtype", "device", "index", "n_seq",
+                 "n_kv_heads", "head_dim", "page_size", "sizes", "ref", "_struct")
+
+    @staticmethod
+    def pool_shape(n_pages: int, n_kv_heads: int, page_size: int, head_dim: int) -> tuple:
+        """Shape of a pool: 20 * head_dim bytes hold 16 slots' keys and values."""
+        return (n_pages, n_kv_heads, page_size // 16, 20 * head_dim)
+
+    def __init__(self, pool: torch.Tensor, page_table: torch.Tensor, dtype: torch.dtype,
+                 weights: torch.Tensor | None = None, positions: torch.Tensor | None = None):
+        index = pool.get_device()
+        if dtype not in _DTYPES:
+            raise ValueError(f"dtype must be float16 or bfloat16, not {dtype}")
+        if index < 0:
+            raise ValueError("expected a CUDA tensor")
+        shape, st = pool.shape, pool.stride()
+        if len(shape) != 4 or pool.dtype is not torch.uint8 or shape[3] % 20:
+            raise ValueError("pool must be uint8 [n_pages, n_kv_heads, page_size / 16, 20 * head_dim]")
+        n_pages, n_kv, blocks, width = shape
+        if st[3] != 1 or (blocks > 1 and st[2] != width):
+            raise ValueError("the blocks of a head of a page must be adjacent")
+        table_shape, table_st = page_table.shape, page_table.stride()
+        if len(table_shape) != 2 or page_table.dtype is not torch.int32 or \
+                (table_shape[1] > 1 and table_st[1] != 1):
+            raise ValueError("page_table must be int32 [n_seq, max_pages] with adjacent columns")
+        if page_table.get_device() != index:
+            raise ValueError("the cache's tensors must be on one device")
+        n_seq, max_pages = table_shape
+        kept = (n_seq, n_kv, max_pages * 16 * blocks)
+        for name, x, kind in (("weights", weights, torch.float32), ("positions", positions, torch.int32)):
+            if x is not None and (x.shape != kept or x.dtype is not kind or not x.is_contiguous() or
+                                  x.get_device() != index):
+                raise ValueError(f"{name} must be a contiguous {kind} tensor {kept} on the pool's device")
+        self.pool, self.page_table, self.weights, self.positions = pool, page_table, weights, positions
+        self.dtype, self.device, self.index, self.n_seq = dtype, pool.device, index, n_seq
+        self.n_kv_heads, self.head_dim, self.page_size = n_kv, width // 20, 16 * blocks
+        self.sizes = (index, n_seq, n_kv, width, max_pages)
+        # the stride of an axis of one element is never used: any valid value
+        self._struct = PagedKVQ4Struct.from_buffer_copy(_PAGED_KV_Q4.pack(
+            pool.data_ptr(), 0 if weights is None else weights.data_ptr(),
+            0 if positions is None else positions.data_ptr(), page_table.data_ptr(),
+            st[0] if n_pages > 1 else n_kv * blocks * width, st[1] if n_kv > 1 else blocks * width,
+            n_pages, 16 * blocks, n_kv, width // 20, n_seq, max_pages,
+            table_st[0] if n_seq > 1 else max_pages, _DTYPES[dtype]))
+        self.ref = byref(self._struct)
+
+
+def rope_append_paged_q4(kv: PagedKVQ4, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                         seq_len: torch.Tensor, inv_freq: torch.Tensor,
+                         cu_tokens: torch.Tensor | None = None, positions: torch.Tensor | None = None,
+                         pair_axis: torch.Tensor | None = None, interleaved: bool = False,
+                         out: torch.Tensor | None = None) -> torch.Tensor:
+    """rope_append_paged into a 4-bit cache, at given positions
+    (qwen_rope_append_paged_q4).  q, k, v, seq_len, cu_tokens, inv_freq, interleaved and
+    out are as there.
+
+    positions: int32 [n] or [n_axes, n] (rows adjacent), a token's rotary position on
+    each of up to four axes; None: its slot in the cache.  pair_axis: uint8 [rot_dim / 2],
+    the axis that each pair of elements is turned by (time, height or width of images and
+    video); needed where there is more than one.  The cache's positions keep axis 0."""
+    heads, n = _heads(q), q.shape[0]
+    qs = _rows("q", q, kv, n, heads)
+    ks = _rows("k", k, kv, n, kv.n_kv_heads)
+    vs = _rows("v", v, kv, n, kv.n_kv_heads)
+    if out is None:
+        out = q.new_empty(n, heads, kv.head_dim)
+        os_ = heads * kv.head_dim
+    else:
+        os_ = _rows("out", out, kv, n, heads)
+    index = kv.index
+    if inv_freq.dtype is not torch.float32 or inv_freq.get_device() != index or \
+            inv_freq.dim() != 1 or not inv_freq.is_contiguous() or 2 * inv_freq.shape[0] > _UINT32:
+        raise ValueError(f"inv_freq must be a contiguous float32 vector on {kv.device}")
+    axes, pos, pos_stride, which = 1, None, 0, None
+    if positions is not None:
+        shape = positions.shape
+        if positions.dtype is not torch.int32 or positions.get_device() != index or \
+                len(shape) not in (1, 2) or shape[-1] != n or (n > 1 and positions.stride(-1) != 1):
+            raise ValueError(f"positions must be int32 [{n}] or [n_axes, {n}] with adjacent rows on {kv.device}")
+        pos = positions.data_ptr()
+        if len(shape) == 2:
+            axes = shape[0]
+            pos_stride = positions.stride(0) if axes > 1 else n
+        if axes > _UINT32:
+            raise ValueError(f"positions on {axes} axes")
+    if pair_axis is not None:
+        if pair_axis.dtype is not torch.uint8 or pair_axis.get_device() != index or \
+                pair_axis.shape != inv_freq.shape or not pair_axis.is_contiguous():
+            raise ValueError(f"pair_axis must be a contiguous uint8 tensor of {inv_freq.shape[0]} values "
+                             f"on {kv.device}")
+        which = pair_axis.data_ptr()
+    _call(kv, lib().qwen_rope_append_paged_q4, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
+          out.data_ptr(), os_, heads, n, _ints("seq_len", seq_len, kv, kv.n_seq),
+          None if cu_tokens is None else _ints("cu_tokens", cu_tokens, kv, kv.n_seq + 1), pos, pos_stride,
+          axes, which, inv_freq.data_ptr(), 2 * inv_freq.shape[0], 1 if interleaved else 0)
+    return out
+
+
+def attention_paged_q4(kv: PagedKVQ4, q: torch.Tensor, seq_len: torch.Tensor, scale: float | None = None,
+                       out: torch.Tensor | None = None, return_lse: bool = False):
+    """attention_paged over a 4-bit cache (qwen_attention_paged_q4).  Where the cache
+    keeps weights, each slot's is increased by the sum of the softmax weights that the
+    query heads of its kv head give it (out must not be q then)."""
+    return _attend(kv, lib().qwen_attention_paged_q4, "qwen_attention_paged_q4_workspace", (), (), q,
+                   seq_len, (), scale, out, return_lse)
+
+
+def expand_paged_q4(kv: PagedKVQ4, seq_len: torch.Tensor, cu_rows: torch.Tensor | None = None,
+                    n_rows: int | None = None, out: tuple | None = None):
+    """Cached keys and values in the cache's dtype, (k, v) [n_rows, kv_heads, d]
+    (qwen_expand_paged_q4), for a prompt's next chunk to attend.
+
+    seq_len [n_seq]: slots of each sequence.  cu_rows int32 [n_seq + 1]: rows
+    cu_rows[s]:cu_rows[s + 1] get the last slots of sequence s, in order; rows behind
+    the last sequence's are not touched.  n_rows: rows of the outputs (needed with
+    cu_rows unless `out` is given).  cu_rows None: row s is sequence s's last slot."""
+    K, dim = kv.n_kv_heads, kv.head_dim
+    if out is not None:
+        k, v = out
+        if k.dim() != 3 or (n_rows is not None and n_rows != k.shape[0]):
+            raise ValueError(f"out has shape {tuple(k.shape)}: expected [n_rows, {K}, {dim}]")
+        n_rows = k.shape[0]
+        ks, vs = _rows("k", k, kv, n_rows, K), _rows("v", v, kv, n_rows, K)
+    else:
+        if n_rows is None:
+            if cu_rows is not None:
+                raise ValueError("n_rows is needed with cu_rows")
+            n_rows = kv.n_seq
+        if not 0 <= n_rows <= _UINT32:
+            raise ValueError(f"n_rows={n_rows}")
+        k, v = torch.empty((2, n_rows, K, dim), dtype=kv.dtype, device=kv.device)
+        ks = vs = K * dim
+    _call(kv, lib().qwen_expand_paged_q4, _ints("seq_len", seq_len, kv, kv.n_seq),
+          None if cu_rows is None else _ints("cu_rows", cu_rows, kv, kv.n_seq + 1), n_rows,
+          k.data_ptr(), ks, v.data_ptr(), vs)
+    return k, v
+
+
+def evict_paged_q4(kv: PagedKVQ4, seq_len: torch.Tensor, n_keep: int, n_first: int = 4,
+                   n_recent: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Cuts every sequence's cache to n_keep slots by accumulated weight
+    (qwen_evict_paged_q4) and returns the new lengths, int32 [n_seq] (`out` may be
+    seq_len).  Each kv head keeps the slots of positions below n_first, of the n_recent
+    newest positions (a quarter of n_keep by default), and those of the greatest weight,
+    the lower slot where two are equal.  What is kept behind n_keep moves into the slots
+    that become free before it, so the order of slots is not that of positions."""
+    if n_recent is None:
+        n_recent = n_keep // 4
+    if not (1 <= n_keep <= _UINT32 and 0 <= n_first <= _UINT32 and 0 <= n_recent <= _UINT32):
+        raise ValueError(f"n_keep={n_keep} n_first={n_first} n_recent={n_recent}")
+    n = kv.n_seq
+    if out is None:
+        out = kv.page_table.new_empty(n)
+    ws, need = _workspace(kv, "qwen_evict_paged_q4_workspace", n_keep)
+    _call(kv, lib().qwen_evict_paged_q4, _ints("seq_len", seq_len, kv, n), n_keep, n_first, n_recent,
+          _ints("out", out, kv, n), ws.data_ptr(), need)
+    return out
