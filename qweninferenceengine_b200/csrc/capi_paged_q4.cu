@@ -38,6 +38,12 @@ int check_q4(const char* op, const qwen_paged_kv_q4* kv, uint32_t n_heads, int* 
   return QWEN_OK;
 }
 
+int check_q4_tiles(const char* op, const qwen_paged_kv_q4* kv, uint32_t n_heads) {
+  if (attention_q4_fits(*kv, (int)n_heads)) return QWEN_OK;
+  return set_error(QWEN_ERR_INVALID_ARGUMENT,
+                   "%s: %u sequences of %u kv heads and up to %llu positions are more than one call takes", op,
+                   kv->n_seq, kv->n_kv_heads, (unsigned long long)kv->max_pages * kv->page_size);
+}
 int check_keep(const char* op, uint32_t n_keep) {
   if (n_keep != 0 && n_keep <= kMaxPositions) return QWEN_OK;
   return set_error(QWEN_ERR_INVALID_ARGUMENT, "%s: n_keep=%u", op, n_keep);
@@ -104,7 +110,9 @@ int qwen_rope_append_paged_q4(const qwen_paged_kv_q4* kv, const uint16_t* q, int
 
 size_t qwen_attention_paged_q4_workspace(const qwen_paged_kv_q4* kv, uint32_t n_heads) {
   int shift;
-  return kv && kv->n_seq != 0 && check_q4_sizes("attention_paged_q4", kv, n_heads, &shift) == QWEN_OK
+  const char* op = "attention_paged_q4";
+  return kv && kv->n_seq != 0 && check_q4_sizes(op, kv, n_heads, &shift) == QWEN_OK &&
+                 check_q4_tiles(op, kv, n_heads) == QWEN_OK
              ? attention_q4_workspace(*kv, (int)n_heads)
              : 0;
 }
@@ -123,6 +131,7 @@ int qwen_attention_paged_q4(const qwen_paged_kv_q4* kv, const uint16_t* q, int64
     return set_error(QWEN_ERR_INVALID_ARGUMENT, "%s: out must not be q where weights are kept", op);
   if (!seq_len) return set_error(QWEN_ERR_INVALID_ARGUMENT, "%s: null seq_len", op);
   QWEN_TRY(check_workspace(op, workspace, workspace_bytes, qwen_attention_paged_q4_workspace(kv, n_heads)));
+  QWEN_TRY(check_q4_tiles(op, kv, n_heads));
   a.kv = *kv;
   a.q = q;
   a.q_stride = q_stride;

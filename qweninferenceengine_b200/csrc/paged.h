@@ -52,6 +52,7 @@ size_t paged_decode_workspace(const qwen_paged_kv& kv, int n_heads);
 int launch_paged_prefix(const PagedAttnArgs& a, cudaStream_t st);
 size_t paged_prefix_workspace(const qwen_paged_kv& kv, int n_heads, uint32_t prefix_len);
 int paged_sm_count();
+unsigned long long paged_call_tag();
 // Tensor map of a pool, (element of 64, slot, half, head, page), boxes of box_rows
 // slots and box_halves halves; 0 or -1.
 int encode_pages_map(CUtensorMap* map, const qwen_paged_kv& kv, const uint16_t* base, int box_rows, int box_halves);

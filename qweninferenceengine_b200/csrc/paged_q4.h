@@ -54,6 +54,8 @@ struct Q4AttnArgs {
   int* err;
 };
 int launch_attention_q4(const Q4AttnArgs& a, cudaStream_t st);
+// Whether its tiles can be counted in 31 bits.
+bool attention_q4_fits(const qwen_paged_kv_q4& kv, int n_heads);
 size_t attention_q4_workspace(const qwen_paged_kv_q4& kv, int n_heads);
 
 struct Q4EvictArgs {

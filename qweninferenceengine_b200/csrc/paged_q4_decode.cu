@@ -1,92 +1,704 @@
 // paged_q4_decode.cu -- decode attention over a 4-bit paged cache, one query token per
 // sequence, and the weights that each cached slot was given:
 //   out = sum_t softmax(scale q . K_t) V_t,  K_t, V_t = low + code step
+//
+// Work, runs of tiles, partials and their join: as in paged_decode.cu (paged_runs.cuh).  A
+// tile is 128 slots, a unit (sequence, kv head, up to 8 query heads).  A CTA has a producer
+// warp, which looks pages up and copies a tile's blocks of 16 slots (codes and parameters
+// of K and V lie side by side, so a copy takes up to 8 blocks at once), and 8 consumer
+// warps, each with one block of a tile.
+//
+// What bounds it is not the bytes alone, 2.5 KB a block of 128-element heads, but the
+// instructions that turn them into products; so nothing is dequantised.  Per block a warp
+// computes, with m16n8k16 MMAs,
+//   A_g[16 slots x 8 heads] = codes_g q_g^T for each group g of 32 elements,
+//   S = sum_g step_g A_g + sum_g low_g (sum q_g),
+// and with P = exp(S - reference)
+//   o^T[d x 8] += codes^T (step_g P)^T,  o_g += sum_t P low_g  (added at the end).
+// Codes are exact as MMA operands: four bits at the bottom of an fp16 are c 2^-24, so a
+// word's eight keys take four ANDs and a shift (those from bits 4..7 are 16 c 2^-24; their
+// query elements are divided by 16).  Queries are brought to 2^14 .. 2^15 a head by a power
+// of two and are exact in fp16 but for what is 2^-33 of the head's largest.  For the values
+// the codes are 128 + c in bf16, whose product with weights up to any size is in range;
+// 128 sum_t step P is taken off at the end.  The two sums of P with lows and with steps are
+// one MMA over the slots, q's group sums with lows another (three terms of 8 or 11 bits).
+// Weights step P are two bf16 values (16 bits).  Sums, maxima and outputs are fp32.
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
 #include "paged_q4.cuh"
+#include "paged_runs.cuh"
 #include "qwen_internal.h"
 
 namespace qwen {
 namespace {
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 8;                     // consumer warps
+constexpr int kThreads = (kWarps + 1) * 32;
+constexpr int kTile = 16 * kWarps, kTileShift = 7;
+constexpr int kCtasPerSm = 2;
+constexpr int kSlotHeads = 8;                 // query heads of a unit
+constexpr int kQuerySlots = 4;
+constexpr int kMergeRows = kWarps / 2;
 
-// A CTA per (query head, sequence); a warp takes every fourth block of 16 slots: two
-// lanes a slot for the scores, a lane D / 32 elements of the output.
+enum StageFlags { kFirst = 1, kLast = 2, kEnd = 4 };
+
+struct StageMeta {
+  int valid[kWarps];   // slots of each 16 that count
+  int flags;
+  int seq, head, heads;   // the unit: sequence, first query head, query heads
+  int dest;            // partial slot, or -1: the whole unit, or -2: nothing is written
+};
+
+template <int D>
+struct __align__(128) Q4DecodeSmem {
+  static constexpr int kStages = D == 128 ? 4 : 8;
+  uint8_t kv[kStages][kWarps][Q4Block<D>::kBytes];
+  float4 rows[kMergeRows][kSlotHeads][D / 4];   // of the warps' outputs, chunk c of head h at c ^ (h & 6)
+  uint16_t q[kQuerySlots][kSlotHeads * D];
+  float2 ml[2][kWarps][kSlotHeads];   // by piece parity: maximum and sum of each warp
+  StageMeta meta[kStages];
+  uint64_t full[kStages], empty[kStages], qfull[kQuerySlots], qempty[kQuerySlots], joined, early;
+  CutUnit cut[2];
+  int n_cut, n_early;   // cut pieces; of those counted in before the end
+  int runs;
+  int last[2];
+  int abort;
+};
+
+struct Q4DecodeArgs : DecodeArgs {
+  qwen_paged_kv_q4 kv;
+};
+
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((127 + e) << 23); }   // -126 <= e <= 127
+
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t at) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t at) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
+  uint32_t r;
+  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(sel));
+  return r;
+}
+// (step, low) of a word: its low and high half.
+__device__ __forceinline__ float step_of(__half, uint32_t w) { return __low2float(*reinterpret_cast<const __half2*>(&w)); }
+__device__ __forceinline__ float step_of(__nv_bfloat16, uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+// Two fp32 values as two pairs of the type: rounded, and what that left.
+template <typename T>
+__device__ __forceinline__ void split2(float x, float y, uint32_t* hi, uint32_t* lo) {
+  *hi = pack2(T{}, x, y);
+  const float2 r = unpack2(T{}, *hi);
+  *lo = pack2(T{}, x - r.x, y - r.y);
+}
+
+// What a warp keeps of a unit's queries.
+template <int D>
+struct Queries {
+  uint32_t f[D / 32][4];   // B operands: elements 8t + {0, 4}, {2, 6}, then {1, 5} / 16, {3, 7} / 16 of head g
+  uint32_t sums[2];        // of groups (0, 1), (2, 3): term t of three
+  float c1[2], c2[2];      // of heads 2t, 2t + 1: what a score in MMA units is multiplied with
+};
+// From rows of q in shared memory (lane 4 g + t: elements 8 t .. of each group of head g).
 template <typename T, int D>
-__global__ void __launch_bounds__(kWarps * 32) k_attend_q4(const __grid_constant__ Q4AttnArgs a, float* lse) {
+__device__ __forceinline__ void load_queries(Queries<D>& u, const T* q, int heads, float scale_log2, int lane) {
   constexpr int G = D / 32;
-  __shared__ float qs[D], part[kWarps][D], ml[kWarps][2];
-  const int s = blockIdx.y, head = blockIdx.x, h = head / (a.n_heads / (int)a.kv.n_kv_heads);
+  const int g = lane >> 2, t = lane & 3;
+  float x[G][8], top = 0.f;
+#pragma unroll
+  for (int i = 0; i < G; ++i) {
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (g < heads) w = *reinterpret_cast<const uint4*>(q + g * D + 32 * i + 8 * t);
+    const float2 a = unpack2(T{}, w.x), b = unpack2(T{}, w.y), c = unpack2(T{}, w.z), d = unpack2(T{}, w.w);
+    x[i][0] = a.x, x[i][1] = a.y, x[i][2] = b.x, x[i][3] = b.y, x[i][4] = c.x, x[i][5] = c.y, x[i][6] = d.x, x[i][7] = d.y;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[i][e]));
+  }
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  const int k = top > 0.f && top < INFINITY ? 14 - ilogbf(top) : 0;   // -113 .. 163
+  const float f1 = pow2(k / 2), f2 = pow2(k - k / 2);
+  float sum[4] = {};
+#pragma unroll
+  for (int i = 0; i < G; ++i) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[i][e] = x[i][e] * f1 * f2;
+      sum[i] += x[i][e];
+    }
+    u.f[i][0] = pack2(__half{}, x[i][0], x[i][4]);
+    u.f[i][1] = pack2(__half{}, x[i][2], x[i][6]);
+    u.f[i][2] = pack2(__half{}, x[i][1] * 0.0625f, x[i][5] * 0.0625f);
+    u.f[i][3] = pack2(__half{}, x[i][3] * 0.0625f, x[i][7] * 0.0625f);
+    sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
+    sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
+    sum[i] *= 0.015625f;   // at most 2^14: within fp16
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float a = sum[2 * i], b = sum[2 * i + 1];
+    uint32_t r = 0;
+#pragma unroll
+    for (int term = 0; term < 3; ++term) {
+      const uint32_t w = pack2(T{}, a, b);
+      const float2 y = unpack2(T{}, w);
+      a -= y.x;
+      b -= y.y;
+      if (term == t) r = w;
+    }
+    u.sums[i] = r;
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int kk = 6 - __shfl_sync(0xffffffffu, k, 8 * t + 4 * e);
+    u.c1[e] = pow2(kk / 2);
+    u.c2[e] = pow2(kk - kk / 2) * scale_log2;
+  }
+}
+
+// Codes of a word in fp16 units of 2^-24: elements (0, 4), (2, 6), then 16 times (1, 5), (3, 7).
+__device__ __forceinline__ void small_codes(uint32_t w, uint32_t (&c)[4]) {
+  const uint32_t v = w >> 8;
+  c[0] = w & 0x000f000fu;
+  c[1] = v & 0x000f000fu;
+  c[2] = w & 0x00f000f0u;
+  c[3] = v & 0x00f000f0u;
+}
+// 128 + codes in bf16 of bits 4 j .. 4 j + 3 of both halves of a word.
+__device__ __forceinline__ uint32_t large_code(uint32_t w, int j) {
+  return lop3_and_or(w >> (4 * j), 0x000f000fu, 0x43004300u);
+}
+
+// Scores of a block, log2 domain: s = (slot g: heads 2t, 2t+1), (slot g + 8: the same).
+// codes[half][group]: word t of slot 8 half + g; params the same slots' (step, low).
+template <typename T, int D>
+__device__ __forceinline__ void block_scores(const Queries<D>& u, const uint32_t (&codes)[2][D / 32],
+                                             const uint32_t (&params)[2][D / 32], float (&s)[4]) {
+  constexpr int G = D / 32;
+  float low[4] = {}, sum[4] = {};
+  uint32_t a[4];
+  a[0] = prmt(params[0][0], params[0][1], 0x7632);
+  a[1] = prmt(params[1][0], params[1][1], 0x7632);
+  a[2] = a[3] = 0;
+  if constexpr (G == 4) {
+    a[2] = prmt(params[0][2], params[0][3], 0x7632);
+    a[3] = prmt(params[1][2], params[1][3], 0x7632);
+  }
+  mma_16816_t(T{}, low, a, u.sums[0], u.sums[1]);
+#pragma unroll
+  for (int i = 0; i < G; ++i) {
+    uint32_t x[4], y[4];
+    small_codes(codes[0][i], x);
+    small_codes(codes[1][i], y);
+    const uint32_t a0[4] = {x[0], y[0], x[1], y[1]}, a1[4] = {x[2], y[2], x[3], y[3]};
+    float d[4] = {};
+    mma_16816_t(__half{}, d, a0, u.f[i][0], u.f[i][1]);
+    mma_16816_t(__half{}, d, a1, u.f[i][2], u.f[i][3]);
+    const float s0 = step_of(T{}, params[0][i]), s1 = step_of(T{}, params[1][i]);
+    sum[0] = fmaf(d[0], s0, sum[0]);
+    sum[1] = fmaf(d[1], s0, sum[1]);
+    sum[2] = fmaf(d[2], s1, sum[2]);
+    sum[3] = fmaf(d[3], s1, sum[3]);
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) s[e] = fmaf(sum[e], 262144.f, low[e]) * u.c1[e & 1] * u.c2[e & 1];
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) k_q4_decode(const __grid_constant__ Q4DecodeArgs p) {
+  using Block = Q4Block<D>;
+  using Smem = Q4DecodeSmem<D>;
+  constexpr int ST = Smem::kStages, G = D / 32, QS = kQuerySlots;
+  extern __shared__ uint8_t smem_raw[];
+  Smem& s = *reinterpret_cast<Smem*>(smem_raw + ((128u - (smem_u32(smem_raw) & 127u)) & 127u));
+  const PagedAttnArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t L = a.seq_len[s];
-  if (L > q4_capacity(a.kv)) {
-    if (threadIdx.x == 0) raise_error(a.err, kDevBadArgument);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(&s.full[i], 1);
+      mbar_init(&s.empty[i], kWarps);
+    }
+    for (int i = 0; i < QS; ++i) {
+      mbar_init(&s.qfull[i], 1);
+      mbar_init(&s.qempty[i], kWarps);
+    }
+    mbar_init(&s.joined, kWarps);
+    mbar_init(&s.early, kWarps);
+    s.abort = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  pdl_wait();
+  if (threadIdx.x == 0) pdl_launch_dependents();
+  const int c = blockIdx.x;
+
+  if (warp >= kWarps) {
+    // ------------------------------------------------------------ producer --
+    const int P = a.kv.page_size;
+    const uint32_t capacity = a.kv.max_pages * a.kv.page_size;
+    // lane l < 8: block l of a tile; the first of each page's blocks copies them all
+    const int block = lane & (kWarps - 1), per_page = min(P / 16, kWarps);
+    const bool loads = lane < kWarps && block % per_page == 0;
+    uint32_t it = 0, pieces = 0;
+    int seq, n_cut = 0;
+    uint32_t before, L, runs = gridDim.x;
+    const uint32_t total = find_run(p, c, runs, lane, &seq, &before, &L);
+    const uint32_t t1 = c < (int)runs ? run_start(total, c + 1, runs) : 0;
+    uint32_t t = run_start(total, c, runs), ts = seq_tiles(p, L);   // (c >= runs: no run)
+    int cached_seq = -1, cached_base = 0, page = -1, left = 0, next_page = -1;   // lane i: entry cached_base + i
+    bool alive = true, cut_first = false;
+#pragma unroll 1
+    while (t < t1 && alive) {
+#pragma unroll 1
+      while (t >= before + ts * p.units_per_seq) {
+        before += ts * p.units_per_seq;
+        L = a.seq_len[++seq];
+        ts = seq_tiles(p, L);
+      }
+      const uint32_t unit = (t - before) / ts, begin = before + unit * ts, tile0 = t - begin;
+      const uint32_t tile1 = min(ts, tile0 + (t1 - t));
+      t += tile1 - tile0;
+      const int h = p.chunks == 1 ? (int)unit : (int)unit / p.chunks, chunk = (int)unit - h * p.chunks;
+      const int head = h * p.group + chunk * kSlotHeads, heads = min(kSlotHeads, p.group - chunk * kSlotHeads);
+      const bool fits = L <= capacity;
+      if (!fits && lane == 0) raise_error(a.err, kDevBadArgument);
+      const int dest = !fits ? -2 : tile0 == 0 && tile1 == ts ? -1 : 2 * c + (tile0 == 0 ? 1 : 0);
+      const int32_t* table = a.kv.page_table + (long long)seq * a.kv.table_stride;
+      const int n_entries = (int)((L + P - 1) >> a.page_shift);
+      const uint8_t* pool = p.kv.pool + (long long)h * p.kv.head_stride;
+      bool first = true;
+#pragma unroll 1
+      for (uint32_t tile = tile0; tile < tile1; ++tile) {
+        const int first_entry = ((int)tile * kTile) >> a.page_shift;
+        if (cached_seq != seq || first_entry < cached_base ||
+            ((int)tile * kTile + kTile - 1) >> a.page_shift >= cached_base + 32) {
+          // page of the pool, and how many of the sequence's slots begin with it
+          const int e = first_entry + lane;
+          const bool ahead = cached_seq == seq && first_entry == cached_base + 32;
+          page = -1;
+          left = 0;
+          if (fits && e < n_entries) {
+            page = ahead ? next_page : table[e];
+            if (page < 0 || (uint32_t)page >= a.kv.n_pages) raise_error(a.err, kDevBadArgument);
+            else left = (int)(L - (uint32_t)e * P);
+          }
+          cached_seq = seq;
+          cached_base = first_entry;
+          // the next 32 of the table row, asked for now
+          if (e + 32 < n_entries) next_page = table[e + 32];
+        }
+        const int pos = (int)tile * kTile + 16 * block, from = (pos >> a.page_shift) - cached_base;
+        const int off = pos & (P - 1);
+        const int behind = max(__shfl_sync(0xffffffffu, left, from) - off, 0);   // slots from this block's first on
+        const int my_page = __shfl_sync(0xffffffffu, page, from);
+        const uint32_t bytes = loads ? (uint32_t)((min(behind, per_page * 16) + 15) >> 4) * Block::kBytes : 0;
+        const bool last = tile + 1 == tile1;
+        const uint32_t all = __reduce_add_sync(0xffffffffu, bytes);
+        if (all == 0 && !last) continue;
+        const int st = it % ST;
+        if (it >= ST &&
+            !__all_sync(0xffffffffu, paged_wait(&s.empty[st], ((it / ST) - 1) & 1, &s.abort, a.err))) {
+          alive = false;
+          break;
+        }
+        StageMeta& meta = s.meta[st];
+        if (lane < kWarps) meta.valid[lane] = min(behind, 16);
+        if (lane == 0) {
+          meta.flags = (first ? kFirst : 0) | (last ? kLast : 0);
+          meta.heads = heads;
+          if (last) {
+            meta.seq = seq;
+            meta.head = head;
+            meta.dest = dest;
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive_expect_tx(&s.full[st], all);
+        __syncwarp();
+        if (bytes)
+          bulk_g2s(s.kv[st][block], pool + (long long)my_page * p.kv.page_stride + (off >> 4) * Block::kBytes, bytes,
+                   &s.full[st]);
+        ++it;
+        if (first) {   // the unit's queries, behind its first tile
+          const int qs = pieces % QS;
+          if (pieces >= QS &&
+              !__all_sync(0xffffffffu, paged_wait(&s.qempty[qs], (pieces / QS - 1) & 1, &s.abort, a.err))) {
+            alive = false;
+            break;
+          }
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&s.qfull[qs], (uint32_t)heads * D * 2);
+            bulk_g2s(s.q[qs], a.q + (long long)seq * a.q_stride + (long long)head * D, (uint32_t)heads * D * 2,
+                     &s.qfull[qs]);
+          }
+          ++pieces;
+        }
+        first = false;
+      }
+      if (dest >= 0) {
+        CutUnit u;
+        static_cast<CutPiece&>(u) = cut_piece(total, begin, ts, tile0, c, runs);
+        u.seq = seq;
+        u.head = head;
+        u.heads = heads;
+        u.unit = seq * p.units_per_seq + (int)unit;
+        if (lane == 0) s.cut[n_cut] = u;
+        if (pieces == 1) cut_first = true;
+        ++n_cut;
+      }
+    }
+    __syncwarp();
+    // While the last tiles are on their way: the counts of the units it shares, and
+    // the arrival of a piece that is not the run's last.
+    if (lane < n_cut) {
+      const CutUnit& u = s.cut[lane];
+      open_count(p.arrived + 2 * runs + u.unit, p.tag);
+      if (u.pieces > kJoin) open_count(p.arrived + piece_slot(u, u.piece / kJoin * kJoin, runs), p.tag);
+    }
+    const int n_early = alive && n_cut > 0 && pieces > 1 && cut_first ? 1 : 0;
+    if (n_early) {
+      alive = __all_sync(0xffffffffu, paged_wait(&s.early, 0, &s.abort, a.err));
+      if (alive && lane == 0) s.last[0] = arrive_first(p, s.cut[0], runs);
+    }
+    if (lane == 0) {
+      s.n_cut = n_cut;
+      s.runs = (int)runs;
+      s.n_early = n_early;
+    }
+    __syncwarp();
+    uint32_t drained = it >= (uint32_t)ST ? it - ST : 0;
+    if (alive) {   // the end of the run, in a stage whose last copy was consumed
+      const int st = it % ST;
+      alive = it < ST || __all_sync(0xffffffffu, paged_wait(&s.empty[st], ((it / ST) - 1) & 1, &s.abort, a.err));
+      if (alive) {
+        if (it >= ST) ++drained;
+        if (lane == 0) {
+          s.meta[st].flags = kEnd;
+          mbar_arrive(&s.full[st]);
+        }
+      }
+    }
+    __syncwarp();
+    // Every issued copy lands before the CTA may exit.
+#pragma unroll 1
+    for (uint32_t j = drained; j < it; ++j)
+      paged_wait(&s.full[j % ST], (j / ST) & 1, &s.abort, a.err, false);
+#pragma unroll 1
+    for (uint32_t j = pieces > (uint32_t)QS ? pieces - QS : 0; j < pieces; ++j)
+      paged_wait(&s.qfull[j % QS], (j / QS) & 1, &s.abort, a.err, false);
     return;
   }
-  for (int d = threadIdx.x; d < D; d += kWarps * 32)
-    qs[d] = (float)reinterpret_cast<const T*>(a.q)[(long long)s * a.q_stride + head * D + d] * a.scale * kLog2e;
-  __syncthreads();
-  float m = -INFINITY, l = 0.f, o[G] = {};
-  for (uint32_t b = warp; b * 16 < L; b += kWarps) {
-    const int slot = b * 16, page = q4_page(a.kv, a.err, s, slot >> a.page_shift);
-    if (page < 0) continue;
-    const int valid = min(16, (int)L - slot);
-    const uint8_t* block = q4_block<D>(a.kv, page, h, slot & ((int)a.kv.page_size - 1));
-    const int r = lane & 15;
-    float score = 0.f;
-    for (int g = lane >> 4; g < G; g += 2) {
-      const uint4 w = *reinterpret_cast<const uint4*>(block + g * 256 + r * 16);
-      const uint32_t p = *reinterpret_cast<const uint32_t*>(block + Q4Block<D>::kKeySteps + g * 64 + r * 4);
-      const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+
+  // -------------------------------------------------------------- consumers --
+  const int g = lane >> 2, t4 = lane & 3;
+  Queries<D> u;
+  float o[G][2][4], extra[4], m[2], l[2];   // extra: sums of weights with lows (row g < 4) and steps (g - 4)
+  uint32_t pieces = 0, joins = 0;
+  auto join = [&]() {   // the consumer warps' barrier
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&s.joined);
+    return __all_sync(0xffffffffu, paged_wait(&s.joined, joins++ & 1, &s.abort, a.err));
+  };
+#pragma unroll 1
+  for (uint32_t it = 0;; ++it) {
+    const int st = it % ST;
+    if (!__all_sync(0xffffffffu, paged_wait(&s.full[st], (it / ST) & 1, &s.abort, a.err))) return;
+    const StageMeta& meta = s.meta[st];
+    const int flags = meta.flags;
+    if (flags & kEnd) break;
+    if (flags & kFirst) {
+      const int qs = pieces % QS;
+      if (!__all_sync(0xffffffffu, paged_wait(&s.qfull[qs], (pieces / QS) & 1, &s.abort, a.err))) return;
+      ++pieces;
+      load_queries<T, D>(u, reinterpret_cast<const T*>(s.q[qs]), meta.heads, p.scale_log2, lane);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.qempty[qs]);
+      m[0] = m[1] = -INFINITY;
+      l[0] = l[1] = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float x[8];
-        expand_word<T>(ws[i], p, x);
+      for (int e = 0; e < 4; ++e) {
+        extra[e] = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) score += x[e] * qs[32 * g + 8 * i + e];
+        for (int i = 0; i < G; ++i) o[i][0][e] = o[i][1][e] = 0.f;
       }
     }
-    score += __shfl_xor_sync(0xffffffffu, score, 16);
-    if (r >= valid) score = -INFINITY;
-    float top = score;
-    for (int x = 1; x < 16; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-    const float m2 = fmaxf(m, top), ref = m2 == -INFINITY ? 0.f : m2, f = m == -INFINITY ? 0.f : exp2f(m - ref);
-    const float w = r < valid ? exp2f(score - ref) : 0.f;
-    float sum = w;
-    for (int x = 1; x < 16; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-    m = m2;
-    l = l * f + sum;
-    for (int g = 0; g < G; ++g) o[g] *= f;
-    for (int j = 0; j < valid; ++j) {
-      const float wj = __shfl_sync(0xffffffffu, w, j);
-      for (int g = 0; g < G; ++g) {
-        const uint8_t byte = block[Q4Block<D>::kValues + g * 256 + j * 16 + lane / 2];
-        const float2 p = unpack2(T{}, *reinterpret_cast<const uint32_t*>(block + Q4Block<D>::kValueSteps + g * 64 + j * 4));
-        o[g] += wj * fmaf((float)(byte >> (4 * (lane & 1)) & 15), p.x, p.y);
+    const int valid = meta.valid[warp];
+    if (valid > 0) {
+      uint8_t* block = s.kv[st][warp];
+      const uint32_t at = smem_u32(block);
+      if (valid < 16) {
+        // what lies behind the end may be anything, and 0 weight times NaN would be NaN
+        for (int i = lane; i < 16 * G; i += 32)
+          if ((i & 15) >= valid) reinterpret_cast<uint32_t*>(block + Block::kValueSteps)[i] = 0;
+        __syncwarp();
       }
+      // ---- scores: lane 4 g + t has word t of slots g and g + 8
+      float sv[4];
+      {
+        uint32_t codes[2][G], params[2][G], r[4];
+        if constexpr (G == 4) {
+          const uint32_t row = at + (lane >> 3) * 256 + (lane & 7) * 16;
+          ldmatrix_x4(r, row);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) codes[0][i] = r[i];
+          ldmatrix_x4(r, row + 128);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) codes[1][i] = r[i];
+        } else {
+          ldmatrix_x4(r, at + lane * 16);   // group 0: slots 0 .. 7, 8 .. 15, group 1
+          codes[0][0] = r[0], codes[1][0] = r[1], codes[0][1] = r[2], codes[1][1] = r[3];
+        }
+#pragma unroll
+        for (int i = 0; i < G; ++i) {
+          params[0][i] = lds32(at + Block::kKeySteps + i * 64 + g * 4);
+          params[1][i] = lds32(at + Block::kKeySteps + i * 64 + 32 + g * 4);
+        }
+        block_scores<T, D>(u, codes, params, sv);
+      }
+      if (g >= valid) sv[0] = sv[1] = -INFINITY;
+      if (g + 8 >= valid) sv[2] = sv[3] = -INFINITY;
+      // ---- the running reference moves when a score passes it by 8
+      const float mx[2] = {fmaxf(sv[0], sv[2]), fmaxf(sv[1], sv[3])};
+      if (__any_sync(0xffffffffu, mx[0] > m[0] + 8.f || mx[1] > m[1] + 8.f)) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float x = mx[e];
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+          const float r = fmaxf(m[e], x);
+          const float f = r == -INFINITY ? 1.f : exp2_fast(m[e] - r);
+          m[e] = r;
+          l[e] *= f;
+          extra[e] *= f;
+#pragma unroll
+          for (int i = 0; i < G; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              o[i][j][e] *= f;
+              o[i][j][2 + e] *= f;
+            }
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float r = m[e] == -INFINITY ? 0.f : m[e];
+        sv[e] = exp2_fast(sv[e] - r);
+        sv[2 + e] = exp2_fast(sv[2 + e] - r);
+        l[e] += sv[e] + sv[2 + e];
+      }
+      // ---- weights, turned: lane 4 g + t has head g, slots 2t, 2t+1 and 8 + those
+      uint32_t h0, h1, e0, e1;   // in the cache's type, and what rounding left
+      float pw[4];               // fp16: the weights themselves
+      if constexpr (std::is_same<T, __half>::value) {
+        const uint32_t x0 = movmatrix(prmt(__float_as_uint(sv[0]), __float_as_uint(sv[1]), 0x7632));
+        const uint32_t y0 = movmatrix(prmt(__float_as_uint(sv[0]), __float_as_uint(sv[1]), 0x5410));
+        const uint32_t x1 = movmatrix(prmt(__float_as_uint(sv[2]), __float_as_uint(sv[3]), 0x7632));
+        const uint32_t y1 = movmatrix(prmt(__float_as_uint(sv[2]), __float_as_uint(sv[3]), 0x5410));
+        pw[0] = __uint_as_float(prmt(y0, x0, 0x5410));
+        pw[1] = __uint_as_float(prmt(y0, x0, 0x7632));
+        pw[2] = __uint_as_float(prmt(y1, x1, 0x5410));
+        pw[3] = __uint_as_float(prmt(y1, x1, 0x7632));
+        split2<T>(pw[0], pw[1], &h0, &e0);
+        split2<T>(pw[2], pw[3], &h1, &e1);
+      } else {
+        split2<T>(sv[0], sv[1], &h0, &e0);
+        split2<T>(sv[2], sv[3], &h1, &e1);
+        h0 = movmatrix(h0);
+        h1 = movmatrix(h1);
+        e0 = movmatrix(e0);
+        e1 = movmatrix(e1);
+      }
+      const uint32_t vs = at + Block::kValueSteps + t4 * 8;
+      {   // sums of weights with lows and steps: row g is the low of group g, or the step of g - 4
+        const int i = g & 3;
+        uint32_t w[4] = {};
+        if (i < G) {
+          const uint2 v0 = lds64(vs + i * 64), v1 = lds64(vs + i * 64 + 32);
+          const uint32_t sel = g < 4 ? 0x7632 : 0x5410;
+          w[0] = prmt(v0.x, v0.y, sel);
+          w[2] = prmt(v1.x, v1.y, sel);
+        }
+        mma_16816_t(T{}, extra, w, h0, h1);
+        mma_16816_t(T{}, extra, w, e0, e1);
+      }
+      // ---- o^T += (128 + codes)^T (step weights)^T
+      uint32_t vc[G][2];   // [half]: unit g (elements 4 g ..) of slots 2t, 2t+1 of that half
+      {
+        uint32_t r[4];
+        const uint32_t row = at + Block::kValues + lane * 16;
+        ldmatrix_x4_trans(r, row);
+        vc[0][0] = r[0], vc[0][1] = r[1], vc[1][0] = r[2], vc[1][1] = r[3];
+        if constexpr (G == 4) {
+          ldmatrix_x4_trans(r, row + 512);
+          vc[2][0] = r[0], vc[2][1] = r[1], vc[3][0] = r[2], vc[3][1] = r[3];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        const uint2 v0 = lds64(vs + i * 64), v1 = lds64(vs + i * 64 + 32);
+        uint32_t b0, b1, c0, c1;
+        if constexpr (std::is_same<T, __half>::value) {
+          split2<__nv_bfloat16>(pw[0] * step_of(T{}, v0.x), pw[1] * step_of(T{}, v0.y), &b0, &c0);
+          split2<__nv_bfloat16>(pw[2] * step_of(T{}, v1.x), pw[3] * step_of(T{}, v1.y), &b1, &c1);
+        } else {
+          const uint32_t s0 = prmt(v0.x, v0.y, 0x5410), s1 = prmt(v1.x, v1.y, 0x5410);
+          b0 = mul_bf16x2(h0, s0);
+          b1 = mul_bf16x2(h1, s1);
+          c0 = fma_bf16x2(e0, s0, fma_bf16x2(h0, s0, b0 ^ 0x80008000u));
+          c1 = fma_bf16x2(e1, s1, fma_bf16x2(h1, s1, b1 ^ 0x80008000u));
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t w[4] = {large_code(vc[i][0], 2 * j), large_code(vc[i][0], 2 * j + 1),
+                                 large_code(vc[i][1], 2 * j), large_code(vc[i][1], 2 * j + 1)};
+          mma_16816_t(__nv_bfloat16{}, o[i][j], w, b0, b1);
+          mma_16816_t(__nv_bfloat16{}, o[i][j], w, c0, c1);
+        }
+      }
+      if (valid < 16) fence_proxy_async();   // the zeros before the next copy
+    }
+    if (!(flags & kLast)) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.empty[st]);
+      continue;
+    }
+
+    // ---- the end of a piece.  o[i][j][e]: element 32 i + 4 g + 2 j of head 2t + e, [2 + e]:
+    // the next one.  Four warps hand their rows to the other four, whose sums are joined.
+    const StageMeta unit = meta;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&s.empty[st]);
+    float2(*ml)[kSlotHeads] = s.ml[(pieces - 1) & 1];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float x = l[e];
+      x += __shfl_xor_sync(0xffffffffu, x, 4);
+      x += __shfl_xor_sync(0xffffffffu, x, 8);
+      x += __shfl_xor_sync(0xffffffffu, x, 16);
+      if (g == 0) ml[warp][2 * t4 + e] = make_float2(m[e], x);
+    }
+    if (!join()) return;
+    float f[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float M = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) M = fmaxf(M, ml[w][2 * t4 + e].x);
+      f[e] = m[e] == -INFINITY ? 0.f : exp2_fast(m[e] - M);
+    }
+#pragma unroll
+    for (int i = 0; i < G; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float add = __shfl_sync(0xffffffffu, extra[e], 4 * i + t4) -
+                          128.f * __shfl_sync(0xffffffffu, extra[e], 4 * (4 + i) + t4);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          o[i][j][e] = (o[i][j][e] + add) * f[e];
+          o[i][j][2 + e] = (o[i][j][2 + e] + add) * f[e];
+        }
+      }
+    if (warp >= kMergeRows) {
+#pragma unroll
+      for (int i = 0; i < G; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          s.rows[warp - kMergeRows][2 * t4 + e][(8 * i + g) ^ (2 * t4)] =
+              make_float4(o[i][0][e], o[i][0][2 + e], o[i][1][e], o[i][1][2 + e]);
+    }
+    if (!join()) return;
+    if (warp < kMergeRows) {
+#pragma unroll
+      for (int i = 0; i < G; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float4& at = s.rows[warp][2 * t4 + e][(8 * i + g) ^ (2 * t4)];
+          const float4 x = at;
+          at = make_float4(x.x + o[i][0][e], x.y + o[i][0][2 + e], x.z + o[i][1][e], x.w + o[i][1][2 + e]);
+        }
+    }
+    if (!join()) return;
+#pragma unroll 1
+    for (int head = warp; head < unit.heads && unit.dest != -2; head += kWarps) {
+      constexpr int V = D / 32;   // elements of this lane
+      float M = -INFINITY, sum = 0.f, v[V];
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) M = fmaxf(M, ml[w][head].x);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w)   // (a warp without a maximum has the sum 0, or NaN, which stays)
+        sum += ml[w][head].y * (ml[w][head].x == -INFINITY ? 0.f : exp2_fast(ml[w][head].x - M));
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[k] = 0.f;
+#pragma unroll
+      for (int w = 0; w < kMergeRows; ++w) {
+        const float* row = reinterpret_cast<const float*>(s.rows[w][head]) + (((V * lane) ^ (4 * (head & 6))));
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[k] += row[k];
+      }
+      if (unit.dest == -1) finish_row<T, D, false>(p, unit.seq, unit.head + head, as_float4(v), M, sum, lane);
+      else store_partial<D>(p, unit.dest * kSlotHeads + head, as_float4(v), M, sum, lane);
+    }
+    __syncwarp();
+    if (lane == 0 && pieces == 1) mbar_arrive(&s.early);   // the run's first piece is written
+  }
+
+  // ---- the last pieces to arrive join the others'
+  const int n_cut = s.n_cut, n_early = s.n_early, runs = s.runs;
+  if (n_cut == 0) return;
+  if (!join()) return;   // every warp's partials are written
+  if (threadIdx.x == 0 && n_early < n_cut) s.last[n_early] = arrive_first(p, s.cut[n_early], runs);
+  if (!join()) return;
+#pragma unroll 1
+  for (int k = 0; k < n_cut; ++k) {
+    if (!s.last[k]) continue;
+    const CutUnit& cu = s.cut[k];
+    const int groups = (cu.pieces + kJoin - 1) / kJoin, first = cu.piece / kJoin * kJoin;
+    int from = first, step = 1, n = min(kJoin, cu.pieces - first);
+    bool final = groups == 1;
+#pragma unroll 1
+    for (;;) {   // its sixteen, then the unit's sixteens
+      join_pieces<T, D, false, kSlotHeads, kWarps>(p, cu, runs, from, step, n, final, warp, lane);
+      if (final) break;
+      if (!join()) return;
+      if (threadIdx.x == 0) s.last[k] = arrive_last(p.arrived + 2 * runs + cu.unit, p.tag, groups);
+      if (!join()) return;
+      if (!s.last[k]) break;
+      from = 0;
+      step = kJoin;
+      n = groups;
+      final = true;
     }
   }
-  if (lane == 0) {
-    ml[warp][0] = m;
-    ml[warp][1] = l;
-  }
-  for (int g = 0; g < G; ++g) part[warp][32 * g + lane] = o[g];
-  __syncthreads();
-  float M = -INFINITY, sum = 0.f;
-  for (int w = 0; w < kWarps; ++w) M = fmaxf(M, ml[w][0]);
-  float f[kWarps];
-  for (int w = 0; w < kWarps; ++w) {
-    f[w] = ml[w][0] == -INFINITY && ml[w][1] == 0.f ? 0.f : exp2f(ml[w][0] - (M == -INFINITY ? 0.f : M));
-    if (isnan(ml[w][1])) f[w] = ml[w][1];
-    sum += ml[w][1] * f[w];
-  }
-  for (int d = threadIdx.x; d < D; d += kWarps * 32) {
-    float x = 0.f;
-    for (int w = 0; w < kWarps; ++w) x += f[w] == 0.f ? 0.f : part[w][d] * f[w];
-    const uint32_t y = pack2(T{}, sum == 0.f ? 0.f : x / sum, 0.f);
-    a.out[(long long)s * a.out_stride + head * D + d] = (uint16_t)y;
-  }
-  if (threadIdx.x == 0 && lse)
-    lse[(long long)s * a.n_heads + head] = sum == 0.f ? -INFINITY : (M + log2f(sum)) * kLn2;
 }
 
 // weights[s][h][slot] += sum over the query heads of kv head h of exp(scale q k - lse).
@@ -123,27 +735,86 @@ __global__ void __launch_bounds__(128) k_weigh_q4(const __grid_constant__ Q4Attn
   }
 }
 
+
 template <typename T, int D>
-int launch(const Q4AttnArgs& a, cudaStream_t st) {
-  float* lse = a.lse ? a.lse : a.kv.weights ? static_cast<float*>(a.workspace) : nullptr;
-  k_attend_q4<T, D><<<dim3(a.n_heads, a.kv.n_seq), kWarps * 32, 0, st>>>(a, lse);
-  if (a.kv.weights) {
-    const unsigned ctas = std::min(64u, (a.kv.max_pages * a.kv.page_size + 127) / 128);
-    k_weigh_q4<T, D><<<dim3(ctas, a.kv.n_kv_heads, a.kv.n_seq), 128, 0, st>>>(a, lse);
+int launch(const Q4AttnArgs& args, const Q4DecodeArgs& p, int runs, cudaStream_t st) {
+  auto kern = k_q4_decode<T, D>;
+  const int smem = (int)sizeof(Q4DecodeSmem<D>) + 128;
+  static_assert((sizeof(Q4DecodeSmem<D>) + 128 + 1024) * kCtasPerSm <= 228 * 1024, "CTAs per SM");
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(runs);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  static OncePerDevice once;
+  if (once.launch(reinterpret_cast<const void*>(kern), smem, [&] { return cudaLaunchKernelEx(&cfg, kern, p); }) != cudaSuccess)
+    return -1;
+  if (args.kv.weights) {
+    const unsigned ctas = std::min(64u, (args.kv.max_pages * args.kv.page_size + 127) / 128);
+    k_weigh_q4<T, D><<<dim3(ctas, args.kv.n_kv_heads, args.kv.n_seq), 128, 0, st>>>(args, p.a.lse);
   }
   return 0;
 }
 
+int units_per_head(const qwen_paged_kv_q4& kv, int n_heads) {
+  return (n_heads / (int)kv.n_kv_heads + kSlotHeads - 1) / kSlotHeads;
+}
+size_t units_of(const qwen_paged_kv_q4& kv, int n_heads) {
+  return (size_t)kv.n_seq * kv.n_kv_heads * units_per_head(kv, n_heads);
+}
+
 }  // namespace
 
+bool attention_q4_fits(const qwen_paged_kv_q4& kv, int n_heads) {
+  const double tiles = std::ceil((double)kv.max_pages * kv.page_size / kTile);
+  return (double)units_of(kv, n_heads) * tiles < 2147483648.0;
+}
+
+// Partials and arrivals, as DecodeArgs has them, and where weights are kept the lse.
 size_t attention_q4_workspace(const qwen_paged_kv_q4& kv, int n_heads) {
-  return (size_t)kv.n_seq * n_heads * sizeof(float);
+  const size_t runs = kCtasPerSm * paged_sm_count();
+  return 2 * runs * kSlotHeads * (kv.head_dim + 2) * sizeof(float) +
+         (2 * runs + units_of(kv, n_heads)) * sizeof(unsigned long long) + (size_t)kv.n_seq * n_heads * sizeof(float);
 }
 
 int launch_attention_q4(const Q4AttnArgs& a, cudaStream_t st) {
+  Q4DecodeArgs p{};
+  p.kv = a.kv;
+  p.a.kv.page_table = a.kv.page_table;
+  p.a.kv.n_pages = a.kv.n_pages;
+  p.a.kv.page_size = a.kv.page_size;
+  p.a.kv.n_kv_heads = a.kv.n_kv_heads;
+  p.a.kv.head_dim = a.kv.head_dim;
+  p.a.kv.n_seq = a.kv.n_seq;
+  p.a.kv.max_pages = a.kv.max_pages;
+  p.a.kv.table_stride = a.kv.table_stride;
+  p.a.page_shift = a.page_shift;
+  p.a.q = a.q;
+  p.a.q_stride = a.q_stride;
+  p.a.out = a.out;
+  p.a.out_stride = a.out_stride;
+  p.a.n_heads = a.n_heads;
+  p.a.seq_len = a.seq_len;
+  p.a.err = a.err;
+  p.chunks = units_per_head(a.kv, a.n_heads);
+  p.group = a.n_heads / (int)a.kv.n_kv_heads;
+  p.units_per_seq = (int)a.kv.n_kv_heads * p.chunks;
+  p.tile_shift = kTileShift;
+  p.scale_log2 = a.scale * kLog2e;
+  const int runs = kCtasPerSm * paged_sm_count();
+  p.part_o = static_cast<float*>(a.workspace);
+  p.part_ml = p.part_o + (size_t)2 * runs * kSlotHeads * a.kv.head_dim;
+  p.arrived = reinterpret_cast<unsigned long long*>(p.part_ml + (size_t)2 * runs * kSlotHeads * 2);
+  p.a.lse = a.lse ? a.lse : a.kv.weights ? reinterpret_cast<float*>(p.arrived + 2 * runs + units_of(a.kv, a.n_heads)) : nullptr;
+  p.tag = paged_call_tag();
   const bool d64 = a.kv.head_dim == 64;
-  if (a.kv.dtype == QWEN_DTYPE_F16) return d64 ? launch<__half, 64>(a, st) : launch<__half, 128>(a, st);
-  return d64 ? launch<__nv_bfloat16, 64>(a, st) : launch<__nv_bfloat16, 128>(a, st);
+  if (a.kv.dtype == QWEN_DTYPE_F16) return d64 ? launch<__half, 64>(a, p, runs, st) : launch<__half, 128>(a, p, runs, st);
+  return d64 ? launch<__nv_bfloat16, 64>(a, p, runs, st) : launch<__nv_bfloat16, 128>(a, p, runs, st);
 }
 
 }  // namespace qwen
