@@ -5,8 +5,8 @@
 // Work, runs of tiles, partials and their join: as in paged_decode.cu (paged_runs.cuh).  A
 // tile is 128 slots, a unit (sequence, kv head, up to 8 query heads).  A CTA has a producer
 // warp, which looks pages up and copies a tile's blocks of 16 slots (codes and parameters
-// of K and V lie side by side, so a copy takes up to 8 blocks at once), and 8 consumer
-// warps, each with one block of a tile.
+// of K and V lie side by side, so a copy takes up to 8 blocks at once), and 4 consumer
+// warps, each with two blocks of a tile.
 //
 // What bounds it is not the bytes alone, 2.5 KB a block of 128-element heads, but the
 // instructions that turn them into products; so nothing is dequantised.  Per block a warp
@@ -34,18 +34,19 @@
 namespace qwen {
 namespace {
 
-constexpr int kWarps = 8;                     // consumer warps
+constexpr int kWarps = 4;                     // consumer warps
 constexpr int kThreads = (kWarps + 1) * 32;
-constexpr int kTile = 16 * kWarps, kTileShift = 7;
-constexpr int kCtasPerSm = 2;
+constexpr int kBlocks = 8;                    // of a tile: a warp takes two
+constexpr int kTile = 16 * kBlocks, kTileShift = 7;
+constexpr int kCtasPerSm = 3;
 constexpr int kSlotHeads = 8;                 // query heads of a unit
-constexpr int kQuerySlots = 4;
+constexpr int kQuerySlots = 2;
 constexpr int kMergeRows = kWarps / 2;
 
 enum StageFlags { kFirst = 1, kLast = 2, kEnd = 4 };
 
 struct StageMeta {
-  int valid[kWarps];   // slots of each 16 that count
+  int valid[kBlocks];   // slots of each 16 that count
   int flags;
   int seq, head, heads;   // the unit: sequence, first query head, query heads
   int dest;            // partial slot, or -1: the whole unit, or -2: nothing is written
@@ -53,8 +54,8 @@ struct StageMeta {
 
 template <int D>
 struct __align__(128) Q4DecodeSmem {
-  static constexpr int kStages = D == 128 ? 4 : 8;
-  uint8_t kv[kStages][kWarps][Q4Block<D>::kBytes];
+  static constexpr int kStages = D == 128 ? 3 : 6;
+  uint8_t kv[kStages][kBlocks][Q4Block<D>::kBytes];
   float4 rows[kMergeRows][kSlotHeads][D / 4];   // of the warps' outputs, chunk c of head h at c ^ (h & 6)
   uint16_t q[kQuerySlots][kSlotHeads * D];
   float2 ml[2][kWarps][kSlotHeads];   // by piece parity: maximum and sum of each warp
@@ -103,15 +104,13 @@ __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
 // (step, low) of a word: its low and high half.
 __device__ __forceinline__ float step_of(__half, uint32_t w) { return __low2float(*reinterpret_cast<const __half2*>(&w)); }
 __device__ __forceinline__ float step_of(__nv_bfloat16, uint32_t w) { return __uint_as_float(w << 16); }
-__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-__device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t r;
-  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
-  return r;
+// Weights times steps: the product rounded, and what that left of it and of the weight's rest.
+__device__ __forceinline__ void step_weights(uint32_t hi, uint32_t rest, uint32_t step, uint32_t* w, uint32_t* left) {
+  const __nv_bfloat162 h = *reinterpret_cast<__nv_bfloat162*>(&hi), e = *reinterpret_cast<__nv_bfloat162*>(&rest),
+                       s = *reinterpret_cast<__nv_bfloat162*>(&step);
+  const __nv_bfloat162 x = __hmul2(h, s), y = __hfma2(e, s, __hfma2(h, s, __hneg2(x)));
+  *w = *reinterpret_cast<const uint32_t*>(&x);
+  *left = *reinterpret_cast<const uint32_t*>(&y);
 }
 // Two fp32 values as two pairs of the type: rounded, and what that left.
 template <typename T>
@@ -119,6 +118,22 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t* hi, uint32_t*
   *hi = pack2(T{}, x, y);
   const float2 r = unpack2(T{}, *hi);
   *lo = pack2(T{}, x - r.x, y - r.y);
+}
+
+// D = A B from zeros (which need no registers).
+__device__ __forceinline__ void mma_zero(__half, float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void mma_zero(__nv_bfloat16, float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 // What a warp keeps of a unit's queries.
@@ -204,7 +219,7 @@ template <typename T, int D>
 __device__ __forceinline__ void block_scores(const Queries<D>& u, const uint32_t (&codes)[2][D / 32],
                                              const uint32_t (&params)[2][D / 32], float (&s)[4]) {
   constexpr int G = D / 32;
-  float low[4] = {}, sum[4] = {};
+  float low[4], sum[4];
   uint32_t a[4];
   a[0] = prmt(params[0][0], params[0][1], 0x7632);
   a[1] = prmt(params[1][0], params[1][1], 0x7632);
@@ -213,24 +228,188 @@ __device__ __forceinline__ void block_scores(const Queries<D>& u, const uint32_t
     a[2] = prmt(params[0][2], params[0][3], 0x7632);
     a[3] = prmt(params[1][2], params[1][3], 0x7632);
   }
-  mma_16816_t(T{}, low, a, u.sums[0], u.sums[1]);
+  mma_zero(T{}, low, a, u.sums[0], u.sums[1]);
 #pragma unroll
   for (int i = 0; i < G; ++i) {
     uint32_t x[4], y[4];
     small_codes(codes[0][i], x);
     small_codes(codes[1][i], y);
     const uint32_t a0[4] = {x[0], y[0], x[1], y[1]}, a1[4] = {x[2], y[2], x[3], y[3]};
-    float d[4] = {};
-    mma_16816_t(__half{}, d, a0, u.f[i][0], u.f[i][1]);
+    float d[4];
+    mma_zero(__half{}, d, a0, u.f[i][0], u.f[i][1]);
     mma_16816_t(__half{}, d, a1, u.f[i][2], u.f[i][3]);
     const float s0 = step_of(T{}, params[0][i]), s1 = step_of(T{}, params[1][i]);
-    sum[0] = fmaf(d[0], s0, sum[0]);
-    sum[1] = fmaf(d[1], s0, sum[1]);
-    sum[2] = fmaf(d[2], s1, sum[2]);
-    sum[3] = fmaf(d[3], s1, sum[3]);
+    sum[0] = i ? fmaf(d[0], s0, sum[0]) : d[0] * s0;
+    sum[1] = i ? fmaf(d[1], s0, sum[1]) : d[1] * s0;
+    sum[2] = i ? fmaf(d[2], s1, sum[2]) : d[2] * s1;
+    sum[3] = i ? fmaf(d[3], s1, sum[3]) : d[3] * s1;
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e) s[e] = fmaf(sum[e], 262144.f, low[e]) * u.c1[e & 1] * u.c2[e & 1];
+}
+
+// What a warp keeps of a unit.
+template <int D>
+struct Stream {
+  Queries<D> u;
+  float o[D / 32][2][4];      // element 32 i + 4 g + 2 j of heads 2t, 2t + 1, then the next one
+  float extra[4];             // sums of weights with lows (row g < 4) and with steps (g - 4)
+  float m[2], ref[2], l[2];   // of heads 2t, 2t + 1; ref: m, or 0 where there is none
+};
+
+// Takes kN blocks in.  valid: their slots that count (of blocks[0] there may be none).
+template <typename T, int D, int kN>
+__device__ __forceinline__ void take_blocks(Stream<D>& w, uint8_t* const (&blocks)[2], const int (&valid)[2], int lane) {
+  using Block = Q4Block<D>;
+  constexpr int G = D / 32;
+  constexpr bool kF16 = std::is_same<T, __half>::value;
+  const int g = lane >> 2, t4 = lane & 3;
+  const bool whole = kN == 2 ? valid[0] + valid[1] == 32 : valid[0] == 16;
+  if (!whole) {
+    // what lies behind the end may be anything, and 0 weight times NaN would be NaN
+#pragma unroll
+    for (int n = 0; n < kN; ++n)
+      for (int i = lane; i < 16 * G; i += 32)
+        if ((i & 15) >= valid[n]) reinterpret_cast<uint32_t*>(blocks[n] + Block::kValueSteps)[i] = 0;
+    __syncwarp();
+  }
+  // ---- scores: lane 4 g + t has word t of slots g and g + 8
+  float sv[kN][4];
+#pragma unroll
+  for (int n = 0; n < kN; ++n) {
+    const uint32_t at = smem_u32(blocks[n]);
+    uint32_t codes[2][G], params[2][G], r[4];
+    if constexpr (G == 4) {
+      const uint32_t row = at + (lane >> 3) * 256 + (lane & 7) * 16;
+      ldmatrix_x4(r, row);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) codes[0][i] = r[i];
+      ldmatrix_x4(r, row + 128);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) codes[1][i] = r[i];
+    } else {
+      ldmatrix_x4(r, at + lane * 16);   // group 0: slots 0 .. 7, 8 .. 15, group 1
+      codes[0][0] = r[0], codes[1][0] = r[1], codes[0][1] = r[2], codes[1][1] = r[3];
+    }
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      params[0][i] = lds32(at + Block::kKeySteps + i * 64 + g * 4);
+      params[1][i] = lds32(at + Block::kKeySteps + i * 64 + 32 + g * 4);
+    }
+    block_scores<T, D>(w.u, codes, params, sv[n]);
+  }
+  if (!whole) {
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+      if (g >= valid[n]) sv[n][0] = sv[n][1] = -INFINITY;
+      if (g + 8 >= valid[n]) sv[n][2] = sv[n][3] = -INFINITY;
+    }
+  }
+  // ---- the running reference moves when a score passes it by 8
+  float mx[2] = {fmaxf(sv[0][0], sv[0][2]), fmaxf(sv[0][1], sv[0][3])};
+  if constexpr (kN == 2) {
+    mx[0] = fmaxf(mx[0], fmaxf(sv[1][0], sv[1][2]));
+    mx[1] = fmaxf(mx[1], fmaxf(sv[1][1], sv[1][3]));
+  }
+  if (__any_sync(0xffffffffu, mx[0] > w.m[0] + 8.f || mx[1] > w.m[1] + 8.f)) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float x = mx[e];
+      x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+      x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+      x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+      const float r = fmaxf(w.m[e], x);
+      const float f = r == -INFINITY ? 1.f : exp2_fast(w.m[e] - r);
+      w.m[e] = r;
+      w.ref[e] = r == -INFINITY ? 0.f : r;
+      w.l[e] *= f;
+      w.extra[e] *= f;
+#pragma unroll
+      for (int i = 0; i < G; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          w.o[i][j][e] *= f;
+          w.o[i][j][2 + e] *= f;
+        }
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < kN; ++n) {
+    const uint32_t at = smem_u32(blocks[n]);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      sv[n][e] = exp2_fast(sv[n][e] - w.ref[e]);
+      sv[n][2 + e] = exp2_fast(sv[n][2 + e] - w.ref[e]);
+      w.l[e] += sv[n][e] + sv[n][2 + e];
+    }
+    // ---- weights, turned: lane 4 g + t has head g, slots 2t, 2t+1 and 8 + those
+    uint32_t h0, h1, e0, e1;   // in the cache's type, and what rounding left
+    float pw[4];               // fp16: the weights themselves
+    if constexpr (kF16) {
+      const uint32_t x0 = movmatrix(prmt(__float_as_uint(sv[n][0]), __float_as_uint(sv[n][1]), 0x7632));
+      const uint32_t y0 = movmatrix(prmt(__float_as_uint(sv[n][0]), __float_as_uint(sv[n][1]), 0x5410));
+      const uint32_t x1 = movmatrix(prmt(__float_as_uint(sv[n][2]), __float_as_uint(sv[n][3]), 0x7632));
+      const uint32_t y1 = movmatrix(prmt(__float_as_uint(sv[n][2]), __float_as_uint(sv[n][3]), 0x5410));
+      pw[0] = __uint_as_float(prmt(y0, x0, 0x5410));
+      pw[1] = __uint_as_float(prmt(y0, x0, 0x7632));
+      pw[2] = __uint_as_float(prmt(y1, x1, 0x5410));
+      pw[3] = __uint_as_float(prmt(y1, x1, 0x7632));
+      split2<T>(pw[0], pw[1], &h0, &e0);
+      split2<T>(pw[2], pw[3], &h1, &e1);
+    } else {
+      split2<T>(sv[n][0], sv[n][1], &h0, &e0);
+      split2<T>(sv[n][2], sv[n][3], &h1, &e1);
+      h0 = movmatrix(h0);
+      h1 = movmatrix(h1);
+      e0 = movmatrix(e0);
+      e1 = movmatrix(e1);
+    }
+    const uint32_t vs = at + Block::kValueSteps + t4 * 8;
+    {   // sums of weights with lows and steps: row g is the low of group g, or the step of g - 4
+      const int i = g & 3;
+      uint32_t x[4] = {};
+      if (i < G) {
+        const uint2 v0 = lds64(vs + i * 64), v1 = lds64(vs + i * 64 + 32);
+        const uint32_t sel = g < 4 ? 0x7632 : 0x5410;
+        x[0] = prmt(v0.x, v0.y, sel);
+        x[2] = prmt(v1.x, v1.y, sel);
+      }
+      mma_16816_t(T{}, w.extra, x, h0, h1);
+      mma_16816_t(T{}, w.extra, x, e0, e1);
+    }
+    // ---- o^T += (128 + codes)^T (step weights)^T
+    uint32_t vc[G][2];   // [half]: unit g (elements 4 g ..) of slots 2t, 2t+1 of that half
+    {
+      uint32_t r[4];
+      const uint32_t row = at + Block::kValues + lane * 16;
+      ldmatrix_x4_trans(r, row);
+      vc[0][0] = r[0], vc[0][1] = r[1], vc[1][0] = r[2], vc[1][1] = r[3];
+      if constexpr (G == 4) {
+        ldmatrix_x4_trans(r, row + 512);
+        vc[2][0] = r[0], vc[2][1] = r[1], vc[3][0] = r[2], vc[3][1] = r[3];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      const uint2 v0 = lds64(vs + i * 64), v1 = lds64(vs + i * 64 + 32);
+      uint32_t b0, b1, c0, c1;
+      if constexpr (kF16) {
+        split2<__nv_bfloat16>(pw[0] * step_of(T{}, v0.x), pw[1] * step_of(T{}, v0.y), &b0, &c0);
+        split2<__nv_bfloat16>(pw[2] * step_of(T{}, v1.x), pw[3] * step_of(T{}, v1.y), &b1, &c1);
+      } else {
+        step_weights(h0, e0, prmt(v0.x, v0.y, 0x5410), &b0, &c0);
+        step_weights(h1, e1, prmt(v1.x, v1.y, 0x5410), &b1, &c1);
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t x[4] = {large_code(vc[i][0], 2 * j), large_code(vc[i][0], 2 * j + 1),
+                               large_code(vc[i][1], 2 * j), large_code(vc[i][1], 2 * j + 1)};
+        mma_16816_t(__nv_bfloat16{}, w.o[i][j], x, b0, b1);
+        mma_16816_t(__nv_bfloat16{}, w.o[i][j], x, c0, c1);
+      }
+    }
+  }
+  if (!whole) fence_proxy_async();   // the zeros before the next copy
 }
 
 template <typename T, int D>
@@ -266,8 +445,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_q4_decode(const __grid
     const int P = a.kv.page_size;
     const uint32_t capacity = a.kv.max_pages * a.kv.page_size;
     // lane l < 8: block l of a tile; the first of each page's blocks copies them all
-    const int block = lane & (kWarps - 1), per_page = min(P / 16, kWarps);
-    const bool loads = lane < kWarps && block % per_page == 0;
+    const int block = lane & (kBlocks - 1), per_page = min(P / 16, kBlocks);
+    const bool loads = lane < kBlocks && block % per_page == 0;
     uint32_t it = 0, pieces = 0;
     int seq, n_cut = 0;
     uint32_t before, L, runs = gridDim.x;
@@ -331,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_q4_decode(const __grid
           break;
         }
         StageMeta& meta = s.meta[st];
-        if (lane < kWarps) meta.valid[lane] = min(behind, 16);
+        if (lane < kBlocks) meta.valid[lane] = min(behind, 16);
         if (lane == 0) {
           meta.flags = (first ? kFirst : 0) | (last ? kLast : 0);
           meta.heads = heads;
@@ -420,8 +599,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_q4_decode(const __grid
 
   // -------------------------------------------------------------- consumers --
   const int g = lane >> 2, t4 = lane & 3;
-  Queries<D> u;
-  float o[G][2][4], extra[4], m[2], l[2];   // extra: sums of weights with lows (row g < 4) and steps (g - 4)
+  Stream<D> w;
   uint32_t pieces = 0, joins = 0;
   auto join = [&]() {   // the consumer warps' barrier
     __syncwarp();
@@ -439,173 +617,41 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_q4_decode(const __grid
       const int qs = pieces % QS;
       if (!__all_sync(0xffffffffu, paged_wait(&s.qfull[qs], (pieces / QS) & 1, &s.abort, a.err))) return;
       ++pieces;
-      load_queries<T, D>(u, reinterpret_cast<const T*>(s.q[qs]), meta.heads, p.scale_log2, lane);
+      load_queries<T, D>(w.u, reinterpret_cast<const T*>(s.q[qs]), meta.heads, p.scale_log2, lane);
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.qempty[qs]);
-      m[0] = m[1] = -INFINITY;
-      l[0] = l[1] = 0.f;
+      w.m[0] = w.m[1] = -INFINITY;
+      w.ref[0] = w.ref[1] = w.l[0] = w.l[1] = 0.f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        extra[e] = 0.f;
+        w.extra[e] = 0.f;
 #pragma unroll
-        for (int i = 0; i < G; ++i) o[i][0][e] = o[i][1][e] = 0.f;
+        for (int i = 0; i < G; ++i) w.o[i][0][e] = w.o[i][1][e] = 0.f;
       }
     }
-    const int valid = meta.valid[warp];
-    if (valid > 0) {
-      uint8_t* block = s.kv[st][warp];
-      const uint32_t at = smem_u32(block);
-      if (valid < 16) {
-        // what lies behind the end may be anything, and 0 weight times NaN would be NaN
-        for (int i = lane; i < 16 * G; i += 32)
-          if ((i & 15) >= valid) reinterpret_cast<uint32_t*>(block + Block::kValueSteps)[i] = 0;
-        __syncwarp();
-      }
-      // ---- scores: lane 4 g + t has word t of slots g and g + 8
-      float sv[4];
-      {
-        uint32_t codes[2][G], params[2][G], r[4];
-        if constexpr (G == 4) {
-          const uint32_t row = at + (lane >> 3) * 256 + (lane & 7) * 16;
-          ldmatrix_x4(r, row);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) codes[0][i] = r[i];
-          ldmatrix_x4(r, row + 128);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) codes[1][i] = r[i];
-        } else {
-          ldmatrix_x4(r, at + lane * 16);   // group 0: slots 0 .. 7, 8 .. 15, group 1
-          codes[0][0] = r[0], codes[1][0] = r[1], codes[0][1] = r[2], codes[1][1] = r[3];
-        }
-#pragma unroll
-        for (int i = 0; i < G; ++i) {
-          params[0][i] = lds32(at + Block::kKeySteps + i * 64 + g * 4);
-          params[1][i] = lds32(at + Block::kKeySteps + i * 64 + 32 + g * 4);
-        }
-        block_scores<T, D>(u, codes, params, sv);
-      }
-      if (g >= valid) sv[0] = sv[1] = -INFINITY;
-      if (g + 8 >= valid) sv[2] = sv[3] = -INFINITY;
-      // ---- the running reference moves when a score passes it by 8
-      const float mx[2] = {fmaxf(sv[0], sv[2]), fmaxf(sv[1], sv[3])};
-      if (__any_sync(0xffffffffu, mx[0] > m[0] + 8.f || mx[1] > m[1] + 8.f)) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float x = mx[e];
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-          const float r = fmaxf(m[e], x);
-          const float f = r == -INFINITY ? 1.f : exp2_fast(m[e] - r);
-          m[e] = r;
-          l[e] *= f;
-          extra[e] *= f;
-#pragma unroll
-          for (int i = 0; i < G; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              o[i][j][e] *= f;
-              o[i][j][2 + e] *= f;
-            }
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float r = m[e] == -INFINITY ? 0.f : m[e];
-        sv[e] = exp2_fast(sv[e] - r);
-        sv[2 + e] = exp2_fast(sv[2 + e] - r);
-        l[e] += sv[e] + sv[2 + e];
-      }
-      // ---- weights, turned: lane 4 g + t has head g, slots 2t, 2t+1 and 8 + those
-      uint32_t h0, h1, e0, e1;   // in the cache's type, and what rounding left
-      float pw[4];               // fp16: the weights themselves
-      if constexpr (std::is_same<T, __half>::value) {
-        const uint32_t x0 = movmatrix(prmt(__float_as_uint(sv[0]), __float_as_uint(sv[1]), 0x7632));
-        const uint32_t y0 = movmatrix(prmt(__float_as_uint(sv[0]), __float_as_uint(sv[1]), 0x5410));
-        const uint32_t x1 = movmatrix(prmt(__float_as_uint(sv[2]), __float_as_uint(sv[3]), 0x7632));
-        const uint32_t y1 = movmatrix(prmt(__float_as_uint(sv[2]), __float_as_uint(sv[3]), 0x5410));
-        pw[0] = __uint_as_float(prmt(y0, x0, 0x5410));
-        pw[1] = __uint_as_float(prmt(y0, x0, 0x7632));
-        pw[2] = __uint_as_float(prmt(y1, x1, 0x5410));
-        pw[3] = __uint_as_float(prmt(y1, x1, 0x7632));
-        split2<T>(pw[0], pw[1], &h0, &e0);
-        split2<T>(pw[2], pw[3], &h1, &e1);
-      } else {
-        split2<T>(sv[0], sv[1], &h0, &e0);
-        split2<T>(sv[2], sv[3], &h1, &e1);
-        h0 = movmatrix(h0);
-        h1 = movmatrix(h1);
-        e0 = movmatrix(e0);
-        e1 = movmatrix(e1);
-      }
-      const uint32_t vs = at + Block::kValueSteps + t4 * 8;
-      {   // sums of weights with lows and steps: row g is the low of group g, or the step of g - 4
-        const int i = g & 3;
-        uint32_t w[4] = {};
-        if (i < G) {
-          const uint2 v0 = lds64(vs + i * 64), v1 = lds64(vs + i * 64 + 32);
-          const uint32_t sel = g < 4 ? 0x7632 : 0x5410;
-          w[0] = prmt(v0.x, v0.y, sel);
-          w[2] = prmt(v1.x, v1.y, sel);
-        }
-        mma_16816_t(T{}, extra, w, h0, h1);
-        mma_16816_t(T{}, extra, w, e0, e1);
-      }
-      // ---- o^T += (128 + codes)^T (step weights)^T
-      uint32_t vc[G][2];   // [half]: unit g (elements 4 g ..) of slots 2t, 2t+1 of that half
-      {
-        uint32_t r[4];
-        const uint32_t row = at + Block::kValues + lane * 16;
-        ldmatrix_x4_trans(r, row);
-        vc[0][0] = r[0], vc[0][1] = r[1], vc[1][0] = r[2], vc[1][1] = r[3];
-        if constexpr (G == 4) {
-          ldmatrix_x4_trans(r, row + 512);
-          vc[2][0] = r[0], vc[2][1] = r[1], vc[3][0] = r[2], vc[3][1] = r[3];
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < G; ++i) {
-        const uint2 v0 = lds64(vs + i * 64), v1 = lds64(vs + i * 64 + 32);
-        uint32_t b0, b1, c0, c1;
-        if constexpr (std::is_same<T, __half>::value) {
-          split2<__nv_bfloat16>(pw[0] * step_of(T{}, v0.x), pw[1] * step_of(T{}, v0.y), &b0, &c0);
-          split2<__nv_bfloat16>(pw[2] * step_of(T{}, v1.x), pw[3] * step_of(T{}, v1.y), &b1, &c1);
-        } else {
-          const uint32_t s0 = prmt(v0.x, v0.y, 0x5410), s1 = prmt(v1.x, v1.y, 0x5410);
-          b0 = mul_bf16x2(h0, s0);
-          b1 = mul_bf16x2(h1, s1);
-          c0 = fma_bf16x2(e0, s0, fma_bf16x2(h0, s0, b0 ^ 0x80008000u));
-          c1 = fma_bf16x2(e1, s1, fma_bf16x2(h1, s1, b1 ^ 0x80008000u));
-        }
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint32_t w[4] = {large_code(vc[i][0], 2 * j), large_code(vc[i][0], 2 * j + 1),
-                                 large_code(vc[i][1], 2 * j), large_code(vc[i][1], 2 * j + 1)};
-          mma_16816_t(__nv_bfloat16{}, o[i][j], w, b0, b1);
-          mma_16816_t(__nv_bfloat16{}, o[i][j], w, c0, c1);
-        }
-      }
-      if (valid < 16) fence_proxy_async();   // the zeros before the next copy
-    }
+    const int valid[2] = {meta.valid[warp], meta.valid[warp + kWarps]};
+    uint8_t* const blocks[2] = {s.kv[st][warp], s.kv[st][warp + kWarps]};
+    if (valid[1] > 0) take_blocks<T, D, 2>(w, blocks, valid, lane);
+    else if (valid[0] > 0) take_blocks<T, D, 1>(w, blocks, valid, lane);
     if (!(flags & kLast)) {
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.empty[st]);
       continue;
     }
 
-    // ---- the end of a piece.  o[i][j][e]: element 32 i + 4 g + 2 j of head 2t + e, [2 + e]:
-    // the next one.  Four warps hand their rows to the other four, whose sums are joined.
+    // ---- the end of a piece.  Half of the warps hand their rows to the other half, whose
+    // sums are joined.
     const StageMeta unit = meta;
     __syncwarp();
     if (lane == 0) mbar_arrive(&s.empty[st]);
     float2(*ml)[kSlotHeads] = s.ml[(pieces - 1) & 1];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      float x = l[e];
+      float x = w.l[e];
       x += __shfl_xor_sync(0xffffffffu, x, 4);
       x += __shfl_xor_sync(0xffffffffu, x, 8);
       x += __shfl_xor_sync(0xffffffffu, x, 16);
-      if (g == 0) ml[warp][2 * t4 + e] = make_float2(m[e], x);
+      if (g == 0) ml[warp][2 * t4 + e] = make_float2(w.m[e], x);
     }
     if (!join()) return;
     float f[2];
@@ -613,19 +659,19 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_q4_decode(const __grid
     for (int e = 0; e < 2; ++e) {
       float M = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) M = fmaxf(M, ml[w][2 * t4 + e].x);
-      f[e] = m[e] == -INFINITY ? 0.f : exp2_fast(m[e] - M);
+      for (int k = 0; k < kWarps; ++k) M = fmaxf(M, ml[k][2 * t4 + e].x);
+      f[e] = w.m[e] == -INFINITY ? 0.f : exp2_fast(w.m[e] - M);
     }
 #pragma unroll
     for (int i = 0; i < G; ++i)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float add = __shfl_sync(0xffffffffu, extra[e], 4 * i + t4) -
-                          128.f * __shfl_sync(0xffffffffu, extra[e], 4 * (4 + i) + t4);
+        const float add = __shfl_sync(0xffffffffu, w.extra[e], 4 * i + t4) -
+                          128.f * __shfl_sync(0xffffffffu, w.extra[e], 4 * (4 + i) + t4);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          o[i][j][e] = (o[i][j][e] + add) * f[e];
-          o[i][j][2 + e] = (o[i][j][2 + e] + add) * f[e];
+          w.o[i][j][e] = (w.o[i][j][e] + add) * f[e];
+          w.o[i][j][2 + e] = (w.o[i][j][2 + e] + add) * f[e];
         }
       }
     if (warp >= kMergeRows) {
@@ -634,7 +680,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_q4_decode(const __grid
 #pragma unroll
         for (int e = 0; e < 2; ++e)
           s.rows[warp - kMergeRows][2 * t4 + e][(8 * i + g) ^ (2 * t4)] =
-              make_float4(o[i][0][e], o[i][0][2 + e], o[i][1][e], o[i][1][2 + e]);
+              make_float4(w.o[i][0][e], w.o[i][0][2 + e], w.o[i][1][e], w.o[i][1][2 + e]);
     }
     if (!join()) return;
     if (warp < kMergeRows) {
@@ -644,7 +690,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_q4_decode(const __grid
         for (int e = 0; e < 2; ++e) {
           float4& at = s.rows[warp][2 * t4 + e][(8 * i + g) ^ (2 * t4)];
           const float4 x = at;
-          at = make_float4(x.x + o[i][0][e], x.y + o[i][0][2 + e], x.z + o[i][1][e], x.w + o[i][1][2 + e]);
+          at = make_float4(x.x + w.o[i][0][e], x.y + w.o[i][0][2 + e], x.z + w.o[i][1][e], x.w + w.o[i][1][2 + e]);
         }
     }
     if (!join()) return;
