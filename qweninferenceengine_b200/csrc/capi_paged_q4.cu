@@ -127,8 +127,6 @@ int qwen_attention_paged_q4(const qwen_paged_kv_q4* kv, const uint16_t* q, int64
   if (kv->n_seq == 0) return QWEN_OK;
   QWEN_TRY(check_rows(op, "q", q, q_stride, n_heads * kv->head_dim));
   QWEN_TRY(check_rows(op, "out", out, out_stride, n_heads * kv->head_dim));
-  if (kv->weights && q == out)
-    return set_error(QWEN_ERR_INVALID_ARGUMENT, "%s: out must not be q where weights are kept", op);
   if (!seq_len) return set_error(QWEN_ERR_INVALID_ARGUMENT, "%s: null seq_len", op);
   QWEN_TRY(check_workspace(op, workspace, workspace_bytes, qwen_attention_paged_q4_workspace(kv, n_heads)));
   QWEN_TRY(check_q4_tiles(op, kv, n_heads));

@@ -50,6 +50,7 @@ struct StageMeta {
   int flags;
   int seq, head, heads;   // the unit: sequence, first query head, query heads
   int dest;            // partial slot, or -1: the whole unit, or -2: nothing is written
+  float2* scores;      // of the tile's first slot, or null
 };
 
 template <int D>
@@ -70,6 +71,8 @@ struct __align__(128) Q4DecodeSmem {
 
 struct Q4DecodeArgs : DecodeArgs {
   qwen_paged_kv_q4 kv;
+  float* scores;     // where weights are kept: [unit][capacity][2 score_pairs], log2 domain
+  int score_pairs;   // query heads of a unit in pairs
 };
 
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((127 + e) << 23); }   // -126 <= e <= 127
@@ -257,9 +260,11 @@ struct Stream {
   float m[2], ref[2], l[2];   // of heads 2t, 2t + 1; ref: m, or 0 where there is none
 };
 
-// Takes kN blocks in.  valid: their slots that count (of blocks[0] there may be none).
+// Takes kN blocks in.  valid: their slots that count (of blocks[0] there may be none);
+// scores: where blocks[0]'s go, blocks[1]'s 16 kWarps slots behind, or null.
 template <typename T, int D, int kN>
-__device__ __forceinline__ void take_blocks(Stream<D>& w, uint8_t* const (&blocks)[2], const int (&valid)[2], int lane) {
+__device__ __forceinline__ void take_blocks(Stream<D>& w, uint8_t* const (&blocks)[2], const int (&valid)[2], int lane,
+                                            float2* scores, int score_pairs) {
   using Block = Q4Block<D>;
   constexpr int G = D / 32;
   constexpr bool kF16 = std::is_same<T, __half>::value;
@@ -304,6 +309,15 @@ __device__ __forceinline__ void take_blocks(Stream<D>& w, uint8_t* const (&block
       if (g >= valid[n]) sv[n][0] = sv[n][1] = -INFINITY;
       if (g + 8 >= valid[n]) sv[n][2] = sv[n][3] = -INFINITY;
     }
+  }
+  if (scores && t4 < score_pairs) {
+#pragma unroll
+    for (int n = 0; n < kN; ++n)
+      if (valid[n] > 0) {
+        float2* to = scores + (16 * kWarps * n + g) * score_pairs + t4;
+        to[0] = make_float2(sv[n][0], sv[n][1]);
+        to[8 * score_pairs] = make_float2(sv[n][2], sv[n][3]);
+      }
   }
   // ---- the running reference moves when a score passes it by 8
   float mx[2] = {fmaxf(sv[0][0], sv[0][2]), fmaxf(sv[0][1], sv[0][3])};
@@ -514,6 +528,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_q4_decode(const __grid
         if (lane == 0) {
           meta.flags = (first ? kFirst : 0) | (last ? kLast : 0);
           meta.heads = heads;
+          if (p.scores)
+            meta.scores = reinterpret_cast<float2*>(p.scores) +
+                          (((long long)seq * p.units_per_seq + unit) * capacity + tile * kTile) * p.score_pairs;
           if (last) {
             meta.seq = seq;
             meta.head = head;
@@ -631,8 +648,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_q4_decode(const __grid
     }
     const int valid[2] = {meta.valid[warp], meta.valid[warp + kWarps]};
     uint8_t* const blocks[2] = {s.kv[st][warp], s.kv[st][warp + kWarps]};
-    if (valid[1] > 0) take_blocks<T, D, 2>(w, blocks, valid, lane);
-    else if (valid[0] > 0) take_blocks<T, D, 1>(w, blocks, valid, lane);
+    float2* scores = p.scores ? meta.scores + 16 * warp * p.score_pairs : nullptr;
+    if (valid[1] > 0) take_blocks<T, D, 2>(w, blocks, valid, lane, scores, p.score_pairs);
+    else if (valid[0] > 0) take_blocks<T, D, 1>(w, blocks, valid, lane, scores, p.score_pairs);
     if (!(flags & kLast)) {
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.empty[st]);
@@ -747,40 +765,88 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_q4_decode(const __grid
   }
 }
 
-// weights[s][h][slot] += sum over the query heads of kv head h of exp(scale q k - lse).
-template <typename T, int D>
-__global__ void __launch_bounds__(128) k_weigh_q4(const __grid_constant__ Q4AttnArgs a, const float* lse) {
-  const int s = blockIdx.z, h = blockIdx.y, group = a.n_heads / (int)a.kv.n_kv_heads;
-  const uint32_t L = a.seq_len[s];
-  if (L > q4_capacity(a.kv)) return;
-  for (uint32_t slot = blockIdx.x * 128 + threadIdx.x; slot < L; slot += gridDim.x * 128) {
-    const int page = q4_page(a.kv, a.err, s, slot >> a.page_shift);
-    if (page < 0) continue;
-    const int in_page = slot & (a.kv.page_size - 1), r = in_page & 15;
-    const uint8_t* block = q4_block<D>(a.kv, page, h, in_page);
-    float total = 0.f;
-    for (int j = 0; j < group; ++j) {
-      const int head = h * group + j;
-      const T* q = reinterpret_cast<const T*>(a.q) + (long long)s * a.q_stride + head * D;
-      float score = 0.f;
-      for (int g = 0; g < D / 32; ++g) {
-        const uint4 w = *reinterpret_cast<const uint4*>(block + g * 256 + r * 16);
-        const uint32_t p = *reinterpret_cast<const uint32_t*>(block + Q4Block<D>::kKeySteps + g * 64 + r * 4);
-        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float x[8];
-          expand_word<T>(ws[i], p, x);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) score += x[e] * (float)q[32 * g + 8 * i + e];
-        }
-      }
-      total += exp2f(score * a.scale * kLog2e - lse[(long long)s * a.n_heads + head] * kLog2e);
+// weights[s][h][slot] += sum over the query heads of kv head h of exp(scale q k - lse), from
+// the scores that k_q4_decode left.  Each warp has a run of tiles of 32 slots, a lane a slot,
+// as the decode kernel's CTAs have runs of theirs; the next tile is on its way while one is
+// summed.  (A pass over the keys that forms the scores again, 80 B a slot and kv head of 128
+// instead of 8 a query head, took 32 us behind 16 x 8704 of 8 kv heads where this takes
+// 9: it has all the instructions of a score once more.)
+constexpr int kWeighWarps = 8, kWeighTileShift = 5, kWeighCtasPerSm = 4;
+
+template <int kPairs>   // query heads of a unit in pairs
+__global__ void __launch_bounds__(kWeighWarps * 32, kWeighCtasPerSm) k_q4_weigh(const __grid_constant__ Q4DecodeArgs p, int chunks) {
+  const PagedAttnArgs& a = p.a;
+  const int lane = threadIdx.x & 31;
+  // (Lengths and tables were there before the attention, which this need not wait for.)
+  const uint32_t c = blockIdx.x * kWeighWarps + (threadIdx.x >> 5);
+  uint32_t runs = gridDim.x * kWeighWarps, before, L;
+  int seq;
+  const uint32_t total = find_run(p, c, runs, lane, &seq, &before, &L);
+  const uint32_t t1 = run_start(total, c + 1, runs), capacity = a.kv.max_pages * a.kv.page_size;
+  uint32_t t = run_start(total, c, runs), ts = seq_tiles(p, L);
+  struct Slot {
+    float2 s[kPairs];
+    float old;
+    const float2* more;   // the next chunk's scores
+    float* to;            // null: nothing to add to
+    int seq, head;
+  } next;
+  auto load = [&](Slot& x) {
+    while (t >= before + ts * p.units_per_seq) {
+      before += ts * p.units_per_seq;
+      L = a.seq_len[++seq];
+      ts = seq_tiles(p, L);
     }
-    a.kv.weights[((long long)s * a.kv.n_kv_heads + h) * q4_capacity(a.kv) + slot] += total;
+    const int h = (int)((t - before) / ts);
+    const uint32_t slot = ((t - before - h * ts) << kWeighTileShift) + lane, len = L <= capacity ? L : 0;
+    ++t;
+    x.seq = seq;
+    x.head = h;
+    x.to = nullptr;
+    if (slot >= len) return;
+    const int page = a.kv.page_table[(long long)seq * a.kv.table_stride + (slot >> a.page_shift)];
+    if (page < 0 || (uint32_t)page >= a.kv.n_pages) return;   // (reported by the attention)
+    const long long unit = (long long)seq * a.kv.n_kv_heads + h;
+    x.to = p.kv.weights + unit * capacity + slot;
+    x.more = reinterpret_cast<const float2*>(p.scores) + (unit * chunks * capacity + slot) * kPairs;
+    x.old = *x.to;
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) x.s[i] = __ldcs(x.more + i);
+    x.more += (long long)capacity * kPairs;
+  };
+  pdl_wait();
+  if (t >= t1) return;
+  load(next);
+  int l_seq = -1, l_head = -1;
+  float lse[2 * kPairs];
+  while (true) {
+    Slot x = next;
+    const bool more = t < t1;
+    if (more) load(next);
+    if (l_seq != x.seq || l_head != x.head || chunks > 1) {
+#pragma unroll
+      for (int i = 0; i < 2 * kPairs; ++i)   // a head that is not there: no weight
+        lse[i] = i < p.group ? a.lse[(long long)x.seq * a.n_heads + x.head * p.group + i] * kLog2e : INFINITY;
+      l_seq = x.seq;
+      l_head = x.head;
+    }
+    if (x.to) {
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) sum += exp2_fast(x.s[i].x - lse[2 * i]) + exp2_fast(x.s[i].y - lse[2 * i + 1]);
+      for (int chunk = 1; chunk < chunks; ++chunk, x.more += (long long)capacity * kPairs)
+#pragma unroll
+        for (int i = 0; i < 2 * kPairs; ++i) {
+          const int head = chunk * kSlotHeads + i;
+          if (head < p.group)
+            sum += exp2_fast(reinterpret_cast<const float*>(x.more)[i] -
+                             a.lse[(long long)x.seq * a.n_heads + x.head * p.group + head] * kLog2e);
+        }
+      *x.to = x.old + sum;
+    }
+    if (!more) return;
   }
 }
-
 
 template <typename T, int D>
 int launch(const Q4AttnArgs& args, const Q4DecodeArgs& p, int runs, cudaStream_t st) {
@@ -800,15 +866,22 @@ int launch(const Q4AttnArgs& args, const Q4DecodeArgs& p, int runs, cudaStream_t
   static OncePerDevice once;
   if (once.launch(reinterpret_cast<const void*>(kern), smem, [&] { return cudaLaunchKernelEx(&cfg, kern, p); }) != cudaSuccess)
     return -1;
-  if (args.kv.weights) {
-    const unsigned ctas = std::min(64u, (args.kv.max_pages * args.kv.page_size + 127) / 128);
-    k_weigh_q4<T, D><<<dim3(ctas, args.kv.n_kv_heads, args.kv.n_seq), 128, 0, st>>>(args, p.a.lse);
-  }
-  return 0;
+  if (!args.kv.weights) return 0;
+  Q4DecodeArgs w = p;   // its units are whole kv heads
+  w.units_per_seq = (int)args.kv.n_kv_heads;
+  w.tile_shift = kWeighTileShift;
+  cfg.gridDim = dim3(kWeighCtasPerSm * paged_sm_count());
+  cfg.blockDim = dim3(kWeighWarps * 32);
+  cfg.dynamicSmemBytes = 0;
+  auto weigh = p.score_pairs == 1 ? k_q4_weigh<1> : p.score_pairs == 2 ? k_q4_weigh<2> : p.score_pairs == 3 ? k_q4_weigh<3> : k_q4_weigh<4>;
+  return cudaLaunchKernelEx(&cfg, weigh, w, p.chunks) == cudaSuccess ? 0 : -1;
 }
 
 int units_per_head(const qwen_paged_kv_q4& kv, int n_heads) {
   return (n_heads / (int)kv.n_kv_heads + kSlotHeads - 1) / kSlotHeads;
+}
+int score_pairs(const qwen_paged_kv_q4& kv, int n_heads) {
+  return (std::min(kSlotHeads, n_heads / (int)kv.n_kv_heads) + 1) / 2;
 }
 size_t units_of(const qwen_paged_kv_q4& kv, int n_heads) {
   return (size_t)kv.n_seq * kv.n_kv_heads * units_per_head(kv, n_heads);
@@ -817,15 +890,20 @@ size_t units_of(const qwen_paged_kv_q4& kv, int n_heads) {
 }  // namespace
 
 bool attention_q4_fits(const qwen_paged_kv_q4& kv, int n_heads) {
-  const double tiles = std::ceil((double)kv.max_pages * kv.page_size / kTile);
-  return (double)units_of(kv, n_heads) * tiles < 2147483648.0;
+  const double slots = (double)kv.max_pages * kv.page_size;
+  return (double)units_of(kv, n_heads) * std::ceil(slots / kTile) < 2147483648.0 &&
+         (!kv.weights || (double)kv.n_seq * kv.n_kv_heads * std::ceil(slots / (1 << kWeighTileShift)) < 2147483648.0);
 }
 
-// Partials and arrivals, as DecodeArgs has them, and where weights are kept the lse.
+// Partials and arrivals, as DecodeArgs has them, and where weights are kept the scores of
+// every unit at its capacity and the lse.
 size_t attention_q4_workspace(const qwen_paged_kv_q4& kv, int n_heads) {
-  const size_t runs = kCtasPerSm * paged_sm_count();
-  return 2 * runs * kSlotHeads * (kv.head_dim + 2) * sizeof(float) +
-         (2 * runs + units_of(kv, n_heads)) * sizeof(unsigned long long) + (size_t)kv.n_seq * n_heads * sizeof(float);
+  const size_t runs = kCtasPerSm * paged_sm_count(), units = units_of(kv, n_heads);
+  size_t bytes = 2 * runs * kSlotHeads * (kv.head_dim + 2) * sizeof(float) + (2 * runs + units) * sizeof(unsigned long long);
+  if (kv.weights)
+    bytes += units * kv.max_pages * kv.page_size * score_pairs(kv, n_heads) * sizeof(float2) +
+             (size_t)kv.n_seq * n_heads * sizeof(float);
+  return bytes;
 }
 
 int launch_attention_q4(const Q4AttnArgs& a, cudaStream_t st) {
@@ -856,7 +934,13 @@ int launch_attention_q4(const Q4AttnArgs& a, cudaStream_t st) {
   p.part_o = static_cast<float*>(a.workspace);
   p.part_ml = p.part_o + (size_t)2 * runs * kSlotHeads * a.kv.head_dim;
   p.arrived = reinterpret_cast<unsigned long long*>(p.part_ml + (size_t)2 * runs * kSlotHeads * 2);
-  p.a.lse = a.lse ? a.lse : a.kv.weights ? reinterpret_cast<float*>(p.arrived + 2 * runs + units_of(a.kv, a.n_heads)) : nullptr;
+  p.a.lse = a.lse;
+  if (a.kv.weights) {
+    p.score_pairs = score_pairs(a.kv, a.n_heads);
+    p.scores = reinterpret_cast<float*>(p.arrived + 2 * runs + units_of(a.kv, a.n_heads));
+    if (!a.lse)
+      p.a.lse = p.scores + units_of(a.kv, a.n_heads) * a.kv.max_pages * a.kv.page_size * 2 * p.score_pairs;
+  }
   p.tag = paged_call_tag();
   const bool d64 = a.kv.head_dim == 64;
   if (a.kv.dtype == QWEN_DTYPE_F16) return d64 ? launch<__half, 64>(a, p, runs, st) : launch<__half, 128>(a, p, runs, st);

@@ -476,7 +476,8 @@ class PagedKVQ4:
         self.pool, self.page_table, self.weights, self.positions = pool, page_table, weights, positions
         self.dtype, self.device, self.index, self.n_seq = dtype, pool.device, index, n_seq
         self.n_kv_heads, self.head_dim, self.page_size = n_kv, width // 20, 16 * blocks
-        self.sizes = (index, n_seq, n_kv, width, max_pages)
+        # (what workspaces go by: their slots, and whether scores are kept)
+        self.sizes = (index, n_seq, n_kv, width, kept[2], weights is not None)
         # the stride of an axis of one element is never used: any valid value
         self._struct = PagedKVQ4Struct.from_buffer_copy(_PAGED_KV_Q4.pack(
             pool.data_ptr(), 0 if weights is None else weights.data_ptr(),
@@ -542,7 +543,7 @@ def attention_paged_q4(kv: PagedKVQ4, q: torch.Tensor, seq_len: torch.Tensor, sc
                        out: torch.Tensor | None = None, return_lse: bool = False):
     """attention_paged over a 4-bit cache (qwen_attention_paged_q4).  Where the cache
     keeps weights, each slot's is increased by the sum of the softmax weights that the
-    query heads of its kv head give it (out must not be q then)."""
+    query heads of its kv head give it."""
     return _attend(kv, lib().qwen_attention_paged_q4, "qwen_attention_paged_q4_workspace", (), (), q,
                    seq_len, (), scale, out, return_lse)
 

@@ -270,6 +270,10 @@ def test_attention_in_place_strided_and_without_positions():
     ref.check_attention((out, None), want)
     got = ops.attention_paged_q4(c.handle(), q, c.seq_len, out=q, return_lse=True)
     ref.check_attention(got, want)
+    kept = ref.Cache(15, [65, 0, 130], 12, 2, 128, 64, BF16, kept=True)
+    before, want = kept.weights.clone(), ref.attention(kept, 128 ** -0.5)
+    ref.check_attention(ops.attention_paged_q4(kept.handle(), kept.q, kept.seq_len, out=kept.q, return_lse=True), want)
+    ref.check_weights(kept.weights, before, want)
     none = ref.Cache(16, [0, 0], 12, 2, 64, 16, F16, kept=True)
     before = none.weights.clone()
     out, lse = ops.attention_paged_q4(none.handle(), none.q, none.seq_len, return_lse=True)
@@ -591,8 +595,6 @@ def test_refusals_of_the_wrappers():
         ops.rope_append_paged_q4(kv, q, k, v, c.seq_len, inv, pair_axis=torch.zeros(31, dtype=torch.uint8, device="cuda"))
     with pytest.raises(QwenError):   # two axes and no pair_axis
         ops.rope_append_paged_q4(kv, q, k, v, c.seq_len, inv, positions=torch.zeros(2, 2, dtype=torch.int32, device="cuda"))
-    with pytest.raises(QwenError):   # weights are formed from q after out is written
-        ops.attention_paged_q4(kv, c.q, c.seq_len, out=c.q)
     with pytest.raises(ValueError):
         ops.attention_paged_q4(kv, c.q.to(BF16), c.seq_len)
     with pytest.raises(ValueError):
