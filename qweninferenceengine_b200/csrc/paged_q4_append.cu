@@ -1,12 +1,11 @@
 // paged_q4_append.cu -- rotation of new queries and keys at given positions, the keys'
 // and values' way into a 4-bit paged cache, and its rows' way back into 16 bits.
 #include "paged_q4.cuh"
+#include "paged_rotate.cuh"
 #include "qwen_internal.h"
 
 namespace qwen {
 namespace {
-
-constexpr int kThreads = 128;
 
 // Rows of sequence s and its length; false (reported) where they do not fit.
 __device__ __forceinline__ bool rows_of(const qwen_paged_kv_q4& kv, const uint32_t* seq_len, const int32_t* cu,
@@ -23,41 +22,15 @@ __device__ __forceinline__ bool rows_of(const qwen_paged_kv_q4& kv, const uint32
   if (!ok) raise_error(err, kDevBadArgument);
   return ok;
 }
-// Sequence and slot of a row (a token, or a row read back); false: the row is no one's.
-__device__ __forceinline__ bool find_row(const qwen_paged_kv_q4& kv, const uint32_t* seq_len, const int32_t* cu,
-                                         int n_rows, int* err, int row, int* seq, int* slot) {
-  if (row >= n_rows) return false;
-  if (!cu) {
-    const uint32_t len = seq_len[row];
-    if (len > q4_capacity(kv)) raise_error(err, kDevBadArgument);
-    if (len == 0 || len > q4_capacity(kv)) return false;
-    *seq = row;
-    *slot = (int)len - 1;
-    return true;
-  }
-  int lo = 0, hi = (int)kv.n_seq - 1;   // the first s with cu[s + 1] > row
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (cu[mid + 1] > row) hi = mid;
-    else lo = mid + 1;
-  }
-  int row0, row1, L;
-  if (!rows_of(kv, seq_len, cu, n_rows, err, lo, &row0, &row1, &L) || row < row0 || row >= row1) return false;
-  *seq = lo;
-  *slot = L - (row1 - row);
-  return true;
-}
-
 struct Token {
-  int seq, slot, page;   // seq -1: no one's row; page -1: outside the pool
+  int seq, slot;    // seq -1: no one's row
+  uint8_t* block;   // the slot's, of head 0; null: its page is outside the pool
 };
-
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
-  const uint4 w = *reinterpret_cast<const uint4*>(p);
-  const float2 a = unpack2(T{}, w.x), b = unpack2(T{}, w.y), c = unpack2(T{}, w.z), d = unpack2(T{}, w.w);
-  x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y, x[4] = c.x, x[5] = c.y, x[6] = d.x, x[7] = d.y;
+template <int D>
+__device__ __forceinline__ uint8_t* block_of(const qwen_paged_kv_q4& kv, int page, int slot) {
+  return page < 0 ? nullptr : q4_block<D>(kv, page, 0, slot & ((int)kv.page_size - 1));
 }
+
 template <typename T>
 __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
   return make_uint4(pack2(T{}, x[0], x[1]), pack2(T{}, x[2], x[3]), pack2(T{}, x[4], x[5]), pack2(T{}, x[6], x[7]));
@@ -73,131 +46,371 @@ __device__ __forceinline__ void round8(float (&x)[8]) {
   }
 }
 
-// kTile tokens a CTA; D / 8 lanes a head's row, 8 elements each.
-template <typename T, int D, bool kInterleaved, int kTile>
-__global__ void __launch_bounds__(kThreads) k_append_q4(const __grid_constant__ Q4AppendArgs a) {
-  constexpr int NC = D / 8;
-  __shared__ double2 rot[kTile][D / 2];   // cos, sin
-  __shared__ Token tok[kTile];
-  const int tid = threadIdx.x, H = a.n_heads, K = a.kv.n_kv_heads, R = a.rot_dim;
+// 8 elements of a row, and of a key the 8 that theirs are turned with.
+struct Raw {
+  uint4 own, mate;
+};
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4& w, float (&x)[8]) {
+  const float2 a = unpack2(T{}, w.x), b = unpack2(T{}, w.y), c = unpack2(T{}, w.z), d = unpack2(T{}, w.w);
+  x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y, x[4] = c.x, x[5] = c.y, x[6] = d.x, x[7] = d.y;
+}
+// Lane c of a row: elements 8 c .. 8 c + 7; turned: whether they are rotated.
+template <typename T, bool kInterleaved>
+__device__ __forceinline__ Raw load_raw(const T* row, int c, int R, bool turned) {
+  Raw r;
+  r.own = *reinterpret_cast<const uint4*>(row + 8 * c);
+  if (!kInterleaved && turned) r.mate = *reinterpret_cast<const uint4*>(row + (8 * c >= R / 2 ? 8 * c - R / 2 : 8 * c + R / 2));
+  return r;
+}
+// Where a pair's (cos, sin) stands in shared memory: lanes side by side read adjacent ones.
+template <int D, bool kInterleaved>
+__device__ __forceinline__ int rot_at(int pair) {
+  constexpr int kOf = kInterleaved ? 4 : 8;   // pairs of a lane
+  return pair % kOf * (D / 2 / kOf) + pair / kOf;
+}
+// Rotates in the arithmetic of A (double for keys, float for queries).
+template <typename A, typename T, int D, bool kInterleaved>
+__device__ __forceinline__ void rotate_raw(const Raw& r, const double2* rot, int c, int R, float (&x)[8]) {
+  float own[8], mate[8];
+  unpack8<T>(r.own, own);
+  if constexpr (!kInterleaved) unpack8<T>(r.mate, mate);
+  const bool second = !kInterleaved && 8 * c >= R / 2;
+  const double2* at = rot + (kInterleaved ? c : c - (second ? R / 16 : 0));
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const double2 cs = at[rot_at<D, kInterleaved>(kInterleaved ? e / 2 : e)];
+    const bool two = kInterleaved ? e & 1 : second;
+    const A a = (A)own[e], b = (A)(kInterleaved ? own[e ^ 1] : mate[e]), s = (A)(two ? cs.y : -cs.y);
+    x[e] = (float)(a * (A)cs.x + b * s);
+  }
+}
+// Quantises lane c's 8 values of a key's or value's row and stores them (all 32 lanes; of
+// those whose token has a block, and not of others).
+template <typename T, int D>
+__device__ __forceinline__ void store_quantised(const Q4AppendArgs& a, const float (&x)[8], const Token& t, int h, bool is_k,
+                                                int c, bool live) {
+  uint32_t params;
+  const uint32_t codes = quantise_group<T>(x, &params);
+  if (!live || !t.block) return;
+  uint8_t* at = t.block + (long long)h * a.kv.head_stride;
+  const int g = c / 4, r = t.slot & 15;
+  *reinterpret_cast<uint32_t*>(at + (is_k ? 0 : Q4Block<D>::kValues) + g * 256 + r * 16 + (c & 3) * 4) = codes;
+  if ((c & 3) == 0)
+    *reinterpret_cast<uint32_t*>(at + (is_k ? Q4Block<D>::kKeySteps : Q4Block<D>::kValueSteps) + g * 64 + r * 4) = params;
+}
+__device__ __forceinline__ int axis_of(const Q4AppendArgs& a, int pair) {
+  if (!a.pair_axis) return 0;
+  const int axis = a.pair_axis[pair];
+  if (axis < a.n_axes) return axis;
+  raise_error(a.err, kDevBadArgument);
+  return 0;
+}
+__device__ __forceinline__ int position_of(const Q4AppendArgs& a, int pair, int row, int slot) {
+  return a.positions ? a.positions[axis_of(a, pair) * a.position_stride + row] : slot;
+}
+// What the cache keeps of the slot beside its key and value.
+__device__ __forceinline__ void keep_slot(const Q4AppendArgs& a, const Token& t, int h, int row) {
+  const long long at = ((long long)t.seq * a.kv.n_kv_heads + h) * q4_capacity(a.kv) + t.slot;
+  if (a.kv.weights) a.kv.weights[at] = 0.f;
+  if (a.kv.positions) a.kv.positions[at] = a.positions ? a.positions[row] : t.slot;
+}
+
+// One token per sequence: a CTA per token, D / 8 lanes a row.  A row's elements are on their
+// way while length, page and angles are found.
+constexpr int kTokenThreads = 256;
+template <typename T, int D, bool kInterleaved>
+__global__ void __launch_bounds__(kTokenThreads) k_append_token_q4(const __grid_constant__ Q4AppendArgs a) {
+  constexpr int NC = D / 8, kRows = kTokenThreads / NC;
+  __shared__ double2 rot[D / 2];   // cos, sin
+  const int tid = threadIdx.x, H = a.n_heads, K = a.kv.n_kv_heads, R = a.rot_dim, c = tid % NC, row = blockIdx.x;
   pdl_wait();
   if (tid == 0) pdl_launch_dependents();
-  if (tid < kTile) {
-    Token t;
-    t.seq = t.slot = t.page = -1;
-    int s, slot;
-    if (find_row(a.kv, a.seq_len, a.cu_tokens, a.n_tokens, a.err, blockIdx.x * kTile + tid, &s, &slot)) {
-      t.seq = s;
-      t.slot = slot;
-      t.page = q4_page(a.kv, a.err, s, slot >> a.page_shift);
-    }
-    tok[tid] = t;
+  auto source = [&](int head) {
+    return head < H ? reinterpret_cast<const T*>(a.q) + row * a.q_stride + head * D
+           : head < H + K ? reinterpret_cast<const T*>(a.k) + row * a.k_stride + (head - H) * D
+                          : reinterpret_cast<const T*>(a.v) + row * a.v_stride + (head - H - K) * D;
+  };
+  int head = tid / NC;
+  Raw next{};
+  if (head < H + 2 * K) next = load_raw<T, kInterleaved>(source(head), c, R, 8 * c < R && head < H + K);
+  Token t;
+  t.seq = row;
+  const uint32_t len = a.seq_len[row];
+  if (len == 0 || len > q4_capacity(a.kv)) {
+    if (len != 0 && tid == 0) raise_error(a.err, kDevBadArgument);
+    return;
   }
-  __syncthreads();
-  for (int i = tid; i < kTile * (R / 2); i += kThreads) {
-    const int t = i / (R / 2), pair = i - t * (R / 2);
-    if (tok[t].seq < 0) continue;
-    int axis = a.pair_axis ? a.pair_axis[pair] : 0;
-    if (axis >= a.n_axes) {
-      raise_error(a.err, kDevBadArgument);
-      axis = 0;
-    }
-    const int pos = a.positions ? a.positions[axis * a.position_stride + blockIdx.x * kTile + t] : tok[t].slot;
+  t.slot = (int)len - 1;
+  const int entry = a.kv.page_table[(long long)row * a.kv.table_stride + (t.slot >> a.page_shift)];
+  for (int pair = tid; pair < R / 2; pair += kTokenThreads) {
     double sn, cs;
-    sincos((double)pos * (double)a.inv_freq[pair], &sn, &cs);
-    rot[t][pair] = make_double2(cs, sn);
+    sincos((double)position_of(a, pair, row, t.slot) * (double)a.inv_freq[pair], &sn, &cs);
+    rot[rot_at<D, kInterleaved>(pair)] = make_double2(cs, sn);
   }
+  const bool there = entry >= 0 && (uint32_t)entry < a.kv.n_pages;
+  t.block = block_of<D>(a.kv, there ? entry : -1, t.slot);
+  if (!there && tid == 0) raise_error(a.err, kDevBadArgument);
+  if (tid < K) keep_slot(a, t, tid, row);
+  for (int h = tid + kTokenThreads; h < K; h += kTokenThreads) keep_slot(a, t, h, row);
   __syncthreads();
-  const int rows = kTile * (H + 2 * K), c = tid % NC;
-  const int first = tid / NC;
-  for (int base = 0; base < rows; base += kThreads / NC) {   // (the warp's lanes stay together)
-    const int i = base + first, t = min(i / (H + 2 * K), kTile - 1), head = i - t * (H + 2 * K);
-    const bool live = i < rows && tok[t].seq >= 0;
-    const long long row = (long long)blockIdx.x * kTile + t;
-    const bool is_q = head < H, is_k = !is_q && head < H + K;
-    float x[8] = {};
-    if (live) {
-      const T* src = is_q ? reinterpret_cast<const T*>(a.q) + row * a.q_stride + head * D
-                     : is_k ? reinterpret_cast<const T*>(a.k) + row * a.k_stride + (head - H) * D
-                            : reinterpret_cast<const T*>(a.v) + row * a.v_stride + (head - H - K) * D;
-      load8(src + 8 * c, x);
-      if ((is_q || is_k) && 8 * c < R) {
-        float y[8];
-        const bool second = !kInterleaved && 8 * c >= R / 2;
-        const int first_pair = kInterleaved ? 4 * c : 8 * c - (second ? R / 2 : 0);
-        if constexpr (!kInterleaved) load8(src + (second ? 8 * c - R / 2 : 8 * c + R / 2), y);
+  for (int base = 0; base < H + 2 * K; base += kRows, head += kRows) {   // (the warp's lanes stay together)
+    const bool live = head < H + 2 * K, is_q = head < H, is_k = !is_q && head < H + K;
+    const Raw r = next;
+    __syncwarp();   // q_out may be q: every lane has its mates before a row is written
+    if (head + kRows < H + 2 * K)
+      next = load_raw<T, kInterleaved>(source(head + kRows), c, R, 8 * c < R && head + kRows < H + K);
+    float x[8];
+    if ((is_q || is_k) && 8 * c < R) {
+      if (is_q) rotate_raw<float, T, D, kInterleaved>(r, rot, c, R, x);
+      else rotate_raw<double, T, D, kInterleaved>(r, rot, c, R, x);
+      round8<T>(x);
+    } else {
+      unpack8<T>(r.own, x);
+    }
+    if (is_q) *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.q_out) + row * a.q_out_stride + head * D + 8 * c) = pack8<T>(x);
+    if (__any_sync(0xffffffffu, live && !is_q))
+      store_quantised<T, D>(a, x, t, is_k ? head - H : head - H - K, is_k, c, live && !is_q);
+  }
+}
+
+// Ragged tokens.  CTAs 0 .. kv_ctas - 1: keys and values of up to 4 kv heads of 8 tokens, D / 8
+// lanes a row; the rest: 8 query heads of 16 tokens (32 with head_dim 64), a thread 16
+// elements of a token's heads, as in k_append_rows.
+constexpr int kRowThreads = 128, kQHeads = 8, kKvTokens = 8, kKvHeads = 4;
+template <typename T, int D, bool kInterleaved>
+__global__ void __launch_bounds__(kRowThreads, 4) k_append_rows_q4(const __grid_constant__ Q4AppendArgs a, int kv_ctas) {
+  __shared__ double2 rot[kKvTokens][D / 2];   // cos, sin
+  __shared__ Token tok[kKvTokens];
+  const int tid = threadIdx.x, lane = tid & 31, H = a.n_heads, K = a.kv.n_kv_heads, R = a.rot_dim, n_seq = a.kv.n_seq;
+  pdl_wait();
+  if (tid == 0) pdl_launch_dependents();
+  if ((int)blockIdx.x >= kv_ctas) {
+    constexpr int NC = D / 16;
+    const int parts = (H + kQHeads - 1) / kQHeads, cta = (int)blockIdx.x - kv_ctas, tile = cta / parts;
+    const int first = (cta - tile * parts) * kQHeads, count = min(kQHeads, H - first);
+    const int row = tile * (kRowThreads / NC) + tid / NC, c = tid % NC;
+    const bool there = row < a.n_tokens;
+    int pa, pb;
+    places<kInterleaved>(c, R, &pa, &pb);
+    const T* src = reinterpret_cast<const T*>(a.q) + row * a.q_stride + first * D;
+    Chunk x[kQHeads];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const double2 r = rot[t][first_pair + (kInterleaved ? e / 2 : e)];
-          const bool two = kInterleaved ? e & 1 : second;
-          const float mate = kInterleaved ? x[e ^ 1] : y[e];
-          float z;
-          if (is_k) z = (float)(two ? (double)mate * r.y + (double)x[e] * r.x : (double)x[e] * r.x - (double)mate * r.y);
-          else z = two ? mate * (float)r.y + x[e] * (float)r.x : x[e] * (float)r.x - mate * (float)r.y;
-          if constexpr (kInterleaved) {
-            y[e] = z;
-          } else {
-            x[e] = z;
-          }
-        }
-        if constexpr (kInterleaved) {
+    for (int j = 0; j < kQHeads; ++j)
+      if (there && j < count) x[j] = load_chunk(src + j * D + pa, src + j * D + pb);
+    const int s = seq_of<NC>(a.cu_tokens, n_seq, 0, 0, row, lane);
+    int row0, row1, L;
+    if (!there || !rows_of(a.kv, a.seq_len, a.cu_tokens, a.n_tokens, a.err, s, &row0, &row1, &L) || row < row0 || row >= row1)
+      return;
+    T* dst = reinterpret_cast<T*>(a.q_out) + row * a.q_out_stride + first * D;
+    float2 turn[8];
+    const bool turns = 16 * c < R;
+    if (turns) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = y[e];
-        }
-        if (is_k) round8<T>(x);
+      for (int i = 0; i < 8; ++i) {
+        float sn, cs;
+        const double turns = (double)position_of(a, 8 * c + i, row, L - (row1 - row)) * (double)a.inv_freq[8 * c + i] * 0.15915494309189533577;
+        sincospif(2.0f * (float)(turns - rint(turns)), &sn, &cs);
+        turn[i] = make_float2(cs, sn);
       }
     }
-    if (live && is_q) *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.q_out) + row * a.q_out_stride + head * D + 8 * c) = pack8<T>(x);
-    if (!__any_sync(0xffffffffu, live && !is_q)) continue;
-    uint32_t params;
-    const uint32_t codes = quantise_group<T>(x, &params);
-    if (!live || is_q || tok[t].page < 0) continue;
-    const int h = is_k ? head - H : head - H - K, slot = tok[t].slot, in_page = slot & ((int)a.kv.page_size - 1);
-    uint8_t* block = q4_block<D>(a.kv, tok[t].page, h, in_page);
-    const int g = c / 4, r = in_page & 15;
-    *reinterpret_cast<uint32_t*>(block + (is_k ? 0 : Q4Block<D>::kValues) + g * 256 + r * 16 + (c & 3) * 4) = codes;
-    if ((c & 3) == 0)
-      *reinterpret_cast<uint32_t*>(block + (is_k ? Q4Block<D>::kKeySteps : Q4Block<D>::kValueSteps) + g * 64 + r * 4) = params;
-    if (is_k && c == 0) {
-      const long long at = ((long long)tok[t].seq * K + h) * q4_capacity(a.kv) + slot;
-      if (a.kv.weights) a.kv.weights[at] = 0.f;
-      if (a.kv.positions) a.kv.positions[at] = a.positions ? a.positions[row] : slot;
+#pragma unroll
+    for (int j = 0; j < kQHeads; ++j)
+      if (j < count) {
+        if (turns) rotate_chunk<T, kInterleaved>(x[j], turn);
+        store_chunk(dst + j * D + pa, dst + j * D + pb, x[j]);
+      }
+    return;
+  }
+  constexpr int NC = D / 8, kStep = kRowThreads / NC, kAtOnce = 4;   // rows of a thread in flight
+  const int parts = (K + kKvHeads - 1) / kKvHeads, tile = blockIdx.x / parts;
+  const int first = ((int)blockIdx.x - tile * parts) * kKvHeads, heads = min(kKvHeads, K - first);
+  const int c = tid % NC, row0 = tile * kKvTokens, tokens = min(kKvTokens, a.n_tokens - row0);
+  const int rows = tokens * 2 * heads;
+  // Row i is of token i / (2 heads), keys before values, so that a warp's two rows are alike;
+  // a thread's follow one another kStep apart.
+  struct Row {
+    int t, x;
+  };
+  const int per = 2 * heads, add_t = kStep / per, add_x = kStep - add_t * per;
+  auto step = [&](Row& r) {
+    r.t += add_t;
+    r.x += add_x;
+    if (r.x >= per) {
+      r.x -= per;
+      ++r.t;
+    }
+  };
+  auto load = [&](const Row& r) {
+    return r.x >= heads
+               ? load_raw<T, true>(reinterpret_cast<const T*>(a.v) + (row0 + r.t) * a.v_stride + (first + r.x - heads) * D, c, R, false)
+               : load_raw<T, kInterleaved>(reinterpret_cast<const T*>(a.k) + (row0 + r.t) * a.k_stride + (first + r.x) * D, c, R, 8 * c < R);
+  };
+  Row at, ahead;
+  at.t = tid / NC / per;
+  at.x = tid / NC - at.t * per;
+  ahead = at;
+  Raw raw[kAtOnce];
+#pragma unroll
+  for (int j = 0; j < kAtOnce; ++j) {
+    if (ahead.t < tokens) raw[j] = load(ahead);
+    step(ahead);
+  }
+  if (tid < 32) {
+    const int t = lane / (32 / kKvTokens), row = row0 + t;
+    const int s = seq_of<32 / kKvTokens>(a.cu_tokens, n_seq, 0, 0, row, lane);
+    Token x;
+    x.seq = x.slot = -1;
+    x.block = nullptr;
+    int r0, r1, L;
+    if (row < a.n_tokens && lane % (32 / kKvTokens) == 0 &&
+        rows_of(a.kv, a.seq_len, a.cu_tokens, a.n_tokens, a.err, s, &r0, &r1, &L) && row >= r0 && row < r1) {
+      x.seq = s;
+      x.slot = L - (r1 - row);
+      x.block = block_of<D>(a.kv, q4_page(a.kv, a.err, s, x.slot >> a.page_shift), x.slot);
+    }
+    if (lane % (32 / kKvTokens) == 0) tok[t] = x;
+  }
+  __syncthreads();
+  for (int i = tid; i < tokens * (R / 2); i += kRowThreads) {
+    const int t = i / (R / 2), pair = i - t * (R / 2);
+    if (tok[t].seq < 0) continue;
+    double sn, cs;
+    sincos((double)position_of(a, pair, row0 + t, tok[t].slot) * (double)a.inv_freq[pair], &sn, &cs);
+    rot[t][rot_at<D, kInterleaved>(pair)] = make_double2(cs, sn);
+  }
+  for (int i = tid; i < tokens * heads; i += kRowThreads)
+    if (tok[i / heads].seq >= 0) keep_slot(a, tok[i / heads], first + i % heads, row0 + i / heads);
+  __syncthreads();
+#pragma unroll 1
+  for (int base = 0; base < rows; base += kAtOnce * kStep) {   // (the warp's lanes stay together)
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      if (base + j * kStep >= rows) break;
+      const Token& t = tok[min(at.t, tokens - 1)];
+      const bool is_k = at.x < heads, live = at.t < tokens;
+      float x[8];
+      if (is_k && live && t.seq >= 0 && 8 * c < R) {
+        rotate_raw<double, T, D, kInterleaved>(raw[j], rot[at.t], c, R, x);
+        round8<T>(x);
+      } else {
+        unpack8<T>(raw[j].own, x);
+      }
+      if (ahead.t < tokens) raw[j] = load(ahead);
+      step(ahead);
+      store_quantised<T, D>(a, x, t, first + (is_k ? at.x : at.x - heads), is_k, c, live);
+      step(at);
     }
   }
 }
 
 template <typename T, int D, bool kInterleaved>
 int launch(const Q4AppendArgs& a, cudaStream_t st) {
-  if (!a.cu_tokens) k_append_q4<T, D, kInterleaved, 1><<<a.n_tokens, kThreads, 0, st>>>(a);
-  else k_append_q4<T, D, kInterleaved, 8><<<(a.n_tokens + 7) / 8, kThreads, 0, st>>>(a);
-  return 0;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (!a.cu_tokens) {
+    cfg.gridDim = dim3(a.n_tokens);
+    cfg.blockDim = dim3(kTokenThreads);
+    return cudaLaunchKernelEx(&cfg, k_append_token_q4<T, D, kInterleaved>, a) == cudaSuccess ? 0 : -1;
+  }
+  constexpr int kTileRows = kRowThreads / (D / 16);
+  const int q_ctas = (a.n_tokens + kTileRows - 1) / kTileRows * ((a.n_heads + kQHeads - 1) / kQHeads);
+  const int kv_ctas = (a.n_tokens + kKvTokens - 1) / kKvTokens * (((int)a.kv.n_kv_heads + kKvHeads - 1) / kKvHeads);
+  cfg.gridDim = dim3(q_ctas + kv_ctas);
+  cfg.blockDim = dim3(kRowThreads);
+  return cudaLaunchKernelEx(&cfg, k_append_rows_q4<T, D, kInterleaved>, a, kv_ctas) == cudaSuccess ? 0 : -1;
 }
 template <typename T, int D>
 int launch(const Q4AppendArgs& a, cudaStream_t st) {
   return a.interleaved ? launch<T, D, true>(a, st) : launch<T, D, false>(a, st);
 }
 
-// A CTA per row; D / 8 lanes a head's row of k or of v.
+// A CTA per 4 rows; D / 8 lanes a head's row of k or of v.
+constexpr int kExpandRows = 4;
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) k_expand_q4(const __grid_constant__ Q4ExpandArgs a) {
-  constexpr int NC = D / 8;
-  const int row = blockIdx.x, K = a.kv.n_kv_heads, c = threadIdx.x % NC;
-  int s, slot;
-  if (!find_row(a.kv, a.seq_len, a.cu_rows, a.n_rows, a.err, row, &s, &slot)) return;
-  const int page = q4_page(a.kv, a.err, s, slot >> a.page_shift);
-  if (page < 0) return;
-  const int in_page = slot & ((int)a.kv.page_size - 1), g = c / 4, r = in_page & 15;
-  for (int i = threadIdx.x / NC; i < 2 * K; i += kThreads / NC) {
-    const bool is_k = i < K;
-    const int h = is_k ? i : i - K;
-    const uint8_t* block = q4_block<D>(a.kv, page, h, in_page);
-    const uint32_t codes = *reinterpret_cast<const uint32_t*>(block + (is_k ? 0 : Q4Block<D>::kValues) + g * 256 + r * 16 + (c & 3) * 4);
-    const uint32_t params = *reinterpret_cast<const uint32_t*>(block + (is_k ? Q4Block<D>::kKeySteps : Q4Block<D>::kValueSteps) + g * 64 + r * 4);
-    float x[8];
-    expand_word<T>(codes, params, x);
-    T* dst = reinterpret_cast<T*>(is_k ? a.k : a.v) + (long long)row * (is_k ? a.k_stride : a.v_stride) + h * D + 8 * c;
-    *reinterpret_cast<uint4*>(dst) = pack8<T>(x);
+__global__ void __launch_bounds__(kRowThreads) k_expand_q4(const __grid_constant__ Q4ExpandArgs a) {
+  constexpr int NC = D / 8, kStep = kRowThreads / NC, kAtOnce = 8;   // rows of a thread in flight
+  __shared__ const uint8_t* block[kExpandRows];   // of head 0
+  __shared__ int slot_in[kExpandRows];
+  const int tid = threadIdx.x, lane = tid & 31, K = a.kv.n_kv_heads, row0 = blockIdx.x * kExpandRows;
+  pdl_wait();
+  if (tid == 0) pdl_launch_dependents();
+  if (tid < 32) {
+    constexpr int kLanes = 32 / kExpandRows;   // of a row
+    const int t = lane / kLanes, row = row0 + t;
+    int s = row;
+    if (a.cu_rows) s = seq_of<kLanes>(a.cu_rows, a.kv.n_seq, 0, 0, row, lane);
+    if (lane % kLanes == 0) {
+      const uint8_t* at = nullptr;
+      int slot = -1;
+      if (row < a.n_rows) {
+        int r0 = row, r1 = row + 1, L = 0;
+        bool mine;
+        if (a.cu_rows) {
+          mine = rows_of(a.kv, a.seq_len, a.cu_rows, a.n_rows, a.err, s, &r0, &r1, &L) && row >= r0 && row < r1;
+        } else {
+          const uint32_t len = a.seq_len[row];
+          mine = len != 0 && len <= q4_capacity(a.kv);
+          if (len > q4_capacity(a.kv)) raise_error(a.err, kDevBadArgument);
+          L = (int)len;
+        }
+        if (mine) {
+          slot = L - (r1 - row);
+          const int page = q4_page(a.kv, a.err, s, slot >> a.page_shift);
+          slot &= (int)a.kv.page_size - 1;
+          if (page >= 0) at = q4_block<D>(a.kv, page, 0, slot);
+        }
+      }
+      block[t] = at;
+      slot_in[t] = slot & 15;
+    }
   }
+  __syncthreads();
+  const int c = tid % NC, g = c / 4, rows = min(kExpandRows, a.n_rows - row0) * 2 * K;
+#pragma unroll 1
+  for (int base = tid / NC; base < rows; base += kAtOnce * kStep) {
+    uint32_t codes[kAtOnce], params[kAtOnce];
+    T* to[kAtOnce];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      const int i = base + j * kStep, t = min(i / (2 * K), kExpandRows - 1), x = i - t * 2 * K;
+      const bool is_k = x < K;
+      const int h = is_k ? x : x - K;
+      const uint8_t* b = block[t];
+      to[j] = nullptr;
+      if (i >= rows || !b) continue;
+      b += (long long)h * a.kv.head_stride;
+      codes[j] = *reinterpret_cast<const uint32_t*>(b + (is_k ? 0 : Q4Block<D>::kValues) + g * 256 + slot_in[t] * 16 + (c & 3) * 4);
+      params[j] = *reinterpret_cast<const uint32_t*>(b + (is_k ? Q4Block<D>::kKeySteps : Q4Block<D>::kValueSteps) + g * 64 + slot_in[t] * 4);
+      to[j] = reinterpret_cast<T*>(is_k ? a.k : a.v) + (long long)(row0 + t) * (is_k ? a.k_stride : a.v_stride) + h * D + 8 * c;
+    }
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j)
+      if (to[j]) {
+        float x[8];
+        expand_word<T>(codes[j], params[j], x);
+        *reinterpret_cast<uint4*>(to[j]) = pack8<T>(x);
+      }
+  }
+}
+
+template <typename T, int D>
+int launch(const Q4ExpandArgs& a, cudaStream_t st) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((a.n_rows + kExpandRows - 1) / kExpandRows);
+  cfg.blockDim = dim3(kRowThreads);
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, k_expand_q4<T, D>, a) == cudaSuccess ? 0 : -1;
 }
 
 }  // namespace
@@ -210,14 +423,8 @@ int launch_rope_append_q4(const Q4AppendArgs& a, cudaStream_t st) {
 
 int launch_expand_q4(const Q4ExpandArgs& a, cudaStream_t st) {
   const bool d64 = a.kv.head_dim == 64;
-  if (a.kv.dtype == QWEN_DTYPE_F16) {
-    if (d64) k_expand_q4<__half, 64><<<a.n_rows, kThreads, 0, st>>>(a);
-    else k_expand_q4<__half, 128><<<a.n_rows, kThreads, 0, st>>>(a);
-  } else {
-    if (d64) k_expand_q4<__nv_bfloat16, 64><<<a.n_rows, kThreads, 0, st>>>(a);
-    else k_expand_q4<__nv_bfloat16, 128><<<a.n_rows, kThreads, 0, st>>>(a);
-  }
-  return 0;
+  if (a.kv.dtype == QWEN_DTYPE_F16) return d64 ? launch<__half, 64>(a, st) : launch<__half, 128>(a, st);
+  return d64 ? launch<__nv_bfloat16, 64>(a, st) : launch<__nv_bfloat16, 128>(a, st);
 }
 
 }  // namespace qwen

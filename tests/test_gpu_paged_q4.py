@@ -550,6 +550,7 @@ def test_pages_outside_the_pool():
         others = [t for t in range(c.n_pages) if t not in own]
         assert torch.equal(c.pool[others], pool[others])
         c.pool.copy_(pool)
+        c.weights[0, :, 36:40] = -1.0   # of that page: to be filled from behind
         ops.evict_paged_q4(kv, ints(100, 40), 40, 0, 0)   # (the other sequence has no more)
         reported("out-of-range")
         assert torch.equal(c.pool[others], pool[others])
