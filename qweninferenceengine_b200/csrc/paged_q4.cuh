@@ -102,12 +102,36 @@ __device__ __forceinline__ uint32_t quantise_group(const float (&x)[8], uint32_t
   return __byte_perm(__float_as_uint(a + 8388608.f), __float_as_uint(b + 8388608.f), 0x5410);
 }
 
-// Values low + code step of 8 codes, rounded to fp32.
-template <typename T>
-__device__ __forceinline__ void expand_word(uint32_t codes, uint32_t params, float (&x)[8]) {
-  const float2 p = unpack2(T{}, params);
+// Values low + code step of 8 codes in the cache's type, rounded once.  (1024 + code in fp16
+// and 128 + code in bf16 are codes at the bottom of the mantissa.)
+__device__ __forceinline__ uint4 expand_word(__half, uint32_t codes, uint32_t params) {
+  const __half2 p = *reinterpret_cast<const __half2*>(&params), step = __low2half2(p), low = __high2half2(p);
+  const __half2 k1024 = __float2half2_rn(1024.f), k64 = __float2half2_rn(64.f), k16th = __float2half2_rn(0.0625f);
+  const uint32_t v = codes >> 8;
+  uint32_t y[4];   // elements (0, 4), (1, 5), (2, 6), (3, 7)
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = fmaf((float)(codes >> (4 * i) & 15), p.x, p.y);
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = lop3_and_or(i < 2 ? codes : v, i & 1 ? 0x00f000f0u : 0x000f000fu, 0x64006400u);
+    const __half2 h = *reinterpret_cast<const __half2*>(&w);
+    const __half2 c = i & 1 ? __hfma2(h, k16th, __hneg2(k64)) : __hsub2(h, k1024);   // (1024 + 16 code) / 16 - 64
+    const __half2 r = __hfma2(c, step, low);
+    y[i] = *reinterpret_cast<const uint32_t*>(&r);
+  }
+  return make_uint4(__byte_perm(y[0], y[1], 0x5410), __byte_perm(y[2], y[3], 0x5410), __byte_perm(y[0], y[1], 0x7632),
+                    __byte_perm(y[2], y[3], 0x7632));
+}
+__device__ __forceinline__ uint4 expand_word(__nv_bfloat16, uint32_t codes, uint32_t params) {
+  const __nv_bfloat162 p = *reinterpret_cast<const __nv_bfloat162*>(&params), step = __low2bfloat162(p), low = __high2bfloat162(p);
+  const __nv_bfloat162 k128 = __float2bfloat162_rn(128.f);
+  uint32_t y[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = lop3_and_or(codes >> (4 * i), 0x000f000fu, 0x43004300u);
+    const __nv_bfloat162 r = __hfma2(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&w), k128), step, low);
+    y[i] = *reinterpret_cast<const uint32_t*>(&r);
+  }
+  return make_uint4(__byte_perm(y[0], y[1], 0x5410), __byte_perm(y[2], y[3], 0x5410), __byte_perm(y[0], y[1], 0x7632),
+                    __byte_perm(y[2], y[3], 0x7632));
 }
 
 }  // namespace qwen

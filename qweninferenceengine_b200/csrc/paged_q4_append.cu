@@ -1,5 +1,7 @@
 // paged_q4_append.cu -- rotation of new queries and keys at given positions, the keys'
 // and values' way into a 4-bit paged cache, and its rows' way back into 16 bits.
+#include <algorithm>
+
 #include "paged_q4.cuh"
 #include "paged_rotate.cuh"
 #include "qwen_internal.h"
@@ -330,72 +332,92 @@ int launch(const Q4AppendArgs& a, cudaStream_t st) {
   return a.interleaved ? launch<T, D, true>(a, st) : launch<T, D, false>(a, st);
 }
 
-// A CTA per 4 rows; D / 8 lanes a head's row of k or of v.
-constexpr int kExpandRows = 4;
+// Rows back in 16 bits.  Bound: HBM, 160 B in and 512 out a row of K and V of 128.  A CTA has a
+// run of rows, up to 64 of which it looks up at once, each in a thread (a lookup is a chain
+// of four round trips: with 8 rows a CTA its warps spent most of their time behind it); then
+// D / 8 lanes take a head's row of k or of v.
+constexpr int kExpandRows = 64, kExpandThreads = 256, kExpandCtasPerSm = 8, kExpandLeast = 4;
 template <typename T, int D>
-__global__ void __launch_bounds__(kRowThreads) k_expand_q4(const __grid_constant__ Q4ExpandArgs a) {
-  constexpr int NC = D / 8, kStep = kRowThreads / NC, kAtOnce = 8;   // rows of a thread in flight
-  __shared__ const uint8_t* block[kExpandRows];   // of head 0
-  __shared__ int slot_in[kExpandRows];
-  const int tid = threadIdx.x, lane = tid & 31, K = a.kv.n_kv_heads, row0 = blockIdx.x * kExpandRows;
+__global__ void __launch_bounds__(kExpandThreads, kExpandCtasPerSm) k_expand_q4(const __grid_constant__ Q4ExpandArgs a) {
+  constexpr int NC = D / 8, kStep = kExpandThreads / NC, kAtOnce = 4;   // rows of a thread in flight
+  struct Row {
+    const uint8_t *codes, *params;   // of head 0; null: no one's row
+  };
+  __shared__ Row row_at[kExpandRows];
+  const int tid = threadIdx.x, K = a.kv.n_kv_heads, n_seq = a.kv.n_seq;
+  const int begin = (int)((long long)a.n_rows * blockIdx.x / gridDim.x);
+  const int end = (int)((long long)a.n_rows * (blockIdx.x + 1) / gridDim.x);
   pdl_wait();
   if (tid == 0) pdl_launch_dependents();
-  if (tid < 32) {
-    constexpr int kLanes = 32 / kExpandRows;   // of a row
-    const int t = lane / kLanes, row = row0 + t;
-    int s = row;
-    if (a.cu_rows) s = seq_of<kLanes>(a.cu_rows, a.kv.n_seq, 0, 0, row, lane);
-    if (lane % kLanes == 0) {
-      const uint8_t* at = nullptr;
-      int slot = -1;
-      if (row < a.n_rows) {
-        int r0 = row, r1 = row + 1, L = 0;
-        bool mine;
-        if (a.cu_rows) {
-          mine = rows_of(a.kv, a.seq_len, a.cu_rows, a.n_rows, a.err, s, &r0, &r1, &L) && row >= r0 && row < r1;
-        } else {
-          const uint32_t len = a.seq_len[row];
-          mine = len != 0 && len <= q4_capacity(a.kv);
-          if (len > q4_capacity(a.kv)) raise_error(a.err, kDevBadArgument);
-          L = (int)len;
-        }
-        if (mine) {
-          slot = L - (r1 - row);
-          const int page = q4_page(a.kv, a.err, s, slot >> a.page_shift);
-          slot &= (int)a.kv.page_size - 1;
-          if (page >= 0) at = q4_block<D>(a.kv, page, 0, slot);
-        }
-      }
-      block[t] = at;
-      slot_in[t] = slot & 15;
-    }
-  }
-  __syncthreads();
-  const int c = tid % NC, g = c / 4, rows = min(kExpandRows, a.n_rows - row0) * 2 * K;
+  int s0 = 0;   // sequence of the first row
+  if (a.cu_rows)
+    for (int base = 0; base < n_seq - 1; base += kExpandThreads)
+      s0 += __syncthreads_count(base + tid < n_seq - 1 && a.cu_rows[base + tid + 1] <= begin);
+  const int c = tid % NC, per = 2 * K, add_t = kStep / per, add_x = kStep - add_t * per;
+  const int first_t = tid / NC / per, first_x = tid / NC - first_t * per;
 #pragma unroll 1
-  for (int base = tid / NC; base < rows; base += kAtOnce * kStep) {
-    uint32_t codes[kAtOnce], params[kAtOnce];
-    T* to[kAtOnce];
-#pragma unroll
-    for (int j = 0; j < kAtOnce; ++j) {
-      const int i = base + j * kStep, t = min(i / (2 * K), kExpandRows - 1), x = i - t * 2 * K;
-      const bool is_k = x < K;
-      const int h = is_k ? x : x - K;
-      const uint8_t* b = block[t];
-      to[j] = nullptr;
-      if (i >= rows || !b) continue;
-      b += (long long)h * a.kv.head_stride;
-      codes[j] = *reinterpret_cast<const uint32_t*>(b + (is_k ? 0 : Q4Block<D>::kValues) + g * 256 + slot_in[t] * 16 + (c & 3) * 4);
-      params[j] = *reinterpret_cast<const uint32_t*>(b + (is_k ? Q4Block<D>::kKeySteps : Q4Block<D>::kValueSteps) + g * 64 + slot_in[t] * 4);
-      to[j] = reinterpret_cast<T*>(is_k ? a.k : a.v) + (long long)(row0 + t) * (is_k ? a.k_stride : a.v_stride) + h * D + 8 * c;
-    }
-#pragma unroll
-    for (int j = 0; j < kAtOnce; ++j)
-      if (to[j]) {
-        float x[8];
-        expand_word<T>(codes[j], params[j], x);
-        *reinterpret_cast<uint4*>(to[j]) = pack8<T>(x);
+  for (int row0 = begin; row0 < end; row0 += kExpandRows) {
+    const int tokens = min(kExpandRows, end - row0);
+    if (tid < tokens) {
+      const int row = row0 + tid;
+      int r0 = row, r1 = row + 1, L = 0, s = row;
+      bool mine;
+      if (a.cu_rows) {
+        int hi = n_seq - 1;   // the first s with cu[s + 1] > row
+        s = s0;
+        if (s < hi && a.cu_rows[s + 1] > row) hi = s;
+        while (s < hi) {
+          const int mid = (s + hi) >> 1;
+          if (a.cu_rows[mid + 1] > row) hi = mid;
+          else s = mid + 1;
+        }
+        mine = rows_of(a.kv, a.seq_len, a.cu_rows, a.n_rows, a.err, s, &r0, &r1, &L) && row >= r0 && row < r1;
+      } else {
+        const uint32_t len = a.seq_len[row];
+        mine = len != 0 && len <= q4_capacity(a.kv);
+        if (len > q4_capacity(a.kv)) raise_error(a.err, kDevBadArgument);
+        L = (int)len;
       }
+      Row at = {nullptr, nullptr};
+      if (mine) {
+        const int slot = L - (r1 - row), page = q4_page(a.kv, a.err, s, slot >> a.page_shift);
+        if (page >= 0) {
+          const uint8_t* block = block_of<D>(a.kv, page, slot);
+          at.codes = block + (slot & 15) * 16;
+          at.params = block + Q4Block<D>::kKeySteps + (slot & 15) * 4;
+        }
+      }
+      row_at[tid] = at;
+    }
+    __syncthreads();
+    int t = first_t, x = first_x;   // row of the tile, key (x < K) or value of a head
+#pragma unroll 1
+    while (t < tokens) {
+      uint32_t codes[kAtOnce], params[kAtOnce];
+      T* to[kAtOnce];
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        to[j] = nullptr;
+        if (t < tokens && row_at[t].codes) {
+          const bool is_k = x < K;
+          const int h = is_k ? x : x - K;
+          const long long off = (long long)h * a.kv.head_stride + (c / 4) * 64;
+          codes[j] = __ldg(reinterpret_cast<const uint32_t*>(row_at[t].codes + off + (is_k ? 0 : Q4Block<D>::kValues) + (c / 4) * 192 + (c & 3) * 4));
+          params[j] = __ldg(reinterpret_cast<const uint32_t*>(row_at[t].params + off + (is_k ? 0 : Q4Block<D>::kValueSteps - Q4Block<D>::kKeySteps)));
+          to[j] = reinterpret_cast<T*>(is_k ? a.k : a.v) + (long long)(row0 + t) * (is_k ? a.k_stride : a.v_stride) + h * D + 8 * c;
+        }
+        t += add_t;
+        x += add_x;
+        if (x >= per) {
+          x -= per;
+          ++t;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j)
+        if (to[j]) *reinterpret_cast<uint4*>(to[j]) = expand_word(T{}, codes[j], params[j]);
+    }
+    __syncthreads();
   }
 }
 
@@ -405,8 +427,8 @@ int launch(const Q4ExpandArgs& a, cudaStream_t st) {
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((a.n_rows + kExpandRows - 1) / kExpandRows);
-  cfg.blockDim = dim3(kRowThreads);
+  cfg.gridDim = dim3(std::min((a.n_rows + kExpandLeast - 1) / kExpandLeast, kExpandCtasPerSm * paged_sm_count()));
+  cfg.blockDim = dim3(kExpandThreads);
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
