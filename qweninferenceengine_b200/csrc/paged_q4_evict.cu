@@ -1,23 +1,27 @@
 // paged_q4_evict.cu -- cuts the sequences of a 4-bit paged cache to a budget: of each
 // (sequence, kv head) the n_keep slots stay that come first by (guarded, weight, slot).
 //
-// Two launches.  k_evict_select, a CTA per (sequence, kv head): weights and positions are
-// read once into registers (up to 32 slots a thread; longer rows are read again from L2), the
-// n_keep-th weight is found digit by digit (11, 11 and 10 bits of an order-preserving key, a
-// histogram in shared memory each), and the slots that go and those that come are numbered
-// in slot order.  k_evict_move copies the rows, as many CTAs as fill the GPU.  Nothing a row
+// Two launches.  k_evict_select, a CTA or a cluster per (sequence, kv head): weights and positions are
+// read into shared memory as ordered keys (up to 16384 slots a CTA; longer rows are read again
+// from L2), the n_keep-th weight is found digit by digit (11, 11 and 10 bits, a histogram in
+// shared memory each), and the slots that go and those that come are numbered in slot order.
+// Few long rows are divided among the CTAs of a cluster, which add up their histograms.  k_evict_move copies the rows, as many CTAs as fill the GPU.  Nothing a row
 // is copied from is written, so the copies need no order, and what stays below n_keep is not
 // touched: a sequence one token over its budget moves one row.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <climits>
 
 #include "paged_q4.cuh"
 #include "qwen_internal.h"
 
+namespace cg = cooperative_groups;
+
 namespace qwen {
 namespace {
 
-constexpr int kThreads = 1024, kWarps = kThreads / 32, kBins = 2048;
+constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 2048;
 
 // A weight as a number that grows with it: NaN greatest, -0 like 0.
 __device__ __forceinline__ uint32_t weight_key(float w) {
@@ -42,19 +46,31 @@ __host__ __device__ inline Moves moves_of(const Q4EvictArgs& a) {
   return m;
 }
 
-constexpr int kTileSteps = 32, kTile = kTileSteps * kThreads;   // slots numbered at once
+constexpr int kMaxHeld = 16384;              // slots whose keys a CTA holds in shared memory at most
+constexpr int kTile = 32 * kThreads;         // slots numbered at once: a word of bits a thread
+constexpr int kMaxCluster = 8;
 
-struct SelectSmem {
-  int bins[kBins];
-  uint32_t words[kTile / 32];   // a bit a slot
-  int before[kTile / 32];       // bits set in the words before
+// Bits of a tile's slots, and how many are set in the words before.
+struct Bits {
+  uint32_t words[kTile / 32];
+  int before[kTile / 32];
+  __device__ __forceinline__ int rank_of(int i) const {   // (of slot i, in the tile)
+    return before[i / 32] + __popc(words[i / 32] & ((1u << (i & 31)) - 1));
+  }
+};
+struct __align__(16) SelectSmem {
+  int bins[3][kBins];   // a histogram for each digit
+  int all[3][kBins];    // the cluster's, in its first CTA
+  Bits equal, stay;
   int sums[2][kWarps];
   int digit, left, in_bin;
+  int newest, guarded, n_equal, kept, kept_below;   // of this CTA's slots, for the cluster
+  uint32_t keys[1];   // as many as the launch has room for
 };
 
 // Sum of x over the CTA, and (before) over the threads before this one.  `turn` alternates
 // from call to call, so that one barrier is enough.
-__device__ __forceinline__ int block_sum(int x, SelectSmem& s, int turn, int* before = nullptr) {
+__device__ __noinline__ int block_sum(int x, int (&sums)[2][kWarps], int turn, int* before) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int inc = x;
 #pragma unroll
@@ -62,115 +78,130 @@ __device__ __forceinline__ int block_sum(int x, SelectSmem& s, int turn, int* be
     const int v = __shfl_up_sync(0xffffffffu, inc, o);
     if (lane >= o) inc += v;
   }
-  if (lane == 31) s.sums[turn & 1][warp] = inc;
+  if (lane == 31) sums[turn & 1][warp] = inc;
   __syncthreads();
-  int all = s.sums[turn & 1][lane];
-  if (before) *before = inc - x + __reduce_add_sync(0xffffffffu, lane < warp ? all : 0);
+  const int all = lane < kWarps ? sums[turn & 1][lane] : 0;
+  *before = inc - x + __reduce_add_sync(0xffffffffu, lane < warp ? all : 0);
   return __reduce_add_sync(0xffffffffu, all);
 }
 
-// One (sequence, kv head).  kE: slots a thread keeps in registers, slot e * kThreads + tid; 0:
-// any number, read again each time.
-template <int kE>
-struct Row {
-  const float* weights;
-  const int32_t* positions;
-  int L, n_first;
-  long long recent;
-  uint32_t keys[kE ? kE : 1];
-  uint32_t guards[kE ? (kE + 31) / 32 : 1];
-
-  __device__ __forceinline__ int steps() const { return kE ? kE : (L + kThreads - 1) / kThreads; }
-  __device__ __forceinline__ bool guarded(int e) const {
-    if constexpr (kE != 0) {
-      return guards[e / 32] >> (e % 32) & 1;
-    } else {
-      const int p = positions[e * kThreads + threadIdx.x];
-      return p < n_first || (long long)p > recent;
-    }
-  }
-  __device__ __forceinline__ uint32_t key(int e) const {
-    if constexpr (kE != 0) return keys[e];
-    else return weight_key(weights[e * kThreads + threadIdx.x]);
-  }
-  __device__ __forceinline__ bool there(int e) const { return e * kThreads + (int)threadIdx.x < L; }
-};
-
-template <int kE>
-__device__ __forceinline__ void select_row(const Q4EvictArgs& a, int unit, int L, SelectSmem& s) {
+// One (sequence, kv head) by the CTAs of a cluster, or by one.  Latency throughout: for two
+// rows of 32768 slots over eight CTAs each 14 us, of which the six cluster barriers take half;
+// for rows of 1060 slots 5 us.  Loops are rolled, with their loads in flight together: code that
+// runs once is waited for line by line.
+__device__ __forceinline__ void select_row(const Q4EvictArgs& a, int unit, int first, int n, int room, bool wide, SelectSmem& s) {
+  cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const uint32_t capacity = q4_capacity(a.kv);
-  Row<kE> row;
-  row.weights = a.kv.weights + (long long)unit * capacity;
-  row.positions = a.kv.positions + (long long)unit * capacity;
-  row.L = L;
-  row.n_first = a.n_first;
-  int turn = 0;
-  // ---- the newest position, and how many are guarded
-  constexpr bool kHold = kE != 0 && kE <= 8;   // positions in registers (more would not fit: read again)
-  int newest = INT_MIN, pos[kHold ? kE : 1];
-  if constexpr (kE != 0) {
+  const int me = wide ? (int)cluster.block_rank() : 0, ctas = wide ? (int)cluster.num_blocks() : 1;
+  // Lane i's: what CTA i left in x (`none` beyond the last).
+  auto of_cluster = [&](int* x, int none) { return lane >= ctas ? none : wide ? *cluster.map_shared_rank(x, lane) : *x; };
+  auto sum_of = [&](int* x, int upto) { return __reduce_add_sync(0xffffffffu, lane < upto ? of_cluster(x, 0) : 0); };
+  const long long at = (long long)unit * q4_capacity(a.kv) + first;
+  const float* weights = a.kv.weights + at;
+  const int32_t* positions = a.kv.positions + at;
+  const bool held = n <= room;
+  int turn = 0, before;
+  // ---- keys, and the newest position.  NaN is the greatest weight: 0xfffffffe.
+  auto raw_key = [&](int i) { return min(weight_key(__ldg(weights + i)), 0xfffffffeu); };
+  int newest = INT_MIN;
+  constexpr int kAtOnce = 8;   // loads in flight
+  for (int i0 = tid; i0 < n; i0 += kAtOnce * kThreads) {
+    int p[kAtOnce];
+    float w[kAtOnce];
 #pragma unroll
-    for (int e = 0; e < kE; ++e) {
-      const int p = row.there(e) ? row.positions[e * kThreads + tid] : INT_MIN;
-      if constexpr (kHold) pos[e] = p;
-      newest = max(newest, p);
+    for (int j = 0; j < kAtOnce; ++j) {
+      const int i = i0 + j * kThreads;
+      p[j] = i < n ? __ldg(positions + i) : INT_MIN;
+      w[j] = i < n ? __ldg(weights + i) : 0.f;
     }
 #pragma unroll
-    for (int e = 0; e < kE; ++e) row.keys[e] = row.there(e) ? __float_as_uint(row.weights[e * kThreads + tid]) : 0;
-  } else {
-    for (int i = tid; i < L; i += kThreads) newest = max(newest, row.positions[i]);
+    for (int j = 0; j < kAtOnce; ++j) {
+      newest = max(newest, p[j]);
+      if (held && i0 + j * kThreads < n) s.keys[i0 + j * kThreads] = min(weight_key(w[j]), 0xfffffffeu);
+    }
   }
   newest = __reduce_max_sync(0xffffffffu, newest);
   if (lane == 0) s.sums[1][warp] = newest;
-  for (int i = tid; i < kBins; i += kThreads) s.bins[i] = 0;
+  for (int i = tid; i < 2 * 3 * kBins / 4; i += kThreads) reinterpret_cast<int4*>(s.bins[0])[i] = make_int4(0, 0, 0, 0);
   __syncthreads();
-  newest = __reduce_max_sync(0xffffffffu, s.sums[1][lane]);
-  row.recent = (long long)newest - a.n_recent;
-  int n = 0;
-  if constexpr (kE != 0) {
-#pragma unroll
-    for (int i = 0; i < (kE + 31) / 32; ++i) row.guards[i] = 0;
-#pragma unroll
-    for (int e = 0; e < kE; ++e) {
-      row.keys[e] = weight_key(__uint_as_float(row.keys[e]));
-      int p = 0;
-      if constexpr (kHold) p = pos[e];
-      else if (row.there(e)) p = row.positions[e * kThreads + tid];
-      const bool g = row.there(e) && (p < a.n_first || (long long)p > row.recent);
-      row.guards[e / 32] |= (uint32_t)g << (e % 32);
-      n += g;
-    }
-  } else {
-    for (int e = 0; row.there(e); ++e) n += row.guarded(e);
+  newest = __reduce_max_sync(0xffffffffu, s.sums[1][lane % kWarps]);
+  if (wide) {
+    if (tid == 0) s.newest = newest;
+    cluster.sync();
+    newest = __reduce_max_sync(0xffffffffu, of_cluster(&s.newest, INT_MIN));
   }
-  const int n_guarded = block_sum(n, s, turn++);
-  // ---- of the class that is cut (the guarded, if there are more than n_keep, else the
-  // others) the rank-th greatest key; of those equal to it, the first `rank` slots stay
-  const bool cut = n_guarded > a.n_keep;
-  int rank = cut ? a.n_keep : a.n_keep - n_guarded, equal = 0;
-  uint32_t key = 0xffffffffu, mask = 0xffffffffu;   // rank 0: none of the others stays
+  const long long recent = (long long)newest - a.n_recent;
+  // ---- how many are guarded; their key is all ones
+  auto guards = [&](int p) { return p < a.n_first || (long long)p > recent; };
+  auto guarded = [&](int i) { return guards(__ldg(positions + i)); };
+  int count = 0;
+  for (int i0 = tid; i0 < n; i0 += kAtOnce * kThreads) {
+    int p[kAtOnce];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) p[j] = __ldg(positions + min(i0 + j * kThreads, n - 1));
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      const bool g = i0 + j * kThreads < n && guards(p[j]);
+      count += g;
+      if (held && g) s.keys[i0 + j * kThreads] = 0xffffffffu;
+    }
+  }
+  count = block_sum(count, s.sums, turn++, &before);
+  if (wide) {
+    if (tid == 0) s.guarded = count;
+    cluster.sync();
+    count = sum_of(&s.guarded, ctas);
+  }
+  // Of the class that is cut (the guarded, if there are more than n_keep, else the others) the
+  // rank-th greatest key is looked for; `pass_over` is the key of the other class.
+  const bool cut = count > a.n_keep;
+  const uint32_t pass_over = cut ? 0 : 0xffffffffu;
+  if (cut && held) {
+    for (int i = tid; i < n; i += kThreads) s.keys[i] = s.keys[i] == 0xffffffffu ? raw_key(i) : 0;
+    __syncthreads();
+  }
+  auto key_of = [&](int i) { return held ? s.keys[i] : guarded(i) == cut ? raw_key(i) : pass_over; };
+  int rank = cut ? a.n_keep : a.n_keep - count, equal = 0;
+  uint32_t key = 0xffffffffu, mask = 0xffffffffu;   // rank 0: the guarded alone stay
   if (rank > 0) {
     key = mask = 0;
 #pragma unroll 1
-    for (int shift = 21; shift >= 0; shift = shift == 21 ? 10 : shift - 10) {
-      const uint32_t digits = shift == 0 ? 1023 : 2047;
-#pragma unroll
-      for (int e = 0; e < row.steps(); ++e)
-        if (row.there(e) && row.guarded(e) == cut && (row.key(e) & mask) == key)
-          atomicAdd(&s.bins[row.key(e) >> shift & digits], 1);
-      __syncthreads();
-      // thread i has bins 2047 - 2i and 2046 - 2i: the greatest first
-      const int b0 = s.bins[kBins - 1 - 2 * tid], b1 = s.bins[kBins - 2 - 2 * tid];
-      int before;
-      block_sum(b0 + b1, s, turn++, &before);
-      if (before < rank && before + b0 + b1 >= rank) {
-        const bool second = before + b0 < rank;
-        s.digit = kBins - 1 - 2 * tid - second;
-        s.left = rank - before - (second ? b0 : 0);
-        s.in_bin = second ? b1 : b0;
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+      const uint32_t digits = pass == 2 ? 1023 : 2047;
+      int* bins = s.bins[pass];
+#pragma unroll 4
+      for (int i = tid; i < n; i += kThreads) {
+        const uint32_t k = key_of(i);
+        if (k != pass_over && (k & mask) == key) atomicAdd(&bins[k >> shift & digits], 1);
       }
-      s.bins[kBins - 1 - 2 * tid] = s.bins[kBins - 2 - 2 * tid] = 0;
+      __syncthreads();
+      // thread i has bins 2044 - 4i .. 2047 - 4i, the greatest first; the first CTA adds up all's
+      int4 b = *reinterpret_cast<const int4*>(bins + kBins - 4 - 4 * tid);
+      if (wide) {
+        int* to = cluster.map_shared_rank(s.all[pass], 0) + kBins - 4 - 4 * tid;
+        if (b.x) atomicAdd(to, b.x);
+        if (b.y) atomicAdd(to + 1, b.y);
+        if (b.z) atomicAdd(to + 2, b.z);
+        if (b.w) atomicAdd(to + 3, b.w);
+        cluster.sync();
+        b = *reinterpret_cast<const int4*>(to);
+      }
+      const int here = b.x + b.y + b.z + b.w;
+      block_sum(here, s.sums, turn++, &before);
+      if (before < rank && before + here >= rank) {
+        const int in[4] = {b.w, b.z, b.y, b.x};
+        int left = rank - before, j = 0;
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+          if (j == i && left > in[i]) {
+            left -= in[i];
+            ++j;
+          }
+        s.digit = kBins - 1 - 4 * tid - j;
+        s.left = left;
+        s.in_bin = in[j];
+      }
       __syncthreads();
       key |= (uint32_t)s.digit << shift;
       mask |= digits << shift;
@@ -179,94 +210,99 @@ __device__ __forceinline__ void select_row(const Q4EvictArgs& a, int unit, int L
       if (equal == rank) break;   // all that begin like this stay
     }
   }
-  // ---- which stay, and in slot order the holes below n_keep and what comes into them
-  int2* pairs = moves_of(a).pairs + (long long)unit * a.n_keep;
-  // Numbers the set bits of a tile: s.before[] for s.words[], after `seen` before the tile.
-  auto number = [&](int& seen) {
+  // ---- which stay: keys above, and of those equal to it (but the other class) the first `rank`
+  const bool ties = equal > rank, some = rank > 0;
+  auto same = [&](uint32_t k) { return some && k != pass_over && (k & mask) == key; };
+  // Marks and numbers a tile's bits, after `seen`.
+  auto number = [&](Bits& b, int base, int& seen, auto&& bit) {
+    const int words = min(kTile, n - base + 31) / 32;
+#pragma unroll 2
+    for (int w = warp; w < words; w += kWarps) {
+      const int i = base + 32 * w + lane;
+      const uint32_t x = __ballot_sync(0xffffffffu, i < n && bit(i));
+      if (lane == 0) b.words[w] = x;
+    }
     __syncthreads();
-    const uint32_t w = s.words[tid];
-    int before;
-    const int total = block_sum(__popc(w), s, turn++, &before);
-    s.before[tid] = seen + before;
+    const int total = block_sum(tid < words ? __popc(b.words[tid]) : 0, s.sums, turn++, &before);
+    b.before[tid] = seen + before;
     seen += total;
     __syncthreads();
   };
-  s.words[tid] = 0;   // (of steps that the row does not have)
-  __syncthreads();
-  const uint32_t below = (1u << lane) - 1;
-  auto rank_of = [&](int e) { return s.before[e * kWarps + warp] + __popc(s.words[e * kWarps + warp] & below); };
-  int seen = 0, kept = 0, kept_below = 0;   // equal ones, those that stay, and of them below n_keep
-#pragma unroll 1
-  for (int base = 0; base < L; base += kTile) {
-    const int e_base = base / kThreads;   // (0 where registers hold the row)
-    uint32_t stays = 0;                   // bit e: this thread's slot of step e
-    auto each = [&](auto&& f) {   // f(step of the tile, step of the row)
-      if constexpr (kE != 0) {
-#pragma unroll
-        for (int e = 0; e < kE; ++e) f(e, e);
-      } else {
-#pragma unroll 1
-        for (int e = 0; e < kTileSteps; ++e) f(e, e_base + e);
-      }
-    };
-    auto same_as_key = [&](int row_e) {
-      return row.there(row_e) && row.guarded(row_e) == cut && (row.key(row_e) & mask) == key;
-    };
-    if (equal > rank) {   // ties: of those the first stay
-      each([&](int e, int row_e) {
-        const uint32_t w = __ballot_sync(0xffffffffu, same_as_key(row_e));
-        if (lane == 0) s.words[e * kWarps + warp] = w;
-      });
-      number(seen);
-      each([&](int e, int row_e) { stays |= (uint32_t)(same_as_key(row_e) && rank_of(e) < rank) << e; });
-      __syncthreads();
-    } else if (rank > 0) {
-      each([&](int e, int row_e) { stays |= (uint32_t)same_as_key(row_e) << e; });
-    }
-    each([&](int e, int row_e) {
-      const bool in = row.there(row_e);
-      stays |= (uint32_t)(in && (row.guarded(row_e) == cut ? (row.key(row_e) & mask) > key : !cut)) << e;
-      const uint32_t w = __ballot_sync(0xffffffffu, stays >> e & 1);
-      if (lane == 0) s.words[e * kWarps + warp] = w;
+  int equal_before = 0;   // of the CTAs before
+  if (ties && wide) {
+    int mine = 0;
+    for (int i = tid; i < n; i += kThreads) mine += same(key_of(i));
+    mine = block_sum(mine, s.sums, turn++, &before);
+    if (tid == 0) s.n_equal = mine;
+    cluster.sync();
+    equal_before = sum_of(&s.n_equal, me);
+  }
+  int seen = equal_before, kept = 0, kept_below = 0;   // of this CTA: that stay, of them below n_keep
+  auto decide = [&](int base) {
+    if (ties) number(s.equal, base, seen, [&](int i) { return same(key_of(i)); });
+    number(s.stay, base, kept, [&](int i) {
+      const uint32_t k = key_of(i);
+      return same(k) ? !ties || s.equal.rank_of(i - base) < rank
+                     : k == pass_over ? !cut : (k & mask) > key;
     });
-    number(kept);
-    if (base <= a.n_keep && a.n_keep < base + kTile) {
-      const int i = a.n_keep - base;   // slots that stay before slot n_keep
-      kept_below = s.before[i / 32] + __popc(s.words[i / 32] & ((1u << (i % 32)) - 1));
+    const int i = a.n_keep - first - base;   // (of this tile, or the last before n_keep)
+    if (i > 0) kept_below = i >= min(kTile, n - base) ? kept : s.stay.rank_of(i);
+  };
+#pragma unroll 1
+  for (int base = 0; base < n; base += kTile) decide(base);
+  int offset = 0;   // that stay in the CTAs before
+  if (wide) {
+    if (tid == 0) {
+      s.kept = kept;
+      s.kept_below = kept_below;
     }
-    each([&](int e, int row_e) {
-      const int i = row_e * kThreads + tid, r = rank_of(e);
-      const bool stay = stays >> e & 1;
-      if (i < a.n_keep ? !stay : stay) {   // (i < L: n_keep is less)
-        if (stay) pairs[r - kept_below].y = i;
-        else pairs[i - r].x = i;
-      }
-    });
+    cluster.sync();
+    kept_below = sum_of(&s.kept_below, ctas);
+    offset = sum_of(&s.kept, me);
+  }
+  // ---- in slot order the holes below n_keep and what comes into them
+  int2* pairs = moves_of(a).pairs + (long long)unit * a.n_keep;
+  const int below = kept_below;
+  seen = equal_before;
+  kept = 0;
+#pragma unroll 1
+  for (int base = 0; base < n; base += kTile) {
+    if (n > kTile) decide(base);   // (else it stands there)
+    const int end = min(kTile, n - base);
+    for (int i = tid; i < end; i += kThreads) {
+      const int slot = first + base + i;
+      const bool stays = s.stay.words[i / 32] >> (i & 31) & 1;
+      if (slot < a.n_keep ? stays : !stays) continue;
+      const int r = offset + s.stay.rank_of(i);   // that stay before it
+      if (stays) pairs[r - below].y = slot;
+      else pairs[slot - r].x = slot;
+    }
     __syncthreads();
   }
-  if (tid == 0) moves_of(a).count[unit] = a.n_keep - kept_below;
+  if (tid == 0 && me == 0) moves_of(a).count[unit] = a.n_keep - below;
+  if (wide) cluster.sync();   // what others may still read is there until then
 }
 
-__global__ void __launch_bounds__(kThreads) k_evict_select(const __grid_constant__ Q4EvictArgs a) {
-  __shared__ SelectSmem s;
-  const int K = a.kv.n_kv_heads, unit = blockIdx.x, seq = unit / K, tid = threadIdx.x;
+__global__ void __launch_bounds__(kThreads, 2) k_evict_select(const __grid_constant__ Q4EvictArgs a, int ctas, int room) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  SelectSmem& s = *reinterpret_cast<SelectSmem*>(smem);
+  const int K = a.kv.n_kv_heads, unit = blockIdx.x / ctas, me = blockIdx.x - unit * ctas, seq = unit / K, tid = threadIdx.x;
   const Moves out = moves_of(a);
   pdl_wait();
   if (tid == 0) pdl_launch_dependents();
   const uint32_t len = a.seq_len[seq];
   const bool fits = len <= q4_capacity(a.kv);
-  if (tid == 0) {
+  if (tid == 0 && me == 0) {
     if (!fits) raise_error(a.err, kDevBadArgument);
     if (unit % K == 0) out.length[seq] = fits ? min((int)len, a.n_keep) : -1;
   }
   if (!fits || (int)len <= a.n_keep) {
-    if (tid == 0) out.count[unit] = 0;
+    if (tid == 0 && me == 0) out.count[unit] = 0;
     return;
   }
-  if (len <= 2 * kThreads) select_row<2>(a, unit, (int)len, s);
-  else if (len <= 8 * kThreads) select_row<8>(a, unit, (int)len, s);
-  else if (len <= 32 * kThreads) select_row<32>(a, unit, (int)len, s);
-  else select_row<0>(a, unit, (int)len, s);
+  // whole words of bits to each CTA
+  const int share = (((int)len + ctas - 1) / ctas + 31) / 32 * 32, first = me * share;
+  select_row(a, unit, first, max(0, min(share, (int)len - first)), room, ctas > 1, s);
 }
 
 // D / 8 lanes a pair: 16 bytes of codes of each group of K and of V, then their parameters.
@@ -309,16 +345,33 @@ size_t evict_q4_workspace(const qwen_paged_kv_q4& kv, uint32_t n_keep) {
 
 int launch_evict_q4(const Q4EvictArgs& a, cudaStream_t st) {
   const int units = (int)(a.kv.n_seq * a.kv.n_kv_heads);
-  cudaLaunchAttribute attr[1];
+  // CTAs of a row: as many as find room at once (two an SM), where rows can be long enough
+  int cluster = 1;
+  while (cluster < kMaxCluster && 2 * cluster * units <= 2 * paged_sm_count() &&
+         (long long)a.kv.max_pages * a.kv.page_size > 4096 * cluster)
+    cluster *= 2;
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(units);
+  cfg.gridDim = dim3(units * cluster);
   cfg.blockDim = dim3(kThreads);
+  const long long share = ((long long)a.kv.max_pages * a.kv.page_size + cluster - 1) / cluster + 31;
+  const int room = (int)std::min<long long>(kMaxHeld, share);
+  const int smem = (int)sizeof(SelectSmem) + 4 * room;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  static OncePerDevice once;
+  if (once.launch(reinterpret_cast<const void*>(k_evict_select), (int)sizeof(SelectSmem) + 4 * kMaxHeld,
+                  [&] { return cudaLaunchKernelEx(&cfg, k_evict_select, a, cluster, room); }) != cudaSuccess)
+    return -1;
+  cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, k_evict_select, a) != cudaSuccess) return -1;
   const int per_cta = kMoveThreads / ((int)a.kv.head_dim / 8);
   cfg.gridDim = dim3(units, std::max(1, std::min((a.n_keep + per_cta - 1) / per_cta, 8 * paged_sm_count() / units)));
   cfg.blockDim = dim3(kMoveThreads);
