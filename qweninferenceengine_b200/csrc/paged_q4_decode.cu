@@ -19,8 +19,8 @@
 // word's eight keys take four ANDs and a shift (those from bits 4..7 are 16 c 2^-24; their
 // query elements are divided by 16).  Queries are brought to 2^14 .. 2^15 a head by a power
 // of two and are exact in fp16 but for what is 2^-33 of the head's largest.  For the values
-// the codes are 128 + c in bf16, whose product with weights up to any size is in range;
-// 128 sum_t step P is taken off at the end.  The two sums of P with lows and with steps are
+// the codes are 16 + c (fp16 caches) or 128 + c in bf16, whose product with weights up to any
+// size is in range; 16 or 128 sum_t step P is taken off at the end.  The two sums of P with lows and with steps are
 // one MMA over the slots, q's group sums with lows another (three terms of 8 or 11 bits).
 // Weights step P are two bf16 values (16 bits).  Sums, maxima and outputs are fp32.
 #include <algorithm>
@@ -211,9 +211,17 @@ __device__ __forceinline__ void small_codes(uint32_t w, uint32_t (&c)[4]) {
   c[2] = w & 0x00f000f0u;
   c[3] = v & 0x00f000f0u;
 }
-// 128 + codes in bf16 of bits 4 j .. 4 j + 3 of both halves of a word.
+// Bias + codes in bf16 of bits 4 j .. 4 j + 3 of both halves of a word.  The bias is taken off
+// the sums, which are rounded relative to it: with 128, whose codes need no shift for j = 0,
+// outputs over 32768 positions were off by 3.0e-4 (2-norm), more than fp16's own 2.0e-4.
+template <typename T>
+constexpr float kBias = std::is_same<T, __half>::value ? 16.f : 128.f;
+template <typename T>
 __device__ __forceinline__ uint32_t large_code(uint32_t w, int j) {
-  return lop3_and_or(w >> (4 * j), 0x000f000fu, 0x43004300u);
+  if constexpr (std::is_same<T, __half>::value)
+    return lop3_and_or(j ? w >> (4 * j - 3) : w << 3, 0x00780078u, 0x41804180u);
+  else
+    return lop3_and_or(w >> (4 * j), 0x000f000fu, 0x43004300u);
 }
 
 // Scores of a block, log2 domain: s = (slot g: heads 2t, 2t+1), (slot g + 8: the same).
@@ -391,7 +399,7 @@ __device__ __forceinline__ void take_blocks(Stream<D>& w, uint8_t* const (&block
       mma_16816_t(T{}, w.extra, x, h0, h1);
       mma_16816_t(T{}, w.extra, x, e0, e1);
     }
-    // ---- o^T += (128 + codes)^T (step weights)^T
+    // ---- o^T += (bias + codes)^T (step weights)^T
     uint32_t vc[G][2];   // [half]: unit g (elements 4 g ..) of slots 2t, 2t+1 of that half
     {
       uint32_t r[4];
@@ -416,8 +424,8 @@ __device__ __forceinline__ void take_blocks(Stream<D>& w, uint8_t* const (&block
       }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const uint32_t x[4] = {large_code(vc[i][0], 2 * j), large_code(vc[i][0], 2 * j + 1),
-                               large_code(vc[i][1], 2 * j), large_code(vc[i][1], 2 * j + 1)};
+        const uint32_t x[4] = {large_code<T>(vc[i][0], 2 * j), large_code<T>(vc[i][0], 2 * j + 1),
+                               large_code<T>(vc[i][1], 2 * j), large_code<T>(vc[i][1], 2 * j + 1)};
         mma_16816_t(__nv_bfloat16{}, w.o[i][j], x, b0, b1);
         mma_16816_t(__nv_bfloat16{}, w.o[i][j], x, c0, c1);
       }
@@ -685,7 +693,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_q4_decode(const __grid
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const float add = __shfl_sync(0xffffffffu, w.extra[e], 4 * i + t4) -
-                          128.f * __shfl_sync(0xffffffffu, w.extra[e], 4 * (4 + i) + t4);
+                          kBias<T> * __shfl_sync(0xffffffffu, w.extra[e], 4 * (4 + i) + t4);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           w.o[i][j][e] = (w.o[i][j][e] + add) * f[e];

@@ -126,7 +126,8 @@ def attention(c, scale, q=None, lens=None):
     is rounded to fp16 at most once (2^-11; to two values it is 2^-22), sums of L of them
     in fp32 are off by 2^-23 L; what they multiply is at most |low| + code step.  So
     |out error| <= A (2^-11 + 2 d + 2^-22 L) + u |out|, A = sum p (|low| + code step) / sum
-    p, |lse error| <= d + 2^-23 L + 2^-22 |lse|, and a weight exp(s - lse) is off by (d +
+    p; and where codes are multiplied with a bias of up to 128 beside them, that is taken off
+    again, by weights times steps of 16 bits, 143 2^-17 sum p step / sum p.  |lse error| <= d + 2^-23 L + 2^-22 |lse|, and a weight exp(s - lse) is off by (d +
     the lse's) p, the sum of a group's by 2^-23 of it and of what it is added to."""
     q = c.q if q is None else q
     lens = c.lens if lens is None else lens
@@ -143,6 +144,8 @@ def attention(c, scale, q=None, lens=None):
         slots = torch.arange(L, device=q.device)
         k, v = c.rows(i, slots)
         ka, va = c.sizes(i, slots)
+        page, block, r = c.place(i, slots)
+        vstep = views(c.pool, c.dim, c.dtype)[3][page, :, block, :, r][..., 0].double().repeat_interleave(32, -1)
         for h in range(K):
             rows = slice(h * G, (h + 1) * G)
             x = q[i, rows].double()
@@ -150,7 +153,8 @@ def attention(c, scale, q=None, lens=None):
             d = 2.0 ** -23 * (2 * D * (x.abs() @ ka[:, h].T * abs(scale)).amax(-1) + 16 + 2 * s.abs().amax(-1))
             w = torch.softmax(s, -1)
             out[i, rows] = w @ v[:, h]
-            tol[i, rows] = (w @ va[:, h]) * (2.0 ** -11 + 2 * d + 2.0 ** -22 * L)[:, None] + u * out[i, rows].abs()
+            tol[i, rows] = (w @ va[:, h]) * (2.0 ** -11 + 2 * d + 2.0 ** -22 * L)[:, None] + u * out[i, rows].abs() + \
+                143 * 2.0 ** -17 * (w @ vstep[:, h])
             lse[i, rows] = torch.logsumexp(s, -1)
             lse_tol[i, rows] = d + 2.0 ** -23 * L + 2.0 ** -22 * lse[i, rows].abs()
             w_all[i, h, :L] = w.sum(0)
