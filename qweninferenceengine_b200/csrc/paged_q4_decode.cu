@@ -4,9 +4,12 @@
 //
 // Work, runs of tiles, partials and their join: as in paged_decode.cu (paged_runs.cuh).  A
 // tile is 128 slots, a unit (sequence, kv head, up to 8 query heads).  A CTA has a producer
-// warp, which looks pages up and copies a tile's blocks of 16 slots (codes and parameters
-// of K and V lie side by side, so a copy takes up to 8 blocks at once), and 4 consumer
-// warps, each with two blocks of a tile.
+// warp, which looks pages up and copies a tile's 8 blocks of 16 slots (codes and parameters of
+// K and V lie side by side, so a copy takes all of a page's blocks in the tile), and 4 consumer
+// warps, one a scheduler, each with two blocks of a tile, whose instructions fill one another's
+// gaps.  Three such CTAs an SM leave a thread 128 registers.  (16 x 8704 of 8 kv heads, fp16,
+// 36 us: with runs of blocks 46; with 6 such warps in two CTAs, which the schedulers do not
+// divide evenly, 51; with 12 in one, which all wait at a piece's end, 58.)
 //
 // What bounds it is not the bytes alone, 2.5 KB a block of 128-element heads, but the
 // instructions that turn them into products; so nothing is dequantised.  Per block a warp
@@ -36,30 +39,33 @@ namespace {
 
 constexpr int kWarps = 4;                     // consumer warps
 constexpr int kThreads = (kWarps + 1) * 32;
-constexpr int kBlocks = 8;                    // of a tile: a warp takes two
-constexpr int kTile = 16 * kBlocks, kTileShift = 7;
+constexpr int kBlocks = 2 * kWarps;           // of a tile: a warp takes two
+static_assert(16 * kBlocks == 1 << 7, "tile");
+constexpr int kTileShift = 7;
 constexpr int kCtasPerSm = 3;
 constexpr int kSlotHeads = 8;                 // query heads of a unit
-constexpr int kQuerySlots = 2;
-constexpr int kMergeRows = kWarps / 2;
+constexpr int kQuerySlots = 4;
 
-enum StageFlags { kFirst = 1, kLast = 2, kEnd = 4 };
-
-struct StageMeta {
-  int valid[kBlocks];   // slots of each 16 that count
-  int flags;
-  int seq, head, heads;   // the unit: sequence, first query head, query heads
+// A run's part of a unit.
+struct Piece {
+  int heads;           // query heads, or 0: the run has no more pieces
+  int seq, head;       // sequence, first query head
   int dest;            // partial slot, or -1: the whole unit, or -2: nothing is written
-  float2* scores;      // of the tile's first slot, or null
+  float2* scores;      // of the unit's slot 0, or null
+};
+struct StageMeta {
+  int valid[kBlocks];  // slots of each block that count
+  int first;           // the tile's first slot
+  int last;            // of the piece
 };
 
 template <int D>
 struct __align__(128) Q4DecodeSmem {
   static constexpr int kStages = D == 128 ? 3 : 6;
   uint8_t kv[kStages][kBlocks][Q4Block<D>::kBytes];
-  float4 rows[kMergeRows][kSlotHeads][D / 4];   // of the warps' outputs, chunk c of head h at c ^ (h & 6)
   uint16_t q[kQuerySlots][kSlotHeads * D];
   float2 ml[2][kWarps][kSlotHeads];   // by piece parity: maximum and sum of each warp
+  Piece piece[kQuerySlots];
   StageMeta meta[kStages];
   uint64_t full[kStages], empty[kStages], qfull[kQuerySlots], qempty[kQuerySlots], joined, early;
   CutUnit cut[2];
@@ -466,16 +472,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_q4_decode(const __grid
     // ------------------------------------------------------------ producer --
     const int P = a.kv.page_size;
     const uint32_t capacity = a.kv.max_pages * a.kv.page_size;
-    // lane l < 8: block l of a tile; the first of each page's blocks copies them all
-    const int block = lane & (kBlocks - 1), per_page = min(P / 16, kBlocks);
-    const bool loads = lane < kBlocks && block % per_page == 0;
     uint32_t it = 0, pieces = 0;
     int seq, n_cut = 0;
     uint32_t before, L, runs = gridDim.x;
     const uint32_t total = find_run(p, c, runs, lane, &seq, &before, &L);
     const uint32_t t1 = c < (int)runs ? run_start(total, c + 1, runs) : 0;
     uint32_t t = run_start(total, c, runs), ts = seq_tiles(p, L);   // (c >= runs: no run)
-    int cached_seq = -1, cached_base = 0, page = -1, left = 0, next_page = -1;   // lane i: entry cached_base + i
+    // lane i: pages of the table row's entries base + i and base + 32 + i, -1: none
+    int cached_seq = -1, base = 0, page_lo = -1, page_hi = -1;
     bool alive = true, cut_first = false;
 #pragma unroll 1
     while (t < t1 && alive) {
@@ -493,38 +497,62 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_q4_decode(const __grid
       const bool fits = L <= capacity;
       if (!fits && lane == 0) raise_error(a.err, kDevBadArgument);
       const int dest = !fits ? -2 : tile0 == 0 && tile1 == ts ? -1 : 2 * c + (tile0 == 0 ? 1 : 0);
+      // ---- the piece and its queries
+      const int qs = pieces % QS;
+      if (pieces >= QS &&
+          !__all_sync(0xffffffffu, paged_wait(&s.qempty[qs], (pieces / QS - 1) & 1, &s.abort, a.err))) {
+        alive = false;
+        break;
+      }
+      if (lane == 0) {
+        Piece& x = s.piece[qs];
+        x.heads = heads;
+        x.seq = seq;
+        x.head = head;
+        x.dest = dest;
+        x.scores = p.scores ? reinterpret_cast<float2*>(p.scores) +
+                                  ((long long)seq * p.units_per_seq + unit) * capacity * p.score_pairs
+                            : nullptr;
+        mbar_arrive_expect_tx(&s.qfull[qs], (uint32_t)heads * D * 2);
+        bulk_g2s(s.q[qs], a.q + (long long)seq * a.q_stride + (long long)head * D, (uint32_t)heads * D * 2, &s.qfull[qs]);
+      }
+      ++pieces;
       const int32_t* table = a.kv.page_table + (long long)seq * a.kv.table_stride;
-      const int n_entries = (int)((L + P - 1) >> a.page_shift);
+      const int n_entries = fits ? (int)((L + P - 1) >> a.page_shift) : 0;
       const uint8_t* pool = p.kv.pool + (long long)h * p.kv.head_stride;
-      bool first = true;
+      auto look_up = [&](int entry) {
+        int page = -1;
+        if (entry < n_entries) {
+          page = table[entry];
+          if (page < 0 || (uint32_t)page >= a.kv.n_pages) {
+            raise_error(a.err, kDevBadArgument);
+            page = -1;
+          }
+        }
+        return page;
+      };
 #pragma unroll 1
       for (uint32_t tile = tile0; tile < tile1; ++tile) {
-        const int first_entry = ((int)tile * kTile) >> a.page_shift;
-        if (cached_seq != seq || first_entry < cached_base ||
-            ((int)tile * kTile + kTile - 1) >> a.page_shift >= cached_base + 32) {
-          // page of the pool, and how many of the sequence's slots begin with it
-          const int e = first_entry + lane;
-          const bool ahead = cached_seq == seq && first_entry == cached_base + 32;
-          page = -1;
-          left = 0;
-          if (fits && e < n_entries) {
-            page = ahead ? next_page : table[e];
-            if (page < 0 || (uint32_t)page >= a.kv.n_pages) raise_error(a.err, kDevBadArgument);
-            else left = (int)(L - (uint32_t)e * P);
+        // lane l < 8: block l of the tile; the first of each page's copies them all
+        const int first = (int)tile << kTileShift, slot = first + 16 * lane, first_entry = first >> a.page_shift;
+        if (cached_seq != seq || first_entry < base || first_entry >= base + 32) {
+          if (cached_seq == seq && first_entry >= base + 32 && first_entry < base + 64) {
+            base += 32;
+            page_lo = page_hi;
+          } else {
+            base = first_entry;
+            page_lo = look_up(base + lane);
           }
           cached_seq = seq;
-          cached_base = first_entry;
-          // the next 32 of the table row, asked for now
-          if (e + 32 < n_entries) next_page = table[e + 32];
+          page_hi = look_up(base + 32 + lane);   // asked for long before its turn
         }
-        const int pos = (int)tile * kTile + 16 * block, from = (pos >> a.page_shift) - cached_base;
-        const int off = pos & (P - 1);
-        const int behind = max(__shfl_sync(0xffffffffu, left, from) - off, 0);   // slots from this block's first on
-        const int my_page = __shfl_sync(0xffffffffu, page, from);
-        const uint32_t bytes = loads ? (uint32_t)((min(behind, per_page * 16) + 15) >> 4) * Block::kBytes : 0;
+        const int from = (slot >> a.page_shift) - base, off = slot & (P - 1);
+        const int lo = __shfl_sync(0xffffffffu, page_lo, from & 31), hi = __shfl_sync(0xffffffffu, page_hi, from & 31);
+        const int page = from < 32 ? lo : hi;
+        const int valid = lane < kBlocks && page >= 0 ? max(0, min(16, (int)L - slot)) : 0;
+        const uint32_t there = __ballot_sync(0xffffffffu, valid > 0);
         const bool last = tile + 1 == tile1;
-        const uint32_t all = __reduce_add_sync(0xffffffffu, bytes);
-        if (all == 0 && !last) continue;
+        if (there == 0 && !last) continue;
         const int st = it % ST;
         if (it >= ST &&
             !__all_sync(0xffffffffu, paged_wait(&s.empty[st], ((it / ST) - 1) & 1, &s.abort, a.err))) {
@@ -532,41 +560,21 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_q4_decode(const __grid
           break;
         }
         StageMeta& meta = s.meta[st];
-        if (lane < kBlocks) meta.valid[lane] = min(behind, 16);
+        if (lane < kBlocks) meta.valid[lane] = valid;
         if (lane == 0) {
-          meta.flags = (first ? kFirst : 0) | (last ? kLast : 0);
-          meta.heads = heads;
-          if (p.scores)
-            meta.scores = reinterpret_cast<float2*>(p.scores) +
-                          (((long long)seq * p.units_per_seq + unit) * capacity + tile * kTile) * p.score_pairs;
-          if (last) {
-            meta.seq = seq;
-            meta.head = head;
-            meta.dest = dest;
-          }
+          meta.first = first;
+          meta.last = last;
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive_expect_tx(&s.full[st], all);
+        if (lane == 0) mbar_arrive_expect_tx(&s.full[st], __popc(there) * Block::kBytes);
         __syncwarp();
-        if (bytes)
-          bulk_g2s(s.kv[st][block], pool + (long long)my_page * p.kv.page_stride + (off >> 4) * Block::kBytes, bytes,
-                   &s.full[st]);
+        if (valid > 0 && (lane == 0 || off == 0)) {   // (its page's blocks of the tile all count, but what is behind the end)
+          const int of_page = min((P - off) >> 4, kBlocks - lane);
+          const uint32_t mine = there >> lane & ((1u << of_page) - 1);
+          bulk_g2s(s.kv[st][lane], pool + (long long)page * p.kv.page_stride + (off >> 4) * Block::kBytes,
+                   __popc(mine) * Block::kBytes, &s.full[st]);
+        }
         ++it;
-        if (first) {   // the unit's queries, behind its first tile
-          const int qs = pieces % QS;
-          if (pieces >= QS &&
-              !__all_sync(0xffffffffu, paged_wait(&s.qempty[qs], (pieces / QS - 1) & 1, &s.abort, a.err))) {
-            alive = false;
-            break;
-          }
-          if (lane == 0) {
-            mbar_arrive_expect_tx(&s.qfull[qs], (uint32_t)heads * D * 2);
-            bulk_g2s(s.q[qs], a.q + (long long)seq * a.q_stride + (long long)head * D, (uint32_t)heads * D * 2,
-                     &s.qfull[qs]);
-          }
-          ++pieces;
-        }
-        first = false;
       }
       if (dest >= 0) {
         CutUnit u;
@@ -599,25 +607,25 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_q4_decode(const __grid
       s.n_early = n_early;
     }
     __syncwarp();
-    uint32_t drained = it >= (uint32_t)ST ? it - ST : 0;
-    if (alive) {   // the end of the run, in a stage whose last copy was consumed
-      const int st = it % ST;
-      alive = it < ST || __all_sync(0xffffffffu, paged_wait(&s.empty[st], ((it / ST) - 1) & 1, &s.abort, a.err));
+    uint32_t q_drained = pieces > (uint32_t)QS ? pieces - QS : 0;
+    if (alive) {   // the end of the run, in a slot whose last piece was consumed
+      const int qs = pieces % QS;
+      alive = pieces < QS || __all_sync(0xffffffffu, paged_wait(&s.qempty[qs], (pieces / QS - 1) & 1, &s.abort, a.err));
       if (alive) {
-        if (it >= ST) ++drained;
+        if (pieces >= QS) ++q_drained;
         if (lane == 0) {
-          s.meta[st].flags = kEnd;
-          mbar_arrive(&s.full[st]);
+          s.piece[qs].heads = 0;
+          mbar_arrive(&s.qfull[qs]);
         }
       }
     }
     __syncwarp();
     // Every issued copy lands before the CTA may exit.
 #pragma unroll 1
-    for (uint32_t j = drained; j < it; ++j)
+    for (uint32_t j = it > (uint32_t)ST ? it - ST : 0; j < it; ++j)
       paged_wait(&s.full[j % ST], (j / ST) & 1, &s.abort, a.err, false);
 #pragma unroll 1
-    for (uint32_t j = pieces > (uint32_t)QS ? pieces - QS : 0; j < pieces; ++j)
+    for (uint32_t j = q_drained; j < pieces; ++j)
       paged_wait(&s.qfull[j % QS], (j / QS) & 1, &s.abort, a.err, false);
     return;
   }
@@ -625,52 +633,48 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_q4_decode(const __grid
   // -------------------------------------------------------------- consumers --
   const int g = lane >> 2, t4 = lane & 3;
   Stream<D> w;
-  uint32_t pieces = 0, joins = 0;
+  uint32_t joins = 0, it = 0;
   auto join = [&]() {   // the consumer warps' barrier
     __syncwarp();
     if (lane == 0) mbar_arrive(&s.joined);
     return __all_sync(0xffffffffu, paged_wait(&s.joined, joins++ & 1, &s.abort, a.err));
   };
 #pragma unroll 1
-  for (uint32_t it = 0;; ++it) {
-    const int st = it % ST;
-    if (!__all_sync(0xffffffffu, paged_wait(&s.full[st], (it / ST) & 1, &s.abort, a.err))) return;
-    const StageMeta& meta = s.meta[st];
-    const int flags = meta.flags;
-    if (flags & kEnd) break;
-    if (flags & kFirst) {
-      const int qs = pieces % QS;
-      if (!__all_sync(0xffffffffu, paged_wait(&s.qfull[qs], (pieces / QS) & 1, &s.abort, a.err))) return;
-      ++pieces;
-      load_queries<T, D>(w.u, reinterpret_cast<const T*>(s.q[qs]), meta.heads, p.scale_log2, lane);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s.qempty[qs]);
-      w.m[0] = w.m[1] = -INFINITY;
-      w.ref[0] = w.ref[1] = w.l[0] = w.l[1] = 0.f;
+  for (uint32_t pieces = 0;; ++pieces) {
+    const int qs = pieces % QS;
+    if (!__all_sync(0xffffffffu, paged_wait(&s.qfull[qs], (pieces / QS) & 1, &s.abort, a.err))) return;
+    const Piece& piece = s.piece[qs];
+    const int heads = piece.heads;
+    if (heads == 0) break;
+    load_queries<T, D>(w.u, reinterpret_cast<const T*>(s.q[qs]), heads, p.scale_log2, lane);
+    w.m[0] = w.m[1] = -INFINITY;
+    w.ref[0] = w.ref[1] = w.l[0] = w.l[1] = 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        w.extra[e] = 0.f;
+    for (int e = 0; e < 4; ++e) {
+      w.extra[e] = 0.f;
 #pragma unroll
-        for (int i = 0; i < G; ++i) w.o[i][0][e] = w.o[i][1][e] = 0.f;
-      }
+      for (int i = 0; i < G; ++i) w.o[i][0][e] = w.o[i][1][e] = 0.f;
     }
-    const int valid[2] = {meta.valid[warp], meta.valid[warp + kWarps]};
-    uint8_t* const blocks[2] = {s.kv[st][warp], s.kv[st][warp + kWarps]};
-    float2* scores = p.scores ? meta.scores + 16 * warp * p.score_pairs : nullptr;
-    if (valid[1] > 0) take_blocks<T, D, 2>(w, blocks, valid, lane, scores, p.score_pairs);
-    else if (valid[0] > 0) take_blocks<T, D, 1>(w, blocks, valid, lane, scores, p.score_pairs);
-    if (!(flags & kLast)) {
+    int st;
+#pragma unroll 1
+    for (;; ++it) {
+      st = it % ST;
+      if (!__all_sync(0xffffffffu, paged_wait(&s.full[st], (it / ST) & 1, &s.abort, a.err))) return;
+      const StageMeta& meta = s.meta[st];
+      const int valid[2] = {meta.valid[warp], meta.valid[warp + kWarps]};
+      const bool last = meta.last;
+      uint8_t* const blocks[2] = {s.kv[st][warp], s.kv[st][warp + kWarps]};
+      float2* scores = p.scores ? piece.scores + (long long)(meta.first + 16 * warp) * p.score_pairs : nullptr;
+      if (valid[1] > 0) take_blocks<T, D, 2>(w, blocks, valid, lane, scores, p.score_pairs);
+      else if (valid[0] > 0) take_blocks<T, D, 1>(w, blocks, valid, lane, scores, p.score_pairs);
+      if (last) break;
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.empty[st]);
-      continue;
     }
-
-    // ---- the end of a piece.  Half of the warps hand their rows to the other half, whose
-    // sums are joined.
-    const StageMeta unit = meta;
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&s.empty[st]);
-    float2(*ml)[kSlotHeads] = s.ml[(pieces - 1) & 1];
+    // ---- the end of a piece.  Join the warps: the last stage, which every warp is done with
+    // after the first join, holds their rows, [warp][head][chunk of 4 ^ (head & 6)].
+    ++it;
+    float2(*ml)[kSlotHeads] = s.ml[pieces & 1];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       float x = w.l[e];
@@ -678,15 +682,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_q4_decode(const __grid
       x += __shfl_xor_sync(0xffffffffu, x, 8);
       x += __shfl_xor_sync(0xffffffffu, x, 16);
       if (g == 0) ml[warp][2 * t4 + e] = make_float2(w.m[e], x);
-    }
-    if (!join()) return;
-    float f[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      float M = -INFINITY;
-#pragma unroll
-      for (int k = 0; k < kWarps; ++k) M = fmaxf(M, ml[k][2 * t4 + e].x);
-      f[e] = w.m[e] == -INFINITY ? 0.f : exp2_fast(w.m[e] - M);
     }
 #pragma unroll
     for (int i = 0; i < G; ++i)
@@ -696,52 +691,51 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_q4_decode(const __grid
                           kBias<T> * __shfl_sync(0xffffffffu, w.extra[e], 4 * (4 + i) + t4);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          w.o[i][j][e] = (w.o[i][j][e] + add) * f[e];
-          w.o[i][j][2 + e] = (w.o[i][j][2 + e] + add) * f[e];
+          w.o[i][j][e] += add;
+          w.o[i][j][2 + e] += add;
         }
       }
-    if (warp >= kMergeRows) {
-#pragma unroll
-      for (int i = 0; i < G; ++i)
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          s.rows[warp - kMergeRows][2 * t4 + e][(8 * i + g) ^ (2 * t4)] =
-              make_float4(w.o[i][0][e], w.o[i][0][2 + e], w.o[i][1][e], w.o[i][1][2 + e]);
-    }
     if (!join()) return;
-    if (warp < kMergeRows) {
+    auto rows = reinterpret_cast<float4(*)[kSlotHeads][D / 4]>(s.kv[st][0]);
+    static_assert(sizeof(float4) * kWarps * kSlotHeads * (D / 4) <= kBlocks * Block::kBytes, "the warps' rows exceed a stage");
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float M = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < kWarps; ++k) M = fmaxf(M, ml[k][2 * t4 + e].x);
+      const float f = w.m[e] == -INFINITY ? 0.f : exp2_fast(w.m[e] - M);
 #pragma unroll
       for (int i = 0; i < G; ++i)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float4& at = s.rows[warp][2 * t4 + e][(8 * i + g) ^ (2 * t4)];
-          const float4 x = at;
-          at = make_float4(x.x + w.o[i][0][e], x.y + w.o[i][0][2 + e], x.z + w.o[i][1][e], x.w + w.o[i][1][2 + e]);
-        }
+        rows[warp][2 * t4 + e][(8 * i + g) ^ (2 * t4)] =
+            make_float4(w.o[i][0][e] * f, w.o[i][0][2 + e] * f, w.o[i][1][e] * f, w.o[i][1][2 + e] * f);
     }
     if (!join()) return;
 #pragma unroll 1
-    for (int head = warp; head < unit.heads && unit.dest != -2; head += kWarps) {
+    for (int head = warp; head < heads && piece.dest != -2; head += kWarps) {
       constexpr int V = D / 32;   // elements of this lane
       float M = -INFINITY, sum = 0.f, v[V];
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) M = fmaxf(M, ml[w][head].x);
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w)   // (a warp without a maximum has the sum 0, or NaN, which stays)
-        sum += ml[w][head].y * (ml[w][head].x == -INFINITY ? 0.f : exp2_fast(ml[w][head].x - M));
+      for (int k = 0; k < kWarps; ++k) M = fmaxf(M, ml[k][head].x);
 #pragma unroll
       for (int k = 0; k < V; ++k) v[k] = 0.f;
 #pragma unroll
-      for (int w = 0; w < kMergeRows; ++w) {
-        const float* row = reinterpret_cast<const float*>(s.rows[w][head]) + (((V * lane) ^ (4 * (head & 6))));
+      for (int k = 0; k < kWarps; ++k) {
+        // (a warp without a maximum has the sum 0, or NaN, which stays)
+        sum += ml[k][head].y * (ml[k][head].x == -INFINITY ? 0.f : exp2_fast(ml[k][head].x - M));
+        const float* row = reinterpret_cast<const float*>(rows[k][head]) + ((V * lane) ^ (4 * (head & 6)));
 #pragma unroll
-        for (int k = 0; k < V; ++k) v[k] += row[k];
+        for (int i = 0; i < V; ++i) v[i] += row[i];
       }
-      if (unit.dest == -1) finish_row<T, D, false>(p, unit.seq, unit.head + head, as_float4(v), M, sum, lane);
-      else store_partial<D>(p, unit.dest * kSlotHeads + head, as_float4(v), M, sum, lane);
+      if (piece.dest == -1) finish_row<T, D, false>(p, piece.seq, piece.head + head, as_float4(v), M, sum, lane);
+      else store_partial<D>(p, piece.dest * kSlotHeads + head, as_float4(v), M, sum, lane);
     }
+    fence_proxy_async();   // the rows before the next copy
     __syncwarp();
-    if (lane == 0 && pieces == 1) mbar_arrive(&s.early);   // the run's first piece is written
+    if (lane == 0) {
+      mbar_arrive(&s.empty[st]);
+      mbar_arrive(&s.qempty[qs]);
+      if (pieces == 0) mbar_arrive(&s.early);   // the run's first piece is written
+    }
   }
 
   // ---- the last pieces to arrive join the others'
@@ -899,7 +893,7 @@ size_t units_of(const qwen_paged_kv_q4& kv, int n_heads) {
 
 bool attention_q4_fits(const qwen_paged_kv_q4& kv, int n_heads) {
   const double slots = (double)kv.max_pages * kv.page_size;
-  return (double)units_of(kv, n_heads) * std::ceil(slots / kTile) < 2147483648.0 &&
+  return (double)units_of(kv, n_heads) * std::ceil(slots / (1 << kTileShift)) < 2147483648.0 &&
          (!kv.weights || (double)kv.n_seq * kv.n_kv_heads * std::ceil(slots / (1 << kWeighTileShift)) < 2147483648.0);
 }
 
