@@ -129,21 +129,24 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t* hi, uint32_t*
   *lo = pack2(T{}, x - r.x, y - r.y);
 }
 
-// D = A B from zeros (which need no registers).
-__device__ __forceinline__ void mma_zero(__half, float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-      "{%8,%9}, {%10,%10,%10,%10};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
-}
-__device__ __forceinline__ void mma_zero(__nv_bfloat16, float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-      "{%8,%9}, {%10,%10,%10,%10};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
-}
+// D = A B + D, and from zeros (which need no registers).  Not volatile: what they depend on
+// orders them.
+#define QWEN_MMA(name, type)                                                                                   \
+  __device__ __forceinline__ void mma_add(name, float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) { \
+    asm("mma.sync.aligned.m16n8k16.row.col.f32." type "." type ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "  \
+        "{%0,%1,%2,%3};"                                                                                       \
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])                                                       \
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));                                       \
+  }                                                                                                            \
+  __device__ __forceinline__ void mma_zero(name, float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) { \
+    asm("mma.sync.aligned.m16n8k16.row.col.f32." type "." type ".f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "  \
+        "{%10,%10,%10,%10};"                                                                                   \
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])                                                       \
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));                             \
+  }
+QWEN_MMA(__half, "f16")
+QWEN_MMA(__nv_bfloat16, "bf16")
+#undef QWEN_MMA
 
 // What a warp keeps of a unit's queries.
 template <int D>
@@ -254,7 +257,7 @@ __device__ __forceinline__ void block_scores(const Queries<D>& u, const uint32_t
     const uint32_t a0[4] = {x[0], y[0], x[1], y[1]}, a1[4] = {x[2], y[2], x[3], y[3]};
     float d[4];
     mma_zero(__half{}, d, a0, u.f[i][0], u.f[i][1]);
-    mma_16816_t(__half{}, d, a1, u.f[i][2], u.f[i][3]);
+    mma_add(__half{}, d, a1, u.f[i][2], u.f[i][3]);
     const float s0 = step_of(T{}, params[0][i]), s1 = step_of(T{}, params[1][i]);
     sum[0] = i ? fmaf(d[0], s0, sum[0]) : d[0] * s0;
     sum[1] = i ? fmaf(d[1], s0, sum[1]) : d[1] * s0;
@@ -361,79 +364,77 @@ __device__ __forceinline__ void take_blocks(Stream<D>& w, uint8_t* const (&block
         }
     }
   }
+  // ---- weights, turned: lane 4 g + t has head g, slots 2t, 2t+1 and 8 + those
+  uint32_t h0[kN], h1[kN], e0[kN], e1[kN];   // in the cache's type, and what rounding left
+  float pw[kN][4];                           // fp16: the weights themselves
+  uint32_t vs[kN];
 #pragma unroll
   for (int n = 0; n < kN; ++n) {
-    const uint32_t at = smem_u32(blocks[n]);
+    vs[n] = smem_u32(blocks[n]) + Block::kValueSteps + t4 * 8;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       sv[n][e] = exp2_fast(sv[n][e] - w.ref[e]);
       sv[n][2 + e] = exp2_fast(sv[n][2 + e] - w.ref[e]);
       w.l[e] += sv[n][e] + sv[n][2 + e];
     }
-    // ---- weights, turned: lane 4 g + t has head g, slots 2t, 2t+1 and 8 + those
-    uint32_t h0, h1, e0, e1;   // in the cache's type, and what rounding left
-    float pw[4];               // fp16: the weights themselves
     if constexpr (kF16) {
       const uint32_t x0 = movmatrix(prmt(__float_as_uint(sv[n][0]), __float_as_uint(sv[n][1]), 0x7632));
       const uint32_t y0 = movmatrix(prmt(__float_as_uint(sv[n][0]), __float_as_uint(sv[n][1]), 0x5410));
       const uint32_t x1 = movmatrix(prmt(__float_as_uint(sv[n][2]), __float_as_uint(sv[n][3]), 0x7632));
       const uint32_t y1 = movmatrix(prmt(__float_as_uint(sv[n][2]), __float_as_uint(sv[n][3]), 0x5410));
-      pw[0] = __uint_as_float(prmt(y0, x0, 0x5410));
-      pw[1] = __uint_as_float(prmt(y0, x0, 0x7632));
-      pw[2] = __uint_as_float(prmt(y1, x1, 0x5410));
-      pw[3] = __uint_as_float(prmt(y1, x1, 0x7632));
-      split2<T>(pw[0], pw[1], &h0, &e0);
-      split2<T>(pw[2], pw[3], &h1, &e1);
+      pw[n][0] = __uint_as_float(prmt(y0, x0, 0x5410));
+      pw[n][1] = __uint_as_float(prmt(y0, x0, 0x7632));
+      pw[n][2] = __uint_as_float(prmt(y1, x1, 0x5410));
+      pw[n][3] = __uint_as_float(prmt(y1, x1, 0x7632));
+      split2<T>(pw[n][0], pw[n][1], &h0[n], &e0[n]);
+      split2<T>(pw[n][2], pw[n][3], &h1[n], &e1[n]);
     } else {
-      split2<T>(sv[n][0], sv[n][1], &h0, &e0);
-      split2<T>(sv[n][2], sv[n][3], &h1, &e1);
-      h0 = movmatrix(h0);
-      h1 = movmatrix(h1);
-      e0 = movmatrix(e0);
-      e1 = movmatrix(e1);
+      split2<T>(sv[n][0], sv[n][1], &h0[n], &e0[n]);
+      split2<T>(sv[n][2], sv[n][3], &h1[n], &e1[n]);
+      h0[n] = movmatrix(h0[n]);
+      h1[n] = movmatrix(h1[n]);
+      e0[n] = movmatrix(e0[n]);
+      e1[n] = movmatrix(e1[n]);
     }
-    const uint32_t vs = at + Block::kValueSteps + t4 * 8;
-    {   // sums of weights with lows and steps: row g is the low of group g, or the step of g - 4
-      const int i = g & 3;
-      uint32_t x[4] = {};
-      if (i < G) {
-        const uint2 v0 = lds64(vs + i * 64), v1 = lds64(vs + i * 64 + 32);
-        const uint32_t sel = g < 4 ? 0x7632 : 0x5410;
-        x[0] = prmt(v0.x, v0.y, sel);
-        x[2] = prmt(v1.x, v1.y, sel);
-      }
-      mma_16816_t(T{}, w.extra, x, h0, h1);
-      mma_16816_t(T{}, w.extra, x, e0, e1);
+    // sums of weights with lows and steps: row g is the low of group g, or the step of g - 4
+    const int i = g & 3;
+    uint32_t x[4] = {};
+    if (i < G) {
+      const uint2 v0 = lds64(vs[n] + i * 64), v1 = lds64(vs[n] + i * 64 + 32);
+      const uint32_t sel = g < 4 ? 0x7632 : 0x5410;
+      x[0] = prmt(v0.x, v0.y, sel);
+      x[2] = prmt(v1.x, v1.y, sel);
     }
-    // ---- o^T += (bias + codes)^T (step weights)^T
-    uint32_t vc[G][2];   // [half]: unit g (elements 4 g ..) of slots 2t, 2t+1 of that half
-    {
-      uint32_t r[4];
-      const uint32_t row = at + Block::kValues + lane * 16;
-      ldmatrix_x4_trans(r, row);
-      vc[0][0] = r[0], vc[0][1] = r[1], vc[1][0] = r[2], vc[1][1] = r[3];
-      if constexpr (G == 4) {
-        ldmatrix_x4_trans(r, row + 512);
-        vc[2][0] = r[0], vc[2][1] = r[1], vc[3][0] = r[2], vc[3][1] = r[3];
-      }
-    }
+    mma_add(T{}, w.extra, x, h0[n], h1[n]);
+    mma_add(T{}, w.extra, x, e0[n], e1[n]);
+  }
+  // ---- o^T += (bias + codes)^T (step weights)^T
 #pragma unroll
-    for (int i = 0; i < G; ++i) {
-      const uint2 v0 = lds64(vs + i * 64), v1 = lds64(vs + i * 64 + 32);
-      uint32_t b0, b1, c0, c1;
-      if constexpr (kF16) {
-        split2<__nv_bfloat16>(pw[0] * step_of(T{}, v0.x), pw[1] * step_of(T{}, v0.y), &b0, &c0);
-        split2<__nv_bfloat16>(pw[2] * step_of(T{}, v1.x), pw[3] * step_of(T{}, v1.y), &b1, &c1);
-      } else {
-        step_weights(h0, e0, prmt(v0.x, v0.y, 0x5410), &b0, &c0);
-        step_weights(h1, e1, prmt(v1.x, v1.y, 0x5410), &b1, &c1);
-      }
+  for (int pair = 0; pair < G / 2; ++pair) {
+    uint32_t vc[kN][4];   // [group][half]: unit g (elements 4 g ..) of slots 2t, 2t+1 of that half
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const uint32_t x[4] = {large_code<T>(vc[i][0], 2 * j), large_code<T>(vc[i][0], 2 * j + 1),
-                               large_code<T>(vc[i][1], 2 * j), large_code<T>(vc[i][1], 2 * j + 1)};
-        mma_16816_t(__nv_bfloat16{}, w.o[i][j], x, b0, b1);
-        mma_16816_t(__nv_bfloat16{}, w.o[i][j], x, c0, c1);
+    for (int n = 0; n < kN; ++n) ldmatrix_x4_trans(vc[n], smem_u32(blocks[n]) + Block::kValues + pair * 512 + lane * 16);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int i = 2 * pair + k;
+#pragma unroll
+      for (int n = 0; n < kN; ++n) {
+        const uint2 v0 = lds64(vs[n] + i * 64), v1 = lds64(vs[n] + i * 64 + 32);
+        uint32_t b0, b1, c0, c1;
+        if constexpr (kF16) {
+          split2<__nv_bfloat16>(pw[n][0] * step_of(T{}, v0.x), pw[n][1] * step_of(T{}, v0.y), &b0, &c0);
+          split2<__nv_bfloat16>(pw[n][2] * step_of(T{}, v1.x), pw[n][3] * step_of(T{}, v1.y), &b1, &c1);
+        } else {
+          step_weights(h0[n], e0[n], prmt(v0.x, v0.y, 0x5410), &b0, &c0);
+          step_weights(h1[n], e1[n], prmt(v1.x, v1.y, 0x5410), &b1, &c1);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t x[4] = {large_code<T>(vc[n][2 * k], 2 * j), large_code<T>(vc[n][2 * k], 2 * j + 1),
+                                 large_code<T>(vc[n][2 * k + 1], 2 * j), large_code<T>(vc[n][2 * k + 1], 2 * j + 1)};
+          mma_add(__nv_bfloat16{}, w.o[i][j], x, b0, b1);
+          mma_add(__nv_bfloat16{}, w.o[i][j], x, c0, c1);
+        }
       }
     }
   }
