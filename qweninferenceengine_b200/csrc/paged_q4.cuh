@@ -38,11 +38,17 @@ __device__ __forceinline__ float exact_code(float x, float low, float step, floa
   const float below = b - 0.5f, even = 2.f * rintf(0.5f * b);   // (of below and below + 1)
   return fminf(d == 0.f ? even : d > 0.f ? below + 1.f : below, 15.f);
 }
-// The same where the step's reciprocal is beyond fp32 (bf16 steps below 2^-128): everything
-// times 2^64, which is exact.
-static __device__ __noinline__ uint32_t tiny_codes(float4 a, float4 b, float low, float step) {
+__device__ __forceinline__ float rcp_fast(float x) {   // 1 step of fp32; a subnormal gives infinity
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Codes of 8 values by exact_code alone, for steps near their type's ends: everything times
+// 2^64 or 1/4, which is exact (the reciprocal of bf16's least steps and the difference of its
+// greatest values are beyond fp32).
+static __device__ __noinline__ uint32_t end_codes(float4 a, float4 b, float low, float step) {
   const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-  const float k = 18446744073709551616.f, inv = __frcp_rn(step * k);
+  const float k = step < 1.f ? 18446744073709551616.f : 0.25f, inv = rcp_fast(step * k);
   uint32_t codes = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -51,45 +57,61 @@ static __device__ __noinline__ uint32_t tiny_codes(float4 a, float4 b, float low
   }
   return codes;
 }
-// Quantises a group of 32 values, of which this lane holds 8 (fp32, exact) and its three
-// neighbours (lane ^ 1, ^ 2, ^ 3) the rest; all 32 lanes take part.  Returns the lane's
-// codes, element i in bits 4i .. 4i+3, and (step, low) as the cache keeps them.
+__device__ __forceinline__ uint32_t least2(__half, uint32_t a, uint32_t b) {   // NaN if either is
+  const __half2 r = __hmin2_nan(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t least2(__nv_bfloat16, uint32_t a, uint32_t b) {
+  const __nv_bfloat162 r = __hmin2_nan(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t most2(__half, uint32_t a, uint32_t b) {
+  const __half2 r = __hmax2_nan(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t most2(__nv_bfloat16, uint32_t a, uint32_t b) {
+  const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// Quantises a group of 32 values, of which this lane holds 8 and its three neighbours (lane ^ 1,
+// ^ 2, ^ 3) the rest; all 32 lanes take part.  Returns the lane's codes, element i in bits 4i
+// .. 4i+3, and (step, low) as the cache keeps them.
 //
-// The fp32 quotient is off by at most 15 (2^-24 + 2^-24 + 2^-24) < 3e-6 (difference,
+// The least and the greatest are found in pairs, and exchanged as one word (least, -greatest).
+// The fp32 quotient is off by at most 15 (2^-24 + 2^-23 + 2^-24) < 4e-6 (difference,
 // reciprocal, product); where one stands nearer than 1e-5 to a border between two codes,
 // exact_code decides (of bf16's few values one in some hundred is on one).  Rounded by an
 // addition, and packed four at a time by multiplication: conversions run at an eighth of the
 // rate.
 template <typename T>
-__device__ __forceinline__ uint32_t quantise_group(const float (&x)[8], uint32_t* params) {
-  float lo = x[0], hi = x[0], bad = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    lo = fminf(lo, x[i]);
-    hi = fmaxf(hi, x[i]);
-    bad = fmaf(x[i], 0.f, bad);   // NaN for an infinity or NaN
-  }
-#pragma unroll
-  for (int o = 1; o <= 2; o <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    bad += __shfl_xor_sync(0xffffffffu, bad, o);
-  }
-  if (bad != 0.f) lo = hi = bad;
+__device__ __forceinline__ uint32_t quantise_group(const uint4& v, uint32_t* params) {
+  const uint32_t a = least2(T{}, least2(T{}, v.x, v.y), least2(T{}, v.z, v.w));
+  const uint32_t b = most2(T{}, most2(T{}, v.x, v.y), most2(T{}, v.z, v.w)) ^ 0x80008000u;
+  uint32_t ends = least2(T{}, __byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
+  ends = least2(T{}, ends, __shfl_xor_sync(0xffffffffu, ends, 1));
+  ends = least2(T{}, ends, __shfl_xor_sync(0xffffffffu, ends, 2));
+  float lo = unpack2(T{}, ends).x, hi = -unpack2(T{}, ends).y;
+  if (!(fabsf(lo) < INFINITY && fabsf(hi) < INFINITY)) lo = hi = __int_as_float(0x7fffffff);
   const uint32_t p = pack2(T{}, (float)(((double)hi - (double)lo) * (1.0 / 15.0)), lo);
   *params = p;
   const float step = unpack2(T{}, p).x;
   if (!(step > 0.f)) return 0;   // 0 or NaN
+  const float inv = rcp_fast(step);
+  const float2 v0 = unpack2(T{}, v.x), v1 = unpack2(T{}, v.y), v2 = unpack2(T{}, v.z), v3 = unpack2(T{}, v.w);
+  const float x[8] = {v0.x, v0.y, v1.x, v1.y, v2.x, v2.y, v3.x, v3.y};
+  // (a step far below its type's normal ones can be so much less than a fifteenth that quotients
+  // pass 15.5; and see end_codes)
+  if (!((hi - lo) * inv < 15.4f))
+    return end_codes(make_float4(x[0], x[1], x[2], x[3]), make_float4(x[4], x[5], x[6], x[7]), lo, step);
   constexpr float kMagic = 12582912.f;   // 1.5 2^23: sums are rounded to whole numbers, ties to even
-  const float inv = __frcp_rn(step);
   float c[8], off = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float t = fminf((x[i] - lo) * inv, 15.f);
+    const float t = (x[i] - lo) * inv;
     c[i] = __fadd_rn(__fadd_rn(t, kMagic), -kMagic);
     off = fmaxf(off, fabsf(t - c[i]));
   }
-  if (!(inv < INFINITY)) return tiny_codes(make_float4(x[0], x[1], x[2], x[3]), make_float4(x[4], x[5], x[6], x[7]), lo, step);
   if (off > 0.49999f) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -97,9 +119,9 @@ __device__ __forceinline__ uint32_t quantise_group(const float (&x)[8], uint32_t
       if (fabsf(t - c[i]) > 0.49999f) c[i] = exact_code(x[i], lo, step, t, c[i]);
     }
   }
-  const float a = fmaf(c[3], 4096.f, fmaf(c[2], 256.f, fmaf(c[1], 16.f, c[0])));
-  const float b = fmaf(c[7], 4096.f, fmaf(c[6], 256.f, fmaf(c[5], 16.f, c[4])));
-  return __byte_perm(__float_as_uint(a + 8388608.f), __float_as_uint(b + 8388608.f), 0x5410);
+  const float d = fmaf(c[3], 4096.f, fmaf(c[2], 256.f, fmaf(c[1], 16.f, c[0])));
+  const float e = fmaf(c[7], 4096.f, fmaf(c[6], 256.f, fmaf(c[5], 16.f, c[4])));
+  return __byte_perm(__float_as_uint(d + 8388608.f), __float_as_uint(e + 8388608.f), 0x5410);
 }
 
 // Values low + code step of 8 codes in the cache's type, rounded once.  (1024 + code in fp16

@@ -37,17 +37,6 @@ template <typename T>
 __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
   return make_uint4(pack2(T{}, x[0], x[1]), pack2(T{}, x[2], x[3]), pack2(T{}, x[4], x[5]), pack2(T{}, x[6], x[7]));
 }
-// x rounded to the cache's type.
-template <typename T>
-__device__ __forceinline__ void round8(float (&x)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; i += 2) {
-    const float2 r = unpack2(T{}, pack2(T{}, x[i], x[i + 1]));
-    x[i] = r.x;
-    x[i + 1] = r.y;
-  }
-}
-
 // 8 elements of a row, and of a key the 8 that theirs are turned with.
 struct Raw {
   uint4 own, mate;
@@ -73,8 +62,8 @@ __device__ __forceinline__ int rot_at(int pair) {
 }
 // Rotates in the arithmetic of A (double for keys, float for queries).
 template <typename A, typename T, int D, bool kInterleaved>
-__device__ __forceinline__ void rotate_raw(const Raw& r, const double2* rot, int c, int R, float (&x)[8]) {
-  float own[8], mate[8];
+__device__ __forceinline__ uint4 rotate_raw(const Raw& r, const double2* rot, int c, int R) {
+  float own[8], mate[8], x[8];
   unpack8<T>(r.own, own);
   if constexpr (!kInterleaved) unpack8<T>(r.mate, mate);
   const bool second = !kInterleaved && 8 * c >= R / 2;
@@ -86,11 +75,12 @@ __device__ __forceinline__ void rotate_raw(const Raw& r, const double2* rot, int
     const A a = (A)own[e], b = (A)(kInterleaved ? own[e ^ 1] : mate[e]), s = (A)(two ? cs.y : -cs.y);
     x[e] = (float)(a * (A)cs.x + b * s);
   }
+  return pack8<T>(x);
 }
 // Quantises lane c's 8 values of a key's or value's row and stores them (all 32 lanes; of
 // those whose token has a block, and not of others).
 template <typename T, int D>
-__device__ __forceinline__ void store_quantised(const Q4AppendArgs& a, const float (&x)[8], const Token& t, int h, bool is_k,
+__device__ __forceinline__ void store_quantised(const Q4AppendArgs& a, const uint4& x, const Token& t, int h, bool is_k,
                                                 int c, bool live) {
   uint32_t params;
   const uint32_t codes = quantise_group<T>(x, &params);
@@ -162,15 +152,12 @@ __global__ void __launch_bounds__(kTokenThreads) k_append_token_q4(const __grid_
     __syncwarp();   // q_out may be q: every lane has its mates before a row is written
     if (head + kRows < H + 2 * K)
       next = load_raw<T, kInterleaved>(source(head + kRows), c, R, 8 * c < R && head + kRows < H + K);
-    float x[8];
+    uint4 x = r.own;
     if ((is_q || is_k) && 8 * c < R) {
-      if (is_q) rotate_raw<float, T, D, kInterleaved>(r, rot, c, R, x);
-      else rotate_raw<double, T, D, kInterleaved>(r, rot, c, R, x);
-      round8<T>(x);
-    } else {
-      unpack8<T>(r.own, x);
+      if (is_q) x = rotate_raw<float, T, D, kInterleaved>(r, rot, c, R);
+      else x = rotate_raw<double, T, D, kInterleaved>(r, rot, c, R);
     }
-    if (is_q) *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.q_out) + row * a.q_out_stride + head * D + 8 * c) = pack8<T>(x);
+    if (is_q) *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.q_out) + row * a.q_out_stride + head * D + 8 * c) = x;
     if (__any_sync(0xffffffffu, live && !is_q))
       store_quantised<T, D>(a, x, t, is_k ? head - H : head - H - K, is_k, c, live && !is_q);
   }
@@ -291,13 +278,8 @@ __global__ void __launch_bounds__(kRowThreads, 4) k_append_rows_q4(const __grid_
       if (base + j * kStep >= rows) break;
       const Token& t = tok[min(at.t, tokens - 1)];
       const bool is_k = at.x < heads, live = at.t < tokens;
-      float x[8];
-      if (is_k && live && t.seq >= 0 && 8 * c < R) {
-        rotate_raw<double, T, D, kInterleaved>(raw[j], rot[at.t], c, R, x);
-        round8<T>(x);
-      } else {
-        unpack8<T>(raw[j].own, x);
-      }
+      uint4 x = raw[j].own;
+      if (is_k && live && t.seq >= 0 && 8 * c < R) x = rotate_raw<double, T, D, kInterleaved>(raw[j], rot[at.t], c, R);
       if (ahead.t < tokens) raw[j] = load(ahead);
       step(ahead);
       store_quantised<T, D>(a, x, t, first + (is_k ? at.x : at.x - heads), is_k, c, live);
