@@ -65,7 +65,7 @@ struct __align__(16) SelectSmem {
   int sums[2][kWarps];
   int digit, left, in_bin;
   int newest, guarded, n_equal, kept, kept_below;   // of this CTA's slots, for the cluster
-  uint32_t keys[1];   // as many as the launch has room for
+  uint32_t keys[1];   // as many as the launch has room for, and (`both`) as many positions
 };
 
 // Sum of x over the CTA, and (before) over the threads before this one.  `turn` alternates
@@ -89,7 +89,7 @@ __device__ __noinline__ int block_sum(int x, int (&sums)[2][kWarps], int turn, i
 // rows of 32768 slots over eight CTAs each 14 us, of which the six cluster barriers take half;
 // for rows of 1060 slots 5 us.  Loops are rolled, with their loads in flight together: code that
 // runs once is waited for line by line.
-__device__ __forceinline__ void select_row(const Q4EvictArgs& a, int unit, int first, int n, int room, bool wide, SelectSmem& s) {
+__device__ __forceinline__ void select_row(const Q4EvictArgs& a, int unit, int first, int n, int room, bool both, bool wide, SelectSmem& s) {
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int me = wide ? (int)cluster.block_rank() : 0, ctas = wide ? (int)cluster.num_blocks() : 1;
@@ -100,6 +100,7 @@ __device__ __forceinline__ void select_row(const Q4EvictArgs& a, int unit, int f
   const float* weights = a.kv.weights + at;
   const int32_t* positions = a.kv.positions + at;
   const bool held = n <= room;
+  int32_t* held_positions = reinterpret_cast<int32_t*>(s.keys + room);   // (both)
   int turn = 0, before;
   // ---- keys, and the newest position.  NaN is the greatest weight: 0xfffffffe.
   auto raw_key = [&](int i) { return min(weight_key(__ldg(weights + i)), 0xfffffffeu); };
@@ -117,7 +118,11 @@ __device__ __forceinline__ void select_row(const Q4EvictArgs& a, int unit, int f
 #pragma unroll
     for (int j = 0; j < kAtOnce; ++j) {
       newest = max(newest, p[j]);
-      if (held && i0 + j * kThreads < n) s.keys[i0 + j * kThreads] = min(weight_key(w[j]), 0xfffffffeu);
+      const int i = i0 + j * kThreads;
+      if (held && i < n) {
+        s.keys[i] = min(weight_key(w[j]), 0xfffffffeu);
+        if (both) held_positions[i] = p[j];
+      }
     }
   }
   newest = __reduce_max_sync(0xffffffffu, newest);
@@ -138,7 +143,10 @@ __device__ __forceinline__ void select_row(const Q4EvictArgs& a, int unit, int f
   for (int i0 = tid; i0 < n; i0 += kAtOnce * kThreads) {
     int p[kAtOnce];
 #pragma unroll
-    for (int j = 0; j < kAtOnce; ++j) p[j] = __ldg(positions + min(i0 + j * kThreads, n - 1));
+    for (int j = 0; j < kAtOnce; ++j) {
+      const int i = min(i0 + j * kThreads, n - 1);
+      p[j] = held && both ? held_positions[i] : __ldg(positions + i);
+    }
 #pragma unroll
     for (int j = 0; j < kAtOnce; ++j) {
       const bool g = i0 + j * kThreads < n && guards(p[j]);
@@ -283,7 +291,7 @@ __device__ __forceinline__ void select_row(const Q4EvictArgs& a, int unit, int f
   if (wide) cluster.sync();   // what others may still read is there until then
 }
 
-__global__ void __launch_bounds__(kThreads, 2) k_evict_select(const __grid_constant__ Q4EvictArgs a, int ctas, int room) {
+__global__ void __launch_bounds__(kThreads, 2) k_evict_select(const __grid_constant__ Q4EvictArgs a, int ctas, int room, bool both) {
   extern __shared__ __align__(16) uint8_t smem[];
   SelectSmem& s = *reinterpret_cast<SelectSmem*>(smem);
   const int K = a.kv.n_kv_heads, unit = blockIdx.x / ctas, me = blockIdx.x - unit * ctas, seq = unit / K, tid = threadIdx.x;
@@ -302,14 +310,15 @@ __global__ void __launch_bounds__(kThreads, 2) k_evict_select(const __grid_const
   }
   // whole words of bits to each CTA
   const int share = (((int)len + ctas - 1) / ctas + 31) / 32 * 32, first = me * share;
-  select_row(a, unit, first, max(0, min(share, (int)len - first)), room, ctas > 1, s);
+  select_row(a, unit, first, max(0, min(share, (int)len - first)), room, both, ctas > 1, s);
 }
 
 // D / 8 lanes a pair: 16 bytes of codes of each group of K and of V, then their parameters.
+// A row is 1.25 D bytes in D / 8 sectors of 32, so that scattered ones cost twice that.
 constexpr int kMoveThreads = 256;
 template <int D>
 __global__ void __launch_bounds__(kMoveThreads) k_evict_move(const __grid_constant__ Q4EvictArgs a) {
-  constexpr int G = D / 32, NC = 4 * G, kPairs = kMoveThreads / NC;
+  constexpr int G = D / 32, NC = 4 * G, kPairs = kMoveThreads / NC, kAtOnce = 4;   // pairs of a thread in flight
   const int K = a.kv.n_kv_heads, unit = blockIdx.x, s = unit / K, h = unit - s * K, c = threadIdx.x % NC, P = a.kv.page_size;
   const Moves in = moves_of(a);
   pdl_wait();
@@ -317,21 +326,40 @@ __global__ void __launch_bounds__(kMoveThreads) k_evict_move(const __grid_consta
   if (blockIdx.y == 0 && threadIdx.x == 0 && h == 0 && in.length[s] >= 0) a.new_len[s] = (uint32_t)in.length[s];
   const int n = in.count[unit];
   const long long row = (long long)unit * q4_capacity(a.kv);
-  for (int i = blockIdx.y * kPairs + threadIdx.x / NC; i < n; i += gridDim.y * kPairs) {
-    const int2 p = in.pairs[(long long)unit * a.n_keep + i];
-    const int to = q4_page(a.kv, a.err, s, p.x >> a.page_shift), from = q4_page(a.kv, a.err, s, p.y >> a.page_shift);
-    if (c == 0) a.kv.weights[row + p.x] = a.kv.weights[row + p.y];
-    if (c == 1) a.kv.positions[row + p.x] = a.kv.positions[row + p.y];
-    if (to < 0 || from < 0) continue;
-    uint8_t* dst = q4_block<D>(a.kv, to, h, p.x & (P - 1));
-    const uint8_t* src = q4_block<D>(a.kv, from, h, p.y & (P - 1));
-    const int rd = p.x & 15, rs = p.y & 15;
-    if (c < 2 * G) {
-      *reinterpret_cast<uint4*>(dst + c * 256 + rd * 16) = *reinterpret_cast<const uint4*>(src + c * 256 + rs * 16);
-    } else {
-      const int g = c - 2 * G;
-      *reinterpret_cast<uint32_t*>(dst + Q4Block<D>::kKeySteps + g * 64 + rd * 4) =
-          *reinterpret_cast<const uint32_t*>(src + Q4Block<D>::kKeySteps + g * 64 + rs * 4);
+  // this lane's part of a slot in its block
+  const int part = c < 2 * G ? c * 256 : Q4Block<D>::kKeySteps + (c - 2 * G) * 64, step = c < 2 * G ? 16 : 4;
+  const int2* pairs = in.pairs + (long long)unit * a.n_keep;
+  for (int i0 = blockIdx.y * kPairs * kAtOnce + threadIdx.x / NC; i0 < n; i0 += gridDim.y * kPairs * kAtOnce) {
+    int2 p[kAtOnce];
+    int to[kAtOnce], from[kAtOnce];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) p[j] = pairs[min(i0 + j * kPairs, n - 1)];
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      to[j] = q4_page(a.kv, a.err, s, p[j].x >> a.page_shift);
+      from[j] = q4_page(a.kv, a.err, s, p[j].y >> a.page_shift);
+    }
+    uint4 x[kAtOnce];
+    uint32_t kept[kAtOnce];
+    const uint32_t* slots = reinterpret_cast<const uint32_t*>(c ? (const void*)a.kv.positions : (const void*)a.kv.weights) + row;
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      if (i0 + j * kPairs >= n) to[j] = -2;
+      if (c < 2) kept[j] = slots[p[j].y];
+      if (to[j] >= 0 && from[j] >= 0) {
+        const uint8_t* src = q4_block<D>(a.kv, from[j], h, p[j].y & (P - 1)) + part + (p[j].y & 15) * step;
+        if (c < 2 * G) x[j] = *reinterpret_cast<const uint4*>(src);
+        else x[j].x = *reinterpret_cast<const uint32_t*>(src);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      if (to[j] == -2) continue;
+      if (c < 2) const_cast<uint32_t*>(slots)[p[j].x] = kept[j];
+      if (to[j] < 0 || from[j] < 0) continue;
+      uint8_t* dst = q4_block<D>(a.kv, to[j], h, p[j].x & (P - 1)) + part + (p[j].x & 15) * step;
+      if (c < 2 * G) *reinterpret_cast<uint4*>(dst) = x[j];
+      else *reinterpret_cast<uint32_t*>(dst) = x[j].x;
     }
   }
 }
@@ -361,17 +389,19 @@ int launch_evict_q4(const Q4EvictArgs& a, cudaStream_t st) {
   cfg.blockDim = dim3(kThreads);
   const long long share = ((long long)a.kv.max_pages * a.kv.page_size + cluster - 1) / cluster + 31;
   const int room = (int)std::min<long long>(kMaxHeld, share);
-  const int smem = (int)sizeof(SelectSmem) + 4 * room;
+  const bool both = 2 * room <= kMaxHeld;
+  const int smem = (int)sizeof(SelectSmem) + (both ? 8 : 4) * room;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 2 : 1;
   static OncePerDevice once;
   if (once.launch(reinterpret_cast<const void*>(k_evict_select), (int)sizeof(SelectSmem) + 4 * kMaxHeld,
-                  [&] { return cudaLaunchKernelEx(&cfg, k_evict_select, a, cluster, room); }) != cudaSuccess)
+                  [&] { return cudaLaunchKernelEx(&cfg, k_evict_select, a, cluster, room, both); }) != cudaSuccess)
     return -1;
   cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 1;
+  // (a round of pairs a CTA where there may be many, one pair a thread where few CTAs suffice)
   const int per_cta = kMoveThreads / ((int)a.kv.head_dim / 8);
   cfg.gridDim = dim3(units, std::max(1, std::min((a.n_keep + per_cta - 1) / per_cta, 8 * paged_sm_count() / units)));
   cfg.blockDim = dim3(kMoveThreads);
