@@ -164,11 +164,14 @@ __global__ void __launch_bounds__(kTokenThreads) k_append_token_q4(const __grid_
 }
 
 // Ragged tokens.  CTAs 0 .. kv_ctas - 1: keys and values of up to 4 kv heads of 8 tokens, D / 8
-// lanes a row; the rest: 8 query heads of 16 tokens (32 with head_dim 64), a thread 16
-// elements of a token's heads, as in k_append_rows.
-constexpr int kRowThreads = 128, kQHeads = 8, kKvTokens = 8, kKvHeads = 4;
+// lanes a row; the rest: 4 query heads of 16 tokens (32 with head_dim 64), a thread 16
+// elements of a token's heads, as in k_append_rows.  Both wait for memory and for one another's
+// steps more than they compute, so that CTAs on an SM count for more than what a thread has in
+// flight: 9632 tokens, 32 and 8 heads, pairs half a head apart: 8 CTAs with one row of a kv
+// CTA's thread and 4 query heads at a time 56 us, 4 CTAs with 4 and 8 79 us.
+constexpr int kRowThreads = 128, kRowCtasPerSm = 8, kQHeads = 4, kKvTokens = 8, kKvHeads = 4;
 template <typename T, int D, bool kInterleaved>
-__global__ void __launch_bounds__(kRowThreads, 4) k_append_rows_q4(const __grid_constant__ Q4AppendArgs a, int kv_ctas) {
+__global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) k_append_rows_q4(const __grid_constant__ Q4AppendArgs a, int kv_ctas) {
   __shared__ double2 rot[kKvTokens][D / 2];   // cos, sin
   __shared__ Token tok[kKvTokens];
   const int tid = threadIdx.x, lane = tid & 31, H = a.n_heads, K = a.kv.n_kv_heads, R = a.rot_dim, n_seq = a.kv.n_seq;
@@ -211,13 +214,12 @@ __global__ void __launch_bounds__(kRowThreads, 4) k_append_rows_q4(const __grid_
       }
     return;
   }
-  constexpr int NC = D / 8, kStep = kRowThreads / NC, kAtOnce = 4;   // rows of a thread in flight
+  constexpr int NC = D / 8, kStep = kRowThreads / NC;   // rows at once
   const int parts = (K + kKvHeads - 1) / kKvHeads, tile = blockIdx.x / parts;
   const int first = ((int)blockIdx.x - tile * parts) * kKvHeads, heads = min(kKvHeads, K - first);
   const int c = tid % NC, row0 = tile * kKvTokens, tokens = min(kKvTokens, a.n_tokens - row0);
   const int rows = tokens * 2 * heads;
-  // Row i is of token i / (2 heads), keys before values, so that a warp's two rows are alike;
-  // a thread's follow one another kStep apart.
+  // Row i is of token i / (2 heads), keys before values, so that a warp's two rows are alike.
   struct Row {
     int t, x;
   };
@@ -235,16 +237,11 @@ __global__ void __launch_bounds__(kRowThreads, 4) k_append_rows_q4(const __grid_
                ? load_raw<T, true>(reinterpret_cast<const T*>(a.v) + (row0 + r.t) * a.v_stride + (first + r.x - heads) * D, c, R, false)
                : load_raw<T, kInterleaved>(reinterpret_cast<const T*>(a.k) + (row0 + r.t) * a.k_stride + (first + r.x) * D, c, R, 8 * c < R);
   };
-  Row at, ahead;
+  Row at;
   at.t = tid / NC / per;
   at.x = tid / NC - at.t * per;
-  ahead = at;
-  Raw raw[kAtOnce];
-#pragma unroll
-  for (int j = 0; j < kAtOnce; ++j) {
-    if (ahead.t < tokens) raw[j] = load(ahead);
-    step(ahead);
-  }
+  Raw next{};
+  if (at.t < tokens) next = load(at);
   if (tid < 32) {
     const int t = lane / (32 / kKvTokens), row = row0 + t;
     const int s = seq_of<32 / kKvTokens>(a.cu_tokens, n_seq, 0, 0, row, lane);
@@ -272,19 +269,16 @@ __global__ void __launch_bounds__(kRowThreads, 4) k_append_rows_q4(const __grid_
     if (tok[i / heads].seq >= 0) keep_slot(a, tok[i / heads], first + i % heads, row0 + i / heads);
   __syncthreads();
 #pragma unroll 1
-  for (int base = 0; base < rows; base += kAtOnce * kStep) {   // (the warp's lanes stay together)
-#pragma unroll
-    for (int j = 0; j < kAtOnce; ++j) {
-      if (base + j * kStep >= rows) break;
-      const Token& t = tok[min(at.t, tokens - 1)];
-      const bool is_k = at.x < heads, live = at.t < tokens;
-      uint4 x = raw[j].own;
-      if (is_k && live && t.seq >= 0 && 8 * c < R) x = rotate_raw<double, T, D, kInterleaved>(raw[j], rot[at.t], c, R);
-      if (ahead.t < tokens) raw[j] = load(ahead);
-      step(ahead);
-      store_quantised<T, D>(a, x, t, first + (is_k ? at.x : at.x - heads), is_k, c, live);
-      step(at);
-    }
+  for (int base = 0; base < rows; base += kStep) {   // (the warp's lanes stay together)
+    const Row now = at;
+    const Raw raw = next;
+    step(at);
+    if (at.t < tokens) next = load(at);
+    const Token& t = tok[min(now.t, tokens - 1)];
+    const bool is_k = now.x < heads, live = now.t < tokens;
+    uint4 x = raw.own;
+    if (is_k && live && t.seq >= 0 && 8 * c < R) x = rotate_raw<double, T, D, kInterleaved>(raw, rot[now.t], c, R);
+    store_quantised<T, D>(a, x, t, first + (is_k ? now.x : now.x - heads), is_k, c, live);
   }
 }
 
