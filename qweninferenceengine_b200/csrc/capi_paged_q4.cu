@@ -77,13 +77,14 @@ int qwen_rope_append_paged_q4(const qwen_paged_kv_q4* kv, const uint16_t* q, int
   if (rot_dim == 0 || rot_dim % 16 != 0 || rot_dim > kv->head_dim)
     return set_error(QWEN_ERR_INVALID_ARGUMENT, "%s: rot_dim=%u must be a multiple of 16, at most %u", op,
                      rot_dim, kv->head_dim);
-  if (n_tokens > (1u << 24)) return set_error(QWEN_ERR_INVALID_ARGUMENT, "%s: n_tokens=%u", op, n_tokens);
+  if (n_tokens > (1u << 24) || (uint64_t)n_tokens * (n_heads + kv->n_kv_heads) >= (1ull << 33))   // (blocks of the grid)
+    return set_error(QWEN_ERR_INVALID_ARGUMENT, "%s: n_tokens=%u of %u heads are more than one call takes", op, n_tokens,
+                     n_heads);
   if (n_axes == 0 || n_axes > 4 || (n_axes > 1 && (!positions || !pair_axis)))
     return set_error(QWEN_ERR_INVALID_ARGUMENT,
                      "%s: n_axes=%u must be 1 to 4, with positions and pair_axis where it is over 1", op, n_axes);
-  if (n_axes > 1 && (position_stride < (int64_t)n_tokens || position_stride >= (1ll << 38)))
-    return set_error(QWEN_ERR_INVALID_ARGUMENT, "%s: position_stride=%lld for %u tokens", op,
-                     (long long)position_stride, n_tokens);
+  if (n_axes > 1 && (position_stride < 0 || position_stride >= (1ll << 38)))
+    return set_error(QWEN_ERR_INVALID_ARGUMENT, "%s: position_stride=%lld", op, (long long)position_stride);
   a.kv = *kv;
   a.q = q;
   a.k = k;

@@ -33,15 +33,21 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 // What the first kernel leaves for the second, per (sequence, kv head): pairs of slots,
 // (where to, where from), and their number; per sequence its new length or -1.
 struct Moves {
-  int2* pairs;    // [units][n_keep]
+  int2* pairs;     // [units][most]
   int* count;
   int* length;
+  long long most;  // of a unit: as many as are kept or as are not, whichever are fewer
 };
+__host__ __device__ inline long long most_moves(const qwen_paged_kv_q4& kv, long long n_keep) {
+  const long long rest = (long long)kv.max_pages * kv.page_size - n_keep;
+  return rest < 0 ? 0 : rest < n_keep ? rest : n_keep;
+}
 __host__ __device__ inline Moves moves_of(const Q4EvictArgs& a) {
   const size_t units = (size_t)a.kv.n_seq * a.kv.n_kv_heads;
   Moves m;
+  m.most = most_moves(a.kv, a.n_keep);
   m.pairs = static_cast<int2*>(a.workspace);
-  m.count = reinterpret_cast<int*>(m.pairs + units * a.n_keep);
+  m.count = reinterpret_cast<int*>(m.pairs + units * m.most);
   m.length = m.count + units;
   return m;
 }
@@ -269,7 +275,7 @@ __device__ __forceinline__ void select_row(const Q4EvictArgs& a, int unit, int f
     offset = sum_of(&s.kept, me);
   }
   // ---- in slot order the holes below n_keep and what comes into them
-  int2* pairs = moves_of(a).pairs + (long long)unit * a.n_keep;
+  int2* pairs = moves_of(a).pairs + unit * moves_of(a).most;
   const int below = kept_below;
   seen = equal_before;
   kept = 0;
@@ -328,7 +334,7 @@ __global__ void __launch_bounds__(kMoveThreads) k_evict_move(const __grid_consta
   const long long row = (long long)unit * q4_capacity(a.kv);
   // this lane's part of a slot in its block
   const int part = c < 2 * G ? c * 256 : Q4Block<D>::kKeySteps + (c - 2 * G) * 64, step = c < 2 * G ? 16 : 4;
-  const int2* pairs = in.pairs + (long long)unit * a.n_keep;
+  const int2* pairs = in.pairs + unit * in.most;
   for (int i0 = blockIdx.y * kPairs * kAtOnce + threadIdx.x / NC; i0 < n; i0 += gridDim.y * kPairs * kAtOnce) {
     int2 p[kAtOnce];
     int to[kAtOnce], from[kAtOnce];
@@ -368,7 +374,7 @@ __global__ void __launch_bounds__(kMoveThreads) k_evict_move(const __grid_consta
 
 size_t evict_q4_workspace(const qwen_paged_kv_q4& kv, uint32_t n_keep) {
   const size_t units = (size_t)kv.n_seq * kv.n_kv_heads;
-  return units * n_keep * sizeof(int2) + (units + kv.n_seq) * sizeof(int);
+  return units * most_moves(kv, n_keep) * sizeof(int2) + (units + kv.n_seq) * sizeof(int);
 }
 
 int launch_evict_q4(const Q4EvictArgs& a, cudaStream_t st) {

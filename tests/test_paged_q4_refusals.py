@@ -92,8 +92,10 @@ def test_append_arguments():
     refused(append, kv(), "n_axes", axes=5, which=A)
     refused(append, kv(), "n_axes", axes=2)
     refused(append, kv(), "n_axes", axes=2, which=A, pos=None)
-    refused(append, kv(), "position_stride", axes=2, which=A, ps=2)
     refused(append, kv(), "position_stride", axes=2, which=A, ps=-8)
+    refused(append, kv(), "position_stride", axes=2, which=A, ps=1 << 38)
+    refused(append, kv(n_kv_heads=1024), "n_tokens", heads=1024, qs=1 << 17, os=1 << 17, ks=1 << 17, vs=1 << 17,
+            n=1 << 23, cu=A)
 
 
 def test_attention_arguments():
