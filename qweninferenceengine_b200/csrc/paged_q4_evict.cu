@@ -55,6 +55,7 @@ __host__ __device__ inline Moves moves_of(const Q4EvictArgs& a) {
 constexpr int kMaxHeld = 16384;              // slots whose keys a CTA holds in shared memory at most
 constexpr int kTile = 32 * kThreads;         // slots numbered at once: a word of bits a thread
 constexpr int kMaxCluster = 8;
+constexpr int kAllBins = 2 * kBins + kBins / 2;   // of digits of 11, 11 and 10 bits
 
 // Bits of a tile's slots, and how many are set in the words before.
 struct Bits {
@@ -65,13 +66,18 @@ struct Bits {
   }
 };
 struct __align__(16) SelectSmem {
-  int bins[3][kBins];   // a histogram for each digit
-  int all[3][kBins];    // the cluster's, in its first CTA
+  union {
+    struct {
+      int bins[kAllBins];   // a histogram for each digit
+      int all[kAllBins];    // the cluster's, in its first CTA
+    };
+    int32_t positions[2 * kAllBins];   // before
+  };
   Bits equal, stay;
   int sums[2][kWarps];
   int digit, left, in_bin;
   int newest, guarded, n_equal, kept, kept_below;   // of this CTA's slots, for the cluster
-  uint32_t keys[1];   // as many as the launch has room for, and (`both`) as many positions
+  uint32_t keys[1];   // as many as the launch has room for
 };
 
 // Sum of x over the CTA, and (before) over the threads before this one.  `turn` alternates
@@ -95,7 +101,7 @@ __device__ __noinline__ int block_sum(int x, int (&sums)[2][kWarps], int turn, i
 // rows of 32768 slots over eight CTAs each 14 us, of which the six cluster barriers take half;
 // for rows of 1060 slots 5 us.  Loops are rolled, with their loads in flight together: code that
 // runs once is waited for line by line.
-__device__ __forceinline__ void select_row(const Q4EvictArgs& a, int unit, int first, int n, int room, bool both, bool wide, SelectSmem& s) {
+__device__ __forceinline__ void select_row(const Q4EvictArgs& a, int unit, int first, int n, int room, bool wide, SelectSmem& s) {
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int me = wide ? (int)cluster.block_rank() : 0, ctas = wide ? (int)cluster.num_blocks() : 1;
@@ -105,8 +111,7 @@ __device__ __forceinline__ void select_row(const Q4EvictArgs& a, int unit, int f
   const long long at = (long long)unit * q4_capacity(a.kv) + first;
   const float* weights = a.kv.weights + at;
   const int32_t* positions = a.kv.positions + at;
-  const bool held = n <= room;
-  int32_t* held_positions = reinterpret_cast<int32_t*>(s.keys + room);   // (both)
+  const bool held = n <= room, held_positions = n <= 2 * kAllBins;
   int turn = 0, before;
   // ---- keys, and the newest position.  NaN is the greatest weight: 0xfffffffe.
   auto raw_key = [&](int i) { return min(weight_key(__ldg(weights + i)), 0xfffffffeu); };
@@ -125,15 +130,12 @@ __device__ __forceinline__ void select_row(const Q4EvictArgs& a, int unit, int f
     for (int j = 0; j < kAtOnce; ++j) {
       newest = max(newest, p[j]);
       const int i = i0 + j * kThreads;
-      if (held && i < n) {
-        s.keys[i] = min(weight_key(w[j]), 0xfffffffeu);
-        if (both) held_positions[i] = p[j];
-      }
+      if (held && i < n) s.keys[i] = min(weight_key(w[j]), 0xfffffffeu);
+      if (held_positions && i < n) s.positions[i] = p[j];
     }
   }
   newest = __reduce_max_sync(0xffffffffu, newest);
   if (lane == 0) s.sums[1][warp] = newest;
-  for (int i = tid; i < 2 * 3 * kBins / 4; i += kThreads) reinterpret_cast<int4*>(s.bins[0])[i] = make_int4(0, 0, 0, 0);
   __syncthreads();
   newest = __reduce_max_sync(0xffffffffu, s.sums[1][lane % kWarps]);
   if (wide) {
@@ -151,7 +153,7 @@ __device__ __forceinline__ void select_row(const Q4EvictArgs& a, int unit, int f
 #pragma unroll
     for (int j = 0; j < kAtOnce; ++j) {
       const int i = min(i0 + j * kThreads, n - 1);
-      p[j] = held && both ? held_positions[i] : __ldg(positions + i);
+      p[j] = held_positions ? s.positions[i] : __ldg(positions + i);
     }
 #pragma unroll
     for (int j = 0; j < kAtOnce; ++j) {
@@ -161,10 +163,13 @@ __device__ __forceinline__ void select_row(const Q4EvictArgs& a, int unit, int f
     }
   }
   count = block_sum(count, s.sums, turn++, &before);
+  for (int i = tid; i < 2 * kAllBins / 4; i += kThreads) reinterpret_cast<int4*>(s.bins)[i] = make_int4(0, 0, 0, 0);
   if (wide) {
     if (tid == 0) s.guarded = count;
     cluster.sync();
     count = sum_of(&s.guarded, ctas);
+  } else {
+    __syncthreads();
   }
   // Of the class that is cut (the guarded, if there are more than n_keep, else the others) the
   // rank-th greatest key is looked for; `pass_over` is the key of the other class.
@@ -183,23 +188,25 @@ __device__ __forceinline__ void select_row(const Q4EvictArgs& a, int unit, int f
     for (int pass = 0; pass < 3; ++pass) {
       const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
       const uint32_t digits = pass == 2 ? 1023 : 2047;
-      int* bins = s.bins[pass];
+      int* bins = s.bins + pass * kBins;
 #pragma unroll 4
       for (int i = tid; i < n; i += kThreads) {
         const uint32_t k = key_of(i);
         if (k != pass_over && (k & mask) == key) atomicAdd(&bins[k >> shift & digits], 1);
       }
       __syncthreads();
-      // thread i has bins 2044 - 4i .. 2047 - 4i, the greatest first; the first CTA adds up all's
-      int4 b = *reinterpret_cast<const int4*>(bins + kBins - 4 - 4 * tid);
+      // thread i has bins 4i .. 4i + 3 from the greatest down; the first CTA adds up all's
+      const int top = kBins - 4 - 4 * tid - (pass == 2 ? kBins / 2 : 0);   // (below 0: none)
+      int4 b = make_int4(0, 0, 0, 0);
+      if (top >= 0) b = *reinterpret_cast<const int4*>(bins + top);
       if (wide) {
-        int* to = cluster.map_shared_rank(s.all[pass], 0) + kBins - 4 - 4 * tid;
+        int* to = cluster.map_shared_rank(s.all + pass * kBins, 0) + top;
         if (b.x) atomicAdd(to, b.x);
         if (b.y) atomicAdd(to + 1, b.y);
         if (b.z) atomicAdd(to + 2, b.z);
         if (b.w) atomicAdd(to + 3, b.w);
         cluster.sync();
-        b = *reinterpret_cast<const int4*>(to);
+        if (top >= 0) b = *reinterpret_cast<const int4*>(to);
       }
       const int here = b.x + b.y + b.z + b.w;
       block_sum(here, s.sums, turn++, &before);
@@ -212,7 +219,7 @@ __device__ __forceinline__ void select_row(const Q4EvictArgs& a, int unit, int f
             left -= in[i];
             ++j;
           }
-        s.digit = kBins - 1 - 4 * tid - j;
+        s.digit = top + 3 - j;
         s.left = left;
         s.in_bin = in[j];
       }
@@ -297,7 +304,7 @@ __device__ __forceinline__ void select_row(const Q4EvictArgs& a, int unit, int f
   if (wide) cluster.sync();   // what others may still read is there until then
 }
 
-__global__ void __launch_bounds__(kThreads, 2) k_evict_select(const __grid_constant__ Q4EvictArgs a, int ctas, int room, bool both) {
+__global__ void __launch_bounds__(kThreads, 2) k_evict_select(const __grid_constant__ Q4EvictArgs a, int ctas, int room) {
   extern __shared__ __align__(16) uint8_t smem[];
   SelectSmem& s = *reinterpret_cast<SelectSmem*>(smem);
   const int K = a.kv.n_kv_heads, unit = blockIdx.x / ctas, me = blockIdx.x - unit * ctas, seq = unit / K, tid = threadIdx.x;
@@ -316,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_evict_select(const __grid_const
   }
   // whole words of bits to each CTA
   const int share = (((int)len + ctas - 1) / ctas + 31) / 32 * 32, first = me * share;
-  select_row(a, unit, first, max(0, min(share, (int)len - first)), room, both, ctas > 1, s);
+  select_row(a, unit, first, max(0, min(share, (int)len - first)), room, ctas > 1, s);
 }
 
 // D / 8 lanes a pair: 16 bytes of codes of each group of K and of V, then their parameters.
@@ -395,15 +402,15 @@ int launch_evict_q4(const Q4EvictArgs& a, cudaStream_t st) {
   cfg.blockDim = dim3(kThreads);
   const long long share = ((long long)a.kv.max_pages * a.kv.page_size + cluster - 1) / cluster + 31;
   const int room = (int)std::min<long long>(kMaxHeld, share);
-  const bool both = 2 * room <= kMaxHeld;
-  const int smem = (int)sizeof(SelectSmem) + (both ? 8 : 4) * room;
+  const int smem = (int)sizeof(SelectSmem) + 4 * room;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 2 : 1;
+  static_assert(2 * (sizeof(SelectSmem) + 4 * kMaxHeld + 1024) <= 228 * 1024, "two CTAs an SM");
   static OncePerDevice once;
   if (once.launch(reinterpret_cast<const void*>(k_evict_select), (int)sizeof(SelectSmem) + 4 * kMaxHeld,
-                  [&] { return cudaLaunchKernelEx(&cfg, k_evict_select, a, cluster, room, both); }) != cudaSuccess)
+                  [&] { return cudaLaunchKernelEx(&cfg, k_evict_select, a, cluster, room); }) != cudaSuccess)
     return -1;
   cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 1;

@@ -10,8 +10,7 @@ from ctypes import byref
 
 import torch
 
-from ._lib import (QWEN_DTYPE_BF16, QWEN_DTYPE_F16, PagedKVQ4Struct, PagedKVStruct, check,
-                   lib)
+from ._lib import QWEN_DTYPE_BF16, QWEN_DTYPE_F16, PagedKVStruct, check, lib
 
 HIDDEN, INTER, HEADS, KV_DIM, HEAD_DIM = 1536, 8960, 12, 256, 128
 VOCAB, ACTUAL_VOCAB = 151936, 151666
@@ -441,7 +440,7 @@ class PagedKVQ4:
     addresses must not change."""
 
     __slots__ = ("pool", "page_table", "weights", "positions", "dtype", "device", "index", "n_seq",
-                 "n_kv_heads", "head_dim", "page_size", "sizes", "ref", "_struct")
+                 "n_kv_heads", "head_dim", "page_size", "sizes", "ref")
 
     @staticmethod
     def pool_shape(n_pages: int, n_kv_heads: int, page_size: int, head_dim: int) -> tuple:
@@ -479,13 +478,12 @@ class PagedKVQ4:
         # (what workspaces go by: their slots, and whether scores are kept)
         self.sizes = (index, n_seq, n_kv, width, kept[2], weights is not None)
         # the stride of an axis of one element is never used: any valid value
-        self._struct = PagedKVQ4Struct.from_buffer_copy(_PAGED_KV_Q4.pack(
+        self.ref = _PAGED_KV_Q4.pack(
             pool.data_ptr(), 0 if weights is None else weights.data_ptr(),
             0 if positions is None else positions.data_ptr(), page_table.data_ptr(),
             st[0] if n_pages > 1 else n_kv * blocks * width, st[1] if n_kv > 1 else blocks * width,
             n_pages, 16 * blocks, n_kv, width // 20, n_seq, max_pages,
-            table_st[0] if n_seq > 1 else max_pages, _DTYPES[dtype]))
-        self.ref = byref(self._struct)
+            table_st[0] if n_seq > 1 else max_pages, _DTYPES[dtype])
 
 
 def rope_append_paged_q4(kv: PagedKVQ4, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,

@@ -235,8 +235,8 @@ def test_the_library_reads_a_plain_structure():
     from qweninferenceengine_b200._lib import PagedKVQ4Struct
 
     c = ref.Cache(13, [20], 4, 2, 64, 32, BF16, kept=True, head_gap=1)
-    s = c.handle()._struct
-    assert ctypes.sizeof(PagedKVQ4Struct) == 80
+    s = PagedKVQ4Struct.from_buffer_copy(c.handle().ref)
+    assert ctypes.sizeof(PagedKVQ4Struct) == 80 == len(c.handle().ref)
     assert (s.pool, s.weights, s.positions, s.page_table) == tuple(
         x.data_ptr() for x in (c.pool, c.weights, c.positions, c.table))
     assert (s.page_stride, s.head_stride) == (3 * 2 * 1280, 2 * 1280)
