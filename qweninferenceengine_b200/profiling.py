@@ -24,6 +24,13 @@
         attention_sparse_paged, --reps times; prints each operator's device time and
         is the workload for ncu captures of k_append, k_paged_decode, k_prefix and k_page.
 
+    python -m qweninferenceengine_b200.profiling paged-q4 [--batch 64] [--ctx 2000] [--page 64]
+                                                          [--keep 1024]
+        The same over a cache held in 4 bits: rope_append_paged_q4 (single tokens and
+        whole prompts), attention_paged_q4 without and with weights, evict_paged_q4 and
+        expand_paged_q4; the workload for captures of k_append_.._q4, k_q4, k_evict and
+        k_expand.
+
     python -m qweninferenceengine_b200.profiling tcstep [--batch 64] [--ctx 1024]
         The batched tensor-core step: prefill, then --reps eagerly launched steps
         with an event after every kernel (qwen_engine_profile_step); prints the
@@ -100,6 +107,50 @@ def run_paged(batch: int, ctx: int, page: int, prefix: int, select: int, reps: i
         "select_pages": lambda: ops.select_pages(kv, q, seq_len, select, out=pages),
         "attention_sparse_paged": lambda: ops.attention_sparse_paged(kv, q, seq_len, pages),
     }
+    _time_calls(calls, reps)
+
+
+def run_paged_q4(batch: int, ctx: int, page: int, keep: int, reps: int) -> None:
+    import torch
+
+    from . import ops
+
+    heads, kv_heads, dim = ops.HEADS, ops.KV_DIM // ops.HEAD_DIM, ops.HEAD_DIM
+    width = -(-ctx // page)
+    pool = torch.empty(ops.PagedKVQ4.pool_shape(batch * width, kv_heads, page, dim), dtype=torch.uint8,
+                       device="cuda")
+    table = torch.randperm(batch * width, device="cuda").to(torch.int32).view(batch, width)
+    weights = torch.zeros((batch, kv_heads, width * page), device="cuda")
+    positions = torch.zeros((batch, kv_heads, width * page), dtype=torch.int32, device="cuda")
+    kv = ops.PagedKVQ4(pool, table, torch.float16, weights, positions)
+    plain = ops.PagedKVQ4(pool, table, torch.float16)
+    seq_len = torch.full((batch,), ctx, dtype=torch.int32, device="cuda")
+    inv_freq = 1e6 ** (-torch.arange(0, dim, 2, device="cuda", dtype=torch.float32) / dim)
+    rows = torch.randn((batch * ctx, heads + 2 * kv_heads, dim), device="cuda").half()
+    cu = torch.arange(0, batch * ctx + 1, ctx, device="cuda").to(torch.int32)
+
+    def append(x, **more):
+        return ops.rope_append_paged_q4(kv, x[:, :heads], x[:, heads:heads + kv_heads], x[:, heads + kv_heads:],
+                                        seq_len, inv_freq, **more)
+
+    append(rows, cu_tokens=cu)
+    q = append(rows[:batch])
+    weights.uniform_()
+    lens, cu_keep = seq_len.clone(), torch.arange(0, batch * keep + 1, keep, device="cuda").to(torch.int32)
+    calls = {
+        "rope_append_paged_q4": lambda: append(rows[:batch], out=q),
+        "  of whole prompts": lambda: append(rows, cu_tokens=cu),
+        "attention_paged_q4": lambda: ops.attention_paged_q4(plain, q, seq_len),
+        "  with weights": lambda: ops.attention_paged_q4(kv, q, seq_len),
+        "evict_paged_q4": lambda: ops.evict_paged_q4(kv, seq_len, keep, out=lens),
+        "expand_paged_q4": lambda: ops.expand_paged_q4(kv, lens, cu_keep, n_rows=batch * keep),
+    }
+    _time_calls(calls, reps)
+
+
+def _time_calls(calls: dict, reps: int) -> None:
+    import torch
+
     flush = torch.empty(256 << 20, dtype=torch.uint8, device="cuda")
     for name, call in calls.items():
         times = []
@@ -215,6 +266,9 @@ def main() -> None:
     for name, default in (("batch", 64), ("ctx", 2000), ("page", 64), ("prefix", 8192), ("select", 16),
                           ("reps", 5)):
         pg.add_argument("--" + name, type=int, default=default)
+    p4 = sub.add_parser("paged-q4")
+    for name, default in (("batch", 64), ("ctx", 2000), ("page", 64), ("keep", 1024), ("reps", 5)):
+        p4.add_argument("--" + name, type=int, default=default)
     ts = sub.add_parser("tcstep")
     ts.add_argument("--batch", type=int, default=64)
     ts.add_argument("--ctx", type=int, default=1024)
@@ -244,6 +298,9 @@ def main() -> None:
         return
     if a.cmd == "paged":
         run_paged(a.batch, a.ctx, a.page, a.prefix, a.select, a.reps)
+        return
+    if a.cmd == "paged-q4":
+        run_paged_q4(a.batch, a.ctx, a.page, a.keep, a.reps)
         return
     if a.cmd == "attention":
         run_attention(a.batch, a.ctx, a.reps)

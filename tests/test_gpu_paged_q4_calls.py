@@ -242,3 +242,12 @@ def test_the_library_reads_a_plain_structure():
     assert (s.page_stride, s.head_stride) == (3 * 2 * 1280, 2 * 1280)
     assert (s.n_pages, s.page_size, s.n_kv_heads, s.head_dim, s.n_seq, s.max_pages, s.table_stride, s.dtype) == (
         c.n_pages, 32, 2, 64, 1, 1, 1, 1)
+
+
+def test_profiling_command_runs_them(capsys):
+    from qweninferenceengine_b200.profiling import run_paged_q4
+
+    run_paged_q4(3, 200, 16, 64, 2)
+    out = capsys.readouterr().out
+    for name in ("rope_append_paged_q4", "attention_paged_q4", "with weights", "evict_paged_q4", "expand_paged_q4"):
+        assert name in out
