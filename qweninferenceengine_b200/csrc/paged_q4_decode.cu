@@ -26,6 +26,14 @@
 // size is in range; 16 or 128 sum_t step P is taken off at the end.  The two sums of P with lows and with steps are
 // one MMA over the slots, q's group sums with lows another (three terms of 8 or 11 bits).
 // Weights step P are two bf16 values (16 bits).  Sums, maxima and outputs are fp32.
+//
+// Measured: 32 sequences of 16384 slots, 32 and 8 heads of 128, bf16: 150 us (4.5 TB/s), fp16
+// 167; their 671 MB take 102, and the kernel 106 without its arithmetic, of which the values'
+// dequantisation is 13 and the keys' 6 (a block takes a warp ~340 instructions; the schedulers
+// issue 55% of the time, the integer pipe is busy for 48%, the tensor pipe for 34%).  A call of
+// 512 slots takes 8.4, 64 sequences of 512 .. 2048 slots and 2 kv heads 15.9 (their bytes 3.8):
+// launch, lengths, page numbers, first tile, join.  Warps that load their own blocks, sixteen an
+// SM without producers, took 172 in place of 150.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>

@@ -1,13 +1,15 @@
 // paged_q4_evict.cu -- cuts the sequences of a 4-bit paged cache to a budget: of each
 // (sequence, kv head) the n_keep slots stay that come first by (guarded, weight, slot).
 //
-// Two launches.  k_evict_select, a CTA or a cluster per (sequence, kv head): weights and positions are
-// read into shared memory as ordered keys (up to 16384 slots a CTA; longer rows are read again
-// from L2), the n_keep-th weight is found digit by digit (11, 11 and 10 bits, a histogram in
-// shared memory each), and the slots that go and those that come are numbered in slot order.
-// Few long rows are divided among the CTAs of a cluster, which add up their histograms.  k_evict_move copies the rows, as many CTAs as fill the GPU.  Nothing a row
-// is copied from is written, so the copies need no order, and what stays below n_keep is not
-// touched: a sequence one token over its budget moves one row.
+// Two launches.  k_evict_select, a CTA or a cluster per (sequence, kv head): weights and
+// positions are read into shared memory as ordered keys (up to 16384 slots a CTA; longer rows
+// are read again from L2), the n_keep-th weight is found digit by digit (11, 11 and 10 bits, a
+// histogram in shared memory each), and the slots that go and those that come are numbered in
+// slot order.
+// Few long rows are divided among the CTAs of a cluster, which add up their histograms.
+// k_evict_move copies the rows, as many CTAs as fill the GPU.  Nothing a row is copied from is
+// written, so the copies need no order, and what stays below n_keep is not touched: a sequence
+// one token over its budget moves one row.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -98,9 +100,9 @@ __device__ __noinline__ int block_sum(int x, int (&sums)[2][kWarps], int turn, i
 }
 
 // One (sequence, kv head) by the CTAs of a cluster, or by one.  Latency throughout: for two
-// rows of 32768 slots over eight CTAs each 14 us, of which the six cluster barriers take half;
-// for rows of 1060 slots 5 us.  Loops are rolled, with their loads in flight together: code that
-// runs once is waited for line by line.
+// rows of 32768 slots over eight CTAs each 15 us, of which the six cluster barriers take half;
+// for 128 rows of 1060 slots 6 us, of 16384 slots 21.  Loops are rolled, with their loads in
+// flight together: code that runs once is waited for line by line.
 __device__ __forceinline__ void select_row(const Q4EvictArgs& a, int unit, int first, int n, int room, bool wide, SelectSmem& s) {
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -327,7 +329,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_evict_select(const __grid_const
 }
 
 // D / 8 lanes a pair: 16 bytes of codes of each group of K and of V, then their parameters.
-// A row is 1.25 D bytes in D / 8 sectors of 32, so that scattered ones cost twice that.
+// A row is 1.25 D bytes in D / 8 sectors of 32, so that scattered ones cost three times that:
+// 229,000 pairs of 64-element heads 19 us.
 constexpr int kMoveThreads = 256;
 template <int D>
 __global__ void __launch_bounds__(kMoveThreads) k_evict_move(const __grid_constant__ Q4EvictArgs a) {
