@@ -79,11 +79,11 @@ __device__ __forceinline__ uint32_t most2(__nv_bfloat16, uint32_t a, uint32_t b)
 // .. 4i+3, and (step, low) as the cache keeps them.
 //
 // The least and the greatest are found in pairs, and exchanged as one word (least, -greatest).
-// The fp32 quotient is off by at most 15 (2^-24 + 2^-23 + 2^-24) < 4e-6 (difference,
-// reciprocal, product); where one stands nearer than 1e-5 to a border between two codes,
-// exact_code decides (of bf16's few values one in some hundred is on one).  Rounded by an
-// addition, and packed four at a time by multiplication: conversions run at an eighth of the
-// rate.
+// Quotients are formed in fixed point: 1.5 2^11 + (x - low) / step + 1/2 has steps of 2^-12, so
+// that one multiply-add leaves a code in bits 12 .. 15.  It is off by two roundings (that of
+// its constant, as |low / step| < 1000, and its own: one 2^-12) and 15.1 2^-23 from the
+// reciprocal, less than 1.01 2^-12 in all; where it stands within 2 2^-12 of a border between two
+// codes, exact_code decides (of bf16's few values one in some hundred is on one).
 template <typename T>
 __device__ __forceinline__ uint32_t quantise_group(const uint4& v, uint32_t* params) {
   const uint32_t a = least2(T{}, least2(T{}, v.x, v.y), least2(T{}, v.z, v.w));
@@ -102,26 +102,27 @@ __device__ __forceinline__ uint32_t quantise_group(const uint4& v, uint32_t* par
   const float x[8] = {v0.x, v0.y, v1.x, v1.y, v2.x, v2.y, v3.x, v3.y};
   // (a step far below its type's normal ones can be so much less than a fifteenth that quotients
   // pass 15.5; and see end_codes)
-  if (!((hi - lo) * inv < 15.4f))
+  if (!((hi - lo) * inv < 15.4f && fabsf(lo * inv) < 1000.f))
     return end_codes(make_float4(x[0], x[1], x[2], x[3]), make_float4(x[4], x[5], x[6], x[7]), lo, step);
-  constexpr float kMagic = 12582912.f;   // 1.5 2^23: sums are rounded to whole numbers, ties to even
-  float c[8], off = 0.f;
+  constexpr float kHalf = 1.5f * 2048.f + 0.5f + 2.f / 4096.f;   // (below a border: 0 or 1 2^-12, on it or above: 2 or 3)
+  const float from = fmaf(-lo, inv, kHalf);
+  uint32_t at[4];   // elements i and i + 4
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float t = (x[i] - lo) * inv;
-    c[i] = __fadd_rn(__fadd_rn(t, kMagic), -kMagic);
-    off = fmaxf(off, fabsf(t - c[i]));
-  }
-  if (off > 0.49999f) {
+  for (int i = 0; i < 4; ++i)
+    at[i] = __byte_perm(__float_as_uint(fmaf(x[i], inv, from)), __float_as_uint(fmaf(x[i + 4], inv, from)), 0x5410);
+  uint32_t codes = (at[0] >> 12 & 0x000f000fu) | (at[1] >> 8 & 0x00f000f0u) | (at[2] >> 4 & 0x0f000f00u) | (at[3] & 0xf000f000u);
+  uint32_t clear = 0x80008000u;   // bits 15: no quotient is near a border
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float t = (x[i] - lo) * inv;
-      if (fabsf(t - c[i]) > 0.49999f) c[i] = exact_code(x[i], lo, step, t, c[i]);
-    }
+  for (int i = 0; i < 4; ++i) clear &= (at[i] & 0x0ffc0ffcu) + 0x7fff7fffu;
+  if (clear != 0x80008000u) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if ((at[i & 3] >> (i < 4 ? 0 : 16) & 0xffcu) == 0) {
+        const float t = (x[i] - lo) * inv;
+        codes = (codes & ~(15u << (4 * i))) | (uint32_t)exact_code(x[i], lo, step, t, rintf(t)) << (4 * i);
+      }
   }
-  const float d = fmaf(c[3], 4096.f, fmaf(c[2], 256.f, fmaf(c[1], 16.f, c[0])));
-  const float e = fmaf(c[7], 4096.f, fmaf(c[6], 256.f, fmaf(c[5], 16.f, c[4])));
-  return __byte_perm(__float_as_uint(d + 8388608.f), __float_as_uint(e + 8388608.f), 0x5410);
+  return codes;
 }
 
 // Values low + code step of 8 codes in the cache's type, rounded once.  (1024 + code in fp16

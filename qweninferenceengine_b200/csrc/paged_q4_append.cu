@@ -6,9 +6,9 @@
 //
 // Keys are turned in 64 bits and rounded once, so that their codes are those of the formula;
 // queries, which keep 16 bits, in fp32 from angles formed in 64.  A decode step's tokens are
-// bound by latency (2.4 us for one, 3.1 for 64), prompts by instructions more than by HBM
-// (73% of issue slots, 44% of DRAM): 128,000 tokens of 12 and 2 heads, fp16, take 250 us where
-// their bytes take 146, 9600 of 32 and 8 heads, bf16, 53 for 32.
+// bound by latency (2.4 us for one, 3.1 for 64), prompts by instructions more than by HBM:
+// 52,600 tokens of 12 and 2 heads, fp16, take 93 us where their bytes take 60, 9600 of 32 and 8
+// heads, bf16, 48 for 32.
 #include <algorithm>
 
 #include "paged_q4.cuh"
@@ -86,19 +86,50 @@ __device__ __forceinline__ uint4 rotate_raw(const Raw& r, const double2* rot, in
   }
   return pack8<T>(x);
 }
-// Quantises lane c's 8 values of a key's or value's row and stores them (all 32 lanes; of
-// those whose token has a block, and not of others).
-template <typename T, int D>
-__device__ __forceinline__ void store_quantised(const Q4AppendArgs& a, const uint4& x, const Token& t, int h, bool is_k,
-                                                int c, bool live) {
+// Rotates 16 elements of a key, chunk c, in 64 bits.  Interleaved: elements 8 c .. 8 c + 7 and D / 2
+// + 8 c ..; else pairs 8 c .. 8 c + 7, the first of each in words 0 .. 3.
+template <typename T, int D, bool kInterleaved>
+__device__ __forceinline__ void rotate_key(Chunk& x, const double2* rot, int c, int R) {
+  if constexpr (kInterleaved) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int at = 8 * c + (i < 4 ? 0 : D / 2);
+      if (at >= R) continue;
+      const double2 cs = rot[rot_at<D, true>(at / 2 + i % 4)];
+      const float2 v = unpack2(T{}, x.w[i]);
+      const double a = v.x, b = v.y;
+      x.w[i] = pack2(T{}, (float)(a * cs.x + b * -cs.y), (float)(b * cs.x + a * cs.y));
+    }
+  } else if (16 * c < R) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const double2 r0 = rot[rot_at<D, false>(8 * c + 2 * i)], r1 = rot[rot_at<D, false>(8 * c + 2 * i + 1)];
+      const float2 v = unpack2(T{}, x.w[i]), u = unpack2(T{}, x.w[4 + i]);
+      const double a0 = v.x, a1 = v.y, b0 = u.x, b1 = u.y;
+      x.w[i] = pack2(T{}, (float)(a0 * r0.x + b0 * -r0.y), (float)(a1 * r1.x + b1 * -r1.y));
+      x.w[4 + i] = pack2(T{}, (float)(b0 * r0.x + a0 * r0.y), (float)(b1 * r1.x + a1 * r1.y));
+    }
+  }
+}
+// Quantises 8 values, a quarter of a group, whose others its neighbours have, and stores the codes
+// and (once a group) the parameters (all 32 lanes; of those that are live, and not of others).
+template <typename T>
+__device__ __forceinline__ void store_quantised(const uint4& x, uint8_t* codes_at, uint8_t* params_at, int quarter, bool live) {
   uint32_t params;
   const uint32_t codes = quantise_group<T>(x, &params);
-  if (!live || !t.block) return;
-  uint8_t* at = t.block + (long long)h * a.kv.head_stride;
-  const int g = c / 4, r = t.slot & 15;
-  *reinterpret_cast<uint32_t*>(at + (is_k ? 0 : Q4Block<D>::kValues) + g * 256 + r * 16 + (c & 3) * 4) = codes;
-  if ((c & 3) == 0)
-    *reinterpret_cast<uint32_t*>(at + (is_k ? Q4Block<D>::kKeySteps : Q4Block<D>::kValueSteps) + g * 64 + r * 4) = params;
+  if (!live) return;
+  *reinterpret_cast<uint32_t*>(codes_at) = codes;
+  if (quarter == 0) *reinterpret_cast<uint32_t*>(params_at) = params;
+}
+// Where a head's row of keys or values has the codes of lane c's 8 elements (of group c / 4),
+// and that group's parameters, in slot 0 of a block of head 0.
+template <int D>
+__device__ __forceinline__ long long codes_from(const Q4AppendArgs& a, int h, bool is_k, int c) {
+  return h * a.kv.head_stride + (is_k ? 0 : Q4Block<D>::kValues) + c / 4 * 256 + c % 4 * 4;
+}
+template <int D>
+__device__ __forceinline__ long long params_from(const Q4AppendArgs& a, int h, bool is_k, int c) {
+  return h * a.kv.head_stride + (is_k ? Q4Block<D>::kKeySteps : Q4Block<D>::kValueSteps) + c / 4 * 64;
 }
 __device__ __forceinline__ int axis_of(const Q4AppendArgs& a, int pair) {
   if (!a.pair_axis) return 0;
@@ -167,22 +198,28 @@ __global__ void __launch_bounds__(kTokenThreads) k_append_token_q4(const __grid_
       else x = rotate_raw<double, T, D, kInterleaved>(r, rot, c, R);
     }
     if (is_q) *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.q_out) + row * a.q_out_stride + head * D + 8 * c) = x;
-    if (__any_sync(0xffffffffu, live && !is_q))
-      store_quantised<T, D>(a, x, t, is_k ? head - H : head - H - K, is_k, c, live && !is_q);
+    if (__any_sync(0xffffffffu, live && !is_q)) {
+      const int h = is_k ? head - H : head - H - K, r = t.slot & 15;
+      store_quantised<T>(x, t.block + codes_from<D>(a, h, is_k, c) + r * 16, t.block + params_from<D>(a, h, is_k, c) + r * 4,
+                         c & 3, live && !is_q && t.block);
+    }
   }
 }
 
-// Ragged tokens.  CTAs 0 .. kv_ctas - 1: keys and values of up to 4 kv heads of 8 tokens, D / 8
+// Ragged tokens.  CTAs 0 .. kv_ctas - 1: keys and values of up to 4 kv heads of 8 tokens, D / 16
 // lanes a row; the rest: 4 query heads of 16 tokens (32 with head_dim 64), a thread 16
 // elements of a token's heads, as in k_append_rows.  Both wait for memory and for one another's
 // steps more than they compute, so that CTAs on an SM count for more than what a thread has in
 // flight: 9632 tokens, 32 and 8 heads, pairs half a head apart: 8 CTAs with one row of a kv
-// CTA's thread and 4 query heads at a time 56 us, 4 CTAs with 4 and 8 79 us.
+// CTA's thread and 4 query heads at a time 56 us, 4 CTAs with 4 and 8 79 us.  Sixteen elements
+// a thread share what a row's address, token and place cost (8: 56 us, 16: 50; with quotients in
+// fixed point 46.5; 4 tokens a CTA, whose angles fill fewer lanes, 50; 16 tokens 51).
 constexpr int kRowThreads = 128, kRowCtasPerSm = 8, kQHeads = 4, kKvTokens = 8, kKvHeads = 4;
 template <typename T, int D, bool kInterleaved>
 __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) k_append_rows_q4(const __grid_constant__ Q4AppendArgs a, int kv_ctas) {
   __shared__ double2 rot[kKvTokens][D / 2];   // cos, sin
   __shared__ Token tok[kKvTokens];
+  __shared__ __align__(16) uint16_t stage[kRowThreads / (D / 16)][kInterleaved ? 8 : D];
   const int tid = threadIdx.x, lane = tid & 31, H = a.n_heads, K = a.kv.n_kv_heads, R = a.rot_dim, n_seq = a.kv.n_seq;
   pdl_wait();
   if (tid == 0) pdl_launch_dependents();
@@ -207,10 +244,12 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) k_append_rows_q4(c
     float2 turn[8];
     const bool turns = 16 * c < R;
     if (turns) {
+      const int slot = L - (row1 - row), one = a.positions && !a.pair_axis ? a.positions[row] : slot;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         float sn, cs;
-        const double turns = (double)position_of(a, 8 * c + i, row, L - (row1 - row)) * (double)a.inv_freq[8 * c + i] * 0.15915494309189533577;
+        const int at = a.pair_axis ? position_of(a, 8 * c + i, row, slot) : one;
+        const double turns = (double)at * (double)a.inv_freq[8 * c + i] * 0.15915494309189533577;
         sincospif(2.0f * (float)(turns - rint(turns)), &sn, &cs);
         turn[i] = make_float2(cs, sn);
       }
@@ -223,34 +262,20 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) k_append_rows_q4(c
       }
     return;
   }
-  constexpr int NC = D / 8, kStep = kRowThreads / NC;   // rows at once
+  // A thread takes 16 elements of the rows of one kv head's keys or values, of every dt-th token.
+  constexpr int NC = D / 16, kStep = kRowThreads / NC;   // rows at once
   const int parts = (K + kKvHeads - 1) / kKvHeads, tile = blockIdx.x / parts;
   const int first = ((int)blockIdx.x - tile * parts) * kKvHeads, heads = min(kKvHeads, K - first);
   const int c = tid % NC, row0 = tile * kKvTokens, tokens = min(kKvTokens, a.n_tokens - row0);
-  const int rows = tokens * 2 * heads;
-  // Row i is of token i / (2 heads), keys before values, so that a warp's two rows are alike.
-  struct Row {
-    int t, x;
-  };
-  const int per = 2 * heads, add_t = kStep / per, add_x = kStep - add_t * per;
-  auto step = [&](Row& r) {
-    r.t += add_t;
-    r.x += add_x;
-    if (r.x >= per) {
-      r.x -= per;
-      ++r.t;
-    }
-  };
-  auto load = [&](const Row& r) {
-    return r.x >= heads
-               ? load_raw<T, true>(reinterpret_cast<const T*>(a.v) + (row0 + r.t) * a.v_stride + (first + r.x - heads) * D, c, R, false)
-               : load_raw<T, kInterleaved>(reinterpret_cast<const T*>(a.k) + (row0 + r.t) * a.k_stride + (first + r.x) * D, c, R, 8 * c < R);
-  };
-  Row at;
-  at.t = tid / NC / per;
-  at.x = tid / NC - at.t * per;
-  Raw next{};
-  if (at.t < tokens) next = load(at);
+  const int lg = heads > 2 ? 2 : heads - 1, x = tid / NC & ((2 << lg) - 1), h = x & ((1 << lg) - 1), dt = kStep >> (lg + 1);
+  const bool is_k = x >> lg == 0, live = h < heads, staged = !kInterleaved && R != D;
+  int t = tid / NC >> (lg + 1), pa = 8 * c, pb = D / 2 + 8 * c;
+  if (staged && is_k) places<false>(c, R, &pa, &pb);
+  const long long stride = is_k ? a.k_stride : a.v_stride;
+  const T* src = reinterpret_cast<const T*>(is_k ? a.k : a.v) + (row0 + t) * stride + (first + h) * D;
+  const long long codes_at = codes_from<D>(a, first + h, is_k, c), params_at = params_from<D>(a, first + h, is_k, c);
+  Chunk next{};
+  if (live && t < tokens) next = load_chunk(src + pa, src + pb);
   if (tid < 32) {
     const int t = lane / (32 / kKvTokens), row = row0 + t;
     const int s = seq_of<32 / kKvTokens>(a.cu_tokens, n_seq, 0, 0, row, lane);
@@ -267,27 +292,36 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm) k_append_rows_q4(c
     if (lane % (32 / kKvTokens) == 0) tok[t] = x;
   }
   __syncthreads();
-  for (int i = tid; i < tokens * (R / 2); i += kRowThreads) {
-    const int t = i / (R / 2), pair = i - t * (R / 2);
-    if (tok[t].seq < 0) continue;
-    double sn, cs;
-    sincos((double)position_of(a, pair, row0 + t, tok[t].slot) * (double)a.inv_freq[pair], &sn, &cs);
-    rot[t][rot_at<D, kInterleaved>(pair)] = make_double2(cs, sn);
-  }
+  const int pair = tid % (D / 2);
+  if (pair < R / 2)
+    for (int i = tid / (D / 2); i < tokens; i += kRowThreads / (D / 2)) {
+      if (tok[i].seq < 0) continue;
+      double sn, cs;
+      sincos((double)position_of(a, pair, row0 + i, tok[i].slot) * (double)a.inv_freq[pair], &sn, &cs);
+      rot[i][rot_at<D, kInterleaved>(pair)] = make_double2(cs, sn);
+    }
   for (int i = tid; i < tokens * heads; i += kRowThreads)
     if (tok[i / heads].seq >= 0) keep_slot(a, tok[i / heads], first + i % heads, row0 + i / heads);
   __syncthreads();
 #pragma unroll 1
-  for (int base = 0; base < rows; base += kStep) {   // (the warp's lanes stay together)
-    const Row now = at;
-    const Raw raw = next;
-    step(at);
-    if (at.t < tokens) next = load(at);
-    const Token& t = tok[min(now.t, tokens - 1)];
-    const bool is_k = now.x < heads, live = now.t < tokens;
-    uint4 x = raw.own;
-    if (is_k && live && t.seq >= 0 && 8 * c < R) x = rotate_raw<double, T, D, kInterleaved>(raw, rot[now.t], c, R);
-    store_quantised<T, D>(a, x, t, first + (is_k ? now.x : now.x - heads), is_k, c, live);
+  for (int base = 0; base < tokens; base += dt, t += dt) {   // (the warp's lanes stay together)
+    Chunk now = next;
+    src += dt * stride;
+    if (live && t + dt < tokens) next = load_chunk(src + pa, src + pb);
+    const Token& token = tok[min(t, tokens - 1)];
+    const bool there = live && t < tokens;
+    if (is_k && there && token.seq >= 0) rotate_key<T, D, kInterleaved>(now, rot[t], c, R);
+    if (staged) {   // pairs R / 2 apart: to where the others have theirs
+      T* row = reinterpret_cast<T*>(stage[tid / NC]);
+      store_chunk(row + pa, row + pb, now);
+      __syncwarp();
+      now = load_chunk(row + 8 * c, row + D / 2 + 8 * c);
+      __syncwarp();
+    }
+    uint8_t *codes = token.block + codes_at + (token.slot & 15) * 16, *params = token.block + params_at + (token.slot & 15) * 4;
+    const bool stored = there && token.block;
+    store_quantised<T>(make_uint4(now.w[0], now.w[1], now.w[2], now.w[3]), codes, params, c & 3, stored);
+    store_quantised<T>(make_uint4(now.w[4], now.w[5], now.w[6], now.w[7]), codes + D / 64 * 256, params + D / 64 * 64, c & 3, stored);
   }
 }
 
