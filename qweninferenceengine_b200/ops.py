@@ -569,8 +569,10 @@ def expand_paged_q4(kv: PagedKVQ4, seq_len: torch.Tensor, cu_rows: torch.Tensor 
             n_rows = kv.n_seq
         if not 0 <= n_rows <= _UINT32:
             raise ValueError(f"n_rows={n_rows}")
-        k, v = torch.empty((2, n_rows, K, dim), dtype=kv.dtype, device=kv.device)
         ks = vs = K * dim
+        shape, strides, device = (n_rows, K, dim), (ks, dim, 1), kv.device
+        k = torch.empty_strided(shape, strides, dtype=kv.dtype, device=device)
+        v = torch.empty_strided(shape, strides, dtype=kv.dtype, device=device)
     _call(kv, lib().qwen_expand_paged_q4, _ints("seq_len", seq_len, kv, kv.n_seq),
           None if cu_rows is None else _ints("cu_rows", cu_rows, kv, kv.n_seq + 1), n_rows,
           k.data_ptr(), ks, v.data_ptr(), vs)

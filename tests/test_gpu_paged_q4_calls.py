@@ -251,3 +251,38 @@ def test_profiling_command_runs_them(capsys):
     out = capsys.readouterr().out
     for name in ("rope_append_paged_q4", "attention_paged_q4", "with weights", "evict_paged_q4", "expand_paged_q4"):
         assert name in out
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("H,K,D,P,rot,inter", [
+    (9, 3, 128, 64, 112, False), (7, 7, 64, 16, 48, False), (2, 1, 64, 64, 32, False), (3, 1, 128, 256, 80, True),
+    (6, 6, 128, 16, 32, False), (4, 1, 128, 16, 128, False), (9, 9, 64, 32, 64, True)])
+def test_append_of_kv_heads_that_do_not_fill_a_cta(dtype, H, K, D, P, rot, inter):
+    lens = [P + 3, 1, 0, 200, 77]
+    c = ref.Cache(40, lens, H, K, D, P, dtype, kept=True)
+    check_append(c, [P + 1, 1, 0, 150, 77], rot, inter, ragged=True, pad=3, far=4000)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_codes_of_narrow_groups_far_from_zero(dtype):
+    """Groups whose least value is 1 to 16,000 steps from zero, of random values, of values on
+    and beside the borders between two codes, and of two values."""
+    n, D = 600, 128
+    c = ref.Cache(41, [n], 2, 2, D, 64, dtype)
+    v = c.randn(n, 2, D).double()
+    away = 2.0 ** torch.linspace(-4, 14, n, device="cuda", dtype=torch.float64)[:, None, None]
+    size = 2.0 ** (torch.arange(n, device="cuda") % 9 - 4).double()[:, None, None]
+    sign = (1 - 2 * (torch.arange(n, device="cuda") % 2)).double()[:, None, None]
+    v[::3] = torch.arange(D, device="cuda") % 31 / 2.0
+    v[1::6] = (torch.arange(D, device="cuda") % 2).double()
+    v = ((v + sign * away) * size).to(dtype)
+    k = v.flip(0).contiguous()
+    pool = c.pool.clone()
+    ops.rope_append_paged_q4(c.handle(), c.randn(n, 2, D), k, v, c.seq_len, torch.zeros(D // 2, device="cuda"),
+                             cu_tokens=ints(0, n))
+    c.store(0, torch.arange(n, device="cuda"), k, v, pool=pool)
+    a, b = ref.views(c.pool, D, dtype), ref.views(pool, D, dtype)
+    for x, y in zip(a[:2], b[:2]):
+        assert torch.equal(x, y)
+    for x, y in zip(a[2:], b[2:]):   # (0 of either sign; NaN where nothing was written)
+        assert torch.equal(torch.isnan(x), torch.isnan(y)) and torch.equal(x.nan_to_num(7.0), y.nan_to_num(7.0))
