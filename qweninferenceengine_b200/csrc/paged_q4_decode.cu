@@ -25,15 +25,21 @@
 // the codes are 16 + c (fp16 caches) or 128 + c in bf16, whose product with weights up to any
 // size is in range; 16 or 128 sum_t step P is taken off at the end.  The two sums of P with lows and with steps are
 // one MMA over the slots, q's group sums with lows another (three terms of 8 or 11 bits).
-// Weights step P are two bf16 values (16 bits).  Sums, maxima and outputs are fp32.
+// Weights step P are two bf16 values (16 bits).  Sums, maxima and outputs are fp32.  An MMA cuts
+// its sum off, always toward zero, and the sums of codes with their bias are a thousand times
+// what is left of them, so that each tile's start from 0 and are added to the others' by
+// additions that round (one chain of MMAs a run was off by 3.8e-3 (2-norm) over 24 sequences
+// of 16384 slots, fp16, this 2.1e-4, which is the output's rounding; 97 -> 101 us for 32).
 //
-// Measured: 32 sequences of 16384 slots, 32 and 8 heads of 128, bf16: 150 us (4.5 TB/s), fp16
-// 167; their 671 MB take 102, and the kernel 106 without its arithmetic, of which the values'
-// dequantisation is 13 and the keys' 6 (a block takes a warp ~340 instructions; the schedulers
-// issue 55% of the time, the integer pipe is busy for 48%, the tensor pipe for 34%).  A call of
-// 512 slots takes 8.4, 64 sequences of 512 .. 2048 slots and 2 kv heads 15.9 (their bytes 3.8):
-// launch, lengths, page numbers, first tile, join.  Warps that load their own blocks, sixteen an
-// SM without producers, took 172 in place of 150.
+// Measured: 32 sequences of 16384 slots, 32 and 8 heads of 128, bf16: 156 us (4.3 TB/s), fp16
+// 171; their 671 MB take 102, the kernel without its arithmetic 106, with its pages in L2 154.
+// A block takes a warp some 350 instructions, and no part of them carries the time (without the
+// scores' MMAs 13 us less, the values' dequantisation 13, the weights' second MMAs 6, the steps'
+// products 5, exponentials 2; without all MMAs of the values the same); 8, 12 or 16 warps an
+// SM, with 2 or 4 blocks at once, are within 6%.  A call of 512 slots takes 8.5, 64 sequences of
+// 512 .. 2048 slots and 2 kv heads 16.3 (their bytes 3.8): launch, lengths, page numbers, first
+// tile, join.  Warps that load their own blocks, sixteen an SM without producers, took 172 in
+// place of 150.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -376,6 +382,7 @@ __device__ __forceinline__ void take_blocks(Stream<D>& w, uint8_t* const (&block
   uint32_t h0[kN], h1[kN], e0[kN], e1[kN];   // in the cache's type, and what rounding left
   float pw[kN][4];                           // fp16: the weights themselves
   uint32_t vs[kN];
+  float extra[4];
 #pragma unroll
   for (int n = 0; n < kN; ++n) {
     vs[n] = smem_u32(blocks[n]) + Block::kValueSteps + t4 * 8;
@@ -413,9 +420,12 @@ __device__ __forceinline__ void take_blocks(Stream<D>& w, uint8_t* const (&block
       x[0] = prmt(v0.x, v0.y, sel);
       x[2] = prmt(v1.x, v1.y, sel);
     }
-    mma_add(T{}, w.extra, x, h0[n], h1[n]);
-    mma_add(T{}, w.extra, x, e0[n], e1[n]);
+    if (n == 0) mma_zero(T{}, extra, x, h0[n], h1[n]);
+    else mma_add(T{}, extra, x, h0[n], h1[n]);
+    mma_add(T{}, extra, x, e0[n], e1[n]);
   }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w.extra[e] += extra[e];
   // ---- o^T += (bias + codes)^T (step weights)^T
 #pragma unroll
   for (int pair = 0; pair < G / 2; ++pair) {
@@ -425,6 +435,7 @@ __device__ __forceinline__ void take_blocks(Stream<D>& w, uint8_t* const (&block
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const int i = 2 * pair + k;
+      float o[2][4];
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
         const uint2 v0 = lds64(vs[n] + i * 64), v1 = lds64(vs[n] + i * 64 + 32);
@@ -440,10 +451,15 @@ __device__ __forceinline__ void take_blocks(Stream<D>& w, uint8_t* const (&block
         for (int j = 0; j < 2; ++j) {
           const uint32_t x[4] = {large_code<T>(vc[n][2 * k], 2 * j), large_code<T>(vc[n][2 * k], 2 * j + 1),
                                  large_code<T>(vc[n][2 * k + 1], 2 * j), large_code<T>(vc[n][2 * k + 1], 2 * j + 1)};
-          mma_add(__nv_bfloat16{}, w.o[i][j], x, b0, b1);
-          mma_add(__nv_bfloat16{}, w.o[i][j], x, c0, c1);
+          if (n == 0) mma_zero(__nv_bfloat16{}, o[j], x, b0, b1);
+          else mma_add(__nv_bfloat16{}, o[j], x, b0, b1);
+          mma_add(__nv_bfloat16{}, o[j], x, c0, c1);
         }
       }
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w.o[i][j][e] += o[j][e];
     }
   }
   if (!whole) fence_proxy_async();   // the zeros before the next copy

@@ -286,3 +286,30 @@ def test_codes_of_narrow_groups_far_from_zero(dtype):
         assert torch.equal(x, y)
     for x, y in zip(a[2:], b[2:]):   # (0 of either sign; NaN where nothing was written)
         assert torch.equal(torch.isnan(x), torch.isnan(y)) and torch.equal(x.nan_to_num(7.0), y.nan_to_num(7.0))
+
+
+def test_attention_of_long_contexts_is_not_off_to_one_side():
+    """Outputs near zero, whose parts (lows, steps times codes, the codes' bias) are not: what the
+    sums lose must not add up.
+
+    The mean error over a sequence's outputs.  A tile's four MMAs cut off at most 2^-23 of
+    their sums each, together 2^-21 A of A = sum of weights (|low| + 31 step), codes with a
+    bias of 16 being at most 31.  All else errs to both sides: the output's rounding, u |out|
+    at most, and the additions of the T tiles, 2^-24 A each, so that the mean of N such
+    errors is within 6 of its deviations, 6 sqrt((u^2 mean(out^2) + T 2^-48 A^2) / N)."""
+    n, L, H, K, D = 12, 16384, 32, 8, 128
+    c = ref.Cache(50, [L] * n, H, K, D, 64, F16)
+    out = ops.attention_paged_q4(c.handle(), c.q, c.seq_len)[3].double()
+    slots = c.all_slots(3)
+    k, v = c.rows(3, slots)
+    page, block, r = c.place(3, slots)
+    step, low = ref.views(c.pool, D, F16)[3][page, :, block, :, r].double().abs().unbind(-1)   # [L, K, D / 32]
+    want, size = [], []
+    for h in range(K):
+        w = torch.softmax(c.q[3, h * 4: h * 4 + 4].double() @ k[:, h].T * D ** -0.5, -1)
+        want.append(w @ v[:, h])
+        size.append((w @ (low + 31 * step)[:, h]).amax())
+    want, A = torch.cat(want), torch.stack(size).amax().item()
+    off = (out - want).mean().abs().item()
+    both = (2.0 ** -22 * want.pow(2).mean().item() + L / 128 * 2.0 ** -48 * A ** 2) / want.numel()
+    assert off <= 2.0 ** -21 * A + 6 * both ** 0.5, (off, A)
