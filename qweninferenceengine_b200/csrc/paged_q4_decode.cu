@@ -22,14 +22,12 @@
 // word's eight keys take four ANDs and a shift (those from bits 4..7 are 16 c 2^-24; their
 // query elements are divided by 16).  Queries are brought to 2^14 .. 2^15 a head by a power
 // of two and are exact in fp16 but for what is 2^-33 of the head's largest.  For the values
-// the codes are 16 + c (fp16 caches) or 128 + c in bf16, whose product with weights up to any
-// size is in range; 16 or 128 sum_t step P is taken off at the end.  The two sums of P with lows and with steps are
-// one MMA over the slots, q's group sums with lows another (three terms of 8 or 11 bits).
-// Weights step P are two bf16 values (16 bits).  Sums, maxima and outputs are fp32.  An MMA cuts
-// its sum off, always toward zero, and the sums of codes with their bias are a thousand times
-// what is left of them, so that each tile's start from 0 and are added to the others' by
-// additions that round (one chain of MMAs a run was off by 3.8e-3 (2-norm) over 24 sequences
-// of 16384 slots, fp16, this 2.1e-4, which is the output's rounding; 97 -> 101 us for 32).
+// the codes are bf16, whose products with steps and weights are in range.  The sums of P with
+// lows are one MMA over the slots, q's group sums with lows another (three terms of 8 or 11
+// bits).  Weights step P are two bf16 values (off by at most 2^-17 of one, a 64th of what fp16
+// outputs are rounded by).  Sums, maxima and outputs are fp32.  An MMA cuts its sum off, always
+// toward zero, which over a run would add up, so that each tile's start from 0 and are added to
+// the others' by additions that round (4% of a long call).
 //
 // Measured: 32 sequences of 16384 slots, 32 and 8 heads of 128, bf16: 156 us (4.3 TB/s), fp16
 // 171; their 671 MB take 102, the kernel without its arithmetic 106, with its pages in L2 154.
@@ -234,17 +232,15 @@ __device__ __forceinline__ void small_codes(uint32_t w, uint32_t (&c)[4]) {
   c[2] = w & 0x00f000f0u;
   c[3] = v & 0x00f000f0u;
 }
-// Bias + codes in bf16 of bits 4 j .. 4 j + 3 of both halves of a word.  The bias is taken off
-// the sums, which are rounded relative to it: with 128, whose codes need no shift for j = 0,
-// outputs over 32768 positions were off by 3.0e-4 (2-norm), more than fp16's own 2.0e-4.
-template <typename T>
-constexpr float kBias = std::is_same<T, __half>::value ? 16.f : 128.f;
-template <typename T>
-__device__ __forceinline__ uint32_t large_code(uint32_t w, int j) {
-  if constexpr (std::is_same<T, __half>::value)
-    return lop3_and_or(j ? w >> (4 * j - 3) : w << 3, 0x00780078u, 0x41804180u);
-  else
-    return lop3_and_or(w >> (4 * j), 0x000f000fu, 0x43004300u);
+// Codes in bf16 of bits 4 j .. 4 j + 3 of both halves of a word.  128 + code are the code's bits
+// at the bottom of a mantissa; the 128 is taken off here, where that is exact, and not from the
+// sums: there it stood against weights that had been rounded otherwise (elements whose codes and
+// lows are all 0 came out as 3e-6 in place of 0, bf16, 1000 slots; and 128 or 16 times a weight's
+// error against a code of 7.5).  An addition for two codes: 32 x 16384 bf16 156 -> 161 us.
+__device__ __forceinline__ uint32_t value_code(uint32_t w, int j) {
+  const uint32_t v = lop3_and_or(w >> (4 * j), 0x000f000fu, 0x43004300u);
+  const __nv_bfloat162 c = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), __float2bfloat162_rn(128.f));
+  return *reinterpret_cast<const uint32_t*>(&c);
 }
 
 // Scores of a block, log2 domain: s = (slot g: heads 2t, 2t+1), (slot g + 8: the same).
@@ -287,7 +283,7 @@ template <int D>
 struct Stream {
   Queries<D> u;
   float o[D / 32][2][4];      // element 32 i + 4 g + 2 j of heads 2t, 2t + 1, then the next one
-  float extra[4];             // sums of weights with lows (row g < 4) and with steps (g - 4)
+  float extra[4];             // sums of weights with lows (row g: of group g)
   float m[2], ref[2], l[2];   // of heads 2t, 2t + 1; ref: m, or 0 where there is none
 };
 
@@ -411,14 +407,12 @@ __device__ __forceinline__ void take_blocks(Stream<D>& w, uint8_t* const (&block
       e0[n] = movmatrix(e0[n]);
       e1[n] = movmatrix(e1[n]);
     }
-    // sums of weights with lows and steps: row g is the low of group g, or the step of g - 4
-    const int i = g & 3;
+    // sums of weights with lows: row g is the low of group g
     uint32_t x[4] = {};
-    if (i < G) {
-      const uint2 v0 = lds64(vs[n] + i * 64), v1 = lds64(vs[n] + i * 64 + 32);
-      const uint32_t sel = g < 4 ? 0x7632 : 0x5410;
-      x[0] = prmt(v0.x, v0.y, sel);
-      x[2] = prmt(v1.x, v1.y, sel);
+    if (g < G) {
+      const uint2 v0 = lds64(vs[n] + g * 64), v1 = lds64(vs[n] + g * 64 + 32);
+      x[0] = prmt(v0.x, v0.y, 0x7632);
+      x[2] = prmt(v1.x, v1.y, 0x7632);
     }
     if (n == 0) mma_zero(T{}, extra, x, h0[n], h1[n]);
     else mma_add(T{}, extra, x, h0[n], h1[n]);
@@ -426,7 +420,7 @@ __device__ __forceinline__ void take_blocks(Stream<D>& w, uint8_t* const (&block
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e) w.extra[e] += extra[e];
-  // ---- o^T += (bias + codes)^T (step weights)^T
+  // ---- o^T += codes^T (step weights)^T
 #pragma unroll
   for (int pair = 0; pair < G / 2; ++pair) {
     uint32_t vc[kN][4];   // [group][half]: unit g (elements 4 g ..) of slots 2t, 2t+1 of that half
@@ -449,8 +443,8 @@ __device__ __forceinline__ void take_blocks(Stream<D>& w, uint8_t* const (&block
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const uint32_t x[4] = {large_code<T>(vc[n][2 * k], 2 * j), large_code<T>(vc[n][2 * k], 2 * j + 1),
-                                 large_code<T>(vc[n][2 * k + 1], 2 * j), large_code<T>(vc[n][2 * k + 1], 2 * j + 1)};
+          const uint32_t x[4] = {value_code(vc[n][2 * k], 2 * j), value_code(vc[n][2 * k], 2 * j + 1),
+                                 value_code(vc[n][2 * k + 1], 2 * j), value_code(vc[n][2 * k + 1], 2 * j + 1)};
           if (n == 0) mma_zero(__nv_bfloat16{}, o[j], x, b0, b1);
           else mma_add(__nv_bfloat16{}, o[j], x, b0, b1);
           mma_add(__nv_bfloat16{}, o[j], x, c0, c1);
@@ -712,8 +706,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_q4_decode(const __grid
     for (int i = 0; i < G; ++i)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float add = __shfl_sync(0xffffffffu, w.extra[e], 4 * i + t4) -
-                          kBias<T> * __shfl_sync(0xffffffffu, w.extra[e], 4 * (4 + i) + t4);
+        const float add = __shfl_sync(0xffffffffu, w.extra[e], 4 * i + t4);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           w.o[i][j][e] += add;

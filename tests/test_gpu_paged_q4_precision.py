@@ -1,0 +1,67 @@
+"""What decode attention over a 4-bit paged cache must not lose: weights, codes and sums
+where the bounds of test_gpu_paged_q4.py, which grow with the length, are wide."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+import paged_q4_reference as ref  # noqa: E402
+from paged_reference import U  # noqa: E402
+from qweninferenceengine_b200 import ops  # noqa: E402
+from qweninferenceengine_b200._lib import QWEN_OK, lib  # noqa: E402
+
+F16, BF16 = torch.float16, torch.bfloat16
+DTYPES = [F16, BF16]
+
+
+@pytest.fixture(autouse=True)
+def clean_status(cuda):
+    yield
+    assert lib().qwen_ops_status(torch.cuda.current_stream().cuda_stream) == QWEN_OK
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens,H,K,D,P", [([1000], 12, 2, 128, 64), ([16, 70, 1777], 16, 8, 64, 16),
+                                          ([4096] * 9, 40, 2, 128, 256)])
+def test_attention_of_elements_that_are_zero(dtype, lens, H, K, D, P):
+    """An element that is 0 in every slot, the least of its groups, has code 0 and low 0 whatever
+    the groups' steps: products with it are 0, and so is the output, exactly."""
+    c = ref.Cache(1, [0] * len(lens), H, K, D, P, dtype, width=-(-max(lens) // P))
+    c.lens, c.seq_len = lens, torch.tensor(lens, dtype=torch.int32, device="cuda")
+    zero = torch.ones(D, dtype=torch.bool, device="cuda")
+    zero[5::32] = False
+    for i, x in enumerate(lens):
+        v = c.randn(x, K, D).abs()
+        v[..., zero] = 0
+        c.store(i, c.all_slots(i), c.randn(x, K, D), v)
+    out = ops.attention_paged_q4(c.handle(), c.q, c.seq_len)
+    assert (out[..., zero] == 0).all()
+    assert (out[..., ~zero] > 0).all()
+
+
+def test_attention_of_long_bf16_contexts_is_not_off_to_one_side():
+    """The mean error over a sequence's outputs near zero, whose parts (lows, steps times codes)
+    are not.
+
+    A tile's MMAs (four for lows, four for codes) cut off at most 2^-23 of their sums each:
+    together 2^-20 A of A = sum of weights (|low| + 15 step).  All else errs to both sides: the
+    output's rounding, u |out| at most, weights of 16 bits, 2^-17 A at most each and, as their
+    errors are independent, 2^-17 A / sqrt(L / 16) in the sum of L slots whose weights, over
+    L / 16, differ little, and the additions of the T tiles, 2^-24 A each.  The mean of N outputs'
+    errors is within 6 of its deviations."""
+    n, L, H, K, D = 12, 16384, 32, 8, 128
+    c = ref.Cache(50, [L] * n, H, K, D, 64, BF16)
+    out = ops.attention_paged_q4(c.handle(), c.q, c.seq_len)[3].double()
+    slots = c.all_slots(3)
+    k, v = c.rows(3, slots)
+    page, block, r = c.place(3, slots)
+    step, low = ref.views(c.pool, D, BF16)[3][page, :, block, :, r].double().abs().unbind(-1)
+    want, size = [], []
+    for h in range(K):
+        w = torch.softmax(c.q[3, h * 4: h * 4 + 4].double() @ k[:, h].T * D ** -0.5, -1)
+        want.append(w @ v[:, h])
+        size.append((w @ (low + 15 * step)[:, h]).amax())
+    want, A = torch.cat(want), torch.stack(size).amax().item()
+    off = (out - want).mean().abs().item()
+    each = U[BF16] ** 2 * want.pow(2).mean().item() + (2.0 ** -34 * 16 / L + L / 128 * 2.0 ** -48) * A ** 2
+    assert off <= 2.0 ** -20 * A + 6 * (each / want.numel()) ** 0.5, (off, A)
