@@ -24,7 +24,7 @@
 // of two and are exact in fp16 but for what is 2^-33 of the head's largest.  For the values
 // the codes are bf16, whose products with steps and weights are in range.  The sums of P with
 // lows are one MMA over the slots, q's group sums with lows another (three terms of 8 or 11
-// bits).  Weights step P are two bf16 values (off by at most 2^-17 of one, a 64th of what fp16
+// bits).  Weights P and step P are two bf16 values (off by at most 2^-17 of one, a 64th of what fp16
 // outputs are rounded by).  Sums, maxima and outputs are fp32.  An MMA cuts its sum off, always
 // toward zero, which over a run would add up, so that each tile's start from 0 and are added to
 // the others' by additions that round (4% of a long call).
@@ -283,7 +283,7 @@ template <int D>
 struct Stream {
   Queries<D> u;
   float o[D / 32][2][4];      // element 32 i + 4 g + 2 j of heads 2t, 2t + 1, then the next one
-  float extra[4];             // sums of weights with lows (row g: of group g)
+  float extra[4];             // sums of weights with lows (row g: of group g; fp16: and g - 4)
   float m[2], ref[2], l[2];   // of heads 2t, 2t + 1; ref: m, or 0 where there is none
 };
 
@@ -375,7 +375,7 @@ __device__ __forceinline__ void take_blocks(Stream<D>& w, uint8_t* const (&block
     }
   }
   // ---- weights, turned: lane 4 g + t has head g, slots 2t, 2t+1 and 8 + those
-  uint32_t h0[kN], h1[kN], e0[kN], e1[kN];   // in the cache's type, and what rounding left
+  uint32_t h0[kN], h1[kN], e0[kN], e1[kN];   // in bf16, and what rounding left
   float pw[kN][4];                           // fp16: the weights themselves
   uint32_t vs[kN];
   float extra[4];
@@ -397,8 +397,8 @@ __device__ __forceinline__ void take_blocks(Stream<D>& w, uint8_t* const (&block
       pw[n][1] = __uint_as_float(prmt(y0, x0, 0x7632));
       pw[n][2] = __uint_as_float(prmt(y1, x1, 0x5410));
       pw[n][3] = __uint_as_float(prmt(y1, x1, 0x7632));
-      split2<T>(pw[n][0], pw[n][1], &h0[n], &e0[n]);
-      split2<T>(pw[n][2], pw[n][3], &h1[n], &e1[n]);
+      split2<__nv_bfloat16>(pw[n][0], pw[n][1], &h0[n], &e0[n]);
+      split2<__nv_bfloat16>(pw[n][2], pw[n][3], &h1[n], &e1[n]);
     } else {
       split2<T>(sv[n][0], sv[n][1], &h0[n], &e0[n]);
       split2<T>(sv[n][2], sv[n][3], &h1[n], &e1[n]);
@@ -407,16 +407,28 @@ __device__ __forceinline__ void take_blocks(Stream<D>& w, uint8_t* const (&block
       e0[n] = movmatrix(e0[n]);
       e1[n] = movmatrix(e1[n]);
     }
-    // sums of weights with lows: row g is the low of group g
+    // Sums of weights with lows: row g is the low of group g.  Weights as bf16, whatever the
+    // cache's type: fp16 ends at 2^-24, and sums over thousands of slots far below the heaviest
+    // lose what lies under it.  Lows of fp16 are two bf16 each, the second in rows 4 ..
     uint32_t x[4] = {};
-    if (g < G) {
-      const uint2 v0 = lds64(vs[n] + g * 64), v1 = lds64(vs[n] + g * 64 + 32);
+    const int i = kF16 ? g & 3 : g;
+    if (i < G) {
+      const uint2 v0 = lds64(vs[n] + i * 64), v1 = lds64(vs[n] + i * 64 + 32);
       x[0] = prmt(v0.x, v0.y, 0x7632);
       x[2] = prmt(v1.x, v1.y, 0x7632);
+      if constexpr (kF16) {   // the 8 bits that cutting it to bf16 leaves, or the others
+        const uint32_t cut = g < 4 ? 0 : 0xffff0000u;
+        auto part = [&](float y) { return __float_as_uint(y - __uint_as_float(__float_as_uint(y) & cut)); };
+#pragma unroll
+        for (int k = 0; k < 4; k += 2) {
+          const float2 low = unpack2(T{}, x[k]);
+          x[k] = prmt(part(low.x), part(low.y), 0x7632);
+        }
+      }
     }
-    if (n == 0) mma_zero(T{}, extra, x, h0[n], h1[n]);
-    else mma_add(T{}, extra, x, h0[n], h1[n]);
-    mma_add(T{}, extra, x, e0[n], e1[n]);
+    if (n == 0) mma_zero(__nv_bfloat16{}, extra, x, h0[n], h1[n]);
+    else mma_add(__nv_bfloat16{}, extra, x, h0[n], h1[n]);
+    mma_add(__nv_bfloat16{}, extra, x, e0[n], e1[n]);
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e) w.extra[e] += extra[e];
@@ -706,7 +718,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_q4_decode(const __grid
     for (int i = 0; i < G; ++i)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float add = __shfl_sync(0xffffffffu, w.extra[e], 4 * i + t4);
+        float add = __shfl_sync(0xffffffffu, w.extra[e], 4 * i + t4);
+        if (std::is_same<T, __half>::value) add += __shfl_sync(0xffffffffu, w.extra[e], 4 * (4 + i) + t4);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           w.o[i][j][e] += add;

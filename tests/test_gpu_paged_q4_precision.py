@@ -65,3 +65,43 @@ def test_attention_of_long_bf16_contexts_is_not_off_to_one_side():
     off = (out - want).mean().abs().item()
     each = U[BF16] ** 2 * want.pow(2).mean().item() + (2.0 ** -34 * 16 / L + L / 128 * 2.0 ** -48) * A ** 2
     assert off <= 2.0 ** -20 * A + 6 * (each / want.numel()) ** 0.5, (off, A)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,L,H,K,D", [(1, 16384, 12, 2, 128), (8, 16384, 32, 8, 128), (3, 20011, 16, 8, 64)])
+@pytest.mark.parametrize("above", [10.0, 18.0, 20.0])
+@pytest.mark.parametrize("alike", [False, True])
+def test_attention_beside_a_heavy_slot(dtype, n, L, H, K, D, above, alike):
+    """One slot of a score `above` the others' and a value near zero, as the first tokens of a
+    text have: the output is what the many others add up to, each of a weight of e^-above.
+
+    Bounds: scores are off by d as in paged_q4_reference.py, all weights alike (2 d, relative
+    to the sum that each is divided by); a weight with its step and low 2^-16 of them; sums of
+    T tiles, over up to 32 pieces, at random to both sides, at most (2^-20 + 6 2^-24 sqrt(T))
+    of what is summed, B = sum of weights (|low| + 15 step); and the output's rounding."""
+    c = ref.Cache(51, [0] * n, H, K, D, 64, dtype, width=L // 64 + 1)
+    c.lens, c.seq_len = [L] * n, torch.full((n,), L, dtype=torch.int32, device="cuda")
+    slots = c.all_slots(0)
+    for i in range(n):
+        k, v = c.randn(L, K, D) * 0.02, c.randn(L, K, D)
+        if alike:
+            k = k[:1].expand(L, -1, -1).clone()
+        k[7], v[7] = above * D ** -0.5, v[7] * 2.0 ** -13
+        c.store(i, slots, k, v)
+    c.q = (1 + 0.01 * c.randn(n, H, D).double()).to(dtype)
+    out = ops.attention_paged_q4(c.handle(), c.q, c.seq_len)[0].double()
+    k, v = c.rows(0, slots)
+    ka = c.sizes(0, slots)[0]
+    page, block, r = c.place(0, slots)
+    step, low = ref.views(c.pool, D, dtype)[3][page, :, block, :, r].double().abs().unbind(-1)
+    G = H // K
+    for h in range(K):
+        x = c.q[0, h * G: (h + 1) * G].double()
+        s = x @ k[:, h].T * D ** -0.5
+        d = 2.0 ** -23 * (2 * D * (x.abs() @ ka[:, h].T * D ** -0.5).amax() + 16 + 2 * s.abs().amax())
+        w = torch.softmax(s, -1)
+        want = w @ v[:, h]
+        B = (w @ (low + 15 * step)[:, h]).repeat_interleave(32, -1)
+        tol = B * (2 * d + 2.0 ** -16 + 2.0 ** -20 + 6 * 2.0 ** -24 * (L / 128) ** 0.5) + U[dtype] * want.abs() + 2.0 ** -25
+        off = (out[h * G: (h + 1) * G] - want).abs() - tol
+        assert off.max().item() <= 0, (off.max().item(), tol.max().item(), want.abs().max().item())
