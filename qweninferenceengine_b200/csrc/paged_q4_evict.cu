@@ -270,6 +270,7 @@ __device__ __forceinline__ void select_row(const Q4EvictArgs& a, int unit, int f
     });
     const int i = a.n_keep - first - base;   // (of this tile, or the last before n_keep)
     if (i > 0) kept_below = i >= min(kTile, n - base) ? kept : s.stay.rank_of(i);
+    if (n > kTile) __syncthreads();   // every thread has read the tile's bits: the next one's take their place
   };
 #pragma unroll 1
   for (int base = 0; base < n; base += kTile) decide(base);
