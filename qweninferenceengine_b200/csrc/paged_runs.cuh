@@ -28,8 +28,8 @@ struct DecodeArgs {
   unsigned long long tag;
   float* own_o;             // if set: unnormalised rows [n_seq][n_heads][D] and their (max,
   float2* own_ml;           //   sum) go here instead of outputs, for the shared-prefix join
-  uint32_t few_tiles;       // up to so many tiles are divided among `few` CTAs only
-  int few;
+  uint32_t few_tiles = 0;   // up to so many tiles are divided among `few` CTAs only (no tiles at all: a call
+  int few = 1;              // of lengths beyond the table alone; the number of runs is divided by)
 };
 
 __device__ __forceinline__ uint32_t seq_tiles(const DecodeArgs& p, uint32_t L) {
