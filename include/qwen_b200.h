@@ -377,7 +377,8 @@ int qwen_rope_append_paged_q4(const qwen_paged_kv_q4* kv, const uint16_t* q, int
  * the weight that they give it; the workspace then holds the scores too, 4 bytes a query
  * head and slot at full capacity.  What multiplies codes and lows, a softmax weight and
  * its product with a group's step, is held in 16 bits of any size (two bf16), all that is
- * summed in fp32. */
+ * summed in fp32: finite while a sequence's length times its greatest value is below 10^35,
+ * which only bf16 caches can pass. */
 size_t qwen_attention_paged_q4_workspace(const qwen_paged_kv_q4* kv, uint32_t n_heads);
 int qwen_attention_paged_q4(const qwen_paged_kv_q4* kv, const uint16_t* q, int64_t q_stride,
                             uint16_t* out, int64_t out_stride, float* lse, uint32_t n_heads,

@@ -22,12 +22,14 @@
 // word's eight keys take four ANDs and a shift (those from bits 4..7 are 16 c 2^-24; their
 // query elements are divided by 16).  Queries are brought to 2^14 .. 2^15 a head by a power
 // of two and are exact in fp16 but for what is 2^-33 of the head's largest.  For the values
-// the codes are bf16, whose products with steps and weights are in range.  The sums of P with
-// lows are one MMA over the slots, q's group sums with lows another (three terms of 8 or 11
-// bits).  Weights P and step P are two bf16 values (off by at most 2^-17 of one, a 64th of what fp16
-// outputs are rounded by).  Sums, maxima and outputs are fp32.  An MMA cuts its sum off, always
-// toward zero, which over a run would add up, so that each tile's start from 0 and are added to
-// the others' by additions that round (4% of a long call).
+// the codes are bf16.  Weights are at most 2^8, so that the sums over L slots are finite while
+// L times the greatest value is below 10^35 (weights of at most 1, by a reference that is moved 8
+// above the greatest score, would give 10^38, but not the very value where there is one slot).
+// The sums of P with lows are one MMA over the slots, q's group sums with lows another (three
+// terms of 8 or 11 bits).  Weights P and step P are two bf16 values (off by at most 2^-17 of one,
+// a 64th of what fp16 outputs are rounded by).  Sums, maxima and outputs are fp32.  An MMA cuts
+// its sum off, always toward zero, which over a run would add up, so that each tile's start from
+// 0 and are added to the others' by additions that round (4% of a long call).
 //
 // Measured: 32 sequences of 16384 slots, 32 and 8 heads of 128, bf16: 156 us (4.3 TB/s), fp16
 // 171; their 671 MB take 102, the kernel without its arithmetic 106, with its pages in L2 154.

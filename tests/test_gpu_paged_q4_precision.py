@@ -105,3 +105,28 @@ def test_attention_beside_a_heavy_slot(dtype, n, L, H, K, D, above, alike):
         tol = B * (2 * d + 2.0 ** -16 + 2.0 ** -20 + 6 * 2.0 ** -24 * (L / 128) ** 0.5) + U[dtype] * want.abs() + 2.0 ** -25
         off = (out[h * G: (h + 1) * G] - want).abs() - tol
         assert off.max().item() <= 0, (off.max().item(), tol.max().item(), want.abs().max().item())
+
+
+@pytest.mark.parametrize("big,grow", [(6e33, 0.0), (6e30, 5.0)])
+def test_attention_of_bf16_values_near_the_types_end(big, grow):
+    """Length times value 10^35, with scores that grow, so that weights pass those that a run
+    began with (they are below 2^8); and 10^38 with scores around one value, whose weights stay
+    about 1: 2 10^38 is the most that their sums come to.  So many sequences that one run
+    has a whole one."""
+    n, L, H, K, D = 128, 16384, 16, 8, 64
+    c = ref.Cache(60, [0] * n, H, K, D, 64, BF16, width=L // 64)
+    c.lens, c.seq_len = [L] * n, torch.full((n,), L, dtype=torch.int32, device="cuda")
+    c.pool.copy_(torch.randint(0, 256, (1, *c.pool.shape[1:]), generator=c.g, device="cuda", dtype=torch.uint8))
+    _, _, ks, vs = ref.views(c.pool, D, BF16)
+    vs[..., 0], vs[..., 1] = 2 * big / 15, -big
+    ks[..., 0] = 2.0 ** -6
+    for i in range(n):   # every element of a slot's key alike, but for its codes
+        page, block, r = c.place(i, c.all_slots(i))
+        ks[page, :, block, :, r, 1] = (torch.arange(L, device="cuda") * (grow * D ** -0.5 / L)).to(BF16)[:, None, None]
+    c.q = (1 + 0.01 * c.randn(n, H, D).double()).to(BF16)
+    got = ops.attention_paged_q4(c.handle(), c.q, c.seq_len, return_lse=True)
+    assert torch.isfinite(got[0]).all() and torch.isfinite(got[1]).all()
+    for i in (0, n - 1):
+        only = [L if j == i else 0 for j in range(n)]
+        want = ref.attention(c, D ** -0.5, lens=only)
+        ref.check_attention(tuple(x[i: i + 1] for x in got), tuple(x[i: i + 1] for x in want))
