@@ -234,12 +234,18 @@ __device__ __forceinline__ void small_codes(uint32_t w, uint32_t (&c)[4]) {
   c[2] = w & 0x00f000f0u;
   c[3] = v & 0x00f000f0u;
 }
-// Codes in bf16 of bits 4 j .. 4 j + 3 of both halves of a word.  128 + code are the code's bits
-// at the bottom of a mantissa; the 128 is taken off here, where that is exact, and not from the
-// sums: there it stood against weights that had been rounded otherwise (elements whose codes and
-// lows are all 0 came out as 3e-6 in place of 0, bf16, 1000 slots; and 128 or 16 times a weight's
-// error against a code of 7.5).  An addition for two codes: 32 x 16384 bf16 156 -> 161 us.
+// Codes in bf16 of bits 4 j .. 4 j + 3 of both halves of a word, as they are and not with a bias
+// that is taken off the sums: there it stood against weights that had been rounded otherwise
+// (elements whose codes and lows are all 0 came out as 3e-6 in place of 0, bf16, 1000 slots; and
+// 128 or 16 times a weight's error against a code of 7.5).
+// fp16 caches: a code at the bottom of a bf16 is c 2^-133, for odd j 16 times that (bit 7, the
+// exponent's first, counts on), and weights are brought to 2^kRaise: an AND for two codes.  The
+// steps of bf16 caches leave no room for that: there 128 + code less 128, which is exact
+// (32 x 16384: bf16 156 -> 161 us with it, fp16 171 -> 179 and without it 167).
+constexpr int kRaise = 72;   // 2^(72 + 8 + 13 + 24) at most: weight, step, slots
+template <typename T>
 __device__ __forceinline__ uint32_t value_code(uint32_t w, int j) {
+  if constexpr (std::is_same<T, __half>::value) return (j & 2 ? w >> 8 : w) & (j & 1 ? 0x00f000f0u : 0x000f000fu);
   const uint32_t v = lop3_and_or(w >> (4 * j), 0x000f000fu, 0x43004300u);
   const __nv_bfloat162 c = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), __float2bfloat162_rn(128.f));
   return *reinterpret_cast<const uint32_t*>(&c);
@@ -378,7 +384,7 @@ __device__ __forceinline__ void take_blocks(Stream<D>& w, uint8_t* const (&block
   }
   // ---- weights, turned: lane 4 g + t has head g, slots 2t, 2t+1 and 8 + those
   uint32_t h0[kN], h1[kN], e0[kN], e1[kN];   // in bf16, and what rounding left
-  float pw[kN][4];                           // fp16: the weights themselves
+  float pw[kN][4];                           // fp16: the weights themselves, raised
   uint32_t vs[kN];
   float extra[4];
 #pragma unroll
@@ -395,10 +401,10 @@ __device__ __forceinline__ void take_blocks(Stream<D>& w, uint8_t* const (&block
       const uint32_t y0 = movmatrix(prmt(__float_as_uint(sv[n][0]), __float_as_uint(sv[n][1]), 0x5410));
       const uint32_t x1 = movmatrix(prmt(__float_as_uint(sv[n][2]), __float_as_uint(sv[n][3]), 0x7632));
       const uint32_t y1 = movmatrix(prmt(__float_as_uint(sv[n][2]), __float_as_uint(sv[n][3]), 0x5410));
-      pw[n][0] = __uint_as_float(prmt(y0, x0, 0x5410));
-      pw[n][1] = __uint_as_float(prmt(y0, x0, 0x7632));
-      pw[n][2] = __uint_as_float(prmt(y1, x1, 0x5410));
-      pw[n][3] = __uint_as_float(prmt(y1, x1, 0x7632));
+      pw[n][0] = __uint_as_float(prmt(y0, x0, 0x5410)) * pow2(kRaise);
+      pw[n][1] = __uint_as_float(prmt(y0, x0, 0x7632)) * pow2(kRaise);
+      pw[n][2] = __uint_as_float(prmt(y1, x1, 0x5410)) * pow2(kRaise);
+      pw[n][3] = __uint_as_float(prmt(y1, x1, 0x7632)) * pow2(kRaise);
       split2<__nv_bfloat16>(pw[n][0], pw[n][1], &h0[n], &e0[n]);
       split2<__nv_bfloat16>(pw[n][2], pw[n][3], &h1[n], &e1[n]);
     } else {
@@ -457,8 +463,8 @@ __device__ __forceinline__ void take_blocks(Stream<D>& w, uint8_t* const (&block
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const uint32_t x[4] = {value_code(vc[n][2 * k], 2 * j), value_code(vc[n][2 * k], 2 * j + 1),
-                                 value_code(vc[n][2 * k + 1], 2 * j), value_code(vc[n][2 * k + 1], 2 * j + 1)};
+          const uint32_t x[4] = {value_code<T>(vc[n][2 * k], 2 * j), value_code<T>(vc[n][2 * k], 2 * j + 1),
+                                 value_code<T>(vc[n][2 * k + 1], 2 * j), value_code<T>(vc[n][2 * k + 1], 2 * j + 1)};
           if (n == 0) mma_zero(__nv_bfloat16{}, o[j], x, b0, b1);
           else mma_add(__nv_bfloat16{}, o[j], x, b0, b1);
           mma_add(__nv_bfloat16{}, o[j], x, c0, c1);
@@ -721,7 +727,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_q4_decode(const __grid
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         float add = __shfl_sync(0xffffffffu, w.extra[e], 4 * i + t4);
-        if (std::is_same<T, __half>::value) add += __shfl_sync(0xffffffffu, w.extra[e], 4 * (4 + i) + t4);
+        if constexpr (std::is_same<T, __half>::value) {
+          add = (add + __shfl_sync(0xffffffffu, w.extra[e], 4 * (4 + i) + t4)) * pow2(-kRaise);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            w.o[i][j][e] *= pow2(133 - kRaise);
+            w.o[i][j][2 + e] *= pow2(133 - kRaise - 4);
+          }
+        }
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           w.o[i][j][e] += add;

@@ -130,3 +130,23 @@ def test_attention_of_bf16_values_near_the_types_end(big, grow):
         only = [L if j == i else 0 for j in range(n)]
         want = ref.attention(c, D ** -0.5, lens=only)
         ref.check_attention(tuple(x[i: i + 1] for x in got), tuple(x[i: i + 1] for x in want))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H,K,D", [(12, 2, 128), (16, 8, 64)])
+def test_attention_of_one_slot_is_its_value(dtype, H, K, D):
+    """A weight of 1 and a sum of 1: low + code step, formed in fp32 and rounded to the type."""
+    n = 400
+    c = ref.Cache(70, [1] * n, H, K, D, 16, dtype)
+    _, vc, _, vs = ref.views(c.pool, D, dtype)
+    vc.copy_(torch.randint(0, 256, vc.shape, generator=c.g, device="cuda", dtype=torch.uint8))
+    scale = 2.0 ** torch.randint(-8, 9, vs.shape[:-1], generator=c.g, device="cuda")
+    vs[..., 0] = (torch.rand(vs.shape[:-1], generator=c.g, device="cuda") * scale).to(dtype)
+    vs[..., 1] = (torch.randn(vs.shape[:-1], generator=c.g, device="cuda") * scale).to(dtype)
+    out = ops.attention_paged_q4(c.handle(), c.q, c.seq_len)
+    page = c.table[:, 0].long()
+    code = torch.stack((vc[page, :, 0, :, 0] & 15, vc[page, :, 0, :, 0] >> 4), -1).flatten(-2)
+    assert code.unique().numel() == 16
+    p = vs[page, :, 0, :, 0].float()
+    want = (p[..., 1:] + code.float() * p[..., :1]).flatten(-2).to(dtype)   # (the product is exact)
+    assert torch.equal(out, want.repeat_interleave(H // K, 1))
