@@ -445,6 +445,8 @@ class PagedKVQ4:
     @staticmethod
     def pool_shape(n_pages: int, n_kv_heads: int, page_size: int, head_dim: int) -> tuple:
         """Shape of a pool: 20 * head_dim bytes hold 16 slots' keys and values."""
+        if page_size < 16 or page_size % 16:   # (a pool of whole blocks would have shorter pages)
+            raise ValueError(f"page_size={page_size} must be a multiple of 16")
         return (n_pages, n_kv_heads, page_size // 16, 20 * head_dim)
 
     def __init__(self, pool: torch.Tensor, page_table: torch.Tensor, dtype: torch.dtype,
