@@ -401,7 +401,8 @@ int qwen_expand_paged_q4(const qwen_paged_kv_q4* kv, const uint32_t* seq_len,
  * are; the i-th that goes is taken by the i-th that stays of those behind: its key,
  * value, weight and position.  What lies behind n_keep is left as it was and may be
  * overwritten.  A sequence of at most n_keep slots stays as it is.  new_len[n_seq]
- * (device; may be seq_len) gets min(seq_len, n_keep).  kv->weights and kv->positions must
+ * (device; may be seq_len) gets min(seq_len, n_keep); that of a sequence beyond its table,
+ * which is reported, is left as it was.  kv->weights and kv->positions must
  * be set; 1 <= n_keep <= 2^24. */
 size_t qwen_evict_paged_q4_workspace(const qwen_paged_kv_q4* kv, uint32_t n_keep);
 int qwen_evict_paged_q4(const qwen_paged_kv_q4* kv, const uint32_t* seq_len, uint32_t n_keep,

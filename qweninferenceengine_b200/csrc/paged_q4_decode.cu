@@ -8,8 +8,8 @@
 // K and V lie side by side, so a copy takes all of a page's blocks in the tile), and 4 consumer
 // warps, one a scheduler, each with two blocks of a tile, whose instructions fill one another's
 // gaps.  Three such CTAs an SM leave a thread 128 registers.  (16 x 8704 of 8 kv heads, fp16,
-// 36 us: with runs of blocks 46; with 6 such warps in two CTAs, which the schedulers do not
-// divide evenly, 51; with 12 in one, which all wait at a piece's end, 58.)
+// now 34 us, when it took 36: with runs of blocks 46; with 6 such warps in two CTAs, which the
+// schedulers do not divide evenly, 51; with 12 in one, which all wait at a piece's end, 58.)
 //
 // What bounds it is not the bytes alone, 2.5 KB a block of 128-element heads, but the
 // instructions that turn them into products; so nothing is dequantised.  Per block a warp
@@ -31,15 +31,14 @@
 // its sum off, always toward zero, which over a run would add up, so that each tile's start from
 // 0 and are added to the others' by additions that round (4% of a long call).
 //
-// Measured: 32 sequences of 16384 slots, 32 and 8 heads of 128, bf16: 156 us (4.3 TB/s), fp16
-// 171; their 671 MB take 102, the kernel without its arithmetic 106, with its pages in L2 154.
-// A block takes a warp some 350 instructions, and no part of them carries the time (without the
-// scores' MMAs 13 us less, the values' dequantisation 13, the weights' second MMAs 6, the steps'
-// products 5, exponentials 2; without all MMAs of the values the same); 8, 12 or 16 warps an
-// SM, with 2 or 4 blocks at once, are within 6%.  A call of 512 slots takes 8.5, 64 sequences of
-// 512 .. 2048 slots and 2 kv heads 16.3 (their bytes 3.8): launch, lengths, page numbers, first
+// Measured: 32 sequences of 16384 slots, 32 and 8 heads of 128, bf16: 161 us (4.2 TB/s), fp16
+// 167; their 671 MB take 102.  A block takes a warp some 395 instructions (bf16, starts and
+// joins included); with lengths of a quarter to all of that, 104 us, the schedulers issue 58% of
+// the time, the integer pipe is busy for 46%, the tensor pipe for 31%.  8, 12 or 16 warps an SM,
+// with 2 or 4 blocks at once, are within 6%.  A call of 512 slots takes 8.5, 64 sequences of
+// 512 .. 2048 slots and 2 kv heads 16.4 (their bytes 3.8): launch, lengths, page numbers, first
 // tile, join.  Warps that load their own blocks, sixteen an SM without producers, took 172 in
-// place of 150.
+// place of 150 at that time.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -818,7 +817,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) k_q4_decode(const __grid
 // as the decode kernel's CTAs have runs of theirs; the next tile is on its way while one is
 // summed.  (A pass over the keys that forms the scores again, 80 B a slot and kv head of 128
 // instead of 8 a query head, took 32 us behind 16 x 8704 of 8 kv heads where this takes
-// 9: it has all the instructions of a score once more.)
+// 8: it has all the instructions of a score once more.  Groups of more than 8 query heads read
+// their further lse's slot by slot: 32 x 16384 of 2 kv heads with 16 each 58 us, and 76 with weights.)
 constexpr int kWeighWarps = 8, kWeighTileShift = 5, kWeighCtasPerSm = 4;
 
 template <int kPairs>   // query heads of a unit in pairs

@@ -16,14 +16,14 @@ struct CutUnit : CutPiece {
 
 struct DecodeArgs {
   PagedAttnArgs a;
-  int units_per_seq;        // kv heads x chunks of at most 16 query heads
+  int units_per_seq;        // kv heads x chunks of query heads (of a partial slot's number at most, S)
   int chunks;               // chunks per kv head
   int group;                // query heads per kv head
   int list_tiles;           // tiles of a listed unit
   int tile_shift;           // positions of a tile: 1 << tile_shift
   float scale_log2;
-  float* part_o;            // [2 G][16][D]
-  float* part_ml;           // [2 G][16][2]
+  float* part_o;            // [2 G][S][D], S the kernel's query heads of a unit: 16 (16-bit pages), 8 (4-bit)
+  float* part_ml;           // [2 G][S][2]
   unsigned long long* arrived;   // [2 G] by partial slot, then [units]: tag << 16 | arrivals
   unsigned long long tag;
   float* own_o;             // if set: unnormalised rows [n_seq][n_heads][D] and their (max,

@@ -588,7 +588,8 @@ def evict_paged_q4(kv: PagedKVQ4, seq_len: torch.Tensor, n_keep: int, n_first: i
     seq_len).  Each kv head keeps the slots of positions below n_first, of the n_recent
     newest positions (a quarter of n_keep by default), and those of the greatest weight,
     the lower slot where two are equal.  What is kept behind n_keep moves into the slots
-    that become free before it, so the order of slots is not that of positions."""
+    that become free before it, so the order of slots is not that of positions.  A sequence
+    whose length is beyond its table is reported; its entry of `out` is not written."""
     if n_recent is None:
         n_recent = n_keep // 4
     if not (1 <= n_keep <= _UINT32 and 0 <= n_first <= _UINT32 and 0 <= n_recent <= _UINT32):
