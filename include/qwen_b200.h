@@ -385,8 +385,8 @@ int qwen_attention_paged_q4(const qwen_paged_kv_q4* kv, const uint16_t* q, int64
                             const uint32_t* seq_len, float scale, void* workspace,
                             size_t workspace_bytes, void* stream);
 
-/* Keys and values of cached slots in the cache's type, what a further chunk of a
- * prompt attends: rows cu_rows[s] .. cu_rows[s+1]-1 of k and v ([n_rows][n_kv_heads *
+/* Keys and values of cached slots in the cache's type, for the caller's attention of a
+ * further chunk of a prompt (the paged ones here take one query token a sequence): rows cu_rows[s] .. cu_rows[s+1]-1 of k and v ([n_rows][n_kv_heads *
  * head_dim], device) get the last slots of sequence s, in order; rows from
  * cu_rows[n_seq] on are not touched.  cu_rows NULL: row s is sequence s's last slot
  * (n_rows = n_seq; seq_len 0: the row is not touched). */

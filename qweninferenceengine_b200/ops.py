@@ -551,7 +551,8 @@ def attention_paged_q4(kv: PagedKVQ4, q: torch.Tensor, seq_len: torch.Tensor, sc
 def expand_paged_q4(kv: PagedKVQ4, seq_len: torch.Tensor, cu_rows: torch.Tensor | None = None,
                     n_rows: int | None = None, out: tuple | None = None):
     """Cached keys and values in the cache's dtype, (k, v) [n_rows, kv_heads, d]
-    (qwen_expand_paged_q4), for a prompt's next chunk to attend.
+    (qwen_expand_paged_q4), for a prompt's next chunk to attend with an attention of the
+    caller's.
 
     seq_len [n_seq]: slots of each sequence.  cu_rows int32 [n_seq + 1]: rows
     cu_rows[s]:cu_rows[s + 1] get the last slots of sequence s, in order; rows behind
